@@ -272,6 +272,37 @@ int triturus_b200_mm_f32(const float* a, const float* b, float* out, int64_t M, 
                          int precision, int32_t* status_dev, void* stream);
 
 /*
+ * Operators for models around the contractions: layer norm with its gradients, clipping of gradients by their global norm, and
+ * sampling from log-probabilities.  (No counterpart in the reference.)  Their elements are 32-bit floats, bfloat16 or 16-bit
+ * floats; the arithmetic between loads and stores has 32 bits or more.  None of them waits on a barrier that it could miss, so
+ * none takes a status word.
+ */
+#define TRITURUS_B200_TYPE_F32 0
+#define TRITURUS_B200_TYPE_BF16 1
+#define TRITURUS_B200_TYPE_F16 2
+
+/*
+ * Layer norm over rows of `width` consecutive elements, x_stride elements apart:
+ *   mean = sum(x) / width,  rstd = 1 / sqrt(sum((x - mean)^2) / width + eps),  y = (x - mean) rstd weight + bias.
+ * y holds rows back to back.  weight, bias (of weight_type: `type` or TRITURUS_B200_TYPE_F32), mean and rstd (32-bit, [rows]) may be NULL:
+ * no weight, no bias, not wanted.  Pointers need the alignment of their elements alone; rows on 16-byte boundaries are
+ * faster.  rows == 0 is no work.
+ */
+int triturus_b200_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, int64_t rows,
+                             int64_t width, int64_t x_stride, int type, int weight_type, float eps, void* stream);
+/*
+ * Its gradients, with g = dy weight and h = (x - mean) rstd:
+ *   dx = rstd (g - sum(g) / width - h sum(g h) / width),  dweight = sum over rows of dy h,  dbias = sum over rows of dy.
+ * dx holds rows back to back; dweight and dbias (of weight_type) may be NULL.  The workspace (16-byte aligned,
+ * triturus_b200_layer_norm_backward_workspace_bytes, may hold anything) takes each block's share of dweight and dbias, which a second launch
+ * adds in a fixed order.
+ */
+size_t triturus_b200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width, int type);
+int triturus_b200_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
+                                      void* dweight, void* dbias, int64_t rows, int64_t width, int64_t dy_stride, int64_t x_stride,
+                                      int type, int weight_type, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Self-test of the error path behind `status_dev` (no counterpart in the reference, whose kernels have no waits
  * that could time out apart from the unbounded spin lock of triturus/lt2exp.py:498-506).  Launches one 64-thread
  * block in which a warp waits on a barrier that nobody signals, with a wait limit of `limit_cycles` GPU clock

@@ -11,6 +11,7 @@ from .host import lm2exp_host, lt2exp_host
 from .lm2exp import lm2exp
 from .lt2exp import lt2exp
 from .mm import mm
+from .norm import layer_norm, layer_norm_backward
 from .utils import (
     ensure_reproducibility,
     is_torch_tf32_enabled,
@@ -25,6 +26,8 @@ __all__ = [
     "ensure_reproducibility",
     "is_torch_tf32_enabled",
     "is_triturus_tf32_enabled",
+    "layer_norm",
+    "layer_norm_backward",
     "lm2exp",
     "lm2exp_host",
     "lt2exp",

@@ -8,7 +8,7 @@ CUDA device raises.
 import ctypes
 import os
 import warnings
-from ctypes import POINTER, c_char_p, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -42,6 +42,9 @@ EXPORTED_SYMBOLS = (
     "triturus_b200_pad_rows_f32",
     "triturus_b200_selftest_wait_timeout",
     "triturus_b200_mm_f32",
+    "triturus_b200_layer_norm",
+    "triturus_b200_layer_norm_backward",
+    "triturus_b200_layer_norm_backward_workspace_bytes",
     "triturus_b200_lm2exp_static_max_columns",
     "triturus_b200_lm2exp_f32_static",
 )
@@ -159,6 +162,14 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.triturus_b200_colmax_f32.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_int64, i64p, c_void_p]
     lib.triturus_b200_pad_rows_f32.restype = c_int
     lib.triturus_b200_pad_rows_f32.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p]
+    lib.triturus_b200_layer_norm.restype = c_int
+    lib.triturus_b200_layer_norm.argtypes = [*[c_void_p] * 6, c_int64, c_int64, c_int64, c_int, c_int, c_float, c_void_p]
+    lib.triturus_b200_layer_norm_backward_workspace_bytes.restype = c_size_t
+    lib.triturus_b200_layer_norm_backward_workspace_bytes.argtypes = [c_int64, c_int64, c_int]
+    lib.triturus_b200_layer_norm_backward.restype = c_int
+    lib.triturus_b200_layer_norm_backward.argtypes = [
+        *[c_void_p] * 8, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p,
+    ]  # fmt: skip
     return lib
 
 
@@ -182,7 +193,7 @@ _IN_PLACE_MAX_FLOP_STRIDED = 8e9
 class _NoHost:
     """In the place of the extension module where there is none: no call is a small one to it, all go through ctypes."""
 
-    lm2exp = lt2exp = staticmethod(lambda *args: None)
+    lm2exp = lt2exp = layer_norm = layer_norm_backward = staticmethod(lambda *args: None)
 
 
 def _load_host():
@@ -636,3 +647,88 @@ def _lm2exp_chain_fake(a, b, b_colmax, want_colmax, precision, variant):
 @lt2exp_op.register_fake
 def _lt2exp_fake(w, a, b, precision, variant):
     return a.new_empty((w.shape[0], w.shape[1], a.shape[2]))
+
+
+# ---------------------------------------------------------------------------- layer norm
+
+_TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """`t` [..., D] as rows of consecutive elements at one distance, and that distance; copied where its strides are none of that."""
+    D = t.shape[-1]
+    if t.is_contiguous():
+        return t, D
+    if t.stride(-1) == 1 or D == 1:
+        try:
+            view = t.view(-1, D)
+            return view, view.stride(0)
+        except RuntimeError:
+            pass
+    return t.contiguous(), D
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _layer_norm_impl(
+    x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _require_cuda(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    rows, stride = _rows(x)
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    given = weight if weight is not None else bias
+    with _on_device(x.device) as idx:
+        rc = LIB.triturus_b200_layer_norm(
+            rows.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), mean.numel(), x.shape[-1], stride,
+            _TYPE_CODES[x.dtype], _TYPE_CODES[x.dtype if given is None else given.dtype], eps, _raw_stream(idx),
+        )  # fmt: skip
+    _check(rc, "triturus_b200_layer_norm")
+    return y, mean, rstd
+
+
+def _layer_norm_backward_impl(
+    dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None, weight_grad: bool, bias_grad: bool
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """dweight and dbias that are not wanted are empty tensors."""
+    _require_cuda(x)
+    D = x.shape[-1]
+    kind = x.dtype if weight is None else weight.dtype
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dweight, dbias = (torch.empty((D if want else 0,), dtype=kind, device=x.device) for want in (weight_grad, bias_grad))
+    (dy_rows, dy_stride), (x_rows, x_stride) = _rows(dy), _rows(x)
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    code = _TYPE_CODES[x.dtype]
+    ws_bytes = int(LIB.triturus_b200_layer_norm_backward_workspace_bytes(mean.numel(), D, code))
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
+    with _on_device(x.device) as idx:
+        rc = LIB.triturus_b200_layer_norm_backward(
+            dy_rows.data_ptr(), x_rows.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
+            _ptr(dweight) if weight_grad else None, _ptr(dbias) if bias_grad else None, mean.numel(), D, dy_stride, x_stride,
+            code, _TYPE_CODES[kind], ws.data_ptr(), ws_bytes, _raw_stream(idx),
+        )  # fmt: skip
+    _check(rc, "triturus_b200_layer_norm_backward")
+    return dx, dweight, dbias
+
+
+layer_norm_op = torch.library.custom_op("triturus::layer_norm", _layer_norm_impl, mutates_args=(), device_types="cuda")
+layer_norm_backward_op = torch.library.custom_op(
+    "triturus::layer_norm_backward", _layer_norm_backward_impl, mutates_args=(), device_types="cuda"
+)
+
+
+@layer_norm_op.register_fake
+def _layer_norm_fake(x, weight, bias, eps):
+    stats = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    return x.new_empty(x.shape), stats, torch.empty_like(stats)
+
+
+@layer_norm_backward_op.register_fake
+def _layer_norm_backward_fake(dy, x, mean, rstd, weight, weight_grad, bias_grad):
+    kind = x.dtype if weight is None else weight.dtype
+    return x.new_empty(x.shape), *(x.new_empty((x.shape[-1] if want else 0,), dtype=kind) for want in (weight_grad, bias_grad))

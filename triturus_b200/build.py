@@ -1,6 +1,6 @@
 """In-tree build of libtriturus_b200.so (the extern "C" launcher and the sm_100a kernels).
 
-`python -m triturus_b200.build` compiles `csrc/api.cu` with nvcc for sm_100a only and leaves the shared
+`python -m triturus_b200.build` compiles `csrc/*.cu` with nvcc for sm_100a only and leaves the shared
 library next to this file, where `triturus_b200._native` loads it with ctypes; then `csrc/host.cpp`, the Python extension
 that makes small calls of it.  nvcc cross-compiles, so no
 GPU is needed to build.
@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -26,7 +27,6 @@ NVCC_FLAGS = [
     "-lineinfo",
     "-O3",
     "-std=c++17",
-    "-shared",
     "-Xcompiler",
     "-fPIC",
 ]
@@ -122,20 +122,26 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     nvcc = find_nvcc()
     if nvcc is None:
         raise RuntimeError("nvcc not found: cannot build libtriturus_b200.so (set NVCC or add nvcc to PATH)")
-    cmd = [nvcc, *NVCC_FLAGS]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    # one temporary file per process: ranks of one job that all find the library stale do not write into each
-    # other's output, and os.replace makes whichever finishes last the library (they are identical)
+    # one folder and one temporary file per process: ranks of one job that all find the library stale do not write into
+    # each other's output, and os.replace makes whichever finishes last the library (they are identical)
     tmp = LIB_PATH.with_suffix(f".so.tmp{os.getpid()}")
-    cmd += ["-o", str(tmp), *[str(p) for p in sorted(CSRC.glob("*.cu"))]]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+    with tempfile.TemporaryDirectory() as folder:
+        runs = []  # the sources at the same time
+        for src in sorted(CSRC.glob("*.cu")):
+            cmd = [nvcc, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-c", "-o", f"{folder}/{src.stem}.o", str(src)]
+            runs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True))
+        outs = [run.communicate() for run in runs]
+        for run, (out, err) in zip(runs, outs):
+            if run.returncode != 0:
+                raise RuntimeError(f"nvcc failed ({run.returncode}):\n{out}\n{err}")
+            if verbose:
+                sys.stderr.write(err)
+        objects = [f"{folder}/{src.stem}.o" for src in sorted(CSRC.glob("*.cu"))]
+        proc = subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", str(tmp), *objects], capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, LIB_PATH)
     STAMP_PATH.write_text(_digest() + "\n")
-    if verbose:
-        sys.stderr.write(proc.stderr)
     return LIB_PATH
 
 

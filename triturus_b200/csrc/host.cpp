@@ -1,8 +1,9 @@
 // Small calls from Python without the interpreter between the check of the arguments and the launch: lm2exp and lt2exp on
 // ordinary CUDA tensors, for the sizes that one launch of the direct kernels takes.  A call of 4 us on the device took 17 us
-// of Python (shape and stride objects, ctypes conversions); here 5.
+// of Python (shape and stride objects, ctypes conversions); here 5.  The operators around them, which have one kernel for
+// all sizes or a rule inside the library, are here for ordinary tensors of any size.
 //
-// Both functions return None, having done nothing, for every call that is not such a one: other tensor types and modes,
+// All functions return None, having done nothing, for every call that is not such a one: other tensor types and modes,
 // wrong shapes, larger problems.  The Python code behind them then does what it would have done without them.
 #include <Python.h>
 
@@ -29,7 +30,7 @@ bool plain_mode() {
 
 // A float32 CUDA tensor that is nothing but its storage, shape and strides: the dispatch keys are those of an ordinary (or an
 // inference) tensor, so no wrapper, lazy conjugation or negation, quantisation, subclass.
-const at::Tensor* plain_tensor(PyObject* o, int64_t dim) {
+const at::Tensor* plain_object(PyObject* o) {
   using c10::DispatchKey;
   static const c10::DispatchKeySet ordinary(
       {DispatchKey::CUDA, DispatchKey::AutogradCUDA, DispatchKey::ADInplaceOrView, DispatchKey::AutocastCUDA});
@@ -38,8 +39,28 @@ const at::Tensor* plain_tensor(PyObject* o, int64_t dim) {
   const at::Tensor& t = THPVariable_Unpack(o);
   const c10::DispatchKeySet ks = t.key_set();
   if (ks != ordinary && ks != inference) return nullptr;
-  if (t.scalar_type() != at::kFloat || t.layout() != at::kStrided || t.dim() != dim || t.numel() == 0) return nullptr;
-  return &t;
+  return t.layout() == at::kStrided && t.numel() != 0 ? &t : nullptr;
+}
+
+const at::Tensor* plain_tensor(PyObject* o, int64_t dim) {
+  const at::Tensor* t = plain_object(o);
+  return t != nullptr && t->scalar_type() == at::kFloat && t->dim() == dim ? t : nullptr;
+}
+
+// The library's code for an element type, or -1.
+int type_code(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return TRITURUS_B200_TYPE_F32;
+    case at::kBFloat16: return TRITURUS_B200_TYPE_BF16;
+    case at::kHalf: return TRITURUS_B200_TYPE_F16;
+    default: return -1;
+  }
+}
+
+// Rows of consecutive elements at one distance, without a copy: that distance, or -1 where the strides may be something else.
+int64_t row_stride(const at::Tensor& t) {
+  if (t.is_contiguous()) return t.size(-1);
+  return t.dim() == 2 && t.stride(1) == 1 ? t.stride(0) : -1;
 }
 
 bool int_arg(PyObject* o, int* v) {
@@ -139,6 +160,107 @@ PyObject* lt2exp(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// None, or a vector of `n` elements of x's type or 32 bits on x's device; sets *type to its code.  False: not an ordinary one.
+bool weight_arg(PyObject* o, const at::Tensor& x, int64_t n, const at::Tensor** t, int* type) {
+  *t = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* w = plain_object(o);
+  if (w == nullptr || w->dim() != 1 || w->size(0) != n || (n != 1 && w->stride(0) != 1) || w->device() != x.device()) return false;
+  const int code = type_code(*w);
+  if (code != TRITURUS_B200_TYPE_F32 && w->scalar_type() != x.scalar_type()) return false;
+  if (*type >= 0 && *type != code) return false;
+  *type = code;
+  *t = w;
+  return true;
+}
+
+const void* data_of(const at::Tensor* t) { return t != nullptr ? t->const_data_ptr() : nullptr; }
+
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType type) {
+  return at::empty(shape, at::TensorOptions().dtype(type).device(like.device()));
+}
+
+PyObject* tuple3(at::Tensor* a, at::Tensor* b, at::Tensor* c) {
+  PyObject* out = PyTuple_New(3);
+  if (out == nullptr) return nullptr;
+  at::Tensor* all[3] = {a, b, c};
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(out, i, all[i] != nullptr ? THPVariable_Wrap(std::move(*all[i])) : Py_NewRef(Py_None));
+  return out;
+}
+
+// layer_norm(x, weight, bias, eps, return_stats)
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5 || !PyFloat_Check(args[3]) || !PyBool_Check(args[4]) || !plain_mode()) return none();
+  const at::Tensor* x = plain_object(args[0]);
+  if (x == nullptr || x->dim() < 1 || x->get_device() != c10::cuda::current_device()) return none();
+  const int type = type_code(*x);
+  const int64_t stride = row_stride(*x), width = x->size(-1), rows = x->numel() / width;
+  const at::Tensor *weight, *bias;
+  int weight_type = -1;
+  if (type < 0 || stride < 0 || !weight_arg(args[1], *x, width, &weight, &weight_type) || !weight_arg(args[2], *x, width, &bias, &weight_type))
+    return none();
+  const bool stats = args[4] == Py_True;
+  at::Tensor y = empty_on(*x, x->sizes(), x->scalar_type()), mean, rstd;
+  float *mp = nullptr, *rp = nullptr;
+  if (stats) {
+    const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+    mean = empty_on(*x, lead, at::kFloat);
+    rstd = empty_on(*x, lead, at::kFloat);
+    mp = mean.mutable_data_ptr<float>();
+    rp = rstd.mutable_data_ptr<float>();
+  }
+  const auto stream = c10::cuda::getCurrentCUDAStream(x->get_device()).stream();
+  int rc;
+  {
+    ThreadsRun unlocked;
+    rc = triturus_b200_layer_norm(x->const_data_ptr(), data_of(weight), data_of(bias), y.mutable_data_ptr(), mp, rp, rows, width, stride, type,
+                                  weight_type < 0 ? type : weight_type, static_cast<float>(PyFloat_AS_DOUBLE(args[3])), stream);
+  }
+  if (rc != TRITURUS_B200_OK) return failed("triturus_b200_layer_norm", rc);
+  return stats ? tuple3(&y, &mean, &rstd) : THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// layer_norm_backward(dy, x, mean, rstd, weight, weight_grad, bias_grad)
+PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7 || !PyBool_Check(args[5]) || !PyBool_Check(args[6]) || !plain_mode()) return none();
+  const at::Tensor* x = plain_object(args[1]);
+  const at::Tensor* dy = x != nullptr ? plain_object(args[0]) : nullptr;
+  const at::Tensor* mean = dy != nullptr ? plain_object(args[2]) : nullptr;
+  const at::Tensor* rstd = mean != nullptr ? plain_object(args[3]) : nullptr;
+  if (rstd == nullptr || x->dim() < 1 || x->get_device() != c10::cuda::current_device()) return none();
+  const int type = type_code(*x);
+  if (type < 0 || dy->scalar_type() != x->scalar_type() || dy->sizes() != x->sizes() || dy->device() != x->device()) return none();
+  const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+  for (const at::Tensor* t : {mean, rstd})
+    if (t->scalar_type() != at::kFloat || t->sizes() != lead || !t->is_contiguous() || t->device() != x->device()) return none();
+  const int64_t x_stride = row_stride(*x), dy_stride = row_stride(*dy), width = x->size(-1), rows = x->numel() / width;
+  const at::Tensor* weight;
+  int weight_type = -1;
+  if (x_stride < 0 || dy_stride < 0 || !weight_arg(args[4], *x, width, &weight, &weight_type)) return none();
+  const at::ScalarType kind = weight != nullptr ? weight->scalar_type() : x->scalar_type();
+  const bool want_weight = args[5] == Py_True, want_bias = args[6] == Py_True;
+  at::Tensor dx = empty_on(*x, x->sizes(), x->scalar_type()), dweight, dbias;
+  if (want_weight) dweight = empty_on(*x, {width}, kind);
+  if (want_bias) dbias = empty_on(*x, {width}, kind);
+  const size_t bytes = triturus_b200_layer_norm_backward_workspace_bytes(rows, width, type);
+  at::Tensor ws = empty_on(*x, {static_cast<int64_t>(bytes)}, at::kByte);
+  const auto stream = c10::cuda::getCurrentCUDAStream(x->get_device()).stream();
+  int rc;
+  {
+    ThreadsRun unlocked;
+    rc = triturus_b200_layer_norm_backward(dy->const_data_ptr(), x->const_data_ptr(), data_of(weight), mean->const_data_ptr<float>(),
+                                           rstd->const_data_ptr<float>(), dx.mutable_data_ptr(), want_weight ? dweight.mutable_data_ptr() : nullptr,
+                                           want_bias ? dbias.mutable_data_ptr() : nullptr, rows, width, dy_stride, x_stride, type,
+                                           weight_type < 0 ? type : weight_type, ws.mutable_data_ptr(), bytes, stream);
+  }
+  if (rc != TRITURUS_B200_OK) return failed("triturus_b200_layer_norm_backward", rc);
+  return tuple3(&dx, want_weight ? &dweight : nullptr, want_bias ? &dbias : nullptr);
+  END_HANDLE_TH_ERRORS
+}
+
 // set_up(error_class, copy_flop_rows, copy_flop_strided)
 PyObject* set_up(PyObject*, PyObject* args) {
   PyObject* cls;
@@ -152,6 +274,10 @@ PyMethodDef methods[] = {
     {"set_up", set_up, METH_VARARGS, "set_up(error_class, copy_flop_rows, copy_flop_strided)"},
     {"lm2exp", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(lm2exp)), METH_FASTCALL, "lm2exp(a, b, precision, variant) -> Tensor or None"},
     {"lt2exp", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(lt2exp)), METH_FASTCALL, "lt2exp(w, a, b, precision, variant) -> Tensor or None"},
+    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm)), METH_FASTCALL,
+     "layer_norm(x, weight, bias, eps, return_stats) -> Tensor, tuple or None"},
+    {"layer_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_backward)), METH_FASTCALL,
+     "layer_norm_backward(dy, x, mean, rstd, weight, weight_grad, bias_grad) -> tuple or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Small calls of triturus_b200 from C++.", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -610,7 +610,7 @@ __device__ __forceinline__ void fold_staged_colmax(const uint8_t* stg, int rows_
 // warp writes 32 consecutive floats of one row (`dst` points at this lane's column of row 0).  For results
 // that cannot go through a TMA store.  Kept out of line: inlined, its address arithmetic competes for
 // registers with the accumulator chunks the epilogue holds.
-__device__ __noinline__ void store_staged_rows(const uint8_t* stg, float* dst, int64_t row_stride, int nrows,
+static __device__ __noinline__ void store_staged_rows(const uint8_t* stg, float* dst, int64_t row_stride, int nrows,
                                                int lane) {
   const uint8_t* src = stg + (lane & 3) * 4;
 #pragma unroll 4
