@@ -303,6 +303,18 @@ int triturus_b200_layer_norm_backward(const void* dy, const void* x, const void*
                                       int type, int weight_type, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * The norm of `count` tensors taken as one vector, sqrt(sum x^2) or (`largest` != 0) max |x|, into *norm (device memory); with `scale` != 0
+ * their elements are then multiplied by min(1, max_norm / (norm + 1e-6)) in place, or left as they are where that is 1 (also where
+ * *norm itself is beyond 32 bits).
+ * tensors, numels and types are HOST arrays: device pointers of dense tensors that do not overlap, numbers of elements (0 is none), and
+ * TRITURUS_B200_TYPE_*.  Pointers need the alignment of their elements alone.  The sum of squares is held in 64 bits and added in a fixed
+ * order; a NaN makes the norm NaN, and all elements with it.  Workspace: 8-byte aligned, may hold anything.
+ */
+size_t triturus_b200_clip_grad_norm_workspace_bytes(int64_t count);
+int triturus_b200_clip_grad_norm(void* const* tensors, const int64_t* numels, const int* types, int64_t count, double max_norm, int largest,
+                                 int scale, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Self-test of the error path behind `status_dev` (no counterpart in the reference, whose kernels have no waits
  * that could time out apart from the unbounded spin lock of triturus/lt2exp.py:498-506).  Launches one 64-thread
  * block in which a warp waits on a barrier that nobody signals, with a wait limit of `limit_cycles` GPU clock

@@ -7,6 +7,7 @@ registers `torch.ops.triturus.lm2exp` / `torch.ops.triturus.lt2exp`.  There is n
 from . import lm2exp as _lm2exp_module
 from . import lt2exp as _lt2exp_module
 from ._native import NativeLibraryError, check_status, colmax
+from .clip import clip_grad_norm_, grad_norm
 from .host import lm2exp_host, lt2exp_host
 from .lm2exp import lm2exp
 from .lt2exp import lt2exp
@@ -22,8 +23,10 @@ from .utils import (
 __all__ = [
     "NativeLibraryError",
     "check_status",
+    "clip_grad_norm_",
     "colmax",
     "ensure_reproducibility",
+    "grad_norm",
     "is_torch_tf32_enabled",
     "is_triturus_tf32_enabled",
     "layer_norm",

@@ -8,7 +8,7 @@ CUDA device raises.
 import ctypes
 import os
 import warnings
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -42,6 +42,8 @@ EXPORTED_SYMBOLS = (
     "triturus_b200_pad_rows_f32",
     "triturus_b200_selftest_wait_timeout",
     "triturus_b200_mm_f32",
+    "triturus_b200_clip_grad_norm",
+    "triturus_b200_clip_grad_norm_workspace_bytes",
     "triturus_b200_layer_norm",
     "triturus_b200_layer_norm_backward",
     "triturus_b200_layer_norm_backward_workspace_bytes",
@@ -170,6 +172,12 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.triturus_b200_layer_norm_backward.argtypes = [
         *[c_void_p] * 8, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_size_t, c_void_p,
     ]  # fmt: skip
+    lib.triturus_b200_clip_grad_norm_workspace_bytes.restype = c_size_t
+    lib.triturus_b200_clip_grad_norm_workspace_bytes.argtypes = [c_int64]
+    lib.triturus_b200_clip_grad_norm.restype = c_int
+    lib.triturus_b200_clip_grad_norm.argtypes = [
+        POINTER(c_void_p), i64p, POINTER(c_int), c_int64, c_double, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p,
+    ]  # fmt: skip
     return lib
 
 
@@ -193,7 +201,7 @@ _IN_PLACE_MAX_FLOP_STRIDED = 8e9
 class _NoHost:
     """In the place of the extension module where there is none: no call is a small one to it, all go through ctypes."""
 
-    lm2exp = lt2exp = layer_norm = layer_norm_backward = staticmethod(lambda *args: None)
+    lm2exp = lt2exp = layer_norm = layer_norm_backward = clip_grad_norm = staticmethod(lambda *args: None)
 
 
 def _load_host():
@@ -732,3 +740,59 @@ def _layer_norm_fake(x, weight, bias, eps):
 def _layer_norm_backward_fake(dy, x, mean, rstd, weight, weight_grad, bias_grad):
     kind = x.dtype if weight is None else weight.dtype
     return x.new_empty(x.shape), *(x.new_empty((x.shape[-1] if want else 0,), dtype=kind) for want in (weight_grad, bias_grad))
+
+
+# ---------------------------------------------------------------------------- norm of the gradients
+
+
+def _norm_of(grads: list[torch.Tensor], max_norm: float, largest: bool, scale: bool) -> torch.Tensor:
+    """`grads`: dense tensors of one device."""
+    device = grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
+    n = len(grads)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    nbytes = int(LIB.triturus_b200_clip_grad_norm_workspace_bytes(n))
+    ws = torch.empty(nbytes // 8, dtype=torch.float64, device=device)
+    data = (c_void_p * n)(*(g.data_ptr() for g in grads))
+    numels = (c_int64 * n)(*(g.numel() for g in grads))
+    types = (c_int * n)(*(_TYPE_CODES[g.dtype] for g in grads))
+    with _on_device(device) as idx:
+        rc = LIB.triturus_b200_clip_grad_norm(
+            data, numels, types, n, max_norm, int(largest), int(scale), norm.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(idx)
+        )
+    _check(rc, "triturus_b200_clip_grad_norm")
+    return norm
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    from .clip import _dense
+
+    return t.is_contiguous() or _dense(t)
+
+
+def _clip_grad_norm_impl(grads: list[torch.Tensor], max_norm: float, largest: bool) -> torch.Tensor:
+    dense = [g if _is_dense(g) else g.contiguous() for g in grads]
+    norm = _norm_of(dense, max_norm, largest, True)
+    for g, d in zip(grads, dense):
+        if d is not g:
+            g.copy_(d)
+        elif g.numel():
+            torch.autograd.graph.increment_version(g)
+    return norm
+
+
+def _grad_norm_impl(grads: list[torch.Tensor], largest: bool) -> torch.Tensor:
+    return _norm_of([g if _is_dense(g) else g.contiguous() for g in grads], 0.0, largest, False)
+
+
+clip_grad_norm_op = torch.library.custom_op("triturus::clip_grad_norm_", _clip_grad_norm_impl, mutates_args=("grads",), device_types="cuda")
+grad_norm_op = torch.library.custom_op("triturus::grad_norm", _grad_norm_impl, mutates_args=(), device_types="cuda")
+
+
+@clip_grad_norm_op.register_fake
+def _clip_grad_norm_fake(grads, max_norm, largest):
+    return grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device="cuda")
+
+
+@grad_norm_op.register_fake
+def _grad_norm_fake(grads, largest):
+    return grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device="cuda")

@@ -13,7 +13,12 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <c10/util/SmallVector.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <cmath>
+#include <utility>
 
 #include "../../include/triturus_b200.h"
 
@@ -261,6 +266,60 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs
   END_HANDLE_TH_ERRORS
 }
 
+// clip_grad_norm(grads, max_norm, norm_type, scale): a list or tuple of dense tensors and None
+PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 4 || !(PyList_CheckExact(args[0]) || PyTuple_CheckExact(args[0])) || !PyFloat_CheckExact(args[1]) || !PyFloat_CheckExact(args[2]) ||
+      !plain_mode())
+    return none();
+  const double max_norm = PyFloat_AS_DOUBLE(args[1]), norm_type = PyFloat_AS_DOUBLE(args[2]);
+  const bool scale = args[3] == Py_True;
+  if (norm_type != 2.0 && !(std::isinf(norm_type) && norm_type > 0)) return none();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(args[0]);
+  c10::SmallVector<void*, 64> data;
+  c10::SmallVector<int64_t, 64> numels;
+  c10::SmallVector<int, 64> types;
+  c10::SmallVector<const at::Tensor*, 64> tensors;
+  c10::SmallVector<std::pair<uintptr_t, uintptr_t>, 64> ranges;
+  const auto device = c10::cuda::current_device();
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(args[0], i);
+    if (o == Py_None) continue;
+    const at::Tensor* t = plain_object(o);
+    const int type = t != nullptr ? type_code(*t) : -1;
+    if (type < 0 || t->get_device() != device || !t->is_non_overlapping_and_dense() || (scale && t->requires_grad())) return none();
+    void* p = const_cast<void*>(t->const_data_ptr());
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    data.push_back(p);
+    numels.push_back(t->numel());
+    types.push_back(type);
+    tensors.push_back(t);
+    if (scale) ranges.emplace_back(at, at + t->numel() * t->element_size());
+  }
+  if (tensors.empty()) return none();
+  std::sort(ranges.begin(), ranges.end());
+  for (size_t i = 1; i < ranges.size(); ++i)
+    if (ranges[i].first < ranges[i - 1].second) return none();
+  const int64_t count = static_cast<int64_t>(tensors.size());
+  const size_t bytes = triturus_b200_clip_grad_norm_workspace_bytes(count);
+  at::Tensor norm = empty_on(*tensors[0], {}, at::kFloat);
+  at::Tensor ws = empty_on(*tensors[0], {static_cast<int64_t>(bytes / 8)}, at::kDouble);
+  float* np = norm.mutable_data_ptr<float>();
+  const auto stream = c10::cuda::getCurrentCUDAStream(device).stream();
+  int rc;
+  {
+    ThreadsRun unlocked;
+    rc = triturus_b200_clip_grad_norm(data.data(), numels.data(), types.data(), count, max_norm, norm_type != 2.0, scale, np,
+                                      ws.mutable_data_ptr(), bytes, stream);
+  }
+  if (rc != TRITURUS_B200_OK) return failed("triturus_b200_clip_grad_norm", rc);
+  if (scale)
+    for (const at::Tensor* t : tensors)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return THPVariable_Wrap(std::move(norm));
+  END_HANDLE_TH_ERRORS
+}
+
 // set_up(error_class, copy_flop_rows, copy_flop_strided)
 PyObject* set_up(PyObject*, PyObject* args) {
   PyObject* cls;
@@ -278,6 +337,8 @@ PyMethodDef methods[] = {
      "layer_norm(x, weight, bias, eps, return_stats) -> Tensor, tuple or None"},
     {"layer_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_backward)), METH_FASTCALL,
      "layer_norm_backward(dy, x, mean, rstd, weight, weight_grad, bias_grad) -> tuple or None"},
+    {"clip_grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(clip_grad_norm)), METH_FASTCALL,
+     "clip_grad_norm(grads, max_norm, norm_type, scale) -> Tensor or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Small calls of triturus_b200 from C++.", -1, methods, nullptr, nullptr, nullptr, nullptr};
