@@ -315,6 +315,20 @@ int triturus_b200_clip_grad_norm(void* const* tensors, const int64_t* numels, co
                                  int scale, float* norm, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * One symbol for each row of logits [rows, symbols] (elements adjacent, rows logits_stride elements apart) from exponential noise
+ * (32-bit, positive, rows noise_stride apart): p_i = exp((x_i - max x) / temperature); in the order of falling x, equal ones by index, the
+ * first top_k are kept (all for a value below 1), of these the fewest whose sum of p reaches top_p times theirs (1 or more: all), of these the ones
+ * with p >= min_p.  token[row] is the kept symbol with the largest p / noise, the lower index of equal ones, and logprob[row] (may be
+ * NULL) = log(p / sum of p kept).  A temperature that is not positive gives the first of the largest logits, with logprob 0.  A symbol of -inf is never given;
+ * a row of nothing else gives token -1 and logprob -inf, one with a NaN -1 and NaN.  Each parameter is a device array [rows], or
+ * NULL and the number behind it.  Pointers need the alignment of their elements alone.  No workspace; at most 2^30 symbols
+ * and 2^28 - 1 rows.
+ */
+int triturus_b200_sample(const void* logits, const float* noise, int64_t* token, float* logprob, int64_t rows, int64_t symbols,
+                         int64_t logits_stride, int64_t noise_stride, int type, const float* temperature, float temperature0,
+                         const int32_t* top_k, int32_t top_k0, const float* top_p, float top_p0, const float* min_p, float min_p0, void* stream);
+
+/*
  * Self-test of the error path behind `status_dev` (no counterpart in the reference, whose kernels have no waits
  * that could time out apart from the unbounded spin lock of triturus/lt2exp.py:498-506).  Launches one 64-thread
  * block in which a warp waits on a barrier that nobody signals, with a wait limit of `limit_cycles` GPU clock

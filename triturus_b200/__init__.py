@@ -13,6 +13,7 @@ from .lm2exp import lm2exp
 from .lt2exp import lt2exp
 from .mm import mm
 from .norm import layer_norm, layer_norm_backward
+from .sample import sample
 from .utils import (
     ensure_reproducibility,
     is_torch_tf32_enabled,
@@ -36,5 +37,6 @@ __all__ = [
     "lt2exp",
     "lt2exp_host",
     "mm",
+    "sample",
     "set_tf32_enabled",
 ]

@@ -47,6 +47,7 @@ EXPORTED_SYMBOLS = (
     "triturus_b200_layer_norm",
     "triturus_b200_layer_norm_backward",
     "triturus_b200_layer_norm_backward_workspace_bytes",
+    "triturus_b200_sample",
     "triturus_b200_lm2exp_static_max_columns",
     "triturus_b200_lm2exp_f32_static",
 )
@@ -178,6 +179,11 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.triturus_b200_clip_grad_norm.argtypes = [
         POINTER(c_void_p), i64p, POINTER(c_int), c_int64, c_double, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p,
     ]  # fmt: skip
+    lib.triturus_b200_sample.restype = c_int
+    lib.triturus_b200_sample.argtypes = [
+        *[c_void_p] * 4, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_float, c_void_p, c_int32, c_void_p, c_float,
+        c_void_p, c_float, c_void_p,
+    ]  # fmt: skip
     return lib
 
 
@@ -201,7 +207,7 @@ _IN_PLACE_MAX_FLOP_STRIDED = 8e9
 class _NoHost:
     """In the place of the extension module where there is none: no call is a small one to it, all go through ctypes."""
 
-    lm2exp = lt2exp = layer_norm = layer_norm_backward = clip_grad_norm = staticmethod(lambda *args: None)
+    lm2exp = lt2exp = layer_norm = layer_norm_backward = clip_grad_norm = sample = staticmethod(lambda *args: None)
 
 
 def _load_host():
@@ -796,3 +802,35 @@ def _clip_grad_norm_fake(grads, max_norm, largest):
 @grad_norm_op.register_fake
 def _grad_norm_fake(grads, largest):
     return grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device="cuda")
+
+
+# ---------------------------------------------------------------------------- sampling
+
+
+def _sample_impl(
+    logits: torch.Tensor, noise: torch.Tensor, temperature: torch.Tensor | None, temperature0: float, top_k: torch.Tensor | None, top_k0: int,
+    top_p: torch.Tensor | None, top_p0: float, min_p: torch.Tensor | None, min_p0: float,
+) -> tuple[torch.Tensor, torch.Tensor]:  # fmt: skip
+    """Each parameter is a tensor of the shape of the rows, or None and the number behind it."""
+    _require_cuda(logits)
+    lead = logits.shape[:-1]
+    token = torch.empty(lead, dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    (x, x_stride), (q, q_stride) = _rows(logits), _rows(noise)
+    params = [None if t is None else t.contiguous() for t in (temperature, top_k, top_p, min_p)]
+    with _on_device(logits.device) as idx:
+        rc = LIB.triturus_b200_sample(
+            x.data_ptr(), q.data_ptr(), token.data_ptr(), logprob.data_ptr(), token.numel(), logits.shape[-1], x_stride, q_stride,
+            _TYPE_CODES[logits.dtype], _ptr(params[0]), temperature0, _ptr(params[1]), top_k0, _ptr(params[2]), top_p0, _ptr(params[3]), min_p0,
+            _raw_stream(idx),
+        )  # fmt: skip
+    _check(rc, "triturus_b200_sample")
+    return token, logprob
+
+
+sample_op = torch.library.custom_op("triturus::sample", _sample_impl, mutates_args=(), device_types="cuda")
+
+
+@sample_op.register_fake
+def _sample_fake(logits, noise, temperature, temperature0, top_k, top_k0, top_p, top_p0, min_p, min_p0):
+    return logits.new_empty(logits.shape[:-1], dtype=torch.int64), logits.new_empty(logits.shape[:-1], dtype=torch.float32)

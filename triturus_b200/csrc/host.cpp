@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <utility>
 
 #include "../../include/triturus_b200.h"
@@ -320,6 +321,69 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// A parameter of sample: a number in [least, most], None (`off`), or a contiguous tensor of the rows' shape.
+bool sample_arg(PyObject* o, const at::Tensor& logits, at::ScalarType kind, double least, double most, const void** array, double* number) {
+  *array = nullptr;
+  if (o == Py_None) return true;
+  if (PyFloat_CheckExact(o) || PyLong_CheckExact(o)) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+    *number = v;
+    return v >= least && v <= most && (kind != at::kInt || PyLong_CheckExact(o));
+  }
+  const at::Tensor* t = plain_object(o);
+  if (t == nullptr || t->scalar_type() != kind || t->device() != logits.device() || !t->is_contiguous()) return false;
+  if (t->sizes() != logits.sizes().slice(0, logits.dim() - 1)) return false;
+  *array = t->const_data_ptr();
+  return true;
+}
+
+// sample(logits, noise, temperature, top_k, top_p, min_p, return_logprob)
+PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7 || !PyBool_Check(args[6]) || args[2] == Py_None || !plain_mode()) return none();
+  const at::Tensor* logits = plain_object(args[0]);
+  const at::Tensor* noise = logits != nullptr ? plain_object(args[1]) : nullptr;
+  if (noise == nullptr || logits->dim() < 1 || logits->get_device() != c10::cuda::current_device()) return none();
+  const int type = type_code(*logits);
+  if (type < 0 || noise->scalar_type() != at::kFloat || noise->sizes() != logits->sizes() || noise->device() != logits->device()) return none();
+  const int64_t stride = row_stride(*logits), noise_stride = row_stride(*noise), symbols = logits->size(-1), rows = logits->numel() / symbols;
+  const void *temperature, *top_k, *top_p, *min_p;
+  double t0 = 1.0, k0 = 0.0, p0 = 1.0, m0 = 0.0;
+  if (stride < 0 || noise_stride < 0 || !sample_arg(args[2], *logits, at::kFloat, 0.0, std::numeric_limits<float>::max(), &temperature, &t0) ||
+      !sample_arg(args[3], *logits, at::kInt, 1.0, std::numeric_limits<int32_t>::max(), &top_k, &k0) ||
+      !sample_arg(args[4], *logits, at::kFloat, 0.0, 1.0, &top_p, &p0) || !sample_arg(args[5], *logits, at::kFloat, 0.0, 1.0, &min_p, &m0))
+    return none();
+  const at::IntArrayRef lead = logits->sizes().slice(0, logits->dim() - 1);
+  const bool want = args[6] == Py_True;
+  at::Tensor token = empty_on(*logits, lead, at::kLong), logprob;
+  float* lp = nullptr;
+  if (want) {
+    logprob = empty_on(*logits, lead, at::kFloat);
+    lp = logprob.mutable_data_ptr<float>();
+  }
+  const auto stream = c10::cuda::getCurrentCUDAStream(logits->get_device()).stream();
+  int rc;
+  {
+    ThreadsRun unlocked;
+    rc = triturus_b200_sample(logits->const_data_ptr(), noise->const_data_ptr<float>(), token.mutable_data_ptr<int64_t>(), lp, rows, symbols, stride,
+                              noise_stride, type, static_cast<const float*>(temperature), static_cast<float>(t0),
+                              static_cast<const int32_t*>(top_k), static_cast<int32_t>(k0), static_cast<const float*>(top_p),
+                              static_cast<float>(p0), static_cast<const float*>(min_p), static_cast<float>(m0), stream);
+  }
+  if (rc != TRITURUS_B200_OK) return failed("triturus_b200_sample", rc);
+  if (!want) return THPVariable_Wrap(std::move(token));
+  PyObject* out = PyTuple_New(2);
+  if (out == nullptr) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(token)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(logprob)));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
 // set_up(error_class, copy_flop_rows, copy_flop_strided)
 PyObject* set_up(PyObject*, PyObject* args) {
   PyObject* cls;
@@ -339,6 +403,8 @@ PyMethodDef methods[] = {
      "layer_norm_backward(dy, x, mean, rstd, weight, weight_grad, bias_grad) -> tuple or None"},
     {"clip_grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(clip_grad_norm)), METH_FASTCALL,
      "clip_grad_norm(grads, max_norm, norm_type, scale) -> Tensor or None"},
+    {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sample)), METH_FASTCALL,
+     "sample(logits, noise, temperature, top_k, top_p, min_p, return_logprob) -> Tensor, tuple or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Small calls of triturus_b200 from C++.", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,75 @@
+"""Sampling of symbols from the log-probabilities that a circuit gives them (no counterpart in the reference)."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native
+
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _parameter(name: str, value, lead: torch.Size, device: torch.device, kind: torch.dtype, off, valid):
+    """(tensor of the rows' shape or None, number)"""
+    if isinstance(value, torch.Tensor):
+        assert value.dtype == kind
+        assert value.shape == lead
+        assert value.device == device
+        return value, off
+    if value is None:
+        return None, off
+    if not valid(value):
+        raise ValueError(f"sample: {name} is out of range, got {value!r}")
+    return None, type(off)(value)
+
+
+def sample(
+    logits: torch.Tensor,
+    noise: torch.Tensor,
+    *,
+    temperature: float | torch.Tensor = 1.0,
+    top_k: int | torch.Tensor | None = None,
+    top_p: float | torch.Tensor | None = None,
+    min_p: float | torch.Tensor | None = None,
+    return_logprob: bool = False,
+):
+    """One symbol for each row of the CUDA tensor `logits` [..., V] (float32, bfloat16 or float16; log-probabilities or any others) from
+    given random numbers: `noise` of the same shape in float32, positive and exponentially distributed
+    (`torch.empty(shape, device="cuda").exponential_()`).  Returns int64 tokens of shape logits.shape[:-1].
+
+    With p_i = exp((x_i - max x) / temperature), and the symbols in the order of falling x, equal ones by index, the filters keep in turn
+      top_k: the first top_k;
+      top_p: of these the fewest whose sum of p reaches top_p times theirs (the first in any case);
+      min_p: of these the ones with p_i >= min_p, that is min_p times the probability of the most probable one.
+    The token is the kept symbol with the largest p_i / noise_i (the lower index of equal ones): symbol i with probability
+    p_i / sum of the p kept.  `return_logprob=True` returns (token, logprob) with the float32 logarithm of that probability.
+
+    A parameter is a number, None (no filter) or a tensor of the rows' shape (float32, top_k int32), where a top_k below 1, a top_p of 1
+    and a min_p of 0 are no filter.  A temperature of 0 (in a tensor: any that is not positive) gives the first of the largest
+    logits with logprob 0.  Symbols of -inf are impossible and never given; a row of nothing else gives token -1 and logprob
+    -inf, a row with a NaN -1 and NaN.  Infinity counts as the largest number.  logits and noise may have any strides: rows of consecutive elements
+    at one distance are read in place (noise only where a symbol is kept), other views are copied first."""
+    if not torch.compiler.is_compiling():
+        out = _native.HOST.sample(logits, noise, temperature, top_k, top_p, min_p, return_logprob)  # None: not an ordinary call
+        if out is not None:
+            return out
+    assert len(logits.shape) >= 1
+    assert logits.dtype in _TYPES
+    assert noise.shape == logits.shape
+    assert noise.dtype == torch.float32
+    assert noise.device == logits.device
+    lead, device = logits.shape[:-1], logits.device
+    params = (
+        *_parameter("temperature", temperature, lead, device, torch.float32, 1.0, lambda v: 0.0 <= v < math.inf),
+        *_parameter("top_k", top_k, lead, device, torch.int32, 0, lambda v: 1 <= v == int(v)),
+        *_parameter("top_p", top_p, lead, device, torch.float32, 1.0, lambda v: 0.0 <= v <= 1.0),
+        *_parameter("min_p", min_p, lead, device, torch.float32, 0.0, lambda v: 0.0 <= v <= 1.0),
+    )
+    _native._require_cuda(logits)
+    if logits.shape[-1] == 0:
+        raise ValueError("sample: rows of no symbols are not supported")
+    params = (*params[:3], min(params[3], 2**31 - 1), *params[4:])
+    token, logprob = (_native.sample_op if torch.compiler.is_compiling() else _native._sample_impl)(logits, noise, *params)
+    return (token, logprob) if return_logprob else token
