@@ -7,12 +7,16 @@
 // For exponential noise the largest p / noise falls on i with probability p_i / sum p.  No place on a cumulative sum decides, and so no order
 // of additions: what is kept is a prefix of the sorted row, and only its end depends on sums.
 //
-// A row belongs to a cluster of blocks, each of which holds its slice in shared memory.  No row is sorted.  Filters find the end of the
-// kept prefix from a histogram of (max - x) / T in steps of 1/16 (a factor of 1.06 of p): the bins down to one that surely reach far
-// enough hold some tens to hundreds of symbols as a rule, which the first block of the cluster gathers, sorts and finishes alone.  Where there
-// are more than it has room for (flat rows, many equal values), the end is found by radix selection over the bits of x and then over
-// the index.  Counts and, as multiples of a power of two, masses are added as integers, so that a result does not depend on the order of
-// the atomic additions.
+// A row belongs to a cluster of blocks, each of which holds its slice in shared memory.  No row is sorted.
+//
+// A small top_k: a block's own symbols below the k-th largest of its threads' maxima cannot be among the row's first k; what remains, some
+// tens of symbols of each block, the first block gathers, sorts and finishes alone.
+//
+// Else the end of the kept prefix is found from a histogram of (max - x) / T in steps of 1/16, a factor of 1.06 of p: the counts alone give the bin
+// where a number of symbols is reached, and bounds of the bins where a mass is; the masses are then added for the bins between the bounds only.  The
+// symbols of the one bin that is left are gathered and sorted; where they are too many (flat rows, many equal values), the end is
+// found among them by radix selection over the bits of x and then over the index.  Counts and, as multiples of a power of two, masses are added as
+// integers, so that a result does not depend on the order of the atomic additions.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -28,6 +32,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 256;
 constexpr int kList = 2048;  // symbols that are sorted
+constexpr int kFew = kThreads / 2;  // a small top_k
 
 struct SampleArgs {
   const void* logits;
@@ -47,15 +52,15 @@ struct SampleArgs {
 
 struct Shared {
   unsigned long long list[kList];
-  uint32_t count[kBins];     // the block's
-  uint32_t mass[kBins];      // the block's, as multiples of 2^-clz(count)
-  uint32_t all_count[kBins]; // the cluster's
   double all_mass[kBins];
+  double pick_d;
+  uint32_t count[kBins];      // the block's
+  uint32_t mass[kBins];       // the block's, as multiples of 2^-clz(count)
+  uint32_t all_count[kBins];  // the cluster's
   float red[2][kWarps];
   int red_i[2][kWarps];
-  float out_f[4];            // read by the other blocks
-  int out_i[4];
-  double pick_d[2];
+  float out_f[4];             // read by the other blocks
+  uint32_t out_i[4];
   uint32_t pick[4];
   uint32_t listed;
 };
@@ -82,26 +87,39 @@ __device__ __forceinline__ void row_sync() {
     __syncthreads();
 }
 
-// Bits in the order of the values.
+// Bits in the order of the values; -0 is 0.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);
   return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
+// A place in the sorted row, lower ones first.
+__device__ __forceinline__ unsigned long long place_of(float x, int idx) {
+  return static_cast<unsigned long long>(~key_of(x)) << 32 | static_cast<uint32_t>(idx);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr float kStep = LOG2E_F / 16.f;  // of a bin, in powers of two of p
 
 // What the blocks of a row share of it.
 struct Row {
   float top;      // its largest value
   float k2;       // log2(e) / T
-  uint32_t ckey;  // kept so far: keys above ckey, and of those equal to it the indexes up to cidx
+  float to_bin;   // 16 / T
+  float cut;      // kept so far: values above cut, and of those equal to it the indexes up to cidx
   int cidx;
 };
 __device__ __forceinline__ float prob(const Row& r, float x) { return ex2_approx((x - r.top) * r.k2); }
-__device__ __forceinline__ bool keeps(const Row& r, uint32_t key, int idx) { return key > r.ckey || (key == r.ckey && idx <= r.cidx); }
+__device__ __forceinline__ int bin_of(const Row& r, float x) { return static_cast<int>(fminf((r.top - x) * r.to_bin, 255.f)); }
+__device__ __forceinline__ bool keeps(const Row& r, float x, int idx) { return x > r.cut || (x == r.cut && idx <= r.cidx); }
 
-// The block's slice: element j (0 ... slice) is symbol first + j of the row, those below 0 and from `symbols` on are -inf.
+// The block's slice: element j (0 ... size) is symbol first + j of the row, those below 0 and from `symbols` on are -inf.
 template <class T, bool HELD>
 struct Slice {
   const T* row;
@@ -110,17 +128,16 @@ struct Slice {
   __device__ __forceinline__ float at(int j) const {
     if (HELD) return held[j];
     const int i = first + j;
-    if (i < 0 || i >= symbols) return -INFINITY;
-    return fminf(to_float(row[i]), FLT_MAX) + 0.f;
+    return i < 0 || i >= symbols ? -INFINITY : fminf(to_float(row[i]), FLT_MAX);
   }
 };
 
-// Loads the slice; the thread's largest value, and whether it saw a NaN.  Infinity counts as the largest number, -0 as 0.
+// Loads the slice; the thread's largest value, NaN if it saw one.
 template <class T, bool HELD>
-__device__ __forceinline__ void load_slice(const Slice<T, HELD>& s, float& top, int& nan) {
+__device__ __forceinline__ float load_slice(const Slice<T, HELD>& s) {
   constexpr int N = Pack<T, 16>::N;
-  top = -INFINITY;
-  nan = 0;
+  float top = -INFINITY;
+#pragma unroll 4
   for (int j = static_cast<int>(threadIdx.x) * N; j < s.size; j += kThreads * N) {
     const int i = s.first + j;
     float v[N];
@@ -133,20 +150,36 @@ __device__ __forceinline__ void load_slice(const Slice<T, HELD>& s, float& top, 
       for (int e = 0; e < N; ++e) v[e] = i + e >= 0 && i + e < s.symbols ? to_float(s.row[i + e]) : -INFINITY;
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      nan |= v[e] != v[e];
-      v[e] = fminf(v[e], FLT_MAX) + 0.f;
-      top = fmaxf(top, v[e]);
-      if (HELD) s.held[j + e] = v[e];
+    for (int e = 0; e < N; ++e) top = max_nan(top, v[e]);
+    if (HELD) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) *reinterpret_cast<float4*>(s.held + j + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
     }
+  }
+  return top;
+}
+
+// f(x, j) for the thread's elements of the slice.
+template <class T, bool HELD, class F>
+__device__ __forceinline__ void for_slice(const Slice<T, HELD>& s, F f) {
+  if (HELD) {
+#pragma unroll 2
+    for (int j = static_cast<int>(threadIdx.x) * 4; j < s.size; j += kThreads * 4) {
+      const float4 v = *reinterpret_cast<const float4*>(s.held + j);
+      f(v.x, j);
+      f(v.y, j + 1);
+      f(v.z, j + 2);
+      f(v.w, j + 3);
+    }
+  } else {
+    for (int j = threadIdx.x; j < s.size; j += kThreads) f(s.at(j), j);
   }
 }
 
 // Sum over the row of a value of each thread: warps, the block, then the blocks by rank.  Every thread has it.
 template <int C>
 __device__ __forceinline__ float row_sum(float v, Shared& sh) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  v = block_sum(v, sh.red[0], warp, lane, kWarps);
+  v = block_sum(v, sh.red[0], threadIdx.x >> 5, threadIdx.x & 31, kWarps);
   if (C == 1) {
     __syncthreads();
     return v;
@@ -160,9 +193,14 @@ __device__ __forceinline__ float row_sum(float v, Shared& sh) {
   return s;
 }
 
-// The cluster's counts (and masses, each block's in units of its own) from the blocks' ones.  `mass_of_bin(b)`: p at the upper end of a bin.
+__device__ __forceinline__ void clear_bins(uint32_t* bins) {
+  for (int b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
+}
+
+// The cluster's counts (and masses, each block's in units of its own) from the blocks' ones.  `upper(b)`: the p that bin b's masses are
+// multiples of.
 template <int C, class F>
-__device__ __forceinline__ void merge_bins(Shared& sh, bool masses, F mass_of_bin) {
+__device__ __forceinline__ void merge_bins(Shared& sh, bool counts, bool masses, F upper) {
   row_sync<C>();
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
     uint32_t n = 0;
@@ -173,64 +211,173 @@ __device__ __forceinline__ void merge_bins(Shared& sh, bool masses, F mass_of_bi
       n += c;
       if (masses && c != 0) m += ldexp(static_cast<double>(C > 1 ? peer_u32(&sh.mass[b], r) : sh.mass[b]), -__clz(static_cast<int>(c)));
     }
-    sh.all_count[b] = n;
-    if (masses) sh.all_mass[b] = n != 0 ? m * static_cast<double>(mass_of_bin(b)) : 0.0;
+    if (counts) sh.all_count[b] = n;
+    if (masses) sh.all_mass[b] = m > 0.0 ? m * static_cast<double>(upper(b)) : 0.0;
   }
   row_sync<C>();
 }
 
-// The end of the prefix of the kept symbols whose number, or mass, first reaches `target` (more than nothing, at most what there is), by
-// radix selection over all of the row.  Sets r.ckey and r.cidx.
+// Warp 0: the first bin with something where the running sum of `value(b)` from `start` on reaches `target`, or -1; *before: the sum before
+// it, *filled: the last bin with something, or -1, and *before_filled.  Lane l has bins 8 l ... 8 l + 7.
+template <class V>
+struct Found {
+  int bin, filled;
+  V before, before_filled;
+};
+template <class V, class F>
+__device__ __forceinline__ Found<V> first_bin(V start, V target, F value) {
+  const int lane = threadIdx.x & 31;
+  V v[8], total = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = value(lane * 8 + i);
+    total += v[i];
+  }
+  V upto = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
+  }
+  V sum = __shfl_up_sync(0xffffffffu, upto, 1);
+  sum = start + (lane == 0 ? V(0) : sum);
+  Found<V> f = {-1, -1, sum, sum};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const V next = sum + v[i];
+    if (v[i] > 0) {
+      f.filled = lane * 8 + i;
+      f.before_filled = sum;
+      if (next >= target && f.bin < 0) {
+        f.bin = lane * 8 + i;
+        f.before = sum;
+      }
+    }
+    sum = next;
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, f.bin >= 0), any = __ballot_sync(0xffffffffu, f.filled >= 0);
+  const int first = who != 0 ? __ffs(static_cast<int>(who)) - 1 : 0, last = any != 0 ? 31 - __clz(static_cast<int>(any)) : 0;
+  f.bin = __shfl_sync(0xffffffffu, f.bin, first);
+  f.before = __shfl_sync(0xffffffffu, f.before, first);
+  f.filled = __shfl_sync(0xffffffffu, f.filled, last);
+  f.before_filled = __shfl_sync(0xffffffffu, f.before_filled, last);
+  return f;
+}
+// ... and the last one with something where none reaches it: the sums were rounded on two ways.
+template <class V>
+__device__ __forceinline__ int bin_or_last(const Found<V>& f, V* before) {
+  *before = f.bin >= 0 ? f.before : f.before_filled;
+  return max(f.bin >= 0 ? f.bin : f.filled, 0);
+}
+
+__device__ __forceinline__ uint32_t mass_units(float share, uint32_t count) {  // (the count's bits and the mass's make 32: no overflow)
+  return static_cast<uint32_t>(ldexpf(fminf(share, 1.f), __clz(static_cast<int>(count))));
+}
+
+// Sorts list[0 ... n) and fills it up to the next power of two.
+__device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
+  int size = 2;
+  while (size < n) size *= 2;
+  for (int i = n + static_cast<int>(threadIdx.x); i < size; i += kThreads) list[i] = ~0ull;
+  __syncthreads();
+  for (int span = 2; span <= size; span *= 2) {
+    for (int step = span / 2; step > 0; step /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+        const int a = 2 * i - (i & (step - 1)), b = a + step;
+        const unsigned long long u = list[a], v = list[b];
+        if ((u > v) == ((a & span) == 0)) {
+          list[a] = v;
+          list[b] = u;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// The first block's list and behind it the others'; their number.
+template <int C>
+__device__ __forceinline__ int gather_lists(Shared& sh) {
+  int have = static_cast<int>(sh.listed);
+  for (int q = 1; q < C; ++q) {
+    const int more = static_cast<int>(peer_u32(&sh.listed, q));
+    for (int i = threadIdx.x; i < more; i += kThreads) sh.list[have + i] = peer_u64(&sh.list[i], q);
+    have += more;
+  }
+  __syncthreads();
+  return have;
+}
+
+// The sums of p before each of the thread's kPart symbols of the sorted list's first `have`, and of all of them.
+constexpr int kPart = kList / kThreads;
+__device__ __forceinline__ void sorted_sums(Shared& sh, const Row& r, int have, float (&pr)[kPart], float& before, float& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPart; ++i) {
+    const int at = static_cast<int>(threadIdx.x) * kPart + i;
+    pr[i] = at < have ? prob(r, value_of(~static_cast<uint32_t>(sh.list[at] >> 32))) : 0.f;
+    sum += pr[i];
+  }
+  float upto = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float f = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += f;
+  }
+  if (lane == 31) sh.red[0][warp] = upto;
+  before = __shfl_up_sync(0xffffffffu, upto, 1);
+  if (lane == 0) before = 0.f;
+  __syncthreads();
+  all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sh.red[0][w];
+    all += sh.red[0][w];
+  }
+  __syncthreads();
+}
+
+// The end of the prefix of the kept symbols whose number, or mass, with the `above` of keys above `hi`, first reaches `target`, by radix selection over
+// the keys of lo ... hi.  Sets r.cut and r.cidx.
 template <int C, class T, bool HELD>
-__device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target) {
-  const int tid = threadIdx.x;
-  uint32_t hi = key_of(r.top), lo = max(r.ckey, key_of(-FLT_MAX));
-  double above = 0.0;
+__device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, uint32_t lo, uint32_t hi, double above) {
   uint32_t ties = 0;
   for (;;) {
-    const uint32_t range = hi - lo;
-    const int shift = max(0, 24 - __clz(static_cast<int>(range)));  // at most 256 bins
-    for (int b = tid; b < kBins; b += kThreads) sh.count[b] = sh.mass[b] = 0;
+    const int shift = max(0, 24 - __clz(static_cast<int>(hi - lo)));  // at most 256 bins
+    clear_bins(sh.count);
+    clear_bins(sh.mass);
     __syncthreads();
-    for (int j = tid; j < s.size; j += kThreads) {
-      const float x = s.at(j);
+    for_slice(s, [&](float x, int j) {
       const uint32_t key = key_of(x);
-      if (x > -INFINITY && key >= lo && key <= hi && keeps(r, key, s.first + j)) atomicAdd(&sh.count[(hi - key) >> shift], 1u);
-    }
+      if (key >= lo && key <= hi && keeps(r, x, s.first + j)) atomicAdd(&sh.count[(hi - key) >> shift], 1u);
+    });
     auto upper = [&](int b) { return fminf(value_of(hi - (static_cast<uint32_t>(b) << shift)), r.top); };
     if (by_mass) {
       __syncthreads();
-      for (int j = tid; j < s.size; j += kThreads) {
-        const float x = s.at(j);
+      for_slice(s, [&](float x, int j) {
         const uint32_t key = key_of(x);
-        if (x > -INFINITY && key >= lo && key <= hi && keeps(r, key, s.first + j)) {
+        if (key >= lo && key <= hi && keeps(r, x, s.first + j)) {
           const int b = static_cast<int>((hi - key) >> shift);
-          // (the count's bits and the mass's make 32: no overflow)
-          const float e = fminf(ex2_approx((x - upper(b)) * r.k2), 1.f);
-          atomicAdd(&sh.mass[b], static_cast<uint32_t>(ldexpf(e, __clz(static_cast<int>(sh.count[b])))));
+          atomicAdd(&sh.mass[b], mass_units(ex2_approx((x - upper(b)) * r.k2), sh.count[b]));
         }
-      }
+      });
     }
-    merge_bins<C>(sh, by_mass, [&](int b) { return prob(r, upper(b)); });
-    if (tid == 0) {
-      double sum = above;
-      int b = 0, last = 0;
-      double before = above;
-      for (; b < kBins; ++b) {
-        if (sh.all_count[b] == 0) continue;
-        last = b;
-        before = sum;
-        sum += by_mass ? sh.all_mass[b] : static_cast<double>(sh.all_count[b]);
-        if (sum >= target) break;
+    merge_bins<C>(sh, true, by_mass, [&](int b) { return prob(r, upper(b)); });
+    if (threadIdx.x < 32) {
+      double before;
+      const int b = bin_or_last(
+          first_bin<double>(above, target, [&](int i) { return by_mass ? sh.all_mass[i] : static_cast<double>(sh.all_count[i]); }), &before);
+      if (threadIdx.x == 0) {
+        sh.pick[0] = static_cast<uint32_t>(b);
+        sh.pick[1] = sh.all_count[b];
+        sh.pick_d = before;
       }
-      sh.pick[0] = static_cast<uint32_t>(last);
-      sh.pick[1] = sh.all_count[last];
-      sh.pick_d[0] = before;
     }
     __syncthreads();
     const uint32_t b = sh.pick[0];
     ties = sh.pick[1];
-    above = sh.pick_d[0];
+    above = sh.pick_d;
     hi -= b << shift;
     lo = max(lo, hi - ((1u << shift) - 1u));
     __syncthreads();
@@ -244,19 +391,20 @@ __device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_
   if (want < ties) {
     while (to - from > 1) {
       const int width = (to - from + kBins - 1) / kBins;
-      for (int b = tid; b < kBins; b += kThreads) sh.count[b] = 0;
+      clear_bins(sh.count);
       __syncthreads();
-      for (int j = tid; j < s.size; j += kThreads) {
+      for_slice(s, [&](float x, int j) {
         const int i = s.first + j;
-        if (i >= from && i < to && key_of(s.at(j)) == hi && keeps(r, hi, i)) atomicAdd(&sh.count[(i - from) / width], 1u);
-      }
-      merge_bins<C>(sh, false, [](int) { return 0.f; });
-      if (tid == 0) {
-        uint32_t sum = 0;
-        int b = 0;
-        while (b < kBins - 1 && sum + sh.all_count[b] < want) sum += sh.all_count[b++];
-        sh.pick[0] = static_cast<uint32_t>(b);
-        sh.pick[1] = sum;
+        if (i >= from && i < to && key_of(x) == hi && keeps(r, x, i)) atomicAdd(&sh.count[(i - from) / width], 1u);
+      });
+      merge_bins<C>(sh, true, false, [](int) { return 0.f; });
+      if (threadIdx.x < 32) {
+        uint32_t before;
+        const int b = bin_or_last(first_bin<uint32_t>(0u, want, [&](int i) { return sh.all_count[i]; }), &before);
+        if (threadIdx.x == 0) {
+          sh.pick[0] = static_cast<uint32_t>(b);
+          sh.pick[1] = before;
+        }
       }
       __syncthreads();
       from += static_cast<int>(sh.pick[0]) * width;
@@ -265,10 +413,163 @@ __device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_
       __syncthreads();
     }
     r.cidx = from;
-  } else if (hi != r.ckey) {
+  } else if (value_of(hi) != r.cut) {
     r.cidx = INT32_MAX;
   }
-  r.ckey = hi;
+  r.cut = value_of(hi);
+}
+
+// The row's histogram of what is kept so far, in bins up to `last`: the blocks' in sh.count, all of it in sh.all_count.  Returns the row's sum of p where
+// `want_sum`.
+template <int C, class T, bool HELD>
+__device__ __forceinline__ float histogram(const Slice<T, HELD>& s, Shared& sh, const Row& r, int last, bool want_sum) {
+  clear_bins(sh.count);
+  __syncthreads();
+  float z = 0.f;
+  for_slice(s, [&](float x, int j) {
+    if (keeps(r, x, s.first + j)) {
+      const int b = bin_of(r, x);
+      if (b <= last) atomicAdd(&sh.count[b], 1u);
+      if (want_sum) z += prob(r, x);
+    }
+  });
+  if (want_sum) {
+    z = block_sum(z, sh.red[0], threadIdx.x >> 5, threadIdx.x & 31, kWarps);
+    if (threadIdx.x == 0) sh.out_f[1] = z;
+  }
+  merge_bins<C>(sh, true, false, [](int) { return 0.f; });
+  if (!want_sum) return 0.f;
+  z = 0.f;
+#pragma unroll
+  for (int q = 0; q < C; ++q) z += C > 1 ? peer_f32(&sh.out_f[1], q) : sh.out_f[1];
+  row_sync<C>();
+  return z;
+}
+
+// The end of the prefix of the kept symbols whose number, or mass, first reaches `target`, from their histogram.  Sets r.cut and r.cidx.
+template <int C, class T, bool HELD>
+__device__ void find_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int rank) {
+  const int tid = threadIdx.x;
+  if (by_mass) {
+    // a bin's symbols have p between 2^(-b kStep) and 2^(-(b + 1) kStep), but for the last bin's: the bins where the end may be
+    if (tid < 32) {
+      const float goal = static_cast<float>(target);
+      const Found<float> first = first_bin<float>(
+          0.f, goal * 0.9999f, [&](int b) { return static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b)); });
+      const Found<float> last = first_bin<float>(0.f, goal * 1.0001f, [&](int b) {
+        return b < kBins - 1 ? static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b + 1)) : 0.f;
+      });
+      if (tid == 0) {
+        sh.pick[0] = static_cast<uint32_t>(max(first.bin >= 0 ? first.bin : first.filled, 0));
+        sh.pick[1] = static_cast<uint32_t>(last.bin >= 0 ? last.bin : kBins - 1);
+      }
+    }
+    clear_bins(sh.mass);
+    __syncthreads();
+    const int from = static_cast<int>(sh.pick[0]), to = static_cast<int>(sh.pick[1]);
+    float sure = 0.f;
+    for_slice(s, [&](float x, int j) {
+      if (keeps(r, x, s.first + j)) {
+        const int b = bin_of(r, x);
+        if (b <= to) {
+          const float e = (x - r.top) * r.k2;
+          if (b < from)
+            sure += ex2_approx(e);
+          else
+            atomicAdd(&sh.mass[b], mass_units(ex2_approx(e + kStep * static_cast<float>(b)), sh.count[b]));
+        }
+      }
+    });
+    sure = block_sum(sure, sh.red[0], tid >> 5, tid & 31, kWarps);
+    if (tid == 0) sh.out_f[1] = sure;
+    merge_bins<C>(sh, false, true, [](int b) { return ex2_approx(-kStep * static_cast<float>(b)); });
+    if (tid < 32) {
+      double above = 0.0, before;
+#pragma unroll
+      for (int q = 0; q < C; ++q) above += static_cast<double>(C > 1 ? peer_f32(&sh.out_f[1], q) : sh.out_f[1]);
+      const int b = bin_or_last(first_bin<double>(above, target, [&](int i) { return sh.all_mass[i]; }), &before);
+      if (tid == 0) {
+        sh.pick[2] = static_cast<uint32_t>(b);
+        sh.pick_d = before;
+      }
+    }
+  } else if (tid < 32) {
+    uint32_t before;
+    const int b = bin_or_last(first_bin<uint32_t>(0u, static_cast<uint32_t>(target), [&](int i) { return sh.all_count[i]; }), &before);
+    if (tid == 0) {
+      sh.pick[2] = static_cast<uint32_t>(b);
+      sh.pick_d = static_cast<double>(before);
+    }
+  }
+  if (tid == 0) {
+    sh.listed = 0;
+    sh.pick[0] = 0xffffffffu;
+    sh.pick[1] = 0;
+  }
+  __syncthreads();
+  const int bin = static_cast<int>(sh.pick[2]);
+  const double above = sh.pick_d;
+  if (sh.all_count[bin] <= kList) {
+    for_slice(s, [&](float x, int j) {
+      if (keeps(r, x, s.first + j) && bin_of(r, x) == bin) sh.list[atomicAdd(&sh.listed, 1u)] = place_of(x, s.first + j);
+    });
+    row_sync<C>();
+    if (rank == 0) {
+      const int have = gather_lists<C>(sh);
+      sort_list(sh.list, have);
+      if (by_mass) {
+        float pr[kPart], before, all;
+        sorted_sums(sh, r, have, pr, before, all);
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) {
+          before += pr[i];
+          const int at = tid * kPart + i;
+          if (at < have && above + static_cast<double>(before) >= target) atomicMin(&sh.pick[0], static_cast<uint32_t>(at));
+        }
+        __syncthreads();
+      }
+      if (tid == 0) {
+        const double at = by_mass ? static_cast<double>(sh.pick[0]) : target - above - 1.0;
+        const unsigned long long place = sh.list[at < have - 1 ? static_cast<int>(fmax(at, 0.0)) : have - 1];
+        sh.out_f[2] = value_of(~static_cast<uint32_t>(place >> 32));
+        sh.out_i[1] = static_cast<uint32_t>(place);
+      }
+    }
+    row_sync<C>();
+    r.cut = C > 1 ? peer_f32(&sh.out_f[2], 0) : sh.out_f[2];
+    r.cidx = static_cast<int>(C > 1 ? peer_u32(&sh.out_i[1], 0) : sh.out_i[1]);
+    row_sync<C>();
+    return;
+  }
+  // the range of the bin's keys
+  uint32_t lo = 0xffffffffu, hi = 0;
+  for_slice(s, [&](float x, int j) {
+    if (keeps(r, x, s.first + j) && bin_of(r, x) == bin) {
+      lo = min(lo, key_of(x));
+      hi = max(hi, key_of(x));
+    }
+  });
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if ((tid & 31) == 0) {
+    atomicMin(&sh.pick[0], lo);
+    atomicMax(&sh.pick[1], hi);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    sh.out_i[2] = sh.pick[0];
+    sh.out_i[3] = sh.pick[1];
+  }
+  row_sync<C>();
+  lo = 0xffffffffu;
+  hi = 0;
+#pragma unroll
+  for (int q = 0; q < C; ++q) {
+    lo = min(lo, C > 1 ? peer_u32(&sh.out_i[2], q) : sh.out_i[2]);
+    hi = max(hi, C > 1 ? peer_u32(&sh.out_i[3], q) : sh.out_i[3]);
+  }
+  row_sync<C>();
+  select_end<C>(s, sh, r, by_mass, target, lo, hi, above);
 }
 
 // The better of two candidates: the larger score, of equal ones the lower index.
@@ -300,9 +601,12 @@ __device__ __forceinline__ void block_best(float& score, int& idx, float& sum, S
   }
 }
 
-__device__ __forceinline__ void write_answer(const SampleArgs& p, int64_t row, const Row& r, int idx, float x, float sum) {
-  p.token[row] = idx;
-  if (p.logprob != nullptr) p.logprob[row] = (x - r.top) * r.k2 * 0.6931471805599453f - logf(sum);
+template <class T, bool HELD>
+__device__ __forceinline__ void write_answer(const SampleArgs& p, int64_t row, const Slice<T, HELD>& s, const Row& r, int idx, float sum) {
+  const bool none = idx == INT32_MAX;  // (noise that is no number)
+  p.token[row] = none ? -1 : idx;
+  if (p.logprob != nullptr)
+    p.logprob[row] = none ? NAN : (fminf(to_float(s.row[idx]), FLT_MAX) - r.top) * r.k2 * 0.6931471805599453f - logf(sum);
 }
 
 template <class T, bool HELD, int C>
@@ -332,253 +636,135 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
     top_k = 1;
   }
 
-  float top;
-  int nan;
-  load_slice(s, top, nan);
+  const float mine = load_slice(s);
+  float top = mine;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  nan = __any_sync(0xffffffffu, nan);
-  if (lane == 0) {
-    sh.red[0][warp] = top;
-    sh.red_i[0][warp] = nan;
-  }
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) sh.red[0][warp] = top;
   if (tid == 0) sh.listed = 0;
-  for (int b = tid; b < kBins; b += kThreads) sh.count[b] = 0;
+  clear_bins(sh.count);
   __syncthreads();
-  top = -INFINITY;
-  nan = 0;
+  top = sh.red[0][0];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    top = fmaxf(top, sh.red[0][w]);
-    nan |= sh.red_i[0][w];
-  }
+  for (int w = 1; w < kWarps; ++w) top = max_nan(top, sh.red[0][w]);
   if (C > 1) {
-    if (tid == 0) {
-      sh.out_f[0] = top;
-      sh.out_i[0] = nan;
-    }
+    if (tid == 0) sh.out_f[0] = top;
     cluster_sync_all();
 #pragma unroll
-    for (int q = 0; q < C; ++q) {
-      top = fmaxf(top, peer_f32(&sh.out_f[0], q));
-      nan |= static_cast<int>(peer_u32(&sh.out_i[0], q));
-    }
+    for (int q = 0; q < C; ++q) top = max_nan(top, peer_f32(&sh.out_f[0], q));
   } else {
+    __syncthreads();
+  }
+  // (the same for all blocks of the row)
+  if (!(top > -INFINITY)) {
+    if (rank == 0 && tid == 0) {
+      p.token[row] = -1;
+      if (p.logprob != nullptr) p.logprob[row] = top;
+    }
+    if (C > 1) cluster_sync_all();
+    return;
+  }
+  if (top == INFINITY) {  // counts as the largest number
+    top = FLT_MAX;
+    if (HELD)
+      for (int j = tid; j < s.size; j += kThreads) s.held[j] = fminf(s.held[j], FLT_MAX);
     __syncthreads();
   }
   Row r;
   r.top = top;
   r.k2 = fminf(fmaxf(LOG2E_F / temperature, 1e-38f), FLT_MAX);
-  r.ckey = 0;
-  r.cidx = INT32_MAX;
+  r.to_bin = fminf(r.k2 / kStep, FLT_MAX);
+  r.cut = -INFINITY;
+  r.cidx = INT32_MIN;
 
-  if (nan || top == -INFINITY) {  // (the same for all blocks of the row)
-    if (rank == 0 && tid == 0) {
-      p.token[row] = -1;
-      if (p.logprob != nullptr) p.logprob[row] = nan ? NAN : -INFINITY;
-    }
-    if (C > 1) cluster_sync_all();
-    return;
-  }
-
-  bool by_count = top_k > 0 && top_k < p.symbols;
-  const bool by_mass = top_p < 1.f;
-  if (by_count || by_mass) {
-    // ---- the histogram
-    const float to_bin = r.k2 * (16.f / LOG2E_F);
-    auto bin_of = [&](float x) { return static_cast<int>(fminf((r.top - x) * to_bin, 255.f)); };
-    float z = 0.f;
-    for (int j = tid; j < s.size; j += kThreads) {
-      const float x = s.at(j);
-      if (x > -INFINITY) {
-        atomicAdd(&sh.count[bin_of(x)], 1u);
-        z += prob(r, x);
-      }
-    }
-    if (!by_count) z = row_sum<C>(z, sh);
-    merge_bins<C>(sh, false, [](int) { return 0.f; });
+  const bool by_count = top_k > 0 && top_k < p.symbols, by_mass = top_p < 1.f;
+  if (by_count && top_k <= kFew) {
+    // ---- what is below the k-th largest of the threads' maxima is not among the first k
+    if (mine > -INFINITY) atomicAdd(&sh.count[bin_of(r, mine)], 1u);
+    __syncthreads();
     if (tid < 32) {
-      // lane l has bins 8 l ... 8 l + 7
-      uint32_t n[8], total = 0;
-      float least[8], mass = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        n[i] = sh.all_count[lane * 8 + i];
-        total += n[i];
-        least[i] = lane * 8 + i < kBins - 1 ? static_cast<float>(n[i]) * ex2_approx(-LOG2E_F / 16.f * static_cast<float>(lane * 8 + i + 1)) : 0.f;
-        mass += least[i];
-      }
-      uint32_t upto = total;
-      float mass_upto = mass;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
-        const float f = __shfl_up_sync(0xffffffffu, mass_upto, o);
-        if (lane >= o) {
-          upto += u;
-          mass_upto += f;
-        }
-      }
-      const uint32_t everything = __shfl_sync(0xffffffffu, upto, 31);
-      uint32_t cum = upto - total;
-      float cum_mass = mass_upto - mass;
-      int bin = kBins;  // the first that surely reaches the end
-      uint32_t listed = 0;
-      const bool count_first = by_count && static_cast<uint32_t>(top_k) < everything;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        cum += n[i];
-        cum_mass += least[i];
-        const bool there = count_first ? cum >= static_cast<uint32_t>(top_k) : by_mass && !by_count && cum_mass >= top_p * z * 1.0001f;
-        if (there && bin == kBins) {
-          bin = lane * 8 + i;
-          listed = cum;
-        }
-      }
-      const unsigned who = __ballot_sync(0xffffffffu, bin < kBins);
-      const int src = who != 0 ? __ffs(static_cast<int>(who)) - 1 : 31;
-      bin = __shfl_sync(0xffffffffu, bin, src);
-      listed = who != 0 ? __shfl_sync(0xffffffffu, listed, src) : everything;
-      if (lane == 0) {
-        sh.pick[0] = static_cast<uint32_t>(min(bin, kBins - 1));
-        sh.pick[1] = listed;
-      }
+      const Found<uint32_t> f = first_bin<uint32_t>(0u, static_cast<uint32_t>(top_k), [&](int b) { return sh.count[b]; });
+      if (tid == 0) sh.pick[0] = static_cast<uint32_t>(f.bin >= 0 ? f.bin : kBins - 1);
     }
     __syncthreads();
-    const int end_bin = static_cast<int>(sh.pick[0]);
-    const uint32_t listed = sh.pick[1];
-
-    if (listed <= kList) {
-      // ---- few enough: the first block sorts them
-      for (int j = tid; j < s.size; j += kThreads) {
-        const float x = s.at(j);
-        if (x > -INFINITY && bin_of(x) <= end_bin) {
-          const uint32_t at = atomicAdd(&sh.listed, 1u);
-          sh.list[at] = static_cast<unsigned long long>(~key_of(x)) << 32 | static_cast<uint32_t>(s.first + j);
-        }
+    const int bound = static_cast<int>(sh.pick[0]);
+    for_slice(s, [&](float x, int j) {
+      if (x > -INFINITY && bin_of(r, x) <= bound) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kList) sh.list[at] = place_of(x, s.first + j);
       }
-      row_sync<C>();
+    });
+    row_sync<C>();
+    uint32_t listed = 0;
+#pragma unroll
+    for (int q = 0; q < C; ++q) listed += C > 1 ? peer_u32(&sh.listed, q) : sh.listed;
+    if (listed <= kList) {
       if (rank == 0) {
-        int have = static_cast<int>(sh.listed);
-        for (int q = 1; q < C; ++q) {
-          const int more = static_cast<int>(peer_u32(&sh.listed, q));
-          for (int i = tid; i < more; i += kThreads) sh.list[have + i] = peer_u64(&sh.list[i], q);
-          have += more;
-        }
-        int size = 2;
-        while (size < have) size *= 2;
-        for (int i = have + tid; i < size; i += kThreads) sh.list[i] = ~0ull;
-        __syncthreads();
-        for (int span = 2; span <= size; span *= 2) {
-          for (int step = span / 2; step > 0; step /= 2) {
-            for (int i = tid; i < size / 2; i += kThreads) {
-              const int a = 2 * i - (i & (step - 1)), b = a + step;
-              const unsigned long long u = sh.list[a], v = sh.list[b];
-              if ((u > v) == ((a & span) == 0)) {
-                sh.list[a] = v;
-                sh.list[b] = u;
-              }
-            }
-            __syncthreads();
-          }
-        }
-        // the thread's part of the sorted list, and the sum of p before it
-        constexpr int kPart = kList / kThreads;
-        if (by_count) have = min(have, top_k);
-        float pr[kPart], sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < kPart; ++i) {
-          const int at = tid * kPart + i;
-          pr[i] = at < have ? prob(r, value_of(~static_cast<uint32_t>(sh.list[at] >> 32))) : 0.f;
-          sum += pr[i];
-        }
-        float upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const float f = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += f;
-        }
-        if (lane == 31) sh.red[0][warp] = upto;
-        __syncthreads();
-        float before = upto - sum, all = 0.f;
-        if (lane == 0) before = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          if (w < warp) before += sh.red[0][w];
-          all += sh.red[0][w];
-        }
-        __syncthreads();
-        const float goal = by_mass ? top_p * (by_count ? all : z) : INFINITY;
+        const int have = min(gather_lists<C>(sh), top_k);
+        sort_list(sh.list, static_cast<int>(listed));
+        float pr[kPart], before, all;
+        sorted_sums(sh, r, have, pr, before, all);
+        const float goal = by_mass ? top_p * all : INFINITY;
         float score = -1.f, kept = 0.f;
         int idx = INT32_MAX;
 #pragma unroll
         for (int i = 0; i < kPart; ++i) {
           const int at = tid * kPart + i;
           if (at < have && (before < goal || at == 0) && pr[i] >= min_p) {
-            const int sym = static_cast<int>(static_cast<uint32_t>(sh.list[at]));
-            better(score, idx, pr[i] / noise[sym], sym);
+            const int symbol = static_cast<int>(static_cast<uint32_t>(sh.list[at]));
+            better(score, idx, pr[i] / noise[symbol], symbol);
             kept += pr[i];
           }
           before += pr[i];
         }
         block_best(score, idx, kept, sh);
-        if (tid == 0) write_answer(p, row, r, idx == INT32_MAX ? -1 : idx, idx == INT32_MAX ? r.top : fminf(to_float(s.row[idx]), FLT_MAX), kept);
+        if (tid == 0) write_answer(p, row, s, r, idx, kept);
       }
       if (C > 1) cluster_sync_all();  // (the other blocks' lists are read until here)
       return;
     }
-    // ---- too many
-    if (by_count) {
-      uint32_t possible = 0;
-      for (int b = 0; b < kBins; ++b) possible += sh.all_count[b];
-      __syncthreads();
-      if (static_cast<uint32_t>(top_k) < possible) select_end<C>(s, sh, r, false, static_cast<double>(top_k));
-      if (by_mass) {
-        z = 0.f;
-        for (int j = tid; j < s.size; j += kThreads) {
-          const float x = s.at(j);
-          if (x > -INFINITY && keeps(r, key_of(x), s.first + j)) z += prob(r, x);
-        }
-        z = row_sum<C>(z, sh);
-      }
-    }
-    __syncthreads();
-    if (by_mass) select_end<C>(s, sh, r, true, fmax(static_cast<double>(top_p), 0.0) * static_cast<double>(z));
-    __syncthreads();
+    row_sync<C>();
+  }
+  if (by_count) {
+    histogram<C>(s, sh, r, kBins - 1, false);
+    find_end<C>(s, sh, r, false, static_cast<double>(top_k), rank);
+  }
+  if (by_mass) {
+    // a symbol with p below (1 - top_p) / symbols is behind the end: all such ones together have less than 1 - top_p, the first alone has 1
+    const float last = by_count ? 255.f : 16.f * logf(static_cast<float>(p.symbols) / (1.f - fmaxf(top_p, 0.f))) + 1.f;
+    const float z = histogram<C>(s, sh, r, static_cast<int>(fminf(last, 255.f)), true);
+    find_end<C>(s, sh, r, true, static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(z), rank);
   }
 
   // ---- all that is kept
   float score = -1.f, kept = 0.f;
   int idx = INT32_MAX;
-#pragma unroll 4
-  for (int j = tid; j < s.size; j += kThreads) {
-    const float x = s.at(j);
+  for_slice(s, [&](float x, int j) {
     const int i = s.first + j;
     const float pr = prob(r, x);
-    if (x > -INFINITY && pr >= min_p && keeps(r, key_of(x), i)) {
+    if (keeps(r, x, i) && pr >= min_p) {
       better(score, idx, pr / __ldg(noise + i), i);
       kept += pr;
     }
-  }
+  });
   block_best(score, idx, kept, sh);
   if (C > 1) {
     if (tid == 0) {
       sh.out_f[2] = score;
       sh.out_f[3] = kept;
-      sh.out_i[2] = idx;
+      sh.out_i[0] = static_cast<uint32_t>(idx);
     }
     cluster_sync_all();
     if (rank == 0 && tid == 0) {
 #pragma unroll
       for (int q = 1; q < C; ++q) {
-        better(score, idx, peer_f32(&sh.out_f[2], q), static_cast<int>(peer_u32(&sh.out_i[2], q)));
+        better(score, idx, peer_f32(&sh.out_f[2], q), static_cast<int>(peer_u32(&sh.out_i[0], q)));
         kept += peer_f32(&sh.out_f[3], q);
       }
     }
     cluster_sync_all();
   }
-  if (rank == 0 && tid == 0)
-    write_answer(p, row, r, idx == INT32_MAX ? -1 : idx, idx == INT32_MAX ? r.top : fminf(to_float(s.row[idx]), FLT_MAX), kept);
+  if (rank == 0 && tid == 0) write_answer(p, row, s, r, idx, kept);
 }
 
 // ----------------------------------------------------------------------------- launches
