@@ -31,7 +31,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 256;
-constexpr int kList = 2048;  // symbols that are sorted
+constexpr int kList = 2048;  // symbols that the first block of a row can gather
+constexpr int kWarpKept = 256;  // symbols that a warp can set apart
 constexpr int kFew = kThreads / 2;  // a small top_k
 
 struct SampleArgs {
@@ -57,10 +58,14 @@ struct Shared {
   uint32_t count[kBins];      // the block's
   uint32_t mass[kBins];       // the block's, as multiples of 2^-clz(count)
   uint32_t all_count[kBins];  // the cluster's
+  uint16_t kept[kWarps][kWarpKept];
+  unsigned long long few[33];
   float red[2][kWarps];
   int red_i[2][kWarps];
-  float out_f[4];             // read by the other blocks
-  uint32_t out_i[4];
+  // read by the other blocks, each written once or with a row_sync between
+  float out_top, out_z, out_sure, out_cut, out_score, out_sum;
+  int out_cidx, out_idx;
+  uint32_t out_lo, out_hi;
   uint32_t pick[4];
   uint32_t listed;
 };
@@ -116,7 +121,15 @@ struct Row {
   int cidx;
 };
 __device__ __forceinline__ float prob(const Row& r, float x) { return ex2_approx((x - r.top) * r.k2); }
-__device__ __forceinline__ int bin_of(const Row& r, float x) { return static_cast<int>(fminf((r.top - x) * r.to_bin, 255.f)); }
+// (the whole part of a number below 2^23 stands in the last bits of its sum with 2^23: no conversion)
+__device__ __forceinline__ int whole_part(float t) { return __float_as_int(__fadd_rz(t, 8388608.f)) & 0x3ff; }
+__device__ __forceinline__ float bin_place(const Row& r, float x) { return (r.top - x) * r.to_bin; }
+// (a symbol so far below the top that 32 bits do not hold how far has p = 0: it is in no bin, as one of -inf)
+constexpr int kNoBin = 0x7fff;
+__device__ __forceinline__ int bin_of(const Row& r, float x) {
+  const float t = bin_place(r, x);
+  return t < FLT_MAX ? whole_part(fminf(t, 255.f)) : kNoBin;
+}
 __device__ __forceinline__ bool keeps(const Row& r, float x, int idx) { return x > r.cut || (x == r.cut && idx <= r.cidx); }
 
 // The block's slice: element j (0 ... size) is symbol first + j of the row, those below 0 and from `symbols` on are -inf.
@@ -125,6 +138,8 @@ struct Slice {
   const T* row;
   float* held;
   int first, size, symbols;
+  const uint16_t* kept;  // what the warp has set apart, or nullptr
+  int kept_count;
   __device__ __forceinline__ float at(int j) const {
     if (HELD) return held[j];
     const int i = first + j;
@@ -176,21 +191,45 @@ __device__ __forceinline__ void for_slice(const Slice<T, HELD>& s, F f) {
   }
 }
 
-// Sum over the row of a value of each thread: warps, the block, then the blocks by rank.  Every thread has it.
-template <int C>
-__device__ __forceinline__ float row_sum(float v, Shared& sh) {
-  v = block_sum(v, sh.red[0], threadIdx.x >> 5, threadIdx.x & 31, kWarps);
-  if (C == 1) {
-    __syncthreads();
-    return v;
+// ... or for all of the thread's that can still be kept, where those were set apart.
+template <class T, bool HELD, class F>
+__device__ __forceinline__ void for_kept(const Slice<T, HELD>& s, F f) {
+  if (HELD && s.kept != nullptr) {
+    for (int i = threadIdx.x & 31; i < s.kept_count; i += 32) {
+      const int j = s.kept[i];
+      f(s.held[j], j);
+    }
+  } else {
+    for_slice(s, f);
   }
-  if (threadIdx.x == 0) sh.out_f[1] = v;
-  cluster_sync_all();
-  float s = 0.f;
+}
+
+// Sets apart the symbols of the bins up to `last`, each warp its own.  What follows goes over some percent of the slice, and its lanes have work.
+template <class T, bool HELD>
+__device__ __forceinline__ void set_apart(Slice<T, HELD>& s, Shared& sh, const Row& r, int last) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float limit = last < kBins - 1 ? static_cast<float>(last + 1) : FLT_MAX;
+  uint16_t* kept = sh.kept[warp];
+  int n = 0;
+  for (int j0 = warp * 128; j0 < s.size; j0 += kThreads * 4) {
+    const int j = j0 + lane * 4;
+    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (j < s.size) v = *reinterpret_cast<const float4*>(s.held + j);
+    const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int r = 0; r < C; ++r) s += peer_f32(&sh.out_f[1], r);
-  cluster_sync_all();
-  return s;
+    for (int e = 0; e < 4; ++e) {
+      const bool in = bin_place(r, x[e]) < limit;
+      const unsigned who = __ballot_sync(0xffffffffu, in);
+      const int at = n + __popc(who & ((1u << lane) - 1u));
+      if (in && at < kWarpKept) kept[at] = static_cast<uint16_t>(j + e);
+      n += __popc(who);
+    }
+  }
+  __syncwarp();
+  if (n <= kWarpKept) {  // (else the warp goes over all of its part: its lanes' elements of the slice, as before)
+    s.kept = kept;
+    s.kept_count = n;
+  }
 }
 
 __device__ __forceinline__ void clear_bins(uint32_t* bins) {
@@ -198,7 +237,7 @@ __device__ __forceinline__ void clear_bins(uint32_t* bins) {
 }
 
 // The cluster's counts (and masses, each block's in units of its own) from the blocks' ones.  `upper(b)`: the p that bin b's masses are
-// multiples of.
+// multiples of.  The blocks' bins are read until the next row_sync.
 template <int C, class F>
 __device__ __forceinline__ void merge_bins(Shared& sh, bool counts, bool masses, F upper) {
   row_sync<C>();
@@ -214,7 +253,7 @@ __device__ __forceinline__ void merge_bins(Shared& sh, bool counts, bool masses,
     if (counts) sh.all_count[b] = n;
     if (masses) sh.all_mass[b] = m > 0.0 ? m * static_cast<double>(upper(b)) : 0.0;
   }
-  row_sync<C>();
+  __syncthreads();
 }
 
 // Warp 0: the first bin with something where the running sum of `value(b)` from `start` on reaches `target`, or -1; *before: the sum before
@@ -274,8 +313,21 @@ __device__ __forceinline__ uint32_t mass_units(float share, uint32_t count) {  /
   return static_cast<uint32_t>(ldexpf(fminf(share, 1.f), __clz(static_cast<int>(count))));
 }
 
-// Sorts list[0 ... n) and fills it up to the next power of two.
+// Sorts list[0 ... n) and fills it up to the next power of two.  A list of up to 128 by counting for each what is before it.
 __device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
+  if (n <= 128) {
+    constexpr int kShare = kThreads / 128;  // threads to an element
+    const int i = static_cast<int>(threadIdx.x) / kShare, part = static_cast<int>(threadIdx.x) % kShare;
+    const unsigned long long mine = i < n ? list[i] : ~0ull;
+    int before = 0;
+    for (int j = part; j < n; j += kShare) before += list[j] < mine;
+#pragma unroll
+    for (int o = 1; o < kShare; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    __syncthreads();
+    if (part == 0 && i < n) list[before] = mine;
+    __syncthreads();
+    return;
+  }
   int size = 2;
   while (size < n) size *= 2;
   for (int i = n + static_cast<int>(threadIdx.x); i < size; i += kThreads) list[i] = ~0ull;
@@ -348,14 +400,14 @@ __device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_
     clear_bins(sh.count);
     clear_bins(sh.mass);
     __syncthreads();
-    for_slice(s, [&](float x, int j) {
+    for_kept(s, [&](float x, int j) {
       const uint32_t key = key_of(x);
       if (key >= lo && key <= hi && keeps(r, x, s.first + j)) atomicAdd(&sh.count[(hi - key) >> shift], 1u);
     });
     auto upper = [&](int b) { return fminf(value_of(hi - (static_cast<uint32_t>(b) << shift)), r.top); };
     if (by_mass) {
       __syncthreads();
-      for_slice(s, [&](float x, int j) {
+      for_kept(s, [&](float x, int j) {
         const uint32_t key = key_of(x);
         if (key >= lo && key <= hi && keeps(r, x, s.first + j)) {
           const int b = static_cast<int>((hi - key) >> shift);
@@ -380,7 +432,7 @@ __device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_
     above = sh.pick_d;
     hi -= b << shift;
     lo = max(lo, hi - ((1u << shift) - 1u));
-    __syncthreads();
+    row_sync<C>();  // (all have read the bins)
     if (shift == 0) break;
   }
   // all that is left has one value: the first few by index
@@ -393,7 +445,7 @@ __device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_
       const int width = (to - from + kBins - 1) / kBins;
       clear_bins(sh.count);
       __syncthreads();
-      for_slice(s, [&](float x, int j) {
+      for_kept(s, [&](float x, int j) {
         const int i = s.first + j;
         if (i >= from && i < to && key_of(x) == hi && keeps(r, x, i)) atomicAdd(&sh.count[(i - from) / width], 1u);
       });
@@ -410,13 +462,135 @@ __device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_
       from += static_cast<int>(sh.pick[0]) * width;
       to = min(to, from + width);
       want -= sh.pick[1];
-      __syncthreads();
+      row_sync<C>();
     }
     r.cidx = from;
   } else if (value_of(hi) != r.cut) {
     r.cidx = INT32_MAX;
   }
   r.cut = value_of(hi);
+}
+
+// One round of radix selection over list[0 ... n), of which the places with their upper halves in lo ... hi are in question and `above` (a number or
+// mass) lies before them: narrows the range to the bin where `target` is reached.  Returns how many are in it.
+__device__ __forceinline__ uint32_t narrow_list(Shared& sh, const Row& r, int n, bool by_mass, double target, uint32_t& lo, uint32_t& hi, double& above) {
+  const int shift = max(0, 24 - __clz(static_cast<int>(hi - lo)));
+  clear_bins(sh.count);
+  clear_bins(sh.mass);
+  __syncthreads();
+  auto upper = [&](int b) { return fminf(value_of(~(lo + (static_cast<uint32_t>(b) << shift))), r.top); };
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+    if (k >= lo && k <= hi) atomicAdd(&sh.count[(k - lo) >> shift], 1u);
+  }
+  __syncthreads();
+  if (by_mass) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+      if (k >= lo && k <= hi) {
+        const int b = static_cast<int>((k - lo) >> shift);
+        atomicAdd(&sh.mass[b], mass_units(ex2_approx((value_of(~k) - upper(b)) * r.k2), sh.count[b]));
+      }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x < 32) {
+    double before;
+    const int b = bin_or_last(first_bin<double>(above, target, [&](int i) {
+                                const uint32_t c = sh.count[i];
+                                return !by_mass ? static_cast<double>(c)
+                                       : c == 0 ? 0.0
+                                                : ldexp(static_cast<double>(sh.mass[i]), -__clz(static_cast<int>(c))) * static_cast<double>(prob(r, upper(i)));
+                              }),
+                              &before);
+    if (threadIdx.x == 0) {
+      sh.pick[0] = static_cast<uint32_t>(b);
+      sh.pick[1] = sh.count[b];
+      sh.pick_d = before;
+    }
+  }
+  __syncthreads();
+  above = sh.pick_d;
+  lo += sh.pick[0] << shift;
+  if (shift > 0) hi = min(hi, lo + ((1u << shift) - 1u));
+  else hi = lo;
+  const uint32_t in = sh.pick[1];
+  __syncthreads();
+  return in;
+}
+
+// The range of the upper halves of list[0 ... n).
+__device__ __forceinline__ void range_of_list(Shared& sh, int n, uint32_t& lo, uint32_t& hi) {
+  lo = 0xffffffffu;
+  hi = 0;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+    lo = min(lo, k);
+    hi = max(hi, k);
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    sh.red_i[0][warp] = static_cast<int>(lo);
+    sh.red_i[1][warp] = static_cast<int>(hi);
+  }
+  __syncthreads();
+  lo = __reduce_min_sync(0xffffffffu, lane < kWarps ? static_cast<uint32_t>(sh.red_i[0][lane]) : 0xffffffffu);
+  hi = __reduce_max_sync(0xffffffffu, lane < kWarps ? static_cast<uint32_t>(sh.red_i[1][lane]) : 0u);
+  __syncthreads();
+}
+
+// The place in list[0 ... n) where, with the `above` before the list, `target` is reached.  The list's order is lost.
+__device__ __forceinline__ unsigned long long end_in_list(Shared& sh, const Row& r, int n, bool by_mass, double target, double above) {
+  uint32_t lo, hi, in = static_cast<uint32_t>(n);
+  range_of_list(sh, n, lo, hi);
+  while (in > 32 && lo != hi) in = narrow_list(sh, r, n, by_mass, target, lo, hi, above);
+  // what is outside goes to the end
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+    if (k < lo || k > hi) sh.list[i] = ~0ull;
+  }
+  if (threadIdx.x == 0) sh.pick[0] = 0;
+  __syncthreads();
+  if (in <= 32) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const unsigned long long place = sh.list[i];
+      if (place != ~0ull) sh.few[atomicAdd(&sh.pick[0], 1u)] = place;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const int lane = threadIdx.x, have = static_cast<int>(in);
+      const unsigned long long mine = lane < have ? sh.few[lane] : ~0ull;
+      int rank = 0;
+#pragma unroll 8
+      for (int l = 0; l < have; ++l) rank += __shfl_sync(0xffffffffu, mine, l) < mine;
+      __syncwarp();
+      if (lane < have) sh.few[rank] = mine;
+      __syncwarp();
+      int at;
+      if (by_mass) {
+        float upto = lane < have ? prob(r, value_of(~static_cast<uint32_t>(sh.few[lane] >> 32))) : 0.f;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float f = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += f;
+        }
+        const unsigned reached = __ballot_sync(0xffffffffu, lane < have && above + static_cast<double>(upto) >= target);
+        at = reached != 0 ? __ffs(static_cast<int>(reached)) - 1 : have - 1;
+      } else {
+        at = min(max(static_cast<int>(target - above) - 1, 0), have - 1);
+      }
+      if (lane == 0) sh.few[32] = sh.few[at];
+    }
+    __syncthreads();
+    return sh.few[32];
+  }
+  // more than that of one value: by index
+  sort_list(sh.list, n);
+  const double each = by_mass ? static_cast<double>(prob(r, value_of(~lo))) : 1.0;
+  const double wanted = each > 0.0 ? ceil((target - above) / each) : 1.0;
+  return sh.list[wanted < 1.0 ? 0u : min(wanted < 4e9 ? static_cast<uint32_t>(wanted) : in, in) - 1u];
 }
 
 // The row's histogram of what is kept so far, in bins up to `last`: the blocks' in sh.count, all of it in sh.all_count.  Returns the row's sum of p where
@@ -426,147 +600,146 @@ __device__ __forceinline__ float histogram(const Slice<T, HELD>& s, Shared& sh, 
   clear_bins(sh.count);
   __syncthreads();
   float z = 0.f;
-  for_slice(s, [&](float x, int j) {
-    if (keeps(r, x, s.first + j)) {
-      const int b = bin_of(r, x);
-      if (b <= last) atomicAdd(&sh.count[b], 1u);
+  const float limit = last < kBins - 1 ? static_cast<float>(last + 1) : FLT_MAX;
+  if (r.cut == -INFINITY) {
+    for_slice(s, [&](float x, int) {
+      const float t = bin_place(r, x);  // (infinite for -inf)
+      if (t < limit) atomicAdd(&sh.count[whole_part(fminf(t, 255.f))], 1u);
       if (want_sum) z += prob(r, x);
-    }
-  });
+    });
+  } else {
+    for_kept(s, [&](float x, int j) {
+      if (keeps(r, x, s.first + j)) {
+        const int b = bin_of(r, x);
+        if (b < kBins) atomicAdd(&sh.count[b], 1u);
+        z += prob(r, x);
+      }
+    });
+  }
   if (want_sum) {
     z = block_sum(z, sh.red[0], threadIdx.x >> 5, threadIdx.x & 31, kWarps);
-    if (threadIdx.x == 0) sh.out_f[1] = z;
+    if (threadIdx.x == 0) sh.out_z = z;
   }
   merge_bins<C>(sh, true, false, [](int) { return 0.f; });
-  if (!want_sum) return 0.f;
   z = 0.f;
 #pragma unroll
-  for (int q = 0; q < C; ++q) z += C > 1 ? peer_f32(&sh.out_f[1], q) : sh.out_f[1];
-  row_sync<C>();
+  for (int q = 0; q < C; ++q) z += C > 1 ? peer_f32(&sh.out_z, q) : sh.out_z;
   return z;
 }
 
 // The end of the prefix of the kept symbols whose number, or mass, first reaches `target`, from their histogram.  Sets r.cut and r.cidx.
 template <int C, class T, bool HELD>
-__device__ void find_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int rank) {
+__device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int rank) {
   const int tid = threadIdx.x;
-  if (by_mass) {
-    // a bin's symbols have p between 2^(-b kStep) and 2^(-(b + 1) kStep), but for the last bin's: the bins where the end may be
-    if (tid < 32) {
+  // the bins where the end may be: of masses, a bin's symbols have p between 2^(-b kStep) and 2^(-(b + 1) kStep), but for the last bin's
+  if (tid < 32) {
+    int from, to;
+    uint32_t before = 0;
+    if (by_mass) {
       const float goal = static_cast<float>(target);
       const Found<float> first = first_bin<float>(
           0.f, goal * 0.9999f, [&](int b) { return static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b)); });
       const Found<float> last = first_bin<float>(0.f, goal * 1.0001f, [&](int b) {
         return b < kBins - 1 ? static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b + 1)) : 0.f;
       });
-      if (tid == 0) {
-        sh.pick[0] = static_cast<uint32_t>(max(first.bin >= 0 ? first.bin : first.filled, 0));
-        sh.pick[1] = static_cast<uint32_t>(last.bin >= 0 ? last.bin : kBins - 1);
-      }
+      from = max(first.bin >= 0 ? first.bin : first.filled, 0);
+      to = last.bin >= 0 ? last.bin : kBins - 1;
+    } else {
+      from = to = bin_or_last(first_bin<uint32_t>(0u, static_cast<uint32_t>(target), [&](int i) { return sh.all_count[i]; }), &before);
     }
-    clear_bins(sh.mass);
-    __syncthreads();
-    const int from = static_cast<int>(sh.pick[0]), to = static_cast<int>(sh.pick[1]);
+    uint32_t mine = 0;  // how many of the block's symbols are in the bins up to `to`
+    for (int b = tid; b <= to; b += 32) mine += sh.count[b];
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (tid == 0) {
+      sh.pick[0] = static_cast<uint32_t>(from);
+      sh.pick[1] = static_cast<uint32_t>(to);
+      sh.pick[2] = mine;
+      sh.pick_d = static_cast<double>(before);
+    }
+  }
+  clear_bins(sh.mass);
+  __syncthreads();
+  const int from = static_cast<int>(sh.pick[0]), to = static_cast<int>(sh.pick[1]);
+  int bin = from;
+  double above = sh.pick_d;
+  if (HELD && s.kept == nullptr && sh.pick[2] <= kWarps * kWarpKept / 2) set_apart(s, sh, r, to);
+  if (by_mass) {
     float sure = 0.f;
-    for_slice(s, [&](float x, int j) {
+    for_kept(s, [&](float x, int j) {
       if (keeps(r, x, s.first + j)) {
         const int b = bin_of(r, x);
-        if (b <= to) {
-          const float e = (x - r.top) * r.k2;
-          if (b < from)
-            sure += ex2_approx(e);
-          else
-            atomicAdd(&sh.mass[b], mass_units(ex2_approx(e + kStep * static_cast<float>(b)), sh.count[b]));
-        }
+        const float e = (x - r.top) * r.k2;
+        if (b < from)
+          sure += ex2_approx(e);
+        else if (b <= to)
+          atomicAdd(&sh.mass[b], mass_units(ex2_approx(e + kStep * static_cast<float>(b)), sh.count[b]));
       }
     });
     sure = block_sum(sure, sh.red[0], tid >> 5, tid & 31, kWarps);
-    if (tid == 0) sh.out_f[1] = sure;
+    if (tid == 0) sh.out_sure = sure;
     merge_bins<C>(sh, false, true, [](int b) { return ex2_approx(-kStep * static_cast<float>(b)); });
     if (tid < 32) {
-      double above = 0.0, before;
+      double before;
+      above = 0.0;
 #pragma unroll
-      for (int q = 0; q < C; ++q) above += static_cast<double>(C > 1 ? peer_f32(&sh.out_f[1], q) : sh.out_f[1]);
+      for (int q = 0; q < C; ++q) above += static_cast<double>(C > 1 ? peer_f32(&sh.out_sure, q) : sh.out_sure);
       const int b = bin_or_last(first_bin<double>(above, target, [&](int i) { return sh.all_mass[i]; }), &before);
       if (tid == 0) {
         sh.pick[2] = static_cast<uint32_t>(b);
         sh.pick_d = before;
       }
     }
-  } else if (tid < 32) {
-    uint32_t before;
-    const int b = bin_or_last(first_bin<uint32_t>(0u, static_cast<uint32_t>(target), [&](int i) { return sh.all_count[i]; }), &before);
-    if (tid == 0) {
-      sh.pick[2] = static_cast<uint32_t>(b);
-      sh.pick_d = static_cast<double>(before);
-    }
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+    bin = static_cast<int>(sh.pick[2]);
+    above = sh.pick_d;
+  } else {
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
   }
-  if (tid == 0) {
-    sh.listed = 0;
-    sh.pick[0] = 0xffffffffu;
-    sh.pick[1] = 0;
-  }
-  __syncthreads();
-  const int bin = static_cast<int>(sh.pick[2]);
-  const double above = sh.pick_d;
   if (sh.all_count[bin] <= kList) {
-    for_slice(s, [&](float x, int j) {
+    for_kept(s, [&](float x, int j) {
       if (keeps(r, x, s.first + j) && bin_of(r, x) == bin) sh.list[atomicAdd(&sh.listed, 1u)] = place_of(x, s.first + j);
     });
     row_sync<C>();
     if (rank == 0) {
-      const int have = gather_lists<C>(sh);
-      sort_list(sh.list, have);
-      if (by_mass) {
-        float pr[kPart], before, all;
-        sorted_sums(sh, r, have, pr, before, all);
-#pragma unroll
-        for (int i = 0; i < kPart; ++i) {
-          before += pr[i];
-          const int at = tid * kPart + i;
-          if (at < have && above + static_cast<double>(before) >= target) atomicMin(&sh.pick[0], static_cast<uint32_t>(at));
-        }
-        __syncthreads();
-      }
+      const unsigned long long place = end_in_list(sh, r, gather_lists<C>(sh), by_mass, target, above);
       if (tid == 0) {
-        const double at = by_mass ? static_cast<double>(sh.pick[0]) : target - above - 1.0;
-        const unsigned long long place = sh.list[at < have - 1 ? static_cast<int>(fmax(at, 0.0)) : have - 1];
-        sh.out_f[2] = value_of(~static_cast<uint32_t>(place >> 32));
-        sh.out_i[1] = static_cast<uint32_t>(place);
+        sh.out_cut = value_of(~static_cast<uint32_t>(place >> 32));
+        sh.out_cidx = static_cast<int>(static_cast<uint32_t>(place));
       }
     }
     row_sync<C>();
-    r.cut = C > 1 ? peer_f32(&sh.out_f[2], 0) : sh.out_f[2];
-    r.cidx = static_cast<int>(C > 1 ? peer_u32(&sh.out_i[1], 0) : sh.out_i[1]);
-    row_sync<C>();
+    r.cut = C > 1 ? peer_f32(&sh.out_cut, 0) : sh.out_cut;
+    r.cidx = static_cast<int>(C > 1 ? peer_u32(&sh.out_cidx, 0) : sh.out_cidx);
     return;
   }
   // the range of the bin's keys
   uint32_t lo = 0xffffffffu, hi = 0;
-  for_slice(s, [&](float x, int j) {
+  for_kept(s, [&](float x, int j) {
     if (keeps(r, x, s.first + j) && bin_of(r, x) == bin) {
       lo = min(lo, key_of(x));
       hi = max(hi, key_of(x));
     }
   });
+  if (tid == 0) {
+    sh.out_lo = 0xffffffffu;
+    sh.out_hi = 0;
+  }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
-  if ((tid & 31) == 0) {
-    atomicMin(&sh.pick[0], lo);
-    atomicMax(&sh.pick[1], hi);
-  }
   __syncthreads();
-  if (tid == 0) {
-    sh.out_i[2] = sh.pick[0];
-    sh.out_i[3] = sh.pick[1];
+  if ((tid & 31) == 0) {
+    atomicMin(&sh.out_lo, lo);
+    atomicMax(&sh.out_hi, hi);
   }
   row_sync<C>();
   lo = 0xffffffffu;
   hi = 0;
 #pragma unroll
   for (int q = 0; q < C; ++q) {
-    lo = min(lo, C > 1 ? peer_u32(&sh.out_i[2], q) : sh.out_i[2]);
-    hi = max(hi, C > 1 ? peer_u32(&sh.out_i[3], q) : sh.out_i[3]);
+    lo = min(lo, C > 1 ? peer_u32(&sh.out_lo, q) : sh.out_lo);
+    hi = max(hi, C > 1 ? peer_u32(&sh.out_hi, q) : sh.out_hi);
   }
   row_sync<C>();
   select_end<C>(s, sh, r, by_mass, target, lo, hi, above);
@@ -625,6 +798,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
   s.first = rank * p.slice - skip;
   s.size = p.slice;
   s.symbols = p.symbols;
+  s.kept = nullptr;
+  s.kept_count = 0;
   const float* noise = p.noise + row * p.noise_stride;
 
   float temperature = p.temperature != nullptr ? p.temperature[row] : p.temperature0;
@@ -648,10 +823,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) top = max_nan(top, sh.red[0][w]);
   if (C > 1) {
-    if (tid == 0) sh.out_f[0] = top;
+    if (tid == 0) sh.out_top = top;
     cluster_sync_all();
 #pragma unroll
-    for (int q = 0; q < C; ++q) top = max_nan(top, peer_f32(&sh.out_f[0], q));
+    for (int q = 0; q < C; ++q) top = max_nan(top, peer_f32(&sh.out_top, q));
   } else {
     __syncthreads();
   }
@@ -680,7 +855,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
   const bool by_count = top_k > 0 && top_k < p.symbols, by_mass = top_p < 1.f;
   if (by_count && top_k <= kFew) {
     // ---- what is below the k-th largest of the threads' maxima is not among the first k
-    if (mine > -INFINITY) atomicAdd(&sh.count[bin_of(r, mine)], 1u);
+    const int mine_bin = bin_of(r, mine);
+    if (mine_bin < kBins) atomicAdd(&sh.count[mine_bin], 1u);
     __syncthreads();
     if (tid < 32) {
       const Found<uint32_t> f = first_bin<uint32_t>(0u, static_cast<uint32_t>(top_k), [&](int b) { return sh.count[b]; });
@@ -689,7 +865,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
     __syncthreads();
     const int bound = static_cast<int>(sh.pick[0]);
     for_slice(s, [&](float x, int j) {
-      if (x > -INFINITY && bin_of(r, x) <= bound) {
+      if (bin_of(r, x) <= bound) {
         const uint32_t at = atomicAdd(&sh.listed, 1u);
         if (at < kList) sh.list[at] = place_of(x, s.first + j);
       }
@@ -700,8 +876,27 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
     for (int q = 0; q < C; ++q) listed += C > 1 ? peer_u32(&sh.listed, q) : sh.listed;
     if (listed <= kList) {
       if (rank == 0) {
-        const int have = min(gather_lists<C>(sh), top_k);
-        sort_list(sh.list, static_cast<int>(listed));
+        int n = gather_lists<C>(sh);
+        if (n > 128 && n <= kList / 2) {  // the first few of them, or all of the last value's
+          uint32_t lo, hi, first;
+          double above = 0.0;
+          range_of_list(sh, n, lo, hi);
+          first = lo;
+          narrow_list(sh, r, n, false, static_cast<double>(top_k), lo, hi, above);
+          if (tid == 0) sh.pick[2] = 0;
+          __syncthreads();
+          for (int i = tid; i < n; i += kThreads) {
+            const unsigned long long place = sh.list[i];
+            const uint32_t k = static_cast<uint32_t>(place >> 32);
+            if (k >= first && k <= hi) sh.list[kList / 2 + atomicAdd(&sh.pick[2], 1u)] = place;
+          }
+          __syncthreads();
+          n = static_cast<int>(sh.pick[2]);
+          for (int i = tid; i < n; i += kThreads) sh.list[i] = sh.list[kList / 2 + i];
+          __syncthreads();
+        }
+        sort_list(sh.list, n);
+        const int have = min(n, top_k);
         float pr[kPart], before, all;
         sorted_sums(sh, r, have, pr, before, all);
         const float goal = by_mass ? top_p * all : INFINITY;
@@ -739,7 +934,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
   // ---- all that is kept
   float score = -1.f, kept = 0.f;
   int idx = INT32_MAX;
-  for_slice(s, [&](float x, int j) {
+  for_kept(s, [&](float x, int j) {
     const int i = s.first + j;
     const float pr = prob(r, x);
     if (keeps(r, x, i) && pr >= min_p) {
@@ -750,16 +945,16 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
   block_best(score, idx, kept, sh);
   if (C > 1) {
     if (tid == 0) {
-      sh.out_f[2] = score;
-      sh.out_f[3] = kept;
-      sh.out_i[0] = static_cast<uint32_t>(idx);
+      sh.out_score = score;
+      sh.out_sum = kept;
+      sh.out_idx = idx;
     }
     cluster_sync_all();
     if (rank == 0 && tid == 0) {
 #pragma unroll
       for (int q = 1; q < C; ++q) {
-        better(score, idx, peer_f32(&sh.out_f[2], q), static_cast<int>(peer_u32(&sh.out_i[0], q)));
-        kept += peer_f32(&sh.out_f[3], q);
+        better(score, idx, peer_f32(&sh.out_score, q), static_cast<int>(peer_u32(&sh.out_idx, q)));
+        kept += peer_f32(&sh.out_sum, q);
       }
     }
     cluster_sync_all();
