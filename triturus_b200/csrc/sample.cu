@@ -31,8 +31,9 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 256;
-constexpr int kList = 2048;  // symbols that the first block of a row can gather
-constexpr int kWarpKept = 256;  // symbols that a warp can set apart
+constexpr int kList = 1024;  // symbols that the first block of a row can gather
+constexpr int kWarpKept = 256;  // symbols of a slice in shared memory that a warp can set apart
+constexpr int kWarpCopied = 768;  // ... and of one that is not, with their values
 constexpr int kFew = kThreads / 2;  // a small top_k
 
 struct SampleArgs {
@@ -51,21 +52,21 @@ struct SampleArgs {
   int top_k0;
 };
 
-struct Shared {
+struct alignas(16) Shared {
   unsigned long long list[kList];
   double all_mass[kBins];
   double pick_d;
   uint32_t count[kBins];      // the block's
   uint32_t mass[kBins];       // the block's, as multiples of 2^-clz(count)
   uint32_t all_count[kBins];  // the cluster's
-  uint16_t kept[kWarps][kWarpKept];
+  uint32_t fine_count[kBins];
   unsigned long long few[33];
   float red[2][kWarps];
   int red_i[2][kWarps];
   // read by the other blocks, each written once or with a row_sync between
   float out_top, out_z, out_sure, out_cut, out_score, out_sum;
   int out_cidx, out_idx;
-  uint32_t out_lo, out_hi;
+  uint32_t out_lo, out_hi, out_units;
   uint32_t pick[4];
   uint32_t listed;
 };
@@ -138,8 +139,11 @@ struct Slice {
   const T* row;
   float* held;
   int first, size, symbols;
-  const uint16_t* kept;  // what the warp has set apart, or nullptr
-  int kept_count;
+  bool apart;            // the warp has set apart what can still be kept:
+  int kept_count;        // so many
+  uint16_t* kept;        // HELD: their elements' numbers
+  float* kept_x;         // else their values
+  int* kept_j;           // and numbers
   __device__ __forceinline__ float at(int j) const {
     if (HELD) return held[j];
     const int i = first + j;
@@ -174,30 +178,49 @@ __device__ __forceinline__ float load_slice(const Slice<T, HELD>& s) {
   return top;
 }
 
+// The N elements from j on, of memory where the slice is not held.
+template <class T, int N>
+__device__ __forceinline__ void load_elements(const Slice<T, false>& s, int j, float (&v)[N]) {
+  const int i = s.first + j;
+  if (i >= 0 && i + N <= s.symbols) {
+    const Pack<T, 16> p = *reinterpret_cast<const Pack<T, 16>*>(s.row + i);
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = fminf(to_float(p.v[e]), FLT_MAX);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = s.at(j + e);
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ void load_elements(const Slice<T, true>& s, int j, float (&v)[N]) {
+  const float4 p = *reinterpret_cast<const float4*>(s.held + j);
+  v[0] = p.x;
+  v[1] = p.y;
+  v[2] = p.z;
+  v[3] = p.w;
+}
+template <class T, bool HELD>
+constexpr int kRun = HELD ? 4 : Pack<T, 16>::N;  // elements of one load
+
 // f(x, j) for the thread's elements of the slice.
 template <class T, bool HELD, class F>
 __device__ __forceinline__ void for_slice(const Slice<T, HELD>& s, F f) {
-  if (HELD) {
-#pragma unroll 2
-    for (int j = static_cast<int>(threadIdx.x) * 4; j < s.size; j += kThreads * 4) {
-      const float4 v = *reinterpret_cast<const float4*>(s.held + j);
-      f(v.x, j);
-      f(v.y, j + 1);
-      f(v.z, j + 2);
-      f(v.w, j + 3);
-    }
-  } else {
-    for (int j = threadIdx.x; j < s.size; j += kThreads) f(s.at(j), j);
+  constexpr int N = kRun<T, HELD>;
+#pragma unroll(HELD ? 2 : 16 / N)
+  for (int j = static_cast<int>(threadIdx.x) * N; j < s.size; j += kThreads * N) {
+    float v[N];
+    load_elements(s, j, v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f(v[e], j + e);
   }
 }
-
 // ... or for all of the thread's that can still be kept, where those were set apart.
 template <class T, bool HELD, class F>
 __device__ __forceinline__ void for_kept(const Slice<T, HELD>& s, F f) {
-  if (HELD && s.kept != nullptr) {
+  if (s.apart) {
     for (int i = threadIdx.x & 31; i < s.kept_count; i += 32) {
-      const int j = s.kept[i];
-      f(s.held[j], j);
+      const int j = HELD ? s.kept[i] : s.kept_j[i];
+      f(HELD ? s.held[j] : s.kept_x[i], j);
     }
   } else {
     for_slice(s, f);
@@ -206,34 +229,52 @@ __device__ __forceinline__ void for_kept(const Slice<T, HELD>& s, F f) {
 
 // Sets apart the symbols of the bins up to `last`, each warp its own.  What follows goes over some percent of the slice, and its lanes have work.
 template <class T, bool HELD>
-__device__ __forceinline__ void set_apart(Slice<T, HELD>& s, Shared& sh, const Row& r, int last) {
+__device__ __forceinline__ void set_apart(Slice<T, HELD>& s, const Row& r, int last) {
+  constexpr int N = kRun<T, HELD>;
+  constexpr int kMost = HELD ? kWarpKept : kWarpCopied;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float limit = last < kBins - 1 ? static_cast<float>(last + 1) : FLT_MAX;
-  uint16_t* kept = sh.kept[warp];
   int n = 0;
-  for (int j0 = warp * 128; j0 < s.size; j0 += kThreads * 4) {
-    const int j = j0 + lane * 4;
-    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    if (j < s.size) v = *reinterpret_cast<const float4*>(s.held + j);
-    const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll(HELD ? 1 : 16 / N)
+  for (int j0 = warp * (32 * N); j0 < s.size; j0 += kThreads * N) {
+    const int j = j0 + lane * N;
+    float v[N];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool in = bin_place(r, x[e]) < limit;
+    for (int e = 0; e < N; ++e) v[e] = -INFINITY;
+    if (j < s.size) load_elements(s, j, v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const bool in = bin_place(r, v[e]) < limit;
       const unsigned who = __ballot_sync(0xffffffffu, in);
       const int at = n + __popc(who & ((1u << lane) - 1u));
-      if (in && at < kWarpKept) kept[at] = static_cast<uint16_t>(j + e);
+      if (in && at < kMost) {
+        if (HELD) {
+          s.kept[at] = static_cast<uint16_t>(j + e);
+        } else {
+          s.kept_x[at] = v[e];
+          s.kept_j[at] = j + e;
+        }
+      }
       n += __popc(who);
     }
   }
   __syncwarp();
-  if (n <= kWarpKept) {  // (else the warp goes over all of its part: its lanes' elements of the slice, as before)
-    s.kept = kept;
+  if (n <= kMost) {  // (else the warp goes over all of its part: its lanes' elements of the slice, as before)
+    s.apart = true;
     s.kept_count = n;
   }
 }
 
 __device__ __forceinline__ void clear_bins(uint32_t* bins) {
   for (int b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
+}
+
+// A mass is counted in units of 2^-clz(count) of the p at the upper end of its bin: the count's bits and the mass's make 32, no overflow.
+__device__ __forceinline__ uint32_t mass_units(float share, uint32_t count) {
+  return __float2uint_rn(fminf(share, 1.f) * __int_as_float((127 + min(__clz(static_cast<int>(count)), 31)) << 23));
+}
+__device__ __forceinline__ double unit_of(uint32_t count) {
+  return __hiloint2double((1023 - min(__clz(static_cast<int>(count)), 31)) << 20, 0);
 }
 
 // The cluster's counts (and masses, each block's in units of its own) from the blocks' ones.  `upper(b)`: the p that bin b's masses are
@@ -248,7 +289,7 @@ __device__ __forceinline__ void merge_bins(Shared& sh, bool counts, bool masses,
     for (int r = 0; r < C; ++r) {
       const uint32_t c = C > 1 ? peer_u32(&sh.count[b], r) : sh.count[b];
       n += c;
-      if (masses && c != 0) m += ldexp(static_cast<double>(C > 1 ? peer_u32(&sh.mass[b], r) : sh.mass[b]), -__clz(static_cast<int>(c)));
+      if (masses) m += static_cast<double>(C > 1 ? peer_u32(&sh.mass[b], r) : sh.mass[b]) * unit_of(c);
     }
     if (counts) sh.all_count[b] = n;
     if (masses) sh.all_mass[b] = m > 0.0 ? m * static_cast<double>(upper(b)) : 0.0;
@@ -309,10 +350,6 @@ __device__ __forceinline__ int bin_or_last(const Found<V>& f, V* before) {
   return max(f.bin >= 0 ? f.bin : f.filled, 0);
 }
 
-__device__ __forceinline__ uint32_t mass_units(float share, uint32_t count) {  // (the count's bits and the mass's make 32: no overflow)
-  return static_cast<uint32_t>(ldexpf(fminf(share, 1.f), __clz(static_cast<int>(count))));
-}
-
 // Sorts list[0 ... n) and fills it up to the next power of two.  A list of up to 128 by counting for each what is before it.
 __device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
   if (n <= 128) {
@@ -347,17 +384,24 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
   }
 }
 
-// The first block's list and behind it the others'; their number.
+// The first block's list and behind it the others', each fetched by warps of its own; their number.
 template <int C>
 __device__ __forceinline__ int gather_lists(Shared& sh) {
-  int have = static_cast<int>(sh.listed);
-  for (int q = 1; q < C; ++q) {
-    const int more = static_cast<int>(peer_u32(&sh.listed, q));
-    for (int i = threadIdx.x; i < more; i += kThreads) sh.list[have + i] = peer_u64(&sh.list[i], q);
-    have += more;
+  if (C == 1) return static_cast<int>(sh.listed);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int mine = lane < C ? static_cast<int>(peer_u32(&sh.listed, lane)) : 0;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < C; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
   }
+  constexpr int kEach = kWarps / C;
+  const int q = warp / kEach, more = __shfl_sync(0xffffffffu, mine, q), from = __shfl_sync(0xffffffffu, upto, q) - more;
+  if (q > 0)
+    for (int i = (warp % kEach) * 32 + lane; i < more; i += kEach * 32) sh.list[from + i] = peer_u64(&sh.list[i], q);
   __syncthreads();
-  return have;
+  return __shfl_sync(0xffffffffu, upto, C - 1);
 }
 
 // The sums of p before each of the thread's kPart symbols of the sorted list's first `have`, and of all of them.
@@ -500,7 +544,7 @@ __device__ __forceinline__ uint32_t narrow_list(Shared& sh, const Row& r, int n,
                                 const uint32_t c = sh.count[i];
                                 return !by_mass ? static_cast<double>(c)
                                        : c == 0 ? 0.0
-                                                : ldexp(static_cast<double>(sh.mass[i]), -__clz(static_cast<int>(c))) * static_cast<double>(prob(r, upper(i)));
+                                                : static_cast<double>(sh.mass[i]) * unit_of(c) * static_cast<double>(prob(r, upper(i)));
                               }),
                               &before);
     if (threadIdx.x == 0) {
@@ -627,57 +671,87 @@ __device__ __forceinline__ float histogram(const Slice<T, HELD>& s, Shared& sh, 
   return z;
 }
 
-// The end of the prefix of the kept symbols whose number, or mass, first reaches `target`, from their histogram.  Sets r.cut and r.cidx.
+// The end of the prefix of the kept symbols whose number, or mass, first reaches `target`, from their histogram in bins up to `last_bin`.  Sets r.cut
+// and r.cidx.
 template <int C, class T, bool HELD>
-__device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int rank) {
+__device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int last_bin, int rank) {
   const int tid = threadIdx.x;
   // the bins where the end may be: of masses, a bin's symbols have p between 2^(-b kStep) and 2^(-(b + 1) kStep), but for the last bin's
   if (tid < 32) {
-    int from, to;
-    uint32_t before = 0;
     if (by_mass) {
-      const float goal = static_cast<float>(target);
-      const Found<float> first = first_bin<float>(
-          0.f, goal * 0.9999f, [&](int b) { return static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b)); });
-      const Found<float> last = first_bin<float>(0.f, goal * 1.0001f, [&](int b) {
-        return b < kBins - 1 ? static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b + 1)) : 0.f;
+      const Found<float> first = first_bin<float>(0.f, static_cast<float>(target) * 0.9999f, [&](int b) {
+        return static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b));
       });
-      from = max(first.bin >= 0 ? first.bin : first.filled, 0);
-      to = last.bin >= 0 ? last.bin : kBins - 1;
+      if (tid == 0) sh.pick[0] = static_cast<uint32_t>(max(first.bin >= 0 ? first.bin : first.filled, 0));
     } else {
-      from = to = bin_or_last(first_bin<uint32_t>(0u, static_cast<uint32_t>(target), [&](int i) { return sh.all_count[i]; }), &before);
+      uint32_t before;
+      const int b = bin_or_last(first_bin<uint32_t>(0u, static_cast<uint32_t>(target), [&](int i) { return sh.all_count[i]; }), &before);
+      if (tid == 0) {
+        sh.pick[0] = sh.pick[1] = static_cast<uint32_t>(b);
+        sh.pick_d = static_cast<double>(before);
+      }
     }
-    uint32_t mine = 0;  // how many of the block's symbols are in the bins up to `to`
-    for (int b = tid; b <= to; b += 32) mine += sh.count[b];
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (tid == 0) {
-      sh.pick[0] = static_cast<uint32_t>(from);
-      sh.pick[1] = static_cast<uint32_t>(to);
-      sh.pick[2] = mine;
-      sh.pick_d = static_cast<double>(before);
-    }
+  } else if (tid < 64 && by_mass) {
+    const Found<float> last = first_bin<float>(0.f, static_cast<float>(target) * 1.0001f, [&](int b) {
+      return b < kBins - 1 ? static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b + 1)) : 0.f;
+    });
+    if (tid == 32) sh.pick[1] = static_cast<uint32_t>(last.bin >= 0 ? last.bin : last_bin);
   }
   clear_bins(sh.mass);
+  clear_bins(sh.fine_count);
+  if (tid == 0) sh.listed = 0;
   __syncthreads();
   const int from = static_cast<int>(sh.pick[0]), to = static_cast<int>(sh.pick[1]);
-  int bin = from;
   double above = sh.pick_d;
-  if (HELD && s.kept == nullptr && sh.pick[2] <= kWarps * kWarpKept / 2) set_apart(s, sh, r, to);
+  // (in the bins from ... to that are left, a step as fine as 256 bins allow)
+  const float scale = by_mass ? static_cast<float>(kBins) / static_cast<float>(to + 1 - from) : 1.f;
+  auto fine_of = [&](float x) {
+    const float t = bin_place(r, x);
+    if (!(t < FLT_MAX)) return kNoBin;
+    if (!by_mass) return whole_part(fminf(t, 255.f)) - from;
+    if (t < static_cast<float>(from)) return -1;
+    return t < static_cast<float>(to + 1) || to == kBins - 1 ? whole_part(fminf((t - static_cast<float>(from)) * scale, 255.f)) : kNoBin;
+  };
+  int bin = 0;
+  uint32_t in_bin, mine = 0;  // (mine: how many of the block's symbols are in the bins up to `to`)
+  {
+    for (int b = tid & 31; b <= to; b += 32) mine += sh.count[b];
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (!s.apart && mine <= kWarps * (HELD ? kWarpKept * 3 / 4 : kWarpCopied * 7 / 8)) set_apart(s, r, to);
+  }
   if (by_mass) {
+    const float fine_step = kStep / scale;
     float sure = 0.f;
     for_kept(s, [&](float x, int j) {
       if (keeps(r, x, s.first + j)) {
-        const int b = bin_of(r, x);
+        const int b = fine_of(x);
         const float e = (x - r.top) * r.k2;
-        if (b < from)
+        if (b < 0) {
           sure += ex2_approx(e);
-        else if (b <= to)
-          atomicAdd(&sh.mass[b], mass_units(ex2_approx(e + kStep * static_cast<float>(b)), sh.count[b]));
+        } else if (b < kBins) {
+          atomicAdd(&sh.fine_count[b], 1u);
+          atomicAdd(&sh.mass[b], mass_units(ex2_approx(e + (kStep * static_cast<float>(from) + fine_step * static_cast<float>(b))), mine));
+        }
       }
     });
     sure = block_sum(sure, sh.red[0], tid >> 5, tid & 31, kWarps);
-    if (tid == 0) sh.out_sure = sure;
-    merge_bins<C>(sh, false, true, [](int b) { return ex2_approx(-kStep * static_cast<float>(b)); });
+    if (tid == 0) {
+      sh.out_sure = sure;
+      sh.out_units = mine;
+    }
+    row_sync<C>();
+    for (int b = tid; b < kBins; b += kThreads) {
+      uint32_t n = 0;
+      double m = 0.0;
+#pragma unroll
+      for (int q = 0; q < C; ++q) {
+        n += C > 1 ? peer_u32(&sh.fine_count[b], q) : sh.fine_count[b];
+        m += static_cast<double>(C > 1 ? peer_u32(&sh.mass[b], q) : sh.mass[b]) * unit_of(C > 1 ? peer_u32(&sh.out_units, q) : sh.out_units);
+      }
+      sh.all_count[b] = n;
+      sh.all_mass[b] = m * static_cast<double>(ex2_approx(-(kStep * static_cast<float>(from) + fine_step * static_cast<float>(b))));
+    }
+    __syncthreads();
     if (tid < 32) {
       double before;
       above = 0.0;
@@ -689,17 +763,16 @@ __device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
         sh.pick_d = before;
       }
     }
-    if (tid == 0) sh.listed = 0;
     __syncthreads();
     bin = static_cast<int>(sh.pick[2]);
     above = sh.pick_d;
+    in_bin = sh.all_count[bin];
   } else {
-    if (tid == 0) sh.listed = 0;
-    __syncthreads();
+    in_bin = sh.all_count[from];
   }
-  if (sh.all_count[bin] <= kList) {
+  if (in_bin <= kList) {
     for_kept(s, [&](float x, int j) {
-      if (keeps(r, x, s.first + j) && bin_of(r, x) == bin) sh.list[atomicAdd(&sh.listed, 1u)] = place_of(x, s.first + j);
+      if (keeps(r, x, s.first + j) && fine_of(x) == bin) sh.list[atomicAdd(&sh.listed, 1u)] = place_of(x, s.first + j);
     });
     row_sync<C>();
     if (rank == 0) {
@@ -717,7 +790,7 @@ __device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
   // the range of the bin's keys
   uint32_t lo = 0xffffffffu, hi = 0;
   for_kept(s, [&](float x, int j) {
-    if (keeps(r, x, s.first + j) && bin_of(r, x) == bin) {
+    if (keeps(r, x, s.first + j) && fine_of(x) == bin) {
       lo = min(lo, key_of(x));
       hi = max(hi, key_of(x));
     }
@@ -792,14 +865,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
 
   Slice<T, HELD> s;
   s.row = static_cast<const T*>(p.logits) + row * p.logits_stride;
-  s.held = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
+  s.held = reinterpret_cast<float*>(smem_raw + sizeof(Shared) + kWarps * kWarpKept * sizeof(uint16_t));
   // the row's slices begin on 16-byte boundaries of memory
   const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(s.row) & 15) / sizeof(T));
   s.first = rank * p.slice - skip;
   s.size = p.slice;
   s.symbols = p.symbols;
-  s.kept = nullptr;
+  s.apart = false;
   s.kept_count = 0;
+  s.kept = reinterpret_cast<uint16_t*>(smem_raw + sizeof(Shared)) + warp * kWarpKept;
+  s.kept_x = reinterpret_cast<float*>(smem_raw + sizeof(Shared)) + warp * kWarpCopied;
+  s.kept_j = reinterpret_cast<int*>(smem_raw + sizeof(Shared)) + (kWarps + warp) * kWarpCopied;
   const float* noise = p.noise + row * p.noise_stride;
 
   float temperature = p.temperature != nullptr ? p.temperature[row] : p.temperature0;
@@ -907,7 +983,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
           const int at = tid * kPart + i;
           if (at < have && (before < goal || at == 0) && pr[i] >= min_p) {
             const int symbol = static_cast<int>(static_cast<uint32_t>(sh.list[at]));
-            better(score, idx, pr[i] / noise[symbol], symbol);
+            better(score, idx, __fdividef(pr[i], __ldg(noise + symbol)), symbol);
             kept += pr[i];
           }
           before += pr[i];
@@ -922,26 +998,73 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
   }
   if (by_count) {
     histogram<C>(s, sh, r, kBins - 1, false);
-    find_end<C>(s, sh, r, false, static_cast<double>(top_k), rank);
+    find_end<C>(s, sh, r, false, static_cast<double>(top_k), kBins - 1, rank);
   }
   if (by_mass) {
     // a symbol with p below (1 - top_p) / symbols is behind the end: all such ones together have less than 1 - top_p, the first alone has 1
     const float last = by_count ? 255.f : 16.f * logf(static_cast<float>(p.symbols) / (1.f - fmaxf(top_p, 0.f))) + 1.f;
-    const float z = histogram<C>(s, sh, r, static_cast<int>(fminf(last, 255.f)), true);
-    find_end<C>(s, sh, r, true, static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(z), rank);
+    const int last_bin = static_cast<int>(fminf(last, 255.f));
+    const float z = histogram<C>(s, sh, r, last_bin, true);
+    find_end<C>(s, sh, r, true, static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(z), last_bin, rank);
   }
 
   // ---- all that is kept
   float score = -1.f, kept = 0.f;
   int idx = INT32_MAX;
-  for_kept(s, [&](float x, int j) {
-    const int i = s.first + j;
+  // (the noise is fetched for several at once: its latency is what this takes)
+  auto weigh = [&](float x, int j) {
     const float pr = prob(r, x);
-    if (keeps(r, x, i) && pr >= min_p) {
-      better(score, idx, pr / __ldg(noise + i), i);
+    return keeps(r, x, s.first + j) && pr >= min_p ? pr : -1.f;
+  };
+  auto add = [&](float pr, float q, int j) {
+    if (pr >= 0.f) {
+      better(score, idx, __fdividef(pr, q), s.first + j);
       kept += pr;
     }
-  });
+  };
+  if (s.apart) {
+    for (int i = lane; i < s.kept_count; i += 32 * 4) {
+      float pr[4], q[4];
+      int j[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pr[e] = -1.f;
+        q[e] = 1.f;
+        j[e] = 0;
+        if (i + e * 32 < s.kept_count) {
+          j[e] = HELD ? s.kept[i + e * 32] : s.kept_j[i + e * 32];
+          pr[e] = weigh(HELD ? s.held[j[e]] : s.kept_x[i + e * 32], j[e]);
+        }
+        if (pr[e] >= 0.f) q[e] = __ldg(noise + s.first + j[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add(pr[e], q[e], j[e]);
+    }
+  } else {
+    constexpr int N = kRun<T, HELD>;
+    const float* mine_noise = noise + s.first;
+    const bool four = (reinterpret_cast<uintptr_t>(mine_noise) & 15) == 0;
+#pragma unroll 2
+    for (int j = tid * N; j < s.size; j += kThreads * N) {
+      float x[N], q[N];
+      load_elements(s, j, x);
+      if (four && s.first + j >= 0 && s.first + j + N <= s.symbols) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const float4 f = __ldg(reinterpret_cast<const float4*>(mine_noise + j + e));
+          q[e] = f.x;
+          q[e + 1] = f.y;
+          q[e + 2] = f.z;
+          q[e + 3] = f.w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) q[e] = s.first + j + e >= 0 && s.first + j + e < s.symbols ? __ldg(mine_noise + j + e) : 1.f;
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) add(weigh(x[e], j + e), q[e], j + e);
+    }
+  }
   block_best(score, idx, kept, sh);
   if (C > 1) {
     if (tid == 0) {
@@ -965,16 +1088,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
 // ----------------------------------------------------------------------------- launches
 
 constexpr int kMostHeld = 48 * 1024;  // symbols of a slice that shared memory holds
+constexpr int kMostShared = 227 * 1024;
 
 template <class T, bool HELD, int C>
 int run_sample(const SampleArgs& p, int64_t rows, cudaStream_t stream) {
-  const size_t smem = sizeof(Shared) + (HELD ? static_cast<size_t>(p.slice) * sizeof(float) : 0);
+  static_assert(sizeof(Shared) % 16 == 0, "the slice is read four at a time");
+  const size_t smem =
+      sizeof(Shared) + (HELD ? kWarps * kWarpKept * sizeof(uint16_t) + static_cast<size_t>(p.slice) * sizeof(float) : kWarps * kWarpCopied * 8);
   static std::atomic<bool> set[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TRITURUS_B200_ELAUNCH;
-  if (HELD && !set[dev]) {
-    if (cudaFuncSetAttribute(sample_kernel<T, HELD, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(sizeof(Shared) + kMostHeld * sizeof(float))) != cudaSuccess)
+  if (!set[dev]) {
+    if (cudaFuncSetAttribute(sample_kernel<T, HELD, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess)
       return TRITURUS_B200_ELAUNCH;
     set[dev] = true;
   }
@@ -993,19 +1118,28 @@ int run_sample(const SampleArgs& p, int64_t rows, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, sample_kernel<T, HELD, C>, p) == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
 }
 
+template <class T, bool HELD>
+int run_sample(const SampleArgs& p, int64_t rows, int c, cudaStream_t stream) {
+  switch (c) {
+    case 1: return run_sample<T, HELD, 1>(p, rows, stream);
+    case 2: return run_sample<T, HELD, 2>(p, rows, stream);
+    case 4: return run_sample<T, HELD, 4>(p, rows, stream);
+    default: return run_sample<T, HELD, 8>(p, rows, stream);
+  }
+}
+
+// Blocks to a row: as many as the GPU holds at once (two to an SM, by their registers), if they have 4096 symbols each; more of them where a block's
+// warps could not set enough apart.  A slice is held in shared memory where two such blocks fit an SM or one to an SM is all there is; else it is
+// read again from the L2 cache.
 template <class T>
 int sample_rows(SampleArgs p, int64_t rows, cudaStream_t stream) {
   const int64_t most = static_cast<int64_t>(p.symbols) + 16 / static_cast<int64_t>(sizeof(T));  // (with what lies before a 16-byte boundary)
+  const int64_t sms = device_sms();
   int c = 1;
-  while (c < 8 && (most > c * 16384 || (rows * c * 2 <= device_sms() && most > c * 4096))) c *= 2;
+  while (c < 8 && (most > c * INT64_C(65552) || (rows * c <= sms && most > c * 4096))) c *= 2;
   p.slice = static_cast<int>((((most + c - 1) / c) + 7) / 8 * 8);
-  if (p.slice > kMostHeld) return run_sample<T, false, 8>(p, rows, stream);
-  switch (c) {
-    case 1: return run_sample<T, true, 1>(p, rows, stream);
-    case 2: return run_sample<T, true, 2>(p, rows, stream);
-    case 4: return run_sample<T, true, 4>(p, rows, stream);
-    default: return run_sample<T, true, 8>(p, rows, stream);
-  }
+  const bool held = p.slice <= 16400 || (rows * c <= sms && p.slice <= kMostHeld);
+  return held ? run_sample<T, true>(p, rows, c, stream) : run_sample<T, false>(p, rows, c, stream);
 }
 
 }  // namespace
