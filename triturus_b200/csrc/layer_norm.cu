@@ -3,10 +3,17 @@
 //   mean = sum(x) / D,  rstd = 1 / sqrt(sum((x - mean)^2) / D + eps),  h = (x - mean) rstd,  y = h w + b
 //   with g = dy w:  dx = rstd (g - sum(g) / D - h sum(g h) / D),  dw = sum over rows of dy h,  db = sum over rows of dy
 //
+// Bound by memory: 2 row lengths are moved forwards and 3 backwards.  A block of threads goes from row to row; each thread has the same columns in
+// every row, fetches them some rows ahead into shared memory that only it uses (cp.async: no registers and no barrier for what is
+// under way), and backwards keeps its columns' shares of dw and db in registers until the end.  Rows of up to 512 elements belong to a
+// warp.
+//
 // Everything between the loads and the stores is in 32 bits.  The variance is the sum of squares about the mean and not the
 // difference of two sums: a feature at a high level would cancel its digits.  Nothing here adds atomically: the results
 // of a call are the same each time.
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "../../include/triturus_b200.h"
 #include "packs.cuh"
@@ -27,84 +34,161 @@ struct NormArgs {
   int64_t rows;
   int64_t x_stride, dy_stride;
   int width;
+  int stages;          // rows under way: 1, 2 or 4
   int weight32;        // weight, bias and their gradients are 32-bit (else of x's type)
   float eps;
 };
 
-// Weights or biases of the thread's elements [c0, c0 + N), as floats.
-template <class T, int BYTES>
-__device__ __forceinline__ void load_weights(const void* w, int weight32, int c0, float fill, float (&out)[Pack<T, BYTES>::N]) {
-  constexpr int N = Pack<T, BYTES>::N;
-#pragma unroll
-  for (int e = 0; e < N; ++e) out[e] = fill;
-  if (w == nullptr) return;
-  if (weight32) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) out[e] = __ldg(static_cast<const float*>(w) + c0 + e);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) out[e] = to_float(static_cast<const T*>(w)[c0 + e]);
-  }
+// BYTES from global to shared memory without a register.  (16-bit rows on odd addresses: a plain load.)
+template <int BYTES>
+__device__ __forceinline__ void fetch(void* dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  else if constexpr (BYTES == 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  else
+    *static_cast<uint16_t*>(dst) = *static_cast<const uint16_t*>(src);
+}
+__device__ __forceinline__ void wait_for_row(int stages) {
+  if (stages == 4)
+    cp_async_wait<3>();
+  else if (stages == 2)
+    cp_async_wait<1>();
+  else
+    cp_async_wait<0>();
 }
 
-// A row is `nv` vectors of N elements (BYTES divides the rows' bytes, pitch and base), vector v belongs to thread v % threads.
-// `threads` are those of a row: a warp (WARP, blockDim.y rows to a block) or the block.
-template <class T, int BYTES, int NV, bool WARP>
-__global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs p) {
+// How the elements of a row are dealt out: vectors of N elements, vector v to thread v % TH of the row's group of TH threads, NV to a thread.  What
+// lies behind the row's end is never fetched and stays zero.
+template <class T, int BYTES, int NV, int TH>
+struct Deal {
   using P = Pack<T, BYTES>;
-  constexpr int N = P::N;
-  __shared__ float part[2][32];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, threads = blockDim.x, warps = threads >> 5;
-  const int nv = p.width / N;
-  const float inv = 1.f / static_cast<float>(p.width);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (WARP ? blockDim.y : 1);
-  for (int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y : blockIdx.x; row < p.rows; row += step) {
-    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-    P v[NV];
-    float s = 0.f;
+  static constexpr int N = P::N;
+  int left;  // vectors of the row from the thread's first one on
+  int first_column;
+  __device__ __forceinline__ Deal(int t, int width) : left(width / N - t), first_column(t * N) {}
+  __device__ __forceinline__ bool has(int i) const { return left > i * TH; }
+  __device__ __forceinline__ int column(int i) const { return first_column + i * TH * N; }
+};
+
+// The thread's weights, zeros behind the row's end.
+template <class T, class D, int NV>
+__device__ __forceinline__ void load_weights(const D& d, const void* w, int weight32, float fill, float (&out)[NV][D::N]) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = t + i * threads;
-      if (c < nv) v[i] = *reinterpret_cast<const P*>(x + c * N);
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < D::N; ++e) {
+      out[i][e] = d.has(i) ? fill : 0.f;
+      if (w != nullptr && d.has(i))
+        out[i][e] = weight32 ? __ldg(static_cast<const float*>(w) + d.column(i) + e) : to_float(static_cast<const T*>(w)[d.column(i) + e]);
     }
+}
+
+// The sums over a group of TH threads of K values, in each of them.  A group of warps meets at a barrier of its own; two calls in a row use different
+// `part`.
+template <int TH, int K, int WARPS>
+__device__ __forceinline__ void group_sums(float (&v)[K], float (*part)[WARPS], int group) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+  if constexpr (TH > 32) {
+    constexpr int kWarps = TH / 32;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) part[k][threadIdx.x >> 5] = v[k];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TH) : "memory");
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float* mine = part[k] + group * kWarps;
+      if constexpr (kWarps <= 4) {
+        v[k] = mine[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) v[k] += mine[w];
+      } else {
+        v[k] = warp_sum(lane < kWarps ? mine[lane] : 0.f);
+      }
+    }
+  }
+}
+template <int TH, int WARPS>
+__device__ __forceinline__ float group_sum(float v, float (*part)[WARPS], int group) {
+  float one[1] = {v};
+  group_sums<TH>(one, part, group);
+  return one[0];
+}
+
+template <class T, int BYTES, int NV, int TH, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, BLOCK >= 512 ? 1 : 768 / BLOCK) norm_forward_kernel(const NormArgs p) {
+  using D = Deal<T, BYTES, NV, TH>;
+  using P = typename D::P;
+  constexpr int kGroups = BLOCK / TH;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float part[2][BLOCK / 32];
+  const int group = threadIdx.x / TH, t = threadIdx.x % TH;
+  const D d(t, p.width);
+  P* const ring = reinterpret_cast<P*>(smem) + threadIdx.x;
+  const float inv = 1.f / static_cast<float>(p.width);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + group, step = static_cast<int64_t>(gridDim.x) * kGroups;
+  auto ask = [&](int64_t row, int stage) {
+    if (row < p.rows) {
+      const T* x = static_cast<const T*>(p.x) + row * p.x_stride + d.first_column;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (d.has(i)) fetch<BYTES>(&ring[(stage * NV + i) * BLOCK], x + i * TH * D::N);
+    }
+    cp_async_commit();
+  };
+  for (int s = 0; s < p.stages; ++s) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (t + i * threads < nv) {
+      if (!d.has(i)) ring[(s * NV + i) * BLOCK] = P{};
+    ask(first + s * step, s);
+  }
+  float weight[NV][D::N], bias[NV][D::N];
+  load_weights<T>(d, p.weight, p.weight32, 1.f, weight);
+  load_weights<T>(d, p.bias, p.weight32, 0.f, bias);
+  int stage = 0;
+  for (int64_t row = first; row < p.rows; row += step) {
+    wait_for_row(p.stages);
+    float v[NV][D::N], s = 0.f;
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += to_float(v[i].v[e]);
-      }
-    const float mean = (WARP ? warp_sum(s) : block_sum(s, part[0], warp, lane, warps)) * inv;
+    for (int i = 0; i < NV; ++i) {
+      const P x = ring[(stage * NV + i) * BLOCK];
+#pragma unroll
+      for (int e = 0; e < D::N; ++e) s += v[i][e] = to_float(x.v[e]);
+    }
+    const float mean = group_sum<TH>(s, part, group) * inv;
+    ask(row + p.stages * step, stage);  // (the values are in registers: they are part of the sum)
+    stage = stage + 1 == p.stages ? 0 : stage + 1;
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (t + i * threads < nv) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float d = to_float(v[i].v[e]) - mean;
-          q += d * d;
-        }
+      for (int e = 0; e < D::N; ++e) {
+        v[i][e] = d.has(i) ? v[i][e] - mean : 0.f;
+        q = fmaf(v[i][e], v[i][e], q);
       }
-    const float var = (WARP ? warp_sum(q) : block_sum(q, part[1], warp, lane, warps)) * inv;
-    const float rstd = 1.f / sqrtf(var + p.eps);
+    const float rstd = 1.f / sqrtf(fmaf(group_sum<TH>(q, part + 1, group), inv, p.eps));
     if (t == 0) {
       if (p.mean != nullptr) p.mean[row] = mean;
       if (p.rstd != nullptr) p.rstd[row] = rstd;
     }
-    T* y = static_cast<T*>(p.y) + row * p.width;
+    T* y = static_cast<T*>(p.y) + row * p.width + d.first_column;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = t + i * threads;
-      if (c < nv) {
-        float w[N], b[N];
-        load_weights<T, BYTES>(p.weight, p.weight32, c * N, 1.f, w);
-        load_weights<T, BYTES>(p.bias, p.weight32, c * N, 0.f, b);
+    for (int i = 0; i < NV; ++i)
+      if (d.has(i)) {
         P o;
 #pragma unroll
-        for (int e = 0; e < N; ++e) o.v[e] = from_float<T>((to_float(v[i].v[e]) - mean) * rstd * w[e] + b[e]);
-        *reinterpret_cast<P*>(y + c * N) = o;
+        for (int e = 0; e < D::N; ++e) o.v[e] = from_float<T>(fmaf(v[i][e] * rstd, weight[i][e], bias[i][e]));
+        *reinterpret_cast<P*>(y + i * TH * D::N) = o;
       }
-    }
   }
+}
+
+template <class T>
+__device__ __forceinline__ float weight_at(const void* w, int weight32, int c, float fill) {
+  return w == nullptr ? fill : weight32 ? static_cast<const float*>(w)[c] : to_float(static_cast<const T*>(w)[c]);
 }
 
 // Rows that do not fit a block's registers: read three times, from the L2 cache after the first.
@@ -130,91 +214,126 @@ __global__ void __launch_bounds__(1024) norm_forward_long_kernel(const NormArgs 
     }
     T* y = static_cast<T*>(p.y) + row * p.width;
     for (int c = t; c < p.width; c += 1024) {
-      float w[1], b[1];
-      load_weights<T, sizeof(T)>(p.weight, p.weight32, c, 1.f, w);
-      load_weights<T, sizeof(T)>(p.bias, p.weight32, c, 0.f, b);
-      y[c] = from_float<T>((to_float(x[c]) - mean) * rstd * w[0] + b[0]);
+      const float w = weight_at<T>(p.weight, p.weight32, c, 1.f), b = weight_at<T>(p.bias, p.weight32, c, 0.f);
+      y[c] = from_float<T>((to_float(x[c]) - mean) * rstd * w + b);
     }
   }
 }
 
-// dx of a block's rows, and the block's share of dw and db: a thread has the same columns in every row and keeps their sums.
-template <class T, int BYTES, int NV>
-__global__ void __launch_bounds__(1024) norm_backward_kernel(const NormArgs p) {
-  using P = Pack<T, BYTES>;
-  constexpr int N = P::N;
-  __shared__ float part[2][2][32];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, threads = blockDim.x, warps = threads >> 5;
-  const int nv = p.width / N;
+// dx of a block's rows, and the block's share of dw and db.  The block is kBack threads, as many groups as rows fit it.
+constexpr int kBack = 512;
+template <class T, int BYTES, int NV, int TH>
+__global__ void __launch_bounds__(kBack) norm_backward_kernel(const NormArgs p) {
+  using D = Deal<T, BYTES, NV, TH>;
+  using P = typename D::P;
+  constexpr int kGroups = kBack / TH;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float part[2][2][kBack / 32];
+  const int group = threadIdx.x / TH, t = threadIdx.x % TH;
+  const D d(t, p.width);
+  P* const ring = reinterpret_cast<P*>(smem) + threadIdx.x;
   const float inv = 1.f / static_cast<float>(p.width);
-  float w[NV][N], dw[NV][N], db[NV][N];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + group, step = static_cast<int64_t>(gridDim.x) * kGroups;
+  auto ask = [&](int64_t row, int stage) {
+    if (row < p.rows) {
+      const T* x = static_cast<const T*>(p.x) + row * p.x_stride + d.first_column;
+      const T* dy = static_cast<const T*>(p.dy) + row * p.dy_stride + d.first_column;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = t + i * threads;
-    if (c < nv) load_weights<T, BYTES>(p.weight, p.weight32, c * N, 1.f, w[i]);
-#pragma unroll
-    for (int e = 0; e < N; ++e) dw[i][e] = db[i][e] = 0.f;
-  }
-  int odd = 0;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, odd ^= 1) {
-    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-    const T* dy = static_cast<const T*>(p.dy) + row * p.dy_stride;
-    const float mean = p.mean[row], rstd = p.rstd[row];
-    P v[NV], d[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = t + i * threads;
-      if (c < nv) {
-        v[i] = *reinterpret_cast<const P*>(x + c * N);
-        d[i] = *reinterpret_cast<const P*>(dy + c * N);
-      }
+      for (int i = 0; i < NV; ++i)
+        if (d.has(i)) {
+          fetch<BYTES>(&ring[(stage * 2 * NV + i) * kBack], x + i * TH * D::N);
+          fetch<BYTES>(&ring[(stage * 2 * NV + NV + i) * kBack], dy + i * TH * D::N);
+        }
     }
-    float sg = 0.f, sgh = 0.f;
+    cp_async_commit();
+  };
+  for (int s = 0; s < p.stages; ++s) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (t + i * threads < nv) {
+      if (!d.has(i)) ring[(s * 2 * NV + i) * kBack] = ring[(s * 2 * NV + NV + i) * kBack] = P{};
+    ask(first + s * step, s);
+  }
+  float weight[NV][D::N];
+  load_weights<T>(d, p.weight, p.weight32, 1.f, weight);
+  float mean = 0.f, rstd = 0.f;
+  if (first < p.rows) {
+    mean = p.mean[first];
+    rstd = p.rstd[first];
+  }
+  float dw[NV][D::N], db[NV][D::N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float dd = to_float(d[i].v[e]), h = (to_float(v[i].v[e]) - mean) * rstd, g = dd * w[i][e];
-          sg += g;
-          sgh += g * h;
-          dw[i][e] += dd * h;
-          db[i][e] += dd;
-        }
-      }
-    sg = warp_sum(sg);
-    sgh = warp_sum(sgh);
-    if (lane == 0) {
-      part[odd][0][warp] = sg;
-      part[odd][1][warp] = sgh;
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < D::N; ++e) dw[i][e] = db[i][e] = 0.f;
+  int stage = 0, odd = 0;
+  for (int64_t row = first; row < p.rows; row += step, odd ^= 1) {
+    float next_mean = 0.f, next_rstd = 0.f;
+    if (row + step < p.rows) {
+      next_mean = p.mean[row + step];
+      next_rstd = p.rstd[row + step];
     }
-    __syncthreads();
-    const float mg = warp_sum(lane < warps ? part[odd][0][lane] : 0.f) * inv;
-    const float mgh = warp_sum(lane < warps ? part[odd][1][lane] : 0.f) * inv;
-    T* dx = static_cast<T*>(p.y) + row * p.width;
+    wait_for_row(p.stages);
+    float sums_of[2] = {0.f, 0.f};  // of g and g h
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = t + i * threads;
-      if (c < nv) {
-        P o;
+      const P x = ring[(stage * 2 * NV + i) * kBack], dy = ring[(stage * 2 * NV + NV + i) * kBack];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float h = (to_float(v[i].v[e]) - mean) * rstd;
-          o.v[e] = from_float<T>(rstd * (to_float(d[i].v[e]) * w[i][e] - mg - h * mgh));
-        }
-        *reinterpret_cast<P*>(dx + c * N) = o;
+      for (int e = 0; e < D::N; ++e) {
+        const float dd = to_float(dy.v[e]), h = (to_float(x.v[e]) - mean) * rstd, g = dd * weight[i][e];
+        sums_of[0] += g;
+        sums_of[1] = fmaf(g, h, sums_of[1]);
+        dw[i][e] = fmaf(dd, h, dw[i][e]);
+        db[i][e] += dd;
       }
     }
+    group_sums<TH>(sums_of, part[odd], group);
+    const float mg = sums_of[0] * inv, mgh = sums_of[1] * inv;
+    T* dx = static_cast<T*>(p.y) + row * p.width + d.first_column;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const P x = ring[(stage * 2 * NV + i) * kBack], dy = ring[(stage * 2 * NV + NV + i) * kBack];
+      P o;
+#pragma unroll
+      for (int e = 0; e < D::N; ++e) {
+        const float h = (to_float(x.v[e]) - mean) * rstd;
+        o.v[e] = from_float<T>(rstd * fmaf(-h, mgh, fmaf(to_float(dy.v[e]), weight[i][e], -mg)));
+      }
+      if (d.has(i)) *reinterpret_cast<P*>(dx + i * TH * D::N) = o;
+    }
+    ask(row + p.stages * step, stage);  // (what the stage held went into the stores)
+    stage = stage + 1 == p.stages ? 0 : stage + 1;
+    mean = next_mean;
+    rstd = next_rstd;
   }
   float* mine = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.width;
+  if constexpr (kGroups == 1) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = t + i * threads;
-    if (c < nv) {
+    for (int i = 0; i < NV; ++i)
+      if (d.has(i)) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        mine[c * N + e] = dw[i][e];
-        mine[p.width + c * N + e] = db[i][e];
+        for (int e = 0; e < D::N; ++e) {
+          mine[d.column(i) + e] = dw[i][e];
+          mine[p.width + d.column(i) + e] = db[i][e];
+        }
+      }
+  } else {  // the groups' shares, added in their order
+    cp_async_wait<0>();
+    float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (d.has(i)) {
+#pragma unroll
+          for (int e = 0; e < D::N; ++e) sums[group * p.width + d.column(i) + e] = which == 0 ? dw[i][e] : db[i][e];
+        }
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.width; c += kBack) {
+        float v = sums[c];
+#pragma unroll
+        for (int g = 1; g < kGroups; ++g) v += sums[g * p.width + c];
+        mine[which * p.width + c] = v;
       }
     }
   }
@@ -232,9 +351,8 @@ __global__ void __launch_bounds__(1024) norm_backward_long_kernel(const NormArgs
     const float mean = p.mean[row], rstd = p.rstd[row];
     float sg = 0.f, sgh = 0.f;
     for (int c = t; c < p.width; c += 1024) {
-      float w[1];
-      load_weights<T, sizeof(T)>(p.weight, p.weight32, c, 1.f, w);
-      const float g = to_float(dy[c]) * w[0];
+      const float w = weight_at<T>(p.weight, p.weight32, c, 1.f);
+      const float g = to_float(dy[c]) * w;
       sg += g;
       sgh += g * ((to_float(x[c]) - mean) * rstd);
     }
@@ -242,10 +360,9 @@ __global__ void __launch_bounds__(1024) norm_backward_long_kernel(const NormArgs
     const float mgh = block_sum(sgh, part[1], warp, lane, 32) * inv;
     T* dx = static_cast<T*>(p.y) + row * p.width;
     for (int c = t; c < p.width; c += 1024) {
-      float w[1];
-      load_weights<T, sizeof(T)>(p.weight, p.weight32, c, 1.f, w);
+      const float w = weight_at<T>(p.weight, p.weight32, c, 1.f);
       const float h = (to_float(x[c]) - mean) * rstd;
-      dx[c] = from_float<T>(rstd * (to_float(dy[c]) * w[0] - mg - h * mgh));
+      dx[c] = from_float<T>(rstd * (to_float(dy[c]) * w - mg - h * mgh));
     }
   }
 }
@@ -266,24 +383,26 @@ __global__ void __launch_bounds__(256) norm_backward_columns_kernel(const NormAr
   mine[p.width + c] = db;
 }
 
-// dw and db from the blocks' shares [blocks, 2, width]: 32 columns to a block, its warps add every 8th share.
+// dw and db from the blocks' shares [blocks, 2, width]: 32 columns to a block, its warps add every 16th share.
 template <class W>
-__global__ void __launch_bounds__(256) norm_reduce_kernel(const float* __restrict__ part, W* __restrict__ dweight, W* __restrict__ dbias,
+__global__ void __launch_bounds__(512) norm_reduce_kernel(const float* __restrict__ part, W* __restrict__ dweight, W* __restrict__ dbias,
                                                           int blocks, int width) {
-  __shared__ float sums[8][33];
+  __shared__ float sums[16][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   W* out = blockIdx.y == 0 ? dweight : dbias;
   if (out == nullptr) return;
   pdl_wait();
   float s = 0.f;
-  if (c < width)
-    for (int b = warp; b < blocks; b += 8) s += part[(static_cast<int64_t>(b) * 2 + blockIdx.y) * width + c];
+  if (c < width) {
+#pragma unroll 4
+    for (int b = warp; b < blocks; b += 16) s += part[(static_cast<int64_t>(b) * 2 + blockIdx.y) * width + c];
+  }
   sums[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < width) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += sums[i][lane];
+    for (int i = 1; i < 16; ++i) s += sums[i][lane];
     out[c] = from_float<W>(s);
   }
 }
@@ -301,116 +420,136 @@ int vector_bytes(const void* base, int64_t stride, int64_t rows, int64_t width, 
   return size;
 }
 
-struct RowShape {
-  int threads;  // of a row
-  int nv;       // vectors to a thread; 0: the row does not fit
-};
-// The fewest threads that hold a row with at most `most` vectors each.
-RowShape row_shape(int64_t vectors, int most, int least_threads) {
-  for (int threads = least_threads; threads <= 1024; threads *= 2) {
-    if (vectors <= static_cast<int64_t>(threads) * most) return {threads, static_cast<int>((vectors + threads - 1) / threads)};
+constexpr int kMostShared = 220 * 1024;
+constexpr int kEach = 16;  // elements of a thread, twice that in the longest rows
+
+// The blocks of a kernel that an SM holds, 0 where something failed.
+template <class Kern>
+int blocks_of_sm(Kern kern, std::atomic<int> (&known)[64], int threads, size_t smem) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n <= 0) return 0;
+    known[dev].store(n, std::memory_order_relaxed);
   }
-  return {0, 0};
+  return n;
 }
 
-template <class T, int BYTES, int NV>
-void run_forward(const NormArgs& p, int threads, cudaStream_t stream) {
-  const int sms = device_sms();
-  if (threads == 32) {
-    const int64_t blocks = std::min<int64_t>((p.rows + 7) / 8, static_cast<int64_t>(sms) * 8);
-    norm_forward_kernel<T, BYTES, NV, true><<<static_cast<unsigned>(blocks), dim3(32, 8), 0, stream>>>(p);
-  } else {
-    const int64_t blocks = std::min<int64_t>(p.rows, static_cast<int64_t>(sms) * (2048 / threads));
-    norm_forward_kernel<T, BYTES, NV, false><<<static_cast<unsigned>(blocks), threads, 0, stream>>>(p);
-  }
+// Rows under way, of what shared memory holds.
+constexpr int stages_for(size_t row_bytes, int bytes) {
+  return bytes < 4 ? 1 : 4 * row_bytes <= kMostShared ? 4 : 2 * row_bytes <= kMostShared ? 2 : 1;
 }
 
-template <class T, int BYTES>
-bool forward_by_size(const NormArgs& p, cudaStream_t stream) {
-  constexpr int N = Pack<T, BYTES>::N;
-  constexpr int MOST = BYTES == 16 ? 4 : 16;
-  const RowShape s = row_shape(p.width / N, MOST, 32);
-  if (s.nv == 0) return false;
-  if (s.nv <= MOST / 4)
-    run_forward<T, BYTES, MOST / 4>(p, s.threads, stream);
-  else if (s.nv <= MOST / 2)
-    run_forward<T, BYTES, MOST / 2>(p, s.threads, stream);
-  else
-    run_forward<T, BYTES, MOST>(p, s.threads, stream);
-  return true;
+template <class T, int BYTES, int NV, int TH>
+int run_forward(NormArgs p, cudaStream_t stream) {
+  constexpr int BLOCK = TH < 128 ? 128 : TH, kGroups = BLOCK / TH;
+  constexpr size_t row_bytes = static_cast<size_t>(BLOCK) * NV * BYTES;
+  constexpr int stages = stages_for(row_bytes, BYTES);
+  static std::atomic<int> known[64];
+  const auto kern = norm_forward_kernel<T, BYTES, NV, TH, BLOCK>;
+  const int fit = blocks_of_sm(kern, known, BLOCK, stages * row_bytes);
+  if (fit == 0) return TRITURUS_B200_ELAUNCH;
+  p.stages = stages;
+  const int64_t blocks = std::min<int64_t>((p.rows + kGroups - 1) / kGroups, static_cast<int64_t>(device_sms()) * fit);
+  kern<<<static_cast<unsigned>(blocks), BLOCK, stages * row_bytes, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+}
+
+// Blocks of the backward pass: each has a share of dw and db to write and to be added.
+int most_shares(int64_t rows) { return static_cast<int>(std::min<int64_t>(rows, device_sms())); }
+
+template <class T, int BYTES, int NV, int TH>
+int run_backward(NormArgs p, int* blocks, cudaStream_t stream) {
+  constexpr int kGroups = kBack / TH;
+  constexpr size_t row_bytes = static_cast<size_t>(kBack) * NV * BYTES * 2;
+  constexpr int stages = stages_for(row_bytes, BYTES);
+  constexpr size_t smem = std::max<size_t>(stages * row_bytes, kGroups > 1 ? static_cast<size_t>(kBack) * NV * BYTES / sizeof(T) * sizeof(float) : 0);
+  static std::atomic<int> known[64];
+  const auto kern = norm_backward_kernel<T, BYTES, NV, TH>;
+  if (blocks_of_sm(kern, known, kBack, smem) == 0) return TRITURUS_B200_ELAUNCH;
+  p.stages = stages;
+  *blocks = static_cast<int>(std::min<int64_t>((p.rows + kGroups - 1) / kGroups, device_sms()));
+  kern<<<static_cast<unsigned>(*blocks), kBack, smem, stream>>>(p);
+  return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+}
+
+// run(NV, TH) as constants: the fewest threads that hold a row with kEach elements each.
+template <class T, int BYTES, class F>
+int by_width(int64_t width, F run) {
+  constexpr int NV = kEach / Pack<T, BYTES>::N;
+  using C = std::integral_constant<int, NV>;
+  if (width <= 32 * kEach) return run(C(), std::integral_constant<int, 32>());
+  if (width <= 64 * kEach) return run(C(), std::integral_constant<int, 64>());
+  if (width <= 128 * kEach) return run(C(), std::integral_constant<int, 128>());
+  if (width <= 256 * kEach) return run(C(), std::integral_constant<int, 256>());
+  if (width <= 512 * kEach) return run(C(), std::integral_constant<int, 512>());
+  return run(std::integral_constant<int, 2 * NV>(), std::integral_constant<int, 512>());
+}
+constexpr int64_t kLongest = 1024 * kEach;  // rows that by_width takes
+
+// fn(bytes) as a constant.
+template <class T, class F>
+int by_bytes(int bytes, F fn) {
+  if (bytes == 16) return fn(std::integral_constant<int, 16>());
+  if (bytes == 4) return fn(std::integral_constant<int, 4>());
+  return fn(std::integral_constant<int, static_cast<int>(sizeof(T))>());
 }
 
 template <class T>
 int forward(const NormArgs& p, cudaStream_t stream) {
   constexpr int SIZE = static_cast<int>(sizeof(T));
+  if (p.width > kLongest) {
+    norm_forward_long_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(p.rows, device_sms() * 2)), 1024, 0, stream>>>(p);
+    return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+  }
   const int bytes = std::min(vector_bytes(p.x, p.x_stride, p.rows, p.width, SIZE), vector_bytes(p.y, p.width, p.rows, p.width, SIZE));
-  const bool done = bytes == 16  ? forward_by_size<T, 16>(p, stream)
-                    : bytes == 4 ? forward_by_size<T, 4>(p, stream)
-                                 : forward_by_size<T, SIZE>(p, stream);
-  if (!done) norm_forward_long_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(p.rows, device_sms() * 2)), 1024, 0, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
-}
-
-struct BackwardPlan {
-  int bytes, threads, nv;  // nv == 0: the kernels for long rows
-  int blocks;              // shares of dw and db
-};
-
-BackwardPlan plan_backward(int64_t rows, int64_t width, int size, int bytes) {
-  BackwardPlan b = {bytes, 0, 0, 0};
-  const int n = bytes / size;
-  const RowShape s = row_shape(width / n, 16 / n, 128);
-  b.threads = s.threads;
-  b.nv = s.nv;
-  if (s.nv == 0)
-    b.blocks = static_cast<int>(std::min<int64_t>(rows, 64));
-  else
-    b.blocks = static_cast<int>(std::min<int64_t>(rows, device_sms() * std::max(1, std::min(4, 1024 / s.threads))));
-  return b;
-}
-
-template <class T, int BYTES>
-void run_backward(const NormArgs& p, const BackwardPlan& b, cudaStream_t stream) {
-  constexpr int N = Pack<T, BYTES>::N;
-  constexpr int MOST = 16 / N;  // 16 elements to a thread at most
-  if (b.nv <= MOST / 2)
-    norm_backward_kernel<T, BYTES, MOST / 2><<<b.blocks, b.threads, 0, stream>>>(p);
-  else
-    norm_backward_kernel<T, BYTES, MOST><<<b.blocks, b.threads, 0, stream>>>(p);
+  return by_bytes<T>(bytes, [&](auto b) {
+    return by_width<T, b()>(p.width, [&](auto nv, auto th) { return run_forward<T, b(), nv(), th()>(p, stream); });
+  });
 }
 
 template <class W>
-int run_reduce(const float* part, void* dweight, void* dbias, int blocks, int width, cudaStream_t stream) {
+int run_reduce(const NormArgs& p, void* dweight, void* dbias, int blocks, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((width + 31) / 32), 2, 1);
-  cfg.blockDim = dim3(256, 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>((p.width + 31) / 32), 2, 1);
+  cfg.blockDim = dim3(512, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, norm_reduce_kernel<W>, part, static_cast<W*>(dweight), static_cast<W*>(dbias), blocks, width) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, norm_reduce_kernel<W>, p.part, static_cast<W*>(dweight), static_cast<W*>(dbias), blocks, p.width) == cudaSuccess
              ? TRITURUS_B200_OK
              : TRITURUS_B200_ELAUNCH;
 }
 
 template <class T>
-int backward(const NormArgs& p, const BackwardPlan& b, void* dweight, void* dbias, cudaStream_t stream) {
-  if (b.nv == 0) {
+int backward(const NormArgs& p, void* dweight, void* dbias, cudaStream_t stream) {
+  constexpr int SIZE = static_cast<int>(sizeof(T));
+  int blocks = 0, rc;
+  if (p.width > kLongest) {
+    blocks = most_shares(std::min<int64_t>(p.rows, 64));
     norm_backward_long_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(p.rows, device_sms() * 2)), 1024, 0, stream>>>(p);
-    norm_backward_columns_kernel<T><<<dim3(static_cast<unsigned>((p.width + 255) / 256), static_cast<unsigned>(b.blocks)), 256, 0, stream>>>(p);
-  } else if (b.bytes == 16) {
-    run_backward<T, 16>(p, b, stream);
-  } else if (b.bytes == 4) {
-    run_backward<T, 4>(p, b, stream);
+    norm_backward_columns_kernel<T><<<dim3(static_cast<unsigned>((p.width + 255) / 256), static_cast<unsigned>(blocks)), 256, 0, stream>>>(p);
+    rc = cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
   } else {
-    run_backward<T, sizeof(T)>(p, b, stream);
+    const int bytes = std::min({vector_bytes(p.x, p.x_stride, p.rows, p.width, SIZE), vector_bytes(p.dy, p.dy_stride, p.rows, p.width, SIZE),
+                                vector_bytes(p.y, p.width, p.rows, p.width, SIZE)});
+    rc = by_bytes<T>(bytes, [&](auto b) {
+      return by_width<T, b()>(p.width, [&](auto nv, auto th) { return run_backward<T, b(), nv(), th()>(p, &blocks, stream); });
+    });
   }
-  if (cudaGetLastError() != cudaSuccess) return TRITURUS_B200_ELAUNCH;
-  if (dweight == nullptr && dbias == nullptr) return TRITURUS_B200_OK;
-  return p.weight32 ? run_reduce<float>(p.part, dweight, dbias, b.blocks, p.width, stream)
-                    : run_reduce<T>(p.part, dweight, dbias, b.blocks, p.width, stream);
+  if (rc != TRITURUS_B200_OK || (dweight == nullptr && dbias == nullptr)) return rc;
+  return p.weight32 ? run_reduce<float>(p, dweight, dbias, blocks, stream) : run_reduce<T>(p, dweight, dbias, blocks, stream);
+}
+
+// fn(T()) for the type of the elements.
+template <class F>
+int by_type(int type, F fn) {
+  return type == TRITURUS_B200_TYPE_F32 ? fn(0.f) : type == TRITURUS_B200_TYPE_BF16 ? fn(__nv_bfloat16()) : fn(__half());
 }
 
 bool norm_sizes_ok(int64_t rows, int64_t width, int type, int weight_type) {
@@ -445,18 +584,12 @@ int triturus_b200_layer_norm(const void* x, const void* weight, const void* bias
   p.width = static_cast<int>(width);
   p.weight32 = weight_type == TRITURUS_B200_TYPE_F32;
   p.eps = eps;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return type == TRITURUS_B200_TYPE_F32    ? forward<float>(p, st)
-         : type == TRITURUS_B200_TYPE_BF16 ? forward<__nv_bfloat16>(p, st)
-                                           : forward<__half>(p, st);
+  return by_type(type, [&](auto t) { return forward<decltype(t)>(p, static_cast<cudaStream_t>(stream)); });
 }
 
 size_t triturus_b200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width, int type) {
   if (!norm_sizes_ok(rows, width, type, type)) return 0;
-  int blocks = 0;  // (the shares are fewer or more by the alignment of the operands: room for either)
-  for (int bytes : {16, 4, size_of(type)})
-    if (width * size_of(type) % bytes == 0) blocks = std::max(blocks, plan_backward(rows, width, size_of(type), bytes).blocks);
-  return static_cast<size_t>(blocks) * 2 * static_cast<size_t>(width) * sizeof(float);
+  return static_cast<size_t>(most_shares(rows)) * 2 * static_cast<size_t>(width) * sizeof(float);
 }
 
 int triturus_b200_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
@@ -489,12 +622,7 @@ int triturus_b200_layer_norm_backward(const void* dy, const void* x, const void*
   p.dy_stride = dy_stride;
   p.width = static_cast<int>(width);
   p.weight32 = weight_type == TRITURUS_B200_TYPE_F32;
-  const int bytes = std::min({vector_bytes(x, x_stride, rows, width, size), vector_bytes(dy, dy_stride, rows, width, size),
-                              vector_bytes(dx, width, rows, width, size)});
-  const BackwardPlan b = plan_backward(rows, width, size, bytes);
-  return type == TRITURUS_B200_TYPE_F32    ? backward<float>(p, b, dweight, dbias, st)
-         : type == TRITURUS_B200_TYPE_BF16 ? backward<__nv_bfloat16>(p, b, dweight, dbias, st)
-                                           : backward<__half>(p, b, dweight, dbias, st);
+  return by_type(type, [&](auto t) { return backward<decltype(t)>(p, dweight, dbias, st); });
 }
 
 }  // extern "C"
