@@ -2,10 +2,13 @@
 //
 //   n = sqrt(sum x^2) or max |x| over all elements of all tensors;  c = min(1, limit / (n + 1e-6));  x <- c x
 //
-// The tensors are cut into chunks of kChunk bytes that begin on 16-byte boundaries of memory (the first of a tensor may begin with
-// a partial vector), and the blocks take the chunks in turn.  First launch: each block's sum of squares, in 64 bits.  Second launch: every
-// block adds those sums in the same order, so that all have the same n, and scales its chunks; it goes through them backwards, because
-// what the first launch read last is still in the L2 cache.  Where c is 1 nothing is written.
+// The tensors are cut into chunks of kChunk bytes that begin on 16-byte boundaries of memory (the first of a tensor may begin with a partial
+// vector), and each block has a run of them.  Bound by memory: all is read once for the norm and, where the norm is above the limit, read again
+// and written.  First launch: each block's sum of squares, in 64 bits.  Second launch: every block adds those sums in the same order, so
+// that all have the same n, and scales its chunks, the last one first: what the first launch read last is still in the L2 cache.  Where c is
+// 1 nothing is written.
+//
+// A few small tensors are one launch: a cluster of blocks that keep their chunks in registers from the sum to the product.
 #include <algorithm>
 #include <cstring>
 
@@ -42,13 +45,18 @@ struct ClipArgs {
 };
 
 struct Chunk {
-  uint8_t* base;     // on a 16-byte boundary: the chunk's first byte, if the tensor began there
-  int begin, end;    // the tensor's bytes of the chunk
+  uint8_t* base;   // on a 16-byte boundary: the chunk's first byte, if the tensor began there
+  int begin, end;  // the tensor's bytes of the chunk
   int type;
 };
 
+// A place in the list: a chunk and its tensor.
+struct Cursor {
+  uint32_t chunk;
+  int tensor;
+};
 template <int MOST>
-__device__ __forceinline__ Chunk find_chunk(const TensorList<MOST>& l, uint32_t c) {
+__device__ __forceinline__ Cursor cursor_at(const TensorList<MOST>& l, uint32_t c) {
   int lo = 0, hi = l.count;  // the last tensor whose first chunk is not behind c
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -57,97 +65,128 @@ __device__ __forceinline__ Chunk find_chunk(const TensorList<MOST>& l, uint32_t 
     else
       hi = mid;
   }
-  const uintptr_t at = reinterpret_cast<uintptr_t>(l.data[lo]);
-  const int skip = static_cast<int>(at & 15);
-  const int64_t off = static_cast<int64_t>(c - l.first[lo]) * kChunk;
-  const int64_t left = skip + l.bytes[lo] - off;
+  return {c, lo};
+}
+template <int MOST>
+__device__ __forceinline__ Chunk chunk_at(const TensorList<MOST>& l, const Cursor& at) {
+  const uintptr_t data = reinterpret_cast<uintptr_t>(l.data[at.tensor]);
+  const int skip = static_cast<int>(data & 15);
+  const int64_t off = static_cast<int64_t>(at.chunk - l.first[at.tensor]) * kChunk;
+  const int64_t left = skip + l.bytes[at.tensor] - off;
   Chunk k;
-  k.base = reinterpret_cast<uint8_t*>(at - skip) + off;
+  k.base = reinterpret_cast<uint8_t*>(data - skip) + off;
   k.begin = off == 0 ? skip : 0;
   k.end = static_cast<int>(left < kChunk ? left : kChunk);
-  k.type = l.type[lo];
+  k.type = l.type[at.tensor];
   return k;
 }
 
-// The vectors of a chunk that are the thread's; elements outside of the tensor are zeros.
-template <class T>
-__device__ __forceinline__ void load_chunk(const Chunk& k, Pack<T, 16> (&v)[kVectors]) {
-  constexpr int N = Pack<T, 16>::N;
+// The vectors of a chunk that are the thread's, as bits; what lies outside of the tensor is zero.
+struct Bits {
+  uint4 v[kVectors];
+};
+__device__ __forceinline__ int offset_of(int i) { return (i * kThreads + static_cast<int>(threadIdx.x)) * 16; }
+__device__ __forceinline__ void load_chunk(const Chunk& k, Bits& b) {
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int o = (i * kThreads + static_cast<int>(threadIdx.x)) * 16;
+    const int o = offset_of(i);
     if (o >= k.begin && o + 16 <= k.end) {
-      v[i] = *reinterpret_cast<const Pack<T, 16>*>(k.base + o);
+      b.v[i] = *reinterpret_cast<const uint4*>(k.base + o);
     } else {
+      uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int at = o + e * static_cast<int>(sizeof(T));
-        v[i].v[e] = from_float<T>(0.f);
-        if (at >= k.begin && at < k.end) v[i].v[e] = *reinterpret_cast<const T*>(k.base + at);
-      }
+      for (int h = 0; h < 8; ++h)
+        if (o + 2 * h >= k.begin && o + 2 * h < k.end) w[h / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(k.base + o + 2 * h)) << (h % 2 * 16);
+      b.v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+__device__ __forceinline__ void store_chunk(const Chunk& k, const Bits& b) {
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const int o = offset_of(i);
+    if (o >= k.begin && o + 16 <= k.end) {
+      __stcs(reinterpret_cast<uint4*>(k.base + o), b.v[i]);
+    } else {
+      const uint32_t w[4] = {b.v[i].x, b.v[i].y, b.v[i].z, b.v[i].w};
+#pragma unroll
+      for (int h = 0; h < 8; ++h)
+        if (o + 2 * h >= k.begin && o + 2 * h < k.end) *reinterpret_cast<uint16_t*>(k.base + o + 2 * h) = static_cast<uint16_t>(w[h / 2] >> (h % 2 * 16));
     }
   }
 }
 
-template <class T>
-__device__ __forceinline__ void scale_chunk(const Chunk& k, float c) {
+// f(numbers) for each vector, with T's N numbers of it.
+template <class T, class F>
+__device__ __forceinline__ void for_vectors(const Bits& b, F f) {
   constexpr int N = Pack<T, 16>::N;
-  Pack<T, 16> v[kVectors];
-  load_chunk<T>(k, v);
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int o = (i * kThreads + static_cast<int>(threadIdx.x)) * 16;
+    const Pack<T, 16> p = *reinterpret_cast<const Pack<T, 16>*>(&b.v[i]);
+    float x[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[i].v[e] = from_float<T>(to_float(v[i].v[e]) * c);
-    if (o >= k.begin && o + 16 <= k.end) {
-      *reinterpret_cast<Pack<T, 16>*>(k.base + o) = v[i];
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int at = o + e * static_cast<int>(sizeof(T));
-        if (at >= k.begin && at < k.end) *reinterpret_cast<T*>(k.base + at) = v[i].v[e];
-      }
-    }
+    for (int e = 0; e < N; ++e) x[e] = to_float(p.v[e]);
+    f(x);
   }
+}
+template <class T>
+__device__ __forceinline__ void scale_bits(Bits& b, float c) {
+  constexpr int N = Pack<T, 16>::N;
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    Pack<T, 16>& p = *reinterpret_cast<Pack<T, 16>*>(&b.v[i]);
+#pragma unroll
+    for (int e = 0; e < N; ++e) p.v[e] = from_float<T>(to_float(p.v[e]) * c);
+  }
+}
+__device__ __forceinline__ void scale_bits(Bits& b, int type, float c) {
+  if (type == TRITURUS_B200_TYPE_F32)
+    scale_bits<float>(b, c);
+  else if (type == TRITURUS_B200_TYPE_BF16)
+    scale_bits<__nv_bfloat16>(b, c);
+  else
+    scale_bits<__half>(b, c);
 }
 
 // Adds the squares of a chunk's elements.  A vector's squares are added in 32 bits where they neither overflow nor lose digits
-// below the least normal number, else in 64 bits: a norm that 32 bits can hold is not lost to its square.
+// below the least normal number, else in 64 bits: a norm that 32 bits can hold is not lost to its square.  The largest magnitude is held as
+// bits: those of a NaN are above those of infinity.
+struct Sum {
+  double squares;
+  uint32_t most;
+};
 template <class T>
-__device__ __forceinline__ void add_squares(const Chunk& k, double& sum) {
+__device__ __forceinline__ void add_bits(const Bits& b, bool largest, Sum& sum) {
   constexpr int N = Pack<T, 16>::N;
-  Pack<T, 16> v[kVectors];
-  load_chunk<T>(k, v);
+  if (largest) {
+    for_vectors<T>(b, [&](const float(&x)[N]) {
 #pragma unroll
-  for (int i = 0; i < kVectors; ++i) {
-    float s = 0.f;
+      for (int e = 0; e < N; ++e) sum.most = max(sum.most, __float_as_uint(x[e]) & 0x7fffffffu);
+    });
+  } else {
+    for_vectors<T>(b, [&](const float(&x)[N]) {
+      float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float x = to_float(v[i].v[e]);
-      s = fmaf(x, x, s);
-    }
-    if (s > 1e-25f && s < 1e38f) {
-      sum += static_cast<double>(s);
-    } else {
+      for (int e = 0; e < N; ++e) s = fmaf(x[e], x[e], s);
+      if (s > 1e-25f && s < 1e38f) {
+        sum.squares += static_cast<double>(s);
+      } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const double x = static_cast<double>(to_float(v[i].v[e]));
-        sum = fma(x, x, sum);
+        for (int e = 0; e < N; ++e) sum.squares = fma(static_cast<double>(x[e]), static_cast<double>(x[e]), sum.squares);
       }
-    }
+    });
   }
 }
-
-// The largest magnitude, as bits: those of a NaN are above those of infinity.
-template <class T>
-__device__ __forceinline__ void raise_largest(const Chunk& k, uint32_t& most) {
-  constexpr int N = Pack<T, 16>::N;
-  Pack<T, 16> v[kVectors];
-  load_chunk<T>(k, v);
-#pragma unroll
-  for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-    for (int e = 0; e < N; ++e) most = max(most, __float_as_uint(to_float(v[i].v[e])) & 0x7fffffffu);
+__device__ __forceinline__ void add_bits(const Bits& b, int type, bool largest, Sum& sum) {
+  if (type == TRITURUS_B200_TYPE_F32)
+    add_bits<float>(b, largest, sum);
+  else if (type == TRITURUS_B200_TYPE_BF16)
+    add_bits<__nv_bfloat16>(b, largest, sum);
+  else
+    add_bits<__half>(b, largest, sum);
+}
+__device__ __forceinline__ double sum_of(const Sum& sum, bool largest) {
+  return largest ? static_cast<double>(__uint_as_float(sum.most)) : sum.squares;
 }
 
 __device__ __forceinline__ double combine(double a, double b, bool largest) {
@@ -169,33 +208,46 @@ __device__ __forceinline__ double block_combine(double v, double* part, bool lar
   return v;
 }
 
+// The norm and the factor from the sum of all, for thread 0.
+__device__ __forceinline__ float factor_of(const ClipArgs& p, double sum, float* norm) {
+  const double n = p.largest ? sum : sqrt(sum);
+  *norm = static_cast<float>(n);
+  // (a norm beyond 32 bits still has its factor; a NaN among the elements makes all of them NaN)
+  return n + 1e-6 <= p.limit ? 1.f : static_cast<float>(p.limit / (n + 1e-6));
+}
+
+// The block's run of chunks.
+__device__ __forceinline__ uint32_t run_start(uint32_t chunks, uint32_t block, uint32_t blocks) {
+  return static_cast<uint32_t>(static_cast<uint64_t>(chunks) * block / blocks);
+}
+
 template <int MOST>
 __global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_constant__ TensorList<MOST> l, const ClipArgs p) {
   __shared__ double part[kThreads / 32];
-  double sum = 0.0;
-  uint32_t most = 0;
-  for (uint32_t c = blockIdx.x; c < l.chunks; c += gridDim.x) {
-    const Chunk k = find_chunk(l, c);
-    if (!p.largest) {
-      if (k.type == TRITURUS_B200_TYPE_F32)
-        add_squares<float>(k, sum);
-      else if (k.type == TRITURUS_B200_TYPE_BF16)
-        add_squares<__nv_bfloat16>(k, sum);
-      else
-        add_squares<__half>(k, sum);
-    } else {
-      if (k.type == TRITURUS_B200_TYPE_F32)
-        raise_largest<float>(k, most);
-      else if (k.type == TRITURUS_B200_TYPE_BF16)
-        raise_largest<__nv_bfloat16>(k, most);
-      else
-        raise_largest<__half>(k, most);
+  Sum sum = {0.0, 0};
+  Cursor at = cursor_at(l, run_start(l.chunks, blockIdx.x, gridDim.x));
+  const uint32_t end = run_start(l.chunks, blockIdx.x + 1, gridDim.x);
+  if (at.chunk < end) {
+    Chunk k = chunk_at(l, at);
+    Bits now;
+    load_chunk(k, now);
+    for (;;) {  // (the next chunk is under way while one is added)
+      const int type = k.type;
+      Bits next;
+      const bool more = ++at.chunk < end;
+      if (more) {
+        if (at.tensor + 1 < l.count && at.chunk >= l.first[at.tensor + 1]) ++at.tensor;
+        k = chunk_at(l, at);
+        load_chunk(k, next);
+      }
+      add_bits(now, type, p.largest, sum);
+      if (!more) break;
+      now = next;
     }
   }
   pdl_launch_dependents();
-  if (p.largest) sum = static_cast<double>(__uint_as_float(most));
-  sum = block_combine(sum, part, p.largest);
-  if (threadIdx.x == 0) p.sums[p.sums_here + blockIdx.x] = sum;
+  const double v = block_combine(sum_of(sum, p.largest), part, p.largest);
+  if (threadIdx.x == 0) p.sums[p.sums_here + blockIdx.x] = v;
 }
 
 // `scale` == 0: the norm alone (one block).
@@ -208,24 +260,83 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   for (int i = threadIdx.x; i < p.sums_in_all; i += kThreads) v = combine(v, p.sums[i], p.largest);
   v = block_combine(v, part, p.largest);
   if (threadIdx.x == 0) {
-    const double n = p.largest ? v : sqrt(v);
-    // (a norm beyond 32 bits still has its factor; a NaN among the elements makes all of them NaN)
-    factor = n + 1e-6 <= p.limit ? 1.f : static_cast<float>(p.limit / (n + 1e-6));
-    if (blockIdx.x == 0 && p.sums_here == 0) *p.norm = static_cast<float>(n);
+    float n;
+    factor = factor_of(p, v, &n);
+    if (blockIdx.x == 0 && p.sums_here == 0) *p.norm = n;
   }
   __syncthreads();
   const float c = factor;
   if (!scale || c == 1.f) return;
-  const uint32_t last = (l.chunks - 1 - blockIdx.x) / gridDim.x;  // (no more blocks than chunks)
-  for (uint32_t i = 0; i <= last; ++i) {
-    const Chunk k = find_chunk(l, blockIdx.x + (last - i) * gridDim.x);
-    if (k.type == TRITURUS_B200_TYPE_F32)
-      scale_chunk<float>(k, c);
-    else if (k.type == TRITURUS_B200_TYPE_BF16)
-      scale_chunk<__nv_bfloat16>(k, c);
-    else
-      scale_chunk<__half>(k, c);
+  const uint32_t begin = run_start(l.chunks, blockIdx.x, gridDim.x);
+  Cursor at = cursor_at(l, run_start(l.chunks, blockIdx.x + 1, gridDim.x) - 1);  // (no more blocks than chunks)
+  Chunk k = chunk_at(l, at);
+  Bits now;
+  load_chunk(k, now);
+  for (;;) {
+    const Chunk here = k;
+    Bits next;
+    const bool more = at.chunk > begin;
+    if (more) {
+      --at.chunk;
+      if (at.chunk < l.first[at.tensor]) --at.tensor;
+      k = chunk_at(l, at);
+      load_chunk(k, next);
+    }
+    scale_bits(now, here.type, c);
+    store_chunk(here, now);
+    if (!more) break;
+    now = next;
   }
+}
+
+// All in one launch, for up to C * kHeld chunks: the blocks of a cluster hold them.
+constexpr int kHeld = 2;
+template <int C>
+__global__ void __launch_bounds__(kThreads) clip_small_kernel(const __grid_constant__ TensorList<64> l, const ClipArgs p, int scale) {
+  __shared__ double part[kThreads / 32];
+  __shared__ double block_sum;
+  __shared__ float factor;
+  Chunk k[kHeld];
+  Bits held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const uint32_t c = blockIdx.x + i * C;
+    if (c < l.chunks) {
+      k[i] = chunk_at(l, cursor_at(l, c));
+      load_chunk(k[i], held[i]);
+    }
+  }
+  Sum sum = {0.0, 0};
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (blockIdx.x + i * C < l.chunks) add_bits(held[i], k[i].type, p.largest, sum);
+  double v = block_combine(sum_of(sum, p.largest), part, p.largest);
+  if (threadIdx.x == 0) block_sum = v;
+  if (C > 1) cluster_sync_all();
+  if (threadIdx.x == 0) {
+    if (C > 1) {
+      v = 0.0;
+      for (int q = 0; q < C; ++q) {
+        double other;
+        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(other) : "r"(map_to_cta(smem_u32(&block_sum), q)) : "memory");
+        v = combine(v, other, p.largest);
+      }
+    }
+    float n;
+    factor = factor_of(p, v, &n);
+    if (blockIdx.x == 0) *p.norm = n;
+  }
+  __syncthreads();
+  const float c = factor;
+  if (scale && c != 1.f) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (blockIdx.x + i * C < l.chunks) {
+        scale_bits(held[i], k[i].type, c);
+        store_chunk(k[i], held[i]);
+      }
+  }
+  if (C > 1) cluster_sync_all();  // (the others' sums are read until here)
 }
 
 // ----------------------------------------------------------------------------- launches
@@ -265,6 +376,22 @@ bool launch(Kern kern, int blocks, bool dependent, cudaStream_t stream, const Te
   return cudaLaunchKernelEx(&cfg, kern, l, p, more...) == cudaSuccess;
 }
 
+template <int C>
+int run_small(const TensorList<64>& l, const ClipArgs& p, int scale, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = C;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, clip_small_kernel<C>, l, p, scale) == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+}
+
 template <int MOST>
 int run_clip(void* const* data, const int64_t* numels, const int* types, int64_t count, ClipArgs p, int scale, cudaStream_t stream) {
   const int64_t lists = std::max<int64_t>(1, (count + MOST - 1) / MOST);
@@ -272,6 +399,10 @@ int run_clip(void* const* data, const int64_t* numels, const int* types, int64_t
   p.sums_in_all = 0;
   for (int64_t i = 0; i < lists; ++i) {
     if (!fill_list(&l, data, numels, types, i * MOST, std::min(count, (i + 1) * MOST))) return TRITURUS_B200_EINVAL;
+    if constexpr (MOST == 64) {
+      if (l.chunks <= kHeld) return run_small<1>(l, p, scale, stream);
+      if (l.chunks <= 8 * kHeld) return run_small<8>(l, p, scale, stream);
+    }
     p.sums_here = p.sums_in_all;
     const int blocks = blocks_for(l.chunks);
     p.sums_in_all += blocks;

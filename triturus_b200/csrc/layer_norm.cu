@@ -39,16 +39,24 @@ struct NormArgs {
   float eps;
 };
 
-// BYTES from global to shared memory without a register.  (16-bit rows on odd addresses: a plain load.)
+// A vector of a row on its way through shared memory.  Rows of 16-bit elements on addresses that 4 does not divide have no copy of their own: an element
+// comes as the 4-byte word that it is a half of.
+template <class T, int BYTES>
+struct alignas(BYTES < 4 ? 4 : BYTES) Slot {
+  static constexpr int N = BYTES / static_cast<int>(sizeof(T));
+  Pack<T, (BYTES < 4 ? 4 : BYTES)> p;
+  // `half`: the address's second bit
+  __device__ __forceinline__ float get(int e, int half) const { return to_float(BYTES < 4 ? (half ? p.v[1] : p.v[0]) : p.v[e]); }
+};
+// ... from global to shared memory without a register.
 template <int BYTES>
 __device__ __forceinline__ void fetch(void* dst, const void* src) {
   if constexpr (BYTES == 16)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-  else if constexpr (BYTES == 4)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
   else
-    *static_cast<uint16_t*>(dst) = *static_cast<const uint16_t*>(src);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(3)) : "memory");
 }
+__device__ __forceinline__ int half_of(const void* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1; }
 __device__ __forceinline__ void wait_for_row(int stages) {
   if (stages == 4)
     cp_async_wait<3>();
@@ -58,30 +66,163 @@ __device__ __forceinline__ void wait_for_row(int stages) {
     cp_async_wait<0>();
 }
 
+// Two 32-bit numbers that are worked on at once: what these kernels would otherwise be bound by is the number of their instructions.
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 parts_of(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float both(Pair p) {
+  const float2 f = parts_of(p);
+  return f.x + f.y;
+}
+// Of 16-bit elements, as they lie in a word.
+template <class T>
+__device__ __forceinline__ Pair unpack(uint32_t w);
+template <>
+__device__ __forceinline__ Pair unpack<__nv_bfloat16>(uint32_t w) {  // (a bfloat16 is the upper half of a 32-bit number)
+  return pair_of(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ Pair unpack<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pair_of(f.x, f.y);
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack(Pair p);
+template <>
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(Pair p) {
+  const float2 f = parts_of(p);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack<__half>(Pair p) {
+  const float2 f = parts_of(p);
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // How the elements of a row are dealt out: vectors of N elements, vector v to thread v % TH of the row's group of TH threads, NV to a thread.  What
 // lies behind the row's end is never fetched and stays zero.
 template <class T, int BYTES, int NV, int TH>
 struct Deal {
   using P = Pack<T, BYTES>;
   static constexpr int N = P::N;
-  int left;  // vectors of the row from the thread's first one on
+  // A thread's elements are worked on in chunks of pairs: a vector, or two of one element.
+  static constexpr int kVectors = N == 1 ? 2 : 1, kPairs = N == 1 ? 1 : N / 2, kChunks = NV / kVectors;
+  int vectors;       // of the row
+  int left;          // from the thread's first one on
   int first_column;
-  __device__ __forceinline__ Deal(int t, int width) : left(width / N - t), first_column(t * N) {}
+  __device__ __forceinline__ Deal(int t, int width) : vectors(width / N), left(width / N - t), first_column(t * N) {}
   __device__ __forceinline__ bool has(int i) const { return left > i * TH; }
   __device__ __forceinline__ int column(int i) const { return first_column + i * TH * N; }
+  __device__ __forceinline__ bool beyond(int c) const { return vectors <= c * kVectors * TH; }            // for all threads
+  __device__ __forceinline__ bool whole(int c) const { return vectors >= (c + 1) * kVectors * TH; }       // for all threads
+
+  // Chunk c of a row in shared memory, `pitch` slots from vector to vector.
+  __device__ __forceinline__ void read(const Slot<T, BYTES>* ring, int pitch, int c, int half, Pair (&out)[kPairs]) const {
+    if constexpr (N == 1) {
+      out[0] = pair_of(ring[2 * c * pitch].get(0, half), ring[(2 * c + 1) * pitch].get(0, half));
+    } else if constexpr (sizeof(T) == 2) {
+      using U = Pack<uint32_t, BYTES>;
+      const U u = *reinterpret_cast<const U*>(ring + c * pitch);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) out[k] = unpack<T>(u.v[k]);
+    } else {
+      const Slot<T, BYTES> x = ring[c * pitch];
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) out[k] = pair_of(x.get(2 * k, 0), x.get(2 * k + 1, 0));
+    }
+  }
+  // ... into a row of global memory; `row` is where the thread's first vector goes.
+  __device__ __forceinline__ void write(T* row, int c, const Pair (&v)[kPairs]) const {
+    if constexpr (N == 1) {
+      const float2 f = parts_of(v[0]);
+      if (has(2 * c)) row[2 * c * TH] = from_float<T>(f.x);
+      if (has(2 * c + 1)) row[(2 * c + 1) * TH] = from_float<T>(f.y);
+    } else if (has(c)) {
+      if constexpr (sizeof(T) == 2) {
+        Pack<uint32_t, BYTES> u;
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) u.v[k] = pack<T>(v[k]);
+        *reinterpret_cast<Pack<uint32_t, BYTES>*>(row + c * TH * N) = u;
+      } else {
+        P o;
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          const float2 f = parts_of(v[k]);
+          o.v[2 * k] = f.x;
+          o.v[2 * k + 1] = f.y;
+        }
+        *reinterpret_cast<P*>(row + c * TH * N) = o;
+      }
+    }
+  }
+  // The column of the first or second number of pair k of chunk c.
+  __device__ __forceinline__ int column(int c, int k, int second) const {
+    return N == 1 ? column(2 * c + second) : column(c) + 2 * k + second;
+  }
+  __device__ __forceinline__ bool has(int c, int second) const { return N == 1 ? has(2 * c + second) : has(c); }
 };
 
-// The thread's weights, zeros behind the row's end.
-template <class T, class D, int NV>
-__device__ __forceinline__ void load_weights(const D& d, const void* w, int weight32, float fill, float (&out)[NV][D::N]) {
+// The thread's weights, zeros behind the row's end; 16 bytes at a time where the vectors are that and begin on such a boundary.
+template <class W, int N>
+__device__ __forceinline__ void load_vector(const W* w, bool aligned, float (&out)[N]) {
+  constexpr int BYTES = N * static_cast<int>(sizeof(W));
+  if (BYTES % 16 == 0 && aligned) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+    for (int part = 0; part < BYTES / 16; ++part) {
+      using P = Pack<W, 16>;
+      const P v = reinterpret_cast<const P*>(w)[part];
 #pragma unroll
-    for (int e = 0; e < D::N; ++e) {
-      out[i][e] = d.has(i) ? fill : 0.f;
-      if (w != nullptr && d.has(i))
-        out[i][e] = weight32 ? __ldg(static_cast<const float*>(w) + d.column(i) + e) : to_float(static_cast<const T*>(w)[d.column(i) + e]);
+      for (int e = 0; e < P::N; ++e) out[part * P::N + e] = to_float(v.v[e]);
     }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = to_float(w[e]);
+  }
+}
+template <class T, class D, int NV>
+__device__ __forceinline__ void load_weights(const D& d, const void* w, int weight32, float fill, Pair (&out)[NV * D::N / 2]) {
+  const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+  float f[NV][D::N];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int e = 0; e < D::N; ++e) f[i][e] = d.has(i) ? fill : 0.f;
+    if (w != nullptr && d.has(i)) {
+      if (weight32)
+        load_vector(static_cast<const float*>(w) + d.column(i), aligned, f[i]);
+      else
+        load_vector(static_cast<const T*>(w) + d.column(i), aligned, f[i]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < NV * D::N / 2; ++k) out[k] = pair_of(f[2 * k / D::N][2 * k % D::N], f[(2 * k + 1) / D::N][(2 * k + 1) % D::N]);
 }
 
 // The sums over a group of TH threads of K values, in each of them.  A group of warps meets at a barrier of its own; two calls in a row use different
@@ -119,15 +260,15 @@ __device__ __forceinline__ float group_sum(float v, float (*part)[WARPS], int gr
 }
 
 template <class T, int BYTES, int NV, int TH, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, BLOCK >= 512 ? 1 : 768 / BLOCK) norm_forward_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(BLOCK, NV * Pack<T, BYTES>::N > 16 ? 1 : BLOCK == 512 ? 2 : 768 / BLOCK) norm_forward_kernel(const NormArgs p) {
   using D = Deal<T, BYTES, NV, TH>;
-  using P = typename D::P;
   constexpr int kGroups = BLOCK / TH;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float part[2][BLOCK / 32];
   const int group = threadIdx.x / TH, t = threadIdx.x % TH;
   const D d(t, p.width);
-  P* const ring = reinterpret_cast<P*>(smem) + threadIdx.x;
+  using S = Slot<T, BYTES>;
+  S* const ring = reinterpret_cast<S*>(smem) + threadIdx.x;
   const float inv = 1.f / static_cast<float>(p.width);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + group, step = static_cast<int64_t>(gridDim.x) * kGroups;
   auto ask = [&](int64_t row, int stage) {
@@ -142,47 +283,58 @@ __global__ void __launch_bounds__(BLOCK, BLOCK >= 512 ? 1 : 768 / BLOCK) norm_fo
   for (int s = 0; s < p.stages; ++s) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (!d.has(i)) ring[(s * NV + i) * BLOCK] = P{};
+      if (!d.has(i)) ring[(s * NV + i) * BLOCK] = S{};
     ask(first + s * step, s);
   }
-  float weight[NV][D::N], bias[NV][D::N];
-  load_weights<T>(d, p.weight, p.weight32, 1.f, weight);
-  load_weights<T>(d, p.bias, p.weight32, 0.f, bias);
+  Pair weight[D::kChunks * D::kPairs], bias[D::kChunks * D::kPairs];
+  load_weights<T, D, NV>(d, p.weight, p.weight32, 1.f, weight);
+  load_weights<T, D, NV>(d, p.bias, p.weight32, 0.f, bias);
   int stage = 0;
   for (int64_t row = first; row < p.rows; row += step) {
     wait_for_row(p.stages);
-    float v[NV][D::N], s = 0.f;
+    const int half = BYTES < 4 ? half_of(static_cast<const T*>(p.x) + row * p.x_stride + d.first_column) : 0;  // (the same for all i: TH is even)
+    Pair v[D::kChunks][D::kPairs], sum = pair_of(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const P x = ring[(stage * NV + i) * BLOCK];
+    for (int c = 0; c < D::kChunks; ++c) {
+      if (d.beyond(c)) break;
+      d.read(ring + stage * NV * BLOCK, BLOCK, c, half, v[c]);
 #pragma unroll
-      for (int e = 0; e < D::N; ++e) s += v[i][e] = to_float(x.v[e]);
+      for (int k = 0; k < D::kPairs; ++k) sum = sum + v[c][k];
     }
-    const float mean = group_sum<TH>(s, part, group) * inv;
+    const float mean = group_sum<TH>(both(sum), part, group) * inv;
     ask(row + p.stages * step, stage);  // (the values are in registers: they are part of the sum)
     stage = stage + 1 == p.stages ? 0 : stage + 1;
-    float q = 0.f;
+    const Pair down = pair_of(-mean, -mean);
+    Pair squares = pair_of(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int c = 0; c < D::kChunks; ++c) {
+      if (d.beyond(c)) break;
 #pragma unroll
-      for (int e = 0; e < D::N; ++e) {
-        v[i][e] = d.has(i) ? v[i][e] - mean : 0.f;
-        q = fmaf(v[i][e], v[i][e], q);
+      for (int k = 0; k < D::kPairs; ++k) v[c][k] = v[c][k] + down;
+      if (!d.whole(c)) {
+#pragma unroll
+        for (int k = 0; k < D::kPairs; ++k) {
+          const float2 f = parts_of(v[c][k]);
+          v[c][k] = pair_of(d.has(c, 0) ? f.x : 0.f, d.has(c, 1) ? f.y : 0.f);
+        }
       }
-    const float rstd = 1.f / sqrtf(fmaf(group_sum<TH>(q, part + 1, group), inv, p.eps));
+#pragma unroll
+      for (int k = 0; k < D::kPairs; ++k) squares = fma2(v[c][k], v[c][k], squares);
+    }
+    const float rstd = 1.f / sqrtf(fmaf(group_sum<TH>(both(squares), part + 1, group), inv, p.eps));
     if (t == 0) {
       if (p.mean != nullptr) p.mean[row] = mean;
       if (p.rstd != nullptr) p.rstd[row] = rstd;
     }
+    const Pair scale = pair_of(rstd, rstd);
     T* y = static_cast<T*>(p.y) + row * p.width + d.first_column;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (d.has(i)) {
-        P o;
+    for (int c = 0; c < D::kChunks; ++c) {
+      if (d.beyond(c)) break;
 #pragma unroll
-        for (int e = 0; e < D::N; ++e) o.v[e] = from_float<T>(fmaf(v[i][e] * rstd, weight[i][e], bias[i][e]));
-        *reinterpret_cast<P*>(y + i * TH * D::N) = o;
-      }
+      for (int k = 0; k < D::kPairs; ++k) v[c][k] = fma2(v[c][k] * scale, weight[c * D::kPairs + k], bias[c * D::kPairs + k]);
+      d.write(y, c, v[c]);
+    }
   }
 }
 
@@ -225,13 +377,13 @@ constexpr int kBack = 512;
 template <class T, int BYTES, int NV, int TH>
 __global__ void __launch_bounds__(kBack) norm_backward_kernel(const NormArgs p) {
   using D = Deal<T, BYTES, NV, TH>;
-  using P = typename D::P;
   constexpr int kGroups = kBack / TH;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float part[2][2][kBack / 32];
   const int group = threadIdx.x / TH, t = threadIdx.x % TH;
   const D d(t, p.width);
-  P* const ring = reinterpret_cast<P*>(smem) + threadIdx.x;
+  using S = Slot<T, BYTES>;
+  S* const ring = reinterpret_cast<S*>(smem) + threadIdx.x;
   const float inv = 1.f / static_cast<float>(p.width);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + group, step = static_cast<int64_t>(gridDim.x) * kGroups;
   auto ask = [&](int64_t row, int stage) {
@@ -250,21 +402,21 @@ __global__ void __launch_bounds__(kBack) norm_backward_kernel(const NormArgs p) 
   for (int s = 0; s < p.stages; ++s) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (!d.has(i)) ring[(s * 2 * NV + i) * kBack] = ring[(s * 2 * NV + NV + i) * kBack] = P{};
+      if (!d.has(i)) ring[(s * 2 * NV + i) * kBack] = ring[(s * 2 * NV + NV + i) * kBack] = S{};
     ask(first + s * step, s);
   }
-  float weight[NV][D::N];
-  load_weights<T>(d, p.weight, p.weight32, 1.f, weight);
+  Pair weight[D::kChunks * D::kPairs];
+  load_weights<T, D, NV>(d, p.weight, p.weight32, 1.f, weight);
   float mean = 0.f, rstd = 0.f;
   if (first < p.rows) {
     mean = p.mean[first];
     rstd = p.rstd[first];
   }
-  float dw[NV][D::N], db[NV][D::N];
+  Pair dw[D::kChunks][D::kPairs], db[D::kChunks][D::kPairs];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int c = 0; c < D::kChunks; ++c)
 #pragma unroll
-    for (int e = 0; e < D::N; ++e) dw[i][e] = db[i][e] = 0.f;
+    for (int k = 0; k < D::kPairs; ++k) dw[c][k] = db[c][k] = pair_of(0.f, 0.f);
   int stage = 0, odd = 0;
   for (int64_t row = first; row < p.rows; row += step, odd ^= 1) {
     float next_mean = 0.f, next_rstd = 0.f;
@@ -272,62 +424,73 @@ __global__ void __launch_bounds__(kBack) norm_backward_kernel(const NormArgs p) 
       next_mean = p.mean[row + step];
       next_rstd = p.rstd[row + step];
     }
+    const int half_x = BYTES < 4 ? half_of(static_cast<const T*>(p.x) + row * p.x_stride + d.first_column) : 0;
+    const int half_dy = BYTES < 4 ? half_of(static_cast<const T*>(p.dy) + row * p.dy_stride + d.first_column) : 0;
     wait_for_row(p.stages);
-    float sums_of[2] = {0.f, 0.f};  // of g and g h
+    const Pair down = pair_of(-mean, -mean), scale = pair_of(rstd, rstd);
+    Pair sg = pair_of(0.f, 0.f), sgh = sg;
+    const S* const x_row = ring + stage * 2 * NV * kBack;
+    const S* const dy_row = x_row + NV * kBack;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const P x = ring[(stage * 2 * NV + i) * kBack], dy = ring[(stage * 2 * NV + NV + i) * kBack];
+    for (int c = 0; c < D::kChunks; ++c) {
+      if (d.beyond(c)) break;
+      Pair x[D::kPairs], dy[D::kPairs];
+      d.read(x_row, kBack, c, half_x, x);
+      d.read(dy_row, kBack, c, half_dy, dy);
 #pragma unroll
-      for (int e = 0; e < D::N; ++e) {
-        const float dd = to_float(dy.v[e]), h = (to_float(x.v[e]) - mean) * rstd, g = dd * weight[i][e];
-        sums_of[0] += g;
-        sums_of[1] = fmaf(g, h, sums_of[1]);
-        dw[i][e] = fmaf(dd, h, dw[i][e]);
-        db[i][e] += dd;
+      for (int k = 0; k < D::kPairs; ++k) {
+        const Pair h = (x[k] + down) * scale, g = dy[k] * weight[c * D::kPairs + k];
+        sg = sg + g;
+        sgh = fma2(g, h, sgh);
+        dw[c][k] = fma2(dy[k], h, dw[c][k]);
+        db[c][k] = db[c][k] + dy[k];
       }
     }
+    float sums_of[2] = {both(sg), both(sgh)};
     group_sums<TH>(sums_of, part[odd], group);
     const float mg = sums_of[0] * inv, mgh = sums_of[1] * inv;
+    const Pair minus_mg = pair_of(-mg, -mg), minus_mgh = pair_of(-mgh, -mgh);
     T* dx = static_cast<T*>(p.y) + row * p.width + d.first_column;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const P x = ring[(stage * 2 * NV + i) * kBack], dy = ring[(stage * 2 * NV + NV + i) * kBack];
-      P o;
+    for (int c = 0; c < D::kChunks; ++c) {
+      if (d.beyond(c)) break;
+      Pair x[D::kPairs], dy[D::kPairs];
+      d.read(x_row, kBack, c, half_x, x);
+      d.read(dy_row, kBack, c, half_dy, dy);
 #pragma unroll
-      for (int e = 0; e < D::N; ++e) {
-        const float h = (to_float(x.v[e]) - mean) * rstd;
-        o.v[e] = from_float<T>(rstd * fmaf(-h, mgh, fmaf(to_float(dy.v[e]), weight[i][e], -mg)));
+      for (int k = 0; k < D::kPairs; ++k) {
+        const Pair h = (x[k] + down) * scale;
+        x[k] = scale * fma2(h, minus_mgh, fma2(dy[k], weight[c * D::kPairs + k], minus_mg));
       }
-      if (d.has(i)) *reinterpret_cast<P*>(dx + i * TH * D::N) = o;
+      d.write(dx, c, x);
     }
     ask(row + p.stages * step, stage);  // (what the stage held went into the stores)
     stage = stage + 1 == p.stages ? 0 : stage + 1;
     mean = next_mean;
     rstd = next_rstd;
   }
+  pdl_launch_dependents();
   float* mine = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.width;
-  if constexpr (kGroups == 1) {
+  auto each_sum = [&](const Pair (&sums)[D::kChunks][D::kPairs], float* to) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (d.has(i)) {
+    for (int c = 0; c < D::kChunks; ++c)
 #pragma unroll
-        for (int e = 0; e < D::N; ++e) {
-          mine[d.column(i) + e] = dw[i][e];
-          mine[p.width + d.column(i) + e] = db[i][e];
-        }
+      for (int k = 0; k < D::kPairs; ++k) {
+        const float2 f = parts_of(sums[c][k]);
+        if (d.has(c, 0)) to[d.column(c, k, 0)] = f.x;
+        if (d.has(c, 1)) to[d.column(c, k, 1)] = f.y;
       }
+  };
+  if constexpr (kGroups == 1) {
+    each_sum(dw, mine);
+    each_sum(db, mine + p.width);
   } else {  // the groups' shares, added in their order
     cp_async_wait<0>();
     float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (d.has(i)) {
-#pragma unroll
-          for (int e = 0; e < D::N; ++e) sums[group * p.width + d.column(i) + e] = which == 0 ? dw[i][e] : db[i][e];
-        }
+      each_sum(which == 0 ? dw : db, sums + group * p.width);
       __syncthreads();
       for (int c = threadIdx.x; c < p.width; c += kBack) {
         float v = sums[c];
@@ -437,23 +600,24 @@ int blocks_of_sm(Kern kern, std::atomic<int> (&known)[64], int threads, size_t s
   return n;
 }
 
-// Rows under way, of what shared memory holds.
-constexpr int stages_for(size_t row_bytes, int bytes) {
-  return bytes < 4 ? 1 : 4 * row_bytes <= kMostShared ? 4 : 2 * row_bytes <= kMostShared ? 2 : 1;
+// Rows under way, of what shared memory holds; no more than a group has in all.
+constexpr int stages_for(size_t row_bytes) {
+  return 4 * row_bytes <= kMostShared ? 4 : 2 * row_bytes <= kMostShared ? 2 : 1;
 }
+int stages_of(int most, int64_t rows, int64_t groups) { return rows <= groups ? 1 : rows <= 2 * groups ? std::min(most, 2) : most; }
 
 template <class T, int BYTES, int NV, int TH>
 int run_forward(NormArgs p, cudaStream_t stream) {
   constexpr int BLOCK = TH < 128 ? 128 : TH, kGroups = BLOCK / TH;
-  constexpr size_t row_bytes = static_cast<size_t>(BLOCK) * NV * BYTES;
-  constexpr int stages = stages_for(row_bytes, BYTES);
+  constexpr size_t row_bytes = static_cast<size_t>(BLOCK) * NV * sizeof(Slot<T, BYTES>);
+  constexpr int stages = stages_for(row_bytes);
   static std::atomic<int> known[64];
   const auto kern = norm_forward_kernel<T, BYTES, NV, TH, BLOCK>;
   const int fit = blocks_of_sm(kern, known, BLOCK, stages * row_bytes);
   if (fit == 0) return TRITURUS_B200_ELAUNCH;
-  p.stages = stages;
   const int64_t blocks = std::min<int64_t>((p.rows + kGroups - 1) / kGroups, static_cast<int64_t>(device_sms()) * fit);
-  kern<<<static_cast<unsigned>(blocks), BLOCK, stages * row_bytes, stream>>>(p);
+  p.stages = stages_of(stages, p.rows, blocks * kGroups);
+  kern<<<static_cast<unsigned>(blocks), BLOCK, p.stages * row_bytes, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
 }
 
@@ -463,15 +627,15 @@ int most_shares(int64_t rows) { return static_cast<int>(std::min<int64_t>(rows, 
 template <class T, int BYTES, int NV, int TH>
 int run_backward(NormArgs p, int* blocks, cudaStream_t stream) {
   constexpr int kGroups = kBack / TH;
-  constexpr size_t row_bytes = static_cast<size_t>(kBack) * NV * BYTES * 2;
-  constexpr int stages = stages_for(row_bytes, BYTES);
-  constexpr size_t smem = std::max<size_t>(stages * row_bytes, kGroups > 1 ? static_cast<size_t>(kBack) * NV * BYTES / sizeof(T) * sizeof(float) : 0);
+  constexpr size_t row_bytes = static_cast<size_t>(kBack) * NV * sizeof(Slot<T, BYTES>) * 2;
+  constexpr int stages = stages_for(row_bytes);
+  constexpr size_t sums = kGroups > 1 ? static_cast<size_t>(kBack) * NV * BYTES / sizeof(T) * sizeof(float) : 0;
   static std::atomic<int> known[64];
   const auto kern = norm_backward_kernel<T, BYTES, NV, TH>;
-  if (blocks_of_sm(kern, known, kBack, smem) == 0) return TRITURUS_B200_ELAUNCH;
-  p.stages = stages;
+  if (blocks_of_sm(kern, known, kBack, std::max(stages * row_bytes, sums)) == 0) return TRITURUS_B200_ELAUNCH;
   *blocks = static_cast<int>(std::min<int64_t>((p.rows + kGroups - 1) / kGroups, device_sms()));
-  kern<<<static_cast<unsigned>(*blocks), kBack, smem, stream>>>(p);
+  p.stages = stages_of(stages, p.rows, static_cast<int64_t>(*blocks) * kGroups);
+  kern<<<static_cast<unsigned>(*blocks), kBack, std::max(p.stages * row_bytes, sums), stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
 }
 
