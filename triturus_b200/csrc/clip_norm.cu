@@ -224,6 +224,7 @@ __device__ __forceinline__ uint32_t run_start(uint32_t chunks, uint32_t block, u
 template <int MOST>
 __global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_constant__ TensorList<MOST> l, const ClipArgs p) {
   __shared__ double part[kThreads / 32];
+  pdl_launch_dependents();  // (all blocks are resident: the next launch's take their places as they leave)
   Sum sum = {0.0, 0};
   Cursor at = cursor_at(l, run_start(l.chunks, blockIdx.x, gridDim.x));
   const uint32_t end = run_start(l.chunks, blockIdx.x + 1, gridDim.x);
@@ -245,7 +246,6 @@ __global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_const
       now = next;
     }
   }
-  pdl_launch_dependents();
   const double v = block_combine(sum_of(sum, p.largest), part, p.largest);
   if (threadIdx.x == 0) p.sums[p.sums_here + blockIdx.x] = v;
 }
@@ -255,6 +255,15 @@ template <int MOST>
 __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ TensorList<MOST> l, const ClipArgs p, int scale) {
   __shared__ double part[kThreads / 32];
   __shared__ float factor;
+  const uint32_t begin = run_start(l.chunks, blockIdx.x, gridDim.x);
+  Cursor at = {0, 0};
+  Chunk k = {};
+  Bits now;
+  if (scale) {  // (no launch before this one writes the elements, but for an earlier list's: they are read while it ends)
+    at = cursor_at(l, run_start(l.chunks, blockIdx.x + 1, gridDim.x) - 1);  // (no more blocks than chunks)
+    k = chunk_at(l, at);
+    load_chunk(k, now);
+  }
   pdl_wait();
   double v = 0.0;
   for (int i = threadIdx.x; i < p.sums_in_all; i += kThreads) v = combine(v, p.sums[i], p.largest);
@@ -267,11 +276,6 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   __syncthreads();
   const float c = factor;
   if (!scale || c == 1.f) return;
-  const uint32_t begin = run_start(l.chunks, blockIdx.x, gridDim.x);
-  Cursor at = cursor_at(l, run_start(l.chunks, blockIdx.x + 1, gridDim.x) - 1);  // (no more blocks than chunks)
-  Chunk k = chunk_at(l, at);
-  Bits now;
-  load_chunk(k, now);
   for (;;) {
     const Chunk here = k;
     Bits next;
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) clip_small_kernel(const __grid_const
 
 // ----------------------------------------------------------------------------- launches
 
-int blocks_for(uint32_t chunks) { return static_cast<int>(std::min<int64_t>(chunks, std::min(kMostBlocks, device_sms() * 4))); }
+int blocks_for(uint32_t chunks) { return static_cast<int>(std::min<int64_t>(chunks, std::min(kMostBlocks, device_sms() * 2))); }
 
 // Tensors [from, to) that have elements, as a list; false: more chunks than 32 bits count.
 template <int MOST>
