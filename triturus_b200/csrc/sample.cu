@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
+#include <cstdlib>
 
 #include "../../include/triturus_b200.h"
 #include "packs.cuh"
@@ -32,8 +33,8 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 256;
 constexpr int kList = 1024;  // symbols that the first block of a row can gather
-constexpr int kWarpKept = 256;  // symbols of a slice in shared memory that a warp can set apart
-constexpr int kWarpCopied = 768;  // ... and of one that is not, with their values
+constexpr int kKept = 16;    // symbols of a slice in shared memory that a thread can set apart
+constexpr int kCopied = 20;  // ... and of one that is not, with their values
 constexpr int kFew = kThreads / 2;  // a small top_k
 
 struct SampleArgs {
@@ -60,6 +61,7 @@ struct alignas(16) Shared {
   uint32_t mass[kBins];       // the block's, as multiples of 2^-clz(count)
   uint32_t all_count[kBins];  // the cluster's
   uint32_t fine_count[kBins];
+  uint32_t all_fine[kBins];
   unsigned long long few[33];
   float red[2][kWarps];
   int red_i[2][kWarps];
@@ -121,10 +123,11 @@ struct Row {
   float cut;      // kept so far: values above cut, and of those equal to it the indexes up to cidx
   int cidx;
 };
-__device__ __forceinline__ float prob(const Row& r, float x) { return ex2_approx((x - r.top) * r.k2); }
 // (the whole part of a number below 2^23 stands in the last bits of its sum with 2^23: no conversion)
 __device__ __forceinline__ int whole_part(float t) { return __float_as_int(__fadd_rz(t, 8388608.f)) & 0x3ff; }
 __device__ __forceinline__ float bin_place(const Row& r, float x) { return (r.top - x) * r.to_bin; }
+__device__ __forceinline__ float prob_at(float place) { return ex2_approx(place * -kStep); }
+__device__ __forceinline__ float prob(const Row& r, float x) { return prob_at(bin_place(r, x)); }
 // (a symbol so far below the top that 32 bits do not hold how far has p = 0: it is in no bin, as one of -inf)
 constexpr int kNoBin = 0x7fff;
 __device__ __forceinline__ int bin_of(const Row& r, float x) {
@@ -139,9 +142,9 @@ struct Slice {
   const T* row;
   float* held;
   int first, size, symbols;
-  bool apart;            // the warp has set apart what can still be kept:
-  int kept_count;        // so many
-  uint16_t* kept;        // HELD: their elements' numbers
+  bool apart;            // the thread has set apart which of its elements can still be kept:
+  int kept_count;        // so many, kThreads places apart
+  uint16_t* kept;        // HELD: their numbers
   float* kept_x;         // else their values
   int* kept_j;           // and numbers
   __device__ __forceinline__ float at(int j) const {
@@ -178,22 +181,23 @@ __device__ __forceinline__ float load_slice(const Slice<T, HELD>& s) {
   return top;
 }
 
-// The N elements from j on, of memory where the slice is not held.
+// The N elements from j on, of memory where the slice is not held; -inf from the slice's end on.
 template <class T, int N>
 __device__ __forceinline__ void load_elements(const Slice<T, false>& s, int j, float (&v)[N]) {
   const int i = s.first + j;
-  if (i >= 0 && i + N <= s.symbols) {
+  if (i >= 0 && i + N <= s.symbols && j < s.size) {
     const Pack<T, 16> p = *reinterpret_cast<const Pack<T, 16>*>(s.row + i);
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = fminf(to_float(p.v[e]), FLT_MAX);
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = s.at(j + e);
+    for (int e = 0; e < N; ++e) v[e] = j < s.size ? s.at(j + e) : -INFINITY;
   }
 }
 template <class T, int N>
 __device__ __forceinline__ void load_elements(const Slice<T, true>& s, int j, float (&v)[N]) {
-  const float4 p = *reinterpret_cast<const float4*>(s.held + j);
+  float4 p = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  if (j < s.size) p = *reinterpret_cast<const float4*>(s.held + j);
   v[0] = p.x;
   v[1] = p.y;
   v[2] = p.z;
@@ -201,65 +205,56 @@ __device__ __forceinline__ void load_elements(const Slice<T, true>& s, int j, fl
 }
 template <class T, bool HELD>
 constexpr int kRun = HELD ? 4 : Pack<T, 16>::N;  // elements of one load
+template <class T, bool HELD>
+constexpr int kRuns = HELD ? 2 : 16 / Pack<T, 16>::N;  // loads under way: what f does may keep the compiler from starting them early
 
 // f(x, j) for the thread's elements of the slice.
 template <class T, bool HELD, class F>
 __device__ __forceinline__ void for_slice(const Slice<T, HELD>& s, F f) {
-  constexpr int N = kRun<T, HELD>;
-#pragma unroll(HELD ? 2 : 16 / N)
-  for (int j = static_cast<int>(threadIdx.x) * N; j < s.size; j += kThreads * N) {
-    float v[N];
-    load_elements(s, j, v);
+  constexpr int N = kRun<T, HELD>, U = kRuns<T, HELD>;
+#pragma unroll 1
+  for (int j = static_cast<int>(threadIdx.x) * N; j < s.size; j += kThreads * N * U) {
+    float v[U][N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) f(v[e], j + e);
+    for (int u = 0; u < U; ++u) load_elements(s, j + u * kThreads * N, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(v[u][e], j + u * kThreads * N + e);
   }
 }
 // ... or for all of the thread's that can still be kept, where those were set apart.
 template <class T, bool HELD, class F>
 __device__ __forceinline__ void for_kept(const Slice<T, HELD>& s, F f) {
   if (s.apart) {
-    for (int i = threadIdx.x & 31; i < s.kept_count; i += 32) {
-      const int j = HELD ? s.kept[i] : s.kept_j[i];
-      f(HELD ? s.held[j] : s.kept_x[i], j);
+    for (int i = 0; i < s.kept_count; ++i) {
+      const int j = HELD ? s.kept[i * kThreads] : s.kept_j[i * kThreads];
+      f(HELD ? s.held[j] : s.kept_x[i * kThreads], j);
     }
   } else {
     for_slice(s, f);
   }
 }
 
-// Sets apart the symbols of the bins up to `last`, each warp its own.  What follows goes over some percent of the slice, and its lanes have work.
+// Sets apart the symbols of the bins up to `last`, each thread its own.  What follows goes over some percent of the slice.
 template <class T, bool HELD>
 __device__ __forceinline__ void set_apart(Slice<T, HELD>& s, const Row& r, int last) {
-  constexpr int N = kRun<T, HELD>;
-  constexpr int kMost = HELD ? kWarpKept : kWarpCopied;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kMost = HELD ? kKept : kCopied;
   const float limit = last < kBins - 1 ? static_cast<float>(last + 1) : FLT_MAX;
   int n = 0;
-#pragma unroll(HELD ? 1 : 16 / N)
-  for (int j0 = warp * (32 * N); j0 < s.size; j0 += kThreads * N) {
-    const int j = j0 + lane * N;
-    float v[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = -INFINITY;
-    if (j < s.size) load_elements(s, j, v);
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const bool in = bin_place(r, v[e]) < limit;
-      const unsigned who = __ballot_sync(0xffffffffu, in);
-      const int at = n + __popc(who & ((1u << lane) - 1u));
-      if (in && at < kMost) {
-        if (HELD) {
-          s.kept[at] = static_cast<uint16_t>(j + e);
-        } else {
-          s.kept_x[at] = v[e];
-          s.kept_j[at] = j + e;
-        }
+  for_slice(s, [&](float x, int j) {
+    if (bin_place(r, x) < limit) {
+      const int at = min(n, kMost - 1) * kThreads;
+      if (HELD) {
+        s.kept[at] = static_cast<uint16_t>(j);
+      } else {
+        s.kept_x[at] = x;
+        s.kept_j[at] = j;
       }
-      n += __popc(who);
+      ++n;
     }
-  }
-  __syncwarp();
-  if (n <= kMost) {  // (else the warp goes over all of its part: its lanes' elements of the slice, as before)
+  });
+  if (n <= kMost) {  // (else the thread goes over all of its part, as before)
     s.apart = true;
     s.kept_count = n;
   }
@@ -637,25 +632,38 @@ __device__ __forceinline__ unsigned long long end_in_list(Shared& sh, const Row&
   return sh.list[wanted < 1.0 ? 0u : min(wanted < 4e9 ? static_cast<uint32_t>(wanted) : in, in) - 1u];
 }
 
-// The row's histogram of what is kept so far, in bins up to `last`: the blocks' in sh.count, all of it in sh.all_count.  Returns the row's sum of p where
-// `want_sum`.
+// The row's histogram of what is kept so far, in bins up to `last`: the blocks' in sh.count, all of it in sh.all_count.  Where `want_sum`, returns the row's
+// sum of p, and leaves in sh.all_mass an estimate of the bins' masses: of the first kHeavy, where a few symbols can be most of the row, from
+// their p, of the others from their numbers.
+constexpr int kHeavy = 96;  // p > 0.0025
 template <int C, class T, bool HELD>
 __device__ __forceinline__ float histogram(const Slice<T, HELD>& s, Shared& sh, const Row& r, int last, bool want_sum) {
   clear_bins(sh.count);
+  clear_bins(sh.mass);
   __syncthreads();
   float z = 0.f;
   const float limit = last < kBins - 1 ? static_cast<float>(last + 1) : FLT_MAX;
+  const int unit_bits = min(__clz(s.size), 31);  // (no overflow, should all of the slice be in one bin)
+  const float unit = __int_as_float((127 + unit_bits) << 23);
   if (r.cut == -INFINITY) {
     for_slice(s, [&](float x, int) {
       const float t = bin_place(r, x);  // (infinite for -inf)
-      if (t < limit) atomicAdd(&sh.count[whole_part(fminf(t, 255.f))], 1u);
-      if (want_sum) z += prob(r, x);
+      const float pr = prob_at(t);
+      if (t < limit) {
+        const int b = whole_part(fminf(t, 255.f));
+        atomicAdd(&sh.count[b], 1u);
+        if (want_sum && t < static_cast<float>(kHeavy)) atomicAdd(&sh.mass[b], __float2uint_rn(fminf(pr, 1.f) * unit));
+      }
+      z += pr;
     });
   } else {
     for_kept(s, [&](float x, int j) {
       if (keeps(r, x, s.first + j)) {
         const int b = bin_of(r, x);
-        if (b < kBins) atomicAdd(&sh.count[b], 1u);
+        if (b < kBins) {
+          atomicAdd(&sh.count[b], 1u);
+          if (want_sum && b < kHeavy) atomicAdd(&sh.mass[b], __float2uint_rn(fminf(prob(r, x), 1.f) * unit));
+        }
         z += prob(r, x);
       }
     });
@@ -664,25 +672,42 @@ __device__ __forceinline__ float histogram(const Slice<T, HELD>& s, Shared& sh, 
     z = block_sum(z, sh.red[0], threadIdx.x >> 5, threadIdx.x & 31, kWarps);
     if (threadIdx.x == 0) sh.out_z = z;
   }
-  merge_bins<C>(sh, true, false, [](int) { return 0.f; });
+  row_sync<C>();
+  constexpr float kMean = 0.96929f;  // of p over a bin, in units of its upper end: 16 (1 - e^(-1/16))
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    uint32_t n = 0;
+    float m = 0.f;
+#pragma unroll
+    for (int q = 0; q < C; ++q) {
+      n += C > 1 ? peer_u32(&sh.count[b], q) : sh.count[b];
+      if (want_sum && b < kHeavy) m += static_cast<float>(C > 1 ? peer_u32(&sh.mass[b], q) : sh.mass[b]);
+    }
+    sh.all_count[b] = n;
+    if (want_sum) sh.all_mass[b] = b < kHeavy ? m / unit : b < kBins - 1 ? static_cast<float>(n) * (kMean * ex2_approx(-kStep * static_cast<float>(b))) : 0.f;
+  }
+  __syncthreads();
+  if (!want_sum) return 0.f;
   z = 0.f;
 #pragma unroll
   for (int q = 0; q < C; ++q) z += C > 1 ? peer_f32(&sh.out_z, q) : sh.out_z;
   return z;
 }
 
-// The end of the prefix of the kept symbols whose number, or mass, first reaches `target`, from their histogram in bins up to `last_bin`.  Sets r.cut
-// and r.cidx.
+// False, and nothing done, where `all_bins` has to be set.
 template <int C, class T, bool HELD>
-__device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int last_bin, int rank) {
+__device__ bool find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int last_bin, bool all_bins, int rank) {
   const int tid = threadIdx.x;
-  // the bins where the end may be: of masses, a bin's symbols have p between 2^(-b kStep) and 2^(-(b + 1) kStep), but for the last bin's
+  const bool kept_before = s.apart;
+  // The bin of the end: by number it is known, by mass estimated, and two bins to either side are taken for certain, which the masses
+  // themselves confirm; else all bins are in question.
   if (tid < 32) {
     if (by_mass) {
-      const Found<float> first = first_bin<float>(0.f, static_cast<float>(target) * 0.9999f, [&](int b) {
-        return static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b));
-      });
-      if (tid == 0) sh.pick[0] = static_cast<uint32_t>(max(first.bin >= 0 ? first.bin : first.filled, 0));
+      const Found<float> f = first_bin<float>(0.f, static_cast<float>(target), [&](int b) { return static_cast<float>(sh.all_mass[b]); });
+      const bool guess = !all_bins && f.bin >= 0;
+      if (tid == 0) {
+        sh.pick[0] = static_cast<uint32_t>(guess ? max(f.bin - 2, 0) : 0);
+        sh.pick[1] = static_cast<uint32_t>(guess ? min(f.bin + 2, last_bin) : last_bin);
+      }
     } else {
       uint32_t before;
       const int b = bin_or_last(first_bin<uint32_t>(0u, static_cast<uint32_t>(target), [&](int i) { return sh.all_count[i]; }), &before);
@@ -691,15 +716,11 @@ __device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
         sh.pick_d = static_cast<double>(before);
       }
     }
-  } else if (tid < 64 && by_mass) {
-    const Found<float> last = first_bin<float>(0.f, static_cast<float>(target) * 1.0001f, [&](int b) {
-      return b < kBins - 1 ? static_cast<float>(sh.all_count[b]) * ex2_approx(-kStep * static_cast<float>(b + 1)) : 0.f;
-    });
-    if (tid == 32) sh.pick[1] = static_cast<uint32_t>(last.bin >= 0 ? last.bin : last_bin);
   }
-  clear_bins(sh.mass);
-  clear_bins(sh.fine_count);
   if (tid == 0) sh.listed = 0;
+  clear_bins(sh.fine_count);
+  row_sync<C>();  // (all have read the masses that the estimate is of)
+  clear_bins(sh.mass);
   __syncthreads();
   const int from = static_cast<int>(sh.pick[0]), to = static_cast<int>(sh.pick[1]);
   double above = sh.pick_d;
@@ -717,7 +738,7 @@ __device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
   {
     for (int b = tid & 31; b <= to; b += 32) mine += sh.count[b];
     mine = __reduce_add_sync(0xffffffffu, mine);
-    if (!s.apart && mine <= kWarps * (HELD ? kWarpKept * 3 / 4 : kWarpCopied * 7 / 8)) set_apart(s, r, to);
+    if (!s.apart && mine <= kThreads * (HELD ? kKept : kCopied) / 2) set_apart(s, r, to);
   }
   if (by_mass) {
     const float fine_step = kStep / scale;
@@ -748,7 +769,7 @@ __device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
         n += C > 1 ? peer_u32(&sh.fine_count[b], q) : sh.fine_count[b];
         m += static_cast<double>(C > 1 ? peer_u32(&sh.mass[b], q) : sh.mass[b]) * unit_of(C > 1 ? peer_u32(&sh.out_units, q) : sh.out_units);
       }
-      sh.all_count[b] = n;
+      sh.all_fine[b] = n;
       sh.all_mass[b] = m * static_cast<double>(ex2_approx(-(kStep * static_cast<float>(from) + fine_step * static_cast<float>(b))));
     }
     __syncthreads();
@@ -757,16 +778,23 @@ __device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
       above = 0.0;
 #pragma unroll
       for (int q = 0; q < C; ++q) above += static_cast<double>(C > 1 ? peer_f32(&sh.out_sure, q) : sh.out_sure);
-      const int b = bin_or_last(first_bin<double>(above, target, [&](int i) { return sh.all_mass[i]; }), &before);
+      const Found<double> f = first_bin<double>(above, target, [&](int i) { return sh.all_mass[i]; });
+      const int b = bin_or_last(f, &before);
       if (tid == 0) {
         sh.pick[2] = static_cast<uint32_t>(b);
+        sh.pick[3] = (f.bin >= 0 || to == last_bin) && (above < target || from == 0);
         sh.pick_d = before;
       }
     }
     __syncthreads();
+    if (!sh.pick[3]) {
+      s.apart = kept_before;
+      row_sync<C>();  // (all have read the bins)
+      return false;
+    }
     bin = static_cast<int>(sh.pick[2]);
     above = sh.pick_d;
-    in_bin = sh.all_count[bin];
+    in_bin = sh.all_fine[bin];
   } else {
     in_bin = sh.all_count[from];
   }
@@ -785,7 +813,7 @@ __device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
     row_sync<C>();
     r.cut = C > 1 ? peer_f32(&sh.out_cut, 0) : sh.out_cut;
     r.cidx = static_cast<int>(C > 1 ? peer_u32(&sh.out_cidx, 0) : sh.out_cidx);
-    return;
+    return true;
   }
   // the range of the bin's keys
   uint32_t lo = 0xffffffffu, hi = 0;
@@ -816,6 +844,7 @@ __device__ void find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
   }
   row_sync<C>();
   select_end<C>(s, sh, r, by_mass, target, lo, hi, above);
+  return true;
 }
 
 // The better of two candidates: the larger score, of equal ones the lower index.
@@ -865,7 +894,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
 
   Slice<T, HELD> s;
   s.row = static_cast<const T*>(p.logits) + row * p.logits_stride;
-  s.held = reinterpret_cast<float*>(smem_raw + sizeof(Shared) + kWarps * kWarpKept * sizeof(uint16_t));
+  s.held = reinterpret_cast<float*>(smem_raw + sizeof(Shared) + kThreads * kKept * sizeof(uint16_t));
   // the row's slices begin on 16-byte boundaries of memory
   const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(s.row) & 15) / sizeof(T));
   s.first = rank * p.slice - skip;
@@ -873,9 +902,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
   s.symbols = p.symbols;
   s.apart = false;
   s.kept_count = 0;
-  s.kept = reinterpret_cast<uint16_t*>(smem_raw + sizeof(Shared)) + warp * kWarpKept;
-  s.kept_x = reinterpret_cast<float*>(smem_raw + sizeof(Shared)) + warp * kWarpCopied;
-  s.kept_j = reinterpret_cast<int*>(smem_raw + sizeof(Shared)) + (kWarps + warp) * kWarpCopied;
+  s.kept = reinterpret_cast<uint16_t*>(smem_raw + sizeof(Shared)) + tid;
+  s.kept_x = reinterpret_cast<float*>(smem_raw + sizeof(Shared)) + tid;
+  s.kept_j = reinterpret_cast<int*>(smem_raw + sizeof(Shared)) + kCopied * kThreads + tid;
   const float* noise = p.noise + row * p.noise_stride;
 
   float temperature = p.temperature != nullptr ? p.temperature[row] : p.temperature0;
@@ -998,32 +1027,37 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
   }
   if (by_count) {
     histogram<C>(s, sh, r, kBins - 1, false);
-    find_end<C>(s, sh, r, false, static_cast<double>(top_k), kBins - 1, rank);
+    find_end<C>(s, sh, r, false, static_cast<double>(top_k), kBins - 1, false, rank);
   }
   if (by_mass) {
     // a symbol with p below (1 - top_p) / symbols is behind the end: all such ones together have less than 1 - top_p, the first alone has 1
     const float last = by_count ? 255.f : 16.f * logf(static_cast<float>(p.symbols) / (1.f - fmaxf(top_p, 0.f))) + 1.f;
     const int last_bin = static_cast<int>(fminf(last, 255.f));
     const float z = histogram<C>(s, sh, r, last_bin, true);
-    find_end<C>(s, sh, r, true, static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(z), last_bin, rank);
+    const double target = static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(z);
+    if (!find_end<C>(s, sh, r, true, target, last_bin, false, rank)) find_end<C>(s, sh, r, true, target, last_bin, true, rank);
   }
 
   // ---- all that is kept
-  float score = -1.f, kept = 0.f;
+  float score = 0.f, kept = 0.f;
   int idx = INT32_MAX;
   // (the noise is fetched for several at once: its latency is what this takes)
   auto weigh = [&](float x, int j) {
     const float pr = prob(r, x);
     return keeps(r, x, s.first + j) && pr >= min_p ? pr : -1.f;
   };
-  auto add = [&](float pr, float q, int j) {
+  auto add = [&](float pr, float q, int j) {  // (by rising index: of equal scores the first stays)
     if (pr >= 0.f) {
-      better(score, idx, __fdividef(pr, q), s.first + j);
+      const float sc = __fdividef(pr, q);
+      if (sc > score) {
+        score = sc;
+        idx = s.first + j;
+      }
       kept += pr;
     }
   };
   if (s.apart) {
-    for (int i = lane; i < s.kept_count; i += 32 * 4) {
+    for (int i = 0; i < s.kept_count; i += 4) {
       float pr[4], q[4];
       int j[4];
 #pragma unroll
@@ -1031,9 +1065,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
         pr[e] = -1.f;
         q[e] = 1.f;
         j[e] = 0;
-        if (i + e * 32 < s.kept_count) {
-          j[e] = HELD ? s.kept[i + e * 32] : s.kept_j[i + e * 32];
-          pr[e] = weigh(HELD ? s.held[j[e]] : s.kept_x[i + e * 32], j[e]);
+        if (i + e < s.kept_count) {
+          j[e] = HELD ? s.kept[(i + e) * kThreads] : s.kept_j[(i + e) * kThreads];
+          pr[e] = weigh(HELD ? s.held[j[e]] : s.kept_x[(i + e) * kThreads], j[e]);
         }
         if (pr[e] >= 0.f) q[e] = __ldg(noise + s.first + j[e]);
       }
@@ -1041,28 +1075,49 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
       for (int e = 0; e < 4; ++e) add(pr[e], q[e], j[e]);
     }
   } else {
-    constexpr int N = kRun<T, HELD>;
+    constexpr int N = kRun<T, HELD>, U = kRuns<T, HELD>;
     const float* mine_noise = noise + s.first;
     const bool four = (reinterpret_cast<uintptr_t>(mine_noise) & 15) == 0;
-#pragma unroll 2
-    for (int j = tid * N; j < s.size; j += kThreads * N) {
-      float x[N], q[N];
-      load_elements(s, j, x);
-      if (four && s.first + j >= 0 && s.first + j + N <= s.symbols) {
+    const bool all = r.cut == -INFINITY && !(min_p > 0.f);
+#pragma unroll 1
+    for (int j0 = tid * N; j0 < s.size; j0 += kThreads * N * U) {
+      float x[U][N], q[U][N];
 #pragma unroll
-        for (int e = 0; e < N; e += 4) {
-          const float4 f = __ldg(reinterpret_cast<const float4*>(mine_noise + j + e));
-          q[e] = f.x;
-          q[e + 1] = f.y;
-          q[e + 2] = f.z;
-          q[e + 3] = f.w;
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * kThreads * N;
+        load_elements(s, j, x[u]);
+        if (four && s.first + j >= 0 && s.first + j + N <= s.symbols && j < s.size) {
+#pragma unroll
+          for (int e = 0; e < N; e += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(mine_noise + j + e));
+            q[u][e] = f.x;
+            q[u][e + 1] = f.y;
+            q[u][e + 2] = f.z;
+            q[u][e + 3] = f.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) q[u][e] = j < s.size && s.first + j + e >= 0 && s.first + j + e < s.symbols ? __ldg(mine_noise + j + e) : 1.f;
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) q[e] = s.first + j + e >= 0 && s.first + j + e < s.symbols ? __ldg(mine_noise + j + e) : 1.f;
       }
 #pragma unroll
-      for (int e = 0; e < N; ++e) add(weigh(x[e], j + e), q[e], j + e);
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * kThreads * N;
+        if (all) {  // (-inf has p = 0, which no score is below)
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float pr = prob(r, x[u][e]), sc = __fdividef(pr, q[u][e]);
+            if (sc > score) {
+              score = sc;
+              idx = s.first + j + e;
+            }
+            kept += pr;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) add(weigh(x[u][e], j + e), q[u][e], j + e);
+        }
+      }
     }
   }
   block_best(score, idx, kept, sh);
@@ -1094,7 +1149,7 @@ template <class T, bool HELD, int C>
 int run_sample(const SampleArgs& p, int64_t rows, cudaStream_t stream) {
   static_assert(sizeof(Shared) % 16 == 0, "the slice is read four at a time");
   const size_t smem =
-      sizeof(Shared) + (HELD ? kWarps * kWarpKept * sizeof(uint16_t) + static_cast<size_t>(p.slice) * sizeof(float) : kWarps * kWarpCopied * 8);
+      sizeof(Shared) + (HELD ? kThreads * kKept * sizeof(uint16_t) + static_cast<size_t>(p.slice) * sizeof(float) : kThreads * kCopied * 8);
   static std::atomic<bool> set[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TRITURUS_B200_ELAUNCH;
@@ -1133,6 +1188,13 @@ int run_sample(const SampleArgs& p, int64_t rows, int c, cudaStream_t stream) {
 // read again from the L2 cache.
 template <class T>
 int sample_rows(SampleArgs p, int64_t rows, cudaStream_t stream) {
+  const char* env = getenv("SAMPLE_PLAN");
+  if (env != nullptr) {
+    const int cc = atoi(env) / 10, held = atoi(env) % 10;
+    const int64_t m = static_cast<int64_t>(p.symbols) + 16 / static_cast<int64_t>(sizeof(T));
+    p.slice = static_cast<int>((((m + cc - 1) / cc) + 7) / 8 * 8);
+    return held ? run_sample<T, true>(p, rows, cc, stream) : run_sample<T, false>(p, rows, cc, stream);
+  }
   const int64_t most = static_cast<int64_t>(p.symbols) + 16 / static_cast<int64_t>(sizeof(T));  // (with what lies before a 16-byte boundary)
   const int64_t sms = device_sms();
   int c = 1;
