@@ -20,7 +20,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
-#include <cstdlib>
 
 #include "../../include/triturus_b200.h"
 #include "packs.cuh"
@@ -32,9 +31,9 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 256;
-constexpr int kList = 1024;  // symbols that the first block of a row can gather
+constexpr int kList = 2048;  // symbols that the first block of a row can gather
 constexpr int kKept = 16;    // symbols of a slice in shared memory that a thread can set apart
-constexpr int kCopied = 20;  // ... and of one that is not, with their values
+constexpr int kCopied = 16;  // ... and of one that is not, with their values
 constexpr int kFew = kThreads / 2;  // a small top_k
 
 struct SampleArgs {
@@ -62,13 +61,12 @@ struct alignas(16) Shared {
   uint32_t all_count[kBins];  // the cluster's
   uint32_t fine_count[kBins];
   uint32_t all_fine[kBins];
-  unsigned long long few[33];
   float red[2][kWarps];
   int red_i[2][kWarps];
   // read by the other blocks, each written once or with a row_sync between
-  float out_top, out_z, out_sure, out_cut, out_score, out_sum;
+  float out_ref, out_top, out_z, out_sure, out_cut, out_score, out_sum;
   int out_cidx, out_idx;
-  uint32_t out_lo, out_hi, out_units;
+  uint32_t out_lo, out_hi;
   uint32_t pick[4];
   uint32_t listed;
 };
@@ -114,6 +112,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays one
 }
 
 constexpr float kStep = LOG2E_F / 16.f;  // of a bin, in powers of two of p
+constexpr float kMean = 0.96929f;        // of p over a bin, in units of its upper end: 16 (1 - e^(-1/16))
+constexpr int kHeavy = 96;               // bins of p > 0.0025, where a few symbols can be most of the row
 
 // What the blocks of a row share of it.
 struct Row {
@@ -207,6 +207,25 @@ template <class T, bool HELD>
 constexpr int kRun = HELD ? 4 : Pack<T, 16>::N;  // elements of one load
 template <class T, bool HELD>
 constexpr int kRuns = HELD ? 2 : 16 / Pack<T, 16>::N;  // loads under way: what f does may keep the compiler from starting them early
+
+// The noise of the N elements from j on; `noise` is the slice's, `four`: it begins on a 16-byte boundary.
+template <class T, bool HELD, int N>
+__device__ __forceinline__ void load_noise(const Slice<T, HELD>& s, const float* noise, bool four, int j, float (&q)[N]) {
+  const int i = s.first + j;
+  if (four && i >= 0 && i + N <= s.symbols && j < s.size) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(noise + j + e));
+      q[e] = f.x;
+      q[e + 1] = f.y;
+      q[e + 2] = f.z;
+      q[e + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[e] = j < s.size && i + e >= 0 && i + e < s.symbols ? __ldg(noise + j + e) : 1.f;
+  }
+}
 
 // f(x, j) for the thread's elements of the slice.
 template <class T, bool HELD, class F>
@@ -432,7 +451,7 @@ __device__ __forceinline__ void sorted_sums(Shared& sh, const Row& r, int have, 
 // The end of the prefix of the kept symbols whose number, or mass, with the `above` of keys above `hi`, first reaches `target`, by radix selection over
 // the keys of lo ... hi.  Sets r.cut and r.cidx.
 template <int C, class T, bool HELD>
-__device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, uint32_t lo, uint32_t hi, double above) {
+__device__ __forceinline__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, uint32_t lo, uint32_t hi, double above) {
   uint32_t ties = 0;
   for (;;) {
     const int shift = max(0, 24 - __clz(static_cast<int>(hi - lo)));  // at most 256 bins
@@ -510,8 +529,13 @@ __device__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_
   r.cut = value_of(hi);
 }
 
-// One round of radix selection over list[0 ... n), of which the places with their upper halves in lo ... hi are in question and `above` (a number or
-// mass) lies before them: narrows the range to the bin where `target` is reached.  Returns how many are in it.
+// One round of radix selection over list[0 ... n), by the upper halves of the places (the values) or, BY_INDEX, the lower ones: those in lo ... hi are in
+// question and `above` (a number or mass) lies before them; narrows the range to the bin where `target` is reached.  Returns how many are in it.
+template <bool BY_INDEX>
+__device__ __forceinline__ uint32_t half_of(unsigned long long place) {
+  return static_cast<uint32_t>(BY_INDEX ? place : place >> 32);
+}
+template <bool BY_INDEX>
 __device__ __forceinline__ uint32_t narrow_list(Shared& sh, const Row& r, int n, bool by_mass, double target, uint32_t& lo, uint32_t& hi, double& above) {
   const int shift = max(0, 24 - __clz(static_cast<int>(hi - lo)));
   clear_bins(sh.count);
@@ -519,13 +543,13 @@ __device__ __forceinline__ uint32_t narrow_list(Shared& sh, const Row& r, int n,
   __syncthreads();
   auto upper = [&](int b) { return fminf(value_of(~(lo + (static_cast<uint32_t>(b) << shift))), r.top); };
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+    const uint32_t k = half_of<BY_INDEX>(sh.list[i]);
     if (k >= lo && k <= hi) atomicAdd(&sh.count[(k - lo) >> shift], 1u);
   }
   __syncthreads();
   if (by_mass) {
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+      const uint32_t k = half_of<BY_INDEX>(sh.list[i]);
       if (k >= lo && k <= hi) {
         const int b = static_cast<int>((k - lo) >> shift);
         atomicAdd(&sh.mass[b], mass_units(ex2_approx((value_of(~k) - upper(b)) * r.k2), sh.count[b]));
@@ -551,19 +575,19 @@ __device__ __forceinline__ uint32_t narrow_list(Shared& sh, const Row& r, int n,
   __syncthreads();
   above = sh.pick_d;
   lo += sh.pick[0] << shift;
-  if (shift > 0) hi = min(hi, lo + ((1u << shift) - 1u));
-  else hi = lo;
+  hi = min(hi, lo + ((1u << shift) - 1u));
   const uint32_t in = sh.pick[1];
   __syncthreads();
   return in;
 }
 
-// The range of the upper halves of list[0 ... n).
+// The range of those halves.
+template <bool BY_INDEX>
 __device__ __forceinline__ void range_of_list(Shared& sh, int n, uint32_t& lo, uint32_t& hi) {
   lo = 0xffffffffu;
   hi = 0;
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
+    const uint32_t k = half_of<BY_INDEX>(sh.list[i]);
     lo = min(lo, k);
     hi = max(hi, k);
   }
@@ -580,62 +604,85 @@ __device__ __forceinline__ void range_of_list(Shared& sh, int n, uint32_t& lo, u
   __syncthreads();
 }
 
-// The place in list[0 ... n) where, with the `above` before the list, `target` is reached.  The list's order is lost.
+// Keeps those of list[0 ... n) whose halves are in lo ... hi; their number.  (Each thread has its own in registers meanwhile.)
+template <bool BY_INDEX>
+__device__ __forceinline__ int filter_list(Shared& sh, int n, uint32_t lo, uint32_t hi) {
+  unsigned long long mine[kPart];
+#pragma unroll
+  for (int i = 0; i < kPart; ++i) {
+    const int at = static_cast<int>(threadIdx.x) + i * kThreads;
+    mine[i] = at < n ? sh.list[at] : 0ull;
+  }
+  if (threadIdx.x == 0) sh.pick[2] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPart; ++i) {
+    const uint32_t k = half_of<BY_INDEX>(mine[i]);
+    if (static_cast<int>(threadIdx.x) + i * kThreads < n && k >= lo && k <= hi) sh.list[atomicAdd(&sh.pick[2], 1u)] = mine[i];
+  }
+  __syncthreads();
+  n = static_cast<int>(sh.pick[2]);
+  __syncthreads();
+  return n;
+}
+
+// The place in list[0 ... n) where, with the `above` before the list, `target` is reached.  The list is lost.
 __device__ __forceinline__ unsigned long long end_in_list(Shared& sh, const Row& r, int n, bool by_mass, double target, double above) {
   uint32_t lo, hi, in = static_cast<uint32_t>(n);
-  range_of_list(sh, n, lo, hi);
-  while (in > 32 && lo != hi) in = narrow_list(sh, r, n, by_mass, target, lo, hi, above);
-  // what is outside goes to the end
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint32_t k = static_cast<uint32_t>(sh.list[i] >> 32);
-    if (k < lo || k > hi) sh.list[i] = ~0ull;
+  range_of_list<false>(sh, n, lo, hi);
+  while (in > 128 && lo != hi) in = narrow_list<false>(sh, r, n, by_mass, target, lo, hi, above);
+  n = filter_list<false>(sh, n, lo, hi);
+  if (n > 128) {  // that many of one value: a number of them, by index
+    const double each = by_mass ? static_cast<double>(prob(r, value_of(~lo))) : 1.0;
+    const double wanted = each > 0.0 ? ceil((target - above) / each) : 1.0;
+    target = fmin(fmax(wanted, 1.0), static_cast<double>(n));
+    above = 0.0;
+    by_mass = false;
+    range_of_list<true>(sh, n, lo, hi);
+    while (in > 128) in = narrow_list<true>(sh, r, n, false, target, lo, hi, above);
+    n = filter_list<true>(sh, n, lo, hi);
   }
-  if (threadIdx.x == 0) sh.pick[0] = 0;
-  __syncthreads();
-  if (in <= 32) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const unsigned long long place = sh.list[i];
-      if (place != ~0ull) sh.few[atomicAdd(&sh.pick[0], 1u)] = place;
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-      const int lane = threadIdx.x, have = static_cast<int>(in);
-      const unsigned long long mine = lane < have ? sh.few[lane] : ~0ull;
-      int rank = 0;
-#pragma unroll 8
-      for (int l = 0; l < have; ++l) rank += __shfl_sync(0xffffffffu, mine, l) < mine;
-      __syncwarp();
-      if (lane < have) sh.few[rank] = mine;
-      __syncwarp();
-      int at;
-      if (by_mass) {
-        float upto = lane < have ? prob(r, value_of(~static_cast<uint32_t>(sh.few[lane] >> 32))) : 0.f;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const float f = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += f;
-        }
-        const unsigned reached = __ballot_sync(0xffffffffu, lane < have && above + static_cast<double>(upto) >= target);
-        at = reached != 0 ? __ffs(static_cast<int>(reached)) - 1 : have - 1;
-      } else {
-        at = min(max(static_cast<int>(target - above) - 1, 0), have - 1);
-      }
-      if (lane == 0) sh.few[32] = sh.few[at];
-    }
-    __syncthreads();
-    return sh.few[32];
-  }
-  // more than that of one value: by index
   sort_list(sh.list, n);
-  const double each = by_mass ? static_cast<double>(prob(r, value_of(~lo))) : 1.0;
-  const double wanted = each > 0.0 ? ceil((target - above) / each) : 1.0;
-  return sh.list[wanted < 1.0 ? 0u : min(wanted < 4e9 ? static_cast<uint32_t>(wanted) : in, in) - 1u];
+  if (by_mass) {
+    float pr[kPart], before, all;
+    sorted_sums(sh, r, n, pr, before, all);
+    if (threadIdx.x == 0) sh.pick[0] = static_cast<uint32_t>(n - 1);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPart; ++i) {
+      before += pr[i];
+      const int at = static_cast<int>(threadIdx.x) * kPart + i;
+      if (at < n && above + static_cast<double>(before) >= target) atomicMin(&sh.pick[0], static_cast<uint32_t>(at));
+    }
+    __syncthreads();
+    return sh.list[sh.pick[0]];
+  }
+  return sh.list[min(max(static_cast<int>(target - above) - 1, 0), n - 1)];
+}
+
+// The row's largest of a value of each thread, NaN where one is; `slot` is read by the other blocks.
+template <int C>
+__device__ __forceinline__ float row_max(float v, Shared& sh, float* slot) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) sh.red[0][threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = sh.red[0][0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) v = max_nan(v, sh.red[0][w]);
+  if (C > 1) {
+    if (threadIdx.x == 0) *slot = v;
+    cluster_sync_all();
+#pragma unroll
+    for (int q = 0; q < C; ++q) v = max_nan(v, peer_f32(slot, q));
+  } else {
+    __syncthreads();
+  }
+  return v;
 }
 
 // The row's histogram of what is kept so far, in bins up to `last`: the blocks' in sh.count, all of it in sh.all_count.  Where `want_sum`, returns the row's
-// sum of p, and leaves in sh.all_mass an estimate of the bins' masses: of the first kHeavy, where a few symbols can be most of the row, from
-// their p, of the others from their numbers.
-constexpr int kHeavy = 96;  // p > 0.0025
+// sum of p, and leaves in sh.all_mass an estimate of the bins' masses: of the first kHeavy from their p, of the others from their numbers.
 template <int C, class T, bool HELD>
 __device__ __forceinline__ float histogram(const Slice<T, HELD>& s, Shared& sh, const Row& r, int last, bool want_sum) {
   clear_bins(sh.count);
@@ -673,7 +720,6 @@ __device__ __forceinline__ float histogram(const Slice<T, HELD>& s, Shared& sh, 
     if (threadIdx.x == 0) sh.out_z = z;
   }
   row_sync<C>();
-  constexpr float kMean = 0.96929f;  // of p over a bin, in units of its upper end: 16 (1 - e^(-1/16))
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
     uint32_t n = 0;
     float m = 0.f;
@@ -695,7 +741,7 @@ __device__ __forceinline__ float histogram(const Slice<T, HELD>& s, Shared& sh, 
 
 // False, and nothing done, where `all_bins` has to be set.
 template <int C, class T, bool HELD>
-__device__ bool find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int last_bin, bool all_bins, int rank) {
+__device__ __forceinline__ bool find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, int last_bin, bool all_bins, int rank) {
   const int tid = threadIdx.x;
   const bool kept_before = s.apart;
   // The bin of the end: by number it is known, by mass estimated, and two bins to either side are taken for certain, which the masses
@@ -734,40 +780,44 @@ __device__ bool find_end(Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, do
     return t < static_cast<float>(to + 1) || to == kBins - 1 ? whole_part(fminf((t - static_cast<float>(from)) * scale, 255.f)) : kNoBin;
   };
   int bin = 0;
-  uint32_t in_bin, mine = 0;  // (mine: how many of the block's symbols are in the bins up to `to`)
+  uint32_t in_bin;
   {
+    uint32_t mine = 0;  // how many of the block's symbols are in the bins up to `to`
     for (int b = tid & 31; b <= to; b += 32) mine += sh.count[b];
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (!s.apart && mine <= kThreads * (HELD ? kKept : kCopied) / 2) set_apart(s, r, to);
   }
   if (by_mass) {
     const float fine_step = kStep / scale;
+    for_kept(s, [&](float x, int j) {
+      if (keeps(r, x, s.first + j)) {
+        const int b = fine_of(x);
+        if (b >= 0 && b < kBins) atomicAdd(&sh.fine_count[b], 1u);
+      }
+    });
+    __syncthreads();
     float sure = 0.f;
     for_kept(s, [&](float x, int j) {
       if (keeps(r, x, s.first + j)) {
         const int b = fine_of(x);
         const float e = (x - r.top) * r.k2;
-        if (b < 0) {
+        if (b < 0)
           sure += ex2_approx(e);
-        } else if (b < kBins) {
-          atomicAdd(&sh.fine_count[b], 1u);
-          atomicAdd(&sh.mass[b], mass_units(ex2_approx(e + (kStep * static_cast<float>(from) + fine_step * static_cast<float>(b))), mine));
-        }
+        else if (b < kBins)
+          atomicAdd(&sh.mass[b], mass_units(ex2_approx(e + (kStep * static_cast<float>(from) + fine_step * static_cast<float>(b))), sh.fine_count[b]));
       }
     });
     sure = block_sum(sure, sh.red[0], tid >> 5, tid & 31, kWarps);
-    if (tid == 0) {
-      sh.out_sure = sure;
-      sh.out_units = mine;
-    }
+    if (tid == 0) sh.out_sure = sure;
     row_sync<C>();
     for (int b = tid; b < kBins; b += kThreads) {
       uint32_t n = 0;
       double m = 0.0;
 #pragma unroll
       for (int q = 0; q < C; ++q) {
-        n += C > 1 ? peer_u32(&sh.fine_count[b], q) : sh.fine_count[b];
-        m += static_cast<double>(C > 1 ? peer_u32(&sh.mass[b], q) : sh.mass[b]) * unit_of(C > 1 ? peer_u32(&sh.out_units, q) : sh.out_units);
+        const uint32_t c = C > 1 ? peer_u32(&sh.fine_count[b], q) : sh.fine_count[b];
+        n += c;
+        m += static_cast<double>(C > 1 ? peer_u32(&sh.mass[b], q) : sh.mass[b]) * unit_of(c);
       }
       sh.all_fine[b] = n;
       sh.all_mass[b] = m * static_cast<double>(ex2_approx(-(kStep * static_cast<float>(from) + fine_step * static_cast<float>(b))));
@@ -885,7 +935,7 @@ __device__ __forceinline__ void write_answer(const SampleArgs& p, int64_t row, c
 }
 
 template <class T, bool HELD, int C>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -916,24 +966,74 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
     top_k = 1;
   }
 
-  const float mine = load_slice(s);
-  float top = mine;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) sh.red[0][warp] = top;
+  Row r;
+  r.k2 = fminf(fmaxf(LOG2E_F / temperature, 1e-38f), FLT_MAX);
+  r.to_bin = fminf(r.k2 / kStep, FLT_MAX);
+  r.cut = -INFINITY;
+  r.cidx = INT32_MIN;
+  const bool by_count = top_k > 0 && top_k < p.symbols, by_mass = top_p < 1.f;
+  // a symbol with p below (1 - top_p) / symbols is behind the end of what top_p keeps: all such ones together have less than 1 - top_p, the first
+  // alone has 1
+  const int mass_bins = by_mass && !by_count ? static_cast<int>(fminf(16.f * logf(static_cast<float>(p.symbols) / (1.f - fmaxf(top_p, 0.f))) + 1.f, 255.f)) : kBins - 1;
   if (tid == 0) sh.listed = 0;
   clear_bins(sh.count);
-  __syncthreads();
-  top = sh.red[0][0];
+  clear_bins(sh.mass);
+  float score = 0.f, kept = 0.f;  // of what is kept: the best p / noise and the sum of p
+  int idx = INT32_MAX;
+  float mine = -INFINITY, top;
+  bool scanned = false;
+  if constexpr (!HELD) {
+    // ---- Where nothing is filtered, memory is read once: p is taken in units of that of the largest of the row's first few thousand
+    // symbols, which cancels in the end.
+    if (!by_count && !by_mass && !(min_p > 0.f)) {
+      constexpr int N = kRun<T, HELD>, U = kRuns<T, HELD>;
+      float ref = -INFINITY;
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) top = max_nan(top, sh.red[0][w]);
-  if (C > 1) {
-    if (tid == 0) sh.out_top = top;
-    cluster_sync_all();
+      for (int u = 0; u < U; ++u) {
+        float v[N];
+        load_elements(s, tid * N + u * kThreads * N, v);
 #pragma unroll
-    for (int q = 0; q < C; ++q) top = max_nan(top, peer_f32(&sh.out_top, q));
-  } else {
-    __syncthreads();
+        for (int e = 0; e < N; ++e) ref = max_nan(ref, v[e]);
+      }
+      ref = row_max<C>(ref, sh, &sh.out_ref);
+      if (ref > -INFINITY && ref < FLT_MAX) {
+        r.top = ref;
+        const float* mine_noise = noise + s.first;
+        const bool four = (reinterpret_cast<uintptr_t>(mine_noise) & 15) == 0;
+#pragma unroll 1
+        for (int j0 = tid * N; j0 < s.size; j0 += kThreads * N * U) {
+          float x[U][N], q[U][N];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            load_elements(s, j0 + u * kThreads * N, x[u]);
+            load_noise(s, mine_noise, four, j0 + u * kThreads * N, q[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              const float pr = prob(r, x[u][e]), sc = __fdividef(pr, q[u][e]);
+              mine = max_nan(mine, x[u][e]);
+              kept += pr;
+              if (sc > score) {  // (-inf has p = 0, which no score is below)
+                score = sc;
+                idx = s.first + j0 + u * kThreads * N + e;
+              }
+            }
+        }
+        top = row_max<C>(mine, sh, &sh.out_top);
+        scanned = !((top - ref) * r.to_bin > 512.f);  // (else p is too large for its units)
+        if (!scanned) {
+          score = kept = 0.f;
+          idx = INT32_MAX;
+          row_sync<C>();
+        }
+      }
+    }
+  }
+  if (!scanned) {
+    mine = load_slice(s);
+    top = row_max<C>(mine, sh, &sh.out_top);
   }
   // (the same for all blocks of the row)
   if (!(top > -INFINITY)) {
@@ -950,14 +1050,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
       for (int j = tid; j < s.size; j += kThreads) s.held[j] = fminf(s.held[j], FLT_MAX);
     __syncthreads();
   }
-  Row r;
-  r.top = top;
-  r.k2 = fminf(fmaxf(LOG2E_F / temperature, 1e-38f), FLT_MAX);
-  r.to_bin = fminf(r.k2 / kStep, FLT_MAX);
-  r.cut = -INFINITY;
-  r.cidx = INT32_MIN;
-
-  const bool by_count = top_k > 0 && top_k < p.symbols, by_mass = top_p < 1.f;
+  if (!scanned) r.top = top;
   if (by_count && top_k <= kFew) {
     // ---- what is below the k-th largest of the threads' maxima is not among the first k
     const int mine_bin = bin_of(r, mine);
@@ -982,23 +1075,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
     if (listed <= kList) {
       if (rank == 0) {
         int n = gather_lists<C>(sh);
-        if (n > 128 && n <= kList / 2) {  // the first few of them, or all of the last value's
+        if (n > 128) {  // the first few of them, or all of the last value's
           uint32_t lo, hi, first;
           double above = 0.0;
-          range_of_list(sh, n, lo, hi);
+          range_of_list<false>(sh, n, lo, hi);
           first = lo;
-          narrow_list(sh, r, n, false, static_cast<double>(top_k), lo, hi, above);
-          if (tid == 0) sh.pick[2] = 0;
-          __syncthreads();
-          for (int i = tid; i < n; i += kThreads) {
-            const unsigned long long place = sh.list[i];
-            const uint32_t k = static_cast<uint32_t>(place >> 32);
-            if (k >= first && k <= hi) sh.list[kList / 2 + atomicAdd(&sh.pick[2], 1u)] = place;
-          }
-          __syncthreads();
-          n = static_cast<int>(sh.pick[2]);
-          for (int i = tid; i < n; i += kThreads) sh.list[i] = sh.list[kList / 2 + i];
-          __syncthreads();
+          narrow_list<false>(sh, r, n, false, static_cast<double>(top_k), lo, hi, above);
+          n = filter_list<false>(sh, n, first, hi);
         }
         sort_list(sh.list, n);
         const int have = min(n, top_k);
@@ -1025,22 +1108,26 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
     }
     row_sync<C>();
   }
-  if (by_count) {
-    histogram<C>(s, sh, r, kBins - 1, false);
-    find_end<C>(s, sh, r, false, static_cast<double>(top_k), kBins - 1, false, rank);
-  }
-  if (by_mass) {
-    // a symbol with p below (1 - top_p) / symbols is behind the end: all such ones together have less than 1 - top_p, the first alone has 1
-    const float last = by_count ? 255.f : 16.f * logf(static_cast<float>(p.symbols) / (1.f - fmaxf(top_p, 0.f))) + 1.f;
-    const int last_bin = static_cast<int>(fminf(last, 255.f));
-    const float z = histogram<C>(s, sh, r, last_bin, true);
-    const double target = static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(z);
-    if (!find_end<C>(s, sh, r, true, target, last_bin, false, rank)) find_end<C>(s, sh, r, true, target, last_bin, true, rank);
+  // ---- the ends of what top_k keeps, then of what top_p does
+  bool count_next = by_count, mass_next = by_mass, all_bins = false;
+  double target = 0.0;
+#pragma unroll 1
+  while (count_next || mass_next) {
+    const bool mass = !count_next;
+    const int last_bin = mass ? mass_bins : kBins - 1;
+    if (!all_bins) {
+      const float z = histogram<C>(s, sh, r, last_bin, mass);
+      target = mass ? static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(z) : static_cast<double>(top_k);
+    }
+    if (find_end<C>(s, sh, r, mass, target, last_bin, all_bins, rank)) {
+      if (mass) mass_next = false;
+      count_next = false;
+    } else {
+      all_bins = true;
+    }
   }
 
   // ---- all that is kept
-  float score = 0.f, kept = 0.f;
-  int idx = INT32_MAX;
   // (the noise is fetched for several at once: its latency is what this takes)
   auto weigh = [&](float x, int j) {
     const float pr = prob(r, x);
@@ -1056,7 +1143,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
       kept += pr;
     }
   };
-  if (s.apart) {
+  if (scanned) {
+    // (done above)
+  } else if (s.apart) {
     for (int i = 0; i < s.kept_count; i += 4) {
       float pr[4], q[4];
       int j[4];
@@ -1086,19 +1175,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs p) {
       for (int u = 0; u < U; ++u) {
         const int j = j0 + u * kThreads * N;
         load_elements(s, j, x[u]);
-        if (four && s.first + j >= 0 && s.first + j + N <= s.symbols && j < s.size) {
-#pragma unroll
-          for (int e = 0; e < N; e += 4) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(mine_noise + j + e));
-            q[u][e] = f.x;
-            q[u][e + 1] = f.y;
-            q[u][e + 2] = f.z;
-            q[u][e + 3] = f.w;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < N; ++e) q[u][e] = j < s.size && s.first + j + e >= 0 && s.first + j + e < s.symbols ? __ldg(mine_noise + j + e) : 1.f;
-        }
+        load_noise(s, mine_noise, four, j, q[u]);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -1188,13 +1265,6 @@ int run_sample(const SampleArgs& p, int64_t rows, int c, cudaStream_t stream) {
 // read again from the L2 cache.
 template <class T>
 int sample_rows(SampleArgs p, int64_t rows, cudaStream_t stream) {
-  const char* env = getenv("SAMPLE_PLAN");
-  if (env != nullptr) {
-    const int cc = atoi(env) / 10, held = atoi(env) % 10;
-    const int64_t m = static_cast<int64_t>(p.symbols) + 16 / static_cast<int64_t>(sizeof(T));
-    p.slice = static_cast<int>((((m + cc - 1) / cc) + 7) / 8 * 8);
-    return held ? run_sample<T, true>(p, rows, cc, stream) : run_sample<T, false>(p, rows, cc, stream);
-  }
   const int64_t most = static_cast<int64_t>(p.symbols) + 16 / static_cast<int64_t>(sizeof(T));  // (with what lies before a 16-byte boundary)
   const int64_t sms = device_sms();
   int c = 1;
