@@ -718,9 +718,9 @@ def _layer_norm_backward_impl(
     mean, rstd = mean.contiguous(), rstd.contiguous()
     weight = None if weight is None else weight.contiguous()
     code = _TYPE_CODES[x.dtype]
-    ws_bytes = int(LIB.triturus_b200_layer_norm_backward_workspace_bytes(mean.numel(), D, code))
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
     with _on_device(x.device) as idx:
+        ws_bytes = int(LIB.triturus_b200_layer_norm_backward_workspace_bytes(mean.numel(), D, code))
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=x.device)
         rc = LIB.triturus_b200_layer_norm_backward(
             dy_rows.data_ptr(), x_rows.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
             _ptr(dweight) if weight_grad else None, _ptr(dbias) if bias_grad else None, mean.numel(), D, dy_stride, x_stride,

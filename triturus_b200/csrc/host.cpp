@@ -282,12 +282,13 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   c10::SmallVector<int, 64> types;
   c10::SmallVector<const at::Tensor*, 64> tensors;
   c10::SmallVector<std::pair<uintptr_t, uintptr_t>, 64> ranges;
-  const auto device = c10::cuda::current_device();
+  c10::DeviceIndex device = -1;
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* o = PySequence_Fast_GET_ITEM(args[0], i);
     if (o == Py_None) continue;
     const at::Tensor* t = plain_object(o);
     const int type = t != nullptr ? type_code(*t) : -1;
+    if (t != nullptr && device < 0) device = c10::cuda::current_device();  // (not asked where there is no GPU)
     if (type < 0 || t->get_device() != device || !t->is_non_overlapping_and_dense() || (scale && t->requires_grad())) return none();
     void* p = const_cast<void*>(t->const_data_ptr());
     const uintptr_t at = reinterpret_cast<uintptr_t>(p);
