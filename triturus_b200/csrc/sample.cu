@@ -7,16 +7,25 @@
 // For exponential noise the largest p / noise falls on i with probability p_i / sum p.  No place on a cumulative sum decides, and so no order
 // of additions: what is kept is a prefix of the sorted row, and only its end depends on sums.
 //
-// A row belongs to a cluster of blocks, each of which holds its slice in shared memory.  No row is sorted.
+// A row belongs to a cluster of up to eight blocks with a slice each, held in shared memory or, where that is too little, read again from the L2 cache.
+// No row is sorted.
+//
+// Nothing filtered: one pass over logits and noise (200 x 10007 in float32 8.2 us a call; 256 x 131072 86 us = 3.1 TB/s).
 //
 // A small top_k: a block's own symbols below the k-th largest of its threads' maxima cannot be among the row's first k; what remains, some
-// tens of symbols of each block, the first block gathers, sorts and finishes alone.
+// tens of symbols of each block, the first block gathers, sorts and finishes alone (1 x 32768, top_k 50 and top_p 0.9: 11.5 us a call, 9.3 of the
+// GPU, half a dozen steps that wait for each other).
 //
-// Else the end of the kept prefix is found from a histogram of (max - x) / T in steps of 1/16, a factor of 1.06 of p: the counts alone give the bin
-// where a number of symbols is reached, and bounds of the bins where a mass is; the masses are then added for the bins between the bounds only.  The
-// symbols of the one bin that is left are gathered and sorted; where they are too many (flat rows, many equal values), the end is
-// found among them by radix selection over the bits of x and then over the index.  Counts and, as multiples of a power of two, masses are added as
-// integers, so that a result does not depend on the order of the atomic additions.
+// Else the end of the kept prefix is found from a histogram of (max - x) / T in steps of 1/16, a factor of 1.06 of p.  The numbers in its bins give the
+// bin where a number of symbols is reached, and an estimate of the one where a mass is; the masses are then added in fine steps around
+// that, and have to confirm the estimate.  The threads set apart the few percent that can still be kept, so that only these are gone over from
+// there on.  The symbols of the one fine bin that is left are gathered and narrowed down; where they are too many for that (flat rows), the end is found
+// by radix selection over the bits of x and then over the index.  Numbers and, as multiples of a power of two, masses are added as integers, so
+// that a result does not depend on the order of the atomic additions.
+//
+// 256 x 131072 in float32 with top_p 0.95 takes 146 us, seven times what reading the logits does: three passes over each row (maximum,
+// histogram, setting apart) of 11, 21 and 11 us to a wave of 148 rows, the first two thirds of what an L2 cache pass costs at best, and some
+// 15 us of steps that wait for the cluster; the instructions of the histogram bound its pass (ncu: issue 47 %, DRAM 16 %).
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
