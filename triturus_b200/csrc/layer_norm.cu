@@ -48,7 +48,6 @@ struct NormArgs {
 // comes as the 4-byte word that it is a half of.
 template <class T, int BYTES>
 struct alignas(BYTES < 4 ? 4 : BYTES) Slot {
-  static constexpr int N = BYTES / static_cast<int>(sizeof(T));
   Pack<T, (BYTES < 4 ? 4 : BYTES)> p;
   // `half`: the address's second bit
   __device__ __forceinline__ float get(int e, int half) const { return to_float(BYTES < 4 ? (half ? p.v[1] : p.v[0]) : p.v[e]); }

@@ -24,8 +24,8 @@
 // that a result does not depend on the order of the atomic additions.
 //
 // 256 x 131072 in float32 with top_p 0.95 takes 146 us, seven times what reading the logits does: three passes over each row (maximum,
-// histogram, setting apart) of 11, 21 and 11 us to a wave of 148 rows, the first two thirds of what an L2 cache pass costs at best, and some
-// 15 us of steps that wait for the cluster; the instructions of the histogram bound its pass (ncu: issue 47 %, DRAM 16 %).
+// histogram, setting apart) of 11, 21 and 11 us to a wave of 148 rows, where 11 is what the L2 cache takes to hand out so much, and some 15 us of
+// steps that wait for the cluster; the instructions of the histogram bound its pass (ncu: issue 47 %, DRAM 16 %).
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -947,7 +947,7 @@ template <class T, bool HELD, int C>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x;
   const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int64_t row = blockIdx.x / C;
 
