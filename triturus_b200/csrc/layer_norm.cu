@@ -54,11 +54,13 @@ struct alignas(BYTES < 4 ? 4 : BYTES) Slot {
 };
 // ... from global to shared memory without a register.
 template <int BYTES>
-__device__ __forceinline__ void fetch(void* dst, const void* src) {
+__device__ __forceinline__ void fetch(uint32_t dst, const void* src) {
   if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else if constexpr (BYTES == 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(3)) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(3)) : "memory");
 }
 __device__ __forceinline__ int half_of(const void* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1; }
 __device__ __forceinline__ void wait_for_row(int stages) {
@@ -273,14 +275,16 @@ __global__ void __launch_bounds__(BLOCK, NV * Pack<T, BYTES>::N > 16 ? 1 : BLOCK
   const D d(t, p.width);
   using S = Slot<T, BYTES>;
   S* const ring = reinterpret_cast<S*>(smem) + threadIdx.x;
+  const uint32_t ring_at = smem_u32(ring);
   const float inv = 1.f / static_cast<float>(p.width);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + group, step = static_cast<int64_t>(gridDim.x) * kGroups;
   auto ask = [&](int64_t row, int stage) {
     if (row < p.rows) {
       const T* x = static_cast<const T*>(p.x) + row * p.x_stride + d.first_column;
+      const uint32_t at = ring_at + stage * (NV * BLOCK * static_cast<int>(sizeof(S)));
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (d.has(i)) fetch<BYTES>(&ring[(stage * NV + i) * BLOCK], x + i * TH * D::N);
+        if (d.has(i)) fetch<BYTES>(at + i * BLOCK * static_cast<int>(sizeof(S)), x + i * TH * D::N);
     }
     cp_async_commit();
   };
@@ -388,17 +392,19 @@ __global__ void __launch_bounds__(kBack) norm_backward_kernel(const NormArgs p) 
   const D d(t, p.width);
   using S = Slot<T, BYTES>;
   S* const ring = reinterpret_cast<S*>(smem) + threadIdx.x;
+  const uint32_t ring_at = smem_u32(ring);
   const float inv = 1.f / static_cast<float>(p.width);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + group, step = static_cast<int64_t>(gridDim.x) * kGroups;
   auto ask = [&](int64_t row, int stage) {
     if (row < p.rows) {
       const T* x = static_cast<const T*>(p.x) + row * p.x_stride + d.first_column;
       const T* dy = static_cast<const T*>(p.dy) + row * p.dy_stride + d.first_column;
+      const uint32_t at = ring_at + stage * (2 * NV * kBack * static_cast<int>(sizeof(S)));
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (d.has(i)) {
-          fetch<BYTES>(&ring[(stage * 2 * NV + i) * kBack], x + i * TH * D::N);
-          fetch<BYTES>(&ring[(stage * 2 * NV + NV + i) * kBack], dy + i * TH * D::N);
+          fetch<BYTES>(at + i * kBack * static_cast<int>(sizeof(S)), x + i * TH * D::N);
+          fetch<BYTES>(at + (NV + i) * kBack * static_cast<int>(sizeof(S)), dy + i * TH * D::N);
         }
     }
     cp_async_commit();
