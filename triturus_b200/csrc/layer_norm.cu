@@ -53,14 +53,25 @@ struct alignas(BYTES < 4 ? 4 : BYTES) Slot {
   __device__ __forceinline__ float get(int e, int half) const { return to_float(BYTES < 4 ? (half ? p.v[1] : p.v[0]) : p.v[e]); }
 };
 // ... from global to shared memory without a register.
+// (`read`: the bytes that are read of 4, the others are zero.)
 template <int BYTES>
-__device__ __forceinline__ void fetch(uint32_t dst, const void* src) {
+__device__ __forceinline__ void fetch(uint32_t dst, const void* src, uint32_t read) {
   if constexpr (BYTES == 16)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else if constexpr (BYTES == 4)
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(3)) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(read) : "memory");
+}
+// For BYTES < 4, the same for all of a thread's elements of a row: where their words begin, and what is read of them.  Of a word whose first half is the
+// element no more than that is read: the tensor may end there.  One whose second half it is begins inside the allocation, which begins on a larger
+// boundary.
+template <int BYTES, class T>
+__device__ __forceinline__ uint32_t to_words(const T*& row) {
+  if constexpr (BYTES >= 4) return 4;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row);
+  row = reinterpret_cast<const T*>(at & ~static_cast<uintptr_t>(3));
+  return 2u + static_cast<uint32_t>(at & 2);
 }
 __device__ __forceinline__ int half_of(const void* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1; }
 __device__ __forceinline__ void wait_for_row(int stages) {
@@ -281,10 +292,11 @@ __global__ void __launch_bounds__(BLOCK, NV * Pack<T, BYTES>::N > 16 ? 1 : BLOCK
   auto ask = [&](int64_t row, int stage) {
     if (row < p.rows) {
       const T* x = static_cast<const T*>(p.x) + row * p.x_stride + d.first_column;
+      const uint32_t x_read = to_words<BYTES>(x);
       const uint32_t at = ring_at + stage * (NV * BLOCK * static_cast<int>(sizeof(S)));
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (d.has(i)) fetch<BYTES>(at + i * BLOCK * static_cast<int>(sizeof(S)), x + i * TH * D::N);
+        if (d.has(i)) fetch<BYTES>(at + i * BLOCK * static_cast<int>(sizeof(S)), x + i * TH * D::N, x_read);
     }
     cp_async_commit();
   };
@@ -399,12 +411,13 @@ __global__ void __launch_bounds__(kBack) norm_backward_kernel(const NormArgs p) 
     if (row < p.rows) {
       const T* x = static_cast<const T*>(p.x) + row * p.x_stride + d.first_column;
       const T* dy = static_cast<const T*>(p.dy) + row * p.dy_stride + d.first_column;
+      const uint32_t x_read = to_words<BYTES>(x), dy_read = to_words<BYTES>(dy);
       const uint32_t at = ring_at + stage * (2 * NV * kBack * static_cast<int>(sizeof(S)));
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (d.has(i)) {
-          fetch<BYTES>(at + i * kBack * static_cast<int>(sizeof(S)), x + i * TH * D::N);
-          fetch<BYTES>(at + (NV + i) * kBack * static_cast<int>(sizeof(S)), dy + i * TH * D::N);
+          fetch<BYTES>(at + i * kBack * static_cast<int>(sizeof(S)), x + i * TH * D::N, x_read);
+          fetch<BYTES>(at + (NV + i) * kBack * static_cast<int>(sizeof(S)), dy + i * TH * D::N, dy_read);
         }
     }
     cp_async_commit();
