@@ -31,6 +31,7 @@
 #include <cfloat>
 
 #include "../../include/triturus_b200.h"
+#include "key_range.cuh"
 #include "packs.cuh"
 #include "ptx.cuh"
 
@@ -462,8 +463,10 @@ __device__ __forceinline__ void sorted_sums(Shared& sh, const Row& r, int have, 
 template <int C, class T, bool HELD>
 __device__ __forceinline__ void select_end(const Slice<T, HELD>& s, Shared& sh, Row& r, bool by_mass, double target, uint32_t lo, uint32_t hi, double above) {
   uint32_t ties = 0;
-  for (;;) {
-    const int shift = max(0, 24 - __clz(static_cast<int>(hi - lo)));  // at most 256 bins
+#pragma unroll 1
+  for (int round = 0; round < kKeyRounds; ++round) {
+    const KeyRange range = {lo, hi};
+    const int shift = range.shift();
     clear_bins(sh.count);
     clear_bins(sh.mass);
     __syncthreads();
@@ -497,8 +500,9 @@ __device__ __forceinline__ void select_end(const Slice<T, HELD>& s, Shared& sh, 
     const uint32_t b = sh.pick[0];
     ties = sh.pick[1];
     above = sh.pick_d;
-    hi -= b << shift;
-    lo = max(lo, hi - ((1u << shift) - 1u));
+    const KeyRange left = range.bin_downwards(b, shift);
+    lo = left.lo;
+    hi = left.hi;
     row_sync<C>();  // (all have read the bins)
     if (shift == 0) break;
   }
@@ -546,7 +550,8 @@ __device__ __forceinline__ uint32_t half_of(unsigned long long place) {
 }
 template <bool BY_INDEX>
 __device__ __forceinline__ uint32_t narrow_list(Shared& sh, const Row& r, int n, bool by_mass, double target, uint32_t& lo, uint32_t& hi, double& above) {
-  const int shift = max(0, 24 - __clz(static_cast<int>(hi - lo)));
+  const KeyRange range = {lo, hi};
+  const int shift = range.shift();
   clear_bins(sh.count);
   clear_bins(sh.mass);
   __syncthreads();
@@ -583,8 +588,9 @@ __device__ __forceinline__ uint32_t narrow_list(Shared& sh, const Row& r, int n,
   }
   __syncthreads();
   above = sh.pick_d;
-  lo += sh.pick[0] << shift;
-  hi = min(hi, lo + ((1u << shift) - 1u));
+  const KeyRange left = range.bin_upwards(sh.pick[0], shift);
+  lo = left.lo;
+  hi = left.hi;
   const uint32_t in = sh.pick[1];
   __syncthreads();
   return in;
