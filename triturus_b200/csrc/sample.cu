@@ -367,6 +367,9 @@ __device__ __forceinline__ Found<V> first_bin(V start, V target, F value) {
   f.before_filled = __shfl_sync(0xffffffffu, f.before_filled, last);
   return f;
 }
+// The mass of a bin with `count` symbols.  What lies far enough below the top has p = 0 in 32 bits, but is something all the same: a bin that is empty
+// must not be taken for the end.
+__device__ __forceinline__ double mass_of(double mass, uint32_t count) { return count == 0 ? 0.0 : fmax(mass, 1e-300); }
 // ... and the last one with something where none reaches it: the sums were rounded on two ways.
 template <class V>
 __device__ __forceinline__ int bin_or_last(const Found<V>& f, V* before) {
@@ -489,7 +492,8 @@ __device__ __forceinline__ void select_end(const Slice<T, HELD>& s, Shared& sh, 
     if (threadIdx.x < 32) {
       double before;
       const int b = bin_or_last(
-          first_bin<double>(above, target, [&](int i) { return by_mass ? sh.all_mass[i] : static_cast<double>(sh.all_count[i]); }), &before);
+          first_bin<double>(above, target, [&](int i) { return by_mass ? mass_of(sh.all_mass[i], sh.all_count[i]) : static_cast<double>(sh.all_count[i]); }),
+          &before);
       if (threadIdx.x == 0) {
         sh.pick[0] = static_cast<uint32_t>(b);
         sh.pick[1] = sh.all_count[b];
@@ -575,9 +579,8 @@ __device__ __forceinline__ uint32_t narrow_list(Shared& sh, const Row& r, int n,
     double before;
     const int b = bin_or_last(first_bin<double>(above, target, [&](int i) {
                                 const uint32_t c = sh.count[i];
-                                return !by_mass ? static_cast<double>(c)
-                                       : c == 0 ? 0.0
-                                                : static_cast<double>(sh.mass[i]) * unit_of(c) * static_cast<double>(prob(r, upper(i)));
+                                if (!by_mass || c == 0) return static_cast<double>(c);
+                                return mass_of(static_cast<double>(sh.mass[i]) * unit_of(c) * static_cast<double>(prob(r, upper(i))), c);
                               }),
                               &before);
     if (threadIdx.x == 0) {
@@ -641,8 +644,10 @@ __device__ __forceinline__ int filter_list(Shared& sh, int n, uint32_t lo, uint3
   return n;
 }
 
-// The place in list[0 ... n) where, with the `above` before the list, `target` is reached.  The list is lost.
+// The place in list[0 ... n) where, with the `above` before the list, `target` is reached.  The list is lost.  (n > 0, as the list is that of a bin
+// with something; behind an empty one all is kept.)
 __device__ __forceinline__ unsigned long long end_in_list(Shared& sh, const Row& r, int n, bool by_mass, double target, double above) {
+  if (n == 0) return place_of(-INFINITY, INT32_MAX);
   uint32_t lo, hi, in = static_cast<uint32_t>(n);
   range_of_list<false>(sh, n, lo, hi);
   while (in > 128 && lo != hi) in = narrow_list<false>(sh, r, n, by_mass, target, lo, hi, above);
@@ -843,7 +848,7 @@ __device__ __forceinline__ bool find_end(Slice<T, HELD>& s, Shared& sh, Row& r, 
       above = 0.0;
 #pragma unroll
       for (int q = 0; q < C; ++q) above += static_cast<double>(C > 1 ? peer_f32(&sh.out_sure, q) : sh.out_sure);
-      const Found<double> f = first_bin<double>(above, target, [&](int i) { return sh.all_mass[i]; });
+      const Found<double> f = first_bin<double>(above, target, [&](int i) { return mass_of(sh.all_mass[i], sh.all_fine[i]); });
       const int b = bin_or_last(f, &before);
       if (tid == 0) {
         sh.pick[2] = static_cast<uint32_t>(b);
