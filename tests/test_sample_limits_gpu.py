@@ -1,0 +1,23 @@
+"""GPU: sample on rows around the limits of its kernels' forms, against the definition of test_sample_gpu."""
+
+import pytest
+import torch
+
+from test_sample_gpu import BF16, F16, F32, check, inputs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("symbols", [384_312, 384_316, 384_317, 384_325, 390_000, 393_208, 393_212, 393_217])
+def test_longest_rows_in_shared_memory(symbols, kind):
+    """Eight blocks with 48040 symbols each fill the shared memory that a block can have; longer rows are read again."""
+    x, q = inputs(1, symbols, kind)
+    check(x, q)
+    check(x, q, top_k=40)
+    check(x, q, top_p=0.9)
+
+
+def test_longest_rows_of_a_batch():
+    x, q = inputs(18, 390_000)
+    check(x, q, top_k=20, top_p=0.7, temperature=0.6)

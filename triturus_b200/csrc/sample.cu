@@ -43,6 +43,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 256;
 constexpr int kList = 2048;  // symbols that the first block of a row can gather
 constexpr int kKept = 16;    // symbols of a slice in shared memory that a thread can set apart
+constexpr size_t kKeptBytes = kThreads * kKept * sizeof(uint16_t);
 constexpr int kCopied = 16;  // ... and of one that is not, with their values
 constexpr int kFew = kThreads / 2;  // a small top_k
 
@@ -964,7 +965,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p)
 
   Slice<T, HELD> s;
   s.row = static_cast<const T*>(p.logits) + row * p.logits_stride;
-  s.held = reinterpret_cast<float*>(smem_raw + sizeof(Shared) + kThreads * kKept * sizeof(uint16_t));
+  s.held = reinterpret_cast<float*>(smem_raw + sizeof(Shared) + kKeptBytes);
   // the row's slices begin on 16-byte boundaries of memory
   const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(s.row) & 15) / sizeof(T));
   s.first = rank * p.slice - skip;
@@ -1239,19 +1240,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p)
 
 // ----------------------------------------------------------------------------- launches
 
-constexpr int kMostHeld = 48 * 1024;  // symbols of a slice that shared memory holds
-constexpr int kMostShared = 227 * 1024;
+constexpr size_t kMostShared = 227 * 1024;
+constexpr int kMostHeld = (kMostShared - sizeof(Shared) - kKeptBytes) / sizeof(float) / 8 * 8;  // symbols of a slice that shared memory holds
+static_assert(kMostHeld <= 1 << 16, "their numbers have 16 bits");
+constexpr size_t shared_bytes(bool held, int slice) {
+  return sizeof(Shared) + (held ? kKeptBytes + static_cast<size_t>(slice) * sizeof(float) : kThreads * kCopied * 8);
+}
+static_assert(shared_bytes(true, kMostHeld) <= kMostShared && shared_bytes(false, 0) <= kMostShared, "");
 
 template <class T, bool HELD, int C>
 int run_sample(const SampleArgs& p, int64_t rows, cudaStream_t stream) {
   static_assert(sizeof(Shared) % 16 == 0, "the slice is read four at a time");
-  const size_t smem =
-      sizeof(Shared) + (HELD ? kThreads * kKept * sizeof(uint16_t) + static_cast<size_t>(p.slice) * sizeof(float) : kThreads * kCopied * 8);
+  const size_t smem = shared_bytes(HELD, p.slice);
   static std::atomic<bool> set[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TRITURUS_B200_ELAUNCH;
   if (!set[dev]) {
-    if (cudaFuncSetAttribute(sample_kernel<T, HELD, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess)
+    if (cudaFuncSetAttribute(sample_kernel<T, HELD, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostShared)) != cudaSuccess)
       return TRITURUS_B200_ELAUNCH;
     set[dev] = true;
   }
