@@ -280,7 +280,7 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   c10::SmallVector<void*, 64> data;
   c10::SmallVector<int64_t, 64> numels;
   c10::SmallVector<int, 64> types;
-  c10::SmallVector<const at::Tensor*, 64> tensors;
+  c10::SmallVector<at::Tensor, 64> tensors;  // held: while other Python threads run, the list may lose its own
   c10::SmallVector<std::pair<uintptr_t, uintptr_t>, 64> ranges;
   c10::DeviceIndex device = -1;
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -295,7 +295,7 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     data.push_back(p);
     numels.push_back(t->numel());
     types.push_back(type);
-    tensors.push_back(t);
+    tensors.push_back(*t);
     if (scale) ranges.emplace_back(at, at + t->numel() * t->element_size());
   }
   if (tensors.empty()) return none();
@@ -304,8 +304,8 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (ranges[i].first < ranges[i - 1].second) return none();
   const int64_t count = static_cast<int64_t>(tensors.size());
   const size_t bytes = triturus_b200_clip_grad_norm_workspace_bytes(count);
-  at::Tensor norm = empty_on(*tensors[0], {}, at::kFloat);
-  at::Tensor ws = empty_on(*tensors[0], {static_cast<int64_t>(bytes / 8)}, at::kDouble);
+  at::Tensor norm = empty_on(tensors[0], {}, at::kFloat);
+  at::Tensor ws = empty_on(tensors[0], {static_cast<int64_t>(bytes / 8)}, at::kDouble);
   float* np = norm.mutable_data_ptr<float>();
   const auto stream = c10::cuda::getCurrentCUDAStream(device).stream();
   int rc;
@@ -316,8 +316,8 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   if (rc != TRITURUS_B200_OK) return failed("triturus_b200_clip_grad_norm", rc);
   if (scale)
-    for (const at::Tensor* t : tensors)
-      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    for (const at::Tensor& t : tensors)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   return THPVariable_Wrap(std::move(norm));
   END_HANDLE_TH_ERRORS
 }
