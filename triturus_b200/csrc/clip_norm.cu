@@ -371,39 +371,16 @@ bool fill_list(TensorList<MOST>* l, void* const* data, const int64_t* numels, co
   return chunks <= INT64_C(0x7fffffff);
 }
 
-template <int MOST, class Kern, class... More>
-bool launch(Kern kern, int blocks, bool dependent, cudaStream_t stream, const TensorList<MOST>& l, const ClipArgs& p, More... more) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = dependent ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, l, p, more...) == cudaSuccess;
-}
-
 template <int C>
 int run_small(const TensorList<64>& l, const ClipArgs& p, int scale, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(C, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = C > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, clip_small_kernel<C>, l, p, scale) == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+  const cudaLaunchAttribute cluster = cluster_of(C);
+  return launch_of(clip_small_kernel<C>, dim3(C), kThreads, 0, stream, C > 1 ? &cluster : nullptr, l, p, scale);
 }
 
 template <int MOST>
 int run_clip(void* const* data, const int64_t* numels, const int* types, int64_t count, ClipArgs p, int scale, cudaStream_t stream) {
   const int64_t lists = std::max<int64_t>(1, (count + MOST - 1) / MOST);
+  const cudaLaunchAttribute dependent = dependent_launch();
   TensorList<MOST> l;
   p.sums_in_all = 0;
   for (int64_t i = 0; i < lists; ++i) {
@@ -415,7 +392,9 @@ int run_clip(void* const* data, const int64_t* numels, const int* types, int64_t
     p.sums_here = p.sums_in_all;
     const int blocks = blocks_for(l.chunks);
     p.sums_in_all += blocks;
-    if (blocks > 0 && !launch<MOST>(norm_parts_kernel<MOST>, blocks, false, stream, l, p)) return TRITURUS_B200_ELAUNCH;
+    if (blocks == 0) continue;
+    const int rc = launch_of(norm_parts_kernel<MOST>, dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream, nullptr, l, p);
+    if (rc != TRITURUS_B200_OK) return rc;
   }
   for (int64_t i = 0; i < (scale ? lists : 1); ++i) {
     if (lists > 1 && !fill_list(&l, data, numels, types, i * MOST, std::min(count, (i + 1) * MOST))) return TRITURUS_B200_EINVAL;
@@ -423,7 +402,8 @@ int run_clip(void* const* data, const int64_t* numels, const int* types, int64_t
     const int blocks = scale ? std::max(1, blocks_for(l.chunks)) : 1;
     const int work = scale && l.chunks > 0;
     if (i > 0 && !work) continue;
-    if (!launch<MOST>(clip_kernel<MOST>, blocks, true, stream, l, p, work)) return TRITURUS_B200_ELAUNCH;
+    const int rc = launch_of(clip_kernel<MOST>, dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream, &dependent, l, p, work);
+    if (rc != TRITURUS_B200_OK) return rc;
   }
   return TRITURUS_B200_OK;
 }

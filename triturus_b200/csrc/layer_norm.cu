@@ -613,11 +613,11 @@ constexpr int kEach = 16;  // elements of a thread, twice that in the longest ro
 template <class Kern>
 int blocks_of_sm(Kern kern, std::atomic<int> (&known)[64], int threads, size_t smem) {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (code_of(cudaGetDevice(&dev)) != TRITURUS_B200_OK || dev < 0 || dev >= 64) return 0;
   int n = known[dev].load(std::memory_order_relaxed);
   if (n == 0) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n <= 0) return 0;
+    if (code_of(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared)) != TRITURUS_B200_OK) return 0;
+    if (code_of(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem)) != TRITURUS_B200_OK || n <= 0) return 0;
     known[dev].store(n, std::memory_order_relaxed);
   }
   return n;
@@ -640,8 +640,7 @@ int run_forward(NormArgs p, cudaStream_t stream) {
   if (fit == 0) return TRITURUS_B200_ELAUNCH;
   const int64_t blocks = std::min<int64_t>((p.rows + kGroups - 1) / kGroups, static_cast<int64_t>(device_sms()) * fit);
   p.stages = stages_of(stages, p.rows, blocks * kGroups);
-  kern<<<static_cast<unsigned>(blocks), BLOCK, p.stages * row_bytes, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+  return launch_of(kern, dim3(static_cast<unsigned>(blocks)), BLOCK, p.stages * row_bytes, stream, nullptr, p);
 }
 
 // Blocks of the backward pass: each has a share of dw and db to write and to be added.
@@ -658,8 +657,7 @@ int run_backward(NormArgs p, int* blocks, cudaStream_t stream) {
   if (blocks_of_sm(kern, known, kBack, std::max(stages * row_bytes, sums)) == 0) return TRITURUS_B200_ELAUNCH;
   *blocks = static_cast<int>(std::min<int64_t>((p.rows + kGroups - 1) / kGroups, device_sms()));
   p.stages = stages_of(stages, p.rows, static_cast<int64_t>(*blocks) * kGroups);
-  kern<<<static_cast<unsigned>(*blocks), kBack, std::max(p.stages * row_bytes, sums), stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+  return launch_of(kern, dim3(static_cast<unsigned>(*blocks)), kBack, std::max(p.stages * row_bytes, sums), stream, nullptr, p);
 }
 
 // run(NV, TH) as constants: the fewest threads that hold a row with kEach elements each.
@@ -688,8 +686,7 @@ template <class T>
 int forward(const NormArgs& p, cudaStream_t stream) {
   constexpr int SIZE = static_cast<int>(sizeof(T));
   if (p.width > kLongest) {
-    norm_forward_long_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(p.rows, device_sms() * 2)), 1024, 0, stream>>>(p);
-    return cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+    return launch_of(norm_forward_long_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(p.rows, device_sms() * 2))), 1024, 0, stream, nullptr, p);
   }
   const int bytes = std::min(vector_bytes(p.x, p.x_stride, p.rows, p.width, SIZE), vector_bytes(p.y, p.width, p.rows, p.width, SIZE));
   return by_bytes<T>(bytes, [&](auto b) {
@@ -699,18 +696,9 @@ int forward(const NormArgs& p, cudaStream_t stream) {
 
 template <class W>
 int run_reduce(const NormArgs& p, void* dweight, void* dbias, int blocks, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.width + 31) / 32), 2, 1);
-  cfg.blockDim = dim3(512, 1, 1);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, norm_reduce_kernel<W>, p.part, static_cast<W*>(dweight), static_cast<W*>(dbias), blocks, p.width) == cudaSuccess
-             ? TRITURUS_B200_OK
-             : TRITURUS_B200_ELAUNCH;
+  const cudaLaunchAttribute dependent = dependent_launch();
+  return launch_of(norm_reduce_kernel<W>, dim3(static_cast<unsigned>((p.width + 31) / 32), 2), 512, 0, stream, &dependent, p.part, static_cast<W*>(dweight),
+                   static_cast<W*>(dbias), blocks, p.width);
 }
 
 template <class T>
@@ -719,9 +707,10 @@ int backward(const NormArgs& p, void* dweight, void* dbias, cudaStream_t stream)
   int blocks = 0, rc;
   if (p.width > kLongest) {
     blocks = most_shares(std::min<int64_t>(p.rows, 64));
-    norm_backward_long_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(p.rows, device_sms() * 2)), 1024, 0, stream>>>(p);
-    norm_backward_columns_kernel<T><<<dim3(static_cast<unsigned>((p.width + 255) / 256), static_cast<unsigned>(blocks)), 256, 0, stream>>>(p);
-    rc = cudaGetLastError() == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+    rc = launch_of(norm_backward_long_kernel<T>, dim3(static_cast<unsigned>(std::min<int64_t>(p.rows, device_sms() * 2))), 1024, 0, stream, nullptr, p);
+    if (rc == TRITURUS_B200_OK)
+      rc = launch_of(norm_backward_columns_kernel<T>, dim3(static_cast<unsigned>((p.width + 255) / 256), static_cast<unsigned>(blocks)), 256, 0, stream,
+                     nullptr, p);
   } else {
     const int bytes = std::min({vector_bytes(p.x, p.x_stride, p.rows, p.width, SIZE), vector_bytes(p.dy, p.dy_stride, p.rows, p.width, SIZE),
                                 vector_bytes(p.y, p.width, p.rows, p.width, SIZE)});
@@ -787,7 +776,10 @@ int triturus_b200_layer_norm_backward(const void* dy, const void* x, const void*
   const int size = size_of(type);
   if (rows == 0) {  // sums over no rows
     for (void* d : {dweight, dbias})
-      if (d != nullptr && cudaMemsetAsync(d, 0, static_cast<size_t>(width) * size_of(weight_type), st) != cudaSuccess) return TRITURUS_B200_ELAUNCH;
+      if (d != nullptr) {
+        const int rc = code_of(cudaMemsetAsync(d, 0, static_cast<size_t>(width) * size_of(weight_type), st));
+        if (rc != TRITURUS_B200_OK) return rc;
+      }
     return TRITURUS_B200_OK;
   }
   if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || dx == nullptr || workspace == nullptr) return TRITURUS_B200_EINVAL;

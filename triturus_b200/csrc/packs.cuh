@@ -1,5 +1,5 @@
 // What the kernels of the operators around the contractions share: vectors of 32- or 16-bit floats moved as one access,
-// reductions over a block in a fixed order, and the SM count.
+// reductions over a block in a fixed order, launches, and the SM count.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -7,7 +7,43 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/triturus_b200.h"
+
 namespace tb200 {
+
+// The library's code for a CUDA call.  CUDA keeps an error until it is asked for: one that is reported here is not left for
+// a later call to find.
+inline int code_of(cudaError_t rc) {
+  if (rc == cudaSuccess) return TRITURUS_B200_OK;
+  cudaGetLastError();
+  return TRITURUS_B200_ELAUNCH;
+}
+// A launch whose own error is returned, and no earlier one that was left.
+template <class... Params, class... Args>
+int launch_of(void (*kern)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const cudaLaunchAttribute* attribute, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = const_cast<cudaLaunchAttribute*>(attribute);
+  cfg.numAttrs = attribute != nullptr ? 1 : 0;
+  return code_of(cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...));
+}
+inline cudaLaunchAttribute dependent_launch() {
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  return at;
+}
+inline cudaLaunchAttribute cluster_of(int blocks) {
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = static_cast<unsigned>(blocks);
+  at.val.clusterDim.y = 1;
+  at.val.clusterDim.z = 1;
+  return at;
+}
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -52,10 +88,10 @@ __device__ __forceinline__ float block_sum(float v, float* part, int warp, int l
 inline int device_sms() {
   static int sms[64] = {};
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (code_of(cudaGetDevice(&dev)) != TRITURUS_B200_OK || dev < 0 || dev >= 64) return 148;
   if (sms[dev] == 0) {
     int n = 0;
-    sms[dev] = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
+    sms[dev] = code_of(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev)) == TRITURUS_B200_OK && n > 0 ? n : 148;
   }
   return sms[dev];
 }

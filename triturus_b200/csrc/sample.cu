@@ -1254,25 +1254,14 @@ int run_sample(const SampleArgs& p, int64_t rows, cudaStream_t stream) {
   const size_t smem = shared_bytes(HELD, p.slice);
   static std::atomic<bool> set[64];
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TRITURUS_B200_ELAUNCH;
+  if (code_of(cudaGetDevice(&dev)) != TRITURUS_B200_OK || dev < 0 || dev >= 64) return TRITURUS_B200_ELAUNCH;
   if (!set[dev]) {
-    if (cudaFuncSetAttribute(sample_kernel<T, HELD, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostShared)) != cudaSuccess)
-      return TRITURUS_B200_ELAUNCH;
+    const int rc = code_of(cudaFuncSetAttribute(sample_kernel<T, HELD, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostShared)));
+    if (rc != TRITURUS_B200_OK) return rc;
     set[dev] = true;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * C), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = C > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T, HELD, C>, p) == cudaSuccess ? TRITURUS_B200_OK : TRITURUS_B200_ELAUNCH;
+  const cudaLaunchAttribute cluster = cluster_of(C);
+  return launch_of(sample_kernel<T, HELD, C>, dim3(static_cast<unsigned>(rows * C)), kThreads, smem, stream, C > 1 ? &cluster : nullptr, p);
 }
 
 template <class T, bool HELD>
