@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import triturus_b200 as tb
 from test_sample_gpu import BF16, F16, F32, check, inputs
 
 pytestmark = pytest.mark.gpu
@@ -21,3 +22,15 @@ def test_longest_rows_in_shared_memory(symbols, kind):
 def test_longest_rows_of_a_batch():
     x, q = inputs(18, 390_000)
     check(x, q, top_k=20, top_p=0.7, temperature=0.6)
+
+
+def test_nan_in_long_rows_at_any_temperature():
+    x, q = inputs(200, 40_000)
+    x[7, 123] = float("nan")
+    x[9, 39_999] = float("nan")
+    x[11, 20_000] = float("inf")
+    for temperature in (1.0, 1e30, 1e38, 3e38):
+        token, logprob = tb.sample(x, q, temperature=temperature, return_logprob=True)
+        for i in (7, 9):
+            assert int(token[i]) == -1 and bool(logprob[i].isnan())
+        assert int((token < 0).sum()) == 2 and int(logprob.isnan().sum()) == 2

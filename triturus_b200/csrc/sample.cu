@@ -122,6 +122,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays one
   return r;
 }
 
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 constexpr float kStep = LOG2E_F / 16.f;  // of a bin, in powers of two of p
 constexpr float kMean = 0.96929f;        // of p over a bin, in units of its upper end: 16 (1 - e^(-1/16))
 constexpr int kHeavy = 96;               // bins of p > 0.0025, where a few symbols can be most of the row
@@ -161,7 +167,7 @@ struct Slice {
   __device__ __forceinline__ float at(int j) const {
     if (HELD) return held[j];
     const int i = first + j;
-    return i < 0 || i >= symbols ? -INFINITY : fminf(to_float(row[i]), FLT_MAX);
+    return i < 0 || i >= symbols ? -INFINITY : min_nan(to_float(row[i]), FLT_MAX);
   }
 };
 
@@ -199,7 +205,7 @@ __device__ __forceinline__ void load_elements(const Slice<T, false>& s, int j, f
   if (i >= 0 && i + N <= s.symbols && j < s.size) {
     const Pack<T, 16> p = *reinterpret_cast<const Pack<T, 16>*>(s.row + i);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = fminf(to_float(p.v[e]), FLT_MAX);
+    for (int e = 0; e < N; ++e) v[e] = min_nan(to_float(p.v[e]), FLT_MAX);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = j < s.size ? s.at(j + e) : -INFINITY;
