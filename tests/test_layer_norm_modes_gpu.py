@@ -1,0 +1,31 @@
+"""GPU: layer_norm through autograd: gradients in a type of their own."""
+
+import pytest
+import torch
+
+import triturus_b200 as tb
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows,width", [(50, 200), (700, 33), (3, 20_000)])
+def test_gradient_of_a_wide_bias_without_a_weight(rows, width, kind):
+    """A bias in 32 bits has a gradient in 32 bits: a sum of `rows` terms one by one, (rows + 64) u of their magnitudes, and no rounding
+    to the 16 bits of x."""
+    g = torch.Generator().manual_seed(rows + width)
+    x = torch.randn(rows, width, generator=g).to(kind).cuda()
+    dy = torch.randn(rows, width, generator=g).to(kind).cuda()
+    terms = dy.double().cpu()
+    bound = (rows + 64) * U * terms.abs().sum(0) + 1e-37
+    for call in (lambda bias: tb.layer_norm(x, None, bias), lambda bias: torch.ops.triturus.layer_norm(x, None, bias, 1e-5)[0]):
+        bias = torch.randn(width, generator=g).cuda().requires_grad_()
+        (grad,) = torch.autograd.grad(call(bias), bias, dy)
+        assert grad.dtype == torch.float32
+        assert bool(((grad.double().cpu() - terms.sum(0)).abs() <= bound).all())
+    leaf = x.clone().requires_grad_()
+    dx, db = torch.autograd.grad(tb.layer_norm(leaf, None, bias), (leaf, bias), dy)
+    _, mean, rstd = tb.layer_norm(x, None, bias.detach(), return_stats=True)
+    assert torch.equal(dx, tb.layer_norm_backward(dy, x, mean, rstd)[0]) and torch.equal(db, grad)

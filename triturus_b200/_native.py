@@ -705,13 +705,18 @@ def _layer_norm_impl(
     return y, mean, rstd
 
 
+def _gradient_type(x: torch.Tensor, weight: torch.Tensor | None, wide: bool) -> torch.dtype:
+    return weight.dtype if weight is not None else torch.float32 if wide else x.dtype
+
+
 def _layer_norm_backward_impl(
-    dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None, weight_grad: bool, bias_grad: bool
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """dweight and dbias that are not wanted are empty tensors."""
+    dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None, weight_grad: bool, bias_grad: bool,
+    wide: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:  # fmt: skip
+    """dweight and dbias that are not wanted are empty tensors.  They are of weight's type; without a weight, of x's or, `wide`, float32 ones."""
     _require_cuda(x)
     D = x.shape[-1]
-    kind = x.dtype if weight is None else weight.dtype
+    kind = _gradient_type(x, weight, wide)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dweight, dbias = (torch.empty((D if want else 0,), dtype=kind, device=x.device) for want in (weight_grad, bias_grad))
     (dy_rows, dy_stride), (x_rows, x_stride) = _rows(dy), _rows(x)
@@ -743,8 +748,8 @@ def _layer_norm_fake(x, weight, bias, eps):
 
 
 @layer_norm_backward_op.register_fake
-def _layer_norm_backward_fake(dy, x, mean, rstd, weight, weight_grad, bias_grad):
-    kind = x.dtype if weight is None else weight.dtype
+def _layer_norm_backward_fake(dy, x, mean, rstd, weight, weight_grad, bias_grad, wide=False):
+    kind = _gradient_type(x, weight, wide)
     return x.new_empty(x.shape), *(x.new_empty((x.shape[-1] if want else 0,), dtype=kind) for want in (weight_grad, bias_grad))
 
 

@@ -104,9 +104,8 @@ class _LayerNorm(torch.autograd.Function):
 
 def _gradients(ctx, dy, x, mean, rstd, weight, impl):
     need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
-    dx, dweight, dbias = impl(dy, x, mean, rstd, weight, need_weight, need_bias)
-    if need_bias and dbias.dtype != ctx.bias_type:  # (a bias in 32 bits without a weight to say so)
-        dbias = dbias.to(ctx.bias_type)
+    wide = ctx.bias_type == torch.float32  # (a bias in 32 bits, without a weight to say so)
+    dx, dweight, dbias = impl(dy, x, mean, rstd, weight, need_weight, need_bias, wide)
     return dx if need_x else None, dweight if need_weight else None, dbias if need_bias else None
 
 
