@@ -1,13 +1,33 @@
-"""GPU: layer_norm through autograd: gradients in a type of their own."""
+"""GPU: layer_norm under the modes of differentiation, and gradients in a type of their own."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 import triturus_b200 as tb
 
 pytestmark = pytest.mark.gpu
 
 U = 2.0**-24
+
+
+def test_forward_mode_is_refused():
+    """There is no forward-mode derivative: a call that asks for one fails, and does not give a result without a tangent."""
+    x, w, b = torch.randn(5, 24, device="cuda"), torch.ones(24, device="cuda"), torch.zeros(24, device="cuda")
+    want = tb.layer_norm(x, w, b)
+    with fw.dual_level():
+        for i in range(3):
+            for view in (False, True):
+                given = [x, w, b]
+                given[i] = fw.make_dual(given[i], torch.ones_like(given[i]))
+                if view:
+                    given[i] = given[i].view_as(given[i])
+                with pytest.raises(NotImplementedError):
+                    tb.layer_norm(*given)
+                with torch.no_grad(), pytest.raises(NotImplementedError):
+                    tb.layer_norm(*given, return_stats=True)
+        assert torch.equal(tb.layer_norm(x, w, b), want)  # (in a dual level, with ordinary tensors)
+    assert torch.equal(tb.layer_norm(x, w, b), want)
 
 
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])

@@ -194,6 +194,9 @@ PyObject* tuple3(at::Tensor* a, at::Tensor* b, at::Tensor* c) {
   return out;
 }
 
+// A tensor of forward-mode differentiation, which looks like any other.
+bool has_tangent(const at::Tensor* t) { return t != nullptr && t->_fw_grad(0).defined(); }
+
 // layer_norm(x, weight, bias, eps, return_stats)
 PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -206,6 +209,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   int weight_type = -1;
   if (type < 0 || stride < 0 || !weight_arg(args[1], *x, width, &weight, &weight_type) || !weight_arg(args[2], *x, width, &bias, &weight_type))
     return none();
+  if (has_tangent(x) || has_tangent(weight) || has_tangent(bias)) return none();  // (refused there)
   const bool stats = args[4] == Py_True;
   at::Tensor y = empty_on(*x, x->sizes(), x->scalar_type()), mean, rstd;
   float *mp = nullptr, *rp = nullptr;

@@ -36,7 +36,8 @@ def layer_norm(
     weight and bias [D] are optional and float32 or of x's type, both the same.  The sums are in 32 bits whatever x's type; y has x's
     type and shape and is contiguous.  x may have any strides: rows of consecutive elements at one distance are read in
     place, other views are copied first.  `return_stats=True` returns (y, mean, rstd) with float32 statistics of shape x.shape[:-1],
-    which `layer_norm_backward` takes.  Differentiable in x, weight and bias (once)."""
+    which `layer_norm_backward` takes.  y is differentiable in x, weight and bias, once and backwards; a tensor with a forward-mode
+    tangent is refused."""
     if not torch.compiler.is_compiling() and not (
         torch.is_grad_enabled()
         and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))
