@@ -49,3 +49,22 @@ def test_gradient_of_a_wide_bias_without_a_weight(rows, width, kind):
     dx, db = torch.autograd.grad(tb.layer_norm(leaf, None, bias), (leaf, bias), dy)
     _, mean, rstd = tb.layer_norm(x, None, bias.detach(), return_stats=True)
     assert torch.equal(dx, tb.layer_norm_backward(dy, x, mean, rstd)[0]) and torch.equal(db, grad)
+
+
+def test_statistics_have_no_gradient():
+    """In the registered operator, and where it is compiled, as in the function: a loss of y and the statistics has y's gradient alone, and
+    the statistics say so."""
+    x = torch.randn(6, 40, device="cuda")
+    dy = torch.randn(6, 40, device="cuda")
+
+    def stats(t):
+        return tb.layer_norm(t, return_stats=True)
+
+    want = None
+    for call in (stats, lambda t: torch.ops.triturus.layer_norm(t, None, None, 1e-5), torch.compile(stats, backend="aot_eager", fullgraph=True)):
+        leaf = x.clone().requires_grad_()
+        y, mean, rstd = call(leaf)
+        assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
+        (grad,) = torch.autograd.grad((y * dy).sum() + mean.sum() + rstd.sum(), leaf)
+        want = grad if want is None else want
+        assert torch.equal(grad, want)

@@ -113,6 +113,7 @@ def _gradients(ctx, dy, x, mean, rstd, weight, impl):
 def _setup_context(ctx, inputs, output):
     x, weight, bias, _eps = inputs
     _y, mean, rstd = output
+    ctx.mark_non_differentiable(mean, rstd)
     ctx.save_for_backward(x, mean, rstd, weight)
     ctx.bias_type = None if bias is None else bias.dtype
 
