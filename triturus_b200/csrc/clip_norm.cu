@@ -134,23 +134,29 @@ __device__ __forceinline__ void for_vectors(const Bits& b, F f) {
     f(x);
   }
 }
+// What the elements are multiplied by: c, then unit.  A factor below the least normal number has no 24 digits of its own; it is held in units of
+// 2^-126, else unit is 1.
+struct Factor {
+  float c, unit;
+  __device__ __forceinline__ bool one() const { return c == 1.f; }
+};
 template <class T>
-__device__ __forceinline__ void scale_bits(Bits& b, float c) {
+__device__ __forceinline__ void scale_bits(Bits& b, Factor f) {
   constexpr int N = Pack<T, 16>::N;
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
     Pack<T, 16>& p = *reinterpret_cast<Pack<T, 16>*>(&b.v[i]);
 #pragma unroll
-    for (int e = 0; e < N; ++e) p.v[e] = from_float<T>(to_float(p.v[e]) * c);
+    for (int e = 0; e < N; ++e) p.v[e] = from_float<T>(to_float(p.v[e]) * f.c * f.unit);
   }
 }
-__device__ __forceinline__ void scale_bits(Bits& b, int type, float c) {
+__device__ __forceinline__ void scale_bits(Bits& b, int type, Factor f) {
   if (type == TRITURUS_B200_TYPE_F32)
-    scale_bits<float>(b, c);
+    scale_bits<float>(b, f);
   else if (type == TRITURUS_B200_TYPE_BF16)
-    scale_bits<__nv_bfloat16>(b, c);
+    scale_bits<__nv_bfloat16>(b, f);
   else
-    scale_bits<__half>(b, c);
+    scale_bits<__half>(b, f);
 }
 
 // Adds the squares of a chunk's elements.  A vector's squares are added in 32 bits where they neither overflow nor lose digits
@@ -214,11 +220,13 @@ __device__ __forceinline__ double block_combine(double v, double* part, bool lar
 }
 
 // The norm and the factor from the sum of all, for thread 0.
-__device__ __forceinline__ float factor_of(const ClipArgs& p, double sum, float* norm) {
+__device__ __forceinline__ Factor factor_of(const ClipArgs& p, double sum, float* norm) {
   const double n = p.largest ? sum : sqrt(sum);
   *norm = static_cast<float>(n);
   // (a norm beyond 32 bits still has its factor; a NaN among the elements makes all of them NaN)
-  return n + 1e-6 <= p.limit ? 1.f : static_cast<float>(p.limit / (n + 1e-6));
+  if (n + 1e-6 <= p.limit) return {1.f, 1.f};
+  const double c = p.limit / (n + 1e-6);
+  return c < 0x1p-126 ? Factor{static_cast<float>(c * 0x1p126), 0x1p-126f} : Factor{static_cast<float>(c), 1.f};
 }
 
 // The block's run of chunks.
@@ -259,7 +267,7 @@ __global__ void __launch_bounds__(kThreads) norm_parts_kernel(const __grid_const
 template <int MOST>
 __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ TensorList<MOST> l, const ClipArgs p, int scale) {
   __shared__ double part[kThreads / 32];
-  __shared__ float factor;
+  __shared__ Factor factor;
   const uint32_t begin = run_start(l.chunks, blockIdx.x, gridDim.x);
   Cursor at = {0, 0};
   Chunk k = {};
@@ -279,8 +287,8 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
     if (blockIdx.x == 0 && p.sums_here == 0) *p.norm = n;
   }
   __syncthreads();
-  const float c = factor;
-  if (!scale || c == 1.f) return;
+  const Factor c = factor;
+  if (!scale || c.one()) return;
   for (;;) {
     const Chunk here = k;
     Bits next;
@@ -304,7 +312,7 @@ template <int C>
 __global__ void __launch_bounds__(kThreads) clip_small_kernel(const __grid_constant__ TensorList<64> l, const ClipArgs p, int scale) {
   __shared__ double part[kThreads / 32];
   __shared__ double block_sum;
-  __shared__ float factor;
+  __shared__ Factor factor;
   Chunk k[kHeld];
   Bits held[kHeld];
 #pragma unroll
@@ -336,8 +344,8 @@ __global__ void __launch_bounds__(kThreads) clip_small_kernel(const __grid_const
     if (blockIdx.x == 0) *p.norm = n;
   }
   __syncthreads();
-  const float c = factor;
-  if (scale && c != 1.f) {
+  const Factor c = factor;
+  if (scale && !c.one()) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
       if (blockIdx.x + i * C < l.chunks) {
