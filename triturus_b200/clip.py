@@ -6,6 +6,7 @@ import math
 from collections.abc import Iterable
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native
 
@@ -31,6 +32,8 @@ def _checked(name: str, grads: torch.Tensor | Iterable[torch.Tensor | None], nor
         assert g.device == grads[0].device
         if in_place and g.requires_grad:
             raise ValueError(f"{name}: a gradient that requires a gradient itself cannot be clipped in place")
+        if in_place and not torch.compiler.is_compiling() and unpack_dual(g).tangent is not None:
+            raise ValueError(f"{name}: a gradient with a forward-mode tangent cannot be clipped in place")
         if in_place and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
             raise ValueError(f"{name}: an expanded tensor cannot be clipped in place")
     _native._require_cuda(*grads)

@@ -293,7 +293,7 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const at::Tensor* t = plain_object(o);
     const int type = t != nullptr ? type_code(*t) : -1;
     if (t != nullptr && device < 0) device = c10::cuda::current_device();  // (not asked where there is no GPU)
-    if (type < 0 || t->get_device() != device || !t->is_non_overlapping_and_dense() || (scale && t->requires_grad())) return none();
+    if (type < 0 || t->get_device() != device || !t->is_non_overlapping_and_dense() || (scale && (t->requires_grad() || has_tangent(t)))) return none();
     void* p = const_cast<void*>(t->const_data_ptr());
     const uintptr_t at = reinterpret_cast<uintptr_t>(p);
     data.push_back(p);
