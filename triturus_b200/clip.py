@@ -37,7 +37,7 @@ def _checked(name: str, grads: torch.Tensor | Iterable[torch.Tensor | None], nor
         if in_place and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
             raise ValueError(f"{name}: an expanded tensor cannot be clipped in place")
     _native._require_cuda(*grads)
-    if in_place:
+    if in_place and not torch.compiler.is_compiling():  # (tensors that are traced have no addresses)
         ranges = sorted((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()) for g in grads if g.numel() and _dense(g))
         if any(first[1] > second[0] for first, second in zip(ranges, ranges[1:])):
             raise ValueError(f"{name}: gradients that share memory cannot be clipped in place")
