@@ -1,4 +1,4 @@
-"""GPU: the registered operators, compiled, do what the functions of the package do."""
+"""GPU: the registered operators, called by themselves and compiled, check and do what the functions of the package do."""
 
 import pytest
 import torch
@@ -6,6 +6,33 @@ import torch
 import triturus_b200 as tb
 
 pytestmark = pytest.mark.gpu
+
+OPS = torch.ops.triturus
+
+
+def test_arguments_are_checked():
+    x, w = torch.randn(4, 32, device="cuda"), torch.ones(32, device="cuda")
+    q, lead = torch.rand(4, 32, device="cuda"), torch.ones(4, device="cuda")
+    for call in (
+        lambda: OPS.layer_norm(x, w[:31], None, 1e-5),
+        lambda: OPS.layer_norm(x.bfloat16(), w, w.bfloat16(), 1e-5),
+        lambda: OPS.layer_norm(x, w.cpu(), None, 1e-5),
+        lambda: OPS.layer_norm_backward(x, x, lead[:3], lead, None, True, True),
+        lambda: OPS.layer_norm_backward(x[:, :31], x, lead, lead, None, True, True),
+        lambda: OPS.grad_norm([x.double()], False),
+        lambda: OPS.sample(x, q[:3], None, 1.0, None, 0, None, 1.0, None, 0.0),
+        lambda: OPS.sample(x, q.half(), None, 1.0, None, 0, None, 1.0, None, 0.0),
+        lambda: OPS.sample(x, q, lead[:2], 1.0, None, 0, None, 1.0, None, 0.0),
+    ):
+        with pytest.raises(AssertionError):
+            call()
+    for call, what in (
+        (lambda: OPS.clip_grad_norm_([x, x[1:]], 1.0, False), "share memory"),
+        (lambda: OPS.clip_grad_norm_([x[:1].expand(4, 32)], 1.0, False), "expanded"),
+        (lambda: OPS.layer_norm(torch.empty(3, 0, device="cuda"), None, None, 1e-5), "no elements"),
+    ):
+        with pytest.raises(ValueError, match=what):
+            call()
 
 
 def test_compiled_calls():

@@ -735,20 +735,44 @@ def _layer_norm_backward_impl(
     return dx, dweight, dbias
 
 
-layer_norm_op = torch.library.custom_op("triturus::layer_norm", _layer_norm_impl, mutates_args=(), device_types="cuda")
-layer_norm_backward_op = torch.library.custom_op(
-    "triturus::layer_norm_backward", _layer_norm_backward_impl, mutates_args=(), device_types="cuda"
-)
+# The registered operators are called by themselves too: they check what the functions of the package check.
+
+
+@torch.library.custom_op("triturus::layer_norm", mutates_args=(), device_types="cuda")
+def layer_norm_op(
+    x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from .norm import _check as check
+
+    check(x, weight, bias)
+    return _layer_norm_impl(x, weight, bias, eps)
+
+
+@torch.library.custom_op("triturus::layer_norm_backward", mutates_args=(), device_types="cuda")
+def layer_norm_backward_op(
+    dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None, weight_grad: bool, bias_grad: bool,
+    wide: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:  # fmt: skip
+    from .norm import _check_backward
+
+    _check_backward(dy, x, mean, rstd, weight)
+    return _layer_norm_backward_impl(dy, x, mean, rstd, weight, weight_grad, bias_grad, wide)
 
 
 @layer_norm_op.register_fake
 def _layer_norm_fake(x, weight, bias, eps):
+    from .norm import _check as check
+
+    check(x, weight, bias)
     stats = x.new_empty(x.shape[:-1], dtype=torch.float32)
     return x.new_empty(x.shape), stats, torch.empty_like(stats)
 
 
 @layer_norm_backward_op.register_fake
 def _layer_norm_backward_fake(dy, x, mean, rstd, weight, weight_grad, bias_grad, wide=False):
+    from .norm import _check_backward
+
+    _check_backward(dy, x, mean, rstd, weight)
     kind = _gradient_type(x, weight, wide)
     return x.new_empty(x.shape), *(x.new_empty((x.shape[-1] if want else 0,), dtype=kind) for want in (weight_grad, bias_grad))
 
@@ -795,17 +819,35 @@ def _grad_norm_impl(grads: list[torch.Tensor], largest: bool) -> torch.Tensor:
     return _norm_of([g if _is_dense(g) else g.contiguous() for g in grads], 0.0, largest, False)
 
 
-clip_grad_norm_op = torch.library.custom_op("triturus::clip_grad_norm_", _clip_grad_norm_impl, mutates_args=("grads",), device_types="cuda")
-grad_norm_op = torch.library.custom_op("triturus::grad_norm", _grad_norm_impl, mutates_args=(), device_types="cuda")
+@torch.library.custom_op("triturus::clip_grad_norm_", mutates_args=("grads",), device_types="cuda")
+def clip_grad_norm_op(grads: list[torch.Tensor], max_norm: float, largest: bool) -> torch.Tensor:
+    from .clip import _check as check
+
+    check("clip_grad_norm_", grads, True, True)
+    return _clip_grad_norm_impl(grads, max_norm, largest)
+
+
+@torch.library.custom_op("triturus::grad_norm", mutates_args=(), device_types="cuda")
+def grad_norm_op(grads: list[torch.Tensor], largest: bool) -> torch.Tensor:
+    from .clip import _check as check
+
+    check("grad_norm", grads, False, True)
+    return _grad_norm_impl(grads, largest)
 
 
 @clip_grad_norm_op.register_fake
 def _clip_grad_norm_fake(grads, max_norm, largest):
+    from .clip import _check as check
+
+    check("clip_grad_norm_", grads, True, False)
     return grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device="cuda")
 
 
 @grad_norm_op.register_fake
 def _grad_norm_fake(grads, largest):
+    from .clip import _check as check
+
+    check("grad_norm", grads, False, False)
     return grads[0].new_empty((), dtype=torch.float32) if grads else torch.empty((), device="cuda")
 
 
@@ -833,9 +875,24 @@ def _sample_impl(
     return token, logprob
 
 
-sample_op = torch.library.custom_op("triturus::sample", _sample_impl, mutates_args=(), device_types="cuda")
+@torch.library.custom_op("triturus::sample", mutates_args=(), device_types="cuda")
+def sample_op(
+    logits: torch.Tensor, noise: torch.Tensor, temperature: torch.Tensor | None, temperature0: float, top_k: torch.Tensor | None, top_k0: int,
+    top_p: torch.Tensor | None, top_p0: float, min_p: torch.Tensor | None, min_p0: float,
+) -> tuple[torch.Tensor, torch.Tensor]:  # fmt: skip
+    from .sample import _check as check
+    from .sample import _check_device
+
+    check(logits, noise, temperature, top_k, top_p, min_p)
+    _check_device(logits)
+    return _sample_impl(logits, noise, temperature, temperature0, top_k, top_k0, top_p, top_p0, min_p, min_p0)
 
 
 @sample_op.register_fake
 def _sample_fake(logits, noise, temperature, temperature0, top_k, top_k0, top_p, top_p0, min_p, min_p0):
+    from .sample import _check as check
+    from .sample import _check_device
+
+    check(logits, noise, temperature, top_k, top_p, min_p)
+    _check_device(logits)
     return logits.new_empty(logits.shape[:-1], dtype=torch.int64), logits.new_empty(logits.shape[:-1], dtype=torch.float32)

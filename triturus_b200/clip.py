@@ -23,24 +23,31 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _check(name: str, grads: list[torch.Tensor], in_place: bool, memory: bool) -> None:
+    """`memory`: the tensors have some, whose places are compared."""
+    for g in grads:
+        assert g.dtype in _TYPES
+        assert g.device == grads[0].device
+        if in_place and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+            raise ValueError(f"{name}: an expanded tensor cannot be clipped in place")
+    _native._require_cuda(*grads)
+    if in_place and memory:
+        ranges = sorted((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()) for g in grads if g.numel() and _dense(g))
+        if any(first[1] > second[0] for first, second in zip(ranges, ranges[1:])):
+            raise ValueError(f"{name}: gradients that share memory cannot be clipped in place")
+
+
 def _checked(name: str, grads: torch.Tensor | Iterable[torch.Tensor | None], norm_type: float, in_place: bool) -> tuple[list[torch.Tensor], bool]:
     grads = [grads] if isinstance(grads, torch.Tensor) else [g for g in grads if g is not None]
     if norm_type not in (2, math.inf):
         raise ValueError(f"{name}: norm_type is 2 or infinity, got {norm_type!r}")
-    for g in grads:
-        assert g.dtype in _TYPES
-        assert g.device == grads[0].device
-        if in_place and g.requires_grad:
-            raise ValueError(f"{name}: a gradient that requires a gradient itself cannot be clipped in place")
-        if in_place and not torch.compiler.is_compiling() and unpack_dual(g).tangent is not None:
-            raise ValueError(f"{name}: a gradient with a forward-mode tangent cannot be clipped in place")
-        if in_place and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
-            raise ValueError(f"{name}: an expanded tensor cannot be clipped in place")
-    _native._require_cuda(*grads)
-    if in_place and not torch.compiler.is_compiling():  # (tensors that are traced have no addresses)
-        ranges = sorted((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()) for g in grads if g.numel() and _dense(g))
-        if any(first[1] > second[0] for first, second in zip(ranges, ranges[1:])):
-            raise ValueError(f"{name}: gradients that share memory cannot be clipped in place")
+    if in_place:
+        for g in grads:
+            if g.requires_grad:
+                raise ValueError(f"{name}: a gradient that requires a gradient itself cannot be clipped in place")
+            if not torch.compiler.is_compiling() and unpack_dual(g).tangent is not None:
+                raise ValueError(f"{name}: a gradient with a forward-mode tangent cannot be clipped in place")
+    _check(name, grads, in_place, not torch.compiler.is_compiling())
     return grads, norm_type != 2
 
 

@@ -9,6 +9,24 @@ from . import _native
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
+def _check(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None) -> None:
+    assert len(x.shape) >= 1
+    assert x.dtype in _TYPES
+    _check_weights("layer_norm", x, weight, bias)
+    _native._require_cuda(x)
+
+
+def _check_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None) -> None:
+    assert len(x.shape) >= 1
+    assert x.dtype in _TYPES
+    assert dy.shape == x.shape and dy.dtype == x.dtype
+    assert mean.shape == rstd.shape == x.shape[:-1]
+    assert mean.dtype == rstd.dtype == torch.float32
+    assert dy.device == x.device == mean.device == rstd.device
+    _check_weights("layer_norm_backward", x, weight)
+    _native._require_cuda(x)
+
+
 def _check_weights(name: str, x: torch.Tensor, *weights: torch.Tensor | None) -> None:
     kinds = set()
     for t in weights:
@@ -45,10 +63,7 @@ def layer_norm(
         out = _native.HOST.layer_norm(x, weight, bias, eps, return_stats)  # None: not an ordinary call
         if out is not None:
             return out
-    assert len(x.shape) >= 1
-    assert x.dtype in _TYPES
-    _check_weights("layer_norm", x, weight, bias)
-    _native._require_cuda(x)
+    _check(x, weight, bias)
     if torch.compiler.is_compiling():
         out = _native.layer_norm_op(x, weight, bias, float(eps))
     else:
@@ -75,14 +90,7 @@ def layer_norm_backward(
         out = _native.HOST.layer_norm_backward(dy, x, mean, rstd, weight, weight_grad, bias_grad)
         if out is not None:
             return out
-    assert len(x.shape) >= 1
-    assert x.dtype in _TYPES
-    assert dy.shape == x.shape and dy.dtype == x.dtype
-    assert mean.shape == rstd.shape == x.shape[:-1]
-    assert mean.dtype == rstd.dtype == torch.float32
-    assert dy.device == x.device == mean.device == rstd.device
-    _check_weights("layer_norm_backward", x, weight)
-    _native._require_cuda(x)
+    _check_backward(dy, x, mean, rstd, weight)
     impl = _native.layer_norm_backward_op if torch.compiler.is_compiling() else _native._layer_norm_backward_impl
     dx, dweight, dbias = impl(dy, x, mean, rstd, weight, bool(weight_grad), bool(bias_grad))
     return dx, dweight if weight_grad else None, dbias if bias_grad else None

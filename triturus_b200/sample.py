@@ -11,12 +11,29 @@ from . import _native
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _parameter(name: str, value, lead: torch.Size, device: torch.device, kind: torch.dtype, off, valid):
-    """(tensor of the rows' shape or None, number)"""
+def _check(logits: torch.Tensor, noise: torch.Tensor, temperature, top_k, top_p, min_p) -> None:
+    """The parameters as tensors, or anything else for numbers."""
+    assert len(logits.shape) >= 1
+    assert logits.dtype in _TYPES
+    assert noise.shape == logits.shape
+    assert noise.dtype == torch.float32
+    assert noise.device == logits.device
+    for value, kind in ((temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32)):
+        if isinstance(value, torch.Tensor):
+            assert value.dtype == kind
+            assert value.shape == logits.shape[:-1]
+            assert value.device == logits.device
+
+
+def _check_device(logits: torch.Tensor) -> None:
+    _native._require_cuda(logits)
+    if logits.shape[-1] == 0:
+        raise ValueError("sample: rows of no symbols are not supported")
+
+
+def _parameter(name: str, value, off, valid):
+    """(tensor or None, number)"""
     if isinstance(value, torch.Tensor):
-        assert value.dtype == kind
-        assert value.shape == lead
-        assert value.device == device
         return value, off
     if value is None:
         return None, off
@@ -55,21 +72,14 @@ def sample(
         out = _native.HOST.sample(logits, noise, temperature, top_k, top_p, min_p, return_logprob)  # None: not an ordinary call
         if out is not None:
             return out
-    assert len(logits.shape) >= 1
-    assert logits.dtype in _TYPES
-    assert noise.shape == logits.shape
-    assert noise.dtype == torch.float32
-    assert noise.device == logits.device
-    lead, device = logits.shape[:-1], logits.device
+    _check(logits, noise, temperature, top_k, top_p, min_p)
     params = (
-        *_parameter("temperature", temperature, lead, device, torch.float32, 1.0, lambda v: 0.0 <= v < math.inf),
-        *_parameter("top_k", top_k, lead, device, torch.int32, 0, lambda v: 1 <= v == int(v)),
-        *_parameter("top_p", top_p, lead, device, torch.float32, 1.0, lambda v: 0.0 <= v <= 1.0),
-        *_parameter("min_p", min_p, lead, device, torch.float32, 0.0, lambda v: 0.0 <= v <= 1.0),
+        *_parameter("temperature", temperature, 1.0, lambda v: 0.0 <= v < math.inf),
+        *_parameter("top_k", top_k, 0, lambda v: 1 <= v == int(v)),
+        *_parameter("top_p", top_p, 1.0, lambda v: 0.0 <= v <= 1.0),
+        *_parameter("min_p", min_p, 0.0, lambda v: 0.0 <= v <= 1.0),
     )
-    _native._require_cuda(logits)
-    if logits.shape[-1] == 0:
-        raise ValueError("sample: rows of no symbols are not supported")
+    _check_device(logits)
     params = (*params[:3], min(params[3], 2**31 - 1), *params[4:])
     token, logprob = (_native.sample_op if torch.compiler.is_compiling() else _native._sample_impl)(logits, noise, *params)
     return (token, logprob) if return_logprob else token
