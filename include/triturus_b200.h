@@ -293,7 +293,7 @@ int triturus_b200_layer_norm(const void* x, const void* weight, const void* bias
 /*
  * Its gradients, with g = dy weight and h = (x - mean) rstd:
  *   dx = rstd (g - sum(g) / width - h sum(g h) / width),  dweight = sum over rows of dy h,  dbias = sum over rows of dy.
- * dx holds rows back to back; dweight and dbias (of weight_type) may be NULL.  The workspace (16-byte aligned,
+ * dx holds rows back to back; dweight and dbias (of weight_type, also without a weight) may be NULL.  The workspace (16-byte aligned,
  * triturus_b200_layer_norm_backward_workspace_bytes, may hold anything) takes each block's share of dweight and dbias, which a second launch
  * adds in a fixed order.
  */

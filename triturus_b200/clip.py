@@ -57,8 +57,8 @@ def clip_grad_norm_(grads: torch.Tensor | Iterable[torch.Tensor | None], max_nor
     The norm is that of all elements of all tensors taken as one vector: the root of the sum of squares, or with `norm_type=math.inf`
     the largest magnitude.  Every element is multiplied by min(1, max_norm / (norm + 1e-6)); where that is 1 nothing is written.
     The tensors are float32, bfloat16 or float16, mixed as they come, of any number, shape and alignment (dense ones in
-    place, views with gaps through a copy); None and empty ones are skipped.  They may not share memory.  The sum of squares is held in 64 bits
-    and added in a fixed order.  The result is a float32 tensor of no dimensions on the same device: nothing is waited for.  A NaN or an
+    place, views with gaps through a copy); None and empty ones are skipped.  They may not share memory, require a gradient or
+    have a forward-mode tangent.  The sum of squares is held in 64 bits and added in a fixed order.  The result is a float32 tensor of no dimensions on the same device: nothing is waited for.  A NaN or an
     infinity among the gradients makes it NaN or infinite, and the gradients NaN or (but for the infinite ones) zero."""
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm is not negative, got {max_norm!r}")
@@ -73,7 +73,7 @@ def clip_grad_norm_(grads: torch.Tensor | Iterable[torch.Tensor | None], max_nor
 
 
 def grad_norm(grads: torch.Tensor | Iterable[torch.Tensor | None], *, norm_type: float = 2.0) -> torch.Tensor:
-    """The norm that `clip_grad_norm_` returns, and nothing else."""
+    """The norm that `clip_grad_norm_` returns, and nothing else.  It carries no graph: it is not differentiable."""
     norm_type = float(norm_type)
     if not torch.compiler.is_compiling():
         out = _native.HOST.clip_grad_norm(grads, 0.0, norm_type, False)

@@ -8,7 +8,7 @@
 // that all have the same n, and scales its chunks, the last one first: what the first launch read last is still in the L2 cache.  Where c is
 // 1 nothing is written.
 //
-// Measured on one B200: the norm alone of 1 GB and more at the copy bandwidth (146 us a GB), 120 MB 24.7 us; with the product 120 MB 59.5 us, 1.46 GB 714 us =
+// Measured on one B200: the norm alone of 1 GB and more at the copy bandwidth (146 us a GB), 120 MB 24.7 us; with the product 120 MB 59.8 us, 1.46 GB 717 us =
 // 0.94 of three passes.  The second read of what the L2 cache still holds saves little, since the last call's written lines leave the cache
 // at the same time.  (Of the blocks' four 16-byte loads under way and the next four, ncu: DRAM 63 and 61 %.)
 //

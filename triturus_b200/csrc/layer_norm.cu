@@ -11,7 +11,8 @@
 // Measured on one B200 (copy bandwidth 6.54 TB/s): forward 16384 x 2048 bfloat16 26.7 us = 5.0 TB/s, 16384 x 8192 111-117 us = 4.6-4.8; backward 16384 x 8192
 // 159 us = 5.1 TB/s with the shares of dw and db; 4000 x 16384 float32 99 and 138 us = 5.3 and 5.7.  What is missing is the time of a row's steps in turn (issue
 // 0.5-0.6 of a scheduler's cycles): more rows under way than four change nothing.  Rows off 16-byte boundaries come element by element and are
-// bound by instructions: 5003 x 1537 float32 16.5 and 29 us = 3.7 and 3.2 TB/s.  Rows beyond 16384 elements are read three times.
+// bound by instructions: 5003 x 1537 float32 16.5 and 29 us = 3.7 and 3.2 TB/s, 20000 x 1001 bfloat16 45 and 72 us = 1.8 and 1.7 (20000 x 1000: 21 and 34).
+// Rows beyond 16384 elements are read three times, an element at a time: 4000 x 32768 bfloat16 424 and 558 us, float32 288 and 695.
 //
 // Everything between the loads and the stores is in 32 bits.  The variance is the sum of squares about the mean and not the
 // difference of two sums: a feature at a high level would cancel its digits.  Nothing here adds atomically: the results

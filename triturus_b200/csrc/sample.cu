@@ -10,7 +10,8 @@
 // A row belongs to a cluster of up to eight blocks with a slice each, held in shared memory or, where that is too little, read again from the L2 cache.
 // No row is sorted.
 //
-// Nothing filtered: one pass over logits and noise (200 x 10007 in float32 8.2 us a call; 256 x 131072 86 us = 3.1 TB/s).
+// Nothing filtered: one pass over logits and noise (200 x 10007 in float32 8.2 us a call; 256 x 131072 84 us = 3.2 TB/s).  min_p alone: the same pass behind
+// one for the maximum, with all of the noise (256 x 131072 100 us).
 //
 // A small top_k: a block's own symbols below the k-th largest of its threads' maxima cannot be among the row's first k; what remains, some
 // tens of symbols of each block, the first block gathers, sorts and finishes alone (1 x 32768, top_k 50 and top_p 0.9: 11.5 us a call, 9.3 of the
@@ -23,9 +24,10 @@
 // by radix selection over the bits of x and then over the index.  Numbers and, as multiples of a power of two, masses are added as integers, so
 // that a result does not depend on the order of the atomic additions.
 //
-// 256 x 131072 in float32 with top_p 0.95 takes 146 us, seven times what reading the logits does: three passes over each row (maximum,
-// histogram, setting apart) of 11, 21 and 11 us to a wave of 148 rows, where 11 is what the L2 cache takes to hand out so much, and some 15 us of
-// steps that wait for the cluster; the instructions of the histogram bound its pass (ncu: issue 47 %, DRAM 16 %).
+// 256 x 131072 in float32 with top_p 0.95, at a temperature that leaves 2 % of the symbols, takes 146 us, seven times what reading the logits
+// does: three passes over each row (maximum, histogram, setting apart) of 11, 21 and 11 us to a wave of 148 rows, where 11 is what the L2 cache takes to hand out so much, and some 15 us of
+// steps that wait for the cluster; the instructions of the histogram bound its pass (ncu: issue 47 %, DRAM 16 %).  Where more symbols remain
+// than the threads can set apart, each of the later steps goes over the row again: 361 us with 9 % of them (temperature 1; 0.8 leaves the 2).
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -1280,9 +1282,11 @@ int run_sample(const SampleArgs& p, int64_t rows, int c, cudaStream_t stream) {
   }
 }
 
-// Blocks to a row: as many as the GPU holds at once (two to an SM, by their registers), if they have 4096 symbols each; more of them where a block's
-// warps could not set enough apart.  A slice is held in shared memory where two such blocks fit an SM or one to an SM is all there is; else it is
-// read again from the L2 cache.
+// Blocks to a row: as many as the GPU holds at once (two to an SM, by their registers), if they have 4096 symbols each; in any case enough that a
+// block has no more than 64 K symbols (and what lies before a 16-byte boundary).  With fewer its threads set a larger share apart, with more there are
+// fewer steps of a cluster and less to do for it: 256 x 131072 in float32, us, in blocks of 32 K / 64 K / 128 K symbols: top_p 0.95 at temperature
+// 0.6 156 / 120 / 127, 0.8 182 / 146 / 317, 1.0 292 / 361 / 392, 1.2 426 / 381 / 405; unfiltered 98 / 84 / 76.  A slice is held in shared memory where two
+// such blocks fit an SM or one to an SM is all there is; else it is read again from the L2 cache.
 template <class T>
 int sample_rows(SampleArgs p, int64_t rows, cudaStream_t stream) {
   const int64_t most = static_cast<int64_t>(p.symbols) + 16 / static_cast<int64_t>(sizeof(T));  // (with what lies before a 16-byte boundary)

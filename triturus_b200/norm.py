@@ -85,7 +85,7 @@ def layer_norm_backward(
 
     With g = dy * weight and h = (x - mean) * rstd: dx = rstd * (g - sum(g) / D - h * sum(g * h) / D), dweight = sum over rows of dy * h,
     dbias = sum over rows of dy.  dx has x's type, the other two weight's (x's without a weight); they are None where `weight_grad` or
-    `bias_grad` is False.  The sums are in 32 bits and added in a fixed order."""
+    `bias_grad` is False.  The sums are in 32 bits and added in a fixed order.  The results carry no graph."""
     if not torch.compiler.is_compiling():
         out = _native.HOST.layer_norm_backward(dy, x, mean, rstd, weight, weight_grad, bias_grad)
         if out is not None:

@@ -67,7 +67,12 @@ def sample(
     and a min_p of 0 are no filter.  A temperature of 0 (in a tensor: any that is not positive) gives the first of the largest
     logits with logprob 0.  Symbols of -inf are impossible and never given; a row of nothing else gives token -1 and logprob
     -inf, a row with a NaN -1 and NaN.  Infinity counts as the largest number.  logits and noise may have any strides: rows of consecutive elements
-    at one distance are read in place (noise only where a symbol is kept), other views are copied first."""
+    at one distance are read in place, other views are copied first.  Only the noise of kept symbols counts, though that of others may be
+    read.
+
+    The same call gives the same result each time.  The number of rows decides how many blocks share one, and with that the order in which its p
+    are added: in another batch a row's logprob may differ in its last bits, and its token where a sum is that close to top_p.  The results
+    carry no graph: logprob is not differentiable."""
     if not torch.compiler.is_compiling():
         out = _native.HOST.sample(logits, noise, temperature, top_k, top_p, min_p, return_logprob)  # None: not an ordinary call
         if out is not None:
