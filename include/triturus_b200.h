@@ -272,8 +272,8 @@ int triturus_b200_mm_f32(const float* a, const float* b, float* out, int64_t M, 
                          int precision, int32_t* status_dev, void* stream);
 
 /*
- * Operators for models around the contractions: layer norm with its gradients, clipping of gradients by their global norm, and
- * sampling from log-probabilities.  (No counterpart in the reference.)  Their elements are 32-bit floats, bfloat16 or 16-bit
+ * Operators for models around the contractions: layer norm with its gradients, clipping of gradients by their global norm,
+ * sampling from log-probabilities, and the lookup of symbols in a table with its gradient.  (No counterpart in the reference.)  Their elements are 32-bit floats, bfloat16 or 16-bit
  * floats; the arithmetic between loads and stores has 32 bits or more.  None of them waits on a barrier that it could miss, so
  * none takes a status word.
  */
@@ -327,6 +327,23 @@ int triturus_b200_clip_grad_norm(void* const* tensors, const int64_t* numels, co
 int triturus_b200_sample(const void* logits, const float* noise, int64_t* token, float* logprob, int64_t rows, int64_t symbols,
                          int64_t logits_stride, int64_t noise_stride, int type, const float* temperature, float temperature0,
                          const int32_t* top_k, int32_t top_k0, const float* top_p, float top_p0, const float* min_p, float min_p0, void* stream);
+
+/*
+ * y[i, :] = scale weight[t_i, :] for `count` symbols t_i (64- or 32-bit whole numbers by token_bytes, one after the other) and a table of
+ * `symbols` rows of `width` elements, weight_stride elements apart; y holds rows back to back.  A symbol outside of 0 ... symbols - 1 gives
+ * a row of NaN.  Pointers need the alignment of their elements alone.  At most 2^30 positions, 2^30 - 1 symbols.
+ */
+int triturus_b200_embedding(const void* tokens, int token_bytes, const void* weight, void* y, int64_t count, int64_t symbols, int64_t width,
+                            int64_t weight_stride, int type, float scale, void* stream);
+/*
+ * Its gradient: dweight[v, :] = scale sum of dy[i, :] over the i with t_i = v, and zero for v = padding (-1: no such symbol).  dweight holds
+ * `symbols` rows of dy's type back to back, all of which are written.  The positions are sorted by symbol in the workspace (16-byte aligned, may
+ * hold anything) and the rows added in 32 bits in an order that depends on the symbols alone.
+ */
+size_t triturus_b200_embedding_backward_workspace_bytes(int64_t count, int64_t symbols, int64_t width);
+int triturus_b200_embedding_backward(const void* dy, const void* tokens, int token_bytes, void* dweight, int64_t count, int64_t symbols,
+                                     int64_t width, int64_t dy_stride, int type, float scale, int64_t padding, void* workspace,
+                                     size_t workspace_bytes, void* stream);
 
 /*
  * Self-test of the error path behind `status_dev` (no counterpart in the reference, whose kernels have no waits

@@ -8,6 +8,7 @@ from . import lm2exp as _lm2exp_module
 from . import lt2exp as _lt2exp_module
 from ._native import NativeLibraryError, check_status, colmax
 from .clip import clip_grad_norm_, grad_norm
+from .embedding import embedding, embedding_backward
 from .host import lm2exp_host, lt2exp_host
 from .lm2exp import lm2exp
 from .lt2exp import lt2exp
@@ -26,6 +27,8 @@ __all__ = [
     "check_status",
     "clip_grad_norm_",
     "colmax",
+    "embedding",
+    "embedding_backward",
     "ensure_reproducibility",
     "grad_norm",
     "is_torch_tf32_enabled",

@@ -48,6 +48,9 @@ EXPORTED_SYMBOLS = (
     "triturus_b200_layer_norm_backward",
     "triturus_b200_layer_norm_backward_workspace_bytes",
     "triturus_b200_sample",
+    "triturus_b200_embedding",
+    "triturus_b200_embedding_backward",
+    "triturus_b200_embedding_backward_workspace_bytes",
     "triturus_b200_lm2exp_static_max_columns",
     "triturus_b200_lm2exp_f32_static",
 )
@@ -184,6 +187,16 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         *[c_void_p] * 4, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_float, c_void_p, c_int32, c_void_p, c_float,
         c_void_p, c_float, c_void_p,
     ]  # fmt: skip
+    lib.triturus_b200_embedding.restype = c_int
+    lib.triturus_b200_embedding.argtypes = [
+        c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_void_p,
+    ]  # fmt: skip
+    lib.triturus_b200_embedding_backward_workspace_bytes.restype = c_size_t
+    lib.triturus_b200_embedding_backward_workspace_bytes.argtypes = [c_int64] * 3
+    lib.triturus_b200_embedding_backward.restype = c_int
+    lib.triturus_b200_embedding_backward.argtypes = [
+        c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_int64, c_void_p, c_size_t, c_void_p,
+    ]  # fmt: skip
     return lib
 
 
@@ -207,7 +220,7 @@ _IN_PLACE_MAX_FLOP_STRIDED = 8e9
 class _NoHost:
     """In the place of the extension module where there is none: no call is a small one to it, all go through ctypes."""
 
-    lm2exp = lt2exp = layer_norm = layer_norm_backward = clip_grad_norm = sample = staticmethod(lambda *args: None)
+    lm2exp = lt2exp = layer_norm = layer_norm_backward = clip_grad_norm = sample = embedding = embedding_backward = staticmethod(lambda *args: None)
 
 
 def _load_host():
@@ -896,3 +909,70 @@ def _sample_fake(logits, noise, temperature, temperature0, top_k, top_k0, top_p,
     check(logits, noise, temperature, top_k, top_p, min_p)
     _check_device(logits)
     return logits.new_empty(logits.shape[:-1], dtype=torch.int64), logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+
+
+# ---------------------------------------------------------------------------- embeddings
+
+
+def _embedding_impl(tokens: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+    _require_cuda(weight)
+    symbols, width = weight.shape
+    y = torch.empty((*tokens.shape, width), dtype=weight.dtype, device=weight.device)
+    tokens = tokens.contiguous()
+    rows, stride = _rows(weight)
+    with _on_device(weight.device) as idx:
+        rc = LIB.triturus_b200_embedding(
+            tokens.data_ptr(), tokens.element_size(), rows.data_ptr(), y.data_ptr(), tokens.numel(), symbols, width, stride,
+            _TYPE_CODES[weight.dtype], scale, _raw_stream(idx),
+        )  # fmt: skip
+    _check(rc, "triturus_b200_embedding")
+    return y
+
+
+def _embedding_backward_impl(dy: torch.Tensor, tokens: torch.Tensor, symbols: int, scale: float, padding_idx: int | None) -> torch.Tensor:
+    _require_cuda(dy)
+    width, count = dy.shape[-1], tokens.numel()
+    dweight = torch.empty((symbols, width), dtype=dy.dtype, device=dy.device)
+    tokens = tokens.contiguous()
+    rows, stride = _rows(dy)
+    with _on_device(dy.device) as idx:
+        nbytes = int(LIB.triturus_b200_embedding_backward_workspace_bytes(count, symbols, width))
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dy.device)
+        rc = LIB.triturus_b200_embedding_backward(
+            rows.data_ptr(), tokens.data_ptr(), tokens.element_size(), dweight.data_ptr(), count, symbols, width, stride,
+            _TYPE_CODES[dy.dtype], scale, -1 if padding_idx is None else padding_idx, ws.data_ptr(), nbytes, _raw_stream(idx),
+        )  # fmt: skip
+    _check(rc, "triturus_b200_embedding_backward")
+    return dweight
+
+
+@torch.library.custom_op("triturus::embedding", mutates_args=(), device_types="cuda")
+def embedding_op(tokens: torch.Tensor, weight: torch.Tensor, scale: float, padding_idx: int | None) -> torch.Tensor:
+    from .embedding import _check as check
+
+    check(tokens, weight, scale, padding_idx)
+    return _embedding_impl(tokens, weight, scale)
+
+
+@torch.library.custom_op("triturus::embedding_backward", mutates_args=(), device_types="cuda")
+def embedding_backward_op(dy: torch.Tensor, tokens: torch.Tensor, symbols: int, scale: float, padding_idx: int | None) -> torch.Tensor:
+    from .embedding import _check_backward
+
+    _check_backward(dy, tokens, symbols, scale, padding_idx)
+    return _embedding_backward_impl(dy, tokens, symbols, scale, padding_idx)
+
+
+@embedding_op.register_fake
+def _embedding_fake(tokens, weight, scale, padding_idx):
+    from .embedding import _check as check
+
+    check(tokens, weight, scale, padding_idx)
+    return weight.new_empty((*tokens.shape, weight.shape[1]))
+
+
+@embedding_backward_op.register_fake
+def _embedding_backward_fake(dy, tokens, symbols, scale, padding_idx):
+    from .embedding import _check_backward
+
+    _check_backward(dy, tokens, symbols, scale, padding_idx)
+    return dy.new_empty((symbols, dy.shape[-1]))

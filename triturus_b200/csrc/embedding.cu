@@ -1,0 +1,470 @@
+// Rows of a table by symbol, and the table's gradient.
+//
+//   y[i] = s W[t_i];    dW[v] = s sum over {i: t_i = v} of dy[i]
+//
+// The lookup moves each row once, 16 bytes to a thread and four of them under way; bound by memory.
+//
+// The gradient adds rows of dy that belong to the same symbol.  Atomics would add them in any order, so the positions are sorted by
+// symbol first, with a stable radix sort of up to 9 bits a pass (two launches each: every block counts its digits; then it adds up
+// the blocks' counts before it and places its items, ranked by warp and by warps).  Then groups of threads walk runs of kTile or more sorted
+// positions: a thread keeps its 16 bytes of columns as 32-bit sums and writes them where a symbol's run ends.  A run over a border of
+// two tiles is left in the workspace in parts, which a last launch adds in their order: frequent symbols are spread over many
+// blocks, and the same call gives the same result each time.  Bound by memory: dy read once, the table written once.
+#include <algorithm>
+
+#include "packs.cuh"
+
+namespace tb200 {
+namespace {
+
+constexpr int kTile = 32;            // sorted positions of a group of threads, at least
+constexpr int kMostTiles = 8192;     // (more positions than these take longer tiles)
+constexpr int kSortThreads = 1024;
+constexpr int kMostDigits = 512;
+constexpr int kMostSortBlocks = 128;
+constexpr int kGroup = 128;          // threads of a block that adds rows
+
+// A symbol of a list of 64- or 32-bit ones.
+__device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(tokens)[i] : static_cast<int64_t>(static_cast<const int32_t*>(tokens)[i]);
+}
+
+// 16 bytes from any multiple of an element's size: where they are not on a 16-byte boundary, two vectors around them.  [lo, hi) is the
+// tensor's memory, beyond which nothing is read.
+template <class T>
+__device__ __forceinline__ uint4 load_window(const T* p, const char* lo, const char* hi) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const int s = static_cast<int>(at & 15);
+  if (s == 0) return *reinterpret_cast<const uint4*>(p);
+  const char* g = reinterpret_cast<const char*>(p) - s;
+  if (g < lo || g + 32 > hi) {
+    Pack<T, 16> r;
+#pragma unroll
+    for (int e = 0; e < Pack<T, 16>::N; ++e) r.v[e] = p[e];
+    return *reinterpret_cast<const uint4*>(&r);
+  }
+  const uint4 a = *reinterpret_cast<const uint4*>(g), b = *reinterpret_cast<const uint4*>(g + 16);
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (s & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (s & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const int bits = (s & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// ----------------------------------------------------------------------------- lookup
+
+struct LookupArgs {
+  const void* tokens;
+  const void* weight;
+  void* y;
+  const char *lo, *hi;  // the table's memory
+  int64_t count, symbols, stride;
+  int width, wide, lanes;  // lanes: threads of a row, a power of two
+  float scale;
+};
+
+template <class T, bool SCALED>
+__device__ __forceinline__ uint4 scaled(uint4 bits, float scale) {
+  if (!SCALED) return bits;
+  Pack<T, 16> p = *reinterpret_cast<Pack<T, 16>*>(&bits);
+#pragma unroll
+  for (int e = 0; e < Pack<T, 16>::N; ++e) p.v[e] = from_float<T>(to_float(p.v[e]) * scale);
+  return *reinterpret_cast<uint4*>(&p);
+}
+
+template <class T, bool SCALED>
+__global__ void __launch_bounds__(256) embedding_kernel(const LookupArgs p) {
+  constexpr int N = Pack<T, 16>::N;
+  const int lane = static_cast<int>(threadIdx.x) & (p.lanes - 1);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / p.lanes) + threadIdx.x / p.lanes;
+  if (row >= p.count) return;
+  const int64_t t = token_at(p.tokens, p.wide, row);
+  T* dst = static_cast<T*>(p.y) + row * p.width;
+  if (t < 0 || t >= p.symbols) {  // no such symbol: no number either
+    for (int c = lane; c < p.width; c += p.lanes) dst[c] = from_float<T>(__int_as_float(0x7fc00000));
+    return;
+  }
+  const T* src = static_cast<const T*>(p.weight) + t * p.stride;
+  const int head = min(p.width, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / sizeof(T)));
+  const int body = (p.width - head) / N;
+  for (int v = lane; v < body; v += 4 * p.lanes) {
+    uint4 r[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (v + u * p.lanes < body) r[u] = load_window<T>(src + head + (v + u * p.lanes) * N, p.lo, p.hi);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (v + u * p.lanes < body) *reinterpret_cast<uint4*>(dst + head + (v + u * p.lanes) * N) = scaled<T, SCALED>(r[u], p.scale);
+  }
+  const int rest = p.width - body * N;  // what lies before the first and behind the last vector
+  for (int e = lane; e < rest; e += p.lanes) {
+    const int c = e < head ? e : body * N + e;
+    dst[c] = SCALED ? from_float<T>(to_float(src[c]) * p.scale) : src[c];
+  }
+}
+
+// ----------------------------------------------------------------------------- sort
+
+struct SortArgs {
+  const void* tokens;  // of the first pass
+  int64_t symbols, padding;
+  const int32_t *keys, *at;  // of later passes: symbols and positions
+  int32_t *keys_out, *at_out;
+  int* counts;  // [blocks][digits]
+  int count, per_block, blocks, wide, shift, digits;
+};
+
+// What a position is sorted by: its symbol; `symbols` where it has no gradient to give.
+__device__ __forceinline__ int key_at(const SortArgs& p, int i) {
+  if (p.keys != nullptr) return p.keys[i];
+  const int64_t t = token_at(p.tokens, p.wide, i);
+  return static_cast<int>(t < 0 || t >= p.symbols || t == p.padding ? p.symbols : t);
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs p) {
+  __shared__ int n[kMostDigits];
+  for (int d = threadIdx.x; d < p.digits; d += kSortThreads) n[d] = 0;
+  __syncthreads();
+  const int begin = static_cast<int>(blockIdx.x) * p.per_block, end = min(p.count, begin + p.per_block);
+  for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += kSortThreads) atomicAdd(&n[(key_at(p, i) >> p.shift) & (p.digits - 1)], 1);
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.digits; d += kSortThreads) p.counts[static_cast<int>(blockIdx.x) * p.digits + d] = n[d];
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortArgs p) {
+  constexpr int W = kSortThreads / 32;
+  __shared__ int next[kMostDigits];            // where the block's next item of a digit goes
+  __shared__ uint16_t of_warp[W][kMostDigits];  // items of a digit in a warp, then in the warps before
+  __shared__ int sums[W];
+  const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
+  // the items of lower digits in all blocks, and of this digit in the blocks before
+  int before = 0, all = 0;
+  if (tid < p.digits) {
+    for (int b = 0; b < p.blocks; ++b) {
+      const int n = p.counts[b * p.digits + tid];
+      all += n;
+      before += b < static_cast<int>(blockIdx.x) ? n : 0;
+    }
+  }
+  int upto = all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  int lower = 0;
+  for (int w = 0; w < warp; ++w) lower += sums[w];
+  if (tid < p.digits) next[tid] = lower + upto - all + before;
+  const int begin = static_cast<int>(blockIdx.x) * p.per_block, end = min(p.count, begin + p.per_block);
+  for (int base = begin; base < end; base += kSortThreads) {
+    for (int i = tid; i < W * p.digits; i += kSortThreads) of_warp[i / p.digits][i % p.digits] = 0;
+    __syncthreads();
+    const int i = base + tid;
+    const bool valid = i < end;
+    const int key = valid ? key_at(p, i) : 0;
+    const int at = valid && p.at != nullptr ? p.at[i] : i;
+    const int digit = valid ? (key >> p.shift) & (p.digits - 1) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    if (valid && rank == 0) of_warp[warp][digit] = static_cast<uint16_t>(__popc(same));
+    __syncthreads();
+    int total = 0;
+    if (tid < p.digits) {
+#pragma unroll 8
+      for (int w = 0; w < W; ++w) {
+        const int n = of_warp[w][tid];
+        of_warp[w][tid] = static_cast<uint16_t>(total);
+        total += n;
+      }
+    }
+    __syncthreads();
+    if (valid) {
+      const int to = next[digit] + of_warp[warp][digit] + rank;
+      p.keys_out[to] = key;
+      p.at_out[to] = at;
+    }
+    __syncthreads();
+    if (tid < p.digits) next[tid] += total;
+  }
+}
+
+// ----------------------------------------------------------------------------- sums
+
+struct SumArgs {
+  const void* dy;
+  const char *lo, *hi;  // its memory
+  const int32_t *keys, *at;
+  void* dweight;
+  float* part;  // [tiles][2][width]: of the run that began before the tile, and of the one that goes on behind it
+  int64_t stride;
+  int count, symbols, width, tile, lanes, slabs;
+  float scale;
+};
+
+template <class T>
+__device__ __forceinline__ void store_row(const SumArgs& p, int key, int c, const float* acc) {
+  constexpr int N = Pack<T, 16>::N;
+  T* dst = static_cast<T*>(p.dweight) + static_cast<int64_t>(key) * p.width + c;
+  Pack<T, 16> r;
+#pragma unroll
+  for (int e = 0; e < N; ++e) r.v[e] = from_float<T>(acc[e] * p.scale);
+  if (c + N <= p.width && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(&r);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c + e < p.width) dst[e] = r.v[e];
+  }
+}
+
+template <class T>
+__device__ __forceinline__ uint4 load_columns(const SumArgs& p, int at, int c) {
+  constexpr int N = Pack<T, 16>::N;
+  const T* src = static_cast<const T*>(p.dy) + at * p.stride + c;
+  if (c + N <= p.width) return load_window<T>(src, p.lo, p.hi);
+  Pack<T, 16> r;
+#pragma unroll
+  for (int e = 0; e < N; ++e) r.v[e] = c + e < p.width ? src[e] : from_float<T>(0.f);
+  return *reinterpret_cast<const uint4*>(&r);
+}
+
+template <class T>
+__global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) {
+  constexpr int N = Pack<T, 16>::N, AHEAD = 4;
+  const int groups = kGroup / p.lanes;
+  const int64_t tile = static_cast<int64_t>(blockIdx.x) * groups + threadIdx.x / p.lanes;
+  const int c = (static_cast<int>(blockIdx.y) * p.lanes + (static_cast<int>(threadIdx.x) & (p.lanes - 1))) * N;
+  const int64_t first = tile * p.tile;
+  if (first >= p.count || c >= p.width) return;
+  const int begin = static_cast<int>(first), end = static_cast<int>(min(first + p.tile, static_cast<int64_t>(p.count)));
+  float* part = p.part + tile * 2 * p.width + c;
+  const int before = begin > 0 ? p.keys[begin - 1] : -1, behind = end < p.count ? p.keys[end] : -1;
+  float acc[N];
+  int run = -1;  // the symbol whose rows are in acc
+  bool head = false;
+  const auto leave = [&](bool last) {
+    if (run < 0) return;
+    if (head || (last && run == behind)) {
+      float* to = part + (head ? 0 : p.width);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (c + e < p.width) to[e] = acc[e];
+    } else {
+      store_row<T>(p, run, c, acc);
+    }
+  };
+  for (int i = begin; i < end; i += AHEAD) {
+    int key[AHEAD];
+    uint4 row[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) key[u] = i + u < end ? p.keys[i + u] : p.symbols;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (key[u] < p.symbols) row[u] = load_columns<T>(p, p.at[i + u], c);
+    if (key[0] >= p.symbols) break;  // (they are the last ones)
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (key[u] >= p.symbols) break;
+      const Pack<T, 16> r = *reinterpret_cast<const Pack<T, 16>*>(&row[u]);
+      if (key[u] != run) {
+        leave(false);
+        run = key[u];
+        head = i + u == begin && run == before;
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = to_float(r.v[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += to_float(r.v[e]);
+      }
+    }
+  }
+  leave(true);
+}
+
+// Runs over the borders of tiles: the block of the tile in which one begins adds its parts.
+template <class T>
+__global__ void __launch_bounds__(kGroup) embedding_join_kernel(const SumArgs p) {
+  constexpr int N = Pack<T, 16>::N;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tile;
+  const int begin = static_cast<int>(first);
+  int64_t end = first + p.tile;
+  if (end >= p.count) return;
+  const int run = p.keys[end - 1];
+  if (run >= p.symbols || p.keys[end] != run) return;                             // none goes on
+  if (begin > 0 && p.keys[begin] == run && p.keys[begin - 1] == run) return;      // it began before
+  const int c = (static_cast<int>(blockIdx.y) * kGroup + static_cast<int>(threadIdx.x)) * N;
+  if (c >= p.width) return;
+  float acc[N];
+  const float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.width + p.width + c;
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = c + e < p.width ? part[e] : 0.f;
+  part += p.width;  // the first part of the next tile
+  for (;;) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c + e < p.width) acc[e] += part[e];
+    part += 2 * p.width;
+    end += p.tile;
+    if (end >= p.count || p.keys[end - 1] != run || p.keys[end] != run) break;
+  }
+  store_row<T>(p, run, c, acc);
+}
+
+// ----------------------------------------------------------------------------- host
+
+bool type_ok(int type) { return type >= TRITURUS_B200_TYPE_F32 && type <= TRITURUS_B200_TYPE_F16; }
+int size_of(int type) { return type == TRITURUS_B200_TYPE_F32 ? 4 : 2; }
+bool sizes_ok(int64_t count, int64_t symbols, int64_t width, int type, int token_bytes) {
+  return count >= 0 && count <= (1ll << 30) && symbols > 0 && symbols < (1ll << 30) && width > 0 && width <= (1ll << 30) && type_ok(type) &&
+         (token_bytes == 4 || token_bytes == 8);
+}
+template <class F>
+int by_type(int type, F fn) {
+  return type == TRITURUS_B200_TYPE_F32 ? fn(0.f) : type == TRITURUS_B200_TYPE_BF16 ? fn(__nv_bfloat16()) : fn(__half());
+}
+
+// The least power of two that is not below n, of at most `most`.
+int lanes_for(int64_t n, int most) {
+  int l = 1;
+  while (l < most && l < n) l <<= 1;
+  return l;
+}
+int tile_of(int64_t count) { return static_cast<int>(std::max<int64_t>(kTile, (count + kMostTiles - 1) / kMostTiles)); }
+
+struct SumSpace {  // the workspace: keys and positions twice, the counts, the parts
+  size_t list, counts, part, bytes;
+};
+SumSpace space_of(int64_t count, int64_t width) {
+  const auto up = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
+  SumSpace s;
+  s.list = up(static_cast<size_t>(count) * 4);
+  s.counts = up(static_cast<size_t>(kMostSortBlocks) * kMostDigits * 4);
+  const int64_t tiles = (count + tile_of(count) - 1) / tile_of(count);
+  s.part = up(static_cast<size_t>(tiles) * 2 * static_cast<size_t>(width) * 4);
+  s.bytes = 4 * s.list + s.counts + s.part;
+  return s;
+}
+
+}  // namespace
+}  // namespace tb200
+
+using namespace tb200;
+
+extern "C" {
+
+int triturus_b200_embedding(const void* tokens, int token_bytes, const void* weight, void* y, int64_t count, int64_t symbols, int64_t width,
+                            int64_t weight_stride, int type, float scale, void* stream) {
+  if (!sizes_ok(count, symbols, width, type, token_bytes)) return TRITURUS_B200_EINVAL;
+  if (count == 0) return TRITURUS_B200_OK;
+  if (tokens == nullptr || weight == nullptr || y == nullptr) return TRITURUS_B200_EINVAL;
+  const int size = size_of(type);
+  if (!aligned_to(tokens, token_bytes) || !aligned_to(weight, size) || !aligned_to(y, size)) return TRITURUS_B200_EALIGN;
+  LookupArgs p = {};
+  p.tokens = tokens;
+  p.weight = weight;
+  p.y = y;
+  const int64_t far = (symbols - 1) * weight_stride * size;
+  p.lo = static_cast<const char*>(weight) + std::min<int64_t>(far, 0);
+  p.hi = static_cast<const char*>(weight) + std::max<int64_t>(far, 0) + width * size;
+  p.count = count;
+  p.symbols = symbols;
+  p.stride = weight_stride;
+  p.width = static_cast<int>(width);
+  p.wide = token_bytes == 8;
+  p.lanes = lanes_for((width * size / 16 + 3) / 4, 256);
+  p.scale = scale;
+  const int64_t rows = 256 / p.lanes;
+  const dim3 grid(static_cast<unsigned>((count + rows - 1) / rows));
+  return by_type(type, [&](auto t) {
+    using T = decltype(t);
+    return launch_of(scale == 1.f ? embedding_kernel<T, false> : embedding_kernel<T, true>, grid, 256, 0, static_cast<cudaStream_t>(stream), nullptr, p);
+  });
+}
+
+size_t triturus_b200_embedding_backward_workspace_bytes(int64_t count, int64_t symbols, int64_t width) {
+  return sizes_ok(count, symbols, width, 0, 8) ? space_of(count, width).bytes : 0;
+}
+
+int triturus_b200_embedding_backward(const void* dy, const void* tokens, int token_bytes, void* dweight, int64_t count, int64_t symbols,
+                                     int64_t width, int64_t dy_stride, int type, float scale, int64_t padding, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  if (!sizes_ok(count, symbols, width, type, token_bytes) || dweight == nullptr) return TRITURUS_B200_EINVAL;
+  const int size = size_of(type);
+  if (!aligned_to(dweight, size)) return TRITURUS_B200_EALIGN;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = TRITURUS_B200_OK;
+  if (count > 0) {
+    if (dy == nullptr || tokens == nullptr || workspace == nullptr) return TRITURUS_B200_EINVAL;
+    if (!aligned_to(dy, size) || !aligned_to(tokens, token_bytes) || !aligned_to(workspace, 16)) return TRITURUS_B200_EALIGN;
+    if (workspace_bytes < space_of(count, width).bytes) return TRITURUS_B200_EWORKSPACE;
+  }
+  rc = code_of(cudaMemsetAsync(dweight, 0, static_cast<size_t>(symbols) * static_cast<size_t>(width) * size, st));
+  if (rc != TRITURUS_B200_OK || count == 0) return rc;
+
+  const SumSpace space = space_of(count, width);
+  char* ws = static_cast<char*>(workspace);
+  const auto list = [&](int i) { return reinterpret_cast<int32_t*>(ws + i * space.list); };
+  SortArgs s = {};
+  s.tokens = tokens;
+  s.symbols = symbols;
+  s.padding = padding;
+  s.counts = reinterpret_cast<int*>(ws + 4 * space.list);
+  s.count = static_cast<int>(count);
+  s.per_block = static_cast<int>((count + static_cast<int64_t>(kMostSortBlocks) * kSortThreads - 1) / (static_cast<int64_t>(kMostSortBlocks) * kSortThreads)) * kSortThreads;
+  s.blocks = static_cast<int>((count + s.per_block - 1) / s.per_block);
+  s.wide = token_bytes == 8;
+  int bits = 1;
+  while ((symbols >> bits) != 0) ++bits;  // (of 0 ... symbols)
+  const int passes = (bits + 8) / 9, each = (bits + passes - 1) / passes;
+  s.digits = 1 << each;
+  for (int pass = 0; pass < passes && rc == TRITURUS_B200_OK; ++pass) {
+    s.shift = pass * each;
+    s.keys_out = list(pass & 1);
+    s.at_out = list(2 + (pass & 1));
+    rc = launch_of(sort_count_kernel, dim3(static_cast<unsigned>(s.blocks)), kSortThreads, 0, st, nullptr, s);
+    if (rc == TRITURUS_B200_OK) rc = launch_of(sort_place_kernel, dim3(static_cast<unsigned>(s.blocks)), kSortThreads, 0, st, nullptr, s);
+    s.keys = s.keys_out;
+    s.at = s.at_out;
+  }
+  if (rc != TRITURUS_B200_OK) return rc;
+
+  SumArgs p = {};
+  p.dy = dy;
+  const int64_t far = (count - 1) * dy_stride * size;
+  p.lo = static_cast<const char*>(dy) + std::min<int64_t>(far, 0);
+  p.hi = static_cast<const char*>(dy) + std::max<int64_t>(far, 0) + width * size;
+  p.keys = s.keys;
+  p.at = s.at;
+  p.dweight = dweight;
+  p.part = reinterpret_cast<float*>(ws + 4 * space.list + space.counts);
+  p.stride = dy_stride;
+  p.count = static_cast<int>(count);
+  p.symbols = static_cast<int>(symbols);
+  p.width = static_cast<int>(width);
+  p.tile = tile_of(count);
+  p.scale = scale;
+  const int64_t vectors = (width * size + 15) / 16;
+  p.lanes = lanes_for(vectors, kGroup);
+  const int64_t tiles = (count + p.tile - 1) / p.tile, groups = kGroup / p.lanes;
+  const unsigned slabs = static_cast<unsigned>((vectors + p.lanes - 1) / p.lanes);
+  if (slabs > 65535) return TRITURUS_B200_EINVAL;
+  return by_type(type, [&](auto t) {
+    using T = decltype(t);
+    int code = launch_of(embedding_sum_kernel<T>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), slabs), kGroup, 0, st, nullptr, p);
+    if (code == TRITURUS_B200_OK && tiles > 1)
+      code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((vectors + kGroup - 1) / kGroup)), kGroup, 0, st, nullptr, p);
+    return code;
+  });
+}
+
+}  // extern "C"

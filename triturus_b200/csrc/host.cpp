@@ -389,6 +389,87 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// Symbols: 64- or 32-bit whole numbers, one after the other, on `like`'s device.
+const at::Tensor* token_arg(PyObject* o, const at::Tensor& like) {
+  const at::Tensor* t = plain_object(o);
+  if (t == nullptr || (t->scalar_type() != at::kLong && t->scalar_type() != at::kInt)) return nullptr;
+  return t->is_contiguous() && t->device() == like.device() ? t : nullptr;
+}
+// None (-1) or a symbol below `symbols`.
+bool padding_arg(PyObject* o, int64_t symbols, int64_t* padding) {
+  *padding = -1;
+  if (o == Py_None) return true;
+  if (!PyLong_CheckExact(o)) return false;
+  *padding = PyLong_AsLongLong(o);
+  if (*padding == -1 && PyErr_Occurred()) PyErr_Clear();
+  return *padding >= 0 && *padding < symbols;
+}
+bool scale_arg(PyObject* o, float* scale) {
+  if (!PyFloat_CheckExact(o)) return false;
+  *scale = static_cast<float>(PyFloat_AS_DOUBLE(o));
+  return std::isfinite(PyFloat_AS_DOUBLE(o));
+}
+
+// embedding(tokens, weight, scale, padding_idx)
+PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  float scale;
+  int64_t padding;
+  if (nargs != 4 || !scale_arg(args[2], &scale) || !plain_mode()) return none();
+  const at::Tensor* weight = plain_object(args[1]);
+  if (weight == nullptr || weight->dim() != 2 || weight->get_device() != c10::cuda::current_device()) return none();
+  const at::Tensor* tokens = token_arg(args[0], *weight);
+  const int type = type_code(*weight);
+  const int64_t stride = row_stride(*weight), symbols = weight->size(0), width = weight->size(1);
+  if (tokens == nullptr || type < 0 || stride < 0 || !padding_arg(args[3], symbols, &padding) || has_tangent(weight)) return none();
+  at::DimVector shape(tokens->sizes());
+  shape.push_back(width);
+  at::Tensor y = empty_on(*weight, shape, weight->scalar_type());
+  const auto stream = c10::cuda::getCurrentCUDAStream(weight->get_device()).stream();
+  int rc;
+  {
+    ThreadsRun unlocked;
+    rc = triturus_b200_embedding(tokens->const_data_ptr(), static_cast<int>(tokens->element_size()), weight->const_data_ptr(), y.mutable_data_ptr(),
+                                 tokens->numel(), symbols, width, stride, type, scale, stream);
+  }
+  if (rc != TRITURUS_B200_OK) return failed("triturus_b200_embedding", rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// embedding_backward(dy, tokens, symbols, scale, padding_idx)
+PyObject* embedding_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  float scale;
+  int64_t padding;
+  if (nargs != 5 || !PyLong_CheckExact(args[2]) || !scale_arg(args[3], &scale) || !plain_mode()) return none();
+  const int64_t symbols = PyLong_AsLongLong(args[2]);
+  if (symbols == -1 && PyErr_Occurred()) PyErr_Clear();
+  const at::Tensor* dy = plain_object(args[0]);
+  if (symbols < 1 || dy == nullptr || dy->dim() < 1 || dy->get_device() != c10::cuda::current_device()) return none();
+  const at::Tensor* tokens = token_arg(args[1], *dy);
+  const int type = type_code(*dy);
+  const int64_t stride = row_stride(*dy), width = dy->size(-1);
+  if (tokens == nullptr || type < 0 || stride < 0 || tokens->sizes() != dy->sizes().slice(0, dy->dim() - 1) ||
+      !padding_arg(args[4], symbols, &padding))
+    return none();
+  const int64_t count = tokens->numel();
+  const size_t bytes = triturus_b200_embedding_backward_workspace_bytes(count, symbols, width);
+  if (bytes == 0) return none();  // (sizes that the library refuses)
+  at::Tensor dweight = empty_on(*dy, {symbols, width}, dy->scalar_type());
+  at::Tensor ws = empty_on(*dy, {static_cast<int64_t>(bytes)}, at::kByte);
+  const auto stream = c10::cuda::getCurrentCUDAStream(dy->get_device()).stream();
+  int rc;
+  {
+    ThreadsRun unlocked;
+    rc = triturus_b200_embedding_backward(dy->const_data_ptr(), tokens->const_data_ptr(), static_cast<int>(tokens->element_size()),
+                                          dweight.mutable_data_ptr(), count, symbols, width, stride, type, scale, padding, ws.mutable_data_ptr(), bytes, stream);
+  }
+  if (rc != TRITURUS_B200_OK) return failed("triturus_b200_embedding_backward", rc);
+  return THPVariable_Wrap(std::move(dweight));
+  END_HANDLE_TH_ERRORS
+}
+
 // set_up(error_class, copy_flop_rows, copy_flop_strided)
 PyObject* set_up(PyObject*, PyObject* args) {
   PyObject* cls;
@@ -410,6 +491,10 @@ PyMethodDef methods[] = {
      "clip_grad_norm(grads, max_norm, norm_type, scale) -> Tensor or None"},
     {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(sample)), METH_FASTCALL,
      "sample(logits, noise, temperature, top_k, top_p, min_p, return_logprob) -> Tensor, tuple or None"},
+    {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding)), METH_FASTCALL,
+     "embedding(tokens, weight, scale, padding_idx) -> Tensor or None"},
+    {"embedding_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding_backward)), METH_FASTCALL,
+     "embedding_backward(dy, tokens, symbols, scale, padding_idx) -> Tensor or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Small calls of triturus_b200 from C++.", -1, methods, nullptr, nullptr, nullptr, nullptr};
