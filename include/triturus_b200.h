@@ -346,6 +346,38 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
                                      size_t workspace_bytes, void* stream);
 
 /*
+ * Cross entropy of a linear layer over many symbols, whose logits z = x weight^T are never kept as a whole:
+ *   lse[i] = log sum over v of exp z[i, v],  loss_i = lse[i] - z[i, target_i], or 0 where target_i is ignore_index.
+ * x [rows, width] and weight [symbols, width] are of `type`, their rows x_stride and weight_stride elements apart; target holds 64- or 32-bit whole
+ * numbers (target_bytes) one after the other; another target outside of 0 ... symbols - 1 makes the row's loss NaN.  loss is [rows] (reduction NONE), or
+ * one number: the sum, or MEAN, that sum over the number of targets that are not ignored (0 where there is none).
+ * Products of 16-bit operands are exact and added in 32 bits; 32-bit operands are taken apart into three parts of 8 digits each, whose six largest
+ * products give about the accuracy of 32-bit arithmetic.  An infinity among 32-bit operands counts as NaN.
+ * Workspace (256-byte aligned, may hold anything): its size depends on the pointers and strides, since operands whose rows are not on 16-byte
+ * boundaries, and 32-bit ones, are copied into it.  At most 2^30 of each size.  status_dev as above.
+ */
+#define TRITURUS_B200_REDUCTION_NONE 0
+#define TRITURUS_B200_REDUCTION_MEAN 1
+#define TRITURUS_B200_REDUCTION_SUM 2
+size_t triturus_b200_linear_cross_entropy_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width,
+                                                          int64_t x_stride, int64_t weight_stride, int type);
+int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const void* target, int target_bytes, float* loss, float* lse,
+                                       int64_t rows, int64_t symbols, int64_t width, int64_t x_stride, int64_t weight_stride, int type,
+                                       int reduction, int64_t ignore_index, void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream);
+/*
+ * Its gradients for dloss ([rows] or one number, as loss is) and the lse of the forward call, with d[i, v] = g_i (exp(z[i, v] - lse[i]) - [v = target_i])
+ * and g the share of dloss (0 for ignored targets, NaN for those outside): dx = d weight [rows, width], dweight = d^T x [symbols, width], back to
+ * back and of `type`; either may be NULL.  d is computed for a piece of the symbols at a time, 2^28 numbers or, for many rows, 256 symbols, and rounded to
+ * 16 bits where the operands have 16; in float16 relative to the largest finite |dloss|.
+ */
+size_t triturus_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width,
+                                                                   int64_t x_stride, int64_t weight_stride, int type);
+int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* x, const void* weight, const void* target, int target_bytes,
+                                                const float* lse, void* dx, void* dweight, int64_t rows, int64_t symbols, int64_t width,
+                                                int64_t x_stride, int64_t weight_stride, int type, int reduction, int64_t ignore_index,
+                                                void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream);
+
+/*
  * Self-test of the error path behind `status_dev` (no counterpart in the reference, whose kernels have no waits
  * that could time out apart from the unbounded spin lock of triturus/lt2exp.py:498-506).  Launches one 64-thread
  * block in which a warp waits on a barrier that nobody signals, with a wait limit of `limit_cycles` GPU clock

@@ -8,6 +8,7 @@ from . import lm2exp as _lm2exp_module
 from . import lt2exp as _lt2exp_module
 from ._native import NativeLibraryError, check_status, colmax
 from .clip import clip_grad_norm_, grad_norm
+from .cross_entropy import linear_cross_entropy, linear_cross_entropy_backward
 from .embedding import embedding, embedding_backward
 from .host import lm2exp_host, lt2exp_host
 from .lm2exp import lm2exp
@@ -35,6 +36,8 @@ __all__ = [
     "is_triturus_tf32_enabled",
     "layer_norm",
     "layer_norm_backward",
+    "linear_cross_entropy",
+    "linear_cross_entropy_backward",
     "lm2exp",
     "lm2exp_host",
     "lt2exp",

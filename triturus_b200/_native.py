@@ -51,6 +51,10 @@ EXPORTED_SYMBOLS = (
     "triturus_b200_embedding",
     "triturus_b200_embedding_backward",
     "triturus_b200_embedding_backward_workspace_bytes",
+    "triturus_b200_linear_cross_entropy",
+    "triturus_b200_linear_cross_entropy_workspace_bytes",
+    "triturus_b200_linear_cross_entropy_backward",
+    "triturus_b200_linear_cross_entropy_backward_workspace_bytes",
     "triturus_b200_lm2exp_static_max_columns",
     "triturus_b200_lm2exp_f32_static",
 )
@@ -196,6 +200,21 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.triturus_b200_embedding_backward.restype = c_int
     lib.triturus_b200_embedding_backward.argtypes = [
         c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_int64, c_void_p, c_size_t, c_void_p,
+    ]  # fmt: skip
+    operands = [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]
+    lib.triturus_b200_linear_cross_entropy_workspace_bytes.restype = c_size_t
+    lib.triturus_b200_linear_cross_entropy_workspace_bytes.argtypes = operands
+    lib.triturus_b200_linear_cross_entropy_backward_workspace_bytes.restype = c_size_t
+    lib.triturus_b200_linear_cross_entropy_backward_workspace_bytes.argtypes = operands
+    lib.triturus_b200_linear_cross_entropy.restype = c_int
+    lib.triturus_b200_linear_cross_entropy.argtypes = [
+        c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int64,
+        c_void_p, c_size_t, c_void_p, c_void_p,
+    ]  # fmt: skip
+    lib.triturus_b200_linear_cross_entropy_backward.restype = c_int
+    lib.triturus_b200_linear_cross_entropy_backward.argtypes = [
+        c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int,
+        c_int, c_int64, c_void_p, c_size_t, c_void_p, c_void_p,
     ]  # fmt: skip
     return lib
 
@@ -976,3 +995,89 @@ def _embedding_backward_fake(dy, tokens, symbols, scale, padding_idx):
 
     _check_backward(dy, tokens, symbols, scale, padding_idx)
     return dy.new_empty((symbols, dy.shape[-1]))
+
+
+# ---------------------------------------------------------------------------- cross entropy over many symbols
+
+
+def _linear_cross_entropy_impl(
+    x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduction: int, ignore_index: int
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """`reduction`: the library's code."""
+    _require_cuda(x)
+    symbols, width = weight.shape
+    lse = torch.empty(target.shape, dtype=torch.float32, device=x.device)
+    loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=x.device)
+    target = target.contiguous()
+    (xr, xs), (wr, ws) = _rows(x), _rows(weight)
+    sizes = target.numel(), symbols, width, xs, ws, _TYPE_CODES[x.dtype]
+    with _on_device(x.device) as idx:
+        nbytes = int(LIB.triturus_b200_linear_cross_entropy_workspace_bytes(xr.data_ptr(), wr.data_ptr(), *sizes))
+        space = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
+        rc = LIB.triturus_b200_linear_cross_entropy(
+            xr.data_ptr(), wr.data_ptr(), target.data_ptr(), target.element_size(), loss.data_ptr(), lse.data_ptr(), *sizes, reduction, ignore_index,
+            space.data_ptr(), nbytes, _status_word(x.device).data_ptr(), _raw_stream(idx),
+        )  # fmt: skip
+    _check(rc, "triturus_b200_linear_cross_entropy")
+    return loss, lse
+
+
+def _linear_cross_entropy_backward_impl(
+    dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, reduction: int, ignore_index: int,
+    x_grad: bool, weight_grad: bool,
+) -> tuple[torch.Tensor, torch.Tensor]:  # fmt: skip
+    """Gradients that are not wanted are empty tensors."""
+    _require_cuda(x)
+    symbols, width = weight.shape
+    dx = torch.empty(x.shape if x_grad else (0,), dtype=x.dtype, device=x.device)
+    dweight = torch.empty(weight.shape if weight_grad else (0,), dtype=x.dtype, device=x.device)
+    dloss, target, lse = dloss.contiguous(), target.contiguous(), lse.contiguous()
+    (xr, xs), (wr, ws) = _rows(x), _rows(weight)
+    sizes = target.numel(), symbols, width, xs, ws, _TYPE_CODES[x.dtype]
+    with _on_device(x.device) as idx:
+        nbytes = int(LIB.triturus_b200_linear_cross_entropy_backward_workspace_bytes(xr.data_ptr(), wr.data_ptr(), *sizes))
+        space = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
+        rc = LIB.triturus_b200_linear_cross_entropy_backward(
+            dloss.data_ptr(), xr.data_ptr(), wr.data_ptr(), target.data_ptr(), target.element_size(), lse.data_ptr(),
+            _ptr(dx) if x_grad else None, _ptr(dweight) if weight_grad else None, *sizes, reduction, ignore_index,
+            space.data_ptr(), nbytes, _status_word(x.device).data_ptr(), _raw_stream(idx),
+        )  # fmt: skip
+    _check(rc, "triturus_b200_linear_cross_entropy_backward")
+    return dx, dweight
+
+
+@torch.library.custom_op("triturus::linear_cross_entropy", mutates_args=(), device_types="cuda")
+def linear_cross_entropy_op(
+    x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduction: int, ignore_index: int
+) -> tuple[torch.Tensor, torch.Tensor]:
+    from .cross_entropy import _check as check
+
+    check(x, weight, target, ignore_index)
+    return _linear_cross_entropy_impl(x, weight, target, reduction, ignore_index)
+
+
+@torch.library.custom_op("triturus::linear_cross_entropy_backward", mutates_args=(), device_types="cuda")
+def linear_cross_entropy_backward_op(
+    dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, reduction: int, ignore_index: int,
+    x_grad: bool, weight_grad: bool,
+) -> tuple[torch.Tensor, torch.Tensor]:  # fmt: skip
+    from .cross_entropy import _check_backward
+
+    _check_backward(dloss, x, weight, target, lse, reduction, ignore_index)
+    return _linear_cross_entropy_backward_impl(dloss, x, weight, target, lse, reduction, ignore_index, x_grad, weight_grad)
+
+
+@linear_cross_entropy_op.register_fake
+def _linear_cross_entropy_fake(x, weight, target, reduction, ignore_index):
+    from .cross_entropy import _check as check
+
+    check(x, weight, target, ignore_index)
+    return x.new_empty(target.shape if reduction == 0 else (), dtype=torch.float32), x.new_empty(target.shape, dtype=torch.float32)
+
+
+@linear_cross_entropy_backward_op.register_fake
+def _linear_cross_entropy_backward_fake(dloss, x, weight, target, lse, reduction, ignore_index, x_grad, weight_grad):
+    from .cross_entropy import _check_backward
+
+    _check_backward(dloss, x, weight, target, lse, reduction, ignore_index)
+    return x.new_empty(x.shape if x_grad else (0,)), weight.new_empty(weight.shape if weight_grad else (0,))

@@ -21,6 +21,7 @@
 #include "lt2exp_duo_kernel.cuh"
 #include "lt2exp_pair3x_kernel.cuh"
 #include "direct_kernels.cuh"
+#include "tensor_map.cuh"
 
 namespace tb200 {
 
@@ -209,25 +210,7 @@ __global__ void __launch_bounds__(64) wait_timeout_selftest_kernel(int* status, 
   __syncthreads();
 }
 
-// ----------------------------------------------------------------------------- driver entry point for tensor maps
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-    }
-  });
-  return fn;
-}
+// ----------------------------------------------------------------------------- tensor maps
 
 // fp32 tensor map of rank `rank`; dims/strides listed innermost first, strides in elements
 // (strides[0] is the innermost stride and must be 1).

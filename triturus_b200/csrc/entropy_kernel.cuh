@@ -1,0 +1,537 @@
+// Matrix products of the cross entropy over many symbols: one kernel on CTA pairs (tcgen05 cta_group::2), four uses.
+//
+//   STATS   z = x W^T, of which only each row's running maximum and sum of exponentials over a span of symbols is kept,
+//           and the logit of the row's own symbol
+//   PROB    d = (exp(z - lse) - [symbol]) g over a piece of the symbols, rounded to 16 bits for the products that follow
+//   OUT_X   dx = d W       (W's symbols are the contraction)
+//   OUT_W   dW = d^T x     (the positions are the contraction)
+//
+// Both CTAs of a pair hold 128 rows of the 256 x BN tile and half of its columns' operand: a stage of 64 contraction values is 16 KB + 16 KB to
+// a CTA, which TMA brings (no multicast) and signals at the leader's barrier, whose one thread issues the MMAs for both tensor
+// cores.  The accumulator is double-buffered in tensor memory, so that what is done with a tile (8 warps, a row and half
+// of the columns to a thread) runs beside the products of the next one.  Operands are taken as they lie: x and W by rows, d and W and x for the
+// gradients across them (MN-major).
+//
+// 32-bit operands (WIDE) come as three planes of bfloat16 whose sum they are, exactly: 8 + 8 + 8 of the 24 digits.  Six products of planes, the
+// smallest first, leave out what is below 2^-24 of a product of two numbers.  The tensor core cuts off what does not fit its accumulator, half a
+// unit of the last place for each of many additions; so WIDE tiles are 128 columns, and every kDrain k-blocks the accumulator is added to sums in registers.
+#pragma once
+
+#include "packs.cuh"
+#include "ptx.cuh"
+
+namespace tb200 {
+
+enum EntropyMode { ENTROPY_STATS, ENTROPY_PROB, ENTROPY_OUT_X, ENTROPY_OUT_W };
+
+// What OUT_X and OUT_W do with a product.
+enum EntropyDest {
+  DEST_FINAL,      // rounded to the result's type
+  DEST_PART,       // written to a 32-bit part
+  DEST_PART_ADD,   // added to it
+  DEST_FINAL_ADD,  // added to it, rounded and written to the result
+};
+
+template <int MODE_, bool WIDE_>
+struct EntropyCfg {
+  static constexpr int MODE = MODE_;
+  static constexpr bool WIDE = WIDE_;
+  static constexpr bool A_MN = MODE == ENTROPY_OUT_W;
+  static constexpr bool B_MN = MODE == ENTROPY_OUT_X || MODE == ENTROPY_OUT_W;
+  static constexpr int BM = 128;  // rows of a CTA
+  static constexpr int BN = WIDE ? 128 : 256;
+  static constexpr int BNH = BN / 2;
+  static constexpr int BK = 64;
+  static constexpr int NS = WIDE ? 8 : 6;
+  static constexpr int TERMS = WIDE ? 6 : 1;
+  static constexpr int kDrain = 4;  // k-blocks of an accumulator, where WIDE
+  static constexpr int A_TILE = BM * BK * 2;
+  static constexpr int B_TILE = BNH * BK * 2;
+  static constexpr int STAGE = A_TILE + B_TILE;
+  static constexpr int MN_BOX = 64 * BK * 2;  // 64 rows or columns of an MN-major operand
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int NTHREADS = (4 + EPI_WARPS) * 32;
+  static constexpr int BOX = 32 * 128;
+  static constexpr int COLS = BNH;  // columns of a thread: the two halves of the tile go to four warps each
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int NBAR = 2 * NS + 4;
+  static constexpr int SMEM_BYTES = 1024 + NS * STAGE + EPI_WARPS * BOX + NBAR * 8 + 16;
+  static_assert(SMEM_BYTES <= 232448, "shared memory capacity");
+};
+
+struct EntropyParams {
+  int rows, cols;         // of the product
+  int kblocks;            // of the whole contraction
+  int tiles_m, units_n;   // row tiles; column tiles, or spans of them (STATS)
+  int span, tiles_n;      // column tiles of a span; in all
+  int group;              // row tiles that are gone over together
+  int splits, kb_split;   // parts of the contraction, and their k-blocks
+  int units;              // tiles_m * units_n * splits
+  int b_row, b_k;         // where the piece begins in W: as rows of the product's columns, as contraction values
+  uint32_t idesc;
+  int half;               // 16-bit operands are float16 and not bfloat16
+  // STATS: parts [units_n * 2][rows] of maximum and sum, and the logits of the rows' own symbols
+  float2* stats;
+  float* picked;
+  // STATS and PROB
+  const void* target;
+  int target_wide;        // 64 bits
+  int64_t ignore;
+  int64_t symbols;
+  // PROB
+  const float* lse;
+  const float* dloss;     // [rows], or one number
+  int per_row;
+  const float* factors;   // what dloss is multiplied by; what the gradients are
+  uint16_t* d;            // [planes][rows][d_pitch]
+  int64_t d_pitch, d_plane;
+  // OUT
+  int dest;
+  void* out;              // rows of `out_pitch` elements of `out_type`
+  int64_t out_pitch;
+  int out_type;
+  int out_vec;            // its rows are on boundaries of four elements
+  float* part;            // [splits][rows][part_pitch]
+  int64_t part_pitch;
+  int* status;
+};
+
+// f16 or bf16 operands, fp32 accumulator: descriptor of M x N MMAs; `half`: float16.
+__host__ __device__ constexpr uint32_t umma_idesc_16(int m, int n, bool half, bool a_mn, bool b_mn) {
+  return (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Shared-memory descriptor of an MN-major operand of 16-bit elements: boxes of 64 consecutive rows or columns (128 bytes) by BK contraction
+// values with the 128-byte swizzle, one after the other (leading byte offset); groups of eight contraction values are 1024 bytes apart
+// (stride byte offset).  One MMA (16 contraction values) spans two groups: the next adds 2048 bytes, 128 to the encoded address.
+__device__ __forceinline__ uint64_t umma_desc_mn16_sw128(uint32_t smem_addr, uint32_t box_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>((box_bytes >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+__device__ __forceinline__ void umma_16_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// TMA load into this CTA's shared memory whose bytes are counted at a barrier of the pair's leader.
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* tmap, uint32_t leader_bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// The 16 high bits of a number as bfloat16 (cut off, not rounded), and what they leave, exactly.  Three of these take a number apart.
+__device__ __forceinline__ uint32_t plane_bits(float x) { return __float_as_uint(x) >> 16; }
+__device__ __forceinline__ float plane_rest(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (u & 0x7f800000u) == 0x7f800000u ? 0.f : x - __uint_as_float(u & 0xffff0000u);  // (an infinity or NaN is in the first plane alone)
+}
+
+__device__ __forceinline__ int64_t entropy_target(const EntropyParams& p, int64_t row) {
+  return p.target_wide ? static_cast<const int64_t*>(p.target)[row] : static_cast<int64_t>(static_cast<const int32_t*>(p.target)[row]);
+}
+
+template <class Cfg>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg::NTHREADS, 1)
+entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const EntropyParams p) {
+  constexpr int BM = Cfg::BM, BN = Cfg::BN, BNH = Cfg::BNH, BK = Cfg::BK, NS = Cfg::NS, MODE = Cfg::MODE;
+  constexpr bool WIDE = Cfg::WIDE;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* boxes = smem + NS * Cfg::STAGE;  // one to an epilogue warp
+  uint64_t* bars = reinterpret_cast<uint64_t*>(boxes + Cfg::EPI_WARPS * Cfg::BOX);
+  uint64_t* full = bars;              // [NS] (leader's copy is used) the bytes of both CTAs landed
+  uint64_t* stage_empty = bars + NS;  // [NS] the MMAs that read the stage are done (committed by the leader)
+  uint64_t* acc_full = bars + 2 * NS;  // [2] accumulator complete (committed by the leader)
+  uint64_t* acc_empty = acc_full + 2;  // [2] (leader's copy is used) read by the epilogues of both CTAs
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const AbortCtl ctl{abort_flag, p.status};
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&stage_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_empty[s], 2 * Cfg::EPI_WARPS);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+  }
+  cluster_sync_all();  // (both CTAs exist and have their barriers before anything crosses between them, the allocation too)
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+
+  // tile(tm, un, tn, k0, k1, first, last) for each tile of this pair in turn: row tile, column unit (which is a span of tiles in STATS) and tile, k-blocks,
+  // and whether it is the unit's first and last.  A group of row tiles is gone over column by column: the pairs that run at the same
+  // time share rows and columns through the L2 cache.
+  const auto walk = [&](auto&& tile) {
+    for (int u = pair; u < p.units; u += npairs) {
+      const int of_split = p.tiles_m * p.units_n;
+      const int ks = u / of_split, r = u - ks * of_split;
+      const int of_group = p.group * p.units_n;
+      const int g = r / of_group, rg = r - g * of_group;
+      const int rows_here = min(p.group, p.tiles_m - g * p.group);
+      const int un = rg / rows_here, tm = g * p.group + rg - un * rows_here;
+      const int k0 = ks * p.kb_split, k1 = min(p.kblocks, k0 + p.kb_split);
+      const int first = un * p.span, last = min(p.tiles_n, first + p.span) - 1;
+      for (int tn = first; tn <= last; ++tn)
+        if (!tile(tm, un, tn, ks, k0, k1, tn == first, tn == last)) return;
+    }
+  };
+  // k-blocks of an accumulator that begins at kb
+  const auto drain_end = [&](int kb, int k1) { return WIDE ? min(kb + Cfg::kDrain, k1) : k1; };
+  constexpr int plane_a[6] = {2, 0, 1, 1, 0, 0}, plane_b[6] = {0, 2, 1, 0, 1, 0};  // the smallest products first
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (this CTA's halves)
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      walk([&](int tm, int, int tn, int, int k0, int k1, bool, bool) {
+        const int a0 = tm * (2 * BM) + static_cast<int>(rank) * BM;
+        const int b0 = p.b_row + tn * BN + static_cast<int>(rank) * BNH;
+        for (int kd = k0; kd < k1; kd = drain_end(kd, k1)) {
+          const int ke = drain_end(kd, k1);
+#pragma unroll
+          for (int t = 0; t < Cfg::TERMS; ++t) {
+            const int pa = WIDE ? plane_a[t] : 0, pb = WIDE ? plane_b[t] : 0;
+            for (int kb = kd; kb < ke; ++kb, ++it) {
+              const int s = it % NS;
+              if (!(ok = mbar_wait(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
+              if (leader) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE);
+              const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
+              uint8_t* a = smem + s * Cfg::STAGE;
+              uint8_t* b = a + Cfg::A_TILE;
+              const int ka = kb * BK, kw = p.b_k + kb * BK;
+              if constexpr (Cfg::A_MN) {
+#pragma unroll
+                for (int g = 0; g < BM / 64; ++g) tma_load_3d_pair(a + g * Cfg::MN_BOX, &tmap_a, bar, a0 + g * 64, ka, pa);
+              } else {
+                tma_load_3d_pair(a, &tmap_a, bar, ka, a0, pa);
+              }
+              if constexpr (Cfg::B_MN) {
+#pragma unroll
+                for (int g = 0; g < BNH / 64; ++g) tma_load_3d_pair(b + g * Cfg::MN_BOX, &tmap_b, bar, b0 + g * 64, kw, pb);
+              } else {
+                tma_load_3d_pair(b, &tmap_b, bar, kw, b0, pb);
+              }
+            }
+          }
+        }
+        return true;
+      });
+      // The leader's commits arrive on both CTAs' stage_empty barriers: this CTA stays until the last ones are in.
+      for (uint32_t d = ok ? min(it, static_cast<uint32_t>(NS)) : 0u; ok && d > 0; --d)
+        ok = mbar_wait(&stage_empty[(it - d) % NS], ((it - d) / NS) & 1, ctl, STATUS_TIMEOUT_PRODUCER);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (leader only)
+    if (leader && lane == 0) {
+      constexpr uint32_t STAGE_ENC = Cfg::STAGE >> 4;
+      constexpr uint32_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;  // 16 contraction values
+      const uint32_t a_at = smem_u32(smem), b_at = a_at + Cfg::A_TILE;
+      const uint64_t da0 = Cfg::A_MN ? umma_desc_mn16_sw128(a_at, Cfg::MN_BOX) : umma_desc_k_sw128(a_at);
+      const uint64_t db0 = Cfg::B_MN ? umma_desc_mn16_sw128(b_at, Cfg::MN_BOX) : umma_desc_k_sw128(b_at);
+      uint32_t s = 0, ph = 0, drains = 0;
+      walk([&](int, int, int, int, int k0, int k1, bool, bool) {
+        for (int kd = k0; kd < k1; kd = drain_end(kd, k1), ++drains) {
+          const int stages = (drain_end(kd, k1) - kd) * Cfg::TERMS;
+          const int buf = drains & 1;
+          if (!mbar_wait(&acc_empty[buf], ((drains >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
+          tc_fence_after_sync();
+          const uint32_t d = tmem_base + buf * BN;
+          for (int i = 0; i < stages; ++i) {
+            if (!mbar_wait(&full[s], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
+            tc_fence_after_sync();
+            const uint64_t da = da0 + s * STAGE_ENC, db = db0 + s * STAGE_ENC;
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, da + a_step * k, db + b_step * k, p.idesc, i > 0 || k > 0 ? 1u : 0u);
+            umma_commit_pair_mcast(smem_u32(&stage_empty[s]), 3);
+            if (++s == NS) {
+              s = 0;
+              ph ^= 1;
+            }
+          }
+          umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
+        }
+        return true;
+      });
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ epilogue: a row and half of the tile's columns to a thread
+    const int q = warp & 3, h = (warp - 4) >> 2;
+    uint8_t* box = boxes + (warp - 4) * Cfg::BOX;
+    constexpr int CHUNKS = Cfg::COLS / 32;
+    uint32_t drains = 0;
+    float sum[WIDE ? CHUNKS : 1][32];  // WIDE: what the accumulators of a tile add up to
+
+    // of the unit's row (STATS), of the tile's row (PROB)
+    float top = -INFINITY, total = 0.f, lse = 0.f, lse2 = 0.f, g = 0.f;
+    int64_t target = -1;
+    bool ignored = false;
+    const float alpha = MODE == ENTROPY_OUT_X || MODE == ENTROPY_OUT_W ? p.factors[1] : 1.f;
+
+    walk([&](int tm, int un, int tn, int ks, int k0, int k1, bool first, bool last) {
+      const int row0 = tm * (2 * BM) + static_cast<int>(rank) * BM + q * 32;  // of the warp
+      const int row = row0 + lane;
+      const int col0 = tn * BN + h * Cfg::COLS;                               // of the thread
+      const bool valid = row < p.rows;
+      if constexpr (MODE == ENTROPY_STATS || MODE == ENTROPY_PROB) {
+        if (first) {
+          top = -INFINITY;
+          total = 0.f;
+          const int64_t t = valid ? entropy_target(p, row) : p.ignore;
+          ignored = t == p.ignore;
+          target = ignored ? -1 : t - p.b_row;
+          if constexpr (MODE == ENTROPY_PROB) {
+            lse = valid ? p.lse[row] : 0.f;
+            lse2 = lse * LOG2E_F;
+            g = ignored ? 0.f : t < 0 || t >= p.symbols ? __int_as_float(0x7fc00000) : p.dloss[p.per_row ? row : 0] * p.factors[0];
+          }
+        }
+      }
+
+      // 32 columns of the product from column c0 on
+      const auto process = [&](float (&v)[32], int c, int plane) {
+        const int c0 = col0 + c * 32;
+        if constexpr (MODE == ENTROPY_STATS) {
+          if (c0 + 32 > p.cols) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c0 + e >= p.cols) v[e] = -INFINITY;
+          }
+          const int64_t at = target - c0;
+          if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
+            float z = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) z = at == e ? v[e] : z;
+            if (valid && at >= 0 && at < 32) p.picked[row] = z;
+          }
+          float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int e = 4; e < 32; ++e) m[e & 3] = fmaxf(m[e & 3], v[e]);
+          const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
+          const float base = now == -INFINITY ? 0.f : now, base2 = base * LOG2E_F;
+          float s[4] = {total * ex2_approx((top - base) * LOG2E_F), 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e & 3] += ex2_approx(WIDE ? (v[e] - base) * LOG2E_F : fmaf(v[e], LOG2E_F, -base2));
+          total = (s[0] + s[1]) + (s[2] + s[3]);
+          top = now;
+        } else if constexpr (MODE == ENTROPY_PROB) {
+          if (plane == 0) {
+            const bool part = c0 + 32 > p.cols;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              v[e] = ex2_approx(WIDE ? (v[e] - lse) * LOG2E_F : fmaf(v[e], LOG2E_F, -lse2)) * g;
+              if (part && c0 + e >= p.cols) v[e] = 0.f;
+            }
+            const int64_t at = target - c0;
+            if (__any_sync(0xffffffffu, ignored || (at >= 0 && at < 32))) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                if (at == e) v[e] -= g;
+                if (ignored) v[e] = 0.f;  // (whatever its logits are)
+              }
+            }
+          }
+          // 64 bytes of the row's 128 in the box
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if constexpr (WIDE) {
+              w[e] = plane_bits(v[2 * e]) | plane_bits(v[2 * e + 1]) << 16;
+              v[2 * e] = plane_rest(v[2 * e]);
+              v[2 * e + 1] = plane_rest(v[2 * e + 1]);
+            } else if (p.half) {
+              const __half2 x = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+              w[e] = *reinterpret_cast<const uint32_t*>(&x);
+            } else {
+              const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+              w[e] = *reinterpret_cast<const uint32_t*>(&x);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(box + lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4)) =
+                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+          if (c & 1) {
+            __syncwarp();
+            const int cb = c0 - 32 + (lane & 7) * 8;
+            uint16_t* to = p.d + plane * p.d_plane + cb;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3);
+              if (row0 + r < p.rows && cb < p.d_pitch)
+                *reinterpret_cast<uint4*>(to + static_cast<int64_t>(row0 + r) * p.d_pitch) =
+                    *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            }
+            __syncwarp();
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_float4(v[4 * j] * alpha, v[4 * j + 1] * alpha, v[4 * j + 2] * alpha, v[4 * j + 3] * alpha);
+          __syncwarp();
+          const int cb = c0 + (lane & 7) * 4;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            if (row0 + r >= p.rows || cb >= p.cols) continue;
+            float4 x = *reinterpret_cast<const float4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            float4* part = reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(ks) * p.rows + row0 + r) * p.part_pitch + cb);
+            if (p.dest == DEST_PART_ADD || p.dest == DEST_FINAL_ADD) {
+              const float4 y = *part;
+              x.x += y.x;
+              x.y += y.y;
+              x.z += y.z;
+              x.w += y.w;
+            }
+            if (p.dest == DEST_PART || p.dest == DEST_PART_ADD) {
+              *part = x;
+              continue;
+            }
+            const int64_t at = static_cast<int64_t>(row0 + r) * p.out_pitch + cb;
+            const float xs[4] = {x.x, x.y, x.z, x.w};
+            const auto put = [&](auto t) {
+              using T = decltype(t);
+              T* out = static_cast<T*>(p.out) + at;
+              Pack<T, 4 * static_cast<int>(sizeof(T))> y;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y.v[e] = from_float<T>(xs[e]);
+              if (p.out_vec && cb + 4 <= p.cols) {
+                *reinterpret_cast<Pack<T, 4 * static_cast<int>(sizeof(T))>*>(out) = y;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (cb + e < p.cols) out[e] = y.v[e];
+              }
+            };
+            if constexpr (WIDE) {
+              put(0.f);
+            } else if (p.half) {
+              put(__half());
+            } else {
+              put(__nv_bfloat16());
+            }
+          }
+          __syncwarp();
+        }
+      };
+
+      const bool rows_exist = tm * (2 * BM) + static_cast<int>(rank) * BM < p.rows;
+      for (int kd = k0; kd < k1; kd = drain_end(kd, k1), ++drains) {
+        const int buf = drains & 1;
+        if (!mbar_wait_warp(&acc_full[buf], (drains >> 1) & 1, ctl, STATUS_TIMEOUT_EPILOGUE)) return false;
+        tc_fence_after_sync();
+        const uint32_t empty = map_to_cta(smem_u32(&acc_empty[buf]), 0);
+        const uint32_t at = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN + h * Cfg::COLS;
+        const auto release = [&] {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(empty);
+        };
+        // (columns that do not exist are left out too, but not the second half of a box that is written as a whole)
+        const int chunks = !rows_exist ? 0 : min(CHUNKS, ((p.cols - col0 + 63) >> 6) * 2);
+        if (chunks <= 0) {
+          release();
+          continue;
+        }
+        if constexpr (WIDE) {
+          uint32_t v[32];
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c) {
+            tmem_ld_32x32(at + c * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sum[c][e] = (kd == k0 ? 0.f : sum[c][e]) + __uint_as_float(v[e]);
+          }
+          release();
+          if (drain_end(kd, k1) == k1) {
+#pragma unroll
+            for (int plane = 0; plane < (MODE == ENTROPY_PROB ? 3 : 1); ++plane)
+#pragma unroll
+              for (int c = 0; c < CHUNKS; ++c) process(sum[c], c, plane);
+          }
+        } else {
+          uint32_t v[2][32];
+          tmem_ld_32x32(at, v[0]);
+#pragma unroll 1
+          for (int cc = 0; cc < chunks; cc += 2) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int c = cc + k;
+              tmem_ld_wait();
+              if (c + 1 < chunks) {
+                tmem_ld_32x32(at + (c + 1) * 32, v[k ^ 1]);
+              } else {
+                release();
+              }
+              float f[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[k][e]);
+              process(f, c, 0);
+            }
+          }
+        }
+      }
+      if constexpr (MODE == ENTROPY_STATS) {
+        if (last && valid) p.stats[(static_cast<int64_t>(un) * 2 + h) * p.rows + row] = make_float2(top, total);
+      }
+      return true;
+    });
+  }
+
+  // ------------------------------------------------------------------ teardown
+  // Neither CTA may leave while the other can still signal into its shared memory or use its half of the tensor memory.
+  tc_fence_before_sync();
+  cluster_sync_all();
+  if (*abort_flag) {  // copies in flight still write into this block's shared memory
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) {
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+  }
+  cluster_sync_all();
+}
+
+}  // namespace tb200

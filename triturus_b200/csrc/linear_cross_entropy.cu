@@ -1,0 +1,574 @@
+// Cross entropy of a linear layer over many symbols, in pieces of the symbols and without keeping the logits.
+//
+//   z = x W^T,  lse_i = log sum_v exp z_iv,  loss_i = lse_i - z_i,t_i
+//   d_iv = g_i (exp(z_iv - lse_i) - [v = t_i]),  dx = d W,  dW = d^T x
+//
+// Forward: one launch of products whose tiles go no further than registers (entropy_kernel.cuh), and one that joins what the spans
+// of symbols gave.  Backward: for each piece of the symbols the logits once more, as d in 16 bits, which two products then read.  The pieces
+// are as large as kMostLogits allows; what they add to dx is kept in 32 bits.  Bound by the tensor cores (8 N V D operations a training step,
+// of which 2 N V D for the logits that were not kept), for few rows by reading W.
+#include <algorithm>
+#include <atomic>
+
+#include "entropy_kernel.cuh"
+#include "tensor_map.cuh"
+
+namespace tb200 {
+namespace {
+
+constexpr int64_t kMostLogits = 1ll << 28;  // of a piece, times its planes
+constexpr int64_t kPiece = 256;             // symbols of a piece: a multiple of these
+constexpr int64_t kMostStats = 1ll << 26;   // bytes of the spans' maxima and sums, about
+
+// ----------------------------------------------------------------------------- operands that TMA cannot read in place
+
+// Rows of 16-bit elements one after the other on 16-byte boundaries; 32-bit elements as three planes of them.
+template <class T>
+__global__ void __launch_bounds__(256) entropy_planes_kernel(const T* x, int64_t rows, int width, int64_t stride, uint16_t* out, int64_t pitch, int64_t plane) {
+  const int64_t all = rows * (pitch / 8);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / (pitch / 8);
+    const int c = static_cast<int>(i - row * (pitch / 8)) * 8;
+    const T* src = x + row * stride + c;
+    Pack<T, 8 * static_cast<int>(sizeof(T))> v;
+    if (c + 8 <= width && reinterpret_cast<uintptr_t>(src) % sizeof(v) == 0) {
+      v = *reinterpret_cast<const Pack<T, 8 * static_cast<int>(sizeof(T))>*>(src);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.v[e] = c + e < width ? src[e] : from_float<T>(0.f);
+    }
+    uint16_t* to = out + row * pitch + c;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(&v);
+    } else {
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = plane_bits(v.v[2 * e]) | plane_bits(v.v[2 * e + 1]) << 16;
+          v.v[2 * e] = plane_rest(v.v[2 * e]);
+          v.v[2 * e + 1] = plane_rest(v.v[2 * e + 1]);
+        }
+        *reinterpret_cast<uint4*>(to + p * plane) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------- small kernels around the products
+
+struct JoinArgs {
+  const float2* stats;  // [parts][rows]
+  const float* picked;
+  const void* target;
+  float *loss, *lse;
+  double2* sums;  // of each block: losses, and how many there are
+  int64_t ignore, symbols;
+  int rows, parts, target_wide, reduction;
+};
+
+__device__ __forceinline__ int64_t index_at(const void* a, int wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(a)[i] : static_cast<int64_t>(static_cast<const int32_t*>(a)[i]);
+}
+
+// (m, s) stands for s exp(m).
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
+  return make_float2(m, a.y * ex2_approx((a.x - base) * LOG2E_F) + b.y * ex2_approx((b.x - base) * LOG2E_F));
+}
+
+__device__ __forceinline__ void put_loss(const JoinArgs& p, double sum, double count) {
+  *p.loss = static_cast<float>(p.reduction == TRITURUS_B200_REDUCTION_MEAN ? sum / fmax(count, 1.0) : sum);
+}
+
+// 32 rows to a block, a warp to every 32nd part.
+__global__ void __launch_bounds__(1024) entropy_join_kernel(const JoinArgs p) {
+  __shared__ float2 of_warp[32][32];
+  const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+  const int row = static_cast<int>(blockIdx.x) * 32 + lane;
+  const bool valid = row < p.rows;
+  float2 a = make_float2(-INFINITY, 0.f);
+  if (valid) {
+#pragma unroll 4
+    for (int i = warp; i < p.parts; i += 32) a = join(a, p.stats[static_cast<int64_t>(i) * p.rows + row]);
+  }
+  of_warp[warp][lane] = a;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int w = 1; w < 32; ++w) a = join(a, of_warp[w][lane]);
+  const float lse = (a.x == -INFINITY ? 0.f : a.x) + logf(a.y);
+  float loss = 0.f;
+  bool given = false;
+  if (valid) {
+    const int64_t t = index_at(p.target, p.target_wide, row);
+    given = t != p.ignore;
+    if (given) loss = t < 0 || t >= p.symbols ? __int_as_float(0x7fc00000) : lse - p.picked[row];
+    p.lse[row] = lse;
+    if (p.reduction == TRITURUS_B200_REDUCTION_NONE) p.loss[row] = loss;
+  }
+  if (p.reduction == TRITURUS_B200_REDUCTION_NONE) return;
+  double sum = loss;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int count = __popc(__ballot_sync(0xffffffffu, given));
+  if (lane != 0) return;
+  if (gridDim.x == 1)
+    put_loss(p, sum, count);
+  else
+    p.sums[blockIdx.x] = make_double2(sum, count);
+}
+
+__global__ void __launch_bounds__(256) entropy_loss_kernel(const JoinArgs p, int blocks) {
+  __shared__ double2 part[256];
+  double2 a = make_double2(0.0, 0.0);
+  for (int i = static_cast<int>(threadIdx.x); i < blocks; i += 256) {
+    a.x += p.sums[i].x;
+    a.y += p.sums[i].y;
+  }
+  part[threadIdx.x] = a;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (static_cast<int>(threadIdx.x) < o) {
+      part[threadIdx.x].x += part[threadIdx.x + o].x;
+      part[threadIdx.x].y += part[threadIdx.x + o].y;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) put_loss(p, part[0].x, part[0].y);
+}
+
+// factors[0]: what dloss is multiplied by in d; factors[1]: what dx and dW are multiplied by.  In float16 d is scaled so that the largest |dloss|
+// stands for 2^15: |d| is at most that, and a probability of 2^-29 still has all of its digits.
+__global__ void __launch_bounds__(1024) entropy_factors_kernel(const float* dloss, int per_row, const void* target, int target_wide, int64_t ignore, int rows,
+                                                               int mean, int half, float* factors) {
+  __shared__ float top_of[32];
+  __shared__ int count_of[32];
+  const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+  float top = 0.f;
+  int count = 0;
+  for (int i = static_cast<int>(threadIdx.x); i < rows; i += 1024) {
+    if (index_at(target, target_wide, i) == ignore) continue;
+    ++count;
+    if (per_row) {
+      const float g = fabsf(dloss[i]);
+      if (g < INFINITY) top = fmaxf(top, g);
+    }
+  }
+  if (!per_row) {
+    const float g = fabsf(dloss[0]);
+    if (g < INFINITY) top = g;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+  }
+  if (lane == 0) {
+    top_of[warp] = top;
+    count_of[warp] = count;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  count = 0;
+  for (int w = 0; w < 32; ++w) {
+    top = fmaxf(top, top_of[w]);
+    count += count_of[w];
+  }
+  const float share = mean ? 1.f / static_cast<float>(max(count, 1)) : 1.f;
+  if (half) {
+    top = top == 0.f ? 1.f : fmaxf(top, 0x1p-100f);
+    factors[0] = 32768.f / top;
+    factors[1] = top * share * 0x1p-15f;
+  } else {
+    factors[0] = share;
+    factors[1] = 1.f;
+  }
+}
+
+// The parts of a product added up: out[r, c] = sum over s of part[s][r][c].
+template <class T>
+__global__ void __launch_bounds__(256) entropy_sum_kernel(const float* part, int splits, int64_t rows, int cols, int64_t pitch, T* out) {
+  const int64_t all = rows * cols;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = i / cols;
+    const float* from = part + r * pitch + (i - r * cols);
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += from[k * rows * pitch];
+    out[i] = from_float<T>(s);
+  }
+}
+
+// ----------------------------------------------------------------------------- host
+
+int size_of(int type) { return type == TRITURUS_B200_TYPE_F32 ? 4 : 2; }
+bool sizes_ok(int64_t rows, int64_t symbols, int64_t width, int type) {
+  const int64_t most = 1 << 30;
+  return rows >= 0 && rows <= most && symbols > 0 && symbols <= most && width > 0 && width <= most && type >= TRITURUS_B200_TYPE_F32 &&
+         type <= TRITURUS_B200_TYPE_F16;
+}
+int64_t up_to(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+int64_t parts_of(int64_t n, int64_t unit) { return (n + unit - 1) / unit; }
+
+// A 16-bit matrix as TMA reads it.
+struct Matrix {
+  const void* data;
+  int64_t rows, width, pitch, plane;
+  int planes;
+};
+bool in_place(const void* data, int64_t rows, int64_t stride, int type) {
+  return type != TRITURUS_B200_TYPE_F32 && aligned_to(data, 16) && (rows == 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)));
+}
+// Bytes of the copy of an operand that is not read in place.
+size_t copy_bytes(const void* data, int64_t rows, int64_t width, int64_t stride, int type) {
+  if (in_place(data, rows, stride, type)) return 0;
+  return static_cast<size_t>(up_to(rows * up_to(width, 8) * 2 * (type == TRITURUS_B200_TYPE_F32 ? 3 : 1), 256));
+}
+
+int make_map(CUtensorMap* map, const Matrix& m, int box_x, int box_y, int type) {
+  const EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return TRITURUS_B200_EDRIVER;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(m.width), static_cast<cuuint64_t>(m.rows), static_cast<cuuint64_t>(m.planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(m.pitch) * 2, static_cast<cuuint64_t>(m.plane) * 2};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_x), static_cast<cuuint32_t>(box_y), 1}, step[3] = {1, 1, 1};
+  const CUresult rc = fn(map, type == TRITURUS_B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                         const_cast<void*>(m.data), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? TRITURUS_B200_OK : TRITURUS_B200_ETENSORMAP;
+}
+
+int copy_grid(int64_t items) { return static_cast<int>(std::min<int64_t>(parts_of(items, 256), static_cast<int64_t>(device_sms()) * 16)); }
+
+// The operand itself or, copied to `space`, one that TMA can read.
+int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t stride, int type, void* space, cudaStream_t st) {
+  m->rows = rows;
+  m->width = width;
+  m->planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
+  if (in_place(data, rows, stride, type)) {
+    m->data = data;
+    m->pitch = rows == 1 ? up_to(width, 8) : stride;
+    m->plane = rows * m->pitch;
+    return TRITURUS_B200_OK;
+  }
+  m->data = space;
+  m->pitch = up_to(width, 8);
+  m->plane = rows * m->pitch;
+  const dim3 grid(static_cast<unsigned>(copy_grid(rows * (m->pitch / 8))));
+  const auto run = [&](auto t) {
+    using T = decltype(t);
+    return launch_of(entropy_planes_kernel<T>, grid, 256, 0, st, nullptr, static_cast<const T*>(data), rows, static_cast<int>(width), stride,
+                     static_cast<uint16_t*>(space), m->pitch, m->plane);
+  };
+  return type == TRITURUS_B200_TYPE_F32 ? run(0.f) : type == TRITURUS_B200_TYPE_BF16 ? run(__nv_bfloat16()) : run(__half());
+}
+
+int pairs_in_all() { return std::max(1, device_sms() / 2); }
+
+template <class Cfg>
+int launch_products(const Matrix& a, const Matrix& b, EntropyParams p, int type, cudaStream_t st) {
+  CUtensorMap ta, tb;
+  int rc = Cfg::A_MN ? make_map(&ta, a, 64, Cfg::BK, type) : make_map(&ta, a, Cfg::BK, Cfg::BM, type);
+  if (rc == TRITURUS_B200_OK) rc = Cfg::B_MN ? make_map(&tb, b, 64, Cfg::BK, type) : make_map(&tb, b, Cfg::BK, Cfg::BNH, type);
+  if (rc != TRITURUS_B200_OK) return rc;
+  const auto kern = entropy_kernel<Cfg>;
+  static std::atomic<bool> known[64];
+  int dev = 0;
+  if (code_of(cudaGetDevice(&dev)) != TRITURUS_B200_OK || dev < 0 || dev >= 64) return TRITURUS_B200_ELAUNCH;
+  if (!known[dev].load(std::memory_order_relaxed)) {
+    rc = code_of(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+    if (rc != TRITURUS_B200_OK) return rc;
+    known[dev].store(true, std::memory_order_relaxed);
+  }
+  p.half = type == TRITURUS_B200_TYPE_F16;
+  p.idesc = umma_idesc_16(2 * Cfg::BM, Cfg::BN, p.half != 0, Cfg::A_MN, Cfg::B_MN);
+  p.group = 8;
+  const int64_t units = static_cast<int64_t>(p.tiles_m) * p.units_n * p.splits;
+  if (units > INT32_MAX) return TRITURUS_B200_EINVAL;
+  p.units = static_cast<int>(units);
+  const int pairs = static_cast<int>(std::min<int64_t>(units, pairs_in_all()));
+  return launch_of(kern, dim3(static_cast<unsigned>(2 * pairs)), Cfg::NTHREADS, Cfg::SMEM_BYTES, st, nullptr, ta, tb, p);
+}
+template <int MODE>
+int run_products(const Matrix& a, const Matrix& b, const EntropyParams& p, int type, cudaStream_t st) {
+  return type == TRITURUS_B200_TYPE_F32 ? launch_products<EntropyCfg<MODE, true>>(a, b, p, type, st) : launch_products<EntropyCfg<MODE, false>>(a, b, p, type, st);
+}
+
+// Tiles of a product with rows x cols results and a contraction of k.
+EntropyParams tiles_of(int64_t rows, int64_t cols, int64_t k, int type) {
+  EntropyParams p = {};
+  p.rows = static_cast<int>(rows);
+  p.cols = static_cast<int>(cols);
+  p.kblocks = static_cast<int>(parts_of(k, 64));
+  p.tiles_m = static_cast<int>(parts_of(rows, 256));
+  p.tiles_n = static_cast<int>(parts_of(cols, type == TRITURUS_B200_TYPE_F32 ? 128 : 256));
+  p.units_n = p.tiles_n;
+  p.span = 1;
+  p.splits = 1;
+  p.kb_split = p.kblocks;
+  return p;
+}
+
+// Spans of some column tiles, so that each pair has many and what they give is little: their last ones keep few pairs from the end.
+EntropyParams stats_of(int64_t rows, int64_t symbols, int64_t width, int type) {
+  EntropyParams p = tiles_of(rows, symbols, width, type);
+  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  int64_t span = std::clamp<int64_t>(tiles / (static_cast<int64_t>(pairs_in_all()) * 16), 1, 8);
+  span = std::max(span, parts_of(static_cast<int64_t>(p.tiles_n) * rows * 16, kMostStats));
+  p.span = static_cast<int>(std::min<int64_t>(span, p.tiles_n));
+  p.units_n = static_cast<int>(parts_of(p.tiles_n, p.span));
+  return p;
+}
+
+// Where tiles are fewer than pairs of CTAs, the contraction is split among them, in parts of eight k-blocks or more.
+void split(EntropyParams& p) {
+  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(pairs_in_all() / tiles, p.kblocks / 8));
+  p.kb_split = static_cast<int>(parts_of(p.kblocks, most));
+  p.splits = static_cast<int>(parts_of(p.kblocks, p.kb_split));
+}
+
+struct Space {  // the workspace as it is handed out
+  char* at;
+  size_t used;
+  void* take(size_t bytes) {
+    void* p = at + used;
+    used += (bytes + 255) & ~static_cast<size_t>(255);
+    return p;
+  }
+};
+
+struct ForwardSpace {
+  void *x, *weight;
+  float2* stats;
+  float* picked;
+  double2* sums;
+  size_t bytes;
+};
+ForwardSpace forward_space(void* base, const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width, int64_t x_stride,
+                           int64_t weight_stride, int type) {
+  Space s = {static_cast<char*>(base), 0};
+  ForwardSpace f;
+  f.x = s.take(copy_bytes(x, rows, width, x_stride, type));
+  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type));
+  f.stats = static_cast<float2*>(s.take(static_cast<size_t>(stats_of(rows, symbols, width, type).units_n) * 2 * static_cast<size_t>(rows) * sizeof(float2)));
+  f.picked = static_cast<float*>(s.take(static_cast<size_t>(rows) * sizeof(float)));
+  f.sums = static_cast<double2*>(s.take(static_cast<size_t>(parts_of(rows, 32)) * sizeof(double2)));
+  f.bytes = s.used;
+  return f;
+}
+
+struct BackwardPlan {
+  int64_t piece, pieces, d_pitch, part_pitch;
+  EntropyParams x, w;  // of a whole piece
+};
+BackwardPlan backward_plan(int64_t rows, int64_t symbols, int64_t width, int type) {
+  BackwardPlan b;
+  const int planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
+  const int64_t most = std::max(kPiece, kMostLogits / planes / std::max<int64_t>(rows, 1) / kPiece * kPiece);
+  b.pieces = parts_of(symbols, most);
+  b.piece = std::min(up_to(parts_of(symbols, b.pieces), kPiece), symbols);
+  b.pieces = parts_of(symbols, b.piece);
+  b.d_pitch = up_to(b.piece, 64);
+  b.part_pitch = up_to(width, 4);
+  b.x = tiles_of(rows, width, b.piece, type);
+  b.w = tiles_of(b.piece, width, rows, type);
+  split(b.x);
+  split(b.w);
+  return b;
+}
+struct BackwardSpace {
+  void *x, *weight;
+  float *factors, *x_part, *w_part;
+  uint16_t* d;
+  size_t bytes;
+};
+BackwardSpace backward_space(void* base, const BackwardPlan& b, const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width,
+                             int64_t x_stride, int64_t weight_stride, int type) {
+  Space s = {static_cast<char*>(base), 0};
+  BackwardSpace f;
+  f.x = s.take(copy_bytes(x, rows, width, x_stride, type));
+  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type));
+  f.factors = static_cast<float*>(s.take(2 * sizeof(float)));
+  f.d = static_cast<uint16_t*>(s.take(static_cast<size_t>(rows) * static_cast<size_t>(b.d_pitch) * 2 * (type == TRITURUS_B200_TYPE_F32 ? 3 : 1)));
+  const size_t row = static_cast<size_t>(b.part_pitch) * sizeof(float);
+  f.x_part = static_cast<float*>(s.take(b.x.splits > 1 || b.pieces > 1 ? static_cast<size_t>(b.x.splits) * static_cast<size_t>(rows) * row : 0));
+  f.w_part = static_cast<float*>(s.take(b.w.splits > 1 ? static_cast<size_t>(b.w.splits) * static_cast<size_t>(b.piece) * row : 0));
+  f.bytes = s.used;
+  return f;
+}
+
+int sum_parts(const EntropyParams& p, int64_t width, void* out, int type, cudaStream_t st) {
+  const auto run = [&](auto t) {
+    using T = decltype(t);
+    return launch_of(entropy_sum_kernel<T>, dim3(static_cast<unsigned>(copy_grid(static_cast<int64_t>(p.rows) * width))), 256, 0, st, nullptr,
+                     static_cast<const float*>(p.part), p.splits, static_cast<int64_t>(p.rows), static_cast<int>(width), p.part_pitch, static_cast<T*>(out));
+  };
+  return type == TRITURUS_B200_TYPE_F32 ? run(0.f) : type == TRITURUS_B200_TYPE_BF16 ? run(__nv_bfloat16()) : run(__half());
+}
+
+bool reduction_ok(int r) { return r >= TRITURUS_B200_REDUCTION_NONE && r <= TRITURUS_B200_REDUCTION_SUM; }
+
+}  // namespace
+}  // namespace tb200
+
+using namespace tb200;
+
+extern "C" {
+
+size_t triturus_b200_linear_cross_entropy_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width,
+                                                          int64_t x_stride, int64_t weight_stride, int type) {
+  if (!sizes_ok(rows, symbols, width, type) || rows == 0) return 0;
+  return forward_space(nullptr, x, weight, rows, symbols, width, x_stride, weight_stride, type).bytes;
+}
+
+int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const void* target, int target_bytes, float* loss, float* lse,
+                                       int64_t rows, int64_t symbols, int64_t width, int64_t x_stride, int64_t weight_stride, int type,
+                                       int reduction, int64_t ignore_index, void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream) {
+  if (!sizes_ok(rows, symbols, width, type) || !reduction_ok(reduction) || (target_bytes != 4 && target_bytes != 8)) return TRITURUS_B200_EINVAL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    if (reduction == TRITURUS_B200_REDUCTION_NONE) return TRITURUS_B200_OK;
+    if (loss == nullptr) return TRITURUS_B200_EINVAL;
+    return aligned_to(loss, 4) ? code_of(cudaMemsetAsync(loss, 0, sizeof(float), st)) : TRITURUS_B200_EALIGN;
+  }
+  if (x == nullptr || weight == nullptr || target == nullptr || loss == nullptr || lse == nullptr || workspace == nullptr) return TRITURUS_B200_EINVAL;
+  if (!aligned_to(x, size_of(type)) || !aligned_to(weight, size_of(type)) || !aligned_to(target, target_bytes) || !aligned_to(loss, 4) ||
+      !aligned_to(lse, 4) || !aligned_to(workspace, 256))
+    return TRITURUS_B200_EALIGN;
+  const ForwardSpace space = forward_space(workspace, x, weight, rows, symbols, width, x_stride, weight_stride, type);
+  if (workspace_bytes < space.bytes) return TRITURUS_B200_EWORKSPACE;
+
+  Matrix a, b;
+  int rc = prepare(&a, x, rows, width, x_stride, type, space.x, st);
+  if (rc == TRITURUS_B200_OK) rc = prepare(&b, weight, symbols, width, weight_stride, type, space.weight, st);
+  if (rc != TRITURUS_B200_OK) return rc;
+  EntropyParams p = stats_of(rows, symbols, width, type);
+  p.stats = space.stats;
+  p.picked = space.picked;
+  p.target = target;
+  p.target_wide = target_bytes == 8;
+  p.ignore = ignore_index;
+  p.symbols = symbols;
+  p.status = status_dev;
+  rc = run_products<ENTROPY_STATS>(a, b, p, type, st);
+  if (rc != TRITURUS_B200_OK) return rc;
+
+  JoinArgs j = {};
+  j.stats = space.stats;
+  j.picked = space.picked;
+  j.target = target;
+  j.loss = loss;
+  j.lse = lse;
+  j.sums = space.sums;
+  j.ignore = ignore_index;
+  j.symbols = symbols;
+  j.rows = static_cast<int>(rows);
+  j.parts = p.units_n * 2;
+  j.target_wide = p.target_wide;
+  j.reduction = reduction;
+  const int blocks = static_cast<int>(parts_of(rows, 32));
+  rc = launch_of(entropy_join_kernel, dim3(static_cast<unsigned>(blocks)), 1024, 0, st, nullptr, j);
+  if (rc == TRITURUS_B200_OK && reduction != TRITURUS_B200_REDUCTION_NONE && blocks > 1)
+    rc = launch_of(entropy_loss_kernel, dim3(1), 256, 0, st, nullptr, j, blocks);
+  return rc;
+}
+
+size_t triturus_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width,
+                                                                   int64_t x_stride, int64_t weight_stride, int type) {
+  if (!sizes_ok(rows, symbols, width, type) || rows == 0) return 0;
+  return backward_space(nullptr, backward_plan(rows, symbols, width, type), x, weight, rows, symbols, width, x_stride, weight_stride, type).bytes;
+}
+
+int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* x, const void* weight, const void* target, int target_bytes,
+                                                const float* lse, void* dx, void* dweight, int64_t rows, int64_t symbols, int64_t width,
+                                                int64_t x_stride, int64_t weight_stride, int type, int reduction, int64_t ignore_index,
+                                                void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream) {
+  if (!sizes_ok(rows, symbols, width, type) || !reduction_ok(reduction) || (target_bytes != 4 && target_bytes != 8)) return TRITURUS_B200_EINVAL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int size = size_of(type);
+  if (!aligned_to(dx, size) || !aligned_to(dweight, size)) return TRITURUS_B200_EALIGN;
+  if (rows == 0) return dweight == nullptr ? TRITURUS_B200_OK : code_of(cudaMemsetAsync(dweight, 0, static_cast<size_t>(symbols) * static_cast<size_t>(width) * size, st));
+  if (dloss == nullptr || x == nullptr || weight == nullptr || target == nullptr || lse == nullptr || workspace == nullptr) return TRITURUS_B200_EINVAL;
+  if (!aligned_to(x, size) || !aligned_to(weight, size) || !aligned_to(target, target_bytes) || !aligned_to(dloss, 4) || !aligned_to(lse, 4) ||
+      !aligned_to(workspace, 256))
+    return TRITURUS_B200_EALIGN;
+  const BackwardPlan plan = backward_plan(rows, symbols, width, type);
+  const BackwardSpace space = backward_space(workspace, plan, x, weight, rows, symbols, width, x_stride, weight_stride, type);
+  if (workspace_bytes < space.bytes) return TRITURUS_B200_EWORKSPACE;
+  if (dx == nullptr && dweight == nullptr) return TRITURUS_B200_OK;
+
+  Matrix mx, mw;
+  int rc = prepare(&mx, x, rows, width, x_stride, type, space.x, st);
+  if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, type, space.weight, st);
+  const int wide = target_bytes == 8;
+  if (rc == TRITURUS_B200_OK)
+    rc = launch_of(entropy_factors_kernel, dim3(1), 1024, 0, st, nullptr, dloss, reduction == TRITURUS_B200_REDUCTION_NONE ? 1 : 0, target, wide, ignore_index,
+                   static_cast<int>(rows), reduction == TRITURUS_B200_REDUCTION_MEAN ? 1 : 0, type == TRITURUS_B200_TYPE_F16 ? 1 : 0, space.factors);
+  Matrix md = {};
+  md.data = space.d;
+  md.rows = rows;
+  md.pitch = plan.d_pitch;
+  md.plane = rows * plan.d_pitch;
+  md.planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
+  const int vec = width % 4 == 0;
+  for (int64_t i = 0; i < plan.pieces && rc == TRITURUS_B200_OK; ++i) {
+    const int64_t first = i * plan.piece, piece = std::min(plan.piece, symbols - first);
+    EntropyParams p = tiles_of(rows, piece, width, type);
+    p.b_row = static_cast<int>(first);
+    p.target = target;
+    p.target_wide = wide;
+    p.ignore = ignore_index;
+    p.symbols = symbols;
+    p.lse = lse;
+    p.dloss = dloss;
+    p.per_row = reduction == TRITURUS_B200_REDUCTION_NONE;
+    p.factors = space.factors;
+    p.d = space.d;
+    p.d_pitch = md.pitch;
+    p.d_plane = md.plane;
+    p.status = status_dev;
+    rc = run_products<ENTROPY_PROB>(mx, mw, p, type, st);
+    if (rc != TRITURUS_B200_OK) break;
+    md.width = piece;
+    if (dx != nullptr) {
+      EntropyParams q = tiles_of(rows, width, piece, type);
+      q.kb_split = plan.x.kb_split;
+      q.splits = static_cast<int>(parts_of(q.kblocks, q.kb_split));
+      q.b_k = static_cast<int>(first);
+      q.factors = space.factors;
+      const bool begin = i == 0, end = i + 1 == plan.pieces && plan.x.splits == 1;
+      q.dest = begin ? end ? DEST_FINAL : DEST_PART : end ? DEST_FINAL_ADD : DEST_PART_ADD;
+      q.out = dx;
+      q.out_pitch = width;
+      q.out_vec = vec && aligned_to(dx, 4 * size);
+      q.part = space.x_part;
+      q.part_pitch = plan.part_pitch;
+      q.status = status_dev;
+      rc = run_products<ENTROPY_OUT_X>(md, mw, q, type, st);
+      if (rc == TRITURUS_B200_OK && i + 1 == plan.pieces && plan.x.splits > 1) {
+        q.splits = plan.x.splits;
+        rc = sum_parts(q, width, dx, type, st);
+      }
+      if (rc != TRITURUS_B200_OK) break;
+    }
+    if (dweight != nullptr) {
+      EntropyParams q = tiles_of(piece, width, rows, type);
+      q.kb_split = plan.w.kb_split;
+      q.splits = plan.w.splits;
+      q.factors = space.factors;
+      q.dest = q.splits == 1 ? DEST_FINAL : DEST_PART;
+      q.out = static_cast<char*>(dweight) + first * width * size;
+      q.out_pitch = width;
+      q.out_vec = vec && aligned_to(q.out, 4 * size);
+      q.part = space.w_part;
+      q.part_pitch = plan.part_pitch;
+      q.status = status_dev;
+      rc = run_products<ENTROPY_OUT_W>(md, mx, q, type, st);
+      if (rc == TRITURUS_B200_OK && q.splits > 1) rc = sum_parts(q, width, q.out, type, st);
+    }
+  }
+  return rc;
+}
+
+}  // extern "C"
