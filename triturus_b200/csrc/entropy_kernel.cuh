@@ -163,8 +163,8 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  const uint32_t rank = warp_uniform(cluster_ctarank());
   const bool leader = rank == 0;
   const AbortCtl ctl{abort_flag, p.status};
 
@@ -190,7 +190,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   tc_fence_before_sync();
   cluster_sync_all();
   tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
@@ -217,20 +217,22 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (this CTA's halves)
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      walk([&](int tm, int, int tn, int, int k0, int k1, bool, bool) {
-        const int a0 = tm * (2 * BM) + static_cast<int>(rank) * BM;
-        const int b0 = p.b_row + tn * BN + static_cast<int>(rank) * BNH;
-        for (int kd = k0; kd < k1; kd = drain_end(kd, k1)) {
-          const int ke = drain_end(kd, k1);
+    // (Here and in the issuer the whole warp runs the loop and one elected lane issues: control flow and addresses are uniform and stay in
+    // uniform registers.  One lane in a branch of its own took some 600 cycles for a stage whose MMAs take 512, or 256 where WIDE.)
+    uint32_t it = 0;
+    bool ok = true;
+    walk([&](int tm, int, int tn, int, int k0, int k1, bool, bool) {
+      const int a0 = tm * (2 * BM) + static_cast<int>(rank) * BM;
+      const int b0 = p.b_row + tn * BN + static_cast<int>(rank) * BNH;
+      for (int kd = k0; kd < k1; kd = drain_end(kd, k1)) {
+        const int ke = drain_end(kd, k1);
 #pragma unroll
-          for (int t = 0; t < Cfg::TERMS; ++t) {
-            const int pa = WIDE ? plane_a[t] : 0, pb = WIDE ? plane_b[t] : 0;
-            for (int kb = kd; kb < ke; ++kb, ++it) {
-              const int s = it % NS;
-              if (!(ok = mbar_wait(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
+        for (int t = 0; t < Cfg::TERMS; ++t) {
+          const int pa = WIDE ? plane_a[t] : 0, pb = WIDE ? plane_b[t] : 0;
+          for (int kb = kd; kb < ke; ++kb, ++it) {
+            const uint32_t s = it % NS;
+            if (!(ok = mbar_wait_warp(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
+            if (elect_one_sync()) {
               if (leader) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE);
               const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
               uint8_t* a = smem + s * Cfg::STAGE;
@@ -249,18 +251,18 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                 tma_load_3d_pair(b, &tmap_b, bar, kw, b0, pb);
               }
             }
+            __syncwarp();
           }
         }
-        return true;
-      });
-      // The leader's commits arrive on both CTAs' stage_empty barriers: this CTA stays until the last ones are in.
-      for (uint32_t d = ok ? min(it, static_cast<uint32_t>(NS)) : 0u; ok && d > 0; --d)
-        ok = mbar_wait(&stage_empty[(it - d) % NS], ((it - d) / NS) & 1, ctl, STATUS_TIMEOUT_PRODUCER);
-    }
-    __syncwarp();
+      }
+      return true;
+    });
+    // The leader's commits arrive on both CTAs' stage_empty barriers: this CTA stays until the last ones are in.
+    for (uint32_t d = ok ? min(it, static_cast<uint32_t>(NS)) : 0u; ok && d > 0; --d)
+      ok = mbar_wait_warp(&stage_empty[(it - d) % NS], ((it - d) / NS) & 1, ctl, STATUS_TIMEOUT_PRODUCER);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (leader only)
-    if (leader && lane == 0) {
+    if (leader) {
       constexpr uint32_t STAGE_ENC = Cfg::STAGE >> 4;
       constexpr uint32_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;  // 16 contraction values
       const uint32_t a_at = smem_u32(smem), b_at = a_at + Cfg::A_TILE;
@@ -270,28 +272,30 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       walk([&](int, int, int, int, int k0, int k1, bool, bool) {
         for (int kd = k0; kd < k1; kd = drain_end(kd, k1), ++drains) {
           const int stages = (drain_end(kd, k1) - kd) * Cfg::TERMS;
-          const int buf = drains & 1;
-          if (!mbar_wait(&acc_empty[buf], ((drains >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
+          const uint32_t buf = drains & 1;
+          if (!mbar_wait_warp(&acc_empty[buf], ((drains >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
           tc_fence_after_sync();
           const uint32_t d = tmem_base + buf * BN;
           for (int i = 0; i < stages; ++i) {
-            if (!mbar_wait(&full[s], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
+            if (!mbar_wait_warp(&full[s], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
             tc_fence_after_sync();
-            const uint64_t da = da0 + s * STAGE_ENC, db = db0 + s * STAGE_ENC;
+            if (elect_one_sync()) {
+              const uint64_t da = da0 + s * STAGE_ENC, db = db0 + s * STAGE_ENC;
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, da + a_step * k, db + b_step * k, p.idesc, i > 0 || k > 0 ? 1u : 0u);
-            umma_commit_pair_mcast(smem_u32(&stage_empty[s]), 3);
+              for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, da + a_step * k, db + b_step * k, p.idesc, i > 0 || k > 0 ? 1u : 0u);
+              umma_commit_pair_mcast(smem_u32(&stage_empty[s]), 3);
+              if (i + 1 == stages) umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
+            }
+            __syncwarp();
             if (++s == NS) {
               s = 0;
               ph ^= 1;
             }
           }
-          umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
         }
         return true;
       });
     }
-    __syncwarp();
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue: a row and half of the tile's columns to a thread
     const int q = warp & 3, h = (warp - 4) >> 2;
