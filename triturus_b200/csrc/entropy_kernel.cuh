@@ -12,9 +12,13 @@
 // of the columns to a thread) runs beside the products of the next one.  Operands are taken as they lie: x and W by rows, d and W and x for the
 // gradients across them (MN-major).
 //
+// Tiles and spans end where they should for the pairs to have equal shares: a tile may have any multiple of 32 columns for its MMAs.  Where the tiles of a
+// gradient do not fill the pairs evenly, the last ones are cut along the contraction into parts, which a further launch adds.
+//
 // 32-bit operands (WIDE) come as three planes of bfloat16 whose sum they are, exactly: 8 + 8 + 8 of the 24 digits.  Six products of planes, the
-// smallest first, leave out what is below 2^-24 of a product of two numbers.  The tensor core cuts off what does not fit its accumulator, half a
-// unit of the last place for each of many additions; so WIDE tiles are 128 columns, and every kDrain k-blocks the accumulator is added to sums in registers.
+// smallest first, leave out what is below 2^-24 of a product of two numbers.  A stage holds all planes of 64 contraction values, 96 KB to a CTA, and is used
+// for 24 MMAs.  The tensor core cuts off what does not fit its accumulator, half a unit of the last place for each of many additions; so each stage has an
+// accumulator of its own, which is added to sums in registers, and tiles are 192 columns, whose sums are 96 registers of a thread.
 #pragma once
 
 #include "packs.cuh"
@@ -27,8 +31,8 @@ enum EntropyMode { ENTROPY_STATS, ENTROPY_PROB, ENTROPY_OUT_X, ENTROPY_OUT_W };
 // What OUT_X and OUT_W do with a product.
 enum EntropyDest {
   DEST_FINAL,      // rounded to the result's type
-  DEST_PART,       // written to a 32-bit part
-  DEST_PART_ADD,   // added to it
+  DEST_SUM,        // written to a 32-bit sum
+  DEST_SUM_ADD,    // added to it
   DEST_FINAL_ADD,  // added to it, rounded and written to the result
 };
 
@@ -39,21 +43,22 @@ struct EntropyCfg {
   static constexpr bool A_MN = MODE == ENTROPY_OUT_W;
   static constexpr bool B_MN = MODE == ENTROPY_OUT_X || MODE == ENTROPY_OUT_W;
   static constexpr int BM = 128;  // rows of a CTA
-  static constexpr int BN = WIDE ? 128 : 256;
+  static constexpr int BN = WIDE ? 192 : 256;
   static constexpr int BNH = BN / 2;
   static constexpr int BK = 64;
-  static constexpr int NS = WIDE ? 8 : 6;
-  static constexpr int TERMS = WIDE ? 6 : 1;
-  static constexpr int kDrain = 4;  // k-blocks of an accumulator, where WIDE
-  static constexpr int A_TILE = BM * BK * 2;
-  static constexpr int B_TILE = BNH * BK * 2;
-  static constexpr int STAGE = A_TILE + B_TILE;
+  static constexpr int NS = WIDE ? 2 : 6;
+  static constexpr int PLANES = WIDE ? 3 : 1;
   static constexpr int MN_BOX = 64 * BK * 2;  // 64 rows or columns of an MN-major operand
+  static constexpr int A_TILE = BM * BK * 2;
+  static constexpr int B_BOXES = (BNH + 63) / 64;
+  static constexpr int B_TILE = B_MN ? B_BOXES * MN_BOX : BNH * BK * 2;
+  static constexpr int STAGE = PLANES * (A_TILE + B_TILE);
   static constexpr int EPI_WARPS = 8;
   static constexpr int NTHREADS = (4 + EPI_WARPS) * 32;
   static constexpr int BOX = 32 * 128;
   static constexpr int COLS = BNH;  // columns of a thread: the two halves of the tile go to four warps each
-  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int BUF_COLS = 256;
+  static constexpr int TMEM_COLS = 2 * BUF_COLS;
   static constexpr int NBAR = 2 * NS + 4;
   static constexpr int SMEM_BYTES = 1024 + NS * STAGE + EPI_WARPS * BOX + NBAR * 8 + 16;
   static_assert(SMEM_BYTES <= 232448, "shared memory capacity");
@@ -61,16 +66,18 @@ struct EntropyCfg {
 
 struct EntropyParams {
   int rows, cols;         // of the product
-  int kblocks;            // of the whole contraction
-  int tiles_m, units_n;   // row tiles; column tiles, or spans of them (STATS)
-  int span, tiles_n;      // column tiles of a span; in all
-  int group;              // row tiles that are gone over together
-  int splits, kb_split;   // parts of the contraction, and their k-blocks
-  int units;              // tiles_m * units_n * splits
+  int kblocks;              // of the contraction
+  int tiles_m;              // row tiles
+  int units_n, unit_cols;   // a unit is a row tile and so many columns,
+  int tile_cols;            // gone over in tiles of these: one tile but for STATS
+  int group;                // row tiles that are gone over together
+  int whole;                // units that are one pair's
+  int shared;               // and those behind them whose contraction is cut
+  int splits, kb_split;     // into parts of so many k-blocks
   int b_row, b_k;         // where the piece begins in W: as rows of the product's columns, as contraction values
   uint32_t idesc;
   int half;               // 16-bit operands are float16 and not bfloat16
-  // STATS: parts [units_n * 2][rows] of maximum and sum, and the logits of the rows' own symbols
+  // STATS: [units_n * 2][rows] of maximum and sum, and the logits of the rows' own symbols
   float2* stats;
   float* picked;
   // STATS and PROB
@@ -86,20 +93,20 @@ struct EntropyParams {
   uint16_t* d;            // [planes][rows][d_pitch]
   int64_t d_pitch, d_plane;
   // OUT
-  int dest;
-  void* out;              // rows of `out_pitch` elements of `out_type`
+  int dest;               // of whole tiles
+  void* out;              // rows of `out_pitch` elements
   int64_t out_pitch;
-  int out_type;
   int out_vec;            // its rows are on boundaries of four elements
-  float* part;            // [splits][rows][part_pitch]
-  int64_t part_pitch;
+  float* sum;             // [rows][sum_pitch], what earlier pieces gave
+  int64_t sum_pitch;
+  float* part;            // [shared][splits][256][tile_cols]
   int* status;
 };
 
-// f16 or bf16 operands, fp32 accumulator: descriptor of M x N MMAs; `half`: float16.
-__host__ __device__ constexpr uint32_t umma_idesc_16(int m, int n, bool half, bool a_mn, bool b_mn) {
+// f16 or bf16 operands, fp32 accumulator: descriptor of MMAs of m rows, but for their columns n, as n / 8 from bit 17 on; `half`: float16.
+__host__ __device__ constexpr uint32_t umma_idesc_16(int m, bool half, bool a_mn, bool b_mn) {
   return (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+         (static_cast<uint32_t>(m >> 4) << 24);
 }
 
 // Shared-memory descriptor of an MN-major operand of 16-bit elements: boxes of 64 consecutive rows or columns (128 bytes) by BK contraction
@@ -144,6 +151,36 @@ __device__ __forceinline__ float plane_rest(float x) {
 
 __device__ __forceinline__ int64_t entropy_target(const EntropyParams& p, int64_t row) {
   return p.target_wide ? static_cast<const int64_t*>(p.target)[row] : static_cast<int64_t>(static_cast<const int32_t*>(p.target)[row]);
+}
+
+// Four elements of a product, in row `row` from column `col` on (those before column `end`): to the sum of the pieces or to the result.
+template <class T>
+__device__ __forceinline__ void entropy_put(const EntropyParams& p, int row, int col, float4 x, int end) {
+  float4* sum = reinterpret_cast<float4*>(p.sum + static_cast<int64_t>(row) * p.sum_pitch + col);
+  if (p.dest == DEST_SUM_ADD || p.dest == DEST_FINAL_ADD) {
+    const float4 y = *sum;
+    x.x += y.x;
+    x.y += y.y;
+    x.z += y.z;
+    x.w += y.w;
+  }
+  if (p.dest == DEST_SUM || p.dest == DEST_SUM_ADD) {
+    *sum = x;
+    return;
+  }
+  T* out = static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.out_pitch + col;
+  Pack<T, 4 * static_cast<int>(sizeof(T))> y;
+  y.v[0] = from_float<T>(x.x);
+  y.v[1] = from_float<T>(x.y);
+  y.v[2] = from_float<T>(x.z);
+  y.v[3] = from_float<T>(x.w);
+  if (p.out_vec && col + 4 <= end) {
+    *reinterpret_cast<Pack<T, 4 * static_cast<int>(sizeof(T))>*>(out) = y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < end) out[e] = y.v[e];
+  }
 }
 
 template <class Cfg>
@@ -193,26 +230,57 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  pdl_launch_dependents();
+  pdl_wait();
 
-  // tile(tm, un, tn, k0, k1, first, last) for each tile of this pair in turn: row tile, column unit (which is a span of tiles in STATS) and tile, k-blocks,
-  // and whether it is the unit's first and last.  A group of row tiles is gone over column by column: the pairs that run at the same
-  // time share rows and columns through the L2 cache.
+  // tile(t) for each tile of this pair in turn; leaves when one returns false.  A group of row tiles is gone over column by column: the pairs
+  // that run at the same time share rows and columns through the L2 cache.
+  struct Tile {
+    int tm, un;       // row tile, column unit
+    int n0, n1;       // columns
+    int mma;          // columns of its MMAs: the multiple of 32 that holds them
+    int k0, k1;       // k-blocks
+    int part;         // where it goes if it is a part of a shared tile, else -1
+    bool first, last;  // of its unit
+  };
   const auto walk = [&](auto&& tile) {
-    for (int u = pair; u < p.units; u += npairs) {
-      const int of_split = p.tiles_m * p.units_n;
-      const int ks = u / of_split, r = u - ks * of_split;
+    const auto unit = [&](int u, int k0, int k1, int part) {
       const int of_group = p.group * p.units_n;
-      const int g = r / of_group, rg = r - g * of_group;
+      const int g = u / of_group, r = u - g * of_group;
       const int rows_here = min(p.group, p.tiles_m - g * p.group);
-      const int un = rg / rows_here, tm = g * p.group + rg - un * rows_here;
-      const int k0 = ks * p.kb_split, k1 = min(p.kblocks, k0 + p.kb_split);
-      const int first = un * p.span, last = min(p.tiles_n, first + p.span) - 1;
-      for (int tn = first; tn <= last; ++tn)
-        if (!tile(tm, un, tn, ks, k0, k1, tn == first, tn == last)) return;
+      Tile t;
+      t.un = r / rows_here;
+      t.tm = g * p.group + r - t.un * rows_here;
+      t.k0 = k0;
+      t.k1 = k1;
+      t.part = part;
+      const int begin = t.un * p.unit_cols, end = min(begin + p.unit_cols, p.cols);
+      for (t.n0 = begin; t.n0 < end; t.n0 = t.n1) {
+        t.n1 = min(t.n0 + p.tile_cols, end);
+        t.mma = (t.n1 - t.n0 + 31) & ~31;
+        t.first = t.n0 == begin;
+        t.last = t.n1 == end;
+        if (!tile(t)) return false;
+      }
+      return true;
+    };
+    if constexpr (MODE == ENTROPY_OUT_X || MODE == ENTROPY_OUT_W) {
+      // Part by part, so that pairs which run at the same time have the same contraction values: with parts of equal length for all
+      // pairs, each from another place on, the operands came from memory again and again (2048 x 1024 of 50021 float16: 237 us, with two even parts 147).
+      for (int u = pair; u < p.whole + p.shared * p.splits; u += npairs) {
+        const int v = u - p.whole;
+        if (v < 0) {
+          if (!unit(u, 0, p.kblocks, -1)) return;
+        } else {
+          const int ks = v / p.shared, s = v - ks * p.shared, k0 = ks * p.kb_split;
+          if (!unit(p.whole + s, k0, min(p.kblocks, k0 + p.kb_split), s * p.splits + ks)) return;
+        }
+      }
+    } else {
+      for (int u = pair; u < p.whole; u += npairs)
+        if (!unit(u, 0, p.kblocks, -1)) return;
     }
   };
-  // k-blocks of an accumulator that begins at kb
-  const auto drain_end = [&](int kb, int k1) { return WIDE ? min(kb + Cfg::kDrain, k1) : k1; };
   constexpr int plane_a[6] = {2, 0, 1, 1, 0, 0}, plane_b[6] = {0, 2, 1, 0, 1, 0};  // the smallest products first
 
   if (warp == 0) {
@@ -221,39 +289,35 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     // uniform registers.  One lane in a branch of its own took some 600 cycles for a stage whose MMAs take 512, or 256 where WIDE.)
     uint32_t it = 0;
     bool ok = true;
-    walk([&](int tm, int, int tn, int, int k0, int k1, bool, bool) {
-      const int a0 = tm * (2 * BM) + static_cast<int>(rank) * BM;
-      const int b0 = p.b_row + tn * BN + static_cast<int>(rank) * BNH;
-      for (int kd = k0; kd < k1; kd = drain_end(kd, k1)) {
-        const int ke = drain_end(kd, k1);
+    walk([&](const Tile& t) {
+      const int a0 = t.tm * (2 * BM) + static_cast<int>(rank) * BM;
+      const int b0 = p.b_row + t.n0 + static_cast<int>(rank) * (t.mma >> 1);
+      for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
+        const uint32_t s = it % NS;
+        if (!(ok = mbar_wait_warp(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
+        if (elect_one_sync()) {
+          if (leader) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE);
+          const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
+          const int ka = kb * BK, kw = p.b_k + kb * BK;
 #pragma unroll
-        for (int t = 0; t < Cfg::TERMS; ++t) {
-          const int pa = WIDE ? plane_a[t] : 0, pb = WIDE ? plane_b[t] : 0;
-          for (int kb = kd; kb < ke; ++kb, ++it) {
-            const uint32_t s = it % NS;
-            if (!(ok = mbar_wait_warp(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
-            if (elect_one_sync()) {
-              if (leader) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE);
-              const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
-              uint8_t* a = smem + s * Cfg::STAGE;
-              uint8_t* b = a + Cfg::A_TILE;
-              const int ka = kb * BK, kw = p.b_k + kb * BK;
-              if constexpr (Cfg::A_MN) {
+          for (int plane = 0; plane < Cfg::PLANES; ++plane) {
+            uint8_t* a = smem + s * Cfg::STAGE + plane * Cfg::A_TILE;
+            uint8_t* b = smem + s * Cfg::STAGE + Cfg::PLANES * Cfg::A_TILE + plane * Cfg::B_TILE;
+            if constexpr (Cfg::A_MN) {
 #pragma unroll
-                for (int g = 0; g < BM / 64; ++g) tma_load_3d_pair(a + g * Cfg::MN_BOX, &tmap_a, bar, a0 + g * 64, ka, pa);
-              } else {
-                tma_load_3d_pair(a, &tmap_a, bar, ka, a0, pa);
-              }
-              if constexpr (Cfg::B_MN) {
-#pragma unroll
-                for (int g = 0; g < BNH / 64; ++g) tma_load_3d_pair(b + g * Cfg::MN_BOX, &tmap_b, bar, b0 + g * 64, kw, pb);
-              } else {
-                tma_load_3d_pair(b, &tmap_b, bar, kw, b0, pb);
-              }
+              for (int g = 0; g < BM / 64; ++g) tma_load_3d_pair(a + g * Cfg::MN_BOX, &tmap_a, bar, a0 + g * 64, ka, plane);
+            } else {
+              tma_load_3d_pair(a, &tmap_a, bar, ka, a0, plane);
             }
-            __syncwarp();
+            if constexpr (Cfg::B_MN) {
+#pragma unroll
+              for (int g = 0; g < Cfg::B_BOXES; ++g) tma_load_3d_pair(b + g * Cfg::MN_BOX, &tmap_b, bar, b0 + g * 64, kw, plane);
+            } else {
+              tma_load_3d_pair(b, &tmap_b, bar, kw, b0, plane);
+            }
           }
         }
+        __syncwarp();
       }
       return true;
     });
@@ -265,32 +329,40 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     if (leader) {
       constexpr uint32_t STAGE_ENC = Cfg::STAGE >> 4;
       constexpr uint32_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;  // 16 contraction values
-      const uint32_t a_at = smem_u32(smem), b_at = a_at + Cfg::A_TILE;
+      const uint32_t a_at = smem_u32(smem), b_at = a_at + Cfg::PLANES * Cfg::A_TILE;
       const uint64_t da0 = Cfg::A_MN ? umma_desc_mn16_sw128(a_at, Cfg::MN_BOX) : umma_desc_k_sw128(a_at);
       const uint64_t db0 = Cfg::B_MN ? umma_desc_mn16_sw128(b_at, Cfg::MN_BOX) : umma_desc_k_sw128(b_at);
-      uint32_t s = 0, ph = 0, drains = 0;
-      walk([&](int, int, int, int, int k0, int k1, bool, bool) {
-        for (int kd = k0; kd < k1; kd = drain_end(kd, k1), ++drains) {
-          const int stages = (drain_end(kd, k1) - kd) * Cfg::TERMS;
-          const uint32_t buf = drains & 1;
-          if (!mbar_wait_warp(&acc_empty[buf], ((drains >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
-          tc_fence_after_sync();
-          const uint32_t d = tmem_base + buf * BN;
-          for (int i = 0; i < stages; ++i) {
-            if (!mbar_wait_warp(&full[s], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
-            tc_fence_after_sync();
-            if (elect_one_sync()) {
-              const uint64_t da = da0 + s * STAGE_ENC, db = db0 + s * STAGE_ENC;
+      uint32_t s = 0, ph = 0, accs = 0;
+      // one stage into accumulator d
+      const auto multiply = [&](uint32_t d, uint32_t idesc, bool add) {
+        const uint64_t da = da0 + s * STAGE_ENC, db = db0 + s * STAGE_ENC;
 #pragma unroll
-              for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, da + a_step * k, db + b_step * k, p.idesc, i > 0 || k > 0 ? 1u : 0u);
-              umma_commit_pair_mcast(smem_u32(&stage_empty[s]), 3);
-              if (i + 1 == stages) umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
-            }
-            __syncwarp();
-            if (++s == NS) {
-              s = 0;
-              ph ^= 1;
-            }
+        for (int x = 0; x < (WIDE ? 6 : 1); ++x) {
+          const uint64_t pa = da + (WIDE ? plane_a[x] : 0) * (Cfg::A_TILE >> 4), pb = db + (WIDE ? plane_b[x] : 0) * (Cfg::B_TILE >> 4);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, pa + a_step * k, pb + b_step * k, idesc, add || x > 0 || k > 0 ? 1u : 0u);
+        }
+        umma_commit_pair_mcast(smem_u32(&stage_empty[s]), 3);
+      };
+      walk([&](const Tile& t) {
+        const uint32_t idesc = p.idesc | static_cast<uint32_t>(t.mma >> 3) << 17;
+        for (int kb = t.k0; kb < t.k1; ++kb) {
+          const uint32_t buf = accs & 1;
+          if (WIDE || kb == t.k0) {
+            if (!mbar_wait_warp(&acc_empty[buf], ((accs >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
+          }
+          if (!mbar_wait_warp(&full[s], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
+          tc_fence_after_sync();
+          const bool done = WIDE || kb + 1 == t.k1;
+          if (elect_one_sync()) {
+            multiply(tmem_base + buf * Cfg::BUF_COLS, idesc, !WIDE && kb > t.k0);
+            if (done) umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
+          }
+          __syncwarp();
+          if (done) ++accs;
+          if (++s == NS) {
+            s = 0;
+            ph ^= 1;
           }
         }
         return true;
@@ -301,7 +373,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     const int q = warp & 3, h = (warp - 4) >> 2;
     uint8_t* box = boxes + (warp - 4) * Cfg::BOX;
     constexpr int CHUNKS = Cfg::COLS / 32;
-    uint32_t drains = 0;
+    uint32_t accs = 0;
     float sum[WIDE ? CHUNKS : 1][32];  // WIDE: what the accumulators of a tile add up to
 
     // of the unit's row (STATS), of the tile's row (PROB)
@@ -310,36 +382,39 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     bool ignored = false;
     const float alpha = MODE == ENTROPY_OUT_X || MODE == ENTROPY_OUT_W ? p.factors[1] : 1.f;
 
-    walk([&](int tm, int un, int tn, int ks, int k0, int k1, bool first, bool last) {
-      const int row0 = tm * (2 * BM) + static_cast<int>(rank) * BM + q * 32;  // of the warp
+    walk([&](const Tile& t) {
+      const int row0 = t.tm * (2 * BM) + static_cast<int>(rank) * BM + q * 32;  // of the warp
       const int row = row0 + lane;
-      const int col0 = tn * BN + h * Cfg::COLS;                               // of the thread
+      const int col0 = t.n0 + h * Cfg::COLS;                                    // of the thread
       const bool valid = row < p.rows;
       if constexpr (MODE == ENTROPY_STATS || MODE == ENTROPY_PROB) {
-        if (first) {
+        if (t.first) {
           top = -INFINITY;
           total = 0.f;
-          const int64_t t = valid ? entropy_target(p, row) : p.ignore;
-          ignored = t == p.ignore;
-          target = ignored ? -1 : t - p.b_row;
+          const int64_t to = valid ? entropy_target(p, row) : p.ignore;
+          ignored = to == p.ignore;
+          target = ignored ? -1 : to - p.b_row;
           if constexpr (MODE == ENTROPY_PROB) {
             lse = valid ? p.lse[row] : 0.f;
             lse2 = lse * LOG2E_F;
-            g = ignored ? 0.f : t < 0 || t >= p.symbols ? __int_as_float(0x7fc00000) : p.dloss[p.per_row ? row : 0] * p.factors[0];
+            g = ignored ? 0.f : to < 0 || to >= p.symbols ? __int_as_float(0x7fc00000) : p.dloss[p.per_row ? row : 0] * p.factors[0];
           }
         }
       }
+      // chunks of 32 columns that this thread has in the tile
+      const bool rows_exist = t.tm * (2 * BM) + static_cast<int>(rank) * BM < p.rows;
+      const int chunks = rows_exist ? max(0, min(CHUNKS, (t.n1 - col0 + 31) >> 5)) : 0;
 
       // 32 columns of the product from column c0 on
       const auto process = [&](float (&v)[32], int c, int plane) {
         const int c0 = col0 + c * 32;
         if constexpr (MODE == ENTROPY_STATS) {
-          if (c0 + 32 > p.cols) {
+          if (c0 + 32 > t.n1) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (c0 + e >= p.cols) v[e] = -INFINITY;
+              if (c0 + e >= t.n1) v[e] = -INFINITY;
           }
-          const int64_t at = target - c0;
+          const int64_t at = target < t.n1 ? target - c0 : -1;
           if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
             float z = 0.f;
 #pragma unroll
@@ -358,12 +433,8 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           top = now;
         } else if constexpr (MODE == ENTROPY_PROB) {
           if (plane == 0) {
-            const bool part = c0 + 32 > p.cols;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              v[e] = ex2_approx(WIDE ? (v[e] - lse) * LOG2E_F : fmaf(v[e], LOG2E_F, -lse2)) * g;
-              if (part && c0 + e >= p.cols) v[e] = 0.f;
-            }
+            for (int e = 0; e < 32; ++e) v[e] = ex2_approx(WIDE ? (v[e] - lse) * LOG2E_F : fmaf(v[e], LOG2E_F, -lse2)) * g;
             const int64_t at = target - c0;
             if (__any_sync(0xffffffffu, ignored || (at >= 0 && at < 32))) {
 #pragma unroll
@@ -393,14 +464,14 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           for (int j = 0; j < 4; ++j)
             *reinterpret_cast<uint4*>(box + lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4)) =
                 make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-          if (c & 1) {
+          if ((c & 1) != 0 || c + 1 == chunks) {  // (tiles have multiples of 32 columns here, and so has d)
             __syncwarp();
-            const int cb = c0 - 32 + (lane & 7) * 8;
+            const int cb = c0 - (c & 1) * 32 + (lane & 7) * 8;
             uint16_t* to = p.d + plane * p.d_plane + cb;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int r = i * 4 + (lane >> 3);
-              if (row0 + r < p.rows && cb < p.d_pitch)
+              if (row0 + r < p.rows && cb < c0 + 32)
                 *reinterpret_cast<uint4*>(to + static_cast<int64_t>(row0 + r) * p.d_pitch) =
                     *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
             }
@@ -416,63 +487,37 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int r = i * 4 + (lane >> 3);
-            if (row0 + r >= p.rows || cb >= p.cols) continue;
+            if (row0 + r >= p.rows || cb >= t.n1) continue;
             float4 x = *reinterpret_cast<const float4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            float4* part = reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(ks) * p.rows + row0 + r) * p.part_pitch + cb);
-            if (p.dest == DEST_PART_ADD || p.dest == DEST_FINAL_ADD) {
-              const float4 y = *part;
-              x.x += y.x;
-              x.y += y.y;
-              x.z += y.z;
-              x.w += y.w;
-            }
-            if (p.dest == DEST_PART || p.dest == DEST_PART_ADD) {
-              *part = x;
+            if (t.part >= 0) {
+              const int in_tile = static_cast<int>(rank) * BM + q * 32 + r;
+              *reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(t.part) * (2 * BM) + in_tile) * p.tile_cols + (cb - t.n0)) = x;
               continue;
             }
-            const int64_t at = static_cast<int64_t>(row0 + r) * p.out_pitch + cb;
-            const float xs[4] = {x.x, x.y, x.z, x.w};
-            const auto put = [&](auto t) {
-              using T = decltype(t);
-              T* out = static_cast<T*>(p.out) + at;
-              Pack<T, 4 * static_cast<int>(sizeof(T))> y;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y.v[e] = from_float<T>(xs[e]);
-              if (p.out_vec && cb + 4 <= p.cols) {
-                *reinterpret_cast<Pack<T, 4 * static_cast<int>(sizeof(T))>*>(out) = y;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (cb + e < p.cols) out[e] = y.v[e];
-              }
-            };
             if constexpr (WIDE) {
-              put(0.f);
+              entropy_put<float>(p, row0 + r, cb, x, t.n1);
             } else if (p.half) {
-              put(__half());
+              entropy_put<__half>(p, row0 + r, cb, x, t.n1);
             } else {
-              put(__nv_bfloat16());
+              entropy_put<__nv_bfloat16>(p, row0 + r, cb, x, t.n1);
             }
           }
           __syncwarp();
         }
       };
 
-      const bool rows_exist = tm * (2 * BM) + static_cast<int>(rank) * BM < p.rows;
-      for (int kd = k0; kd < k1; kd = drain_end(kd, k1), ++drains) {
-        const int buf = drains & 1;
-        if (!mbar_wait_warp(&acc_full[buf], (drains >> 1) & 1, ctl, STATUS_TIMEOUT_EPILOGUE)) return false;
+      for (int kb = WIDE ? t.k0 : t.k1 - 1; kb < t.k1; ++kb, ++accs) {
+        const uint32_t buf = accs & 1;
+        if (!mbar_wait_warp(&acc_full[buf], (accs >> 1) & 1, ctl, STATUS_TIMEOUT_EPILOGUE)) return false;
         tc_fence_after_sync();
         const uint32_t empty = map_to_cta(smem_u32(&acc_empty[buf]), 0);
-        const uint32_t at = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN + h * Cfg::COLS;
+        const uint32_t at = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * Cfg::BUF_COLS + h * Cfg::COLS;
         const auto release = [&] {
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(empty);
         };
-        // (columns that do not exist are left out too, but not the second half of a box that is written as a whole)
-        const int chunks = !rows_exist ? 0 : min(CHUNKS, ((p.cols - col0 + 63) >> 6) * 2);
-        if (chunks <= 0) {
+        if (chunks == 0) {
           release();
           continue;
         }
@@ -480,17 +525,20 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           uint32_t v[32];
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c) {
-            tmem_ld_32x32(at + c * 32, v);
-            tmem_ld_wait();
+            if (c < chunks) {
+              tmem_ld_32x32(at + c * 32, v);
+              tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) sum[c][e] = (kd == k0 ? 0.f : sum[c][e]) + __uint_as_float(v[e]);
+              for (int e = 0; e < 32; ++e) sum[c][e] = (kb == t.k0 ? 0.f : sum[c][e]) + __uint_as_float(v[e]);
+            }
           }
           release();
-          if (drain_end(kd, k1) == k1) {
+          if (kb + 1 == t.k1) {
 #pragma unroll
             for (int plane = 0; plane < (MODE == ENTROPY_PROB ? 3 : 1); ++plane)
 #pragma unroll
-              for (int c = 0; c < CHUNKS; ++c) process(sum[c], c, plane);
+              for (int c = 0; c < CHUNKS; ++c)
+                if (c < chunks) process(sum[c], c, plane);
           }
         } else {
           uint32_t v[2][32];
@@ -500,22 +548,24 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const int c = cc + k;
-              tmem_ld_wait();
-              if (c + 1 < chunks) {
-                tmem_ld_32x32(at + (c + 1) * 32, v[k ^ 1]);
-              } else {
-                release();
-              }
-              float f[32];
+              if (c < chunks) {
+                tmem_ld_wait();
+                if (c + 1 < chunks) {
+                  tmem_ld_32x32(at + (c + 1) * 32, v[k ^ 1]);
+                } else {
+                  release();
+                }
+                float f[32];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[k][e]);
-              process(f, c, 0);
+                for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[k][e]);
+                process(f, c, 0);
+              }
             }
           }
         }
       }
       if constexpr (MODE == ENTROPY_STATS) {
-        if (last && valid) p.stats[(static_cast<int64_t>(un) * 2 + h) * p.rows + row] = make_float2(top, total);
+        if (t.last && valid) p.stats[(static_cast<int64_t>(t.un) * 2 + h) * p.rows + row] = make_float2(top, total);
       }
       return true;
     });

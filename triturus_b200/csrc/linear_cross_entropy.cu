@@ -25,6 +25,8 @@ constexpr int64_t kMostStats = 1ll << 26;   // bytes of the spans' maxima and su
 // Rows of 16-bit elements one after the other on 16-byte boundaries; 32-bit elements as three planes of them.
 template <class T>
 __global__ void __launch_bounds__(256) entropy_planes_kernel(const T* x, int64_t rows, int width, int64_t stride, uint16_t* out, int64_t pitch, int64_t plane) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int64_t all = rows * (pitch / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t row = i / (pitch / 8);
@@ -89,6 +91,8 @@ __global__ void __launch_bounds__(1024) entropy_join_kernel(const JoinArgs p) {
   const int row = static_cast<int>(blockIdx.x) * 32 + lane;
   const bool valid = row < p.rows;
   float2 a = make_float2(-INFINITY, 0.f);
+  pdl_launch_dependents();
+  pdl_wait();
   if (valid) {
 #pragma unroll 4
     for (int i = warp; i < p.parts; i += 32) a = join(a, p.stats[static_cast<int64_t>(i) * p.rows + row]);
@@ -123,6 +127,8 @@ __global__ void __launch_bounds__(1024) entropy_join_kernel(const JoinArgs p) {
 __global__ void __launch_bounds__(256) entropy_loss_kernel(const JoinArgs p, int blocks) {
   __shared__ double2 part[256];
   double2 a = make_double2(0.0, 0.0);
+  pdl_launch_dependents();
+  pdl_wait();
   for (int i = static_cast<int>(threadIdx.x); i < blocks; i += 256) {
     a.x += p.sums[i].x;
     a.y += p.sums[i].y;
@@ -148,6 +154,8 @@ __global__ void __launch_bounds__(1024) entropy_factors_kernel(const float* dlos
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
   float top = 0.f;
   int count = 0;
+  pdl_launch_dependents();
+  pdl_wait();
   for (int i = static_cast<int>(threadIdx.x); i < rows; i += 1024) {
     if (index_at(target, target_wide, i) == ignore) continue;
     ++count;
@@ -187,17 +195,29 @@ __global__ void __launch_bounds__(1024) entropy_factors_kernel(const float* dlos
   }
 }
 
-// The parts of a product added up: out[r, c] = sum over s of part[s][r][c].
+// The parts of shared tiles added up, four elements to a thread, and what is done with whole tiles.
 template <class T>
-__global__ void __launch_bounds__(256) entropy_sum_kernel(const float* part, int splits, int64_t rows, int cols, int64_t pitch, T* out) {
-  const int64_t all = rows * cols;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = i / cols;
-    const float* from = part + r * pitch + (i - r * cols);
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += from[k * rows * pitch];
-    out[i] = from_float<T>(s);
+__global__ void __launch_bounds__(256) entropy_sum_kernel(const __grid_constant__ EntropyParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int vectors = p.tile_cols / 4;  // of a tile's row, and blocks to a tile
+  const int s = static_cast<int>(blockIdx.x) / vectors;
+  const int i = (static_cast<int>(blockIdx.x) - s * vectors) * 256 + static_cast<int>(threadIdx.x);
+  const int in_tile = i / vectors, c = (i - in_tile * vectors) * 4;
+  const int u = p.whole + s, of_group = p.group * p.units_n;
+  const int g = u / of_group, r = u - g * of_group, rows_here = min(p.group, p.tiles_m - g * p.group);
+  const int row = (g * p.group + r % rows_here) * 256 + in_tile, col = r / rows_here * p.unit_cols + c;
+  if (row >= p.rows || col >= p.cols) return;
+  const float* part = p.part + (static_cast<int64_t>(s) * p.splits * 256 + in_tile) * p.tile_cols + c;
+  float4 x = *reinterpret_cast<const float4*>(part);
+  for (int k = 1; k < p.splits; ++k) {
+    const float4 y = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(k) * 256 * p.tile_cols);
+    x.x += y.x;
+    x.y += y.y;
+    x.z += y.z;
+    x.w += y.w;
   }
+  entropy_put<T>(p, row, col, x, min(p.cols, col + 4));
 }
 
 // ----------------------------------------------------------------------------- host
@@ -238,10 +258,23 @@ int make_map(CUtensorMap* map, const Matrix& m, int box_x, int box_y, int type) 
   return rc == CUDA_SUCCESS ? TRITURUS_B200_OK : TRITURUS_B200_ETENSORMAP;
 }
 
+// The launches of a call: each but the first may begin while the one before it ends, whose results it waits for.
+struct Launches {
+  cudaStream_t stream;
+  bool first = true;
+  template <class... Params, class... Args>
+  int operator()(void (*kern)(Params...), int64_t grid, int threads, size_t smem, Args&&... args) {
+    const cudaLaunchAttribute dependent = dependent_launch();
+    const int rc = launch_of(kern, dim3(static_cast<unsigned>(grid)), threads, smem, stream, first ? nullptr : &dependent, static_cast<Args&&>(args)...);
+    first = false;
+    return rc;
+  }
+};
+
 int copy_grid(int64_t items) { return static_cast<int>(std::min<int64_t>(parts_of(items, 256), static_cast<int64_t>(device_sms()) * 16)); }
 
 // The operand itself or, copied to `space`, one that TMA can read.
-int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t stride, int type, void* space, cudaStream_t st) {
+int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t stride, int type, void* space, Launches& launch) {
   m->rows = rows;
   m->width = width;
   m->planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
@@ -254,10 +287,10 @@ int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t st
   m->data = space;
   m->pitch = up_to(width, 8);
   m->plane = rows * m->pitch;
-  const dim3 grid(static_cast<unsigned>(copy_grid(rows * (m->pitch / 8))));
+  const int grid = copy_grid(rows * (m->pitch / 8));
   const auto run = [&](auto t) {
     using T = decltype(t);
-    return launch_of(entropy_planes_kernel<T>, grid, 256, 0, st, nullptr, static_cast<const T*>(data), rows, static_cast<int>(width), stride,
+    return launch(entropy_planes_kernel<T>, grid, 256, 0, static_cast<const T*>(data), rows, static_cast<int>(width), stride,
                      static_cast<uint16_t*>(space), m->pitch, m->plane);
   };
   return type == TRITURUS_B200_TYPE_F32 ? run(0.f) : type == TRITURUS_B200_TYPE_BF16 ? run(__nv_bfloat16()) : run(__half());
@@ -266,7 +299,7 @@ int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t st
 int pairs_in_all() { return std::max(1, device_sms() / 2); }
 
 template <class Cfg>
-int launch_products(const Matrix& a, const Matrix& b, EntropyParams p, int type, cudaStream_t st) {
+int launch_products(const Matrix& a, const Matrix& b, EntropyParams p, int type, Launches& launch) {
   CUtensorMap ta, tb;
   int rc = Cfg::A_MN ? make_map(&ta, a, 64, Cfg::BK, type) : make_map(&ta, a, Cfg::BK, Cfg::BM, type);
   if (rc == TRITURUS_B200_OK) rc = Cfg::B_MN ? make_map(&tb, b, 64, Cfg::BK, type) : make_map(&tb, b, Cfg::BK, Cfg::BNH, type);
@@ -281,51 +314,119 @@ int launch_products(const Matrix& a, const Matrix& b, EntropyParams p, int type,
     known[dev].store(true, std::memory_order_relaxed);
   }
   p.half = type == TRITURUS_B200_TYPE_F16;
-  p.idesc = umma_idesc_16(2 * Cfg::BM, Cfg::BN, p.half != 0, Cfg::A_MN, Cfg::B_MN);
-  p.group = 8;
-  const int64_t units = static_cast<int64_t>(p.tiles_m) * p.units_n * p.splits;
-  if (units > INT32_MAX) return TRITURUS_B200_EINVAL;
-  p.units = static_cast<int>(units);
-  const int pairs = static_cast<int>(std::min<int64_t>(units, pairs_in_all()));
-  return launch_of(kern, dim3(static_cast<unsigned>(2 * pairs)), Cfg::NTHREADS, Cfg::SMEM_BYTES, st, nullptr, ta, tb, p);
+  p.idesc = umma_idesc_16(2 * Cfg::BM, p.half != 0, Cfg::A_MN, Cfg::B_MN);
+  const int64_t pairs = std::min<int64_t>(p.whole + static_cast<int64_t>(p.shared) * p.splits, pairs_in_all());
+  return launch(kern, 2 * pairs, Cfg::NTHREADS, Cfg::SMEM_BYTES, ta, tb, p);
 }
 template <int MODE>
-int run_products(const Matrix& a, const Matrix& b, const EntropyParams& p, int type, cudaStream_t st) {
-  return type == TRITURUS_B200_TYPE_F32 ? launch_products<EntropyCfg<MODE, true>>(a, b, p, type, st) : launch_products<EntropyCfg<MODE, false>>(a, b, p, type, st);
+int run_products(const Matrix& a, const Matrix& b, const EntropyParams& p, int type, Launches& launch) {
+  int rc = type == TRITURUS_B200_TYPE_F32 ? launch_products<EntropyCfg<MODE, true>>(a, b, p, type, launch) : launch_products<EntropyCfg<MODE, false>>(a, b, p, type, launch);
+  if (rc != TRITURUS_B200_OK || p.shared == 0) return rc;
+  EntropyParams q = p;
+  q.half = type == TRITURUS_B200_TYPE_F16;
+  const int64_t grid = static_cast<int64_t>(p.shared) * (p.tile_cols / 4);
+  return type == TRITURUS_B200_TYPE_F32    ? launch(entropy_sum_kernel<float>, grid, 256, 0, q)
+         : type == TRITURUS_B200_TYPE_BF16 ? launch(entropy_sum_kernel<__nv_bfloat16>, grid, 256, 0, q)
+                                           : launch(entropy_sum_kernel<__half>, grid, 256, 0, q);
 }
 
-// Tiles of a product with rows x cols results and a contraction of k.
-EntropyParams tiles_of(int64_t rows, int64_t cols, int64_t k, int type) {
+// ----------------------------------------------------------------------------- tiles for pairs
+
+int widest(int type) { return type == TRITURUS_B200_TYPE_F32 ? 192 : 256; }
+// Cycles of a k-block of a tile of `cols` columns, by whichever takes longer: the MMAs, or what they and TMA move through 128 bytes a cycle of shared memory.
+int64_t cycles_of(int64_t cols, int type) {
+  return type == TRITURUS_B200_TYPE_F32 ? std::max(12 * cols, 1152 + 9 * cols / 2) : std::max(2 * cols, 256 + cols);
+}
+constexpr int64_t kTileCycles = 2500;    // of a tile beside its MMAs
+constexpr int64_t kSumCycles = 6000;     // of a launch that adds parts
+constexpr int64_t kBytesPerCycle = 3500;
+constexpr int64_t kMostSplits = 74;      // of a contraction
+constexpr int64_t kLeastUnits = 5;       // waves of tiles from which on their rounding up does not matter
+
+EntropyParams product_of(int64_t rows, int64_t cols, int64_t k) {
   EntropyParams p = {};
   p.rows = static_cast<int>(rows);
   p.cols = static_cast<int>(cols);
   p.kblocks = static_cast<int>(parts_of(k, 64));
   p.tiles_m = static_cast<int>(parts_of(rows, 256));
-  p.tiles_n = static_cast<int>(parts_of(cols, type == TRITURUS_B200_TYPE_F32 ? 128 : 256));
-  p.units_n = p.tiles_n;
-  p.span = 1;
-  p.splits = 1;
-  p.kb_split = p.kblocks;
+  p.group = 8;
   return p;
 }
+void set_units(EntropyParams& p, int64_t unit_cols, int64_t tile_cols) {
+  p.unit_cols = static_cast<int>(unit_cols);
+  p.tile_cols = static_cast<int>(tile_cols);
+  p.units_n = static_cast<int>(parts_of(p.cols, unit_cols));
+}
+// All units but the shared ones are whole; false where they are too many.
+bool set_whole(EntropyParams& p) {
+  const int64_t units = static_cast<int64_t>(p.tiles_m) * p.units_n;
+  p.whole = static_cast<int>(units - p.shared);
+  return units <= INT32_MAX;
+}
 
-// Spans of some column tiles, so that each pair has many and what they give is little: their last ones keep few pairs from the end.
+// STATS: spans of columns, of any length, so that the pairs have about the same to do: a number of them for each row tile that makes 1 to 16 units to a
+// pair.  Few long ones where there are few tiles, since each ends with an epilogue that nothing covers.
 EntropyParams stats_of(int64_t rows, int64_t symbols, int64_t width, int type) {
-  EntropyParams p = tiles_of(rows, symbols, width, type);
-  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-  int64_t span = std::clamp<int64_t>(tiles / (static_cast<int64_t>(pairs_in_all()) * 16), 1, 8);
-  span = std::max(span, parts_of(static_cast<int64_t>(p.tiles_n) * rows * 16, kMostStats));
-  p.span = static_cast<int>(std::min<int64_t>(span, p.tiles_n));
-  p.units_n = static_cast<int>(parts_of(p.tiles_n, p.span));
+  EntropyParams p = product_of(rows, symbols, width);
+  const int64_t pairs = pairs_in_all(), wide = widest(type);
+  const int64_t most = std::max<int64_t>(1, std::min(parts_of(symbols, 32), kMostStats / (rows * 2 * static_cast<int64_t>(sizeof(float2)))));
+  int64_t best = INT64_MAX;
+  for (int64_t k = 1; k <= 16; ++k) {
+    const int64_t spans = std::clamp<int64_t>(k * pairs / p.tiles_m, 1, most);
+    const int64_t cols = parts_of(symbols, spans), tiles = parts_of(cols, wide), tile = up_to(parts_of(cols, tiles), 32);
+    const int64_t cost = parts_of(p.tiles_m * parts_of(symbols, cols), pairs) * (tiles * p.kblocks * cycles_of(tile, type) + kTileCycles);
+    if (cost < best) {
+      best = cost;
+      set_units(p, cols, tile);
+    }
+  }
   return p;
 }
 
-// Where tiles are fewer than pairs of CTAs, the contraction is split among them, in parts of eight k-blocks or more.
-void split(EntropyParams& p) {
-  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(pairs_in_all() / tiles, p.kblocks / 8));
-  p.kb_split = static_cast<int>(parts_of(p.kblocks, most));
-  p.splits = static_cast<int>(parts_of(p.kblocks, p.kb_split));
+// PROB: tiles of up to the widest, of fewer columns where that makes the waves of them even.
+EntropyParams prob_of(int64_t rows, int64_t symbols, int64_t width, int type) {
+  EntropyParams p = product_of(rows, symbols, width);
+  const int64_t pairs = pairs_in_all();
+  int64_t best = INT64_MAX;
+  for (int64_t tile = widest(type); tile >= 96; tile -= 32) {
+    const int64_t waves = parts_of(p.tiles_m * parts_of(symbols, tile), pairs);
+    const int64_t cost = waves * (p.kblocks * cycles_of(tile, type) + kTileCycles);
+    if (cost < best) {
+      best = cost;
+      set_units(p, tile, tile);
+    }
+    if (waves > kLeastUnits) break;
+  }
+  return p;
+}
+
+// OUT: the same, and the contraction of the tiles that are left over behind full waves is cut into parts where waves of those take less time.
+EntropyParams out_of(int64_t rows, int64_t cols, int64_t k, int type) {
+  EntropyParams p = product_of(rows, cols, k);
+  const int64_t pairs = pairs_in_all();
+  int64_t best = INT64_MAX;
+  for (int64_t tile = widest(type); tile >= 96; tile -= 32) {
+    const int64_t even = std::min<int64_t>(tile, up_to(parts_of(cols, parts_of(cols, tile)), 32));
+    const int64_t units = p.tiles_m * parts_of(cols, even), full = units / pairs, left = units - full * pairs, cycles = cycles_of(even, type);
+    for (int64_t most = 1; most <= (left == 0 ? 1 : kMostSplits); ++most) {
+      const int64_t kb = parts_of(p.kblocks, most), splits = parts_of(p.kblocks, kb);
+      const int64_t parts = left * splits * 256 * even * 2 * static_cast<int64_t>(sizeof(float)) / kBytesPerCycle;  // written and read
+      const int64_t cost = full * (p.kblocks * cycles + kTileCycles) + parts_of(left * splits, pairs) * (kb * cycles + kTileCycles) +
+                           (splits > 1 ? kSumCycles + parts : 0);
+      if (cost < best) {
+        best = cost;
+        set_units(p, even, even);
+        p.shared = splits > 1 ? static_cast<int>(left) : 0;
+        p.splits = static_cast<int>(splits);
+        p.kb_split = static_cast<int>(kb);
+      }
+    }
+    if (full > kLeastUnits) break;
+  }
+  return p;
+}
+size_t part_bytes(const EntropyParams& p) {
+  return static_cast<size_t>(p.shared) * static_cast<size_t>(p.splits) * 256 * static_cast<size_t>(p.tile_cols) * sizeof(float);
 }
 
 struct Space {  // the workspace as it is handed out
@@ -359,27 +460,23 @@ ForwardSpace forward_space(void* base, const void* x, const void* weight, int64_
 }
 
 struct BackwardPlan {
-  int64_t piece, pieces, d_pitch, part_pitch;
-  EntropyParams x, w;  // of a whole piece
+  int64_t piece, pieces, last, d_pitch, sum_pitch;  // last: symbols of the last piece
 };
 BackwardPlan backward_plan(int64_t rows, int64_t symbols, int64_t width, int type) {
   BackwardPlan b;
   const int planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
-  const int64_t most = std::max(kPiece, kMostLogits / planes / std::max<int64_t>(rows, 1) / kPiece * kPiece);
+  const int64_t most = std::max(kPiece, kMostLogits / planes / rows / kPiece * kPiece);
   b.pieces = parts_of(symbols, most);
   b.piece = std::min(up_to(parts_of(symbols, b.pieces), kPiece), symbols);
   b.pieces = parts_of(symbols, b.piece);
+  b.last = symbols - (b.pieces - 1) * b.piece;
   b.d_pitch = up_to(b.piece, 64);
-  b.part_pitch = up_to(width, 4);
-  b.x = tiles_of(rows, width, b.piece, type);
-  b.w = tiles_of(b.piece, width, rows, type);
-  split(b.x);
-  split(b.w);
+  b.sum_pitch = up_to(width, 4);
   return b;
 }
 struct BackwardSpace {
   void *x, *weight;
-  float *factors, *x_part, *w_part;
+  float *factors, *sum, *part;
   uint16_t* d;
   size_t bytes;
 };
@@ -391,20 +488,13 @@ BackwardSpace backward_space(void* base, const BackwardPlan& b, const void* x, c
   f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type));
   f.factors = static_cast<float*>(s.take(2 * sizeof(float)));
   f.d = static_cast<uint16_t*>(s.take(static_cast<size_t>(rows) * static_cast<size_t>(b.d_pitch) * 2 * (type == TRITURUS_B200_TYPE_F32 ? 3 : 1)));
-  const size_t row = static_cast<size_t>(b.part_pitch) * sizeof(float);
-  f.x_part = static_cast<float*>(s.take(b.x.splits > 1 || b.pieces > 1 ? static_cast<size_t>(b.x.splits) * static_cast<size_t>(rows) * row : 0));
-  f.w_part = static_cast<float*>(s.take(b.w.splits > 1 ? static_cast<size_t>(b.w.splits) * static_cast<size_t>(b.piece) * row : 0));
+  f.sum = static_cast<float*>(s.take(b.pieces > 1 ? static_cast<size_t>(rows) * static_cast<size_t>(b.sum_pitch) * sizeof(float) : 0));
+  size_t parts = 0;  // (one product at a time uses them)
+  for (const int64_t piece : {b.piece, b.last})
+    parts = std::max({parts, part_bytes(out_of(rows, width, piece, type)), part_bytes(out_of(piece, width, rows, type))});
+  f.part = static_cast<float*>(s.take(parts));
   f.bytes = s.used;
   return f;
-}
-
-int sum_parts(const EntropyParams& p, int64_t width, void* out, int type, cudaStream_t st) {
-  const auto run = [&](auto t) {
-    using T = decltype(t);
-    return launch_of(entropy_sum_kernel<T>, dim3(static_cast<unsigned>(copy_grid(static_cast<int64_t>(p.rows) * width))), 256, 0, st, nullptr,
-                     static_cast<const float*>(p.part), p.splits, static_cast<int64_t>(p.rows), static_cast<int>(width), p.part_pitch, static_cast<T*>(out));
-  };
-  return type == TRITURUS_B200_TYPE_F32 ? run(0.f) : type == TRITURUS_B200_TYPE_BF16 ? run(__nv_bfloat16()) : run(__half());
 }
 
 bool reduction_ok(int r) { return r >= TRITURUS_B200_REDUCTION_NONE && r <= TRITURUS_B200_REDUCTION_SUM; }
@@ -427,6 +517,7 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
                                        int reduction, int64_t ignore_index, void* workspace, size_t workspace_bytes, int32_t* status_dev, void* stream) {
   if (!sizes_ok(rows, symbols, width, type) || !reduction_ok(reduction) || (target_bytes != 4 && target_bytes != 8)) return TRITURUS_B200_EINVAL;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Launches launch = {st};
   if (rows == 0) {
     if (reduction == TRITURUS_B200_REDUCTION_NONE) return TRITURUS_B200_OK;
     if (loss == nullptr) return TRITURUS_B200_EINVAL;
@@ -440,10 +531,11 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
   if (workspace_bytes < space.bytes) return TRITURUS_B200_EWORKSPACE;
 
   Matrix a, b;
-  int rc = prepare(&a, x, rows, width, x_stride, type, space.x, st);
-  if (rc == TRITURUS_B200_OK) rc = prepare(&b, weight, symbols, width, weight_stride, type, space.weight, st);
+  int rc = prepare(&a, x, rows, width, x_stride, type, space.x, launch);
+  if (rc == TRITURUS_B200_OK) rc = prepare(&b, weight, symbols, width, weight_stride, type, space.weight, launch);
   if (rc != TRITURUS_B200_OK) return rc;
   EntropyParams p = stats_of(rows, symbols, width, type);
+  if (!set_whole(p)) return TRITURUS_B200_EINVAL;
   p.stats = space.stats;
   p.picked = space.picked;
   p.target = target;
@@ -451,7 +543,7 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
   p.ignore = ignore_index;
   p.symbols = symbols;
   p.status = status_dev;
-  rc = run_products<ENTROPY_STATS>(a, b, p, type, st);
+  rc = run_products<ENTROPY_STATS>(a, b, p, type, launch);
   if (rc != TRITURUS_B200_OK) return rc;
 
   JoinArgs j = {};
@@ -468,9 +560,9 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
   j.target_wide = p.target_wide;
   j.reduction = reduction;
   const int blocks = static_cast<int>(parts_of(rows, 32));
-  rc = launch_of(entropy_join_kernel, dim3(static_cast<unsigned>(blocks)), 1024, 0, st, nullptr, j);
+  rc = launch(entropy_join_kernel, blocks, 1024, 0, j);
   if (rc == TRITURUS_B200_OK && reduction != TRITURUS_B200_REDUCTION_NONE && blocks > 1)
-    rc = launch_of(entropy_loss_kernel, dim3(1), 256, 0, st, nullptr, j, blocks);
+    rc = launch(entropy_loss_kernel, 1, 256, 0, j, blocks);
   return rc;
 }
 
@@ -498,12 +590,13 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
   if (workspace_bytes < space.bytes) return TRITURUS_B200_EWORKSPACE;
   if (dx == nullptr && dweight == nullptr) return TRITURUS_B200_OK;
 
+  Launches launch = {st};
   Matrix mx, mw;
-  int rc = prepare(&mx, x, rows, width, x_stride, type, space.x, st);
-  if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, type, space.weight, st);
+  int rc = prepare(&mx, x, rows, width, x_stride, type, space.x, launch);
+  if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, type, space.weight, launch);
   const int wide = target_bytes == 8;
   if (rc == TRITURUS_B200_OK)
-    rc = launch_of(entropy_factors_kernel, dim3(1), 1024, 0, st, nullptr, dloss, reduction == TRITURUS_B200_REDUCTION_NONE ? 1 : 0, target, wide, ignore_index,
+    rc = launch(entropy_factors_kernel, 1, 1024, 0, dloss, reduction == TRITURUS_B200_REDUCTION_NONE ? 1 : 0, target, wide, ignore_index,
                    static_cast<int>(rows), reduction == TRITURUS_B200_REDUCTION_MEAN ? 1 : 0, type == TRITURUS_B200_TYPE_F16 ? 1 : 0, space.factors);
   Matrix md = {};
   md.data = space.d;
@@ -513,8 +606,9 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
   md.planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
   const int vec = width % 4 == 0;
   for (int64_t i = 0; i < plan.pieces && rc == TRITURUS_B200_OK; ++i) {
-    const int64_t first = i * plan.piece, piece = std::min(plan.piece, symbols - first);
-    EntropyParams p = tiles_of(rows, piece, width, type);
+    const int64_t first = i * plan.piece, piece = i + 1 < plan.pieces ? plan.piece : plan.last;
+    EntropyParams p = prob_of(rows, piece, width, type);
+    if (!set_whole(p)) return TRITURUS_B200_EINVAL;
     p.b_row = static_cast<int>(first);
     p.target = target;
     p.target_wide = wide;
@@ -528,44 +622,29 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
     p.d_pitch = md.pitch;
     p.d_plane = md.plane;
     p.status = status_dev;
-    rc = run_products<ENTROPY_PROB>(mx, mw, p, type, st);
-    if (rc != TRITURUS_B200_OK) break;
+    rc = run_products<ENTROPY_PROB>(mx, mw, p, type, launch);
     md.width = piece;
-    if (dx != nullptr) {
-      EntropyParams q = tiles_of(rows, width, piece, type);
-      q.kb_split = plan.x.kb_split;
-      q.splits = static_cast<int>(parts_of(q.kblocks, q.kb_split));
+    const auto out = [&](EntropyParams q, void* to, int dest) {
+      q.factors = space.factors;
+      q.dest = dest;
+      q.out = to;
+      q.out_pitch = width;
+      q.out_vec = vec && aligned_to(to, 4 * size);
+      q.sum = space.sum;
+      q.sum_pitch = plan.sum_pitch;
+      q.part = space.part;
+      q.status = status_dev;
+      return q;
+    };
+    if (dx != nullptr && rc == TRITURUS_B200_OK) {
+      const bool begin = i == 0, end = i + 1 == plan.pieces;
+      EntropyParams q = out(out_of(rows, width, piece, type), dx, begin ? end ? DEST_FINAL : DEST_SUM : end ? DEST_FINAL_ADD : DEST_SUM_ADD);
       q.b_k = static_cast<int>(first);
-      q.factors = space.factors;
-      const bool begin = i == 0, end = i + 1 == plan.pieces && plan.x.splits == 1;
-      q.dest = begin ? end ? DEST_FINAL : DEST_PART : end ? DEST_FINAL_ADD : DEST_PART_ADD;
-      q.out = dx;
-      q.out_pitch = width;
-      q.out_vec = vec && aligned_to(dx, 4 * size);
-      q.part = space.x_part;
-      q.part_pitch = plan.part_pitch;
-      q.status = status_dev;
-      rc = run_products<ENTROPY_OUT_X>(md, mw, q, type, st);
-      if (rc == TRITURUS_B200_OK && i + 1 == plan.pieces && plan.x.splits > 1) {
-        q.splits = plan.x.splits;
-        rc = sum_parts(q, width, dx, type, st);
-      }
-      if (rc != TRITURUS_B200_OK) break;
+      rc = set_whole(q) ? run_products<ENTROPY_OUT_X>(md, mw, q, type, launch) : TRITURUS_B200_EINVAL;
     }
-    if (dweight != nullptr) {
-      EntropyParams q = tiles_of(piece, width, rows, type);
-      q.kb_split = plan.w.kb_split;
-      q.splits = plan.w.splits;
-      q.factors = space.factors;
-      q.dest = q.splits == 1 ? DEST_FINAL : DEST_PART;
-      q.out = static_cast<char*>(dweight) + first * width * size;
-      q.out_pitch = width;
-      q.out_vec = vec && aligned_to(q.out, 4 * size);
-      q.part = space.w_part;
-      q.part_pitch = plan.part_pitch;
-      q.status = status_dev;
-      rc = run_products<ENTROPY_OUT_W>(md, mx, q, type, st);
-      if (rc == TRITURUS_B200_OK && q.splits > 1) rc = sum_parts(q, width, q.out, type, st);
+    if (dweight != nullptr && rc == TRITURUS_B200_OK) {
+      EntropyParams q = out(out_of(piece, width, rows, type), static_cast<char*>(dweight) + first * width * size, DEST_FINAL);
+      rc = set_whole(q) ? run_products<ENTROPY_OUT_W>(md, mx, q, type, launch) : TRITURUS_B200_EINVAL;
     }
   }
   return rc;
