@@ -2,8 +2,8 @@
 
 Bounds.  u = 2^-24.  S = sum_d |x_d w_d|.
 Logits, 16-bit operands: products are exact; each MMA adds 16 of them and cuts off below a unit of the last place, 2 u of at most S:
-E_z = (D / 16 + 8) 2 u S.  float32: what the six products of parts leave out is below 2^-22.9 = 2.2 u of each product, the four MMAs
-of 64 terms' first parts are cut off (2 u each), those of the others by 2^-8 of that, and D / 64 sums rounded: E_z = (16 + D / 64) u S.
+E_z = (D / 16 + 8) 2 u S.  float32: what the six products of parts leave out is below 2^-22.9 = 2.2 u of each product, the MMAs of the first
+parts of 32 or 64 terms are cut off (2 u each, up to four), those of the others by 2^-8 of that, and the sums of D / 32 of them rounded: E_z = (16 + D / 32) u S.
 lse: max E_z, the exponentials (2^-22 each), their arguments (4 u of the numbers, as far as those count), and some 320 additions in a row: E_lse = max E_z + 2^-15 + 4 u |lse|.
 loss: E_lse + E_z of the target, and u of both for the difference.
 d = g (p - [target]): p is off by exp(E_z + E_lse + 2^-21) - 1 at most, and d is rounded by half a step h of its type (2^-8, 2^-11; float32: 2 u, cut off), in float16 at
@@ -30,7 +30,7 @@ IGNORE = -100
 
 
 def product_error(kind, terms):
-    return (16 + terms / 64) * U if kind == torch.float32 else (terms / 16 + 8) * 2 * U
+    return (16 + terms / 32) * U if kind == torch.float32 else (terms / 16 + 8) * 2 * U
 
 
 def expected(x, weight, target, dloss, reduction, ignore=IGNORE):

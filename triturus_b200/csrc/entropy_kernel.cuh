@@ -16,9 +16,10 @@
 // gradient do not fill the pairs evenly, the last ones are cut along the contraction into parts, which a further launch adds.
 //
 // 32-bit operands (WIDE) come as three planes of bfloat16 whose sum they are, exactly: 8 + 8 + 8 of the 24 digits.  Six products of planes, the
-// smallest first, leave out what is below 2^-24 of a product of two numbers.  A stage holds all planes of 64 contraction values, 96 KB to a CTA, and is used
-// for 24 MMAs.  The tensor core cuts off what does not fit its accumulator, half a unit of the last place for each of many additions; so each stage has an
-// accumulator of its own, which is added to sums in registers, and tiles are 192 columns, whose sums are 96 registers of a thread.
+// smallest first, leave out what is below 2^-24 of a product of two numbers.  Each plane of 64 contraction values is a stage of its own, and is used for
+// 8 or 12 MMAs.  (TMA takes some 2.5 cycles for each row of a box, of 64 bytes or 128: rows of 64 took longer than their MMAs.)  The tensor core cuts
+// off what does not fit its accumulator, half a unit of the last place for each of many additions; so each 64 contraction values have an
+// accumulator of their own, which is added to sums in registers, and tiles are 192 columns, whose sums are 96 registers of a thread.
 #pragma once
 
 #include "packs.cuh"
@@ -46,13 +47,13 @@ struct EntropyCfg {
   static constexpr int BN = WIDE ? 192 : 256;
   static constexpr int BNH = BN / 2;
   static constexpr int BK = 64;
-  static constexpr int NS = WIDE ? 2 : 6;
+  static constexpr int NS = 6;
   static constexpr int PLANES = WIDE ? 3 : 1;
   static constexpr int MN_BOX = 64 * BK * 2;  // 64 rows or columns of an MN-major operand
   static constexpr int A_TILE = BM * BK * 2;
   static constexpr int B_BOXES = (BNH + 63) / 64;
   static constexpr int B_TILE = B_MN ? B_BOXES * MN_BOX : BNH * BK * 2;
-  static constexpr int STAGE = PLANES * (A_TILE + B_TILE);
+  static constexpr int STAGE = A_TILE + B_TILE;  // (WIDE: of one plane)
   static constexpr int EPI_WARPS = 8;
   static constexpr int NTHREADS = (4 + EPI_WARPS) * 32;
   static constexpr int BOX = 32 * 128;
@@ -96,7 +97,8 @@ struct EntropyParams {
   int dest;               // of whole tiles
   void* out;              // rows of `out_pitch` elements
   int64_t out_pitch;
-  int out_vec;            // its rows are on boundaries of four elements
+  int out_vec;            // its rows are on boundaries of four elements,
+  int out_sectors;        // of 32 bytes
   float* sum;             // [rows][sum_pitch], what earlier pieces gave
   int64_t sum_pitch;
   float* part;            // [shared][splits][256][tile_cols]
@@ -142,32 +144,46 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
       : "memory");
 }
 
-// The 16 high bits of a number as bfloat16 (cut off, not rounded), and what they leave, exactly.  Three of these take a number apart.
-__device__ __forceinline__ uint32_t plane_bits(float x) { return __float_as_uint(x) >> 16; }
-__device__ __forceinline__ float plane_rest(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return (u & 0x7f800000u) == 0x7f800000u ? 0.f : x - __uint_as_float(u & 0xffff0000u);  // (an infinity or NaN is in the first plane alone)
-}
+// The 16 high bits of two numbers, each a bfloat16 (cut off, not rounded), and what they leave of a number, exactly.  Three of these take one apart.  (An infinity
+// leaves a NaN.)
+__device__ __forceinline__ uint32_t plane_bits(float x0, float x1) { return __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632); }
+__device__ __forceinline__ float plane_rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
 __device__ __forceinline__ int64_t entropy_target(const EntropyParams& p, int64_t row) {
   return p.target_wide ? static_cast<const int64_t*>(p.target)[row] : static_cast<int64_t>(static_cast<const int32_t*>(p.target)[row]);
 }
 
-// Four elements of a product, in row `row` from column `col` on (those before column `end`): to the sum of the pieces or to the result.
+// 32 bytes, a whole sector, as one access of a thread.
+struct Sector {
+  uint32_t w[8];
+};
+__device__ __forceinline__ void store_sector(void* to, const Sector& x) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x.w[0]), "r"(x.w[1]), "r"(x.w[2]), "r"(x.w[3]), "r"(x.w[4]),
+               "r"(x.w[5]), "r"(x.w[6]), "r"(x.w[7])
+               : "memory");
+}
+__device__ __forceinline__ Sector load_sector(const void* from) {
+  Sector x;
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]), "=r"(x.w[4]), "=r"(x.w[5]), "=r"(x.w[6]), "=r"(x.w[7])
+               : "l"(from)
+               : "memory");
+  return x;
+}
+
+// Two numbers as 16-bit ones.
+__device__ __forceinline__ uint32_t pack16(float x0, float x1, int half) {
+  if (half) {
+    const __half2 x = __floats2half2_rn(x0, x1);
+    return *reinterpret_cast<const uint32_t*>(&x);
+  }
+  const __nv_bfloat162 x = __floats2bfloat162_rn(x0, x1);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// Four elements of a result, in row `row` from column `col` on (those before column `end`).
 template <class T>
 __device__ __forceinline__ void entropy_put(const EntropyParams& p, int row, int col, float4 x, int end) {
-  float4* sum = reinterpret_cast<float4*>(p.sum + static_cast<int64_t>(row) * p.sum_pitch + col);
-  if (p.dest == DEST_SUM_ADD || p.dest == DEST_FINAL_ADD) {
-    const float4 y = *sum;
-    x.x += y.x;
-    x.y += y.y;
-    x.z += y.z;
-    x.w += y.w;
-  }
-  if (p.dest == DEST_SUM || p.dest == DEST_SUM_ADD) {
-    *sum = x;
-    return;
-  }
   T* out = static_cast<T*>(p.out) + static_cast<int64_t>(row) * p.out_pitch + col;
   Pack<T, 4 * static_cast<int>(sizeof(T))> y;
   y.v[0] = from_float<T>(x.x);
@@ -281,8 +297,6 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         if (!unit(u, 0, p.kblocks, -1)) return;
     }
   };
-  constexpr int plane_a[6] = {2, 0, 1, 1, 0, 0}, plane_b[6] = {0, 2, 1, 0, 1, 0};  // the smallest products first
-
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (this CTA's halves)
     // (Here and in the issuer the whole warp runs the loop and one elected lane issues: control flow and addresses are uniform and stay in
@@ -292,17 +306,18 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     walk([&](const Tile& t) {
       const int a0 = t.tm * (2 * BM) + static_cast<int>(rank) * BM;
       const int b0 = p.b_row + t.n0 + static_cast<int>(rank) * (t.mma >> 1);
-      for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
-        const uint32_t s = it % NS;
-        if (!(ok = mbar_wait_warp(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
-        if (elect_one_sync()) {
-          if (leader) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE);
-          const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
-          const int ka = kb * BK, kw = p.b_k + kb * BK;
+      for (int kb = t.k0; kb < t.k1; ++kb) {
+        const int ka = kb * BK, kw = p.b_k + kb * BK;
 #pragma unroll
-          for (int plane = 0; plane < Cfg::PLANES; ++plane) {
-            uint8_t* a = smem + s * Cfg::STAGE + plane * Cfg::A_TILE;
-            uint8_t* b = smem + s * Cfg::STAGE + Cfg::PLANES * Cfg::A_TILE + plane * Cfg::B_TILE;
+        for (int i = 0; i < Cfg::PLANES; ++i, ++it) {
+          const int plane = WIDE ? (i + 2) % 3 : 0;  // 2, 0, 1
+          const uint32_t s = it % NS;
+          if (!(ok = mbar_wait_warp(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
+          if (elect_one_sync()) {
+            if (leader) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE);
+            const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
+            uint8_t* a = smem + s * Cfg::STAGE;
+            uint8_t* b = a + Cfg::A_TILE;
             if constexpr (Cfg::A_MN) {
 #pragma unroll
               for (int g = 0; g < BM / 64; ++g) tma_load_3d_pair(a + g * Cfg::MN_BOX, &tmap_a, bar, a0 + g * 64, ka, plane);
@@ -316,8 +331,8 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               tma_load_3d_pair(b, &tmap_b, bar, kw, b0, plane);
             }
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
       return true;
     });
@@ -329,41 +344,67 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     if (leader) {
       constexpr uint32_t STAGE_ENC = Cfg::STAGE >> 4;
       constexpr uint32_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;  // 16 contraction values
-      const uint32_t a_at = smem_u32(smem), b_at = a_at + Cfg::PLANES * Cfg::A_TILE;
+      const uint32_t a_at = smem_u32(smem), b_at = a_at + Cfg::A_TILE;
       const uint64_t da0 = Cfg::A_MN ? umma_desc_mn16_sw128(a_at, Cfg::MN_BOX) : umma_desc_k_sw128(a_at);
       const uint64_t db0 = Cfg::B_MN ? umma_desc_mn16_sw128(b_at, Cfg::MN_BOX) : umma_desc_k_sw128(b_at);
       uint32_t s = 0, ph = 0, accs = 0;
-      // one stage into accumulator d
-      const auto multiply = [&](uint32_t d, uint32_t idesc, bool add) {
-        const uint64_t da = da0 + s * STAGE_ENC, db = db0 + s * STAGE_ENC;
-#pragma unroll
-        for (int x = 0; x < (WIDE ? 6 : 1); ++x) {
-          const uint64_t pa = da + (WIDE ? plane_a[x] : 0) * (Cfg::A_TILE >> 4), pb = db + (WIDE ? plane_b[x] : 0) * (Cfg::B_TILE >> 4);
-#pragma unroll
-          for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, pa + a_step * k, pb + b_step * k, idesc, add || x > 0 || k > 0 ? 1u : 0u);
+      const auto advance = [&] {
+        if (++s == NS) {
+          s = 0;
+          ph ^= 1;
         }
-        umma_commit_pair_mcast(smem_u32(&stage_empty[s]), 3);
       };
+      // rows of stage sa by columns of stage sb
+      const auto multiply = [&](uint32_t d, uint32_t idesc, uint32_t sa, uint32_t sb, bool add) {
+        const uint64_t da = da0 + sa * STAGE_ENC, db = db0 + sb * STAGE_ENC;
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, da + a_step * k, db + b_step * k, idesc, add || k > 0 ? 1u : 0u);
+      };
+      const auto free_stage = [&](uint32_t stage) { umma_commit_pair_mcast(smem_u32(&stage_empty[stage]), 3); };
       walk([&](const Tile& t) {
         const uint32_t idesc = p.idesc | static_cast<uint32_t>(t.mma >> 3) << 17;
         for (int kb = t.k0; kb < t.k1; ++kb) {
-          const uint32_t buf = accs & 1;
+          const uint32_t buf = accs & 1, d = tmem_base + buf * Cfg::BUF_COLS;
           if (WIDE || kb == t.k0) {
             if (!mbar_wait_warp(&acc_empty[buf], ((accs >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
           }
           if (!mbar_wait_warp(&full[s], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
-          tc_fence_after_sync();
           const bool done = WIDE || kb + 1 == t.k1;
-          if (elect_one_sync()) {
-            multiply(tmem_base + buf * Cfg::BUF_COLS, idesc, !WIDE && kb > t.k0);
-            if (done) umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
+          if constexpr (WIDE) {
+            // planes 2, 0 and 1 in three stages (of six: the three have the same parity of the wait); the first is free again after a third of the MMAs
+            const uint32_t s2 = s, s0 = s + 1, s1 = s + 2;
+            if (!mbar_wait_warp(&full[s0], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
+            tc_fence_after_sync();
+            if (elect_one_sync()) {
+              multiply(d, idesc, s2, s0, false);
+              multiply(d, idesc, s0, s2, true);
+              free_stage(s2);
+            }
+            __syncwarp();
+            if (!mbar_wait_warp(&full[s1], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
+            tc_fence_after_sync();
+            if (elect_one_sync()) {
+              multiply(d, idesc, s1, s1, true);
+              multiply(d, idesc, s1, s0, true);
+              multiply(d, idesc, s0, s1, true);
+              free_stage(s1);
+              multiply(d, idesc, s0, s0, true);
+              free_stage(s0);
+              umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
+            }
+            advance();
+            advance();
+          } else {
+            tc_fence_after_sync();
+            if (elect_one_sync()) {
+              multiply(d, idesc, s, s, kb > t.k0);
+              free_stage(s);
+              if (done) umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
+            }
           }
           __syncwarp();
+          advance();
           if (done) ++accs;
-          if (++s == NS) {
-            s = 0;
-            ph ^= 1;
-          }
         }
         return true;
       });
@@ -374,6 +415,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     uint8_t* box = boxes + (warp - 4) * Cfg::BOX;
     constexpr int CHUNKS = Cfg::COLS / 32;
     uint32_t accs = 0;
+    static_assert(!WIDE || CHUNKS <= 3);
     float sum[WIDE ? CHUNKS : 1][32];  // WIDE: what the accumulators of a tile add up to
 
     // of the unit's row (STATS), of the tile's row (PROB)
@@ -405,21 +447,21 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const bool rows_exist = t.tm * (2 * BM) + static_cast<int>(rank) * BM < p.rows;
       const int chunks = rows_exist ? max(0, min(CHUNKS, (t.n1 - col0 + 31) >> 5)) : 0;
 
-      // 32 columns of the product from column c0 on
-      const auto process = [&](float (&v)[32], int c, int plane) {
-        const int c0 = col0 + c * 32;
+      // 32 columns of the product from column c0 on.  (One copy of this code, in a loop over the chunks: unrolled over them it is fetched as slowly
+      // as it is long, 8 000 cycles for a chunk.)
+      const auto process = [&](float (&v)[32], int c0) {
         if constexpr (MODE == ENTROPY_STATS) {
           if (c0 + 32 > t.n1) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (c0 + e >= t.n1) v[e] = -INFINITY;
           }
-          const int64_t at = target < t.n1 ? target - c0 : -1;
-          if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
+          const int at = target < t.n1 && target >= c0 && target < c0 + 32 ? static_cast<int>(target) - c0 : -1;
+          if (__any_sync(0xffffffffu, at >= 0)) {
             float z = 0.f;
 #pragma unroll
             for (int e = 0; e < 32; ++e) z = at == e ? v[e] : z;
-            if (valid && at >= 0 && at < 32) p.picked[row] = z;
+            if (valid && at >= 0) p.picked[row] = z;
           }
           float m[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
@@ -432,68 +474,106 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           total = (s[0] + s[1]) + (s[2] + s[3]);
           top = now;
         } else if constexpr (MODE == ENTROPY_PROB) {
-          if (plane == 0) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = ex2_approx(WIDE ? (v[e] - lse) * LOG2E_F : fmaf(v[e], LOG2E_F, -lse2)) * g;
-            const int64_t at = target - c0;
-            if (__any_sync(0xffffffffu, ignored || (at >= 0 && at < 32))) {
+          for (int e = 0; e < 32; ++e) v[e] = ex2_approx(WIDE ? (v[e] - lse) * LOG2E_F : fmaf(v[e], LOG2E_F, -lse2)) * g;
+          const int at = target >= c0 && target < c0 + 32 ? static_cast<int>(target) - c0 : -1;
+          if (__any_sync(0xffffffffu, ignored || at >= 0)) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                if (at == e) v[e] -= g;
-                if (ignored) v[e] = 0.f;  // (whatever its logits are)
+            for (int e = 0; e < 32; ++e) {
+              if (at == e) v[e] -= g;
+              if (ignored) v[e] = 0.f;  // (whatever its logits are)
+            }
+          }
+          // 64 bytes of the row, straight from registers: TMA and the MMAs leave no bandwidth of shared memory (through it a WIDE tile took 11 600 cycles,
+          // of which the exponentials 2 800).  Tiles have multiples of 32 columns here, and so has d.
+          uint16_t* to = p.d + static_cast<int64_t>(row) * p.d_pitch + c0;
+#pragma unroll 1
+          for (int plane = 0; plane < Cfg::PLANES; ++plane, to += p.d_plane) {
+            Sector w[2];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              if constexpr (WIDE) {
+                w[e >> 3].w[e & 7] = plane_bits(v[2 * e], v[2 * e + 1]);
+                v[2 * e] = plane_rest(v[2 * e]);
+                v[2 * e + 1] = plane_rest(v[2 * e + 1]);
+              } else {
+                w[e >> 3].w[e & 7] = pack16(v[2 * e], v[2 * e + 1], p.half);
               }
             }
-          }
-          // 64 bytes of the row's 128 in the box
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if constexpr (WIDE) {
-              w[e] = plane_bits(v[2 * e]) | plane_bits(v[2 * e + 1]) << 16;
-              v[2 * e] = plane_rest(v[2 * e]);
-              v[2 * e + 1] = plane_rest(v[2 * e + 1]);
-            } else if (p.half) {
-              const __half2 x = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
-              w[e] = *reinterpret_cast<const uint32_t*>(&x);
-            } else {
-              const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-              w[e] = *reinterpret_cast<const uint32_t*>(&x);
+            if (valid) {
+              store_sector(to, w[0]);
+              store_sector(to + 16, w[1]);
             }
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(box + lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4)) =
-                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-          if ((c & 1) != 0 || c + 1 == chunks) {  // (tiles have multiples of 32 columns here, and so has d)
-            __syncwarp();
-            const int cb = c0 - (c & 1) * 32 + (lane & 7) * 8;
-            uint16_t* to = p.d + plane * p.d_plane + cb;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = i * 4 + (lane >> 3);
-              if (row0 + r < p.rows && cb < c0 + 32)
-                *reinterpret_cast<uint4*>(to + static_cast<int64_t>(row0 + r) * p.d_pitch) =
-                    *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            }
-            __syncwarp();
           }
         } else {
 #pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] *= alpha;
+          const auto sector = [&](int j) {  // eight columns as they are
+            Sector w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w.w[e] = __float_as_uint(v[8 * j + e]);
+            return w;
+          };
+          if (t.part >= 0) {
+            float* to = p.part + (static_cast<int64_t>(t.part) * (2 * BM) + static_cast<int>(rank) * BM + q * 32 + lane) * p.tile_cols + (c0 - t.n0);
+            if (valid) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (c0 + 8 * j < t.n1) store_sector(to + 8 * j, sector(j));
+            }
+            return;
+          }
+          if (p.dest != DEST_FINAL) {
+            float* sums = p.sum + static_cast<int64_t>(row) * p.sum_pitch + c0;
+            if (p.dest != DEST_SUM && valid) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (c0 + 8 * j < t.n1) {
+                  const Sector y = load_sector(sums + 8 * j);
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) v[8 * j + e] += __uint_as_float(y.w[e]);
+                }
+              }
+            }
+            if (p.dest != DEST_FINAL_ADD) {
+              if (valid) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (c0 + 8 * j < t.n1) store_sector(sums + 8 * j, sector(j));
+              }
+              return;
+            }
+          }
+          if (p.out_sectors) {
+            constexpr int EACH = WIDE ? 8 : 16;  // columns of a sector
+            char* to = static_cast<char*>(p.out) + (static_cast<int64_t>(row) * p.out_pitch + c0) * (32 / EACH);
+            if (valid) {
+#pragma unroll
+              for (int j = 0; j < 32 / EACH; ++j) {
+                if (c0 + EACH * j >= t.n1) continue;
+                if constexpr (WIDE) {
+                  store_sector(to + 32 * j, sector(j));
+                } else {
+                  Sector w;
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) w.w[e] = pack16(v[16 * j + 2 * e], v[16 * j + 2 * e + 1], p.half);
+                  store_sector(to + 32 * j, w);
+                }
+              }
+            }
+            return;
+          }
+          // rows that do not begin on sectors: row by row through shared memory
+#pragma unroll
           for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                make_float4(v[4 * j] * alpha, v[4 * j + 1] * alpha, v[4 * j + 2] * alpha, v[4 * j + 3] * alpha);
+            *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           __syncwarp();
           const int cb = c0 + (lane & 7) * 4;
-#pragma unroll
+#pragma unroll 2
           for (int i = 0; i < 8; ++i) {
             const int r = i * 4 + (lane >> 3);
             if (row0 + r >= p.rows || cb >= t.n1) continue;
-            float4 x = *reinterpret_cast<const float4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            if (t.part >= 0) {
-              const int in_tile = static_cast<int>(rank) * BM + q * 32 + r;
-              *reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(t.part) * (2 * BM) + in_tile) * p.tile_cols + (cb - t.n0)) = x;
-              continue;
-            }
+            const float4 x = *reinterpret_cast<const float4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
             if constexpr (WIDE) {
               entropy_put<float>(p, row0 + r, cb, x, t.n1);
             } else if (p.half) {
@@ -521,46 +601,45 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           release();
           continue;
         }
+        uint32_t ld[32];
         if constexpr (WIDE) {
-          uint32_t v[32];
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c) {
             if (c < chunks) {
-              tmem_ld_32x32(at + c * 32, v);
+              tmem_ld_32x32(at + c * 32, ld);
               tmem_ld_wait();
+              if (kb == t.k0) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) sum[c][e] = (kb == t.k0 ? 0.f : sum[c][e]) + __uint_as_float(v[e]);
+                for (int e = 0; e < 32; ++e) sum[c][e] = __uint_as_float(ld[e]);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sum[c][e] += __uint_as_float(ld[e]);
+              }
             }
           }
           release();
-          if (kb + 1 == t.k1) {
+          if (kb + 1 < t.k1) continue;
+#pragma unroll 1
+          for (int c = 0; c < chunks; ++c) {
+            float v[32];
 #pragma unroll
-            for (int plane = 0; plane < (MODE == ENTROPY_PROB ? 3 : 1); ++plane)
-#pragma unroll
-              for (int c = 0; c < CHUNKS; ++c)
-                if (c < chunks) process(sum[c], c, plane);
+            for (int e = 0; e < 32; ++e) v[e] = c == 0 ? sum[0][e] : c == 1 ? sum[CHUNKS > 1 ? 1 : 0][e] : sum[CHUNKS > 2 ? 2 : 0][e];
+            process(v, col0 + c * 32);
           }
         } else {
-          uint32_t v[2][32];
-          tmem_ld_32x32(at, v[0]);
+          tmem_ld_32x32(at, ld);
 #pragma unroll 1
-          for (int cc = 0; cc < chunks; cc += 2) {
+          for (int c = 0; c < chunks; ++c) {
+            tmem_ld_wait();
+            float v[32];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int c = cc + k;
-              if (c < chunks) {
-                tmem_ld_wait();
-                if (c + 1 < chunks) {
-                  tmem_ld_32x32(at + (c + 1) * 32, v[k ^ 1]);
-                } else {
-                  release();
-                }
-                float f[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[k][e]);
-                process(f, c, 0);
-              }
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(ld[e]);
+            if (c + 1 < chunks) {
+              tmem_ld_32x32(at + (c + 1) * 32, ld);
+            } else {
+              release();
             }
+            process(v, col0 + c * 32);
           }
         }
       }

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256) entropy_planes_kernel(const T* x, int64_t
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = plane_bits(v.v[2 * e]) | plane_bits(v.v[2 * e + 1]) << 16;
+          w[e] = plane_bits(v.v[2 * e], v.v[2 * e + 1]);
           v.v[2 * e] = plane_rest(v.v[2 * e]);
           v.v[2 * e + 1] = plane_rest(v.v[2 * e + 1]);
         }
@@ -217,7 +217,21 @@ __global__ void __launch_bounds__(256) entropy_sum_kernel(const __grid_constant_
     x.z += y.z;
     x.w += y.w;
   }
-  entropy_put<T>(p, row, col, x, min(p.cols, col + 4));
+  if (p.dest != DEST_FINAL) {
+    float4* sum = reinterpret_cast<float4*>(p.sum + static_cast<int64_t>(row) * p.sum_pitch + col);
+    if (p.dest != DEST_SUM) {
+      const float4 y = *sum;
+      x.x += y.x;
+      x.y += y.y;
+      x.z += y.z;
+      x.w += y.w;
+    }
+    if (p.dest != DEST_FINAL_ADD) {
+      *sum = x;
+      return;
+    }
+  }
+  entropy_put<T>(p, row, col, x, p.cols);
 }
 
 // ----------------------------------------------------------------------------- host
@@ -332,7 +346,7 @@ int run_products(const Matrix& a, const Matrix& b, const EntropyParams& p, int t
 
 // ----------------------------------------------------------------------------- tiles for pairs
 
-int widest(int type) { return type == TRITURUS_B200_TYPE_F32 ? 192 : 256; }
+int widest(int type) { return type == TRITURUS_B200_TYPE_F32 ? EntropyCfg<0, true>::BN : EntropyCfg<0, false>::BN; }
 // Cycles of a k-block of a tile of `cols` columns, by whichever takes longer: the MMAs, or what they and TMA move through 128 bytes a cycle of shared memory.
 int64_t cycles_of(int64_t cols, int type) {
   return type == TRITURUS_B200_TYPE_F32 ? std::max(12 * cols, 1152 + 9 * cols / 2) : std::max(2 * cols, 256 + cols);
@@ -347,7 +361,7 @@ EntropyParams product_of(int64_t rows, int64_t cols, int64_t k) {
   EntropyParams p = {};
   p.rows = static_cast<int>(rows);
   p.cols = static_cast<int>(cols);
-  p.kblocks = static_cast<int>(parts_of(k, 64));
+  p.kblocks = static_cast<int>(parts_of(k, EntropyCfg<0, false>::BK));
   p.tiles_m = static_cast<int>(parts_of(rows, 256));
   p.group = 8;
   return p;
@@ -471,7 +485,7 @@ BackwardPlan backward_plan(int64_t rows, int64_t symbols, int64_t width, int typ
   b.pieces = parts_of(symbols, b.piece);
   b.last = symbols - (b.pieces - 1) * b.piece;
   b.d_pitch = up_to(b.piece, 64);
-  b.sum_pitch = up_to(width, 4);
+  b.sum_pitch = up_to(width, 8);
   return b;
 }
 struct BackwardSpace {
@@ -630,6 +644,7 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
       q.out = to;
       q.out_pitch = width;
       q.out_vec = vec && aligned_to(to, 4 * size);
+      q.out_sectors = width * size % 32 == 0 && aligned_to(to, 32);
       q.sum = space.sum;
       q.sum_pitch = plan.sum_pitch;
       q.part = space.part;
