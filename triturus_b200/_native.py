@@ -240,6 +240,7 @@ class _NoHost:
     """In the place of the extension module where there is none: no call is a small one to it, all go through ctypes."""
 
     lm2exp = lt2exp = layer_norm = layer_norm_backward = clip_grad_norm = sample = embedding = embedding_backward = staticmethod(lambda *args: None)
+    linear_cross_entropy = linear_cross_entropy_backward = staticmethod(lambda *args: None)
 
 
 def _load_host():
@@ -316,6 +317,20 @@ def _lm2exp_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
         ws = torch.zeros((n + 3) // 4, dtype=torch.float32, device=torch.device("cuda", idx))
         _LM_WORKSPACE[key] = ws
     return ws
+
+
+_STATUS_ADDRESS: dict[int, int] = {}
+
+
+def _status_address(t: torch.Tensor) -> int:
+    """Address of the status word of t's device; 0 where it has none yet (or t is on no GPU), and a call should not be the extension's."""
+    idx = t.get_device() if t.is_cuda else -1
+    at = _STATUS_ADDRESS.get(idx)
+    if at is None:
+        if idx < 0 or torch.compiler.is_compiling():
+            return 0
+        at = _STATUS_ADDRESS[idx] = _status_word(t.device).data_ptr()
+    return at
 
 
 def check_status(device=None) -> None:

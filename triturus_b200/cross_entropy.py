@@ -73,6 +73,10 @@ def linear_cross_entropy(
     parts) are copied first.  The loss is differentiable in x and weight, once and backwards; lse is not.  A tensor with a forward-mode
     tangent is refused."""
     code = _reduction("linear_cross_entropy", reduction)
+    if not torch.compiler.is_compiling() and not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
+        out = _native.HOST.linear_cross_entropy(x, weight, target, code, ignore_index, _native._status_address(x))  # None: not an ordinary call
+        if out is not None:
+            return out if return_lse else out[0]
     _check(x, weight, target, ignore_index)
     if torch.compiler.is_compiling():
         loss, lse = _native.linear_cross_entropy_op(x, weight, target, code, ignore_index)
@@ -100,6 +104,12 @@ def linear_cross_entropy_backward(
     to 16 bits for its two products where x has 16: to bfloat16, or to float16 relative to the largest finite |dloss|.  dweight multiplies x of ignored
     positions by 0: it has to be finite.  Sums are in 32 bits in a fixed order.  The results carry no graph."""
     code = _reduction("linear_cross_entropy_backward", reduction)
+    if not torch.compiler.is_compiling():
+        out = _native.HOST.linear_cross_entropy_backward(
+            x, weight, target, dloss, lse, code, ignore_index, bool(x_grad), bool(weight_grad), _native._status_address(x)
+        )
+        if out is not None:
+            return out
     _check_backward(dloss, x, weight, target, lse, code, ignore_index)
     impl = _native.linear_cross_entropy_backward_op if torch.compiler.is_compiling() else _native._linear_cross_entropy_backward_impl
     dx, dweight = impl(dloss, x, weight, target, lse, code, ignore_index, bool(x_grad), bool(weight_grad))

@@ -470,6 +470,110 @@ PyObject* embedding_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   END_HANDLE_TH_ERRORS
 }
 
+// The operands of the cross entropy: x [..., D], weight [V, D] of its type, targets of x's leading shape.
+struct EntropyOperands {
+  const at::Tensor *x, *weight, *target;
+  int64_t rows, symbols, width, x_stride, weight_stride;
+  int type;
+};
+bool entropy_operands(PyObject* const* args, EntropyOperands* o) {
+  o->x = plain_object(args[0]);
+  o->weight = o->x != nullptr ? plain_object(args[1]) : nullptr;
+  if (o->weight == nullptr || o->x->dim() < 1 || o->weight->dim() != 2 || o->x->get_device() != c10::cuda::current_device()) return false;
+  o->target = token_arg(args[2], *o->x);
+  o->type = type_code(*o->x);
+  o->width = o->x->size(-1);
+  if (o->target == nullptr || o->type < 0 || o->weight->scalar_type() != o->x->scalar_type() || o->weight->device() != o->x->device() ||
+      o->weight->size(1) != o->width || o->target->sizes() != o->x->sizes().slice(0, o->x->dim() - 1))
+    return false;
+  o->rows = o->target->numel();
+  o->symbols = o->weight->size(0);
+  o->x_stride = row_stride(*o->x);
+  o->weight_stride = row_stride(*o->weight);
+  return o->x_stride >= 0 && o->weight_stride >= 0 && !has_tangent(o->x) && !has_tangent(o->weight);
+}
+bool int64_arg(PyObject* o, int64_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  *v = PyLong_AsLongLong(o);
+  if (*v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return true;
+}
+PyObject* tuple2(at::Tensor* a, at::Tensor* b) {
+  PyObject* out = PyTuple_New(2);
+  if (out == nullptr) return nullptr;
+  at::Tensor* all[2] = {a, b};
+  for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(out, i, all[i] != nullptr ? THPVariable_Wrap(std::move(*all[i])) : Py_NewRef(Py_None));
+  return out;
+}
+
+// linear_cross_entropy(x, weight, target, reduction, ignore_index, status) -> (loss, lse); status: address of the device's status word
+PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int reduction;
+  int64_t ignore, status;
+  EntropyOperands o;
+  if (nargs != 6 || !int_arg(args[3], &reduction) || !int64_arg(args[4], &ignore) || !int64_arg(args[5], &status) || !plain_mode() ||
+      !entropy_operands(args, &o))
+    return none();
+  at::Tensor lse = empty_on(*o.x, o.target->sizes(), at::kFloat);
+  at::Tensor loss = empty_on(*o.x, reduction == TRITURUS_B200_REDUCTION_NONE ? o.target->sizes() : at::IntArrayRef(), at::kFloat);
+  const void *xp = o.x->const_data_ptr(), *wp = o.weight->const_data_ptr();
+  const size_t bytes = triturus_b200_linear_cross_entropy_workspace_bytes(xp, wp, o.rows, o.symbols, o.width, o.x_stride, o.weight_stride, o.type);
+  if (bytes == 0) return none();  // (sizes that the library refuses)
+  at::Tensor ws = empty_on(*o.x, {static_cast<int64_t>(bytes)}, at::kByte);
+  const auto stream = c10::cuda::getCurrentCUDAStream(o.x->get_device()).stream();
+  int rc;
+  {
+    ThreadsRun unlocked;
+    rc = triturus_b200_linear_cross_entropy(xp, wp, o.target->const_data_ptr(), static_cast<int>(o.target->element_size()), loss.mutable_data_ptr<float>(),
+                                            lse.mutable_data_ptr<float>(), o.rows, o.symbols, o.width, o.x_stride, o.weight_stride, o.type, reduction, ignore,
+                                            ws.mutable_data_ptr(), bytes, reinterpret_cast<int32_t*>(status), stream);
+  }
+  if (rc != TRITURUS_B200_OK) return failed("triturus_b200_linear_cross_entropy", rc);
+  return tuple2(&loss, &lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_cross_entropy_backward(x, weight, target, dloss, lse, reduction, ignore_index, x_grad, weight_grad, status) -> (dx or None, dweight or None)
+PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int reduction;
+  int64_t ignore, status;
+  EntropyOperands o;
+  if (nargs != 10 || !int_arg(args[5], &reduction) || !int64_arg(args[6], &ignore) || !PyBool_Check(args[7]) || !PyBool_Check(args[8]) ||
+      !int64_arg(args[9], &status) || !plain_mode() || !entropy_operands(args, &o))
+    return none();
+  const at::Tensor* dloss = plain_object(args[3]);
+  const at::Tensor* lse = plain_object(args[4]);
+  if (dloss == nullptr || lse == nullptr) return none();
+  for (const at::Tensor* t : {dloss, lse})
+    if (t->scalar_type() != at::kFloat || !t->is_contiguous() || t->device() != o.x->device()) return none();
+  if (lse->sizes() != o.target->sizes() || dloss->sizes() != (reduction == TRITURUS_B200_REDUCTION_NONE ? o.target->sizes() : at::IntArrayRef())) return none();
+  const bool want_x = args[7] == Py_True, want_weight = args[8] == Py_True;
+  at::Tensor dx, dweight;
+  if (want_x) dx = empty_on(*o.x, o.x->sizes(), o.x->scalar_type());
+  if (want_weight) dweight = empty_on(*o.x, o.weight->sizes(), o.x->scalar_type());
+  const void *xp = o.x->const_data_ptr(), *wp = o.weight->const_data_ptr();
+  const size_t bytes = triturus_b200_linear_cross_entropy_backward_workspace_bytes(xp, wp, o.rows, o.symbols, o.width, o.x_stride, o.weight_stride, o.type);
+  if (bytes == 0) return none();
+  at::Tensor ws = empty_on(*o.x, {static_cast<int64_t>(bytes)}, at::kByte);
+  const auto stream = c10::cuda::getCurrentCUDAStream(o.x->get_device()).stream();
+  int rc;
+  {
+    ThreadsRun unlocked;
+    rc = triturus_b200_linear_cross_entropy_backward(
+        dloss->const_data_ptr<float>(), xp, wp, o.target->const_data_ptr(), static_cast<int>(o.target->element_size()), lse->const_data_ptr<float>(),
+        want_x ? dx.mutable_data_ptr() : nullptr, want_weight ? dweight.mutable_data_ptr() : nullptr, o.rows, o.symbols, o.width, o.x_stride, o.weight_stride,
+        o.type, reduction, ignore, ws.mutable_data_ptr(), bytes, reinterpret_cast<int32_t*>(status), stream);
+  }
+  if (rc != TRITURUS_B200_OK) return failed("triturus_b200_linear_cross_entropy_backward", rc);
+  return tuple2(want_x ? &dx : nullptr, want_weight ? &dweight : nullptr);
+  END_HANDLE_TH_ERRORS
+}
+
 // set_up(error_class, copy_flop_rows, copy_flop_strided)
 PyObject* set_up(PyObject*, PyObject* args) {
   PyObject* cls;
@@ -495,6 +599,10 @@ PyMethodDef methods[] = {
      "embedding(tokens, weight, scale, padding_idx) -> Tensor or None"},
     {"embedding_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding_backward)), METH_FASTCALL,
      "embedding_backward(dy, tokens, symbols, scale, padding_idx) -> Tensor or None"},
+    {"linear_cross_entropy", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_cross_entropy)), METH_FASTCALL,
+     "linear_cross_entropy(x, weight, target, reduction, ignore_index, status) -> tuple or None"},
+    {"linear_cross_entropy_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_cross_entropy_backward)), METH_FASTCALL,
+     "linear_cross_entropy_backward(x, weight, target, dloss, lse, reduction, ignore_index, x_grad, weight_grad, status) -> tuple or None"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Small calls of triturus_b200 from C++.", -1, methods, nullptr, nullptr, nullptr, nullptr};
