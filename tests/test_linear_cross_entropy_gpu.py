@@ -149,6 +149,50 @@ def test_many_rows_and_few_symbols(kind):
     check(*inputs(70_001, 3, 8, kind))
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("n", [2, 15, 16, 17, 32, 33, 48, 49, 63, 64, 65, 96, 127, 128, 129])
+def test_few_rows(n, kind):
+    """On both sides of where rows of x become rows and no columns of the MMAs, and where another one begins."""
+    for v, d, reduction in ((1003, 200, "mean"), (130, 513, "none"), (20_000, 72, "sum")):
+        check(*inputs(n, v, d, kind), reduction=reduction)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("n", [30, 60, 120])
+def test_few_rows_with_masks(n, kind):
+    x, w, t = inputs(n, 700, 96, kind)
+    t[::4] = IGNORE
+    g = torch.exp(rand(n, seed=4)) * (256.0 if kind == torch.float16 else 1.0)
+    want = check(x, w, t, g, "none")
+    check(x, w, torch.full_like(t, IGNORE))
+    check(x, w, t.int())
+    g[::4], x[::4] = float("nan"), float("nan")
+    loss, lse = tb.linear_cross_entropy(x, w, t, reduction="none", return_lse=True)
+    dx, _ = tb.linear_cross_entropy_backward(g, x, w, t, lse, reduction="none", weight_grad=False)
+    assert torch.equal(loss, want[0]) and torch.equal(dx, want[2]) and bool(lse[::4].isnan().all())
+    x, w, t = inputs(n, 700, 96, kind)
+    t[3], t[n - 1] = 700, -1
+    loss, lse = tb.linear_cross_entropy(x, w, t, reduction="none", return_lse=True)
+    dx, dw = tb.linear_cross_entropy_backward(torch.ones_like(loss), x, w, t, lse, reduction="none")
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[[3, n - 1]] = True
+    assert torch.equal(loss.isnan(), bad) and torch.equal(dx.isnan().all(1), bad) and torch.equal(dx.isnan().any(1), bad) and bool(dw.isnan().all())
+    if kind != torch.float32:
+        w[::2] = float("-inf")
+        x, t = x.abs() + 0.1, torch.where(t < 0, t, t // 2 * 2 + 1).clamp(max=699)
+        loss, lse = tb.linear_cross_entropy(x, w, t, reduction="none", return_lse=True)
+        some = tb.linear_cross_entropy(x, w[1::2].contiguous(), torch.where(t < 0, t, t // 2), reduction="none", return_lse=True)
+        assert torch.allclose(lse, some[1], rtol=0, atol=1e-4)
+        w[1::2] = float("-inf")  # nothing is possible
+        loss, lse = tb.linear_cross_entropy(x, w, t.clamp(min=0), reduction="none", return_lse=True)
+        assert bool((lse == float("-inf")).all()) and bool(loss.isnan().all())
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_few_rows_and_pieces_of_the_symbols(kind):
+    check(*inputs(64, 1_500_001 if kind == torch.float32 else 4_300_001, 8, kind))
+
+
 def test_wide_rows():
     check(*inputs(64, 700, 8192, torch.bfloat16))
     check(*inputs(64, 700, 8192, torch.float32))

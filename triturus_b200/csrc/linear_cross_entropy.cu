@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "entropy_few_kernel.cuh"
 #include "entropy_kernel.cuh"
 #include "tensor_map.cuh"
 
@@ -22,9 +23,10 @@ constexpr int64_t kMostStats = 1ll << 26;   // bytes of the spans' maxima and su
 
 // ----------------------------------------------------------------------------- operands that TMA cannot read in place
 
-// Rows of 16-bit elements one after the other on 16-byte boundaries; 32-bit elements as three planes of them.
-template <class T>
-__global__ void __launch_bounds__(256) entropy_planes_kernel(const T* x, int64_t rows, int width, int64_t stride, uint16_t* out, int64_t pitch, int64_t plane) {
+// Rows on 16-byte boundaries, as they are or (PLANES) as three planes of bfloat16.
+template <class T, bool PLANES>
+__global__ void __launch_bounds__(256) entropy_copy_kernel(const T* x, int64_t rows, int width, int64_t stride, void* out, int64_t pitch, int64_t plane) {
+  using Eight = Pack<T, 8 * static_cast<int>(sizeof(T))>;
   pdl_launch_dependents();
   pdl_wait();
   const int64_t all = rows * (pitch / 8);
@@ -32,17 +34,17 @@ __global__ void __launch_bounds__(256) entropy_planes_kernel(const T* x, int64_t
     const int64_t row = i / (pitch / 8);
     const int c = static_cast<int>(i - row * (pitch / 8)) * 8;
     const T* src = x + row * stride + c;
-    Pack<T, 8 * static_cast<int>(sizeof(T))> v;
+    Eight v;
     if (c + 8 <= width && reinterpret_cast<uintptr_t>(src) % sizeof(v) == 0) {
-      v = *reinterpret_cast<const Pack<T, 8 * static_cast<int>(sizeof(T))>*>(src);
+      v = *reinterpret_cast<const Eight*>(src);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v.v[e] = c + e < width ? src[e] : from_float<T>(0.f);
     }
-    uint16_t* to = out + row * pitch + c;
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(&v);
+    if constexpr (!PLANES) {
+      *reinterpret_cast<Eight*>(static_cast<T*>(out) + row * pitch + c) = v;
     } else {
+      uint16_t* to = static_cast<uint16_t*>(out) + row * pitch + c;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
         uint32_t w[4];
@@ -62,7 +64,10 @@ __global__ void __launch_bounds__(256) entropy_planes_kernel(const T* x, int64_t
 
 struct JoinArgs {
   const float2* stats;  // [parts][rows]
-  const float* picked;
+  const float* picked;  // the logits of the rows' own symbols, or null: they are computed here
+  const void *x, *weight;
+  int64_t x_stride, weight_stride;
+  int width, type;
   const void* target;
   float *loss, *lse;
   double2* sums;  // of each block: losses, and how many there are
@@ -84,9 +89,20 @@ __device__ __forceinline__ void put_loss(const JoinArgs& p, double sum, double c
   *p.loss = static_cast<float>(p.reduction == TRITURUS_B200_REDUCTION_MEAN ? sum / fmax(count, 1.0) : sum);
 }
 
+// x[row] W[symbol], by a warp.
+template <class T>
+__device__ __forceinline__ float logit(const JoinArgs& p, int64_t row, int64_t symbol, int lane) {
+  const T *x = static_cast<const T*>(p.x) + row * p.x_stride, *w = static_cast<const T*>(p.weight) + symbol * p.weight_stride;
+  float s = 0.f;
+#pragma unroll 8
+  for (int c = lane; c < p.width; c += 32) s = fmaf(to_float(x[c]), to_float(w[c]), s);
+  return warp_sum(s);
+}
+
 // 32 rows to a block, a warp to every 32nd part.
 __global__ void __launch_bounds__(1024) entropy_join_kernel(const JoinArgs p) {
   __shared__ float2 of_warp[32][32];
+  __shared__ float own[32];
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
   const int row = static_cast<int>(blockIdx.x) * 32 + lane;
   const bool valid = row < p.rows;
@@ -98,6 +114,14 @@ __global__ void __launch_bounds__(1024) entropy_join_kernel(const JoinArgs p) {
     for (int i = warp; i < p.parts; i += 32) a = join(a, p.stats[static_cast<int64_t>(i) * p.rows + row]);
   }
   of_warp[warp][lane] = a;
+  if (p.picked == nullptr) {  // (a row to a warp)
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 32 + warp;
+    const int64_t t = r < p.rows ? index_at(p.target, p.target_wide, r) : -1;
+    float z = 0.f;
+    if (t >= 0 && t < p.symbols)
+      z = p.type == TRITURUS_B200_TYPE_F32 ? logit<float>(p, r, t, lane) : p.type == TRITURUS_B200_TYPE_BF16 ? logit<__nv_bfloat16>(p, r, t, lane) : logit<__half>(p, r, t, lane);
+    if (lane == 0) own[warp] = z;
+  }
   __syncthreads();
   if (warp != 0) return;
 #pragma unroll
@@ -108,7 +132,7 @@ __global__ void __launch_bounds__(1024) entropy_join_kernel(const JoinArgs p) {
   if (valid) {
     const int64_t t = index_at(p.target, p.target_wide, row);
     given = t != p.ignore;
-    if (given) loss = t < 0 || t >= p.symbols ? __int_as_float(0x7fc00000) : lse - p.picked[row];
+    if (given) loss = t < 0 || t >= p.symbols ? __int_as_float(0x7fc00000) : lse - (p.picked != nullptr ? p.picked[row] : own[lane]);
     p.lse[row] = lse;
     if (p.reduction == TRITURUS_B200_REDUCTION_NONE) p.loss[row] = loss;
   }
@@ -234,6 +258,25 @@ __global__ void __launch_bounds__(256) entropy_sum_kernel(const __grid_constant_
   entropy_put<T>(p, row, col, x, p.cols);
 }
 
+// The parts of dx from few rows, [splits][rows][pitch], added up.
+template <class T>
+__global__ void __launch_bounds__(256) entropy_few_sum_kernel(const __grid_constant__ FewParams p, int width) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = static_cast<int>(blockIdx.y), col = (static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x));
+  if (col >= width) return;
+  const float* part = p.e.part + row * p.e.sum_pitch + col;
+  float x = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < p.splits; ++k) x += part[static_cast<int64_t>(k) * p.rows * p.e.sum_pitch];
+  float* sum = p.e.sum + row * p.e.sum_pitch + col;
+  if (p.e.dest == DEST_SUM_ADD || p.e.dest == DEST_FINAL_ADD) x += *sum;
+  if (p.e.dest == DEST_SUM || p.e.dest == DEST_SUM_ADD)
+    *sum = x;
+  else
+    static_cast<T*>(p.e.out)[row * p.e.out_pitch + col] = from_float<T>(x);
+}
+
 // ----------------------------------------------------------------------------- host
 
 int size_of(int type) { return type == TRITURUS_B200_TYPE_F32 ? 4 : 2; }
@@ -245,29 +288,35 @@ bool sizes_ok(int64_t rows, int64_t symbols, int64_t width, int type) {
 int64_t up_to(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
 int64_t parts_of(int64_t n, int64_t unit) { return (n + unit - 1) / unit; }
 
-// A 16-bit matrix as TMA reads it.
+// A matrix as TMA reads it: of 16-bit elements, or of 32-bit ones as they are (`raw`).
 struct Matrix {
   const void* data;
   int64_t rows, width, pitch, plane;
   int planes;
+  bool raw;
 };
-bool in_place(const void* data, int64_t rows, int64_t stride, int type) {
-  return type != TRITURUS_B200_TYPE_F32 && aligned_to(data, 16) && (rows == 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)));
+// Whether an operand is read where it lies: rows on 16-byte boundaries, and 32-bit elements only as they are.
+bool in_place(const void* data, int64_t rows, int64_t stride, int type, bool raw) {
+  if (type == TRITURUS_B200_TYPE_F32 && !raw) return false;
+  return aligned_to(data, 16) && (rows == 1 || (stride > 0 && stride * size_of(type) % 16 == 0 && stride < (1ll << 37)));
 }
-// Bytes of the copy of an operand that is not read in place.
-size_t copy_bytes(const void* data, int64_t rows, int64_t width, int64_t stride, int type) {
-  if (in_place(data, rows, stride, type)) return 0;
-  return static_cast<size_t>(up_to(rows * up_to(width, 8) * 2 * (type == TRITURUS_B200_TYPE_F32 ? 3 : 1), 256));
+// Bytes of the copy of an operand that is not.
+size_t copy_bytes(const void* data, int64_t rows, int64_t width, int64_t stride, int type, bool raw) {
+  if (in_place(data, rows, stride, type, raw)) return 0;
+  return static_cast<size_t>(rows) * static_cast<size_t>(up_to(width, 8)) * (raw ? 4 : type == TRITURUS_B200_TYPE_F32 ? 6 : 2);
 }
 
 int make_map(CUtensorMap* map, const Matrix& m, int box_x, int box_y, int type) {
   const EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr) return TRITURUS_B200_EDRIVER;
+  const cuuint64_t size = m.raw ? 4 : 2;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(m.width), static_cast<cuuint64_t>(m.rows), static_cast<cuuint64_t>(m.planes)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(m.pitch) * 2, static_cast<cuuint64_t>(m.plane) * 2};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(m.pitch) * size, static_cast<cuuint64_t>(m.plane) * size};
   const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_x), static_cast<cuuint32_t>(box_y), 1}, step[3] = {1, 1, 1};
-  const CUresult rc = fn(map, type == TRITURUS_B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                         const_cast<void*>(m.data), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUtensorMapDataType kind = m.raw                            ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : type == TRITURUS_B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult rc = fn(map, kind, 3, const_cast<void*>(m.data), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return rc == CUDA_SUCCESS ? TRITURUS_B200_OK : TRITURUS_B200_ETENSORMAP;
 }
@@ -277,22 +326,27 @@ struct Launches {
   cudaStream_t stream;
   bool first = true;
   template <class... Params, class... Args>
-  int operator()(void (*kern)(Params...), int64_t grid, int threads, size_t smem, Args&&... args) {
+  int operator()(void (*kern)(Params...), dim3 grid, int threads, size_t smem, Args&&... args) {
     const cudaLaunchAttribute dependent = dependent_launch();
-    const int rc = launch_of(kern, dim3(static_cast<unsigned>(grid)), threads, smem, stream, first ? nullptr : &dependent, static_cast<Args&&>(args)...);
+    const int rc = launch_of(kern, grid, threads, smem, stream, first ? nullptr : &dependent, static_cast<Args&&>(args)...);
     first = false;
     return rc;
+  }
+  template <class... Params, class... Args>
+  int operator()(void (*kern)(Params...), int64_t grid, int threads, size_t smem, Args&&... args) {
+    return (*this)(kern, dim3(static_cast<unsigned>(grid)), threads, smem, static_cast<Args&&>(args)...);
   }
 };
 
 int copy_grid(int64_t items) { return static_cast<int>(std::min<int64_t>(parts_of(items, 256), static_cast<int64_t>(device_sms()) * 16)); }
 
 // The operand itself or, copied to `space`, one that TMA can read.
-int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t stride, int type, void* space, Launches& launch) {
+int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t stride, int type, bool raw, void* space, Launches& launch) {
   m->rows = rows;
   m->width = width;
-  m->planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
-  if (in_place(data, rows, stride, type)) {
+  m->raw = raw;
+  m->planes = type == TRITURUS_B200_TYPE_F32 && !raw ? 3 : 1;
+  if (in_place(data, rows, stride, type, raw)) {
     m->data = data;
     m->pitch = rows == 1 ? up_to(width, 8) : stride;
     m->plane = rows * m->pitch;
@@ -302,12 +356,12 @@ int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t st
   m->pitch = up_to(width, 8);
   m->plane = rows * m->pitch;
   const int grid = copy_grid(rows * (m->pitch / 8));
-  const auto run = [&](auto t) {
-    using T = decltype(t);
-    return launch(entropy_planes_kernel<T>, grid, 256, 0, static_cast<const T*>(data), rows, static_cast<int>(width), stride,
-                     static_cast<uint16_t*>(space), m->pitch, m->plane);
+  const auto run = [&](auto kern, auto t) {
+    return launch(kern, grid, 256, 0, static_cast<const decltype(t)*>(data), rows, static_cast<int>(width), stride, space, m->pitch, m->plane);
   };
-  return type == TRITURUS_B200_TYPE_F32 ? run(0.f) : type == TRITURUS_B200_TYPE_BF16 ? run(__nv_bfloat16()) : run(__half());
+  if (type == TRITURUS_B200_TYPE_F32) return raw ? run(entropy_copy_kernel<float, false>, 0.f) : run(entropy_copy_kernel<float, true>, 0.f);
+  if (type == TRITURUS_B200_TYPE_BF16) return run(entropy_copy_kernel<__nv_bfloat16, false>, __nv_bfloat16());
+  return run(entropy_copy_kernel<__half, false>, __half());
 }
 
 int pairs_in_all() { return std::max(1, device_sms() / 2); }
@@ -443,6 +497,79 @@ size_t part_bytes(const EntropyParams& p) {
   return static_cast<size_t>(p.shared) * static_cast<size_t>(p.splits) * 256 * static_cast<size_t>(p.tile_cols) * sizeof(float);
 }
 
+// ----------------------------------------------------------------------------- few rows
+
+// Up to this many rows: XXX
+bool few(int64_t rows, int type) { return rows <= (type == TRITURUS_B200_TYPE_F32 ? 128 : 64); }
+
+FewParams few_of(int64_t rows, int64_t length, int64_t k) {
+  FewParams p = {};
+  p.rows = static_cast<int>(rows);
+  p.length = static_cast<int>(length);
+  p.kblocks = static_cast<int>(parts_of(k, 64));
+  p.mma_n = static_cast<int>(std::min<int64_t>(64, up_to(rows, 16)));
+  return p;
+}
+// STATS, PROB: an even span of the symbols for each SM.
+FewParams few_symbols_of(int64_t rows, int64_t symbols, int64_t width) {
+  FewParams p = few_of(rows, symbols, width);
+  const int64_t row_tiles = parts_of(rows, 64);
+  p.span = static_cast<int>(std::max<int64_t>(16, parts_of(symbols, std::max<int64_t>(1, device_sms() / row_tiles))));
+  p.spans = static_cast<int>(parts_of(symbols, p.span));
+  p.tile = static_cast<int>(parts_of(p.span, parts_of(p.span, 128)));
+  p.splits = 1;
+  p.kb_split = p.kblocks;
+  p.units = static_cast<int>(p.spans * row_tiles);
+  return p;
+}
+// OUT_X: tiles of 128 columns, the contraction cut into parts for the SMs.
+FewParams few_columns_of(int64_t rows, int64_t width, int64_t symbols) {
+  FewParams p = few_of(rows, width, symbols);
+  const int64_t row_tiles = parts_of(rows, 64);
+  p.span = p.tile = 128;
+  p.spans = static_cast<int>(parts_of(width, 128));
+  const int64_t splits = std::clamp<int64_t>(device_sms() / (p.spans * row_tiles), 1, p.kblocks);
+  p.kb_split = static_cast<int>(parts_of(p.kblocks, splits));
+  p.splits = static_cast<int>(parts_of(p.kblocks, p.kb_split));
+  p.units = static_cast<int>(p.spans * p.splits * row_tiles);
+  return p;
+}
+
+// W (a) and x or d (b).
+template <class Cfg>
+int launch_few(const Matrix& a, const Matrix& b, FewParams p, int type, Launches& launch) {
+  CUtensorMap ta, tb;
+  int rc = Cfg::A_MN ? make_map(&ta, a, Cfg::WIDE ? 32 : 64, Cfg::BK, type) : make_map(&ta, a, Cfg::WIDE ? 32 : 64, p.tile, type);
+  if (rc == TRITURUS_B200_OK) rc = make_map(&tb, b, Cfg::BK, p.mma_n, type);
+  if (rc != TRITURUS_B200_OK) return rc;
+  const auto kern = entropy_few_kernel<Cfg>;
+  static std::atomic<bool> known[64];
+  int dev = 0;
+  if (code_of(cudaGetDevice(&dev)) != TRITURUS_B200_OK || dev < 0 || dev >= 64) return TRITURUS_B200_ELAUNCH;
+  if (!known[dev].load(std::memory_order_relaxed)) {
+    rc = code_of(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+    if (rc != TRITURUS_B200_OK) return rc;
+    known[dev].store(true, std::memory_order_relaxed);
+  }
+  p.e.half = type == TRITURUS_B200_TYPE_F16;
+  p.a_bytes = Cfg::A_MN ? Cfg::A_TILE : p.tile * Cfg::BK * (Cfg::WIDE ? 4 : 2);
+  p.b_bytes = Cfg::PLANES * p.mma_n * Cfg::BK * 2;
+  p.idesc = umma_idesc_16(Cfg::BM, p.e.half != 0, Cfg::A_MN && !Cfg::WIDE, false) | static_cast<uint32_t>(p.mma_n >> 3) << 17;
+  return launch(kern, std::min(p.units, device_sms()), Cfg::NTHREADS, Cfg::SMEM_BYTES, ta, tb, p);
+}
+template <int MODE>
+int run_few(const Matrix& a, const Matrix& b, const FewParams& p, int type, Launches& launch) {
+  return type == TRITURUS_B200_TYPE_F32 ? launch_few<FewCfg<MODE, true>>(a, b, p, type, launch) : launch_few<FewCfg<MODE, false>>(a, b, p, type, launch);
+}
+
+int sum_few(const FewParams& p, int64_t width, int type, Launches& launch) {
+  const dim3 grid(static_cast<unsigned>(parts_of(width, 256)), static_cast<unsigned>(p.rows));
+  const int w = static_cast<int>(width);
+  return type == TRITURUS_B200_TYPE_F32    ? launch(entropy_few_sum_kernel<float>, grid, 256, 0, p, w)
+         : type == TRITURUS_B200_TYPE_BF16 ? launch(entropy_few_sum_kernel<__nv_bfloat16>, grid, 256, 0, p, w)
+                                           : launch(entropy_few_sum_kernel<__half>, grid, 256, 0, p, w);
+}
+
 struct Space {  // the workspace as it is handed out
   char* at;
   size_t used;
@@ -464,10 +591,12 @@ ForwardSpace forward_space(void* base, const void* x, const void* weight, int64_
                            int64_t weight_stride, int type) {
   Space s = {static_cast<char*>(base), 0};
   ForwardSpace f;
-  f.x = s.take(copy_bytes(x, rows, width, x_stride, type));
-  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type));
-  f.stats = static_cast<float2*>(s.take(static_cast<size_t>(stats_of(rows, symbols, width, type).units_n) * 2 * static_cast<size_t>(rows) * sizeof(float2)));
-  f.picked = static_cast<float*>(s.take(static_cast<size_t>(rows) * sizeof(float)));
+  const bool is_few = few(rows, type);
+  f.x = s.take(copy_bytes(x, rows, width, x_stride, type, false));
+  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32));
+  const int64_t parts = is_few ? few_symbols_of(rows, symbols, width).spans * 4 : stats_of(rows, symbols, width, type).units_n * 2;
+  f.stats = static_cast<float2*>(s.take(static_cast<size_t>(parts) * static_cast<size_t>(rows) * sizeof(float2)));
+  f.picked = static_cast<float*>(s.take(static_cast<size_t>(is_few ? 0 : rows) * sizeof(float)));
   f.sums = static_cast<double2*>(s.take(static_cast<size_t>(parts_of(rows, 32)) * sizeof(double2)));
   f.bytes = s.used;
   return f;
@@ -498,14 +627,18 @@ BackwardSpace backward_space(void* base, const BackwardPlan& b, const void* x, c
                              int64_t x_stride, int64_t weight_stride, int type) {
   Space s = {static_cast<char*>(base), 0};
   BackwardSpace f;
-  f.x = s.take(copy_bytes(x, rows, width, x_stride, type));
-  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type));
+  const bool is_few = few(rows, type);
+  f.x = s.take(copy_bytes(x, rows, width, x_stride, type, false));
+  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32));
   f.factors = static_cast<float*>(s.take(2 * sizeof(float)));
   f.d = static_cast<uint16_t*>(s.take(static_cast<size_t>(rows) * static_cast<size_t>(b.d_pitch) * 2 * (type == TRITURUS_B200_TYPE_F32 ? 3 : 1)));
   f.sum = static_cast<float*>(s.take(b.pieces > 1 ? static_cast<size_t>(rows) * static_cast<size_t>(b.sum_pitch) * sizeof(float) : 0));
   size_t parts = 0;  // (one product at a time uses them)
-  for (const int64_t piece : {b.piece, b.last})
-    parts = std::max({parts, part_bytes(out_of(rows, width, piece, type)), part_bytes(out_of(piece, width, rows, type))});
+  for (const int64_t piece : {b.piece, b.last}) {
+    const size_t of_x = is_few ? static_cast<size_t>(few_columns_of(rows, width, piece).splits) * static_cast<size_t>(rows * b.sum_pitch) * sizeof(float)
+                               : part_bytes(out_of(rows, width, piece, type));
+    parts = std::max({parts, of_x, part_bytes(out_of(piece, width, rows, type))});
+  }
   f.part = static_cast<float*>(s.take(parts));
   f.bytes = s.used;
   return f;
@@ -545,24 +678,40 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
   if (workspace_bytes < space.bytes) return TRITURUS_B200_EWORKSPACE;
 
   Matrix a, b;
-  int rc = prepare(&a, x, rows, width, x_stride, type, space.x, launch);
-  if (rc == TRITURUS_B200_OK) rc = prepare(&b, weight, symbols, width, weight_stride, type, space.weight, launch);
+  const bool is_few = few(rows, type);
+  int rc = prepare(&a, x, rows, width, x_stride, type, false, space.x, launch);
+  if (rc == TRITURUS_B200_OK) rc = prepare(&b, weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32, space.weight, launch);
   if (rc != TRITURUS_B200_OK) return rc;
-  EntropyParams p = stats_of(rows, symbols, width, type);
-  if (!set_whole(p)) return TRITURUS_B200_EINVAL;
-  p.stats = space.stats;
-  p.picked = space.picked;
-  p.target = target;
-  p.target_wide = target_bytes == 8;
-  p.ignore = ignore_index;
-  p.symbols = symbols;
-  p.status = status_dev;
-  rc = run_products<ENTROPY_STATS>(a, b, p, type, launch);
+  JoinArgs j = {};
+  if (is_few) {
+    FewParams p = few_symbols_of(rows, symbols, width);
+    p.e.stats = space.stats;
+    p.e.status = status_dev;
+    rc = run_few<ENTROPY_STATS>(b, a, p, type, launch);
+    j.parts = p.spans * 4;
+    j.x = x;
+    j.weight = weight;
+    j.x_stride = x_stride;
+    j.weight_stride = weight_stride;
+    j.width = static_cast<int>(width);
+    j.type = type;
+  } else {
+    EntropyParams p = stats_of(rows, symbols, width, type);
+    if (!set_whole(p)) return TRITURUS_B200_EINVAL;
+    p.stats = space.stats;
+    p.picked = space.picked;
+    p.target = target;
+    p.target_wide = target_bytes == 8;
+    p.ignore = ignore_index;
+    p.symbols = symbols;
+    p.status = status_dev;
+    rc = run_products<ENTROPY_STATS>(a, b, p, type, launch);
+    j.parts = p.units_n * 2;
+    j.picked = space.picked;
+  }
   if (rc != TRITURUS_B200_OK) return rc;
 
-  JoinArgs j = {};
   j.stats = space.stats;
-  j.picked = space.picked;
   j.target = target;
   j.loss = loss;
   j.lse = lse;
@@ -570,8 +719,7 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
   j.ignore = ignore_index;
   j.symbols = symbols;
   j.rows = static_cast<int>(rows);
-  j.parts = p.units_n * 2;
-  j.target_wide = p.target_wide;
+  j.target_wide = target_bytes == 8;
   j.reduction = reduction;
   const int blocks = static_cast<int>(parts_of(rows, 32));
   rc = launch(entropy_join_kernel, blocks, 1024, 0, j);
@@ -606,8 +754,9 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
 
   Launches launch = {st};
   Matrix mx, mw;
-  int rc = prepare(&mx, x, rows, width, x_stride, type, space.x, launch);
-  if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, type, space.weight, launch);
+  const bool is_few = few(rows, type);
+  int rc = prepare(&mx, x, rows, width, x_stride, type, false, space.x, launch);
+  if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32, space.weight, launch);
   const int wide = target_bytes == 8;
   if (rc == TRITURUS_B200_OK)
     rc = launch(entropy_factors_kernel, 1, 1024, 0, dloss, reduction == TRITURUS_B200_REDUCTION_NONE ? 1 : 0, target, wide, ignore_index,
@@ -636,7 +785,13 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
     p.d_pitch = md.pitch;
     p.d_plane = md.plane;
     p.status = status_dev;
-    rc = run_products<ENTROPY_PROB>(mx, mw, p, type, launch);
+    if (is_few) {
+      FewParams f = few_symbols_of(rows, piece, width);
+      f.e = p;
+      rc = run_few<ENTROPY_PROB>(mw, mx, f, type, launch);
+    } else {
+      rc = run_products<ENTROPY_PROB>(mx, mw, p, type, launch);
+    }
     md.width = piece;
     const auto out = [&](EntropyParams q, void* to, int dest) {
       q.factors = space.factors;
@@ -655,7 +810,14 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
       const bool begin = i == 0, end = i + 1 == plan.pieces;
       EntropyParams q = out(out_of(rows, width, piece, type), dx, begin ? end ? DEST_FINAL : DEST_SUM : end ? DEST_FINAL_ADD : DEST_SUM_ADD);
       q.b_k = static_cast<int>(first);
-      rc = set_whole(q) ? run_products<ENTROPY_OUT_X>(md, mw, q, type, launch) : TRITURUS_B200_EINVAL;
+      if (is_few) {
+        FewParams f = few_columns_of(rows, width, piece);
+        f.e = q;
+        rc = run_few<ENTROPY_OUT_X>(mw, md, f, type, launch);
+        if (rc == TRITURUS_B200_OK) rc = sum_few(f, width, type, launch);
+      } else {
+        rc = set_whole(q) ? run_products<ENTROPY_OUT_X>(md, mw, q, type, launch) : TRITURUS_B200_EINVAL;
+      }
     }
     if (dweight != nullptr && rc == TRITURUS_B200_OK) {
       EntropyParams q = out(out_of(piece, width, rows, type), static_cast<char*>(dweight) + first * width * size, DEST_FINAL);
