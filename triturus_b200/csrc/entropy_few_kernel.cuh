@@ -47,6 +47,10 @@ struct FewParams {
   int mma_n;              // columns of the MMAs
   int a_bytes, b_bytes;   // of a stage's copies
   uint32_t idesc;
+  int mean;              // PROB: dloss is that of the mean
+  const void *x, *weight;  // STATS: as they were given, for the logits of the rows' own symbols
+  int64_t x_stride, weight_stride;
+  int width;
   EntropyParams e;        // what the forms have in common with those of entropy_kernel
 };
 
@@ -87,6 +91,16 @@ __device__ __forceinline__ float columns_to_lanes(float (&v)[32], int lane, F f)
   return v[0];
 }
 
+// x[row] W[symbol], by a warp.
+template <class T>
+__device__ __forceinline__ float logit(const FewParams& p, int64_t row, int64_t symbol, int lane) {
+  const T *x = static_cast<const T*>(p.x) + row * p.x_stride, *w = static_cast<const T*>(p.weight) + symbol * p.weight_stride;
+  float s = 0.f;
+#pragma unroll 8
+  for (int c = lane; c < p.width; c += 32) s = fmaf(to_float(x[c]), to_float(w[c]), s);
+  return warp_sum(s);
+}
+
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::NTHREADS, 1)
 entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ FewParams p) {
@@ -107,13 +121,16 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
   uint64_t* cut_empty = cut_full + 2;      // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cut_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* of_done = reinterpret_cast<int*>(tmem_slot + 2);          // [2] STATS: warps of a half of the rows that have left their part
   uint8_t* of_rows = reinterpret_cast<uint8_t*>(tmem_slot + 4);  // [8][32 * 20] PROB: what each epilogue warp needs of its rows of x
+  float2* of_stats = reinterpret_cast<float2*>(of_rows);         // [8][32] STATS: those parts
 
   const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const AbortCtl ctl{abort_flag, p.e.status};
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
+    of_done[0] = of_done[1] = 0;
     for (int s = 0; s < NSA; ++s) {
       mbar_init(&a_full[s], 1);
       mbar_init(&a_empty[s], WIDE ? Cfg::CUT_WARPS : 1);
@@ -151,11 +168,11 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     bool first, last;  // of its unit
   };
   const auto walk = [&](auto&& tile) {
-    for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
-      const int of_rows = p.spans * p.splits;
+    for (int u = blockIdx.x; u < p.units; u += gridDim.x) {  // (STATS, PROB: one)
+      const int of_tile = p.spans * p.splits;
       Tile t;
-      t.n0 = u / of_rows * BN;
-      const int r = u % of_rows;
+      t.n0 = u / of_tile * BN;
+      const int r = u % of_tile;
       t.ks = r / p.spans;
       t.span = r - t.ks * p.spans;
       t.k0 = t.ks * p.kb_split;
@@ -250,6 +267,22 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
       }
       return true;
     });
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ STATS: the logits of the rows' own symbols, a row to a CTA
+    if constexpr (MODE == ENTROPY_STATS) {
+      if (blockIdx.x == 0 && lane == 0) *p.e.arrived = 0;
+      for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const int64_t t = entropy_target(p.e, row);
+        if (t < 0 || t >= p.e.symbols) continue;
+        float z;
+        if constexpr (WIDE) {
+          z = logit<float>(p, row, t, lane);
+        } else {
+          z = p.e.half ? logit<__half>(p, row, t, lane) : logit<__nv_bfloat16>(p, row, t, lane);
+        }
+        if (lane == 0) p.e.picked[row] = z;
+      }
+    }
   } else if (warp >= 4 && warp < 12) {
     // ------------------------------------------------------------------ epilogue: a row of the MMAs and 32 of their columns to a thread
     const int q = warp & 3, h = (warp - 4) >> 2;
@@ -261,6 +294,26 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     float* of_lse = reinterpret_cast<float*>(of_target + 32);
     float* of_lse2 = of_lse + 32;
     float* of_g = of_lse2 + 32;
+
+    float factor = 1.f;
+    if constexpr (MODE == ENTROPY_PROB) {  // (few rows: each warp finds this for itself)
+      float largest = 0.f;
+      int count = 0;
+      for (int i = lane; i < p.rows; i += 32) {
+        if (entropy_target(p.e, i) == p.e.ignore) continue;
+        ++count;
+        const float g = fabsf(p.e.dloss[p.e.per_row ? i : 0]);
+        if (g < INFINITY) largest = fmaxf(largest, g);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        count += __shfl_xor_sync(0xffffffffu, count, o);
+      }
+      const float2 f = entropy_factors(largest, count, p.mean, p.e.half);
+      factor = f.x;
+      if (blockIdx.x == 0 && threadIdx.x == 128) p.e.factors[1] = f.y;  // for the products that follow
+    }
 
     walk([&](const Tile& t) {
       const int m = t.m0 + q * 32 + lane;  // symbol of the piece, or column
@@ -282,7 +335,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           of_target[lane] = ignored ? -1 : to - p.e.b_row;
           of_lse[lane] = ignored ? INFINITY : lse;  // (no lse is that: infinite logits make it NaN)
           of_lse2[lane] = lse * LOG2E_F;
-          of_g[lane] = ignored ? 0.f : to < 0 || to >= p.e.symbols ? __int_as_float(0x7fc00000) : p.e.dloss[p.e.per_row ? n + lane : 0] * p.e.factors[0];
+          of_g[lane] = ignored ? 0.f : to < 0 || to >= p.e.symbols ? __int_as_float(0x7fc00000) : p.e.dloss[p.e.per_row ? n + lane : 0] * factor;
           __syncwarp();
         }
       }
@@ -317,7 +370,26 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         for (int e = 0; e < 32; ++e) v[e] = ex2_approx((sum[e] - __shfl_sync(0xffffffffu, base, e)) * LOG2E_F);
         total = total * ex2_approx((top - base) * LOG2E_F) + columns_to_lanes(v, lane, [](float a, float b) { return a + b; });
         top = now;
-        if (t.last && lane < count) p.e.stats[(static_cast<int64_t>(t.span) * 4 + q) * p.rows + n + lane] = make_float2(top, total);
+        if (t.last) {
+          // the four warps of these rows of x leave theirs to the last one of them (a CTA has one unit: this happens once)
+          of_stats[(h * 4 + q) * 32 + lane] = make_float2(top, total);
+          __threadfence_block();
+          __syncwarp();
+          const int order = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(&of_done[h], 1) : 0, 0);
+          if (order == 3) {
+            __threadfence_block();
+            float m4 = -INFINITY, s4 = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m4 = fmaxf(m4, of_stats[(h * 4 + k) * 32 + lane].x);
+            const float b4 = m4 == -INFINITY ? 0.f : m4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 a = of_stats[(h * 4 + k) * 32 + lane];
+              s4 = fmaf(a.y, ex2_approx((a.x - b4) * LOG2E_F), s4);
+            }
+            if (lane < count) p.e.stats[static_cast<int64_t>(t.span) * p.rows + n + lane] = make_float2(m4, s4);
+          }
+        }
       } else if constexpr (MODE == ENTROPY_PROB) {
         if (valid) {
           uint16_t* to = p.e.d + static_cast<int64_t>(n) * p.e.d_pitch + m;

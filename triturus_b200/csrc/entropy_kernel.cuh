@@ -81,6 +81,7 @@ struct EntropyParams {
   // STATS: [units_n * 2][rows] of maximum and sum, and the logits of the rows' own symbols
   float2* stats;
   float* picked;
+  int* arrived;           // set to zero for the launch that joins them
   // STATS and PROB
   const void* target;
   int target_wide;        // 64 bits
@@ -90,7 +91,7 @@ struct EntropyParams {
   const float* lse;
   const float* dloss;     // [rows], or one number
   int per_row;
-  const float* factors;   // what dloss is multiplied by; what the gradients are
+  float* factors;         // what dloss is multiplied by; what the gradients are
   uint16_t* d;            // [planes][rows][d_pitch]
   int64_t d_pitch, d_plane;
   // OUT
@@ -148,6 +149,15 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
 // leaves a NaN.)
 __device__ __forceinline__ uint32_t plane_bits(float x0, float x1) { return __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632); }
 __device__ __forceinline__ float plane_rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+
+// What dloss is multiplied by in d, and what dx and dW are multiplied by, for the largest finite |dloss| and the number of targets that are not ignored.  In
+// float16 d is scaled so that the largest |dloss| stands for 2^15: |d| is at most that, and a probability of 2^-29 still has all of its digits.
+__device__ __forceinline__ float2 entropy_factors(float top, int count, int mean, int half) {
+  const float share = mean ? 1.f / static_cast<float>(max(count, 1)) : 1.f;
+  if (!half) return make_float2(share, 1.f);
+  top = top == 0.f ? 1.f : fmaxf(top, 0x1p-100f);
+  return make_float2(32768.f / top, top * share * 0x1p-15f);
+}
 
 __device__ __forceinline__ int64_t entropy_target(const EntropyParams& p, int64_t row) {
   return p.target_wide ? static_cast<const int64_t*>(p.target)[row] : static_cast<int64_t>(static_cast<const int32_t*>(p.target)[row]);
@@ -248,6 +258,9 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   pdl_launch_dependents();
   pdl_wait();
+  if constexpr (MODE == ENTROPY_STATS) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.arrived = 0;
+  }
 
   // tile(t) for each tile of this pair in turn; leaves when one returns false.  A group of row tiles is gone over column by column: the pairs
   // that run at the same time share rows and columns through the L2 cache.

@@ -62,115 +62,108 @@ __global__ void __launch_bounds__(256) entropy_copy_kernel(const T* x, int64_t r
 
 // ----------------------------------------------------------------------------- small kernels around the products
 
-struct JoinArgs {
-  const float2* stats;  // [parts][rows]
-  const float* picked;  // the logits of the rows' own symbols, or null: they are computed here
-  const void *x, *weight;
-  int64_t x_stride, weight_stride;
-  int width, type;
-  const void* target;
-  float *loss, *lse;
-  double2* sums;  // of each block: losses, and how many there are
-  int64_t ignore, symbols;
-  int rows, parts, target_wide, reduction;
-};
-
 __device__ __forceinline__ int64_t index_at(const void* a, int wide, int64_t i) {
   return wide ? static_cast<const int64_t*>(a)[i] : static_cast<int64_t>(static_cast<const int32_t*>(a)[i]);
 }
 
-// (m, s) stands for s exp(m).
-__device__ __forceinline__ float2 join(float2 a, float2 b) {
-  const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
-  return make_float2(m, a.y * ex2_approx((a.x - base) * LOG2E_F) + b.y * ex2_approx((b.x - base) * LOG2E_F));
+struct JoinArgs {
+  const float2* stats;  // [parts][rows]
+  const float* picked;  // the logits of the rows' own symbols
+  const void* target;
+  float *loss, *lse;
+  double2* sums;  // of each block: losses, and how many there are
+  int* arrived;   // blocks whose sums are there (zero before)
+  int64_t ignore, symbols;
+  int rows, parts, target_wide, reduction;
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
-__device__ __forceinline__ void put_loss(const JoinArgs& p, double sum, double count) {
-  *p.loss = static_cast<float>(p.reduction == TRITURUS_B200_REDUCTION_MEAN ? sum / fmax(count, 1.0) : sum);
-}
-
-// x[row] W[symbol], by a warp.
-template <class T>
-__device__ __forceinline__ float logit(const JoinArgs& p, int64_t row, int64_t symbol, int lane) {
-  const T *x = static_cast<const T*>(p.x) + row * p.x_stride, *w = static_cast<const T*>(p.weight) + symbol * p.weight_stride;
-  float s = 0.f;
-#pragma unroll 8
-  for (int c = lane; c < p.width; c += 32) s = fmaf(to_float(x[c]), to_float(w[c]), s);
-  return warp_sum(s);
-}
-
-// 32 rows to a block, a warp to every 32nd part.
+// 32 rows to a block: their parts are read by a lane to a row and every 32nd part to a warp, and joined by a warp to a row.  The block that comes last
+// adds the blocks' losses, always in the same order.
 __global__ void __launch_bounds__(1024) entropy_join_kernel(const JoinArgs p) {
-  __shared__ float2 of_warp[32][32];
-  __shared__ float own[32];
+  __shared__ float shared[32][33], top_of[32];
+  __shared__ double loss_of[32];
+  __shared__ int given_of[32], last;
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
   const int row = static_cast<int>(blockIdx.x) * 32 + lane;
-  const bool valid = row < p.rows;
-  float2 a = make_float2(-INFINITY, 0.f);
   pdl_launch_dependents();
   pdl_wait();
-  if (valid) {
-#pragma unroll 4
-    for (int i = warp; i < p.parts; i += 32) a = join(a, p.stats[static_cast<int64_t>(i) * p.rows + row]);
+  float top = -INFINITY;
+  if (row < p.rows) {
+#pragma unroll 8
+    for (int i = warp; i < p.parts; i += 32) top = fmaxf(top, p.stats[static_cast<int64_t>(i) * p.rows + row].x);
   }
-  of_warp[warp][lane] = a;
-  if (p.picked == nullptr) {  // (a row to a warp)
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 32 + warp;
-    const int64_t t = r < p.rows ? index_at(p.target, p.target_wide, r) : -1;
-    float z = 0.f;
-    if (t >= 0 && t < p.symbols)
-      z = p.type == TRITURUS_B200_TYPE_F32 ? logit<float>(p, r, t, lane) : p.type == TRITURUS_B200_TYPE_BF16 ? logit<__nv_bfloat16>(p, r, t, lane) : logit<__half>(p, r, t, lane);
-    if (lane == 0) own[warp] = z;
-  }
+  shared[warp][lane] = top;
   __syncthreads();
-  if (warp != 0) return;
-#pragma unroll
-  for (int w = 1; w < 32; ++w) a = join(a, of_warp[w][lane]);
-  const float lse = (a.x == -INFINITY ? 0.f : a.x) + logf(a.y);
-  float loss = 0.f;
-  bool given = false;
-  if (valid) {
-    const int64_t t = index_at(p.target, p.target_wide, row);
-    given = t != p.ignore;
-    if (given) loss = t < 0 || t >= p.symbols ? __int_as_float(0x7fc00000) : lse - (p.picked != nullptr ? p.picked[row] : own[lane]);
-    p.lse[row] = lse;
-    if (p.reduction == TRITURUS_B200_REDUCTION_NONE) p.loss[row] = loss;
+  top = warp_max(shared[lane][warp]);
+  if (lane == 0) top_of[warp] = top == -INFINITY ? 0.f : top;
+  __syncthreads();
+  const float base = top_of[lane];
+  float total = 0.f;
+  if (row < p.rows) {
+#pragma unroll 8
+    for (int i = warp; i < p.parts; i += 32) {
+      const float2 a = p.stats[static_cast<int64_t>(i) * p.rows + row];
+      total = fmaf(a.y, ex2_approx((a.x - base) * LOG2E_F), total);
+    }
+  }
+  shared[warp][lane] = total;
+  __syncthreads();
+  total = warp_sum(shared[lane][warp]);
+  if (lane == 0) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * 32 + warp;
+    const float lse = top_of[warp] + logf(total);
+    float loss = 0.f;
+    bool given = false;
+    if (r < p.rows) {
+      const int64_t t = index_at(p.target, p.target_wide, r);
+      given = t != p.ignore;
+      if (given) loss = t < 0 || t >= p.symbols ? __int_as_float(0x7fc00000) : lse - p.picked[r];
+      p.lse[r] = lse;
+      if (p.reduction == TRITURUS_B200_REDUCTION_NONE) p.loss[r] = loss;
+    }
+    loss_of[warp] = loss;
+    given_of[warp] = given ? 1 : 0;
   }
   if (p.reduction == TRITURUS_B200_REDUCTION_NONE) return;
-  double sum = loss;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const int count = __popc(__ballot_sync(0xffffffffu, given));
-  if (lane != 0) return;
-  if (gridDim.x == 1)
-    put_loss(p, sum, count);
-  else
-    p.sums[blockIdx.x] = make_double2(sum, count);
-}
-
-__global__ void __launch_bounds__(256) entropy_loss_kernel(const JoinArgs p, int blocks) {
-  __shared__ double2 part[256];
-  double2 a = make_double2(0.0, 0.0);
-  pdl_launch_dependents();
-  pdl_wait();
-  for (int i = static_cast<int>(threadIdx.x); i < blocks; i += 256) {
-    a.x += p.sums[i].x;
-    a.y += p.sums[i].y;
-  }
-  part[threadIdx.x] = a;
   __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (static_cast<int>(threadIdx.x) < o) {
-      part[threadIdx.x].x += part[threadIdx.x + o].x;
-      part[threadIdx.x].y += part[threadIdx.x + o].y;
-    }
-    __syncthreads();
+  if (warp != 0) return;
+  double sum = loss_of[lane], count = given_of[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    count += __shfl_xor_sync(0xffffffffu, count, o);
   }
-  if (threadIdx.x == 0) put_loss(p, part[0].x, part[0].y);
+  if (gridDim.x > 1) {
+    if (lane == 0) {
+      p.sums[blockIdx.x] = make_double2(sum, count);
+      __threadfence();
+      last = atomicAdd(p.arrived, 1) == static_cast<int>(gridDim.x) - 1;
+    }
+    __syncwarp();
+    if (!last) return;
+    __threadfence();
+    sum = count = 0.0;
+    for (int i = lane; i < static_cast<int>(gridDim.x); i += 32) {
+      const double2 a = __ldcg(&p.sums[i]);
+      sum += a.x;
+      count += a.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      count += __shfl_xor_sync(0xffffffffu, count, o);
+    }
+  }
+  if (lane == 0) *p.loss = static_cast<float>(p.reduction == TRITURUS_B200_REDUCTION_MEAN ? sum / fmax(count, 1.0) : sum);
 }
 
-// factors[0]: what dloss is multiplied by in d; factors[1]: what dx and dW are multiplied by.  In float16 d is scaled so that the largest |dloss|
-// stands for 2^15: |d| is at most that, and a probability of 2^-29 still has all of its digits.
+// factors[0] and [1]: see entropy_factors.
 __global__ void __launch_bounds__(1024) entropy_factors_kernel(const float* dloss, int per_row, const void* target, int target_wide, int64_t ignore, int rows,
                                                                int mean, int half, float* factors) {
   __shared__ float top_of[32];
@@ -208,15 +201,9 @@ __global__ void __launch_bounds__(1024) entropy_factors_kernel(const float* dlos
     top = fmaxf(top, top_of[w]);
     count += count_of[w];
   }
-  const float share = mean ? 1.f / static_cast<float>(max(count, 1)) : 1.f;
-  if (half) {
-    top = top == 0.f ? 1.f : fmaxf(top, 0x1p-100f);
-    factors[0] = 32768.f / top;
-    factors[1] = top * share * 0x1p-15f;
-  } else {
-    factors[0] = share;
-    factors[1] = 1.f;
-  }
+  const float2 f = entropy_factors(top, count, mean, half);
+  factors[0] = f.x;
+  factors[1] = f.y;
 }
 
 // The parts of shared tiles added up, four elements to a thread, and what is done with whole tiles.
@@ -267,7 +254,7 @@ __global__ void __launch_bounds__(256) entropy_few_sum_kernel(const __grid_const
   if (col >= width) return;
   const float* part = p.e.part + row * p.e.sum_pitch + col;
   float x = 0.f;
-#pragma unroll 8
+#pragma unroll 16
   for (int k = 0; k < p.splits; ++k) x += part[static_cast<int64_t>(k) * p.rows * p.e.sum_pitch];
   float* sum = p.e.sum + row * p.e.sum_pitch + col;
   if (p.e.dest == DEST_SUM_ADD || p.e.dest == DEST_FINAL_ADD) x += *sum;
@@ -528,7 +515,7 @@ FewParams few_columns_of(int64_t rows, int64_t width, int64_t symbols) {
   const int64_t row_tiles = parts_of(rows, 64);
   p.span = p.tile = 128;
   p.spans = static_cast<int>(parts_of(width, 128));
-  const int64_t splits = std::clamp<int64_t>(device_sms() / (p.spans * row_tiles), 1, p.kblocks);
+  const int64_t splits = std::clamp<int64_t>(device_sms() / (p.spans * row_tiles), 1, parts_of(p.kblocks, 4));
   p.kb_split = static_cast<int>(parts_of(p.kblocks, splits));
   p.splits = static_cast<int>(parts_of(p.kblocks, p.kb_split));
   p.units = static_cast<int>(p.spans * p.splits * row_tiles);
@@ -585,6 +572,7 @@ struct ForwardSpace {
   float2* stats;
   float* picked;
   double2* sums;
+  int* arrived;
   size_t bytes;
 };
 ForwardSpace forward_space(void* base, const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width, int64_t x_stride,
@@ -594,10 +582,11 @@ ForwardSpace forward_space(void* base, const void* x, const void* weight, int64_
   const bool is_few = few(rows, type);
   f.x = s.take(copy_bytes(x, rows, width, x_stride, type, false));
   f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32));
-  const int64_t parts = is_few ? few_symbols_of(rows, symbols, width).spans * 4 : stats_of(rows, symbols, width, type).units_n * 2;
+  const int64_t parts = is_few ? few_symbols_of(rows, symbols, width).spans : stats_of(rows, symbols, width, type).units_n * 2;
   f.stats = static_cast<float2*>(s.take(static_cast<size_t>(parts) * static_cast<size_t>(rows) * sizeof(float2)));
-  f.picked = static_cast<float*>(s.take(static_cast<size_t>(is_few ? 0 : rows) * sizeof(float)));
+  f.picked = static_cast<float*>(s.take(static_cast<size_t>(rows) * sizeof(float)));
   f.sums = static_cast<double2*>(s.take(static_cast<size_t>(parts_of(rows, 32)) * sizeof(double2)));
+  f.arrived = static_cast<int*>(s.take(sizeof(int)));
   f.bytes = s.used;
   return f;
 }
@@ -686,20 +675,25 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
   if (is_few) {
     FewParams p = few_symbols_of(rows, symbols, width);
     p.e.stats = space.stats;
+    p.e.picked = space.picked;
+    p.e.arrived = space.arrived;
+    p.e.target = target;
+    p.e.target_wide = target_bytes == 8;
+    p.e.symbols = symbols;
     p.e.status = status_dev;
+    p.x = x;
+    p.weight = weight;
+    p.x_stride = x_stride;
+    p.weight_stride = weight_stride;
+    p.width = static_cast<int>(width);
     rc = run_few<ENTROPY_STATS>(b, a, p, type, launch);
-    j.parts = p.spans * 4;
-    j.x = x;
-    j.weight = weight;
-    j.x_stride = x_stride;
-    j.weight_stride = weight_stride;
-    j.width = static_cast<int>(width);
-    j.type = type;
+    j.parts = p.spans;
   } else {
     EntropyParams p = stats_of(rows, symbols, width, type);
     if (!set_whole(p)) return TRITURUS_B200_EINVAL;
     p.stats = space.stats;
     p.picked = space.picked;
+    p.arrived = space.arrived;
     p.target = target;
     p.target_wide = target_bytes == 8;
     p.ignore = ignore_index;
@@ -707,11 +701,12 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
     p.status = status_dev;
     rc = run_products<ENTROPY_STATS>(a, b, p, type, launch);
     j.parts = p.units_n * 2;
-    j.picked = space.picked;
   }
   if (rc != TRITURUS_B200_OK) return rc;
 
   j.stats = space.stats;
+  j.picked = space.picked;
+  j.arrived = space.arrived;
   j.target = target;
   j.loss = loss;
   j.lse = lse;
@@ -722,10 +717,7 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
   j.target_wide = target_bytes == 8;
   j.reduction = reduction;
   const int blocks = static_cast<int>(parts_of(rows, 32));
-  rc = launch(entropy_join_kernel, blocks, 1024, 0, j);
-  if (rc == TRITURUS_B200_OK && reduction != TRITURUS_B200_REDUCTION_NONE && blocks > 1)
-    rc = launch(entropy_loss_kernel, 1, 256, 0, j, blocks);
-  return rc;
+  return launch(entropy_join_kernel, blocks, 1024, 0, j);
 }
 
 size_t triturus_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width,
@@ -758,7 +750,7 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
   int rc = prepare(&mx, x, rows, width, x_stride, type, false, space.x, launch);
   if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32, space.weight, launch);
   const int wide = target_bytes == 8;
-  if (rc == TRITURUS_B200_OK)
+  if (rc == TRITURUS_B200_OK && !is_few)
     rc = launch(entropy_factors_kernel, 1, 1024, 0, dloss, reduction == TRITURUS_B200_REDUCTION_NONE ? 1 : 0, target, wide, ignore_index,
                    static_cast<int>(rows), reduction == TRITURUS_B200_REDUCTION_MEAN ? 1 : 0, type == TRITURUS_B200_TYPE_F16 ? 1 : 0, space.factors);
   Matrix md = {};
@@ -788,6 +780,7 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
     if (is_few) {
       FewParams f = few_symbols_of(rows, piece, width);
       f.e = p;
+      f.mean = reduction == TRITURUS_B200_REDUCTION_MEAN;
       rc = run_few<ENTROPY_PROB>(mw, mx, f, type, launch);
     } else {
       rc = run_products<ENTROPY_PROB>(mx, mw, p, type, launch);
