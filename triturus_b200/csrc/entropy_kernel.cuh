@@ -65,6 +65,20 @@ struct EntropyCfg {
   static_assert(SMEM_BYTES <= 232448, "shared memory capacity");
 };
 
+// Quotients of numbers below 2^31 by one that the host knows, without the instructions of a division (four of which cost a tile 800 cycles).
+struct Divisor {
+  uint32_t d, mul, shift;
+  Divisor() = default;
+  explicit Divisor(int divisor) : d(static_cast<uint32_t>(divisor)), mul(0), shift(0) {
+    // with 2^shift >= d: floor((2^32 (2^shift - d)) / d) + 1
+    while ((1u << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+
 struct EntropyParams {
   int rows, cols;         // of the product
   int kblocks;              // of the contraction
@@ -75,6 +89,7 @@ struct EntropyParams {
   int whole;                // units that are one pair's
   int shared;               // and those behind them whose contraction is cut
   int splits, kb_split;     // into parts of so many k-blocks
+  Divisor by_group, by_rows, by_last, by_shared;  // a group's units, its row tiles, those of the last group; `shared`
   int b_row, b_k;         // where the piece begins in W: as rows of the product's columns, as contraction values
   uint32_t idesc;
   int half;               // 16-bit operands are float16 and not bfloat16
@@ -98,8 +113,8 @@ struct EntropyParams {
   int dest;               // of whole tiles
   void* out;              // rows of `out_pitch` elements
   int64_t out_pitch;
-  int out_vec;            // its rows are on boundaries of four elements,
-  int out_sectors;        // of 32 bytes
+  int out_vec;            // its rows are on boundaries of 16 bytes
+  int direct;             // of 32 bytes
   float* sum;             // [rows][sum_pitch], what earlier pieces gave
   int64_t sum_pitch;
   float* part;            // [shared][splits][256][tile_cols]
@@ -164,21 +179,16 @@ __device__ __forceinline__ int64_t entropy_target(const EntropyParams& p, int64_
 }
 
 // 32 bytes, a whole sector, as one access of a thread.
-struct Sector {
-  uint32_t w[8];
-};
-__device__ __forceinline__ void store_sector(void* to, const Sector& x) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x.w[0]), "r"(x.w[1]), "r"(x.w[2]), "r"(x.w[3]), "r"(x.w[4]),
-               "r"(x.w[5]), "r"(x.w[6]), "r"(x.w[7])
+__device__ __forceinline__ void store_sector(void* to, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+               "r"(w[6]), "r"(w[7])
                : "memory");
 }
-__device__ __forceinline__ Sector load_sector(const void* from) {
-  Sector x;
+__device__ __forceinline__ void load_sector(uint32_t (&w)[8], const void* from) {
   asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]), "=r"(x.w[4]), "=r"(x.w[5]), "=r"(x.w[6]), "=r"(x.w[7])
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                : "l"(from)
                : "memory");
-  return x;
 }
 
 // Two numbers as 16-bit ones.
@@ -275,10 +285,10 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const auto walk = [&](auto&& tile) {
     const auto unit = [&](int u, int k0, int k1, int part) {
       const int of_group = p.group * p.units_n;
-      const int g = u / of_group, r = u - g * of_group;
+      const int g = p.by_group(u), r = u - g * of_group;
       const int rows_here = min(p.group, p.tiles_m - g * p.group);
       Tile t;
-      t.un = r / rows_here;
+      t.un = rows_here == p.group ? p.by_rows(r) : p.by_last(r);
       t.tm = g * p.group + r - t.un * rows_here;
       t.k0 = k0;
       t.k1 = k1;
@@ -301,7 +311,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         if (v < 0) {
           if (!unit(u, 0, p.kblocks, -1)) return;
         } else {
-          const int ks = v / p.shared, s = v - ks * p.shared, k0 = ks * p.kb_split;
+          const int ks = p.by_shared(v), s = v - ks * p.shared, k0 = ks * p.kb_split;
           if (!unit(p.whole + s, k0, min(p.kblocks, k0 + p.kb_split), s * p.splits + ks)) return;
         }
       }
@@ -460,9 +470,41 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const bool rows_exist = t.tm * (2 * BM) + static_cast<int>(rank) * BM < p.rows;
       const int chunks = rows_exist ? max(0, min(CHUNKS, (t.n1 - col0 + 31) >> 5)) : 0;
 
+      // Results leave straight from registers, a sector of 32 bytes of its row to a thread: beside TMA and the MMAs there is no bandwidth of shared memory
+      // left (through it the planes of a WIDE tile took 11 600 cycles, of which the exponentials 2 800).  Only where the rows do not begin on sectors they go
+      // through a box in shared memory, in rows of 128 bytes.
+      // 16-bit results, two to a word: chunk c of this thread's row into its half of the box; with the second half (or the last chunk) the box to memory.
+      const auto box16 = [&](const uint32_t (&w)[16], int c, int c0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint4*>(box + lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        if ((c & 1) == 0 && c + 1 < chunks) return;
+        __syncwarp();
+        const int begin = c0 - (c & 1) * 32, end = min(c0 + 32, t.n1);
+        uint16_t* out = static_cast<uint16_t*>(p.out);
+        if (p.out_vec) {
+          const int cb = begin + (lane & 7) * 8;
+#pragma unroll 2
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            if (row0 + r < p.rows && cb < end)
+              *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + r) * p.out_pitch + cb) = *reinterpret_cast<const uint4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          }
+        } else {
+#pragma unroll 4
+          for (int i = 0; i < 64; ++i) {
+            const int r = i >> 1, at = (i & 1) * 32 + lane;
+            if (row0 + r < p.rows && begin + at < end)
+              out[static_cast<int64_t>(row0 + r) * p.out_pitch + begin + at] =
+                  *reinterpret_cast<const uint16_t*>(box + r * 128 + (((at >> 3) ^ (r & 7)) << 4) + (at & 7) * 2);
+          }
+        }
+        __syncwarp();
+      };
       // 32 columns of the product from column c0 on.  (One copy of this code, in a loop over the chunks: unrolled over them it is fetched as slowly
       // as it is long, 8 000 cycles for a chunk.)
-      const auto process = [&](float (&v)[32], int c0) {
+      const auto process = [&](float (&v)[32], int c) {
+        const int c0 = col0 + c * 32;
         if constexpr (MODE == ENTROPY_STATS) {
           if (c0 + 32 > t.n1) {
 #pragma unroll
@@ -497,43 +539,46 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
               if (ignored) v[e] = 0.f;  // (whatever its logits are)
             }
           }
-          // 64 bytes of the row, straight from registers: TMA and the MMAs leave no bandwidth of shared memory (through it a WIDE tile took 11 600 cycles,
-          // of which the exponentials 2 800).  Tiles have multiples of 32 columns here, and so has d.
+          // Tiles have multiples of 32 columns here, and so has d.
           uint16_t* to = p.d + static_cast<int64_t>(row) * p.d_pitch + c0;
 #pragma unroll 1
           for (int plane = 0; plane < Cfg::PLANES; ++plane, to += p.d_plane) {
-            Sector w[2];
+            uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               if constexpr (WIDE) {
-                w[e >> 3].w[e & 7] = plane_bits(v[2 * e], v[2 * e + 1]);
+                w[e] = plane_bits(v[2 * e], v[2 * e + 1]);
                 v[2 * e] = plane_rest(v[2 * e]);
                 v[2 * e + 1] = plane_rest(v[2 * e + 1]);
               } else {
-                w[e >> 3].w[e & 7] = pack16(v[2 * e], v[2 * e + 1], p.half);
+                w[e] = pack16(v[2 * e], v[2 * e + 1], p.half);
               }
             }
             if (valid) {
-              store_sector(to, w[0]);
-              store_sector(to + 16, w[1]);
+              store_sector(to, w);
+              store_sector(to + 16, w + 8);
             }
           }
         } else {
+          if (!WIDE && p.half) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] *= alpha;
-          const auto sector = [&](int j) {  // eight columns as they are
-            Sector w;
+            for (int e = 0; e < 32; ++e) v[e] *= alpha;
+          }
+          const auto as_bits = [&](int e) { return __float_as_uint(v[e]); };
+          const auto store_floats = [&](float* to) {  // scratch memory, whose rows are on sectors
+            if (!valid) return;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w.w[e] = __float_as_uint(v[8 * j + e]);
-            return w;
+            for (int j = 0; j < 4; ++j) {
+              if (c0 + 8 * j < t.n1) {
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = as_bits(8 * j + e);
+                store_sector(to + 8 * j, w);
+              }
+            }
           };
           if (t.part >= 0) {
-            float* to = p.part + (static_cast<int64_t>(t.part) * (2 * BM) + static_cast<int>(rank) * BM + q * 32 + lane) * p.tile_cols + (c0 - t.n0);
-            if (valid) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (c0 + 8 * j < t.n1) store_sector(to + 8 * j, sector(j));
-            }
+            store_floats(p.part + (static_cast<int64_t>(t.part) * (2 * BM) + static_cast<int>(rank) * BM + q * 32 + lane) * p.tile_cols + (c0 - t.n0));
             return;
           }
           if (p.dest != DEST_FINAL) {
@@ -542,60 +587,58 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 if (c0 + 8 * j < t.n1) {
-                  const Sector y = load_sector(sums + 8 * j);
+                  uint32_t y[8];
+                  load_sector(y, sums + 8 * j);
 #pragma unroll
-                  for (int e = 0; e < 8; ++e) v[8 * j + e] += __uint_as_float(y.w[e]);
+                  for (int e = 0; e < 8; ++e) v[8 * j + e] += __uint_as_float(y[e]);
                 }
               }
             }
             if (p.dest != DEST_FINAL_ADD) {
-              if (valid) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (c0 + 8 * j < t.n1) store_sector(sums + 8 * j, sector(j));
-              }
+              store_floats(sums);
               return;
             }
           }
-          if (p.out_sectors) {
-            constexpr int EACH = WIDE ? 8 : 16;  // columns of a sector
-            char* to = static_cast<char*>(p.out) + (static_cast<int64_t>(row) * p.out_pitch + c0) * (32 / EACH);
-            if (valid) {
+          if constexpr (WIDE) {
+            float* out = static_cast<float*>(p.out);
+            if (p.direct) {
+              store_floats(out + static_cast<int64_t>(row) * p.out_pitch + c0);
+              return;
+            }
 #pragma unroll
-              for (int j = 0; j < 32 / EACH; ++j) {
-                if (c0 + EACH * j >= t.n1) continue;
-                if constexpr (WIDE) {
-                  store_sector(to + 32 * j, sector(j));
-                } else {
-                  Sector w;
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) w.w[e] = pack16(v[16 * j + 2 * e], v[16 * j + 2 * e + 1], p.half);
-                  store_sector(to + 32 * j, w);
-                }
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            __syncwarp();
+            if (p.out_vec) {
+              const int cb = c0 + (lane & 7) * 4;
+#pragma unroll 2
+              for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3);
+                if (row0 + r < p.rows && cb < t.n1)
+                  *reinterpret_cast<float4*>(out + static_cast<int64_t>(row0 + r) * p.out_pitch + cb) =
+                      *reinterpret_cast<const float4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+              }
+            } else {
+#pragma unroll 4
+              for (int r = 0; r < 32; ++r) {
+                if (row0 + r < p.rows && c0 + lane < t.n1)
+                  out[static_cast<int64_t>(row0 + r) * p.out_pitch + c0 + lane] =
+                      *reinterpret_cast<const float*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
               }
             }
-            return;
-          }
-          // rows that do not begin on sectors: row by row through shared memory
+            __syncwarp();
+          } else {
+            uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          __syncwarp();
-          const int cb = c0 + (lane & 7) * 4;
-#pragma unroll 2
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
-            if (row0 + r >= p.rows || cb >= t.n1) continue;
-            const float4 x = *reinterpret_cast<const float4*>(box + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            if constexpr (WIDE) {
-              entropy_put<float>(p, row0 + r, cb, x, t.n1);
-            } else if (p.half) {
-              entropy_put<__half>(p, row0 + r, cb, x, t.n1);
+            for (int e = 0; e < 16; ++e) w[e] = pack16(v[2 * e], v[2 * e + 1], p.half);
+            if (p.direct) {
+              uint16_t* to = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(row) * p.out_pitch + c0;
+              if (valid && c0 < t.n1) store_sector(to, w);
+              if (valid && c0 + 16 < t.n1) store_sector(to + 16, w + 8);
             } else {
-              entropy_put<__nv_bfloat16>(p, row0 + r, cb, x, t.n1);
+              box16(w, c, c0);
             }
           }
-          __syncwarp();
         }
       };
 
@@ -637,7 +680,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             float v[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = c == 0 ? sum[0][e] : c == 1 ? sum[CHUNKS > 1 ? 1 : 0][e] : sum[CHUNKS > 2 ? 2 : 0][e];
-            process(v, col0 + c * 32);
+            process(v, c);
           }
         } else {
           tmem_ld_32x32(at, ld);
@@ -652,7 +695,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             } else {
               release();
             }
-            process(v, col0 + c * 32);
+            process(v, c);
           }
         }
       }

@@ -415,8 +415,13 @@ void set_units(EntropyParams& p, int64_t unit_cols, int64_t tile_cols) {
 // All units but the shared ones are whole; false where they are too many.
 bool set_whole(EntropyParams& p) {
   const int64_t units = static_cast<int64_t>(p.tiles_m) * p.units_n;
+  if (units > INT32_MAX || static_cast<int64_t>(p.group) * p.units_n > INT32_MAX) return false;
   p.whole = static_cast<int>(units - p.shared);
-  return units <= INT32_MAX;
+  p.by_group = Divisor(p.group * p.units_n);
+  p.by_rows = Divisor(p.group);
+  p.by_last = Divisor(p.tiles_m % p.group != 0 ? p.tiles_m % p.group : p.group);
+  p.by_shared = Divisor(std::max(p.shared, 1));
+  return true;
 }
 
 // STATS: spans of columns, of any length, so that the pairs have about the same to do: a number of them for each row tile that makes 1 to 16 units to a
@@ -759,7 +764,6 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
   md.pitch = plan.d_pitch;
   md.plane = rows * plan.d_pitch;
   md.planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
-  const int vec = width % 4 == 0;
   for (int64_t i = 0; i < plan.pieces && rc == TRITURUS_B200_OK; ++i) {
     const int64_t first = i * plan.piece, piece = i + 1 < plan.pieces ? plan.piece : plan.last;
     EntropyParams p = prob_of(rows, piece, width, type);
@@ -791,8 +795,8 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
       q.dest = dest;
       q.out = to;
       q.out_pitch = width;
-      q.out_vec = vec && aligned_to(to, 4 * size);
-      q.out_sectors = width * size % 32 == 0 && aligned_to(to, 32);
+      q.out_vec = width * size % 16 == 0 && aligned_to(to, 16);
+      q.direct = width * size % 32 == 0 && aligned_to(to, 32);
       q.sum = space.sum;
       q.sum_pitch = plan.sum_pitch;
       q.part = space.part;
