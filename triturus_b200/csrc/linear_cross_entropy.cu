@@ -282,15 +282,26 @@ struct Matrix {
   int planes;
   bool raw;
 };
-// Whether an operand is read where it lies: rows on 16-byte boundaries, and 32-bit elements only as they are.
-bool in_place(const void* data, int64_t rows, int64_t stride, int type, bool raw) {
-  if (type == TRITURUS_B200_TYPE_F32 && !raw) return false;
-  return aligned_to(data, 16) && (rows == 1 || (stride > 0 && stride * size_of(type) % 16 == 0 && stride < (1ll << 37)));
+// How the operands are read: 32-bit ones as planes but for W with few rows of x.  With many rows 16-bit operands whose rows are off 128-byte lines are
+// copied too: TMA fetches two lines for each row of a box (4096 x 50000 of width 1000: forward 497 -> 365 us and 31 us for the copy, gradients 1168 -> 915;
+// at 1024 rows the copy takes what it saves).
+constexpr int64_t kLines = 2048;
+struct Reading {
+  int type;
+  bool raw, lines;
+};
+Reading reading_of(int64_t rows, int type, bool weight);
+// Whether an operand is read where it lies: rows on 16-byte boundaries (or lines), and 32-bit elements only as they are.
+bool in_place(const void* data, int64_t rows, int64_t stride, const Reading& how) {
+  if (how.type == TRITURUS_B200_TYPE_F32 && !how.raw) return false;
+  const int64_t unit = how.lines ? 128 : 16;
+  return aligned_to(data, unit) && (rows == 1 || (stride > 0 && stride * size_of(how.type) % unit == 0 && stride < (1ll << 37)));
 }
-// Bytes of the copy of an operand that is not.
-size_t copy_bytes(const void* data, int64_t rows, int64_t width, int64_t stride, int type, bool raw) {
-  if (in_place(data, rows, stride, type, raw)) return 0;
-  return static_cast<size_t>(rows) * static_cast<size_t>(up_to(width, 8)) * (raw ? 4 : type == TRITURUS_B200_TYPE_F32 ? 6 : 2);
+// A copy's rows are on lines.
+int64_t copy_pitch(int64_t width, const Reading& how) { return up_to(width, how.raw ? 32 : 64); }
+size_t copy_bytes(const void* data, int64_t rows, int64_t width, int64_t stride, const Reading& how) {
+  if (in_place(data, rows, stride, how)) return 0;
+  return static_cast<size_t>(rows) * static_cast<size_t>(copy_pitch(width, how)) * (how.raw ? 4 : how.type == TRITURUS_B200_TYPE_F32 ? 6 : 2);
 }
 
 int make_map(CUtensorMap* map, const Matrix& m, int box_x, int box_y, int type) {
@@ -328,19 +339,21 @@ struct Launches {
 int copy_grid(int64_t items) { return static_cast<int>(std::min<int64_t>(parts_of(items, 256), static_cast<int64_t>(device_sms()) * 16)); }
 
 // The operand itself or, copied to `space`, one that TMA can read.
-int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t stride, int type, bool raw, void* space, Launches& launch) {
+int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t stride, const Reading& how, void* space, Launches& launch) {
+  const int type = how.type;
+  const bool raw = how.raw;
   m->rows = rows;
   m->width = width;
-  m->raw = raw;
+  m->raw = raw && type == TRITURUS_B200_TYPE_F32;
   m->planes = type == TRITURUS_B200_TYPE_F32 && !raw ? 3 : 1;
-  if (in_place(data, rows, stride, type, raw)) {
+  if (in_place(data, rows, stride, how)) {
     m->data = data;
     m->pitch = rows == 1 ? up_to(width, 8) : stride;
     m->plane = rows * m->pitch;
     return TRITURUS_B200_OK;
   }
   m->data = space;
-  m->pitch = up_to(width, 8);
+  m->pitch = copy_pitch(width, how);
   m->plane = rows * m->pitch;
   const int grid = copy_grid(rows * (m->pitch / 8));
   const auto run = [&](auto kern, auto t) {
@@ -493,6 +506,9 @@ size_t part_bytes(const EntropyParams& p) {
 
 // Up to this many rows: XXX
 bool few(int64_t rows, int type) { return rows <= (type == TRITURUS_B200_TYPE_F32 ? 128 : 64); }
+Reading reading_of(int64_t rows, int type, bool weight) {
+  return {type, type == TRITURUS_B200_TYPE_F32 && weight && few(rows, type), type != TRITURUS_B200_TYPE_F32 && rows >= kLines};
+}
 
 FewParams few_of(int64_t rows, int64_t length, int64_t k) {
   FewParams p = {};
@@ -585,8 +601,8 @@ ForwardSpace forward_space(void* base, const void* x, const void* weight, int64_
   Space s = {static_cast<char*>(base), 0};
   ForwardSpace f;
   const bool is_few = few(rows, type);
-  f.x = s.take(copy_bytes(x, rows, width, x_stride, type, false));
-  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32));
+  f.x = s.take(copy_bytes(x, rows, width, x_stride, reading_of(rows, type, false)));
+  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, reading_of(rows, type, true)));
   const int64_t parts = is_few ? few_symbols_of(rows, symbols, width).spans : stats_of(rows, symbols, width, type).units_n * 2;
   f.stats = static_cast<float2*>(s.take(static_cast<size_t>(parts) * static_cast<size_t>(rows) * sizeof(float2)));
   f.picked = static_cast<float*>(s.take(static_cast<size_t>(rows) * sizeof(float)));
@@ -622,8 +638,8 @@ BackwardSpace backward_space(void* base, const BackwardPlan& b, const void* x, c
   Space s = {static_cast<char*>(base), 0};
   BackwardSpace f;
   const bool is_few = few(rows, type);
-  f.x = s.take(copy_bytes(x, rows, width, x_stride, type, false));
-  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32));
+  f.x = s.take(copy_bytes(x, rows, width, x_stride, reading_of(rows, type, false)));
+  f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, reading_of(rows, type, true)));
   f.factors = static_cast<float*>(s.take(2 * sizeof(float)));
   f.d = static_cast<uint16_t*>(s.take(static_cast<size_t>(rows) * static_cast<size_t>(b.d_pitch) * 2 * (type == TRITURUS_B200_TYPE_F32 ? 3 : 1)));
   f.sum = static_cast<float*>(s.take(b.pieces > 1 ? static_cast<size_t>(rows) * static_cast<size_t>(b.sum_pitch) * sizeof(float) : 0));
@@ -673,8 +689,8 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
 
   Matrix a, b;
   const bool is_few = few(rows, type);
-  int rc = prepare(&a, x, rows, width, x_stride, type, false, space.x, launch);
-  if (rc == TRITURUS_B200_OK) rc = prepare(&b, weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32, space.weight, launch);
+  int rc = prepare(&a, x, rows, width, x_stride, reading_of(rows, type, false), space.x, launch);
+  if (rc == TRITURUS_B200_OK) rc = prepare(&b, weight, symbols, width, weight_stride, reading_of(rows, type, true), space.weight, launch);
   if (rc != TRITURUS_B200_OK) return rc;
   JoinArgs j = {};
   if (is_few) {
@@ -752,8 +768,8 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
   Launches launch = {st};
   Matrix mx, mw;
   const bool is_few = few(rows, type);
-  int rc = prepare(&mx, x, rows, width, x_stride, type, false, space.x, launch);
-  if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, type, is_few && type == TRITURUS_B200_TYPE_F32, space.weight, launch);
+  int rc = prepare(&mx, x, rows, width, x_stride, reading_of(rows, type, false), space.x, launch);
+  if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, reading_of(rows, type, true), space.weight, launch);
   const int wide = target_bytes == 8;
   if (rc == TRITURUS_B200_OK && !is_few)
     rc = launch(entropy_factors_kernel, 1, 1024, 0, dloss, reduction == TRITURUS_B200_REDUCTION_NONE ? 1 : 0, target, wide, ignore_index,
