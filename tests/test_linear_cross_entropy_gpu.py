@@ -150,7 +150,7 @@ def test_many_rows_and_few_symbols(kind):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)
-@pytest.mark.parametrize("n", [2, 15, 16, 17, 32, 33, 48, 49, 63, 64, 65, 96, 127, 128, 129])
+@pytest.mark.parametrize("n", [2, 15, 16, 17, 32, 33, 48, 49, 63, 64, 65, 96, 127, 128, 129, 191, 192, 193])
 def test_few_rows(n, kind):
     """On both sides of where rows of x become rows and no columns of the MMAs, and where another one begins."""
     for v, d, reduction in ((1003, 200, "mean"), (130, 513, "none"), (20_000, 72, "sum")):

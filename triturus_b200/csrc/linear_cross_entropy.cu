@@ -504,8 +504,10 @@ size_t part_bytes(const EntropyParams& p) {
 
 // ----------------------------------------------------------------------------- few rows
 
-// Up to this many rows: XXX
-bool few(int64_t rows, int type) { return rows <= (type == TRITURUS_B200_TYPE_F32 ? 128 : 64); }
+// Up to this many rows of x the exchanged forms are used.  Microseconds forwards / gradients, exchanged and not, of 50000 symbols of width 2048: bfloat16 64 rows
+// 47 / 143 and 47 / 149, 96 rows (two tiles of 64) 68 / 184 and 48 / 151; float32 64 rows 100 / 312 and 376 / 714, 192 rows 239 / 774 and
+// 406 / 885, 256 rows 356 / 1064 and 415 / 972.
+bool few(int64_t rows, int type) { return rows <= (type == TRITURUS_B200_TYPE_F32 ? 192 : 64); }
 Reading reading_of(int64_t rows, int type, bool weight) {
   return {type, type == TRITURUS_B200_TYPE_F32 && weight && few(rows, type), type != TRITURUS_B200_TYPE_F32 && rows >= kLines};
 }
