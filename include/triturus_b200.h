@@ -340,7 +340,7 @@ int triturus_b200_embedding(const void* tokens, int token_bytes, const void* wei
  * `symbols` rows of dy's type back to back, all of which are written.  The positions are sorted by symbol in the workspace (16-byte aligned, may
  * hold anything) and the rows added in 32 bits in an order that depends on the symbols alone.
  */
-size_t triturus_b200_embedding_backward_workspace_bytes(int64_t count, int64_t symbols, int64_t width);
+size_t triturus_b200_embedding_backward_workspace_bytes(int64_t count, int64_t symbols, int64_t width, int type);
 int triturus_b200_embedding_backward(const void* dy, const void* tokens, int token_bytes, void* dweight, int64_t count, int64_t symbols,
                                      int64_t width, int64_t dy_stride, int type, float scale, int64_t padding, void* workspace,
                                      size_t workspace_bytes, void* stream);

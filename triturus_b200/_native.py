@@ -196,7 +196,7 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_void_p,
     ]  # fmt: skip
     lib.triturus_b200_embedding_backward_workspace_bytes.restype = c_size_t
-    lib.triturus_b200_embedding_backward_workspace_bytes.argtypes = [c_int64] * 3
+    lib.triturus_b200_embedding_backward_workspace_bytes.argtypes = [*[c_int64] * 3, c_int]
     lib.triturus_b200_embedding_backward.restype = c_int
     lib.triturus_b200_embedding_backward.argtypes = [
         c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_float, c_int64, c_void_p, c_size_t, c_void_p,
@@ -970,7 +970,7 @@ def _embedding_backward_impl(dy: torch.Tensor, tokens: torch.Tensor, symbols: in
     tokens = tokens.contiguous()
     rows, stride = _rows(dy)
     with _on_device(dy.device) as idx:
-        nbytes = int(LIB.triturus_b200_embedding_backward_workspace_bytes(count, symbols, width))
+        nbytes = int(LIB.triturus_b200_embedding_backward_workspace_bytes(count, symbols, width, _TYPE_CODES[dy.dtype]))
         ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dy.device)
         rc = LIB.triturus_b200_embedding_backward(
             rows.data_ptr(), tokens.data_ptr(), tokens.element_size(), dweight.data_ptr(), count, symbols, width, stride,

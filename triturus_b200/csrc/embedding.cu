@@ -5,23 +5,29 @@
 // The lookup moves each row once, 16 bytes to a thread and four of them under way; bound by memory.
 //
 // The gradient adds rows of dy that belong to the same symbol.  Atomics would add them in any order, so the positions are sorted by
-// symbol first, with a stable radix sort of up to 9 bits a pass (two launches each: every block counts its digits; then it adds up
-// the blocks' counts before it and places its items, ranked by warp and by warps).  Then groups of threads walk runs of kTile or more sorted
+// symbol first, with a stable radix sort of up to 9 bits a pass: every block counts its digits, adds up the blocks' counts before it and places its
+// items, ranked by warp and by warps.  Up to kClusterSort positions that is one launch, whose first cluster of eight blocks sorts, with the counts in
+// each other's shared memory, while the others fill the table with zeros; beyond, two launches a pass.  Then groups of threads walk tiles of sorted
 // positions: a thread keeps its 16 bytes of columns as 32-bit sums and writes them where a symbol's run ends.  A run over a border of
 // two tiles is left in the workspace in parts, which a last launch adds in their order: frequent symbols are spread over many
 // blocks, and the same call gives the same result each time.  Bound by memory: dy read once, the table written once.
 #include <algorithm>
 
 #include "packs.cuh"
+#include "ptx.cuh"
 
 namespace tb200 {
 namespace {
 
-constexpr int kTile = 32;            // sorted positions of a group of threads, at least
-constexpr int kMostTiles = 8192;     // (more positions than these take longer tiles)
+constexpr int kLeastTile = 8;        // sorted positions of a group of threads
+constexpr int kMostTile = 128;
+constexpr int kMostTiles = 16384;    // (more positions than these take longer tiles)
+constexpr int kAhead = 8;            // rows of a group under way
 constexpr int kSortThreads = 1024;
 constexpr int kMostDigits = 512;
 constexpr int kMostSortBlocks = 128;
+constexpr int kSortCluster = 8;
+constexpr int kClusterSort = 1 << 16;  // positions
 constexpr int kGroup = 128;          // threads of a block that adds rows
 
 // A symbol of a list of 64- or 32-bit ones.
@@ -139,13 +145,66 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs
   for (int d = threadIdx.x; d < p.digits; d += kSortThreads) p.counts[static_cast<int>(blockIdx.x) * p.digits + d] = n[d];
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortArgs p) {
-  constexpr int W = kSortThreads / 32;
-  __shared__ int next[kMostDigits];            // where the block's next item of a digit goes
-  __shared__ uint16_t of_warp[W][kMostDigits];  // items of a digit in a warp, then in the warps before
-  __shared__ int sums[W];
+struct SortSpace {
+  int next[kMostDigits];                                  // where the block's next item of a digit goes
+  uint16_t of_warp[kSortThreads / 32][kMostDigits];       // items of a digit in a warp, then in the warps before
+  int sums[kSortThreads / 32];
+};
+
+// next[digit] for the items of lower digits in all blocks (`all`: of this thread's digit) and those of this digit in the blocks before.
+__device__ __forceinline__ void sort_begin(const SortArgs& p, SortSpace& sp, int all, int before) {
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
-  // the items of lower digits in all blocks, and of this digit in the blocks before
+  int upto = all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sp.sums[warp] = upto;
+  __syncthreads();
+  int lower = 0;
+  for (int w = 0; w < warp; ++w) lower += sp.sums[w];
+  if (tid < p.digits) sp.next[tid] = lower + upto - all + before;
+}
+// The block's items, a thread to an item, in their order.
+__device__ __forceinline__ void sort_place(const SortArgs& p, SortSpace& sp, int begin, int end) {
+  constexpr int W = kSortThreads / 32;
+  const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
+  for (int base = begin; base < end; base += kSortThreads) {
+    for (int i = lane; i < p.digits; i += 32) sp.of_warp[warp][i] = 0;
+    const int i = base + tid;
+    const bool valid = i < end;
+    const int key = valid ? key_at(p, i) : 0;
+    const int at = valid && p.at != nullptr ? p.at[i] : i;
+    const int digit = valid ? (key >> p.shift) & (p.digits - 1) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (valid && rank == 0) sp.of_warp[warp][digit] = static_cast<uint16_t>(__popc(same));
+    __syncthreads();
+    int total = 0;
+    if (tid < p.digits) {
+#pragma unroll 8
+      for (int w = 0; w < W; ++w) {
+        const int n = sp.of_warp[w][tid];
+        sp.of_warp[w][tid] = static_cast<uint16_t>(total);
+        total += n;
+      }
+    }
+    __syncthreads();
+    if (valid) {
+      const int to = sp.next[digit] + sp.of_warp[warp][digit] + rank;
+      p.keys_out[to] = key;
+      p.at_out[to] = at;
+    }
+    __syncthreads();
+    if (tid < p.digits) sp.next[tid] += total;
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortArgs p) {
+  __shared__ SortSpace sp;
+  const int tid = static_cast<int>(threadIdx.x);
   int before = 0, all = 0;
   if (tid < p.digits) {
     for (int b = 0; b < p.blocks; ++b) {
@@ -154,47 +213,56 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortArgs
       before += b < static_cast<int>(blockIdx.x) ? n : 0;
     }
   }
-  int upto = all;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) sums[warp] = upto;
+  sort_begin(p, sp, all, before);
   __syncthreads();
-  int lower = 0;
-  for (int w = 0; w < warp; ++w) lower += sums[w];
-  if (tid < p.digits) next[tid] = lower + upto - all + before;
-  const int begin = static_cast<int>(blockIdx.x) * p.per_block, end = min(p.count, begin + p.per_block);
-  for (int base = begin; base < end; base += kSortThreads) {
-    for (int i = tid; i < W * p.digits; i += kSortThreads) of_warp[i / p.digits][i % p.digits] = 0;
+  const int begin = static_cast<int>(blockIdx.x) * p.per_block;
+  sort_place(p, sp, begin, min(p.count, begin + p.per_block));
+}
+
+// All passes in one launch: the first cluster sorts, the others fill `bytes` of the table with zeros.  `keys` and `at`: two lists each.
+__global__ void __cluster_dims__(kSortCluster, 1, 1) __launch_bounds__(kSortThreads)
+sort_cluster_kernel(SortArgs p, int32_t* keys0, int32_t* keys1, int32_t* at0, int32_t* at1, int passes, int each, char* table, int64_t bytes) {
+  __shared__ SortSpace sp;
+  __shared__ int counts[kMostDigits];
+  const int tid = static_cast<int>(threadIdx.x);
+  pdl_launch_dependents();
+  if (blockIdx.x >= kSortCluster) {
+    const int64_t head = min(bytes, static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(table) & 15)) & 15)), body = (bytes - head) / 16;
+    uint4* to = reinterpret_cast<uint4*>(table + head);
+    const int64_t first = static_cast<int64_t>(blockIdx.x - kSortCluster) * kSortThreads + tid, step = static_cast<int64_t>(gridDim.x - kSortCluster) * kSortThreads;
+    for (int64_t i = first; i < body; i += step) to[i] = make_uint4(0, 0, 0, 0);
+    if (first < 32) {  // before and behind the vectors, two bytes at a time
+      uint16_t *a = reinterpret_cast<uint16_t*>(table), *b = reinterpret_cast<uint16_t*>(table + head + body * 16);
+      if (2 * first < head) a[first] = 0;
+      if (head + body * 16 + 2 * first < bytes) b[first] = 0;
+    }
+    return;
+  }
+  const int begin = min(p.count, static_cast<int>(blockIdx.x) * p.per_block), end = min(p.count, begin + p.per_block);
+  for (int pass = 0; pass < passes; ++pass) {
+    p.shift = pass * each;
+    p.keys_out = pass & 1 ? keys1 : keys0;
+    p.at_out = pass & 1 ? at1 : at0;
+    for (int d = tid; d < p.digits; d += kSortThreads) counts[d] = 0;
     __syncthreads();
-    const int i = base + tid;
-    const bool valid = i < end;
-    const int key = valid ? key_at(p, i) : 0;
-    const int at = valid && p.at != nullptr ? p.at[i] : i;
-    const int digit = valid ? (key >> p.shift) & (p.digits - 1) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    if (valid && rank == 0) of_warp[warp][digit] = static_cast<uint16_t>(__popc(same));
-    __syncthreads();
-    int total = 0;
+    for (int i = begin + tid; i < end; i += kSortThreads) atomicAdd(&counts[(key_at(p, i) >> p.shift) & (p.digits - 1)], 1);
+    cluster_sync_all();
+    int before = 0, all = 0;
     if (tid < p.digits) {
-#pragma unroll 8
-      for (int w = 0; w < W; ++w) {
-        const int n = of_warp[w][tid];
-        of_warp[w][tid] = static_cast<uint16_t>(total);
-        total += n;
+#pragma unroll
+      for (uint32_t b = 0; b < kSortCluster; ++b) {
+        int n;
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(n) : "r"(map_to_cta(smem_u32(&counts[tid]), b)) : "memory");
+        all += n;
+        before += b < blockIdx.x ? n : 0;
       }
     }
+    sort_begin(p, sp, all, before);
     __syncthreads();
-    if (valid) {
-      const int to = next[digit] + of_warp[warp][digit] + rank;
-      p.keys_out[to] = key;
-      p.at_out[to] = at;
-    }
-    __syncthreads();
-    if (tid < p.digits) next[tid] += total;
+    sort_place(p, sp, begin, end);
+    cluster_sync_all();  // (all have read each other's counts, and what they wrote is seen)
+    p.keys = p.keys_out;
+    p.at = p.at_out;
   }
 }
 
@@ -240,11 +308,13 @@ __device__ __forceinline__ uint4 load_columns(const SumArgs& p, int at, int c) {
 
 template <class T>
 __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) {
-  constexpr int N = Pack<T, 16>::N, AHEAD = 4;
+  constexpr int N = Pack<T, 16>::N;
   const int groups = kGroup / p.lanes;
   const int64_t tile = static_cast<int64_t>(blockIdx.x) * groups + threadIdx.x / p.lanes;
   const int c = (static_cast<int>(blockIdx.y) * p.lanes + (static_cast<int>(threadIdx.x) & (p.lanes - 1))) * N;
   const int64_t first = tile * p.tile;
+  pdl_launch_dependents();
+  pdl_wait();
   if (first >= p.count || c >= p.width) return;
   const int begin = static_cast<int>(first), end = static_cast<int>(min(first + p.tile, static_cast<int64_t>(p.count)));
   float* part = p.part + tile * 2 * p.width + c;
@@ -263,22 +333,33 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
       store_row<T>(p, run, c, acc);
     }
   };
-  for (int i = begin; i < end; i += AHEAD) {
-    int key[AHEAD];
-    uint4 row[AHEAD];
+  // (the symbols and positions of the next rows are fetched with the rows before them)
+  int key[kAhead], at[kAhead];
+  const auto fetch = [&](int i) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) key[u] = i + u < end ? p.keys[i + u] : p.symbols;
+    for (int u = 0; u < kAhead; ++u) {
+      key[u] = i + u < end ? p.keys[i + u] : p.symbols;
+      at[u] = i + u < end ? p.at[i + u] : 0;
+    }
+  };
+  fetch(begin);
+  for (int i = begin; i < end; i += kAhead) {
+    uint4 row[kAhead];
+    int now[kAhead];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      if (key[u] < p.symbols) row[u] = load_columns<T>(p, p.at[i + u], c);
-    if (key[0] >= p.symbols) break;  // (they are the last ones)
+    for (int u = 0; u < kAhead; ++u) {
+      now[u] = key[u];
+      if (key[u] < p.symbols) row[u] = load_columns<T>(p, at[u], c);
+    }
+    if (now[0] >= p.symbols) break;  // (they are the last ones)
+    fetch(i + kAhead);
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      if (key[u] >= p.symbols) break;
+    for (int u = 0; u < kAhead; ++u) {
+      if (now[u] >= p.symbols) break;
       const Pack<T, 16> r = *reinterpret_cast<const Pack<T, 16>*>(&row[u]);
-      if (key[u] != run) {
+      if (now[u] != run) {
         leave(false);
-        run = key[u];
+        run = now[u];
         head = i + u == begin && run == before;
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] = to_float(r.v[e]);
@@ -295,13 +376,29 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
 template <class T>
 __global__ void __launch_bounds__(kGroup) embedding_join_kernel(const SumArgs p) {
   constexpr int N = Pack<T, 16>::N;
+  __shared__ int ends;
+  pdl_launch_dependents();
+  pdl_wait();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tile;
   const int begin = static_cast<int>(first);
-  int64_t end = first + p.tile;
+  const int64_t end = first + p.tile;
   if (end >= p.count) return;
   const int run = p.keys[end - 1];
-  if (run >= p.symbols || p.keys[end] != run) return;                             // none goes on
-  if (begin > 0 && p.keys[begin] == run && p.keys[begin - 1] == run) return;      // it began before
+  if (run >= p.symbols || p.keys[end] != run) return;                         // none goes on
+  if (begin > 0 && p.keys[begin] == run && p.keys[begin - 1] == run) return;  // it began before
+  // how many tiles behind this one it reaches: a thread to a tile looks whether it goes on behind that
+  int tiles = 1;
+  for (int64_t base = end;; base += static_cast<int64_t>(kGroup) * p.tile) {
+    if (threadIdx.x == 0) ends = kGroup;
+    __syncthreads();
+    const int64_t next = base + (static_cast<int64_t>(threadIdx.x) + 1) * p.tile;  // where the tile behind that begins
+    if (next >= p.count || p.keys[next - 1] != run || p.keys[next] != run) atomicMin(&ends, static_cast<int>(threadIdx.x));
+    __syncthreads();
+    const int here = ends;
+    tiles += here;
+    if (here < kGroup) break;
+    __syncthreads();
+  }
   const int c = (static_cast<int>(blockIdx.y) * kGroup + static_cast<int>(threadIdx.x)) * N;
   if (c >= p.width) return;
   float acc[N];
@@ -309,13 +406,11 @@ __global__ void __launch_bounds__(kGroup) embedding_join_kernel(const SumArgs p)
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = c + e < p.width ? part[e] : 0.f;
   part += p.width;  // the first part of the next tile
-  for (;;) {
+#pragma unroll 4
+  for (int k = 0; k < tiles; ++k) {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (c + e < p.width) acc[e] += part[e];
-    part += 2 * p.width;
-    end += p.tile;
-    if (end >= p.count || p.keys[end - 1] != run || p.keys[end] != run) break;
+      if (c + e < p.width) acc[e] += part[static_cast<int64_t>(k) * 2 * p.width + e];
   }
   store_row<T>(p, run, c, acc);
 }
@@ -339,17 +434,22 @@ int lanes_for(int64_t n, int most) {
   while (l < most && l < n) l <<= 1;
   return l;
 }
-int tile_of(int64_t count) { return static_cast<int>(std::max<int64_t>(kTile, (count + kMostTiles - 1) / kMostTiles)); }
+// Sorted positions of a tile: some 12 blocks of threads to an SM, between latency (few long tiles) and the parts of runs over borders (many short ones).
+int tile_of(int64_t count, int64_t width, int size) {
+  const int64_t vectors = (width * size + 15) / 16;
+  const int64_t tile = count * vectors / (static_cast<int64_t>(kGroup) * 12 * device_sms());
+  return static_cast<int>(std::max<int64_t>(std::clamp<int64_t>(tile, kLeastTile, kMostTile), (count + kMostTiles - 1) / kMostTiles));
+}
 
 struct SumSpace {  // the workspace: keys and positions twice, the counts, the parts
   size_t list, counts, part, bytes;
 };
-SumSpace space_of(int64_t count, int64_t width) {
+SumSpace space_of(int64_t count, int64_t width, int size) {
   const auto up = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
   SumSpace s;
   s.list = up(static_cast<size_t>(count) * 4);
   s.counts = up(static_cast<size_t>(kMostSortBlocks) * kMostDigits * 4);
-  const int64_t tiles = (count + tile_of(count) - 1) / tile_of(count);
+  const int64_t tile = tile_of(count, width, size), tiles = (count + tile - 1) / tile;
   s.part = up(static_cast<size_t>(tiles) * 2 * static_cast<size_t>(width) * 4);
   s.bytes = 4 * s.list + s.counts + s.part;
   return s;
@@ -391,8 +491,8 @@ int triturus_b200_embedding(const void* tokens, int token_bytes, const void* wei
   });
 }
 
-size_t triturus_b200_embedding_backward_workspace_bytes(int64_t count, int64_t symbols, int64_t width) {
-  return sizes_ok(count, symbols, width, 0, 8) ? space_of(count, width).bytes : 0;
+size_t triturus_b200_embedding_backward_workspace_bytes(int64_t count, int64_t symbols, int64_t width, int type) {
+  return sizes_ok(count, symbols, width, type, 8) ? space_of(count, width, size_of(type)).bytes : 0;
 }
 
 int triturus_b200_embedding_backward(const void* dy, const void* tokens, int token_bytes, void* dweight, int64_t count, int64_t symbols,
@@ -402,16 +502,16 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   const int size = size_of(type);
   if (!aligned_to(dweight, size)) return TRITURUS_B200_EALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int rc = TRITURUS_B200_OK;
   if (count > 0) {
     if (dy == nullptr || tokens == nullptr || workspace == nullptr) return TRITURUS_B200_EINVAL;
     if (!aligned_to(dy, size) || !aligned_to(tokens, token_bytes) || !aligned_to(workspace, 16)) return TRITURUS_B200_EALIGN;
-    if (workspace_bytes < space_of(count, width).bytes) return TRITURUS_B200_EWORKSPACE;
+    if (workspace_bytes < space_of(count, width, size).bytes) return TRITURUS_B200_EWORKSPACE;
   }
-  rc = code_of(cudaMemsetAsync(dweight, 0, static_cast<size_t>(symbols) * static_cast<size_t>(width) * size, st));
-  if (rc != TRITURUS_B200_OK || count == 0) return rc;
+  const int64_t table = symbols * width * size;
+  int rc = TRITURUS_B200_OK;
+  if (count == 0) return code_of(cudaMemsetAsync(dweight, 0, static_cast<size_t>(table), st));
 
-  const SumSpace space = space_of(count, width);
+  const SumSpace space = space_of(count, width, size);
   char* ws = static_cast<char*>(workspace);
   const auto list = [&](int i) { return reinterpret_cast<int32_t*>(ws + i * space.list); };
   SortArgs s = {};
@@ -420,21 +520,33 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   s.padding = padding;
   s.counts = reinterpret_cast<int*>(ws + 4 * space.list);
   s.count = static_cast<int>(count);
-  s.per_block = static_cast<int>((count + static_cast<int64_t>(kMostSortBlocks) * kSortThreads - 1) / (static_cast<int64_t>(kMostSortBlocks) * kSortThreads)) * kSortThreads;
-  s.blocks = static_cast<int>((count + s.per_block - 1) / s.per_block);
   s.wide = token_bytes == 8;
   int bits = 1;
   while ((symbols >> bits) != 0) ++bits;  // (of 0 ... symbols)
   const int passes = (bits + 8) / 9, each = (bits + passes - 1) / passes;
   s.digits = 1 << each;
-  for (int pass = 0; pass < passes && rc == TRITURUS_B200_OK; ++pass) {
-    s.shift = pass * each;
-    s.keys_out = list(pass & 1);
-    s.at_out = list(2 + (pass & 1));
-    rc = launch_of(sort_count_kernel, dim3(static_cast<unsigned>(s.blocks)), kSortThreads, 0, st, nullptr, s);
-    if (rc == TRITURUS_B200_OK) rc = launch_of(sort_place_kernel, dim3(static_cast<unsigned>(s.blocks)), kSortThreads, 0, st, nullptr, s);
-    s.keys = s.keys_out;
-    s.at = s.at_out;
+  const auto per_block = [&](int64_t blocks) { return static_cast<int>((count + blocks * kSortThreads - 1) / (blocks * kSortThreads)) * kSortThreads; };
+  if (count <= kClusterSort) {
+    s.per_block = per_block(kSortCluster);
+    const int64_t fills = std::clamp<int64_t>(table / (16 * kSortThreads * 4), 1, 2 * device_sms() - kSortCluster);
+    const int64_t grid = (kSortCluster + fills + kSortCluster - 1) / kSortCluster * kSortCluster;
+    rc = launch_of(sort_cluster_kernel, dim3(static_cast<unsigned>(grid)), kSortThreads, 0, st, nullptr, s, list(0), list(1), list(2), list(3), passes, each,
+                   static_cast<char*>(dweight), table);
+    s.keys = list((passes - 1) & 1);
+    s.at = list(2 + ((passes - 1) & 1));
+  } else {
+    rc = code_of(cudaMemsetAsync(dweight, 0, static_cast<size_t>(table), st));
+    s.per_block = per_block(kMostSortBlocks);
+    s.blocks = static_cast<int>((count + s.per_block - 1) / s.per_block);
+    for (int pass = 0; pass < passes && rc == TRITURUS_B200_OK; ++pass) {
+      s.shift = pass * each;
+      s.keys_out = list(pass & 1);
+      s.at_out = list(2 + (pass & 1));
+      rc = launch_of(sort_count_kernel, dim3(static_cast<unsigned>(s.blocks)), kSortThreads, 0, st, nullptr, s);
+      if (rc == TRITURUS_B200_OK) rc = launch_of(sort_place_kernel, dim3(static_cast<unsigned>(s.blocks)), kSortThreads, 0, st, nullptr, s);
+      s.keys = s.keys_out;
+      s.at = s.at_out;
+    }
   }
   if (rc != TRITURUS_B200_OK) return rc;
 
@@ -451,7 +563,7 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   p.count = static_cast<int>(count);
   p.symbols = static_cast<int>(symbols);
   p.width = static_cast<int>(width);
-  p.tile = tile_of(count);
+  p.tile = tile_of(count, width, size);
   p.scale = scale;
   const int64_t vectors = (width * size + 15) / 16;
   p.lanes = lanes_for(vectors, kGroup);
@@ -460,9 +572,10 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   if (slabs > 65535) return TRITURUS_B200_EINVAL;
   return by_type(type, [&](auto t) {
     using T = decltype(t);
-    int code = launch_of(embedding_sum_kernel<T>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), slabs), kGroup, 0, st, nullptr, p);
+    const cudaLaunchAttribute dependent = dependent_launch();
+    int code = launch_of(embedding_sum_kernel<T>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), slabs), kGroup, 0, st, &dependent, p);
     if (code == TRITURUS_B200_OK && tiles > 1)
-      code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((vectors + kGroup - 1) / kGroup)), kGroup, 0, st, nullptr, p);
+      code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((vectors + kGroup - 1) / kGroup)), kGroup, 0, st, &dependent, p);
     return code;
   });
 }

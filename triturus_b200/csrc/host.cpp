@@ -454,7 +454,7 @@ PyObject* embedding_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
       !padding_arg(args[4], symbols, &padding))
     return none();
   const int64_t count = tokens->numel();
-  const size_t bytes = triturus_b200_embedding_backward_workspace_bytes(count, symbols, width);
+  const size_t bytes = triturus_b200_embedding_backward_workspace_bytes(count, symbols, width, type);
   if (bytes == 0) return none();  // (sizes that the library refuses)
   at::Tensor dweight = empty_on(*dy, {symbols, width}, dy->scalar_type());
   at::Tensor ws = empty_on(*dy, {static_cast<int64_t>(bytes)}, at::kByte);
