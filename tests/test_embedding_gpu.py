@@ -78,7 +78,7 @@ def test_matches_definition(count, symbols, width, kind):
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)
 def test_one_symbol_everywhere(kind):
     """A run over all tiles."""
-    for count in (32, 33, 64, 65, 700, 20_000):
+    for count in (32, 33, 64, 65, 700, 8192, 8193, 20_000, 65_537):
         tokens = torch.full((count,), 4, device="cuda")
         check_backward(rand(count, 72, kind=kind), tokens, 9)
         tokens[count // 2 :] = 8  # the last symbol, beside the mark of positions without a gradient

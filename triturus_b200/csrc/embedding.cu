@@ -7,7 +7,7 @@
 // The gradient adds rows of dy that belong to the same symbol.  Atomics would add them in any order, so the positions are sorted by
 // symbol first, with a stable radix sort of up to 9 bits a pass: every block counts its digits, adds up the blocks' counts before it and places its
 // items, ranked by warp and by warps.  Up to kClusterSort positions that is one launch, whose first cluster of eight blocks sorts, with the counts in
-// each other's shared memory, while the others fill the table with zeros; beyond, two launches a pass.  Then groups of threads walk tiles of sorted
+// each other's shared memory; beyond, two launches a pass.  Blocks beside those fill the table with zeros.  Then groups of threads walk tiles of sorted
 // positions: a thread keeps its 16 bytes of columns as 32-bit sums and writes them where a symbol's run ends.  A run over a border of
 // two tiles is left in the workspace in parts, which a last launch adds in their order: frequent symbols are spread over many
 // blocks, and the same call gives the same result each time.  Bound by memory: dy read once, the table written once.
@@ -21,13 +21,16 @@ namespace {
 
 constexpr int kLeastTile = 8;        // sorted positions of a group of threads
 constexpr int kMostTile = 128;
-constexpr int kMostTiles = 16384;    // (more positions than these take longer tiles)
+constexpr int kMostTiles = 4096;     // (more positions than these take longer tiles)
 constexpr int kAhead = 8;            // rows of a group under way
 constexpr int kSortThreads = 1024;
 constexpr int kMostDigits = 512;
 constexpr int kMostSortBlocks = 128;
 constexpr int kSortCluster = 8;
-constexpr int kClusterSort = 1 << 16;  // positions
+constexpr int kRounds = 4;             // items of a thread at a time
+constexpr int kClusterSort = 1 << 14;  // positions (16384: 17 us in one launch of 8 blocks, 65536: 47, and 35 in four launches of 64)
+// Bytes of the table that are filled beside a launch of the sort; what is left over by a launch of its own, which is faster (1 GB: 148 and 190 us).
+constexpr int64_t kFillBeside = 64 << 20, kFillCount = 16 << 20, kFillPlace = 48 << 20;
 constexpr int kGroup = 128;          // threads of a block that adds rows
 
 // A symbol of a list of 64- or 32-bit ones.
@@ -135,7 +138,26 @@ __device__ __forceinline__ int key_at(const SortArgs& p, int i) {
   return static_cast<int>(t < 0 || t >= p.symbols || t == p.padding ? p.symbols : t);
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs p) {
+// `bytes` of the table filled with zeros by blocks of kSortThreads, of which this is number `block` of `blocks`.
+__device__ __forceinline__ void fill_table(char* table, int64_t bytes, int block, int blocks) {
+  const int64_t head = min(bytes, static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(table) & 15)) & 15)), body = (bytes - head) / 16;
+  uint4* to = reinterpret_cast<uint4*>(table + head);
+  const int64_t first = static_cast<int64_t>(block) * kSortThreads + threadIdx.x, step = static_cast<int64_t>(blocks) * kSortThreads;
+  for (int64_t i = first; i < body; i += step) to[i] = make_uint4(0, 0, 0, 0);
+  if (first < 32) {  // before and behind the vectors, two bytes at a time
+    uint16_t *a = reinterpret_cast<uint16_t*>(table), *b = reinterpret_cast<uint16_t*>(table + head + body * 16);
+    if (2 * first < head) a[first] = 0;
+    if (head + body * 16 + 2 * first < bytes) b[first] = 0;
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs p, char* table, int64_t bytes) {
+  pdl_launch_dependents();
+  if (static_cast<int>(blockIdx.x) >= p.blocks) {
+    fill_table(table, bytes, static_cast<int>(blockIdx.x) - p.blocks, static_cast<int>(gridDim.x) - p.blocks);
+    return;
+  }
+  pdl_wait();
   __shared__ int n[kMostDigits];
   for (int d = threadIdx.x; d < p.digits; d += kSortThreads) n[d] = 0;
   __syncthreads();
@@ -166,21 +188,34 @@ __device__ __forceinline__ void sort_begin(const SortArgs& p, SortSpace& sp, int
   for (int w = 0; w < warp; ++w) lower += sp.sums[w];
   if (tid < p.digits) sp.next[tid] = lower + upto - all + before;
 }
-// The block's items, a thread to an item, in their order.
+// The block's items in their order, up to kRounds to a thread at a time: a warp has consecutive ones, 32 in each round.
 __device__ __forceinline__ void sort_place(const SortArgs& p, SortSpace& sp, int begin, int end) {
   constexpr int W = kSortThreads / 32;
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
-  for (int base = begin; base < end; base += kSortThreads) {
+  for (int base = begin; base < end; base += kRounds * kSortThreads) {
+    const int rounds = min(kRounds, (end - base + kSortThreads - 1) / kSortThreads), first = base + warp * rounds * 32 + lane;
+    int key[kRounds], at[kRounds], digit[kRounds], rank[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int i = first + r * 32;
+      const bool valid = r < rounds && i < end;
+      key[r] = valid ? key_at(p, i) : 0;
+      at[r] = valid && p.at != nullptr ? p.at[i] : i;
+      digit[r] = valid ? (key[r] >> p.shift) & (p.digits - 1) : -1;
+    }
     for (int i = lane; i < p.digits; i += 32) sp.of_warp[warp][i] = 0;
-    const int i = base + tid;
-    const bool valid = i < end;
-    const int key = valid ? key_at(p, i) : 0;
-    const int at = valid && p.at != nullptr ? p.at[i] : i;
-    const int digit = valid ? (key >> p.shift) & (p.digits - 1) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
-    const int rank = __popc(same & ((1u << lane) - 1));
     __syncwarp();
-    if (valid && rank == 0) sp.of_warp[warp][digit] = static_cast<uint16_t>(__popc(same));
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      if (r < rounds) {
+        const unsigned same = __match_any_sync(0xffffffffu, digit[r]);
+        const int before = __popc(same & ((1u << lane) - 1)), so_far = digit[r] >= 0 ? sp.of_warp[warp][digit[r]] : 0;
+        rank[r] = so_far + before;
+        __syncwarp();
+        if (digit[r] >= 0 && before == 0) sp.of_warp[warp][digit[r]] = static_cast<uint16_t>(so_far + __popc(same));
+        __syncwarp();
+      }
+    }
     __syncthreads();
     int total = 0;
     if (tid < p.digits) {
@@ -192,18 +227,27 @@ __device__ __forceinline__ void sort_place(const SortArgs& p, SortSpace& sp, int
       }
     }
     __syncthreads();
-    if (valid) {
-      const int to = sp.next[digit] + sp.of_warp[warp][digit] + rank;
-      p.keys_out[to] = key;
-      p.at_out[to] = at;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      if (digit[r] >= 0) {
+        const int to = sp.next[digit[r]] + sp.of_warp[warp][digit[r]] + rank[r];
+        p.keys_out[to] = key[r];
+        p.at_out[to] = at[r];
+      }
     }
     __syncthreads();
     if (tid < p.digits) sp.next[tid] += total;
   }
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortArgs p) {
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs p, char* table, int64_t bytes) {
   __shared__ SortSpace sp;
+  pdl_launch_dependents();
+  if (static_cast<int>(blockIdx.x) >= p.blocks) {
+    fill_table(table, bytes, static_cast<int>(blockIdx.x) - p.blocks, static_cast<int>(gridDim.x) - p.blocks);
+    return;
+  }
+  pdl_wait();
   const int tid = static_cast<int>(threadIdx.x);
   int before = 0, all = 0;
   if (tid < p.digits) {
@@ -227,15 +271,7 @@ sort_cluster_kernel(SortArgs p, int32_t* keys0, int32_t* keys1, int32_t* at0, in
   const int tid = static_cast<int>(threadIdx.x);
   pdl_launch_dependents();
   if (blockIdx.x >= kSortCluster) {
-    const int64_t head = min(bytes, static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(table) & 15)) & 15)), body = (bytes - head) / 16;
-    uint4* to = reinterpret_cast<uint4*>(table + head);
-    const int64_t first = static_cast<int64_t>(blockIdx.x - kSortCluster) * kSortThreads + tid, step = static_cast<int64_t>(gridDim.x - kSortCluster) * kSortThreads;
-    for (int64_t i = first; i < body; i += step) to[i] = make_uint4(0, 0, 0, 0);
-    if (first < 32) {  // before and behind the vectors, two bytes at a time
-      uint16_t *a = reinterpret_cast<uint16_t*>(table), *b = reinterpret_cast<uint16_t*>(table + head + body * 16);
-      if (2 * first < head) a[first] = 0;
-      if (head + body * 16 + 2 * first < bytes) b[first] = 0;
-    }
+    fill_table(table, bytes, static_cast<int>(blockIdx.x) - kSortCluster, static_cast<int>(gridDim.x) - kSortCluster);
     return;
   }
   const int begin = min(p.count, static_cast<int>(blockIdx.x) * p.per_block), end = min(p.count, begin + p.per_block);
@@ -273,8 +309,8 @@ struct SumArgs {
   const char *lo, *hi;  // its memory
   const int32_t *keys, *at;
   void* dweight;
-  float* part;  // [tiles][2][width]: of the run that began before the tile, and of the one that goes on behind it
-  int64_t stride;
+  float* part;  // [tiles][2][pitch]: of the run that began before the tile, and of the one that goes on behind it
+  int64_t stride, pitch;  // pitch: a multiple of eight
   int count, symbols, width, tile, lanes, slabs;
   float scale;
 };
@@ -317,7 +353,7 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
   pdl_wait();
   if (first >= p.count || c >= p.width) return;
   const int begin = static_cast<int>(first), end = static_cast<int>(min(first + p.tile, static_cast<int64_t>(p.count)));
-  float* part = p.part + tile * 2 * p.width + c;
+  float* part = p.part + tile * 2 * p.pitch + c;
   const int before = begin > 0 ? p.keys[begin - 1] : -1, behind = end < p.count ? p.keys[end] : -1;
   float acc[N];
   int run = -1;  // the symbol whose rows are in acc
@@ -325,10 +361,9 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
   const auto leave = [&](bool last) {
     if (run < 0) return;
     if (head || (last && run == behind)) {
-      float* to = part + (head ? 0 : p.width);
+      float4* to = reinterpret_cast<float4*>(part + (head ? 0 : p.pitch));
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (c + e < p.width) to[e] = acc[e];
+      for (int e = 0; e < N / 4; ++e) to[e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
     } else {
       store_row<T>(p, run, c, acc);
     }
@@ -401,16 +436,21 @@ __global__ void __launch_bounds__(kGroup) embedding_join_kernel(const SumArgs p)
   }
   const int c = (static_cast<int>(blockIdx.y) * kGroup + static_cast<int>(threadIdx.x)) * N;
   if (c >= p.width) return;
-  float acc[N];
-  const float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.width + p.width + c;
+  alignas(16) float acc[N];
+  const float4* part = reinterpret_cast<const float4*>(p.part + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.pitch + c);
 #pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] = c + e < p.width ? part[e] : 0.f;
-  part += p.width;  // the first part of the next tile
-#pragma unroll 4
+  for (int e = 0; e < N / 4; ++e) *reinterpret_cast<float4*>(acc + 4 * e) = part[e];
+  part += p.pitch / 4;  // the first part of the next tile
+#pragma unroll 8
   for (int k = 0; k < tiles; ++k) {
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (c + e < p.width) acc[e] += part[static_cast<int64_t>(k) * 2 * p.width + e];
+    for (int e = 0; e < N / 4; ++e) {
+      const float4 x = part[static_cast<int64_t>(k) * (p.pitch / 2) + e];
+      acc[4 * e] += x.x;
+      acc[4 * e + 1] += x.y;
+      acc[4 * e + 2] += x.z;
+      acc[4 * e + 3] += x.w;
+    }
   }
   store_row<T>(p, run, c, acc);
 }
@@ -450,7 +490,7 @@ SumSpace space_of(int64_t count, int64_t width, int size) {
   s.list = up(static_cast<size_t>(count) * 4);
   s.counts = up(static_cast<size_t>(kMostSortBlocks) * kMostDigits * 4);
   const int64_t tile = tile_of(count, width, size), tiles = (count + tile - 1) / tile;
-  s.part = up(static_cast<size_t>(tiles) * 2 * static_cast<size_t>(width) * 4);
+  s.part = up(static_cast<size_t>(tiles) * 2 * static_cast<size_t>((width + 7) / 8 * 8) * 4);
   s.bytes = 4 * s.list + s.counts + s.part;
   return s;
 }
@@ -527,23 +567,40 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   s.digits = 1 << each;
   const auto per_block = [&](int64_t blocks) { return static_cast<int>((count + blocks * kSortThreads - 1) / (blocks * kSortThreads)) * kSortThreads; };
   if (count <= kClusterSort) {
-    s.per_block = per_block(kSortCluster);
-    const int64_t fills = std::clamp<int64_t>(table / (16 * kSortThreads * 4), 1, 2 * device_sms() - kSortCluster);
-    const int64_t grid = (kSortCluster + fills + kSortCluster - 1) / kSortCluster * kSortCluster;
-    rc = launch_of(sort_cluster_kernel, dim3(static_cast<unsigned>(grid)), kSortThreads, 0, st, nullptr, s, list(0), list(1), list(2), list(3), passes, each,
-                   static_cast<char*>(dweight), table);
+    const int64_t beside = std::min(table, kFillBeside), rest = table - beside;
+    const int64_t fills = std::clamp<int64_t>(beside / (16 * kSortThreads * 4), 1, 2 * device_sms());
+    if (rest > 0) rc = code_of(cudaMemsetAsync(static_cast<char*>(dweight) + beside, 0, static_cast<size_t>(rest), st));
+    if (rc == TRITURUS_B200_OK) {
+      s.per_block = per_block(kSortCluster);
+      const int64_t grid = (kSortCluster + fills + kSortCluster - 1) / kSortCluster * kSortCluster;
+      rc = launch_of(sort_cluster_kernel, dim3(static_cast<unsigned>(grid)), kSortThreads, 0, st, nullptr, s, list(0), list(1), list(2), list(3), passes, each,
+                     static_cast<char*>(dweight), beside);
+    }
     s.keys = list((passes - 1) & 1);
     s.at = list(2 + ((passes - 1) & 1));
   } else {
-    rc = code_of(cudaMemsetAsync(dweight, 0, static_cast<size_t>(table), st));
     s.per_block = per_block(kMostSortBlocks);
     s.blocks = static_cast<int>((count + s.per_block - 1) / s.per_block);
+    const int64_t beside = std::min(table, passes * (kFillCount + kFillPlace));
+    if (table > beside) rc = code_of(cudaMemsetAsync(static_cast<char*>(dweight) + beside, 0, static_cast<size_t>(table - beside), st));
+    int64_t filled = 0;
+    bool first = true;
+    const cudaLaunchAttribute dependent = dependent_launch();
+    const auto run = [&](void (*kern)(SortArgs, char*, int64_t), int64_t most) {
+      const int64_t bytes = std::min(most, beside - filled);
+      const int64_t blocks = bytes == 0 ? 0 : std::clamp<int64_t>(bytes / (16 * kSortThreads * 4), 1, device_sms());
+      const int code = launch_of(kern, dim3(static_cast<unsigned>(s.blocks + blocks)), kSortThreads, 0, st, first ? nullptr : &dependent, s,
+                                 static_cast<char*>(dweight) + filled, bytes);
+      filled += bytes;
+      first = false;
+      return code;
+    };
     for (int pass = 0; pass < passes && rc == TRITURUS_B200_OK; ++pass) {
       s.shift = pass * each;
       s.keys_out = list(pass & 1);
       s.at_out = list(2 + (pass & 1));
-      rc = launch_of(sort_count_kernel, dim3(static_cast<unsigned>(s.blocks)), kSortThreads, 0, st, nullptr, s);
-      if (rc == TRITURUS_B200_OK) rc = launch_of(sort_place_kernel, dim3(static_cast<unsigned>(s.blocks)), kSortThreads, 0, st, nullptr, s);
+      rc = run(sort_count_kernel, kFillCount);
+      if (rc == TRITURUS_B200_OK) rc = run(sort_place_kernel, kFillPlace);
       s.keys = s.keys_out;
       s.at = s.at_out;
     }
@@ -560,6 +617,7 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   p.dweight = dweight;
   p.part = reinterpret_cast<float*>(ws + 4 * space.list + space.counts);
   p.stride = dy_stride;
+  p.pitch = (width + 7) / 8 * 8;
   p.count = static_cast<int>(count);
   p.symbols = static_cast<int>(symbols);
   p.width = static_cast<int>(width);
