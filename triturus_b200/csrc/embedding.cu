@@ -32,6 +32,7 @@ constexpr int kClusterSort = 1 << 14;  // positions (16384: 17 us in one launch 
 // Bytes of the table that are filled beside a launch of the sort; what is left over by a launch of its own, which is faster (1 GB: 148 and 190 us).
 constexpr int64_t kFillBeside = 64 << 20, kFillCount = 16 << 20, kFillPlace = 48 << 20;
 constexpr int kGroup = 128;          // threads of a block that adds rows
+constexpr int kJoins = 4;            // groups of them that add the parts of a run
 
 // A symbol of a list of 64- or 32-bit ones.
 __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_t i) {
@@ -309,25 +310,35 @@ struct SumArgs {
   const char *lo, *hi;  // its memory
   const int32_t *keys, *at;
   void* dweight;
-  float* part;  // [tiles][2][pitch]: of the run that began before the tile, and of the one that goes on behind it
+  float* part;  // [tiles][2][pitch], by slots: of the run that began before the tile, and of the one that goes on behind it
   int64_t stride, pitch;  // pitch: a multiple of eight
-  int count, symbols, width, tile, lanes, slabs;
+  int count, symbols, width, tile, lanes;
+  int slots;  // vectors of a row, and one more where rows are off 16-byte boundaries
+  int base;   // elements that the table's first is behind such a boundary
   float scale;
 };
 
+// A thread's columns of symbol key's row begin `slot` vectors behind the 16-byte boundary at or before the row (so that the row is written in whole vectors wherever it
+// lies): with the first of them before the row for the first thread of a row that is off one.
 template <class T>
-__device__ __forceinline__ void store_row(const SumArgs& p, int key, int c, const float* acc) {
+__device__ __forceinline__ int column_of(const SumArgs& p, int key, int slot) {
   constexpr int N = Pack<T, 16>::N;
+  return slot * N - ((p.base + key * p.width) & (N - 1));
+}
+template <class T>
+__device__ __forceinline__ void store_row(const SumArgs& p, int key, int slot, const float* acc) {
+  constexpr int N = Pack<T, 16>::N;
+  const int c = column_of<T>(p, key, slot);
   T* dst = static_cast<T*>(p.dweight) + static_cast<int64_t>(key) * p.width + c;
   Pack<T, 16> r;
 #pragma unroll
   for (int e = 0; e < N; ++e) r.v[e] = from_float<T>(acc[e] * p.scale);
-  if (c + N <= p.width && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+  if (c >= 0 && c + N <= p.width) {
     *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(&r);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (c + e < p.width) dst[e] = r.v[e];
+      if (c + e >= 0 && c + e < p.width) dst[e] = r.v[e];
   }
 }
 
@@ -335,10 +346,10 @@ template <class T>
 __device__ __forceinline__ uint4 load_columns(const SumArgs& p, int at, int c) {
   constexpr int N = Pack<T, 16>::N;
   const T* src = static_cast<const T*>(p.dy) + at * p.stride + c;
-  if (c + N <= p.width) return load_window<T>(src, p.lo, p.hi);
+  if (c >= 0 && c + N <= p.width) return load_window<T>(src, p.lo, p.hi);
   Pack<T, 16> r;
 #pragma unroll
-  for (int e = 0; e < N; ++e) r.v[e] = c + e < p.width ? src[e] : from_float<T>(0.f);
+  for (int e = 0; e < N; ++e) r.v[e] = c + e >= 0 && c + e < p.width ? src[e] : from_float<T>(0.f);
   return *reinterpret_cast<const uint4*>(&r);
 }
 
@@ -347,13 +358,13 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
   constexpr int N = Pack<T, 16>::N;
   const int groups = kGroup / p.lanes;
   const int64_t tile = static_cast<int64_t>(blockIdx.x) * groups + threadIdx.x / p.lanes;
-  const int c = (static_cast<int>(blockIdx.y) * p.lanes + (static_cast<int>(threadIdx.x) & (p.lanes - 1))) * N;
+  const int slot = static_cast<int>(blockIdx.y) * p.lanes + (static_cast<int>(threadIdx.x) & (p.lanes - 1));
   const int64_t first = tile * p.tile;
   pdl_launch_dependents();
   pdl_wait();
-  if (first >= p.count || c >= p.width) return;
+  if (first >= p.count || slot >= p.slots) return;
   const int begin = static_cast<int>(first), end = static_cast<int>(min(first + p.tile, static_cast<int64_t>(p.count)));
-  float* part = p.part + tile * 2 * p.pitch + c;
+  float* part = p.part + tile * 2 * p.pitch + slot * N;
   const int before = begin > 0 ? p.keys[begin - 1] : -1, behind = end < p.count ? p.keys[end] : -1;
   float acc[N];
   int run = -1;  // the symbol whose rows are in acc
@@ -365,7 +376,7 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
 #pragma unroll
       for (int e = 0; e < N / 4; ++e) to[e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
     } else {
-      store_row<T>(p, run, c, acc);
+      store_row<T>(p, run, slot, acc);
     }
   };
   // (the symbols and positions of the next rows are fetched with the rows before them)
@@ -384,7 +395,7 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       now[u] = key[u];
-      if (key[u] < p.symbols) row[u] = load_columns<T>(p, at[u], c);
+      if (key[u] < p.symbols) row[u] = load_columns<T>(p, at[u], column_of<T>(p, key[u], slot));
     }
     if (now[0] >= p.symbols) break;  // (they are the last ones)
     fetch(i + kAhead);
@@ -409,9 +420,10 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
 
 // Runs over the borders of tiles: the block of the tile in which one begins adds its parts.
 template <class T>
-__global__ void __launch_bounds__(kGroup) embedding_join_kernel(const SumArgs p) {
-  constexpr int N = Pack<T, 16>::N;
+__global__ void __launch_bounds__(kGroup * kJoins) embedding_join_kernel(const SumArgs p) {
+  constexpr int N = Pack<T, 16>::N, THREADS = kGroup * kJoins;
   __shared__ int ends;
+  __shared__ float sums[kJoins][N][kGroup];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * p.tile;
@@ -423,36 +435,51 @@ __global__ void __launch_bounds__(kGroup) embedding_join_kernel(const SumArgs p)
   if (begin > 0 && p.keys[begin] == run && p.keys[begin - 1] == run) return;  // it began before
   // how many tiles behind this one it reaches: a thread to a tile looks whether it goes on behind that
   int tiles = 1;
-  for (int64_t base = end;; base += static_cast<int64_t>(kGroup) * p.tile) {
-    if (threadIdx.x == 0) ends = kGroup;
+  for (int64_t base = end;; base += static_cast<int64_t>(THREADS) * p.tile) {
+    if (threadIdx.x == 0) ends = THREADS;
     __syncthreads();
     const int64_t next = base + (static_cast<int64_t>(threadIdx.x) + 1) * p.tile;  // where the tile behind that begins
     if (next >= p.count || p.keys[next - 1] != run || p.keys[next] != run) atomicMin(&ends, static_cast<int>(threadIdx.x));
     __syncthreads();
     const int here = ends;
     tiles += here;
-    if (here < kGroup) break;
+    if (here < THREADS) break;
     __syncthreads();
   }
-  const int c = (static_cast<int>(blockIdx.y) * kGroup + static_cast<int>(threadIdx.x)) * N;
-  if (c >= p.width) return;
-  alignas(16) float acc[N];
-  const float4* part = reinterpret_cast<const float4*>(p.part + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.pitch + c);
+  // each of the kJoins groups of threads has a quarter of the parts (the first one first of all the part of this tile)
+  const int group = static_cast<int>(threadIdx.x) / kGroup, lane = static_cast<int>(threadIdx.x) % kGroup;
+  const int slot = static_cast<int>(blockIdx.y) * kGroup + lane;
+  const bool mine = slot < p.slots;
+  alignas(16) float acc[N] = {};
+  const float4* part = reinterpret_cast<const float4*>(p.part + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.pitch + slot * N);
+  if (mine) {
+    const int each = (tiles + kJoins - 1) / kJoins, last = min(tiles, (group + 1) * each);
+    if (group == 0) {
 #pragma unroll
-  for (int e = 0; e < N / 4; ++e) *reinterpret_cast<float4*>(acc + 4 * e) = part[e];
-  part += p.pitch / 4;  // the first part of the next tile
+      for (int e = 0; e < N / 4; ++e) *reinterpret_cast<float4*>(acc + 4 * e) = part[e];
+    }
+    part += p.pitch / 4;  // the first part of the next tile
 #pragma unroll 8
-  for (int k = 0; k < tiles; ++k) {
+    for (int k = group * each; k < last; ++k) {
 #pragma unroll
-    for (int e = 0; e < N / 4; ++e) {
-      const float4 x = part[static_cast<int64_t>(k) * (p.pitch / 2) + e];
-      acc[4 * e] += x.x;
-      acc[4 * e + 1] += x.y;
-      acc[4 * e + 2] += x.z;
-      acc[4 * e + 3] += x.w;
+      for (int e = 0; e < N / 4; ++e) {
+        const float4 x = part[static_cast<int64_t>(k) * (p.pitch / 2) + e];
+        acc[4 * e] += x.x;
+        acc[4 * e + 1] += x.y;
+        acc[4 * e + 2] += x.z;
+        acc[4 * e + 3] += x.w;
+      }
     }
   }
-  store_row<T>(p, run, c, acc);
+#pragma unroll
+  for (int e = 0; e < N; ++e) sums[group][e][lane] = acc[e];
+  __syncthreads();
+  if (group != 0 || !mine) return;
+#pragma unroll
+  for (int g = 1; g < kJoins; ++g)
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] += sums[g][e][lane];
+  store_row<T>(p, run, slot, acc);
 }
 
 // ----------------------------------------------------------------------------- host
@@ -474,6 +501,9 @@ int lanes_for(int64_t n, int most) {
   while (l < most && l < n) l <<= 1;
   return l;
 }
+// Vectors of a row, and one more.
+int64_t slots_of(int64_t width, int size) { return (width * size + 15) / 16 + 1; }
+int64_t part_pitch(int64_t width, int size) { return slots_of(width, size) * (16 / size); }
 // Sorted positions of a tile: some 12 blocks of threads to an SM, between latency (few long tiles) and the parts of runs over borders (many short ones).
 int tile_of(int64_t count, int64_t width, int size) {
   const int64_t vectors = (width * size + 15) / 16;
@@ -490,7 +520,7 @@ SumSpace space_of(int64_t count, int64_t width, int size) {
   s.list = up(static_cast<size_t>(count) * 4);
   s.counts = up(static_cast<size_t>(kMostSortBlocks) * kMostDigits * 4);
   const int64_t tile = tile_of(count, width, size), tiles = (count + tile - 1) / tile;
-  s.part = up(static_cast<size_t>(tiles) * 2 * static_cast<size_t>((width + 7) / 8 * 8) * 4);
+  s.part = up(static_cast<size_t>(tiles) * 2 * static_cast<size_t>(part_pitch(width, size)) * 4);
   s.bytes = 4 * s.list + s.counts + s.part;
   return s;
 }
@@ -617,23 +647,26 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   p.dweight = dweight;
   p.part = reinterpret_cast<float*>(ws + 4 * space.list + space.counts);
   p.stride = dy_stride;
-  p.pitch = (width + 7) / 8 * 8;
+  p.pitch = part_pitch(width, size);
   p.count = static_cast<int>(count);
   p.symbols = static_cast<int>(symbols);
   p.width = static_cast<int>(width);
   p.tile = tile_of(count, width, size);
   p.scale = scale;
-  const int64_t vectors = (width * size + 15) / 16;
-  p.lanes = lanes_for(vectors, kGroup);
+  const bool off = width * size % 16 != 0 || !aligned_to(dweight, 16);
+  const int64_t vectors = slots_of(width, size);  // (room for one more than rows on boundaries have)
+  p.slots = static_cast<int>(off ? vectors : vectors - 1);
+  p.base = static_cast<int>(reinterpret_cast<uintptr_t>(dweight) % 16) / size;
+  p.lanes = lanes_for(p.slots, kGroup);
   const int64_t tiles = (count + p.tile - 1) / p.tile, groups = kGroup / p.lanes;
-  const unsigned slabs = static_cast<unsigned>((vectors + p.lanes - 1) / p.lanes);
+  const unsigned slabs = static_cast<unsigned>((p.slots + p.lanes - 1) / p.lanes);
   if (slabs > 65535) return TRITURUS_B200_EINVAL;
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     const cudaLaunchAttribute dependent = dependent_launch();
     int code = launch_of(embedding_sum_kernel<T>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), slabs), kGroup, 0, st, &dependent, p);
     if (code == TRITURUS_B200_OK && tiles > 1)
-      code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((vectors + kGroup - 1) / kGroup)), kGroup, 0, st, &dependent, p);
+      code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((p.slots + kGroup - 1) / kGroup)), kGroup * kJoins, 0, st, &dependent, p);
     return code;
   });
 }
