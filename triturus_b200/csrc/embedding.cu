@@ -22,7 +22,6 @@ namespace {
 constexpr int kLeastTile = 8;        // sorted positions of a group of threads
 constexpr int kMostTile = 128;
 constexpr int kMostTiles = 4096;     // (more positions than these take longer tiles)
-constexpr int kAhead = 8;            // rows of a group under way
 constexpr int kSortThreads = 1024;
 constexpr int kMostDigits = 512;
 constexpr int kMostSortBlocks = 128;
@@ -32,7 +31,7 @@ constexpr int kClusterSort = 1 << 14;  // positions (16384: 17 us in one launch 
 // Bytes of the table that are filled beside a launch of the sort; what is left over by a launch of its own, which is faster (1 GB: 148 and 190 us).
 constexpr int64_t kFillBeside = 64 << 20, kFillCount = 16 << 20, kFillPlace = 48 << 20;
 constexpr int kGroup = 128;          // threads of a block that adds rows
-constexpr int kJoins = 4;            // groups of them that add the parts of a run
+constexpr int kJoins = 2;            // groups of them that add the parts of a run
 
 // A symbol of a list of 64- or 32-bit ones.
 __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_t i) {
@@ -40,34 +39,48 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_
 }
 
 // 16 bytes from any multiple of an element's size: where they are not on a 16-byte boundary, two vectors around them.  [lo, hi) is the
-// tensor's memory, beyond which nothing is read.
-template <class T>
-__device__ __forceinline__ uint4 load_window(const T* p, const char* lo, const char* hi) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-  const int s = static_cast<int>(at & 15);
-  if (s == 0) return *reinterpret_cast<const uint4*>(p);
-  const char* g = reinterpret_cast<const char*>(p) - s;
-  if (g < lo || g + 32 > hi) {
-    Pack<T, 16> r;
-#pragma unroll
-    for (int e = 0; e < Pack<T, 16>::N; ++e) r.v[e] = p[e];
-    return *reinterpret_cast<const uint4*>(&r);
+// tensor's memory, beyond which nothing is read.  In two steps, for a thread that has several under way: what the first one loads is not looked at before the
+// second (with one after the other the sums of 5003 x 1537 float32 rows took 22 us for 11).
+template <class T, bool ALIGNED>
+struct Window {
+  uint4 a, b;
+  const T* p;
+  int s;  // bytes behind the boundary; -1: too near to an end of the memory
+  __device__ __forceinline__ void begin(const T* from, const char* lo, const char* hi) {
+    p = from;
+    if constexpr (ALIGNED) {
+      a = *reinterpret_cast<const uint4*>(from);
+    } else {
+      s = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15);
+      const char* g = reinterpret_cast<const char*>(from) - s;
+      if (s != 0 && (g < lo || g + 32 > hi)) s = -1;
+      if (s >= 0) a = *reinterpret_cast<const uint4*>(g);
+      if (s > 0) b = *reinterpret_cast<const uint4*>(g + 16);
+    }
   }
-  const uint4 a = *reinterpret_cast<const uint4*>(g), b = *reinterpret_cast<const uint4*>(g + 16);
-  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  if (s & 8) {
+  __device__ __forceinline__ uint4 end() const {
+    if constexpr (ALIGNED) return a;
+    if (s < 0) {
+      Pack<T, 16> r;
 #pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+      for (int e = 0; e < Pack<T, 16>::N; ++e) r.v[e] = p[e];
+      return *reinterpret_cast<const uint4*>(&r);
+    }
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (s & 8) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (s & 4) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const int bits = (s & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (s & 4) {
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-  }
-  const int bits = (s & 3) * 8;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
+};
 
 // ----------------------------------------------------------------------------- lookup
 
@@ -90,7 +103,7 @@ __device__ __forceinline__ uint4 scaled(uint4 bits, float scale) {
   return *reinterpret_cast<uint4*>(&p);
 }
 
-template <class T, bool SCALED>
+template <class T, bool SCALED, bool ALIGNED>
 __global__ void __launch_bounds__(256) embedding_kernel(const LookupArgs p) {
   constexpr int N = Pack<T, 16>::N;
   const int lane = static_cast<int>(threadIdx.x) & (p.lanes - 1);
@@ -106,13 +119,13 @@ __global__ void __launch_bounds__(256) embedding_kernel(const LookupArgs p) {
   const int head = min(p.width, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / sizeof(T)));
   const int body = (p.width - head) / N;
   for (int v = lane; v < body; v += 4 * p.lanes) {
-    uint4 r[4];
+    Window<T, ALIGNED> r[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (v + u * p.lanes < body) r[u] = load_window<T>(src + head + (v + u * p.lanes) * N, p.lo, p.hi);
+      if (v + u * p.lanes < body) r[u].begin(src + head + (v + u * p.lanes) * N, p.lo, p.hi);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (v + u * p.lanes < body) *reinterpret_cast<uint4*>(dst + head + (v + u * p.lanes) * N) = scaled<T, SCALED>(r[u], p.scale);
+      if (v + u * p.lanes < body) *reinterpret_cast<uint4*>(dst + head + (v + u * p.lanes) * N) = scaled<T, SCALED>(r[u].end(), p.scale);
   }
   const int rest = p.width - body * N;  // what lies before the first and behind the last vector
   for (int e = lane; e < rest; e += p.lanes) {
@@ -342,20 +355,29 @@ __device__ __forceinline__ void store_row(const SumArgs& p, int key, int slot, c
   }
 }
 
-template <class T>
-__device__ __forceinline__ uint4 load_columns(const SumArgs& p, int at, int c) {
-  constexpr int N = Pack<T, 16>::N;
-  const T* src = static_cast<const T*>(p.dy) + at * p.stride + c;
-  if (c >= 0 && c + N <= p.width) return load_window<T>(src, p.lo, p.hi);
-  Pack<T, 16> r;
+// A thread's columns of a row of dy, in two steps as above.
+template <class T, bool ALIGNED>
+struct Columns {
+  Window<T, ALIGNED> w;
+  int c;
+  __device__ __forceinline__ void begin(const SumArgs& p, int at, int column) {
+    c = column;
+    if (inside(p)) w.begin(static_cast<const T*>(p.dy) + at * p.stride + c, p.lo, p.hi);
+    w.p = static_cast<const T*>(p.dy) + at * p.stride + c;
+  }
+  __device__ __forceinline__ bool inside(const SumArgs& p) const { return ALIGNED || (c >= 0 && c + Pack<T, 16>::N <= p.width); }
+  __device__ __forceinline__ uint4 end(const SumArgs& p) const {
+    if (inside(p)) return w.end();
+    Pack<T, 16> r;
 #pragma unroll
-  for (int e = 0; e < N; ++e) r.v[e] = c + e >= 0 && c + e < p.width ? src[e] : from_float<T>(0.f);
-  return *reinterpret_cast<const uint4*>(&r);
-}
+    for (int e = 0; e < Pack<T, 16>::N; ++e) r.v[e] = c + e >= 0 && c + e < p.width ? w.p[e] : from_float<T>(0.f);
+    return *reinterpret_cast<const uint4*>(&r);
+  }
+};
 
-template <class T>
+template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) {
-  constexpr int N = Pack<T, 16>::N;
+  constexpr int N = Pack<T, 16>::N, kAhead = 4;  // rows of a thread under way (65536 x 4096 bfloat16, the whole step: 424 us, 8: 446, 16: 500)
   const int groups = kGroup / p.lanes;
   const int64_t tile = static_cast<int64_t>(blockIdx.x) * groups + threadIdx.x / p.lanes;
   const int slot = static_cast<int>(blockIdx.y) * p.lanes + (static_cast<int>(threadIdx.x) & (p.lanes - 1));
@@ -390,19 +412,20 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
   };
   fetch(begin);
   for (int i = begin; i < end; i += kAhead) {
-    uint4 row[kAhead];
+    Columns<T, ALIGNED> row[kAhead];
     int now[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       now[u] = key[u];
-      if (key[u] < p.symbols) row[u] = load_columns<T>(p, at[u], column_of<T>(p, key[u], slot));
+      if (key[u] < p.symbols) row[u].begin(p, at[u], ALIGNED ? slot * N : column_of<T>(p, key[u], slot));
     }
     if (now[0] >= p.symbols) break;  // (they are the last ones)
     fetch(i + kAhead);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (now[u] >= p.symbols) break;
-      const Pack<T, 16> r = *reinterpret_cast<const Pack<T, 16>*>(&row[u]);
+      const uint4 bits = row[u].end(p);
+      const Pack<T, 16> r = *reinterpret_cast<const Pack<T, 16>*>(&bits);
       if (now[u] != run) {
         leave(false);
         run = now[u];
@@ -446,14 +469,16 @@ __global__ void __launch_bounds__(kGroup * kJoins) embedding_join_kernel(const S
     if (here < THREADS) break;
     __syncthreads();
   }
-  // each of the kJoins groups of threads has a quarter of the parts (the first one first of all the part of this tile)
+  // each of the kJoins groups of threads has a share of the parts (the first one first of all the part of this tile); of few parts the first one all
   const int group = static_cast<int>(threadIdx.x) / kGroup, lane = static_cast<int>(threadIdx.x) % kGroup;
+  const bool alone = tiles < 4 * kJoins;
+  if (alone && group != 0) return;
   const int slot = static_cast<int>(blockIdx.y) * kGroup + lane;
   const bool mine = slot < p.slots;
   alignas(16) float acc[N] = {};
   const float4* part = reinterpret_cast<const float4*>(p.part + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.pitch + slot * N);
   if (mine) {
-    const int each = (tiles + kJoins - 1) / kJoins, last = min(tiles, (group + 1) * each);
+    const int each = alone ? tiles : (tiles + kJoins - 1) / kJoins, last = min(tiles, (group + 1) * each);
     if (group == 0) {
 #pragma unroll
       for (int e = 0; e < N / 4; ++e) *reinterpret_cast<float4*>(acc + 4 * e) = part[e];
@@ -471,15 +496,18 @@ __global__ void __launch_bounds__(kGroup * kJoins) embedding_join_kernel(const S
       }
     }
   }
+  if (!alone) {
 #pragma unroll
-  for (int e = 0; e < N; ++e) sums[group][e][lane] = acc[e];
-  __syncthreads();
-  if (group != 0 || !mine) return;
+    for (int e = 0; e < N; ++e) sums[group][e][lane] = acc[e];
+    __syncthreads();
+    if (group == 0) {
 #pragma unroll
-  for (int g = 1; g < kJoins; ++g)
+      for (int g = 1; g < kJoins; ++g)
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] += sums[g][e][lane];
-  store_row<T>(p, run, slot, acc);
+        for (int e = 0; e < N; ++e) acc[e] += sums[g][e][lane];
+    }
+  }
+  if (group == 0 && mine) store_row<T>(p, run, slot, acc);
 }
 
 // ----------------------------------------------------------------------------- host
@@ -557,7 +585,10 @@ int triturus_b200_embedding(const void* tokens, int token_bytes, const void* wei
   const dim3 grid(static_cast<unsigned>((count + rows - 1) / rows));
   return by_type(type, [&](auto t) {
     using T = decltype(t);
-    return launch_of(scale == 1.f ? embedding_kernel<T, false> : embedding_kernel<T, true>, grid, 256, 0, static_cast<cudaStream_t>(stream), nullptr, p);
+    const bool aligned = aligned_to(weight, 16) && aligned_to(y, 16) && width * size % 16 == 0 && weight_stride * size % 16 == 0;
+    const auto run = [&](auto kern) { return launch_of(kern, grid, 256, 0, static_cast<cudaStream_t>(stream), nullptr, p); };
+    if (scale == 1.f) return aligned ? run(embedding_kernel<T, false, true>) : run(embedding_kernel<T, false, false>);
+    return aligned ? run(embedding_kernel<T, true, true>) : run(embedding_kernel<T, true, false>);
   });
 }
 
@@ -664,7 +695,8 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     const cudaLaunchAttribute dependent = dependent_launch();
-    int code = launch_of(embedding_sum_kernel<T>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), slabs), kGroup, 0, st, &dependent, p);
+    const bool aligned = !off && aligned_to(dy, 16) && dy_stride * size % 16 == 0;
+    int code = launch_of(aligned ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), slabs), kGroup, 0, st, &dependent, p);
     if (code == TRITURUS_B200_OK && tiles > 1)
       code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((p.slots + kGroup - 1) / kGroup)), kGroup * kJoins, 0, st, &dependent, p);
     return code;
