@@ -1066,7 +1066,9 @@ def linear_cross_entropy_op(
     x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, reduction: int, ignore_index: int
 ) -> tuple[torch.Tensor, torch.Tensor]:
     from .cross_entropy import _check as check
+    from .cross_entropy import _check_code
 
+    _check_code(reduction)
     check(x, weight, target, ignore_index)
     return _linear_cross_entropy_impl(x, weight, target, reduction, ignore_index)
 
@@ -1076,8 +1078,9 @@ def linear_cross_entropy_backward_op(
     dloss: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, lse: torch.Tensor, reduction: int, ignore_index: int,
     x_grad: bool, weight_grad: bool,
 ) -> tuple[torch.Tensor, torch.Tensor]:  # fmt: skip
-    from .cross_entropy import _check_backward
+    from .cross_entropy import _check_backward, _check_code
 
+    _check_code(reduction)
     _check_backward(dloss, x, weight, target, lse, reduction, ignore_index)
     return _linear_cross_entropy_backward_impl(dloss, x, weight, target, lse, reduction, ignore_index, x_grad, weight_grad)
 
@@ -1085,14 +1088,17 @@ def linear_cross_entropy_backward_op(
 @linear_cross_entropy_op.register_fake
 def _linear_cross_entropy_fake(x, weight, target, reduction, ignore_index):
     from .cross_entropy import _check as check
+    from .cross_entropy import _check_code
 
+    _check_code(reduction)
     check(x, weight, target, ignore_index)
     return x.new_empty(target.shape if reduction == 0 else (), dtype=torch.float32), x.new_empty(target.shape, dtype=torch.float32)
 
 
 @linear_cross_entropy_backward_op.register_fake
 def _linear_cross_entropy_backward_fake(dloss, x, weight, target, lse, reduction, ignore_index, x_grad, weight_grad):
-    from .cross_entropy import _check_backward
+    from .cross_entropy import _check_backward, _check_code
 
+    _check_code(reduction)
     _check_backward(dloss, x, weight, target, lse, reduction, ignore_index)
     return x.new_empty(x.shape if x_grad else (0,)), weight.new_empty(weight.shape if weight_grad else (0,))

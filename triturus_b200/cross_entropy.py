@@ -18,6 +18,11 @@ def _reduction(name: str, reduction: str) -> int:
     return _REDUCTIONS.index(reduction)
 
 
+def _check_code(reduction: int) -> None:
+    if not 0 <= reduction < len(_REDUCTIONS):
+        raise ValueError(f"linear_cross_entropy: Unknown reduction code {reduction!r}")
+
+
 def _check_operands(name: str, x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int) -> None:
     assert len(x.shape) >= 1
     assert len(weight.shape) == 2 and weight.shape[1] == x.shape[-1]

@@ -22,6 +22,7 @@
 // accumulator of their own, which is added to sums in registers, and tiles are 192 columns, whose sums are 96 registers of a thread.
 #pragma once
 
+#include "divisor.cuh"
 #include "packs.cuh"
 #include "ptx.cuh"
 
@@ -63,20 +64,6 @@ struct EntropyCfg {
   static constexpr int NBAR = 2 * NS + 4;
   static constexpr int SMEM_BYTES = 1024 + NS * STAGE + EPI_WARPS * BOX + NBAR * 8 + 16;
   static_assert(SMEM_BYTES <= 232448, "shared memory capacity");
-};
-
-// Quotients of numbers below 2^31 by one that the host knows, without the instructions of a division (four of which cost a tile 800 cycles).
-struct Divisor {
-  uint32_t d, mul, shift;
-  Divisor() = default;
-  explicit Divisor(int divisor) : d(static_cast<uint32_t>(divisor)), mul(0), shift(0) {
-    // with 2^shift >= d: floor((2^32 (2^shift - d)) / d) + 1
-    while ((1u << shift) < d) ++shift;
-    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  __device__ __forceinline__ int operator()(int n) const {
-    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
-  }
 };
 
 struct EntropyParams {
