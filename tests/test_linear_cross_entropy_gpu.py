@@ -1,13 +1,13 @@
 """GPU: linear_cross_entropy and its gradients against their formulas in float64, elementwise.
 
 Bounds.  u = 2^-24.  S = sum_d |x_d w_d|.
-Logits, 16-bit operands: products are exact; each MMA adds 16 of them and cuts off below a unit of the last place, 2 u of at most S:
-E_z = (D / 16 + 8) 2 u S.  float32: what the six products of parts leave out is below 2^-22.9 = 2.2 u of each product, the MMAs of the first
+Logits, 16-bit operands: products are exact; each MMA adds 16 of them and cuts off below a unit of the last place, 2 u of at most S, for up to 512 terms, which
+are then added up with a rounding: E_z = (min(D / 16, 32) + 8) 2 u S + D / 512 u S.  float32: what the six products of parts leave out is below 2^-22.9 = 2.2 u of each product, the MMAs of the first
 parts of 32 or 64 terms are cut off (2 u each, up to four), those of the others by 2^-8 of that, and the sums of D / 32 of them rounded: E_z = (16 + D / 32) u S.
 lse: max E_z, the exponentials (2^-22 each), their arguments (4 u of the numbers, as far as those count), and some 320 additions in a row: E_lse = max E_z + 2^-15 + 4 u |lse|.
 loss: E_lse + E_z of the target, and u of both for the difference.
 d = g (p - [target]): p is off by exp(E_z + E_lse + 2^-21) - 1 at most, and d is rounded by half a step h of its type (2^-8, 2^-11; float32: 2 u, cut off), in float16 at
-least by 2^-25 2^-15 of the largest g.  A p below 2^-126, the least normal number, is 0, and so are parts of d below 2^-133, the least bfloat16: 2^-126 |g| + 2^-132.  Its products: as for the logits, with K terms and their own S = sum |d| |w|, summed again for each piece.
+least by 2^-25 2^-15 of the largest g.  A p below 2^-126, the least normal number, is 0, and so are parts of d below 2^-133, the least bfloat16: 2^-126 |g| + 2^-132.  Its products: as for the logits, with K terms and their own S = sum |d| |w|, 16384 of 16 bits in an accumulator, summed again for each piece.
 The result is rounded by half a step of its type: to infinity from the largest number and half a step of it on (in float16 65520, of the bfloat16 and
 float32 numbers here none comes near)."""
 
@@ -29,8 +29,8 @@ LARGEST = {k: torch.finfo(k).max * (1 + torch.finfo(k).eps / 4) for k in KINDS}
 IGNORE = -100
 
 
-def product_error(kind, terms):
-    return (16 + terms / 32) * U if kind == torch.float32 else (terms / 16 + 8) * 2 * U
+def product_error(kind, terms, together=16_384):
+    return (16 + terms / 32) * U if kind == torch.float32 else (min(terms, together) / 16 + 8) * 2 * U + terms / together * U
 
 
 def expected(x, weight, target, dloss, reduction, ignore=IGNORE):
@@ -41,7 +41,7 @@ def expected(x, weight, target, dloss, reduction, ignore=IGNORE):
     given = t != ignore
     n = len(t)
     z = x @ w.t()
-    ez = product_error(kind, D) * (x.abs() @ w.abs().t())
+    ez = product_error(kind, D, 512) * (x.abs() @ w.abs().t())
     lse = torch.logsumexp(z, -1)
     elo = ez.amax(-1) + 2.0**-15 + 4 * U * lse.abs()
     at = torch.where(given, t, 0)[:, None]

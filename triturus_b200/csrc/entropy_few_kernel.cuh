@@ -160,6 +160,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
   tc_fence_after_sync();
   const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
+  const int drain = WIDE ? 1 : p.e.drain;  // k-blocks of an accumulator
   struct Tile {
     int span, ks;      // which span and which part of the contraction
     int n0;            // first row of x
@@ -229,9 +230,12 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     const uint64_t db0 = umma_desc_k_sw128(smem_u32(b_base));
     uint32_t it = 0, accs = 0;
     walk([&](const Tile& t) {
+      int sum_end = t.k0;  // of the k-blocks of this accumulator
       for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
         const uint32_t sa = it % NSA, sb = it % NSB, buf = accs & 1, d = tmem_base + buf * BN;
-        if (WIDE || kb == t.k0) {
+        const bool begin = kb == sum_end;
+        if (begin) {
+          sum_end = min(kb + drain, t.k1);
           if (!mbar_wait_warp(&acc_empty[buf], ((accs >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
         }
         if (!mbar_wait_warp(&b_full[sb], (it / NSB) & 1, ctl, STATUS_TIMEOUT_MMA)) return false;
@@ -241,7 +245,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           if (!mbar_wait_warp(&a_full[sa], (it / NSA) & 1, ctl, STATUS_TIMEOUT_MMA)) return false;
         }
         tc_fence_after_sync();
-        const bool done = WIDE || kb + 1 == t.k1;
+        const bool done = kb + 1 == sum_end;
         if (elect_one_sync()) {
           const uint64_t db = db0 + sb * (Cfg::B_TILE >> 4);
           if constexpr (WIDE) {
@@ -256,7 +260,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           } else {
             const uint64_t da = da0 + sa * (Cfg::A_TILE >> 4);
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) umma_16_ss(d, da + (Cfg::A_MN ? 128 : 2) * k, db + 2 * k, p.idesc, kb > t.k0 || k > 0 ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) umma_16_ss(d, da + (Cfg::A_MN ? 128 : 2) * k, db + 2 * k, p.idesc, !begin || k > 0 ? 1u : 0u);
             umma_commit(&a_empty[sa]);
           }
           umma_commit(&b_empty[sb]);
@@ -339,7 +343,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           __syncwarp();
         }
       }
-      for (int kb = WIDE ? t.k0 : t.k1 - 1; kb < t.k1; ++kb, ++accs) {
+      for (int kb = t.k0; kb < t.k1; kb += drain, ++accs) {
         const uint32_t buf = accs & 1;
         if (!mbar_wait_warp(&acc_full[buf], (accs >> 1) & 1, ctl, STATUS_TIMEOUT_EPILOGUE)) return false;
         tc_fence_after_sync();
@@ -347,7 +351,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           uint32_t ld[32];
           tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN + h * 32, ld);
           tmem_ld_wait();
-          if (!WIDE || kb == t.k0) {
+          if (kb == t.k0) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) sum[e] = __uint_as_float(ld[e]);
           } else {

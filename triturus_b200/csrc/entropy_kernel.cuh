@@ -19,7 +19,8 @@
 // smallest first, leave out what is below 2^-24 of a product of two numbers.  Each plane of 64 contraction values is a stage of its own, and is used for
 // 8 or 12 MMAs.  (TMA takes some 2.5 cycles for each row of a box, of 64 bytes or 128: rows of 64 took longer than their MMAs.)  The tensor core cuts
 // off what does not fit its accumulator, half a unit of the last place for each of many additions; so each 64 contraction values have an
-// accumulator of their own, which is added to sums in registers, and tiles are 192 columns, whose sums are 96 registers of a thread.
+// accumulator of their own, which is added to sums in registers, and tiles are 192 columns, whose sums are 96 registers of a thread.  The logits of 16-bit operands
+// are added up like that too, every `drain` k-blocks (8192 values in one accumulator: off by 1e-3 where float32 is by 1e-5).
 #pragma once
 
 #include "divisor.cuh"
@@ -79,6 +80,7 @@ struct EntropyParams {
   Divisor by_group, by_rows, by_last, by_shared;  // a group's units, its row tiles, those of the last group; `shared`
   int b_row, b_k;         // where the piece begins in W: as rows of the product's columns, as contraction values
   uint32_t idesc;
+  int drain;              // k-blocks of an accumulator, where not WIDE
   int half;               // 16-bit operands are float16 and not bfloat16
   // STATS: [units_n * 2][rows] of maximum and sum, and the logits of the rows' own symbols
   float2* stats;
@@ -307,126 +309,136 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         if (!unit(u, 0, p.kblocks, -1)) return;
     }
   };
-  if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer (this CTA's halves)
-    // (Here and in the issuer the whole warp runs the loop and one elected lane issues: control flow and addresses are uniform and stay in
-    // uniform registers.  One lane in a branch of its own took some 600 cycles for a stage whose MMAs take 512, or 256 where WIDE.)
-    uint32_t it = 0;
-    bool ok = true;
-    walk([&](const Tile& t) {
-      const int a0 = t.tm * (2 * BM) + static_cast<int>(rank) * BM;
-      const int b0 = p.b_row + t.n0 + static_cast<int>(rank) * (t.mma >> 1);
-      for (int kb = t.k0; kb < t.k1; ++kb) {
-        const int ka = kb * BK, kw = p.b_k + kb * BK;
-#pragma unroll
-        for (int i = 0; i < Cfg::PLANES; ++i, ++it) {
-          const int plane = WIDE ? (i + 2) % 3 : 0;  // 2, 0, 1
-          const uint32_t s = it % NS;
-          if (!(ok = mbar_wait_warp(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
-          if (elect_one_sync()) {
-            if (leader) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE);
-            const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
-            uint8_t* a = smem + s * Cfg::STAGE;
-            uint8_t* b = a + Cfg::A_TILE;
-            if constexpr (Cfg::A_MN) {
-#pragma unroll
-              for (int g = 0; g < BM / 64; ++g) tma_load_3d_pair(a + g * Cfg::MN_BOX, &tmap_a, bar, a0 + g * 64, ka, plane);
-            } else {
-              tma_load_3d_pair(a, &tmap_a, bar, ka, a0, plane);
-            }
-            if constexpr (Cfg::B_MN) {
-#pragma unroll
-              for (int g = 0; g < Cfg::B_BOXES; ++g) tma_load_3d_pair(b + g * Cfg::MN_BOX, &tmap_b, bar, b0 + g * 64, kw, plane);
-            } else {
-              tma_load_3d_pair(b, &tmap_b, bar, kw, b0, plane);
-            }
-          }
-          __syncwarp();
-        }
-      }
-      return true;
-    });
-    // The leader's commits arrive on both CTAs' stage_empty barriers: this CTA stays until the last ones are in.
-    for (uint32_t d = ok ? min(it, static_cast<uint32_t>(NS)) : 0u; ok && d > 0; --d)
-      ok = mbar_wait_warp(&stage_empty[(it - d) % NS], ((it - d) / NS) & 1, ctl, STATUS_TIMEOUT_PRODUCER);
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer (leader only)
-    if (leader) {
-      constexpr uint32_t STAGE_ENC = Cfg::STAGE >> 4;
-      constexpr uint32_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;  // 16 contraction values
-      const uint32_t a_at = smem_u32(smem), b_at = a_at + Cfg::A_TILE;
-      const uint64_t da0 = Cfg::A_MN ? umma_desc_mn16_sw128(a_at, Cfg::MN_BOX) : umma_desc_k_sw128(a_at);
-      const uint64_t db0 = Cfg::B_MN ? umma_desc_mn16_sw128(b_at, Cfg::MN_BOX) : umma_desc_k_sw128(b_at);
-      uint32_t s = 0, ph = 0, accs = 0;
-      const auto advance = [&] {
-        if (++s == NS) {
-          s = 0;
-          ph ^= 1;
-        }
-      };
-      // rows of stage sa by columns of stage sb
-      const auto multiply = [&](uint32_t d, uint32_t idesc, uint32_t sa, uint32_t sb, bool add) {
-        const uint64_t da = da0 + sa * STAGE_ENC, db = db0 + sb * STAGE_ENC;
-#pragma unroll
-        for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, da + a_step * k, db + b_step * k, idesc, add || k > 0 ? 1u : 0u);
-      };
-      const auto free_stage = [&](uint32_t stage) { umma_commit_pair_mcast(smem_u32(&stage_empty[stage]), 3); };
+  const int drain = WIDE ? 1 : p.drain;  // k-blocks of an accumulator
+  // The sums of a 256-column tile take 128 registers of a thread: the warps that copy and multiply hand theirs over.  (All that the block was launched
+  // with, which launch_products makes sure of: 128 x 72 + 256 x 216 = 384 x 168.)
+  if (warp < 4) {
+    if constexpr (!WIDE) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ------------------------------------------------------------------ TMA producer (this CTA's halves)
+      // (Here and in the issuer the whole warp runs the loop and one elected lane issues: control flow and addresses are uniform and stay in
+      // uniform registers.  One lane in a branch of its own took some 600 cycles for a stage whose MMAs take 512, or 256 where WIDE.)
+      uint32_t it = 0;
+      bool ok = true;
       walk([&](const Tile& t) {
-        const uint32_t idesc = p.idesc | static_cast<uint32_t>(t.mma >> 3) << 17;
+        const int a0 = t.tm * (2 * BM) + static_cast<int>(rank) * BM;
+        const int b0 = p.b_row + t.n0 + static_cast<int>(rank) * (t.mma >> 1);
         for (int kb = t.k0; kb < t.k1; ++kb) {
-          const uint32_t buf = accs & 1, d = tmem_base + buf * Cfg::BUF_COLS;
-          if (WIDE || kb == t.k0) {
-            if (!mbar_wait_warp(&acc_empty[buf], ((accs >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
-          }
-          if (!mbar_wait_warp(&full[s], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
-          const bool done = WIDE || kb + 1 == t.k1;
-          if constexpr (WIDE) {
-            // planes 2, 0 and 1 in three stages (of six: the three have the same parity of the wait); the first is free again after a third of the MMAs
-            const uint32_t s2 = s, s0 = s + 1, s1 = s + 2;
-            if (!mbar_wait_warp(&full[s0], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
-            tc_fence_after_sync();
+          const int ka = kb * BK, kw = p.b_k + kb * BK;
+#pragma unroll
+          for (int i = 0; i < Cfg::PLANES; ++i, ++it) {
+            const int plane = WIDE ? (i + 2) % 3 : 0;  // 2, 0, 1
+            const uint32_t s = it % NS;
+            if (!(ok = mbar_wait_warp(&stage_empty[s], ((it / NS) & 1) ^ 1, ctl, STATUS_TIMEOUT_PRODUCER))) return false;
             if (elect_one_sync()) {
-              multiply(d, idesc, s2, s0, false);
-              multiply(d, idesc, s0, s2, true);
-              free_stage(s2);
+              if (leader) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE);
+              const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
+              uint8_t* a = smem + s * Cfg::STAGE;
+              uint8_t* b = a + Cfg::A_TILE;
+              if constexpr (Cfg::A_MN) {
+#pragma unroll
+                for (int g = 0; g < BM / 64; ++g) tma_load_3d_pair(a + g * Cfg::MN_BOX, &tmap_a, bar, a0 + g * 64, ka, plane);
+              } else {
+                tma_load_3d_pair(a, &tmap_a, bar, ka, a0, plane);
+              }
+              if constexpr (Cfg::B_MN) {
+#pragma unroll
+                for (int g = 0; g < Cfg::B_BOXES; ++g) tma_load_3d_pair(b + g * Cfg::MN_BOX, &tmap_b, bar, b0 + g * 64, kw, plane);
+              } else {
+                tma_load_3d_pair(b, &tmap_b, bar, kw, b0, plane);
+              }
             }
             __syncwarp();
-            if (!mbar_wait_warp(&full[s1], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
-            tc_fence_after_sync();
-            if (elect_one_sync()) {
-              multiply(d, idesc, s1, s1, true);
-              multiply(d, idesc, s1, s0, true);
-              multiply(d, idesc, s0, s1, true);
-              free_stage(s1);
-              multiply(d, idesc, s0, s0, true);
-              free_stage(s0);
-              umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
-            }
-            advance();
-            advance();
-          } else {
-            tc_fence_after_sync();
-            if (elect_one_sync()) {
-              multiply(d, idesc, s, s, kb > t.k0);
-              free_stage(s);
-              if (done) umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
-            }
           }
-          __syncwarp();
-          advance();
-          if (done) ++accs;
         }
         return true;
       });
+      // The leader's commits arrive on both CTAs' stage_empty barriers: this CTA stays until the last ones are in.
+      for (uint32_t d = ok ? min(it, static_cast<uint32_t>(NS)) : 0u; ok && d > 0; --d)
+        ok = mbar_wait_warp(&stage_empty[(it - d) % NS], ((it - d) / NS) & 1, ctl, STATUS_TIMEOUT_PRODUCER);
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMA issuer (leader only)
+      if (leader) {
+        constexpr uint32_t STAGE_ENC = Cfg::STAGE >> 4;
+        constexpr uint32_t a_step = Cfg::A_MN ? 128 : 2, b_step = Cfg::B_MN ? 128 : 2;  // 16 contraction values
+        const uint32_t a_at = smem_u32(smem), b_at = a_at + Cfg::A_TILE;
+        const uint64_t da0 = Cfg::A_MN ? umma_desc_mn16_sw128(a_at, Cfg::MN_BOX) : umma_desc_k_sw128(a_at);
+        const uint64_t db0 = Cfg::B_MN ? umma_desc_mn16_sw128(b_at, Cfg::MN_BOX) : umma_desc_k_sw128(b_at);
+        uint32_t s = 0, ph = 0, accs = 0;
+        const auto advance = [&] {
+          if (++s == NS) {
+            s = 0;
+            ph ^= 1;
+          }
+        };
+        // rows of stage sa by columns of stage sb
+        const auto multiply = [&](uint32_t d, uint32_t idesc, uint32_t sa, uint32_t sb, bool add) {
+          const uint64_t da = da0 + sa * STAGE_ENC, db = db0 + sb * STAGE_ENC;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) umma_16_ss_pair(d, da + a_step * k, db + b_step * k, idesc, add || k > 0 ? 1u : 0u);
+        };
+        const auto free_stage = [&](uint32_t stage) { umma_commit_pair_mcast(smem_u32(&stage_empty[stage]), 3); };
+        walk([&](const Tile& t) {
+          const uint32_t idesc = p.idesc | static_cast<uint32_t>(t.mma >> 3) << 17;
+          int sum_end = t.k0;  // of the k-blocks of this accumulator
+          for (int kb = t.k0; kb < t.k1; ++kb) {
+            const uint32_t buf = accs & 1, d = tmem_base + buf * Cfg::BUF_COLS;
+            const bool begin = kb == sum_end;
+            if (begin) {
+              sum_end = min(kb + drain, t.k1);
+              if (!mbar_wait_warp(&acc_empty[buf], ((accs >> 1) & 1) ^ 1, ctl, STATUS_TIMEOUT_MMA)) return false;
+            }
+            if (!mbar_wait_warp(&full[s], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
+            const bool done = kb + 1 == sum_end;
+            if constexpr (WIDE) {
+              // planes 2, 0 and 1 in three stages (of six: the three have the same parity of the wait); the first is free again after a third of the MMAs
+              const uint32_t s2 = s, s0 = s + 1, s1 = s + 2;
+              if (!mbar_wait_warp(&full[s0], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
+              tc_fence_after_sync();
+              if (elect_one_sync()) {
+                multiply(d, idesc, s2, s0, false);
+                multiply(d, idesc, s0, s2, true);
+                free_stage(s2);
+              }
+              __syncwarp();
+              if (!mbar_wait_warp(&full[s1], ph, ctl, STATUS_TIMEOUT_MMA)) return false;
+              tc_fence_after_sync();
+              if (elect_one_sync()) {
+                multiply(d, idesc, s1, s1, true);
+                multiply(d, idesc, s1, s0, true);
+                multiply(d, idesc, s0, s1, true);
+                free_stage(s1);
+                multiply(d, idesc, s0, s0, true);
+                free_stage(s0);
+                umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
+              }
+              advance();
+              advance();
+            } else {
+              tc_fence_after_sync();
+              if (elect_one_sync()) {
+                multiply(d, idesc, s, s, !begin);
+                free_stage(s);
+                if (done) umma_commit_pair_mcast(smem_u32(&acc_full[buf]), 3);
+              }
+            }
+            __syncwarp();
+            advance();
+            if (done) ++accs;
+          }
+          return true;
+        });
+      }
     }
-  } else if (warp >= 4) {
+  } else {
+    if constexpr (!WIDE) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------------------------ epilogue: a row and half of the tile's columns to a thread
     const int q = warp & 3, h = (warp - 4) >> 2;
     uint8_t* box = boxes + (warp - 4) * Cfg::BOX;
     constexpr int CHUNKS = Cfg::COLS / 32;
     uint32_t accs = 0;
-    static_assert(!WIDE || CHUNKS <= 3);
-    float sum[WIDE ? CHUNKS : 1][32];  // WIDE: what the accumulators of a tile add up to
+    static_assert(CHUNKS == 3 || CHUNKS == 4);
+    float sum[CHUNKS][32];  // what the accumulators of a tile add up to
 
     // of the unit's row (STATS), of the tile's row (PROB)
     float top = -INFINITY, total = 0.f, lse = 0.f, lse2 = 0.f, g = 0.f;
@@ -629,62 +641,40 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         }
       };
 
-      for (int kb = WIDE ? t.k0 : t.k1 - 1; kb < t.k1; ++kb, ++accs) {
+      for (int kb = t.k0; kb < t.k1; kb += drain, ++accs) {
         const uint32_t buf = accs & 1;
         if (!mbar_wait_warp(&acc_full[buf], (accs >> 1) & 1, ctl, STATUS_TIMEOUT_EPILOGUE)) return false;
         tc_fence_after_sync();
         const uint32_t empty = map_to_cta(smem_u32(&acc_empty[buf]), 0);
         const uint32_t at = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * Cfg::BUF_COLS + h * Cfg::COLS;
-        const auto release = [&] {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(empty);
-        };
-        if (chunks == 0) {
-          release();
-          continue;
-        }
-        uint32_t ld[32];
-        if constexpr (WIDE) {
 #pragma unroll
-          for (int c = 0; c < CHUNKS; ++c) {
-            if (c < chunks) {
-              tmem_ld_32x32(at + c * 32, ld);
-              tmem_ld_wait();
-              if (kb == t.k0) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) sum[c][e] = __uint_as_float(ld[e]);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) sum[c][e] += __uint_as_float(ld[e]);
-              }
-            }
-          }
-          release();
-          if (kb + 1 < t.k1) continue;
-#pragma unroll 1
-          for (int c = 0; c < chunks; ++c) {
-            float v[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = c == 0 ? sum[0][e] : c == 1 ? sum[CHUNKS > 1 ? 1 : 0][e] : sum[CHUNKS > 2 ? 2 : 0][e];
-            process(v, c);
-          }
-        } else {
-          tmem_ld_32x32(at, ld);
-#pragma unroll 1
-          for (int c = 0; c < chunks; ++c) {
+        for (int c = 0; c < CHUNKS; ++c) {
+          if (c < chunks) {
+            uint32_t ld[32];
+            tmem_ld_32x32(at + c * 32, ld);
             tmem_ld_wait();
-            float v[32];
+            if (kb == t.k0) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(ld[e]);
-            if (c + 1 < chunks) {
-              tmem_ld_32x32(at + (c + 1) * 32, ld);
+              for (int e = 0; e < 32; ++e) sum[c][e] = __uint_as_float(ld[e]);
             } else {
-              release();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) sum[c][e] += __uint_as_float(ld[e]);
             }
-            process(v, c);
           }
         }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(empty);
+      }
+#pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float low = c == 0 ? sum[0][e] : sum[1][e], high = c == 2 || CHUNKS == 3 ? sum[2][e] : sum[CHUNKS - 1][e];
+          v[e] = c < 2 ? low : high;
+        }
+        process(v, c);
       }
       if constexpr (MODE == ENTROPY_STATS) {
         if (t.last && valid) p.stats[(static_cast<int64_t>(t.un) * 2 + h) * p.rows + row] = make_float2(top, total);
