@@ -445,23 +445,22 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     int64_t target = -1;
     bool ignored = false;
     const float alpha = MODE == ENTROPY_OUT_X || MODE == ENTROPY_OUT_W ? p.factors[1] : 1.f;
+    const float factor = MODE == ENTROPY_PROB ? p.factors[0] : 1.f;
 
     walk([&](const Tile& t) {
       const int row0 = t.tm * (2 * BM) + static_cast<int>(rank) * BM + q * 32;  // of the warp
       const int row = row0 + lane;
       const int col0 = t.n0 + h * Cfg::COLS;                                    // of the thread
       const bool valid = row < p.rows;
+      // (what comes from memory is looked at when the products are there)
+      int64_t own = p.ignore;
+      float own_lse = 0.f, own_dloss = 0.f;
       if constexpr (MODE == ENTROPY_STATS || MODE == ENTROPY_PROB) {
-        if (t.first) {
-          top = -INFINITY;
-          total = 0.f;
-          const int64_t to = valid ? entropy_target(p, row) : p.ignore;
-          ignored = to == p.ignore;
-          target = ignored ? -1 : to - p.b_row;
+        if (t.first && valid) {
+          own = entropy_target(p, row);
           if constexpr (MODE == ENTROPY_PROB) {
-            lse = valid ? p.lse[row] : 0.f;
-            lse2 = lse * LOG2E_F;
-            g = ignored ? 0.f : to < 0 || to >= p.symbols ? __int_as_float(0x7fc00000) : p.dloss[p.per_row ? row : 0] * p.factors[0];
+            own_lse = p.lse[row];
+            own_dloss = p.dloss[p.per_row ? row : 0];
           }
         }
       }
@@ -665,6 +664,17 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(empty);
+      }
+      if constexpr (MODE == ENTROPY_STATS || MODE == ENTROPY_PROB) {
+        if (t.first) {
+          top = -INFINITY;
+          total = 0.f;
+          ignored = own == p.ignore;
+          target = ignored ? -1 : own - p.b_row;
+          lse = own_lse;
+          lse2 = own_lse * LOG2E_F;
+          g = ignored ? 0.f : own < 0 || own >= p.symbols ? __int_as_float(0x7fc00000) : own_dloss * factor;
+        }
       }
 #pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
