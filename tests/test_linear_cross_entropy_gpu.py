@@ -170,6 +170,8 @@ def test_few_rows_with_masks(n, kind):
     loss, lse = tb.linear_cross_entropy(x, w, t, reduction="none", return_lse=True)
     dx, _ = tb.linear_cross_entropy_backward(g, x, w, t, lse, reduction="none", weight_grad=False)
     assert torch.equal(loss, want[0]) and torch.equal(dx, want[2]) and bool(lse[::4].isnan().all())
+    dx, dw = tb.linear_cross_entropy_backward(g, x, w, t, lse, reduction="none")
+    assert torch.equal(dx, want[2]) and torch.equal(dw, want[3])
     x, w, t = inputs(n, 700, 96, kind)
     t[3], t[n - 1] = 700, -1
     loss, lse = tb.linear_cross_entropy(x, w, t, reduction="none", return_lse=True)
@@ -220,12 +222,14 @@ def test_ignored_positions(kind):
     lse = want[1]
     got = tb.linear_cross_entropy_backward(g, x, w, t, lse, reduction="none")
     assert torch.equal(got[0], want[2]) and torch.equal(got[1], want[3])
-    # nor does what x holds there, to the losses and to dx
+    # nor does what x holds there
     x[::3] = float("nan")
     loss, lse = tb.linear_cross_entropy(x, w, t, reduction="none", return_lse=True)
     assert torch.equal(loss, want[0]) and bool(lse[::3].isnan().all())
     dx, none = tb.linear_cross_entropy_backward(torch.ones(300, device="cuda"), x, w, t, lse, reduction="none", weight_grad=False)
     assert torch.equal(dx, want[2]) and none is None
+    dx, dw = tb.linear_cross_entropy_backward(torch.ones(300, device="cuda"), x, w, t, lse, reduction="none")
+    assert torch.equal(dx, want[2]) and torch.equal(dw, want[3])
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)

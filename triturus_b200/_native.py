@@ -965,7 +965,7 @@ def _embedding_impl(tokens: torch.Tensor, weight: torch.Tensor, scale: float) ->
 
 def _embedding_backward_impl(dy: torch.Tensor, tokens: torch.Tensor, symbols: int, scale: float, padding_idx: int | None) -> torch.Tensor:
     _require_cuda(dy)
-    width, count = dy.shape[-1], tokens.numel()
+    width, count, symbols = dy.shape[-1], tokens.numel(), int(symbols)
     dweight = torch.empty((symbols, width), dtype=dy.dtype, device=dy.device)
     tokens = tokens.contiguous()
     rows, stride = _rows(dy)
@@ -974,7 +974,7 @@ def _embedding_backward_impl(dy: torch.Tensor, tokens: torch.Tensor, symbols: in
         ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dy.device)
         rc = LIB.triturus_b200_embedding_backward(
             rows.data_ptr(), tokens.data_ptr(), tokens.element_size(), dweight.data_ptr(), count, symbols, width, stride,
-            _TYPE_CODES[dy.dtype], scale, -1 if padding_idx is None else padding_idx, ws.data_ptr(), nbytes, _raw_stream(idx),
+            _TYPE_CODES[dy.dtype], scale, -1 if padding_idx is None else int(padding_idx), ws.data_ptr(), nbytes, _raw_stream(idx),
         )  # fmt: skip
     _check(rc, "triturus_b200_embedding_backward")
     return dweight

@@ -336,7 +336,7 @@ struct SumArgs {
 template <class T>
 __device__ __forceinline__ int column_of(const SumArgs& p, int key, int slot) {
   constexpr int N = Pack<T, 16>::N;
-  return slot * N - ((p.base + key * p.width) & (N - 1));
+  return slot * N - static_cast<int>((static_cast<uint32_t>(p.base) + static_cast<uint32_t>(key) * static_cast<uint32_t>(p.width)) & (N - 1));
 }
 template <class T>
 __device__ __forceinline__ void store_row(const SumArgs& p, int key, int slot, const float* acc) {

@@ -407,7 +407,7 @@ bool padding_arg(PyObject* o, int64_t symbols, int64_t* padding) {
 bool scale_arg(PyObject* o, float* scale) {
   if (!PyFloat_CheckExact(o)) return false;
   *scale = static_cast<float>(PyFloat_AS_DOUBLE(o));
-  return std::isfinite(PyFloat_AS_DOUBLE(o));
+  return std::isfinite(*scale);
 }
 
 // embedding(tokens, weight, scale, padding_idx)

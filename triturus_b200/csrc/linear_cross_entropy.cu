@@ -23,9 +23,20 @@ constexpr int64_t kMostStats = 1ll << 26;   // bytes of the spans' maxima and su
 
 // ----------------------------------------------------------------------------- operands that TMA cannot read in place
 
+__device__ __forceinline__ int64_t index_at(const void* a, int wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(a)[i] : static_cast<int64_t>(static_cast<const int32_t*>(a)[i]);
+}
+
+// Rows that are not copied but zero: those whose target (null: there are none) is `ignore`.
+struct Mask {
+  const void* target;
+  int64_t ignore;
+  int wide;
+};
+
 // Rows on 16-byte boundaries, as they are or (PLANES) as three planes of bfloat16.
 template <class T, bool PLANES>
-__global__ void __launch_bounds__(256) entropy_copy_kernel(const T* x, int64_t rows, int width, int64_t stride, void* out, int64_t pitch, int64_t plane) {
+__global__ void __launch_bounds__(256) entropy_copy_kernel(const T* x, int64_t rows, int width, int64_t stride, void* out, int64_t pitch, int64_t plane, Mask mask) {
   using Eight = Pack<T, 8 * static_cast<int>(sizeof(T))>;
   pdl_launch_dependents();
   pdl_wait();
@@ -35,7 +46,10 @@ __global__ void __launch_bounds__(256) entropy_copy_kernel(const T* x, int64_t r
     const int c = static_cast<int>(i - row * (pitch / 8)) * 8;
     const T* src = x + row * stride + c;
     Eight v;
-    if (c + 8 <= width && reinterpret_cast<uintptr_t>(src) % sizeof(v) == 0) {
+    if (mask.target != nullptr && index_at(mask.target, mask.wide, row) == mask.ignore) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.v[e] = from_float<T>(0.f);
+    } else if (c + 8 <= width && reinterpret_cast<uintptr_t>(src) % sizeof(v) == 0) {
       v = *reinterpret_cast<const Eight*>(src);
     } else {
 #pragma unroll
@@ -61,10 +75,6 @@ __global__ void __launch_bounds__(256) entropy_copy_kernel(const T* x, int64_t r
 }
 
 // ----------------------------------------------------------------------------- small kernels around the products
-
-__device__ __forceinline__ int64_t index_at(const void* a, int wide, int64_t i) {
-  return wide ? static_cast<const int64_t*>(a)[i] : static_cast<int64_t>(static_cast<const int32_t*>(a)[i]);
-}
 
 struct JoinArgs {
   const float2* stats;  // [parts][rows]
@@ -289,11 +299,12 @@ constexpr int64_t kLines = 2048;
 struct Reading {
   int type;
   bool raw, lines;
+  Mask mask;  // x of the gradients: dW multiplies it with d, and what a position without a loss holds (it may be NaN) must not count
 };
-Reading reading_of(int64_t rows, int type, bool weight);
+Reading reading_of(int64_t rows, int type, bool weight, Mask mask = {});
 // Whether an operand is read where it lies: rows on 16-byte boundaries (or lines), and 32-bit elements only as they are.
 bool in_place(const void* data, int64_t rows, int64_t stride, const Reading& how) {
-  if (how.type == TRITURUS_B200_TYPE_F32 && !how.raw) return false;
+  if ((how.type == TRITURUS_B200_TYPE_F32 && !how.raw) || how.mask.target != nullptr) return false;
   const int64_t unit = how.lines ? 128 : 16;
   return aligned_to(data, unit) && (rows == 1 || (stride > 0 && stride * size_of(how.type) % unit == 0 && stride < (1ll << 37)));
 }
@@ -357,7 +368,7 @@ int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t st
   m->plane = rows * m->pitch;
   const int grid = copy_grid(rows * (m->pitch / 8));
   const auto run = [&](auto kern, auto t) {
-    return launch(kern, grid, 256, 0, static_cast<const decltype(t)*>(data), rows, static_cast<int>(width), stride, space, m->pitch, m->plane);
+    return launch(kern, grid, 256, 0, static_cast<const decltype(t)*>(data), rows, static_cast<int>(width), stride, space, m->pitch, m->plane, how.mask);
   };
   if (type == TRITURUS_B200_TYPE_F32) return raw ? run(entropy_copy_kernel<float, false>, 0.f) : run(entropy_copy_kernel<float, true>, 0.f);
   if (type == TRITURUS_B200_TYPE_BF16) return run(entropy_copy_kernel<__nv_bfloat16, false>, __nv_bfloat16());
@@ -518,8 +529,8 @@ size_t part_bytes(const EntropyParams& p) {
 // 47 / 143 and 47 / 149, 96 rows (two tiles of 64) 68 / 184 and 48 / 151; float32 64 rows 100 / 312 and 376 / 714, 192 rows 239 / 774 and
 // 406 / 885, 256 rows 356 / 1064 and 415 / 972.
 bool few(int64_t rows, int type) { return rows <= (type == TRITURUS_B200_TYPE_F32 ? 192 : 64); }
-Reading reading_of(int64_t rows, int type, bool weight) {
-  return {type, type == TRITURUS_B200_TYPE_F32 && weight && few(rows, type), type != TRITURUS_B200_TYPE_F32 && rows >= kLines};
+Reading reading_of(int64_t rows, int type, bool weight, Mask mask) {
+  return {type, type == TRITURUS_B200_TYPE_F32 && weight && few(rows, type), type != TRITURUS_B200_TYPE_F32 && rows >= kLines, mask};
 }
 
 FewParams few_of(int64_t rows, int64_t length, int64_t k) {
@@ -651,7 +662,7 @@ BackwardSpace backward_space(void* base, const BackwardPlan& b, const void* x, c
   Space s = {static_cast<char*>(base), 0};
   BackwardSpace f;
   const bool is_few = few(rows, type);
-  f.x = s.take(copy_bytes(x, rows, width, x_stride, reading_of(rows, type, false)));
+  f.x = s.take(copy_bytes(x, rows, width, x_stride, reading_of(rows, type, false, {&f, 0, 0})));  // (room for a copy in any case)
   f.weight = s.take(copy_bytes(weight, symbols, width, weight_stride, reading_of(rows, type, true)));
   f.factors = static_cast<float*>(s.take(2 * sizeof(float)));
   f.d = static_cast<uint16_t*>(s.take(static_cast<size_t>(rows) * static_cast<size_t>(b.d_pitch) * 2 * (type == TRITURUS_B200_TYPE_F32 ? 3 : 1)));
@@ -781,7 +792,8 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
   Launches launch = {st};
   Matrix mx, mw;
   const bool is_few = few(rows, type);
-  int rc = prepare(&mx, x, rows, width, x_stride, reading_of(rows, type, false), space.x, launch);
+  const Mask mask = {dweight != nullptr ? target : nullptr, ignore_index, target_bytes == 8};
+  int rc = prepare(&mx, x, rows, width, x_stride, reading_of(rows, type, false, mask), space.x, launch);
   if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, reading_of(rows, type, true), space.weight, launch);
   const int wide = target_bytes == 8;
   if (rc == TRITURUS_B200_OK && !is_few)

@@ -33,8 +33,8 @@ def _check_backward(dy: torch.Tensor, tokens: torch.Tensor, symbols: int, scale:
 def _check_numbers(name: str, symbols: int, width: int, scale: float, padding_idx: int | None) -> None:
     if symbols < 1 or width < 1:
         raise ValueError(f"{name}: a table of {symbols} rows of {width} elements is not supported")
-    if not math.isfinite(scale):
-        raise ValueError(f"{name}: scale must be finite, got {scale!r}")
+    if not (math.isfinite(scale) and abs(scale) <= torch.finfo(torch.float32).max):
+        raise ValueError(f"{name}: scale must be a finite number of 32 bits, got {scale!r}")
     if padding_idx is not None and not 0 <= padding_idx < symbols:
         raise ValueError(f"{name}: padding_idx is out of range, got {padding_idx!r}")
 
