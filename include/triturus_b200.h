@@ -272,10 +272,10 @@ int triturus_b200_mm_f32(const float* a, const float* b, float* out, int64_t M, 
                          int precision, int32_t* status_dev, void* stream);
 
 /*
- * Operators for models around the contractions: layer norm with its gradients, clipping of gradients by their global norm,
- * sampling from log-probabilities, and the lookup of symbols in a table with its gradient.  (No counterpart in the reference.)  Their elements are 32-bit floats, bfloat16 or 16-bit
- * floats; the arithmetic between loads and stores has 32 bits or more.  None of them waits on a barrier that it could miss, so
- * none takes a status word.
+ * Operators for models around the contractions: layer norm with its gradients, clipping of gradients by their global norm, sampling from
+ * log-probabilities, the lookup of symbols in a table with its gradient, and the cross entropy of a linear layer over many symbols with its gradients.
+ * (No counterpart in the reference.)  Their elements are 32-bit floats, bfloat16 or 16-bit floats; the arithmetic between loads and stores has
+ * 32 bits or more.  Only the cross entropy waits on barriers that it could miss, and takes a status word.
  */
 #define TRITURUS_B200_TYPE_F32 0
 #define TRITURUS_B200_TYPE_BF16 1
