@@ -429,7 +429,6 @@ int64_t cycles_of(int64_t cols, int type) {
 constexpr int64_t kTileCycles = 2500;    // of a tile beside its MMAs
 constexpr int64_t kSumCycles = 6000;     // of a launch that adds parts
 constexpr int64_t kBytesPerCycle = 3500;
-constexpr int64_t kMostSplits = 74;      // of a contraction
 constexpr int64_t kLeastUnits = 5;       // waves of tiles from which on their rounding up does not matter
 
 EntropyParams product_of(int64_t rows, int64_t cols, int64_t k) {
@@ -502,7 +501,11 @@ EntropyParams out_of(int64_t rows, int64_t cols, int64_t k, int type) {
   for (int64_t tile = widest(type); tile >= 96; tile -= 32) {
     const int64_t even = std::min<int64_t>(tile, up_to(parts_of(cols, parts_of(cols, tile)), 32));
     const int64_t units = p.tiles_m * parts_of(cols, even), full = units / pairs, left = units - full * pairs, cycles = cycles_of(even, type);
-    for (int64_t most = 1; most <= (left == 0 ? 1 : kMostSplits); ++most) {
+    // (few parts, and the most that 1 to 4 waves of them have)
+    const int candidates = left == 0 ? 1 : 12;
+    for (int i = 0; i < candidates; ++i) {
+      const int64_t most = i < 8 ? i + 1 : (i - 7) * pairs / left;
+      if (most > p.kblocks || (i >= 8 && most <= 8)) continue;
       const int64_t kb = parts_of(p.kblocks, most), splits = parts_of(p.kblocks, kb);
       const int64_t parts = left * splits * 256 * even * 2 * static_cast<int64_t>(sizeof(float)) / kBytesPerCycle;  // written and read
       const int64_t cost = full * (p.kblocks * cycles + kTileCycles) + parts_of(left * splits, pairs) * (kb * cycles + kTileCycles) +
@@ -638,6 +641,7 @@ ForwardSpace forward_space(void* base, const void* x, const void* weight, int64_
 
 struct BackwardPlan {
   int64_t piece, pieces, last, d_pitch, sum_pitch;  // last: symbols of the last piece
+  EntropyParams x[2], w[2];                         // OUT_X (not of few rows) and OUT_W, of a piece and of the last one
 };
 BackwardPlan backward_plan(int64_t rows, int64_t symbols, int64_t width, int type) {
   BackwardPlan b;
@@ -649,6 +653,16 @@ BackwardPlan backward_plan(int64_t rows, int64_t symbols, int64_t width, int typ
   b.last = symbols - (b.pieces - 1) * b.piece;
   b.d_pitch = up_to(b.piece, 64);
   b.sum_pitch = up_to(width, 8);
+  for (int i = 0; i < 2; ++i) {
+    const int64_t piece = i == 0 ? b.piece : b.last;
+    if (i == 1 && b.last == b.piece) {
+      b.x[1] = b.x[0];
+      b.w[1] = b.w[0];
+    } else {
+      b.x[i] = few(rows, type) ? EntropyParams{} : out_of(rows, width, piece, type);
+      b.w[i] = out_of(piece, width, rows, type);
+    }
+  }
   return b;
 }
 struct BackwardSpace {
@@ -668,10 +682,10 @@ BackwardSpace backward_space(void* base, const BackwardPlan& b, const void* x, c
   f.d = static_cast<uint16_t*>(s.take(static_cast<size_t>(rows) * static_cast<size_t>(b.d_pitch) * 2 * (type == TRITURUS_B200_TYPE_F32 ? 3 : 1)));
   f.sum = static_cast<float*>(s.take(b.pieces > 1 ? static_cast<size_t>(rows) * static_cast<size_t>(b.sum_pitch) * sizeof(float) : 0));
   size_t parts = 0;  // (one product at a time uses them)
-  for (const int64_t piece : {b.piece, b.last}) {
-    const size_t of_x = is_few ? static_cast<size_t>(few_columns_of(rows, width, piece).splits) * static_cast<size_t>(rows * b.sum_pitch) * sizeof(float)
-                               : part_bytes(out_of(rows, width, piece, type));
-    parts = std::max({parts, of_x, part_bytes(out_of(piece, width, rows, type))});
+  for (int i = 0; i < 2; ++i) {
+    const size_t of_x = is_few ? static_cast<size_t>(few_columns_of(rows, width, i == 0 ? b.piece : b.last).splits) * static_cast<size_t>(rows * b.sum_pitch) * sizeof(float)
+                               : part_bytes(b.x[i]);
+    parts = std::max({parts, of_x, part_bytes(b.w[i])});
   }
   f.part = static_cast<float*>(s.take(parts));
   f.bytes = s.used;
@@ -807,8 +821,9 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
   md.planes = type == TRITURUS_B200_TYPE_F32 ? 3 : 1;
   for (int64_t i = 0; i < plan.pieces && rc == TRITURUS_B200_OK; ++i) {
     const int64_t first = i * plan.piece, piece = i + 1 < plan.pieces ? plan.piece : plan.last;
-    EntropyParams p = prob_of(rows, piece, width, type);
-    if (!set_whole(p)) return TRITURUS_B200_EINVAL;
+    const int last = i + 1 == plan.pieces ? 1 : 0;
+    EntropyParams p = is_few ? EntropyParams{} : prob_of(rows, piece, width, type);
+    if (!is_few && !set_whole(p)) return TRITURUS_B200_EINVAL;
     p.b_row = static_cast<int>(first);
     p.target = target;
     p.target_wide = wide;
@@ -846,7 +861,7 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
     };
     if (dx != nullptr && rc == TRITURUS_B200_OK) {
       const bool begin = i == 0, end = i + 1 == plan.pieces;
-      EntropyParams q = out(out_of(rows, width, piece, type), dx, begin ? end ? DEST_FINAL : DEST_SUM : end ? DEST_FINAL_ADD : DEST_SUM_ADD);
+      EntropyParams q = out(plan.x[last], dx, begin ? end ? DEST_FINAL : DEST_SUM : end ? DEST_FINAL_ADD : DEST_SUM_ADD);
       q.b_k = static_cast<int>(first);
       if (is_few) {
         FewParams f = few_columns_of(rows, width, piece);
@@ -858,7 +873,7 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
       }
     }
     if (dweight != nullptr && rc == TRITURUS_B200_OK) {
-      EntropyParams q = out(out_of(piece, width, rows, type), static_cast<char*>(dweight) + first * width * size, DEST_FINAL);
+      EntropyParams q = out(plan.w[last], static_cast<char*>(dweight) + first * width * size, DEST_FINAL);
       rc = set_whole(q) ? run_products<ENTROPY_OUT_W>(md, mx, q, type, launch) : TRITURUS_B200_EINVAL;
     }
   }
