@@ -195,6 +195,29 @@ def test_few_rows_and_pieces_of_the_symbols(kind):
     check(*inputs(64, 1_500_001 if kind == torch.float32 else 4_300_001, 8, kind))
 
 
+@pytest.mark.parametrize("n", [16, 80])
+def test_large_offsets(n):
+    """A table beyond 2^31 elements: its last rows are read and their gradients written at 64-bit offsets."""
+    v, d = 270_001, 8192
+    w = torch.zeros(v, d, dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 1, 5, 131_072, 262_143, 262_144, v - 2, v - 1], device="cuda")
+    w[some] = (rand(len(some), d) / 90.0).bfloat16()
+    x = rand(n, d, seed=1).bfloat16()
+    t = some[torch.arange(n, device="cuda") % len(some)]
+    loss, lse = tb.linear_cross_entropy(x, w, t, reduction="sum", return_lse=True)
+    dx, dw = tb.linear_cross_entropy_backward(torch.ones((), device="cuda"), x, w, t, lse, reduction="sum")
+    tb.check_status()
+    z = x.double() @ w[some].double().t()  # (all other logits are 0)
+    want = torch.logsumexp(torch.cat([z, torch.full((n, 1), math.log(v - len(some)), device="cuda", dtype=torch.float64)], 1), 1)
+    assert bool(((lse.double() - want).abs() <= 1e-4).all())
+    p = torch.exp(z - want[:, None]) - (t[:, None] == some).double()
+    for got, exact in ((dx, p @ w[some].double()), (dw[some], p.t() @ x.double())):
+        assert float((got.double() - exact).norm()) <= 2.0**-7 * float(exact.norm())
+    rest = torch.exp(-want) @ x.double()  # every other row's gradient
+    for row in (2, 200_000, 262_145, v - 3):
+        assert float((dw[row].double() - rest).norm()) <= 2.0**-7 * float(rest.norm())
+
+
 def test_wide_rows():
     check(*inputs(64, 700, 8192, torch.bfloat16))
     check(*inputs(64, 700, 8192, torch.float32))
