@@ -76,6 +76,20 @@ def test_matches_definition(count, symbols, width, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("count,symbols,width", [(2, 1, 520), (255, 3, 65), (256, 90, 511), (257, 90, 512), (513, 70_000, 264), (1023, 6, 256), (1024, 2000, 255)])
+def test_few_positions(count, symbols, width, kind):
+    """Numbers of positions, and of vectors of a row, at the borders of what the form without a sort takes at a time."""
+    tokens = draw_tokens(count, symbols)
+    dy = rand(count, width + 3, kind=kind)
+    check_backward(dy[:, :width], tokens, symbols, 0.7)
+    check_backward(dy[:, 1 : 1 + width], tokens.int(), symbols, padding=0)
+    tokens[::3], tokens[1::7] = -1, symbols
+    check_backward(dy[:, 3:], tokens, symbols)
+    check_backward(dy[:, :width].contiguous(), torch.full_like(tokens, symbols - 1), symbols)
+    assert not check_backward(dy[:, 3:], torch.full_like(tokens, symbols), symbols).any()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
 def test_one_symbol_everywhere(kind):
     """A run over all tiles."""
     for count in (32, 33, 64, 65, 700, 8192, 8193, 20_000, 65_537):

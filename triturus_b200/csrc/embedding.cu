@@ -10,7 +10,8 @@
 // each other's shared memory; beyond, two launches a pass.  Blocks beside those fill the table with zeros.  Then groups of threads walk tiles of sorted
 // positions: a thread keeps its 16 bytes of columns as 32-bit sums and writes them where a symbol's run ends.  A run over a border of
 // two tiles is left in the workspace in parts, which a last launch adds in their order: frequent symbols are spread over many
-// blocks, and the same call gives the same result each time.  Bound by memory: dy read once, the table written once.
+// blocks, and the same call gives the same result each time.  Few positions are not sorted but compared with
+// each other.  Bound by memory: dy read once, the table written once.
 #include <algorithm>
 
 #include "packs.cuh"
@@ -31,6 +32,13 @@ constexpr int kClusterSort = 1 << 14;  // positions (16384: 17 us in one launch 
 // Bytes of the table that are filled beside a launch of the sort; what is left over by a launch of its own, which is faster (1 GB: 148 and 190 us).
 constexpr int64_t kFillBeside = 64 << 20, kFillCount = 16 << 20, kFillPlace = 48 << 20;
 constexpr int kGroup = 128;          // threads of a block that adds rows
+// Positions that are not sorted, and blocks of kDirectLanes vectors for them, at most (each looks through all positions).  Microseconds of the whole call in bfloat16
+// without and with the sort: 512 rows of width 512 and 5000 symbols 8.0 and 16.7, 1024 of width 1024 (2048 blocks) 10.7 and 19, 1000 of 2048 (4000) 16.1 and 20.2,
+// 1000 of 4096 (8000) 26.9 and 22.6.  All of one symbol: 1000 of 512 23.5 and 26.8, with a table of 100 MB 54 and 42.
+constexpr int kDirect = 1024;
+constexpr int64_t kDirectBlocks = 4096;
+constexpr int kDirectThreads = 256;
+constexpr int kDirectLanes = 64;
 constexpr int kJoins = 2;            // groups of them that add the parts of a run
 
 // A symbol of a list of 64- or 32-bit ones.
@@ -510,6 +518,95 @@ __global__ void __launch_bounds__(kGroup * kJoins) embedding_join_kernel(const S
   if (group == 0 && mine) store_row<T>(p, run, slot, acc);
 }
 
+// ----------------------------------------------------------------------------- few positions
+
+__global__ void __launch_bounds__(kSortThreads) embedding_fill_kernel(char* table, int64_t bytes) {
+  pdl_launch_dependents();
+  fill_table(table, bytes, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+}
+
+// Without a sort: the block of a position looks through all of them for its symbol and, where none of them comes earlier, adds up the rows of
+// those that have it, a consecutive share of them to each group of threads.  All but the last store runs beside the launch that fills the table.
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(kDirectThreads) embedding_direct_kernel(const SumArgs p, const void* tokens, int wide, int64_t padding) {
+  constexpr int N = Pack<T, 16>::N, kAhead = 8, kRounds = kDirect / kDirectThreads, kWarps = kDirectThreads / 32;
+  static_assert(kRounds * kWarps == 32, "a lane to each warp's round");
+  __shared__ uint16_t list[kDirect];
+  __shared__ int before[kRounds][kWarps], found;
+  __shared__ float sums[kDirectThreads / kDirectLanes - 1][N][kDirectLanes];
+  const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, warp_lane = tid & 31, here = static_cast<int>(blockIdx.x);
+  const int64_t own = token_at(tokens, wide, here);
+  unsigned same[kRounds];
+  bool earlier = own < 0 || own >= p.symbols || own == padding;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int i = r * kDirectThreads + tid;
+    const bool match = i < p.count && token_at(tokens, wide, i) == own;
+    earlier = earlier || (match && i < here);
+    same[r] = __ballot_sync(0xffffffffu, match);
+    if (warp_lane == 0) before[r][warp] = __popc(same[r]);
+  }
+  if (__syncthreads_or(earlier)) {
+    pdl_wait();
+    return;
+  }
+  if (warp == 0) {
+    int* n = &before[0][0] + warp_lane;
+    const int mine = *n;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (warp_lane >= o) upto += v;
+    }
+    *n = upto - mine;
+    if (warp_lane == 31) found = upto;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+    if (same[r] >> warp_lane & 1) list[before[r][warp] + __popc(same[r] & ((1u << warp_lane) - 1))] = static_cast<uint16_t>(r * kDirectThreads + tid);
+  __syncthreads();
+
+  const int groups = kDirectThreads / kDirectLanes, group = tid / kDirectLanes, lane = tid % kDirectLanes;
+  const int slot = static_cast<int>(blockIdx.y) * kDirectLanes + lane, key = static_cast<int>(own);
+  const int each = (found + groups - 1) / groups, end = min(found, (group + 1) * each);
+  const bool mine = slot < p.slots;
+  float acc[N] = {};
+  if (mine) {
+    const int column = ALIGNED ? slot * N : column_of<T>(p, key, slot);
+    for (int i = group * each; i < end; i += kAhead) {
+      Columns<T, ALIGNED> row[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u < end) row[u].begin(p, list[i + u], column);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (i + u >= end) break;
+        const uint4 bits = row[u].end(p);
+        const Pack<T, 16> r = *reinterpret_cast<const Pack<T, 16>*>(&bits);
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += to_float(r.v[e]);
+      }
+    }
+  }
+  if (found > 1) {
+    if (group > 0) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) sums[group - 1][e][lane] = acc[e];
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int g = 0; g < groups - 1; ++g)
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += sums[g][e][lane];
+    }
+  }
+  pdl_wait();
+  if (group == 0 && mine) store_row<T>(p, key, slot, acc);
+}
+
 // ----------------------------------------------------------------------------- host
 
 bool type_ok(int type) { return type >= TRITURUS_B200_TYPE_F32 && type <= TRITURUS_B200_TYPE_F16; }
@@ -612,6 +709,41 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   int rc = TRITURUS_B200_OK;
   if (count == 0) return code_of(cudaMemsetAsync(dweight, 0, static_cast<size_t>(table), st));
 
+  SumArgs p = {};
+  p.dy = dy;
+  const int64_t far = (count - 1) * dy_stride * size;
+  p.lo = static_cast<const char*>(dy) + std::min<int64_t>(far, 0);
+  p.hi = static_cast<const char*>(dy) + std::max<int64_t>(far, 0) + width * size;
+  p.dweight = dweight;
+  p.stride = dy_stride;
+  p.pitch = part_pitch(width, size);
+  p.count = static_cast<int>(count);
+  p.symbols = static_cast<int>(symbols);
+  p.width = static_cast<int>(width);
+  p.tile = tile_of(count, width, size);
+  p.scale = scale;
+  const bool off = width * size % 16 != 0 || !aligned_to(dweight, 16);
+  const int64_t vectors = slots_of(width, size);  // (room for one more than rows on boundaries have)
+  p.slots = static_cast<int>(off ? vectors : vectors - 1);
+  p.base = static_cast<int>(reinterpret_cast<uintptr_t>(dweight) % 16) / size;
+  const bool aligned = !off && aligned_to(dy, 16) && dy_stride * size % 16 == 0;
+  const int64_t direct_slabs = (p.slots + kDirectLanes - 1) / kDirectLanes;
+  if (count <= kDirect && count * direct_slabs <= kDirectBlocks) {
+    const int64_t beside = std::min(table, kFillBeside), rest = table - beside;
+    const int64_t fills = std::clamp<int64_t>(beside / (16 * kSortThreads * 4), 1, device_sms());
+    if (rest > 0) rc = code_of(cudaMemsetAsync(static_cast<char*>(dweight) + beside, 0, static_cast<size_t>(rest), st));
+    if (rc == TRITURUS_B200_OK)
+      rc = launch_of(embedding_fill_kernel, dim3(static_cast<unsigned>(fills)), kSortThreads, 0, st, nullptr, static_cast<char*>(dweight), beside);
+    if (rc != TRITURUS_B200_OK) return rc;
+    return by_type(type, [&](auto t) {
+      using T = decltype(t);
+      const cudaLaunchAttribute dependent = dependent_launch();
+      return launch_of(aligned ? embedding_direct_kernel<T, true> : embedding_direct_kernel<T, false>,
+                       dim3(static_cast<unsigned>(count), static_cast<unsigned>(direct_slabs)), kDirectThreads, 0, st, &dependent, p, tokens,
+                       token_bytes == 8 ? 1 : 0, padding);
+    });
+  }
+
   const SumSpace space = space_of(count, width, size);
   char* ws = static_cast<char*>(workspace);
   const auto list = [&](int i) { return reinterpret_cast<int32_t*>(ws + i * space.list); };
@@ -668,26 +800,9 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   }
   if (rc != TRITURUS_B200_OK) return rc;
 
-  SumArgs p = {};
-  p.dy = dy;
-  const int64_t far = (count - 1) * dy_stride * size;
-  p.lo = static_cast<const char*>(dy) + std::min<int64_t>(far, 0);
-  p.hi = static_cast<const char*>(dy) + std::max<int64_t>(far, 0) + width * size;
   p.keys = s.keys;
   p.at = s.at;
-  p.dweight = dweight;
   p.part = reinterpret_cast<float*>(ws + 4 * space.list + space.counts);
-  p.stride = dy_stride;
-  p.pitch = part_pitch(width, size);
-  p.count = static_cast<int>(count);
-  p.symbols = static_cast<int>(symbols);
-  p.width = static_cast<int>(width);
-  p.tile = tile_of(count, width, size);
-  p.scale = scale;
-  const bool off = width * size % 16 != 0 || !aligned_to(dweight, 16);
-  const int64_t vectors = slots_of(width, size);  // (room for one more than rows on boundaries have)
-  p.slots = static_cast<int>(off ? vectors : vectors - 1);
-  p.base = static_cast<int>(reinterpret_cast<uintptr_t>(dweight) % 16) / size;
   p.lanes = lanes_for(p.slots, kGroup);
   const int64_t tiles = (count + p.tile - 1) / p.tile, groups = kGroup / p.lanes;
   const unsigned slabs = static_cast<unsigned>((p.slots + p.lanes - 1) / p.lanes);
@@ -695,7 +810,6 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     const cudaLaunchAttribute dependent = dependent_launch();
-    const bool aligned = !off && aligned_to(dy, 16) && dy_stride * size % 16 == 0;
     int code = launch_of(aligned ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), slabs), kGroup, 0, st, &dependent, p);
     if (code == TRITURUS_B200_OK && tiles > 1)
       code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((p.slots + kGroup - 1) / kGroup)), kGroup * kJoins, 0, st, &dependent, p);
