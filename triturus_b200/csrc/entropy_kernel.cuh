@@ -104,6 +104,7 @@ struct EntropyParams {
   int64_t out_pitch;
   int out_vec;            // its rows are on boundaries of 16 bytes
   int direct;             // of 32 bytes
+  int boxed;              // 32-bit results of OUT_W leave through TMA
   float* sum;             // [rows][sum_pitch], what earlier pieces gave
   int64_t sum_pitch;
   float* part;            // [shared][splits][256][tile_cols]
@@ -210,7 +211,8 @@ __device__ __forceinline__ void entropy_put(const EntropyParams& p, int row, int
 
 template <class Cfg>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg::NTHREADS, 1)
-entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const EntropyParams p) {
+entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_out,
+               const EntropyParams p) {
   constexpr int BM = Cfg::BM, BN = Cfg::BN, BNH = Cfg::BNH, BK = Cfg::BK, NS = Cfg::NS, MODE = Cfg::MODE;
   constexpr bool WIDE = Cfg::WIDE;
 
@@ -469,8 +471,8 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const int chunks = rows_exist ? max(0, min(CHUNKS, (t.n1 - col0 + 31) >> 5)) : 0;
 
       // Results leave straight from registers, a sector of 32 bytes of its row to a thread: beside TMA and the MMAs there is no bandwidth of shared memory
-      // left (through it the planes of a WIDE tile took 11 600 cycles, of which the exponentials 2 800).  Only where the rows do not begin on sectors they go
-      // through a box in shared memory, in rows of 128 bytes.
+      // left (through it the planes of a WIDE tile took 11 600 cycles, of which the exponentials 2 800).  Where the rows do not begin on sectors they go
+      // through a box in shared memory, in rows of 128 bytes, and 32-bit ones of a short contraction too, from there by TMA (`boxed`).
       // 16-bit results, two to a word: chunk c of this thread's row into its half of the box; with the second half (or the last chunk) the box to memory.
       const auto box16 = [&](const uint32_t (&w)[16], int c, int c0) {
 #pragma unroll
@@ -599,14 +601,25 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           }
           if constexpr (WIDE) {
             float* out = static_cast<float*>(p.out);
-            if (p.direct) {
+            if (p.boxed) {
+              if (lane == 0) tma_store_wait_read<0>();
+              __syncwarp();
+            } else if (p.direct) {
               store_floats(out + static_cast<int64_t>(row) * p.out_pitch + c0);
               return;
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            if (p.boxed) fence_proxy_async_smem();
             __syncwarp();
+            if (p.boxed) {
+              if (lane == 0 && row0 < p.rows) {
+                tma_store_3d(&tmap_out, box, c0, row0, 0);
+                tma_store_commit();
+              }
+              return;
+            }
             if (p.out_vec) {
               const int cb = c0 + (lane & 7) * 4;
 #pragma unroll 2
@@ -646,16 +659,18 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         tc_fence_after_sync();
         const uint32_t empty = map_to_cta(smem_u32(&acc_empty[buf]), 0);
         const uint32_t at = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * Cfg::BUF_COLS + h * Cfg::COLS;
+        if (kb == t.k0) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          if (c < chunks) {
-            uint32_t ld[32];
-            tmem_ld_32x32(at + c * 32, ld);
-            tmem_ld_wait();
-            if (kb == t.k0) {
+          for (int c = 0; c < CHUNKS; ++c)
+            if (c < chunks) tmem_ld_32x32(at + c * 32, reinterpret_cast<uint32_t(&)[32]>(sum[c]));
+          tmem_ld_wait();
+        } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) sum[c][e] = __uint_as_float(ld[e]);
-            } else {
+          for (int c = 0; c < CHUNKS; ++c) {
+            if (c < chunks) {
+              uint32_t ld[32];
+              tmem_ld_32x32(at + c * 32, ld);
+              tmem_ld_wait();
 #pragma unroll
               for (int e = 0; e < 32; ++e) sum[c][e] += __uint_as_float(ld[e]);
             }
@@ -691,6 +706,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       }
       return true;
     });
+    if (WIDE && MODE == ENTROPY_OUT_W && lane == 0) tma_store_wait_all();
   }
 
   // ------------------------------------------------------------------ teardown

@@ -391,14 +391,24 @@ int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t st
 constexpr int kDrainLogits = 8;
 constexpr int kDrainOut = 256;  // (of results that are rounded to 16 bits; 2^-14 of the sum is cut off by then)
 
+// Up to so many k-blocks the 32-bit results of OUT_W leave through TMA: dW alone of 50000 x 2048 with 16 rows 208 -> 184 us, 64: 217 -> 201, 128: 367 -> 360.  (With more
+// rows their planes take the shared memory; 16-bit results gain nothing, 112 and 116.)
+constexpr int kBoxed = 2;
+
 int pairs_in_all() { return std::max(1, device_sms() / 2); }
 
 template <class Cfg>
 int launch_products(const Matrix& a, const Matrix& b, EntropyParams p, int type, Launches& launch) {
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb, to;
   int rc = Cfg::A_MN ? make_map(&ta, a, 64, Cfg::BK, type) : make_map(&ta, a, Cfg::BK, Cfg::BM, type);
   if (rc == TRITURUS_B200_OK) rc = Cfg::B_MN ? make_map(&tb, b, 64, Cfg::BK, type) : make_map(&tb, b, Cfg::BK, Cfg::BNH, type);
   if (rc != TRITURUS_B200_OK) return rc;
+  to = ta;  // (not used)
+  if (p.boxed) {
+    const Matrix out = {p.out, p.rows, p.cols, p.out_pitch, p.rows * p.out_pitch, 1, true};
+    rc = make_map(&to, out, 32, 32, type);
+    if (rc != TRITURUS_B200_OK) return rc;
+  }
   const auto kern = entropy_kernel<Cfg>;
   static std::atomic<bool> known[64];
   int dev = 0;
@@ -416,7 +426,7 @@ int launch_products(const Matrix& a, const Matrix& b, EntropyParams p, int type,
   p.drain = Cfg::MODE == ENTROPY_STATS || Cfg::MODE == ENTROPY_PROB ? kDrainLogits : kDrainOut;
   p.idesc = umma_idesc_16(2 * Cfg::BM, p.half != 0, Cfg::A_MN, Cfg::B_MN);
   const int64_t pairs = std::min<int64_t>(p.whole + static_cast<int64_t>(p.shared) * p.splits, pairs_in_all());
-  return launch(kern, 2 * pairs, Cfg::NTHREADS, Cfg::SMEM_BYTES, ta, tb, p);
+  return launch(kern, 2 * pairs, Cfg::NTHREADS, Cfg::SMEM_BYTES, ta, tb, to, p);
 }
 template <int MODE>
 int run_products(const Matrix& a, const Matrix& b, const EntropyParams& p, int type, Launches& launch) {
@@ -885,6 +895,7 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
     }
     if (dweight != nullptr && rc == TRITURUS_B200_OK) {
       EntropyParams q = out(plan.w[last], static_cast<char*>(dweight) + first * width * size, DEST_FINAL);
+      q.boxed = size == 4 && q.out_vec && q.kblocks <= kBoxed;
       rc = set_whole(q) ? run_products<ENTROPY_OUT_W>(md, mx, q, type, launch) : TRITURUS_B200_EINVAL;
     }
   }
