@@ -195,6 +195,28 @@ def test_few_rows_and_pieces_of_the_symbols(kind):
     check(*inputs(64, 1_500_001 if kind == torch.float32 else 4_300_001, 8, kind))
 
 
+@pytest.mark.parametrize("kind", KINDS[1:], ids=IDS[1:])
+@pytest.mark.parametrize("n", [6, 70, 333])
+def test_common_factors_are_not_rounded(n, kind):
+    """Where the targets have no probability the gradient of a row is -dloss / n of its target's row, however dloss and 1 / n are rounded to 16 bits: d is exact then, four
+    roundings in 32 bits and half a step of the result are left, and the n symbols of probability e^-32 < 2^-46."""
+    v, d = n + 1, 64
+    w = torch.zeros(v, d, device="cuda")
+    x = torch.zeros(n, d, device="cuda")
+    w[n, 0] = 32.0  # the last symbol has all of the probability
+    x[:, 0] = 1.0
+    w[:n, 1:] = rand(n, d - 1)
+    w, x = w.to(kind), x.to(kind)
+    t = torch.arange(n, device="cuda")
+    loss, lse = tb.linear_cross_entropy(x, w, t, return_lse=True)
+    dloss = torch.tensor(0.3, device="cuda")
+    dx, _ = tb.linear_cross_entropy_backward(dloss, x, w, t, lse)
+    g = float(dloss) / n
+    want = -g * w[:n, 1:].double()
+    rest = n * 2.0**-46 * g * float(w[:n, 1:].abs().max())
+    assert bool(((dx[:, 1:].double() - want).abs() <= (HALF[kind] + 5 * U) * want.abs() + rest + LEAST[kind]).all())
+
+
 @pytest.mark.parametrize("n", [16, 80])
 def test_large_offsets(n):
     """A table beyond 2^31 elements: its last rows are read and their gradients written at 64-bit offsets."""

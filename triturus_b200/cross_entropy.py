@@ -106,7 +106,7 @@ def linear_cross_entropy_backward(
 
     With g the share of dloss in each position (0 for ignored ones) and d = g (exp(z - lse) - [target]): dx = d weight, dweight = d^T x, of x's type;
     None where `x_grad` or `weight_grad` is False.  The logits are computed once more, for a piece of the symbols at a time, and d is rounded
-    to 16 bits for its two products where x has 16: to bfloat16, or to float16 relative to the largest finite |dloss|.  What x holds in ignored
+    to 16 bits for its two products where x has 16, without what is common to all positions: in float16 relative to the largest finite |dloss|.  What x holds in ignored
     positions does not count, NaN or not; dx is zero there.  Sums are in 32 bits in a fixed order.  The results carry no graph."""
     code = _reduction("linear_cross_entropy_backward", reduction)
     if not torch.compiler.is_compiling():

@@ -314,7 +314,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
         count += __shfl_xor_sync(0xffffffffu, count, o);
       }
-      const float2 f = entropy_factors(largest, count, p.mean, p.e.half);
+      const float2 f = entropy_factors(largest, count, p.mean, entropy_scale(Cfg::WIDE, p.e.half, p.e.per_row));
       factor = f.x;
       if (blockIdx.x == 0 && threadIdx.x == 128) p.e.factors[1] = f.y;  // for the products that follow
     }

@@ -155,13 +155,16 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
 __device__ __forceinline__ uint32_t plane_bits(float x0, float x1) { return __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632); }
 __device__ __forceinline__ float plane_rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-// What dloss is multiplied by in d, and what dx and dW are multiplied by, for the largest finite |dloss| and the number of targets that are not ignored.  In
-// float16 d is scaled so that the largest |dloss| stands for 2^15: |d| is at most that, and a probability of 2^-29 still has all of its digits.
-__device__ __forceinline__ float2 entropy_factors(float top, int count, int mean, int half) {
+// What the largest |dloss| stands for in d; 0: dloss as it is, times the share of a position.  What is common to all positions is rounded with each d, the same way
+// each time (1/6 of "mean" in bfloat16 by 0.1 %, and with it the gradients of a few positions), so 16-bit d leave it to their products.  In float16 the
+// largest is 2^15, so that a probability of 2^-29 still has all of its digits; of bfloat16 one for each position keeps its own, and its range.
+__host__ __device__ constexpr float entropy_scale(bool wide, int half, int per_row) { return wide ? 0.f : half ? 32768.f : per_row ? 0.f : 1.f; }
+// What dloss is multiplied by in d, and what dx and dW are multiplied by, for the largest finite |dloss| and the number of targets that are not ignored.
+__device__ __forceinline__ float2 entropy_factors(float top, int count, int mean, float scale) {
   const float share = mean ? 1.f / static_cast<float>(max(count, 1)) : 1.f;
-  if (!half) return make_float2(share, 1.f);
+  if (scale == 0.f) return make_float2(share, 1.f);
   top = top == 0.f ? 1.f : fmaxf(top, 0x1p-100f);
-  return make_float2(32768.f / top, top * share * 0x1p-15f);
+  return make_float2(scale / top, top * share * (1.f / scale));
 }
 
 __device__ __forceinline__ int64_t entropy_target(const EntropyParams& p, int64_t row) {
@@ -560,7 +563,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             }
           }
         } else {
-          if (!WIDE && p.half) {
+          if (!WIDE) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] *= alpha;
           }

@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(1024) entropy_join_kernel(const JoinArgs p) {
 
 // factors[0] and [1]: see entropy_factors.
 __global__ void __launch_bounds__(1024) entropy_factors_kernel(const float* dloss, int per_row, const void* target, int target_wide, int64_t ignore, int rows,
-                                                               int mean, int half, float* factors) {
+                                                               int mean, float scale, float* factors) {
   __shared__ float top_of[32];
   __shared__ int count_of[32];
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(1024) entropy_factors_kernel(const float* dlos
     top = fmaxf(top, top_of[w]);
     count += count_of[w];
   }
-  const float2 f = entropy_factors(top, count, mean, half);
+  const float2 f = entropy_factors(top, count, mean, scale);
   factors[0] = f.x;
   factors[1] = f.y;
 }
@@ -831,9 +831,11 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
   int rc = prepare(&mx, x, rows, width, x_stride, reading_of(rows, type, false, mask), space.x, launch);
   if (rc == TRITURUS_B200_OK) rc = prepare(&mw, weight, symbols, width, weight_stride, reading_of(rows, type, true), space.weight, launch);
   const int wide = target_bytes == 8;
+  const int per_row = reduction == TRITURUS_B200_REDUCTION_NONE ? 1 : 0;
   if (rc == TRITURUS_B200_OK && !is_few)
-    rc = launch(entropy_factors_kernel, 1, 1024, 0, dloss, reduction == TRITURUS_B200_REDUCTION_NONE ? 1 : 0, target, wide, ignore_index,
-                   static_cast<int>(rows), reduction == TRITURUS_B200_REDUCTION_MEAN ? 1 : 0, type == TRITURUS_B200_TYPE_F16 ? 1 : 0, space.factors);
+    rc = launch(entropy_factors_kernel, 1, 1024, 0, dloss, per_row, target, wide, ignore_index, static_cast<int>(rows),
+                reduction == TRITURUS_B200_REDUCTION_MEAN ? 1 : 0, entropy_scale(type == TRITURUS_B200_TYPE_F32, type == TRITURUS_B200_TYPE_F16 ? 1 : 0, per_row),
+                space.factors);
   Matrix md = {};
   md.data = space.d;
   md.rows = rows;
@@ -852,7 +854,7 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
     p.symbols = symbols;
     p.lse = lse;
     p.dloss = dloss;
-    p.per_row = reduction == TRITURUS_B200_REDUCTION_NONE;
+    p.per_row = per_row;
     p.factors = space.factors;
     p.d = space.d;
     p.d_pitch = md.pitch;
