@@ -231,3 +231,40 @@ def test_streams_and_graphs():
     want = tb.embedding(tokens, weight, scale=3.0), tb.embedding_backward(dy, tokens, 200, padding_idx=1)
     for _, got in graphs:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_few_positions_in_graphs():
+    """The form without a sort, captured twice and replayed in turn on other symbols and gradients, and beside itself on two streams."""
+    tokens, dy = draw_tokens(300, 200), rand(300, 64)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = tb.embedding_backward(dy, tokens, 200, padding_idx=1)
+        graphs.append((graph, got))
+    tokens.copy_(tokens.flip(0))
+    dy.copy_(dy.flip(0).clone())
+    want = check_backward(dy, tokens, 200, padding=1)
+    for graph, got in graphs + graphs:
+        got.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    out = []
+    for s in streams * 4:
+        with torch.cuda.stream(s):
+            out.append(tb.embedding_backward(dy, tokens, 200, padding_idx=1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) for a in out)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_strides_of_sorted_positions(kind):
+    """Views of more rows than the form without a sort takes, at odd distances and elements, and at the ends of an allocation of their own."""
+    tokens = draw_tokens(1100, 60)
+    d = rand(2200, 120, kind=kind)
+    for dy in (d[:1100, 3:106], d[::2, :64], d[1099:2199, 1:120], d[:1, :80].expand(1100, 80), d[:1100, ::3]):
+        check_backward(dy, tokens, 60)
+    for offset in (1, 3):
+        check_backward(rand(offset + 1100 * 37, kind=kind)[offset:].view(1100, 37), tokens, 60)
