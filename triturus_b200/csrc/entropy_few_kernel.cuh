@@ -33,7 +33,7 @@ struct FewCfg {
   static constexpr int A_COLS = 3 * BK / 2;  // of a stage
   static constexpr int TMEM_COLS = WIDE ? 512 : 128;
   static constexpr int NBAR = 2 * NSA + 2 * NSB + 8;
-  static constexpr int SMEM_BYTES = 1024 + NSA * A_TILE + NSB * B_TILE + NBAR * 8 + 16 + EPI_WARPS * 32 * 20;
+  static constexpr int SMEM_BYTES = 1024 + NSA * A_TILE + NSB * B_TILE + NBAR * 8 + 16 + EPI_WARPS * 32 * 16;
   static_assert(SMEM_BYTES <= 232448, "shared memory capacity");
 };
 
@@ -122,7 +122,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cut_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* of_done = reinterpret_cast<int*>(tmem_slot + 2);          // [2] STATS: warps of a half of the rows that have left their part
-  uint8_t* of_rows = reinterpret_cast<uint8_t*>(tmem_slot + 4);  // [8][32 * 20] PROB: what each epilogue warp needs of its rows of x
+  uint8_t* of_rows = reinterpret_cast<uint8_t*>(tmem_slot + 4);  // [8][32 * 16] PROB: what each epilogue warp needs of its rows of x
   float2* of_stats = reinterpret_cast<float2*>(of_rows);         // [8][32] STATS: those parts
 
   const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
@@ -294,10 +294,9 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     float sum[32];
     float top = -INFINITY, total = 0.f;  // STATS: of row h * 32 + lane of x, over the warp's symbols of the unit
     const float alpha = MODE == ENTROPY_OUT_X ? p.e.factors[1] : 1.f;
-    int64_t* of_target = reinterpret_cast<int64_t*>(of_rows + (warp - 4) * (32 * 20));
+    int64_t* of_target = reinterpret_cast<int64_t*>(of_rows + (warp - 4) * (32 * 16));
     float* of_lse = reinterpret_cast<float*>(of_target + 32);
-    float* of_lse2 = of_lse + 32;
-    float* of_g = of_lse2 + 32;
+    float* of_g = of_lse + 32;
 
     float factor = 1.f;
     if constexpr (MODE == ENTROPY_PROB) {  // (few rows: each warp finds this for itself)
@@ -338,7 +337,6 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           __syncwarp();
           of_target[lane] = ignored ? -1 : to - p.e.b_row;
           of_lse[lane] = ignored ? INFINITY : lse;  // (no lse is that: infinite logits make it NaN)
-          of_lse2[lane] = lse * LOG2E_F;
           of_g[lane] = ignored ? 0.f : to < 0 || to >= p.e.symbols ? __int_as_float(0x7fc00000) : p.e.dloss[p.e.per_row ? n + lane : 0] * factor;
           __syncwarp();
         }
@@ -401,8 +399,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           for (int e = 0; e < 32; ++e) {
             if (e < count) {
               const float lse = of_lse[e], g = of_g[e];
-              float x = WIDE ? ex2_approx((sum[e] - lse) * LOG2E_F) : ex2_approx(fmaf(sum[e], LOG2E_F, -of_lse2[e]));
-              x = lse == INFINITY ? 0.f : x * g;
+              float x = lse == INFINITY ? 0.f : exp_shifted(sum[e], lse) * g;
               if (of_target[e] == m) x -= g;
               if constexpr (WIDE) {
 #pragma unroll

@@ -446,7 +446,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     float sum[CHUNKS][32];  // what the accumulators of a tile add up to
 
     // of the unit's row (STATS), of the tile's row (PROB)
-    float top = -INFINITY, total = 0.f, lse = 0.f, lse2 = 0.f, g = 0.f;
+    float top = -INFINITY, total = 0.f, lse = 0.f, g = 0.f;
     int64_t target = -1;
     bool ignored = false;
     const float alpha = MODE == ENTROPY_OUT_X || MODE == ENTROPY_OUT_W ? p.factors[1] : 1.f;
@@ -525,15 +525,25 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 #pragma unroll
           for (int e = 4; e < 32; ++e) m[e & 3] = fmaxf(m[e & 3], v[e]);
           const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top);
-          const float base = now == -INFINITY ? 0.f : now, base2 = base * LOG2E_F;
+          const float base = now == -INFINITY ? 0.f : now;
           float s[4] = {total * ex2_approx((top - base) * LOG2E_F), 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e & 3] += ex2_approx(WIDE ? (v[e] - base) * LOG2E_F : fmaf(v[e], LOG2E_F, -base2));
+          for (int e = 0; e < 32; e += 2) {
+            float e0, e1;
+            exp_shifted_x2(v[e], v[e + 1], base, e0, e1);  // (multiplied first, a maximum from 1.5e9 on has an exponential of 0 or infinity)
+            s[e & 3] += e0;
+            s[(e + 1) & 3] += e1;
+          }
           total = (s[0] + s[1]) + (s[2] + s[3]);
           top = now;
         } else if constexpr (MODE == ENTROPY_PROB) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = ex2_approx(WIDE ? (v[e] - lse) * LOG2E_F : fmaf(v[e], LOG2E_F, -lse2)) * g;
+          for (int e = 0; e < 32; e += 2) {
+            float e0, e1;
+            exp_shifted_x2(v[e], v[e + 1], lse, e0, e1);
+            v[e] = e0 * g;
+            v[e + 1] = e1 * g;
+          }
           const int at = target >= c0 && target < c0 + 32 ? static_cast<int>(target) - c0 : -1;
           if (__any_sync(0xffffffffu, ignored || at >= 0)) {
 #pragma unroll
@@ -690,7 +700,6 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           ignored = own == p.ignore;
           target = ignored ? -1 : own - p.b_row;
           lse = own_lse;
-          lse2 = own_lse * LOG2E_F;
           g = ignored ? 0.f : own < 0 || own >= p.symbols ? __int_as_float(0x7fc00000) : own_dloss * factor;
         }
       }
