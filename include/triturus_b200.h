@@ -368,7 +368,8 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
  * Its gradients for dloss ([rows] or one number, as loss is) and the lse of the forward call, with d[i, v] = g_i (exp(z[i, v] - lse[i]) - [v = target_i])
  * and g the share of dloss (0 for ignored targets, NaN for those outside): dx = d weight [rows, width], dweight = d^T x [symbols, width], back to
  * back and of `type`; either may be NULL.  d is computed for a piece of the symbols at a time, 2^28 numbers or, for many rows, 256 symbols, and rounded to
- * 16 bits where the operands have 16, without what is common to all positions; in float16 relative to the largest finite |dloss|.  What x holds in rows of ignored targets does not count.
+ * 16 bits where the operands have 16, without what is common to all positions; in float16 relative to the largest finite |dloss|.  What x holds in rows of ignored targets does not count,
+ * and dx is zero there whatever weight holds; elsewhere an infinite element of weight makes its column of dx NaN (0 times infinity).
  */
 size_t triturus_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width,
                                                                    int64_t x_stride, int64_t weight_stride, int type);

@@ -341,6 +341,8 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           __syncwarp();
         }
       }
+      unsigned ignored = 0;  // OUT_X: rows whose d is zero, which 0 times an infinite weight is not
+      if constexpr (MODE == ENTROPY_OUT_X) ignored = __ballot_sync(0xffffffffu, lane < count && entropy_target(p.e, n + lane) == p.e.ignore);
       for (int kb = t.k0; kb < t.k1; kb += drain, ++accs) {
         const uint32_t buf = accs & 1;
         if (!mbar_wait_warp(&acc_full[buf], (accs >> 1) & 1, ctl, STATUS_TIMEOUT_EPILOGUE)) return false;
@@ -419,7 +421,7 @@ entropy_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           float* part = p.e.part + (static_cast<int64_t>(t.ks) * p.rows + n) * p.e.sum_pitch + m;
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            if (e < count) part[e * p.e.sum_pitch] = sum[e] * alpha;
+            if (e < count) part[e * p.e.sum_pitch] = ignored >> e & 1 ? 0.f : sum[e] * alpha;
           }
         }
       }

@@ -86,11 +86,11 @@ struct EntropyParams {
   float2* stats;
   float* picked;
   int* arrived;           // set to zero for the launch that joins them
-  // STATS and PROB
+  // STATS, PROB and OUT_X
   const void* target;
   int target_wide;        // 64 bits
   int64_t ignore;
-  int64_t symbols;
+  int64_t symbols;        // (not OUT_X)
   // PROB
   const float* lse;
   const float* dloss;     // [rows], or one number
@@ -469,6 +469,9 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           }
         }
       }
+      if constexpr (MODE == ENTROPY_OUT_X) {
+        if (valid) own = entropy_target(p, row);
+      }
       // chunks of 32 columns that this thread has in the tile
       const bool rows_exist = t.tm * (2 * BM) + static_cast<int>(rank) * BM < p.rows;
       const int chunks = rows_exist ? max(0, min(CHUNKS, (t.n1 - col0 + 31) >> 5)) : 0;
@@ -576,6 +579,12 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           if (!WIDE) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] *= alpha;
+          }
+          if constexpr (MODE == ENTROPY_OUT_X) {
+            if (__any_sync(0xffffffffu, ignored)) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = ignored ? 0.f : v[e];  // (d is zero there, and 0 times an infinite weight is not)
+            }
           }
           const auto as_bits = [&](int e) { return __float_as_uint(v[e]); };
           const auto store_floats = [&](float* to) {  // scratch memory, whose rows are on sectors
@@ -703,6 +712,7 @@ entropy_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           g = ignored ? 0.f : own < 0 || own >= p.symbols ? __int_as_float(0x7fc00000) : own_dloss * factor;
         }
       }
+      if constexpr (MODE == ENTROPY_OUT_X) ignored = own == p.ignore;
 #pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
         float v[32];

@@ -871,6 +871,9 @@ int triturus_b200_linear_cross_entropy_backward(const float* dloss, const void* 
     md.width = piece;
     const auto out = [&](EntropyParams q, void* to, int dest) {
       q.factors = space.factors;
+      q.target = target;
+      q.target_wide = wide;
+      q.ignore = ignore_index;
       q.dest = dest;
       q.out = to;
       q.out_pitch = width;
