@@ -62,3 +62,23 @@ def test_gradients_with_impossible_symbols(n, kind):
     for name, got, e, b in zip(("loss", "lse", "dx", "dweight"), (loss, lse, dx[:, 1:], dw[1::2]), want, bound):
         e, b = (e[:, 1:], b[:, 1:]) if name == "dx" else (e, b)
         assert bool(((got.double() - e).abs() <= b).all()), name
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("n", [60, 300])
+def test_losses_that_are_no_numbers(n, kind):
+    """Such a dloss reaches dx of all positions that count and of none that are ignored, and dweight; one of them for a single position reaches that row alone."""
+    x, w, t = inputs(n, 1000, 64, kind)
+    t[::9] = IGNORE
+    lse = tb.linear_cross_entropy(x, w, t, return_lse=True)[1]
+    for bad in (INF, -INF, NAN):
+        dx, dw = tb.linear_cross_entropy_backward(torch.tensor(bad, device="cuda"), x, w, t, lse)
+        assert not dx[t != IGNORE].isfinite().any()
+        assert not dx[t == IGNORE].any()
+        assert not dw.isfinite().any()
+        dloss = torch.ones(n, device="cuda")
+        dloss[5] = bad
+        dx, dw = tb.linear_cross_entropy_backward(dloss, x, w, t, lse, reduction="none")
+        assert int(t[5]) != IGNORE and not dx[5].isfinite().any()
+        assert bool(dx[:5].isfinite().all()) and bool(dx[6:].isfinite().all()) and bool(dx[6:].any())
+    tb.check_status()
