@@ -39,6 +39,7 @@ constexpr int kDirect = 1024;
 constexpr int64_t kDirectBlocks = 4096;
 constexpr int kDirectThreads = 256;
 constexpr int kDirectLanes = 64;
+constexpr int kMostSlabs = 65535;    // of a row, in the second dimension of a grid
 constexpr int kJoins = 2;            // groups of them that add the parts of a run
 
 // A symbol of a list of 64- or 32-bit ones.
@@ -335,6 +336,7 @@ struct SumArgs {
   int64_t stride, pitch;  // pitch: a multiple of eight
   int count, symbols, width, tile, lanes;
   int slots;  // vectors of a row, and one more where rows are off 16-byte boundaries
+  int slab;   // of the launch's first blocks: of `lanes` (or, the same where it is not 0, kGroup) vectors of a row
   int base;   // elements that the table's first is behind such a boundary
   float scale;
 };
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kGroup) embedding_sum_kernel(const SumArgs p) 
   constexpr int N = Pack<T, 16>::N, kAhead = 4;  // rows of a thread under way (65536 x 4096 bfloat16, the whole step: 424 us, 8: 446, 16: 500)
   const int groups = kGroup / p.lanes;
   const int64_t tile = static_cast<int64_t>(blockIdx.x) * groups + threadIdx.x / p.lanes;
-  const int slot = static_cast<int>(blockIdx.y) * p.lanes + (static_cast<int>(threadIdx.x) & (p.lanes - 1));
+  const int slot = (p.slab + static_cast<int>(blockIdx.y)) * p.lanes + (static_cast<int>(threadIdx.x) & (p.lanes - 1));
   const int64_t first = tile * p.tile;
   pdl_launch_dependents();
   pdl_wait();
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(kGroup * kJoins) embedding_join_kernel(const S
   const int group = static_cast<int>(threadIdx.x) / kGroup, lane = static_cast<int>(threadIdx.x) % kGroup;
   const bool alone = tiles < 4 * kJoins;
   if (alone && group != 0) return;
-  const int slot = static_cast<int>(blockIdx.y) * kGroup + lane;
+  const int slot = (p.slab + static_cast<int>(blockIdx.y)) * kGroup + lane;
   const bool mine = slot < p.slots;
   alignas(16) float acc[N] = {};
   const float4* part = reinterpret_cast<const float4*>(p.part + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * p.pitch + slot * N);
@@ -805,14 +807,17 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
   p.part = reinterpret_cast<float*>(ws + 4 * space.list + space.counts);
   p.lanes = lanes_for(p.slots, kGroup);
   const int64_t tiles = (count + p.tile - 1) / p.tile, groups = kGroup / p.lanes;
-  const unsigned slabs = static_cast<unsigned>((p.slots + p.lanes - 1) / p.lanes);
-  if (slabs > 65535) return TRITURUS_B200_EINVAL;
+  const int slabs = (p.slots + p.lanes - 1) / p.lanes;
   return by_type(type, [&](auto t) {
     using T = decltype(t);
     const cudaLaunchAttribute dependent = dependent_launch();
-    int code = launch_of(aligned ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), slabs), kGroup, 0, st, &dependent, p);
-    if (code == TRITURUS_B200_OK && tiles > 1)
-      code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>((p.slots + kGroup - 1) / kGroup)), kGroup * kJoins, 0, st, &dependent, p);
+    int code = TRITURUS_B200_OK;
+    for (p.slab = 0; p.slab < slabs && code == TRITURUS_B200_OK; p.slab += kMostSlabs) {
+      const unsigned here = static_cast<unsigned>(std::min(slabs - p.slab, kMostSlabs));
+      code = launch_of(aligned ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>, dim3(static_cast<unsigned>((tiles + groups - 1) / groups), here), kGroup, 0, st, &dependent, p);
+      if (code == TRITURUS_B200_OK && tiles > 1)
+        code = launch_of(embedding_join_kernel<T>, dim3(static_cast<unsigned>(tiles), here), kGroup * kJoins, 0, st, &dependent, p);
+    }
     return code;
   });
 }
