@@ -11,6 +11,7 @@ import warnings
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import build as _build
 
@@ -729,6 +730,12 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     return t.contiguous(), D
 
 
+def _refuse_tangents(name: str, *tensors: torch.Tensor) -> None:
+    """For a result that carries no graph, in which they would be lost."""
+    if any(unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: a tensor with a forward-mode tangent is not supported")
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -965,6 +972,7 @@ def _embedding_impl(tokens: torch.Tensor, weight: torch.Tensor, scale: float) ->
 
 def _embedding_backward_impl(dy: torch.Tensor, tokens: torch.Tensor, symbols: int, scale: float, padding_idx: int | None) -> torch.Tensor:
     _require_cuda(dy)
+    _refuse_tangents("embedding_backward", dy)
     width, count, symbols = dy.shape[-1], tokens.numel(), int(symbols)
     dweight = torch.empty((symbols, width), dtype=dy.dtype, device=dy.device)
     tokens = tokens.contiguous()
@@ -1043,6 +1051,7 @@ def _linear_cross_entropy_backward_impl(
 ) -> tuple[torch.Tensor, torch.Tensor]:  # fmt: skip
     """Gradients that are not wanted are empty tensors."""
     _require_cuda(x)
+    _refuse_tangents("linear_cross_entropy_backward", dloss, x, weight, lse)
     symbols, width = weight.shape
     dx = torch.empty(x.shape if x_grad else (0,), dtype=x.dtype, device=x.device)
     dweight = torch.empty(weight.shape if weight_grad else (0,), dtype=x.dtype, device=x.device)

@@ -108,7 +108,8 @@ def linear_cross_entropy_backward(
     None where `x_grad` or `weight_grad` is False.  The logits are computed once more, for a piece of the symbols at a time, and d is rounded
     to 16 bits for its two products where x has 16, without what is common to all positions: in float16 relative to the largest finite |dloss|.  What x holds in ignored
     positions does not count, NaN or not; dx is zero there, whatever weight holds.  An infinite element of weight makes its column of dx NaN in the other positions, 0 times infinity, also
-    where it makes a symbol impossible (in float32, which counts it as NaN, all columns).  Sums are in 32 bits in a fixed order.  The results carry no graph."""
+    where it makes a symbol impossible (in float32, which counts it as NaN, all columns).  Sums are in 32 bits in a fixed order.  The results carry no graph, and
+    tensors with a forward-mode tangent are refused."""
     code = _reduction("linear_cross_entropy_backward", reduction)
     if not torch.compiler.is_compiling():
         out = _native.HOST.linear_cross_entropy_backward(

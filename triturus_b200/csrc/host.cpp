@@ -451,7 +451,7 @@ PyObject* embedding_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   const int type = type_code(*dy);
   const int64_t stride = row_stride(*dy), width = dy->size(-1);
   if (tokens == nullptr || type < 0 || stride < 0 || tokens->sizes() != dy->sizes().slice(0, dy->dim() - 1) ||
-      !padding_arg(args[4], symbols, &padding))
+      !padding_arg(args[4], symbols, &padding) || has_tangent(dy))
     return none();
   const int64_t count = tokens->numel();
   const size_t bytes = triturus_b200_embedding_backward_workspace_bytes(count, symbols, width, type);
@@ -550,7 +550,7 @@ PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssi
   const at::Tensor* lse = plain_object(args[4]);
   if (dloss == nullptr || lse == nullptr) return none();
   for (const at::Tensor* t : {dloss, lse})
-    if (t->scalar_type() != at::kFloat || !t->is_contiguous() || t->device() != o.x->device()) return none();
+    if (t->scalar_type() != at::kFloat || !t->is_contiguous() || t->device() != o.x->device() || has_tangent(t)) return none();
   if (lse->sizes() != o.target->sizes() || dloss->sizes() != (reduction == TRITURUS_B200_REDUCTION_NONE ? o.target->sizes() : at::IntArrayRef())) return none();
   const bool want_x = args[7] == Py_True, want_weight = args[8] == Py_True;
   at::Tensor dx, dweight;

@@ -66,7 +66,8 @@ def embedding_backward(
     scale * sum of dy over the positions of symbol v, zero where there is none and for v = padding_idx.
 
     Of dy's type; the sums are in 32 bits, taken in an order that depends on `tokens` alone, so that the same call gives the same result.
-    The positions are sorted by symbol on the device, or compared with each other where there are few.  The result carries no graph."""
+    The positions are sorted by symbol on the device, or compared with each other where there are few.  The result carries no graph, and a tensor with a
+    forward-mode tangent is refused."""
     if not torch.compiler.is_compiling():
         out = _native.HOST.embedding_backward(dy, tokens, symbols, scale, padding_idx)
         if out is not None:
