@@ -9,6 +9,7 @@ import ctypes
 import os
 import warnings
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from numbers import Integral
 
 import torch
 from torch.autograd.forward_ad import unpack_dual
@@ -730,6 +731,10 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     return t.contiguous(), D
 
 
+def _whole(n) -> bool:
+    return isinstance(n, (Integral, torch.SymInt)) or (isinstance(n, float) and n.is_integer())
+
+
 def _refuse_tangents(name: str, *tensors: torch.Tensor) -> None:
     """For a result that carries no graph, in which they would be lost."""
     if any(unpack_dual(t).tangent is not None for t in tensors):
@@ -1038,7 +1043,7 @@ def _linear_cross_entropy_impl(
         nbytes = int(LIB.triturus_b200_linear_cross_entropy_workspace_bytes(xr.data_ptr(), wr.data_ptr(), *sizes))
         space = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
         rc = LIB.triturus_b200_linear_cross_entropy(
-            xr.data_ptr(), wr.data_ptr(), target.data_ptr(), target.element_size(), loss.data_ptr(), lse.data_ptr(), *sizes, reduction, ignore_index,
+            xr.data_ptr(), wr.data_ptr(), target.data_ptr(), target.element_size(), loss.data_ptr(), lse.data_ptr(), *sizes, reduction, int(ignore_index),
             space.data_ptr(), nbytes, _status_word(x.device).data_ptr(), _raw_stream(idx),
         )  # fmt: skip
     _check(rc, "triturus_b200_linear_cross_entropy")
@@ -1063,7 +1068,7 @@ def _linear_cross_entropy_backward_impl(
         space = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
         rc = LIB.triturus_b200_linear_cross_entropy_backward(
             dloss.data_ptr(), xr.data_ptr(), wr.data_ptr(), target.data_ptr(), target.element_size(), lse.data_ptr(),
-            _ptr(dx) if x_grad else None, _ptr(dweight) if weight_grad else None, *sizes, reduction, ignore_index,
+            _ptr(dx) if x_grad else None, _ptr(dweight) if weight_grad else None, *sizes, reduction, int(ignore_index),
             space.data_ptr(), nbytes, _status_word(x.device).data_ptr(), _raw_stream(idx),
         )  # fmt: skip
     _check(rc, "triturus_b200_linear_cross_entropy_backward")

@@ -32,8 +32,8 @@ def _check_operands(name: str, x: torch.Tensor, weight: torch.Tensor, target: to
     assert x.device == weight.device == target.device
     if weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"{name}: a weight of {weight.shape[0]} rows of {weight.shape[1]} elements is not supported")
-    if not -(2**63) <= ignore_index < 2**63:
-        raise ValueError(f"{name}: ignore_index is out of range, got {ignore_index!r}")
+    if not (_native._whole(ignore_index) and -(2**63) <= ignore_index < 2**63):
+        raise ValueError(f"{name}: ignore_index must be a whole number of 64 bits, got {ignore_index!r}")
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int) -> None:

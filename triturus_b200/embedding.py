@@ -31,12 +31,14 @@ def _check_backward(dy: torch.Tensor, tokens: torch.Tensor, symbols: int, scale:
 
 
 def _check_numbers(name: str, symbols: int, width: int, scale: float, padding_idx: int | None) -> None:
+    if not _native._whole(symbols):
+        raise ValueError(f"{name}: symbols must be a whole number, got {symbols!r}")
     if symbols < 1 or width < 1:
         raise ValueError(f"{name}: a table of {symbols} rows of {width} elements is not supported")
     if not (math.isfinite(scale) and abs(scale) <= torch.finfo(torch.float32).max):
         raise ValueError(f"{name}: scale must be a finite number of 32 bits, got {scale!r}")
-    if padding_idx is not None and not 0 <= padding_idx < symbols:
-        raise ValueError(f"{name}: padding_idx is out of range, got {padding_idx!r}")
+    if padding_idx is not None and not (_native._whole(padding_idx) and 0 <= padding_idx < symbols):
+        raise ValueError(f"{name}: padding_idx is no symbol of the table, got {padding_idx!r}")
 
 
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
