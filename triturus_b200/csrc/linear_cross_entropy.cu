@@ -313,16 +313,16 @@ struct Reading {
   Mask mask;  // x of the gradients: dW multiplies it with d, and what a position without a loss holds (it may be NaN) must not count
 };
 Reading reading_of(int64_t rows, int type, bool weight, Mask mask = {});
-// Whether an operand is read where it lies: rows on 16-byte boundaries (or lines), and 32-bit elements only as they are.
-bool in_place(const void* data, int64_t rows, int64_t stride, const Reading& how) {
+// Whether an operand is read where it lies: rows on 16-byte boundaries (or lines) that do not overlap, and 32-bit elements only as they are.
+bool in_place(const void* data, int64_t rows, int64_t width, int64_t stride, const Reading& how) {
   if ((how.type == TRITURUS_B200_TYPE_F32 && !how.raw) || how.mask.target != nullptr) return false;
   const int64_t unit = how.lines ? 128 : 16;
-  return aligned_to(data, unit) && (rows == 1 || (stride > 0 && stride * size_of(how.type) % unit == 0 && stride < (1ll << 37)));
+  return aligned_to(data, unit) && (rows == 1 || (stride >= width && stride * size_of(how.type) % unit == 0 && stride < (1ll << 37)));
 }
 // A copy's rows are on lines.
 int64_t copy_pitch(int64_t width, const Reading& how) { return up_to(width, how.raw ? 32 : 64); }
 size_t copy_bytes(const void* data, int64_t rows, int64_t width, int64_t stride, const Reading& how) {
-  if (in_place(data, rows, stride, how)) return 0;
+  if (in_place(data, rows, width, stride, how)) return 0;
   return static_cast<size_t>(rows) * static_cast<size_t>(copy_pitch(width, how)) * (how.raw ? 4 : how.type == TRITURUS_B200_TYPE_F32 ? 6 : 2);
 }
 
@@ -368,7 +368,7 @@ int prepare(Matrix* m, const void* data, int64_t rows, int64_t width, int64_t st
   m->width = width;
   m->raw = raw && type == TRITURUS_B200_TYPE_F32;
   m->planes = type == TRITURUS_B200_TYPE_F32 && !raw ? 3 : 1;
-  if (in_place(data, rows, stride, how)) {
+  if (in_place(data, rows, width, stride, how)) {
     m->data = data;
     m->pitch = rows == 1 ? up_to(width, 8) : stride;
     m->plane = rows * m->pitch;
