@@ -41,6 +41,7 @@ extern "C" {
 #define TRITURUS_B200_ELAUNCH (-5)     /* kernel launch or attribute call failed */
 #define TRITURUS_B200_EDRIVER (-6)     /* driver entry point unavailable */
 #define TRITURUS_B200_ESTATICLIMIT (-7) /* problem exceeds the built-in scratch of the *_static entry point */
+#define TRITURUS_B200_EREGISTERS (-8)   /* a kernel whose warps hand registers over was compiled to another number of them */
 
 #define TRITURUS_B200_PRECISION_TF32 0   /* one tf32 MMA pass; triturus.utils.set_tf32_enabled(True) */
 #define TRITURUS_B200_PRECISION_3XTF32 1 /* hi/lo split, ~fp32 accuracy; set_tf32_enabled(False) */

@@ -662,6 +662,7 @@ const char* triturus_b200_strerror(int code) {
     case TRITURUS_B200_ELAUNCH: return "kernel launch failed";
     case TRITURUS_B200_EDRIVER: return "cuTensorMapEncodeTiled unavailable";
     case TRITURUS_B200_ESTATICLIMIT: return "R * K exceeds the built-in scratch of the static entry point";
+    case TRITURUS_B200_EREGISTERS: return "kernel compiled to other than the 168 registers that its warps share out (built by another nvcc?)";
     case STATUS_TIMEOUT_PRODUCER: return "device: TMA producer wait timed out";
     case STATUS_TIMEOUT_TRANSFORM: return "device: transform warp wait timed out";
     case STATUS_TIMEOUT_MMA: return "device: MMA issuer wait timed out";

@@ -419,7 +419,7 @@ int launch_products(const Matrix& a, const Matrix& b, EntropyParams p, int type,
     cudaFuncAttributes about;
     rc = code_of(cudaFuncGetAttributes(&about, kern));
     if (rc != TRITURUS_B200_OK) return rc;
-    if (!Cfg::WIDE && about.numRegs != 168) return TRITURUS_B200_ELAUNCH;  // (its warps would wait for registers that nobody has)
+    if (!Cfg::WIDE && about.numRegs != 168) return TRITURUS_B200_EREGISTERS;  // (its warps would wait for registers that nobody has)
     known[dev].store(true, std::memory_order_relaxed);
   }
   p.half = type == TRITURUS_B200_TYPE_F16;
