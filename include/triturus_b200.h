@@ -354,8 +354,9 @@ int triturus_b200_embedding_backward(const void* dy, const void* tokens, int tok
  * one number: the sum, or MEAN, that sum over the number of targets that are not ignored (0 where there is none).
  * Products of 16-bit operands are exact and added in 32 bits; 32-bit operands are taken apart into three parts of 8 digits each, whose six largest
  * products give about the accuracy of 32-bit arithmetic.  An infinity among 32-bit operands counts as NaN.
- * Workspace (256-byte aligned, may hold anything): its size depends on the pointers and strides, since operands whose rows are not on 16-byte
- * boundaries, and 32-bit ones, are copied into it.  At most 2^30 of each size.  status_dev as above.
+ * Workspace (256-byte aligned, may hold anything): its size depends on the pointers and strides.  Operands are copied into it if their rows overlap or are not on
+ * 16-byte boundaries, 16-bit ones from 2048 rows of x on also if they are not on 128-byte ones, and 32-bit ones (as three parts of 16 bits) but for
+ * weight with up to 192 rows of x.  At most 2^30 of each size.  status_dev as above.
  */
 #define TRITURUS_B200_REDUCTION_NONE 0
 #define TRITURUS_B200_REDUCTION_MEAN 1
@@ -369,7 +370,8 @@ int triturus_b200_linear_cross_entropy(const void* x, const void* weight, const 
  * Its gradients for dloss ([rows] or one number, as loss is) and the lse of the forward call, with d[i, v] = g_i (exp(z[i, v] - lse[i]) - [v = target_i])
  * and g the share of dloss (0 for ignored targets, NaN for those outside): dx = d weight [rows, width], dweight = d^T x [symbols, width], back to
  * back and of `type`; either may be NULL.  d is computed for a piece of the symbols at a time, 2^28 numbers or, for many rows, 256 symbols, and rounded to
- * 16 bits where the operands have 16, without what is common to all positions; in float16 relative to the largest finite |dloss|.  What x holds in rows of ignored targets does not count,
+ * 16 bits where the operands have 16, without what is common to all positions; in float16 relative to the largest finite |dloss|.  x is copied
+ * for dweight, and has its room in the workspace in any case.  What x holds in rows of ignored targets does not count,
  * and dx is zero there whatever weight holds; elsewhere an infinite element of weight makes its column of dx NaN (0 times infinity).
  */
 size_t triturus_b200_linear_cross_entropy_backward_workspace_bytes(const void* x, const void* weight, int64_t rows, int64_t symbols, int64_t width,

@@ -333,7 +333,7 @@ struct SumArgs {
   const int32_t *keys, *at;
   void* dweight;
   float* part;  // [tiles][2][pitch], by slots: of the run that began before the tile, and of the one that goes on behind it
-  int64_t stride, pitch;  // pitch: a multiple of eight
+  int64_t stride, pitch;  // pitch: a multiple of 16 bytes of elements, so of four (32 bits) or eight
   int count, symbols, width, tile, lanes;
   int slots;  // vectors of a row, and one more where rows are off 16-byte boundaries
   int slab;   // of the launch's first blocks: of `lanes` (or, the same where it is not 0, kGroup) vectors of a row
