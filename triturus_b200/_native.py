@@ -719,7 +719,7 @@ _TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """`t` [..., D] as rows of consecutive elements at one distance, and that distance; copied where its strides are none of that."""
-    D = t.shape[-1]
+    t, D = t.resolve_neg(), t.shape[-1]  # (a view may say that its memory holds the negatives)
     if t.is_contiguous():
         return t, D
     if t.stride(-1) == 1 or D == 1:
@@ -729,6 +729,11 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
         except RuntimeError:
             pass
     return t.contiguous(), D
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """`t` with its elements one after the other in memory."""
+    return t.resolve_neg().contiguous()
 
 
 def _whole(n) -> bool:
@@ -964,7 +969,7 @@ def _embedding_impl(tokens: torch.Tensor, weight: torch.Tensor, scale: float) ->
     _require_cuda(weight)
     symbols, width = weight.shape
     y = torch.empty((*tokens.shape, width), dtype=weight.dtype, device=weight.device)
-    tokens = tokens.contiguous()
+    tokens = _flat(tokens)
     rows, stride = _rows(weight)
     with _on_device(weight.device) as idx:
         rc = LIB.triturus_b200_embedding(
@@ -980,7 +985,7 @@ def _embedding_backward_impl(dy: torch.Tensor, tokens: torch.Tensor, symbols: in
     _refuse_tangents("embedding_backward", dy)
     width, count, symbols = dy.shape[-1], tokens.numel(), int(symbols)
     dweight = torch.empty((symbols, width), dtype=dy.dtype, device=dy.device)
-    tokens = tokens.contiguous()
+    tokens = _flat(tokens)
     rows, stride = _rows(dy)
     with _on_device(dy.device) as idx:
         nbytes = int(LIB.triturus_b200_embedding_backward_workspace_bytes(count, symbols, width, _TYPE_CODES[dy.dtype]))
@@ -1036,7 +1041,7 @@ def _linear_cross_entropy_impl(
     symbols, width = weight.shape
     lse = torch.empty(target.shape, dtype=torch.float32, device=x.device)
     loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=x.device)
-    target = target.contiguous()
+    target = _flat(target)
     (xr, xs), (wr, ws) = _rows(x), _rows(weight)
     sizes = target.numel(), symbols, width, xs, ws, _TYPE_CODES[x.dtype]
     with _on_device(x.device) as idx:
@@ -1060,7 +1065,7 @@ def _linear_cross_entropy_backward_impl(
     symbols, width = weight.shape
     dx = torch.empty(x.shape if x_grad else (0,), dtype=x.dtype, device=x.device)
     dweight = torch.empty(weight.shape if weight_grad else (0,), dtype=x.dtype, device=x.device)
-    dloss, target, lse = dloss.contiguous(), target.contiguous(), lse.contiguous()
+    dloss, target, lse = _flat(dloss), _flat(target), _flat(lse)
     (xr, xs), (wr, ws) = _rows(x), _rows(weight)
     sizes = target.numel(), symbols, width, xs, ws, _TYPE_CODES[x.dtype]
     with _on_device(x.device) as idx:
