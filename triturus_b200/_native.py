@@ -298,8 +298,10 @@ def _status_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     st = _STATUS.get(idx)
     if st is None:
-        st = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _STATUS[idx] = st
+        with torch.inference_mode(False):  # (check_status clears it in any mode)
+            st = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        if type(st) is torch.Tensor:  # and nothing that a mode gave in its place, which has no memory
+            _STATUS[idx] = st
     return st
 
 
@@ -331,7 +333,10 @@ def _status_address(t: torch.Tensor) -> int:
     if at is None:
         if idx < 0 or torch.compiler.is_compiling():
             return 0
-        at = _STATUS_ADDRESS[idx] = _status_word(t.device).data_ptr()
+        word = _status_word(t.device)
+        if type(word) is not torch.Tensor:
+            return 0
+        at = _STATUS_ADDRESS[idx] = word.data_ptr()
     return at
 
 
