@@ -74,9 +74,9 @@ def linear_cross_entropy(
     the accuracy of 32-bit arithmetic whatever `set_tf32_enabled` says; an infinity in float32 counts as NaN.  Logits may be as large as 32 bits
     hold, one of +infinity gives NaN, and symbols of -infinity have probability 0.
 
-    x and weight may have any strides.  Rows of consecutive elements that do not overlap are read in place where they begin on 16-byte boundaries: of 16 bits, from 2048
-    positions on only on 128-byte ones, and weight of float32 with up to 192 positions.  Everything else is copied first, float32 (but for weight with so few positions) as its
-    parts, of 6 bytes for an element.  The loss is differentiable in x and weight, once and backwards; lse is not.  A tensor with a forward-mode
+    x and weight may have any strides.  Rows of consecutive elements that do not overlap are read in place where they begin on 16-byte boundaries:
+    of 16 bits, from 2048 positions on only on 128-byte ones, and weight of float32 with up to 192 positions.  Everything else is copied first,
+    float32 (but for weight with so few positions) as its parts, of 6 bytes for an element.  The loss is differentiable in x and weight, once and backwards; lse is not.  A tensor with a forward-mode
     tangent is refused."""
     code = _reduction("linear_cross_entropy", reduction)
     if not torch.compiler.is_compiling() and not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
@@ -107,11 +107,13 @@ def linear_cross_entropy_backward(
 
     With g the share of dloss in each position (0 for ignored ones) and d = g (exp(z - lse) - [target]): dx = d weight, dweight = d^T x, of x's type;
     None where `x_grad` or `weight_grad` is False.  The logits are computed once more, for a piece of the symbols at a time, and d is rounded
-    to 16 bits for its two products where x has 16, without what is common to all positions: in float16 relative to the largest finite |dloss|.  The operands are read in place or copied as in the forward call, but x is
-    copied whenever weight_grad is set (and has its room in the workspace in any case).  What x holds in ignored
-    positions does not count, NaN or not; dx is zero there, whatever weight holds.  An infinite element of weight makes its column of dx NaN in the other positions, 0 times infinity, also
-    where it makes a symbol impossible (in float32, which counts it as NaN, all columns).  Sums are in 32 bits in a fixed order.  The results carry no graph, and
-    tensors with a forward-mode tangent are refused."""
+    to 16 bits for its two products where x has 16, without what is common to all positions: in float16 relative to the largest finite |dloss|.
+    Sums are in 32 bits in a fixed order.  The operands are read in place or copied as in the forward call, but x is copied whenever weight_grad is
+    set (and has its room in the workspace in any case).
+
+    What x holds in ignored positions does not count, NaN or not; dx is zero there, whatever weight holds.  An infinite element of weight makes its
+    column of dx NaN in the other positions, 0 times infinity, also where it makes a symbol impossible (in float32, which counts it as NaN, all
+    columns).  The results carry no graph, and tensors with a forward-mode tangent are refused."""
     code = _reduction("linear_cross_entropy_backward", reduction)
     if not torch.compiler.is_compiling():
         out = _native.HOST.linear_cross_entropy_backward(

@@ -46,8 +46,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     [...] (int64 or int32), as a contiguous tensor [..., D] of weight's type.
 
     A symbol that is not in 0 ... V - 1 (a negative one is none that counts from the end) gives a row of NaN and has no gradient; nothing is
-    read for it.  The product with a scale other than 1 is rounded once.  weight may have any strides: rows of consecutive elements at one
-    distance are read in place, other views are copied first.
+    read for it.  The product with a scale other than 1 is taken in 32 bits and rounded to weight's type.  weight may have any strides: rows of
+    consecutive elements at one distance are read in place, other views are copied first.
 
     Differentiable in weight, once and backwards: the gradient is that of `embedding_backward`, where positions of the symbol `padding_idx`
     count as nothing.  A tensor with a forward-mode tangent is refused."""
